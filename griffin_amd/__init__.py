@@ -14,6 +14,7 @@ from .hip_scan import (
 )
 from .hip_block_ops import (hip_block_forward, hip_causal_conv, hip_causal_conv_padded, hip_gelu_gate, hip_linear,
                             hip_linear_pair, hip_rmsnorm)
+from .hip_delta import hip_gated_delta, hip_gated_delta_step
 from .modules import (
     BlockDiagonalLinear,
     RG_LRU,
@@ -32,6 +33,8 @@ __all__ = [
     "hip_block_forward",
     "hip_causal_conv",
     "hip_causal_conv_padded",
+    "hip_gated_delta",
+    "hip_gated_delta_step",
     "hip_gelu_gate",
     "hip_linear",
     "hip_linear_pair",

@@ -14,7 +14,7 @@ RGLRU_BF16 = 1
 FLAG_RESET = 1
 FLAG_INACTIVE = 2
 CHUNK = 32
-ABI_VERSION = 24
+ABI_VERSION = 25
 PATH_PORTABLE, PATH_FAST_TILED, PATH_FAST_CHAIN, PATH_WIDE, PATH_PRE = range(5)
 PATH_NAMES = ("portable", "fast_tiled", "fast_chain", "wide", "pre")
 
@@ -73,6 +73,12 @@ _SIGNATURES = {
     "rglru_hip_rmsnorm_fwd": (ctypes.c_int, [_P, _P, _P, _P, _I, _I, ctypes.c_float, ctypes.c_int, ctypes.c_int, _P]),
     "rglru_hip_rmsnorm_scratch_bytes": (ctypes.c_size_t, [_I, _I]),
     "rglru_hip_rmsnorm_bwd": (ctypes.c_int, [_P] * 7 + [_I, _I, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P]),
+    "rglru_hip_gated_delta_max_key_size": (ctypes.c_int, []),
+    "rglru_hip_gated_delta_workspace_bytes": (ctypes.c_size_t, [_I] * 5 + [ctypes.c_int]),
+    "rglru_hip_gated_delta_scratch_bytes": (ctypes.c_size_t, [_I] * 5),
+    "rglru_hip_gated_delta_fwd": (ctypes.c_int, [_P] * 11 + [ctypes.c_int, ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_gated_delta_bwd": (ctypes.c_int, [_P] * 16 + [ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_gated_delta_step": (ctypes.c_int, [_P] * 8 + [ctypes.c_float] + [_I] * 5 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_linear_splits": (ctypes.c_int64, [ctypes.c_int, _I, _I, _I, ctypes.c_int, ctypes.c_int]),
     "rglru_hip_linear": (ctypes.c_int, [ctypes.c_int, _P, _P, _I, _P, _P, _I] + [_P] * 5 + [_I, _P, _P, _I, _I, _I, ctypes.c_int, _P]),
     "rglru_hip_sums": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, _P]),

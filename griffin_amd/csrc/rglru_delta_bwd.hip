@@ -1,0 +1,405 @@
+// Gated delta rule, reverse mode.  With the notation of the forward pass, dO the upstream gradient and dS' the gradient of the
+// state behind a chunk:
+//   dZ = P^T dO + w K dS'            Y = T^T dZ            dV = Y
+//   dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y)
+//   N1 = scale tril(D . dO Z^T)      N2 = -stril(D . Y Z^T)
+//   dQ = scale rho dO S^T + (N1 beta) K          dK = E + beta F,  dbeta = k . F
+//   E  = -rho Y S^T + (N2 beta) K                F  = N1^T Q + N2^T K + e^(G_63 - G) Z dS'^T
+//   dG = q . dQ + k . E - beta dbeta             dlog_decay_t = sum of dG from t on + rho_63 <S, dS'> + sum over j of beta_j k_j . (last term of F)_j
+// (a factor e^(G_i) goes with everything that token i reads, e^(-G_j) with everything that token j writes, so the gradients of the
+// running log decay are products that are there already).  The first kernel walks back along the chunks with dS' as the
+// forward pass walks with S; the second one has no order: a workgroup a chunk and key head, which adds up its value heads.
+
+#include <hip/hip_runtime.h>
+
+#include <cstring>
+
+#include "rglru_delta.h"
+#include "rglru_host.h"
+
+namespace rglru {
+
+template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void delta_backward_kernel(DeltaArgs p) {
+  typedef Mx<IO> M;
+  typedef typename M::Wide Wide;
+  typedef typename M::Frag Frag;
+  constexpr int DK = 32 * KS, PL = M::kPlanes;
+  typedef Tile<IO, DK> Keys;
+  typedef Tile<IO, 64> Square;
+  __shared__ __attribute__((aligned(16))) IO keys[64 * DK], queries[64 * DK], solve[PL * 4096], within[PL * 4096];
+  __shared__ __attribute__((aligned(16))) float gates[kDeltaGates];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = (p.columns + 63) >> 6, total = groups * p.B * p.HV;
+  const int work = xcd_order(blockIdx.x, total);
+  if (work < 0) return;
+  const int group = work % groups, head = work / groups, hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
+  const int col = group * 64 + wave * 16 + c;
+  const bool mine = group * 64 + wave * 16 < p.columns, live = mine && col < p.V;
+
+  f32x4 dstate[2 * KS];
+#pragma unroll
+  for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * t + 4 * g + e;
+      dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
+    }
+
+  KeyRows<IO, DK, kDeltaThreads> next_k, next_q;
+  MatrixRows<IO, 64, 64, kDeltaThreads> next_solve, next_within;
+  float next_gate = 0.f;
+  const long long first = (long long)head * p.nC;
+  auto request = [&](int n) {
+    const long long chunk = first + n;
+    const float* record = p.gates + chunk * kDeltaGates;
+    const unsigned long long counts = (unsigned long long)__float_as_uint(record[128]) | (unsigned long long)__float_as_uint(record[129]) << 32;
+    const int t0 = n * kDeltaChunk, left = p.T - t0;
+    next_k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
+    next_q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
+    next_solve.request((const IO*)p.solve + chunk * (4096 * PL), 4096, 64, tid);
+    next_within.request((const IO*)p.within + chunk * (4096 * PL), 4096, 64, tid);
+    if (tid < kDeltaGates) next_gate = record[tid];
+  };
+  request(p.nC - 1);
+  for (int n = p.nC - 1; n >= 0; --n) {
+    const long long chunk = first + n;
+    const int t0 = n * kDeltaChunk, left = p.T - t0;
+    if (n != p.nC - 1) __syncthreads();                    // the tiles of the chunk behind have been read
+    next_k.put(keys, tid);
+    next_q.put(queries, tid);
+    next_solve.put(solve, tid);
+    next_within.put(within, tid);
+    if (tid < kDeltaGates) gates[tid] = next_gate;
+    __syncthreads();
+    if (n > 0) request(n - 1);
+    if (!mine) continue;
+    const unsigned long long counts = (unsigned long long)__float_as_uint(gates[128]) | (unsigned long long)__float_as_uint(gates[129]) << 32;
+    const ColumnIo<IO> ups((const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, col, live);
+    f32x4 up[4], rho[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * mt + 4 * g + e;
+        up[mt][e] = ups.load(row, (counts >> row) & 1);
+      }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(gates + 16 * mt + 4 * g);
+    Wide d[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) d[ks] = M::wide(dstate[2 * ks], dstate[2 * ks + 1]);
+    {
+      IO* at = (IO*)p.dstates + (chunk * PL * p.columns + col) * DK;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, dstate[t]);
+    }
+    // dZ = P^T dO + w K dS'
+    f32x4 dz[4] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) dz[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), d[ks], dz[mt]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(gates + 64 + 16 * mt + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dz[mt][e] = w[e] == 0.f ? 0.f : w[e] * dz[mt][e];
+    }
+    {
+      const Frag uf[2] = {M::exact(up[0], up[1]), M::exact(up[2], up[3])};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int mt = 0; mt < 2 * ks + 2; ++mt) dz[mt] = M::we(Square::wide_along_row(within, 4096, 16 * mt + c, 32 * ks, g), uf[ks], dz[mt]);
+    }
+    // Y = T^T dZ
+    f32x4 y[4] = {};
+    {
+      const Wide zw[2] = {M::wide(dz[0], dz[1]), M::wide(dz[2], dz[3])};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int mt = 0; mt < 2 * ks + 2; ++mt) y[mt] = M::ww(Square::wide_along_row(solve, 4096, 16 * mt + c, 32 * ks, g), zw[ks], y[mt]);
+    }
+    {
+      IO* at = (IO*)p.dvalues + (chunk * PL * p.columns + col) * 64;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, y[mt]);
+      const ColumnIo<IO> out((const IO*)p.dv + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, col, live);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = 16 * mt + 4 * g + e;
+          out.store(row, row < left, y[mt][e]);
+        }
+    }
+    // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y)
+    {
+      const float carry = gates[63];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          up[mt][e] *= p.scale * rho[mt][e];
+          y[mt][e] *= -rho[mt][e];
+        }
+      const Wide uw[2] = {M::wide(up[0], up[1]), M::wide(up[2], up[3])}, yw[2] = {M::wide(y[0], y[1]), M::wide(y[2], y[3])};
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dstate[t][e] = carry == 0.f ? 0.f : carry * dstate[t][e];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) {
+          dstate[t] = M::ew(Keys::down_rows(queries, 32 * ks, 16 * t, lane), uw[ks], dstate[t]);
+          dstate[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), yw[ks], dstate[t]);
+        }
+    }
+  }
+  if (p.dh0 && live) {
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * t + 4 * g + e;
+        if (row < p.K) p.dh0[((long long)head * p.K + row) * p.V + col] = dstate[t][e];
+      }
+  }
+}
+
+// Sum over the sixteen columns of an accumulator row.
+RGLRU_DEVICE float sixteen_sum(float v) {
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// Gradients of queries, keys and gates of one chunk and key head.  A wave owns 16 tokens.  The contractions over the value
+// columns take 32 of them at a time through LDS; N1 and N2 go through LDS once, where the columns lay.
+template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDeltaThreads) void delta_grads_kernel(DeltaArgs p) {
+  typedef Mx<IO> M;
+  typedef typename M::Wide Wide;
+  typedef typename M::Frag Frag;
+  constexpr int DK = 32 * KS, PL = M::kPlanes, CB = 32;
+  typedef Tile<IO, DK> Keys;
+  typedef Tile<IO, 64> Square;
+  typedef Tile<IO, CB> Ups;
+  constexpr int kUp = 0, kValues = kUp + 64 * CB, kDValues = kValues + PL * CB * 64, kStates = kDValues + PL * CB * 64,
+                kDStates = kStates + PL * CB * DK, kColumns = kDStates + PL * CB * DK, kPairs = 2 * PL * 4096;
+  __shared__ __attribute__((aligned(16))) IO keys[64 * DK], queries[64 * DK], area[kColumns > kPairs ? kColumns : kPairs];
+  __shared__ double total[64];
+  __shared__ float beta[64], to_end[64], dtotal[64], dwrite[64], sums[4];
+  __shared__ int segment[64];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = (int)(blockIdx.x % (unsigned)p.nC), bh = (int)(blockIdx.x / (unsigned)p.nC), h = bh % p.H, b = bh / p.H;
+  const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H, row0 = 16 * wave + 4 * g;
+  f32x4 all_dq[GROUPED ? 2 * KS : 1] = {}, all_dk[GROUPED ? 2 * KS : 1] = {};
+
+  for (int s = 0; s < share; ++s) {
+    const int hv = h * share + s, head = b * p.HV + hv;
+    const long long chunk = (long long)head * p.nC + n;
+    const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
+    const unsigned long long counts = __ballot(gate.counts);
+    const float carry = gate.segments == 0 ? expf((float)gate.end) : 0.f;
+    if (s == 0) {
+      KeyRows<IO, DK, kDeltaThreads> k, q;
+      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
+      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
+      k.put(keys, tid);
+      q.put(queries, tid);
+    } else {
+      __syncthreads();                                     // the head before is through with the shared arrays
+    }
+    if (wave == 0) {
+      total[lane] = gate.total;
+      beta[lane] = gate.beta;
+      segment[lane] = gate.segment;
+      to_end[lane] = gate.segment == gate.segments ? expf((float)(gate.end - gate.total)) : 0.f;
+    }
+    f32x4 dq[2 * KS] = {}, dr[2 * KS] = {}, dw[2 * KS] = {}, n1[4] = {}, n2[4] = {};
+    float carried = 0.f;                                   // <S, dS'>
+    const IO* ups = (const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V;
+    const bool vec_up = ((long long)p.V * sizeof(IO)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dout) % 16 == 0;
+    for (int c0 = 0; c0 < p.columns; c0 += CB) {
+      const int rows = p.columns - c0 < CB ? p.columns - c0 : CB;
+      KeyRows<IO, CB, kDeltaThreads> up;
+      MatrixRows<IO, CB, 64, kDeltaThreads> z, y;
+      MatrixRows<IO, CB, DK, kDeltaThreads> st, ds;
+      up.request(ups + c0, (long long)p.HV * p.V, p.V - c0, left, counts, vec_up, tid);
+      z.request((const IO*)p.values + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
+      y.request((const IO*)p.dvalues + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
+      st.request((const IO*)p.states + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
+      ds.request((const IO*)p.dstates + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
+      __syncthreads();                                     // the columns before have been read
+      up.put(area + kUp, tid);
+      z.put(area + kValues, tid);
+      y.put(area + kDValues, tid);
+      st.put(area + kStates, tid);
+      ds.put(area + kDStates, tid);
+      __syncthreads();
+      const Frag uf = Ups::along_row(area + kUp, 16 * wave + c, 0, g);
+      const Wide zf = Square::wide_down_rows(area + kValues, CB * 64, 0, 16 * wave, lane);
+      const Wide yf = Square::wide_down_rows(area + kDValues, CB * 64, 0, 16 * wave, lane);
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+        if (jt <= wave) {
+          const Wide zj = Square::wide_down_rows(area + kValues, CB * 64, 0, 16 * jt, lane);
+          n1[jt] = M::ew(uf, zj, n1[jt]);
+          n2[jt] = M::ww(yf, zj, n2[jt]);
+        }
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        const Wide sf = Keys::wide_down_rows(area + kStates, CB * DK, 0, 16 * t, lane);
+        const Wide df = Keys::wide_down_rows(area + kDStates, CB * DK, 0, 16 * t, lane);
+        dq[t] = M::ew(uf, sf, dq[t]);
+        dr[t] = M::ww(yf, sf, dr[t]);
+        dw[t] = M::ww(zf, df, dw[t]);
+      }
+      for (int i = tid; i < CB * DK; i += kDeltaThreads) {
+        if constexpr (PL == 2) carried = fmaf((float)area[kStates + i] + (float)area[kStates + CB * DK + i], (float)area[kDStates + i] + (float)area[kDStates + CB * DK + i], carried);
+        else carried = fmaf((float)area[kStates + i], (float)area[kDStates + i], carried);
+      }
+    }
+    // the factors of what reads the carried state and of what is left for the next chunk; the decays of the pairs
+    float dk_written[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = row0 + e;
+      const float rho = segment[i] == 0 ? expf((float)total[i]) : 0.f, end = to_end[i];
+      float dot = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        dq[t][e] *= p.scale * rho;
+        dr[t][e] *= -rho;
+        dw[t][e] *= end;
+        dot = fmaf(dw[t][e], (float)keys[Keys::at(i, 16 * t + c)], dot);
+      }
+      dk_written[e] = beta[i] * sixteen_sum(dot);
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) {
+        const int j = 16 * jt + c;
+        const bool joined = i >= j && segment[i] == segment[j];
+        const float d = joined ? expf((float)(total[i] - total[j])) : 0.f;
+        n1[jt][e] = joined ? p.scale * d * n1[jt][e] : 0.f;
+        n2[jt][e] = joined && i > j ? -d * n2[jt][e] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) carried += __shfl_xor(carried, m, 64);
+    __syncthreads();                                       // the last columns have been read
+    auto put_pairs = [&](bool strengths) {                 // kept [j][i]; blocks above the diagonal that a product touches are zeros
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+        if (jt <= (wave | 1)) {
+          const float f = strengths ? beta[16 * jt + c] : 1.f;
+          const int at = Square::at(16 * jt + c, row0);
+          M::put(area + at, 4096, n1[jt] * f);
+          M::put(area + PL * 4096 + at, 4096, n2[jt] * f);
+        }
+    };
+    put_pairs(false);
+    if (lane == 0) sums[wave] = carried;
+    __syncthreads();
+    // F = N1^T Q + N2^T K + ...: pairs in which the wave's tokens are the written ones
+    for (int ks = wave >> 1; ks < 2; ++ks) {
+      const Wide a = Square::wide_along_row(area, 4096, 16 * wave + c, 32 * ks, g);
+      const Wide a2 = Square::wide_along_row(area + PL * 4096, 4096, 16 * wave + c, 32 * ks, g);
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        dw[t] = M::we(a, Keys::down_rows(queries, 32 * ks, 16 * t, lane), dw[t]);
+        dw[t] = M::we(a2, Keys::down_rows(keys, 32 * ks, 16 * t, lane), dw[t]);
+      }
+    }
+    __syncthreads();
+    put_pairs(true);
+    __syncthreads();
+    for (int ks = 0; ks <= (wave >> 1); ++ks) {
+      const Wide a = Square::wide_down_rows(area, 4096, 32 * ks, 16 * wave, lane);
+      const Wide a2 = Square::wide_down_rows(area + PL * 4096, 4096, 32 * ks, 16 * wave, lane);
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        const Frag kf = Keys::down_rows(keys, 32 * ks, 16 * t, lane);
+        dq[t] = M::we(a, kf, dq[t]);
+        dr[t] = M::we(a2, kf, dr[t]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = row0 + e;
+      float read = 0.f, written = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        const float k = (float)keys[Keys::at(i, 16 * t + c)], q = (float)queries[Keys::at(i, 16 * t + c)];
+        read = fmaf(q, dq[t][e], fmaf(k, dr[t][e], read));
+        written = fmaf(k, dw[t][e], written);
+      }
+      read = sixteen_sum(read);
+      written = sixteen_sum(written);
+      if (c == 0) {
+        dtotal[i] = read - beta[i] * written;
+        dwrite[i] = dk_written[e];
+        if (i < left) delta_put_gate(p.dbeta, ((long long)b * p.T + t0 + i) * p.HV + hv, p.beta_dtype, written);
+      }
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        dr[t][e] = fmaf(beta[i], dw[t][e], dr[t][e]);
+        if constexpr (GROUPED) all_dq[t][e] += dq[t][e], all_dk[t][e] += dr[t][e];
+      }
+    }
+    if (!GROUPED || s == share - 1) {
+      const long long stride = (long long)p.H * p.K, base = ((long long)b * p.T + t0) * stride + (long long)h * p.K;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) {
+        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, 16 * t + c, 16 * t + c < p.K), k_out((const IO*)p.dk + base, stride, 16 * t + c, 16 * t + c < p.K);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          q_out.store(row0 + e, row0 + e < left, GROUPED ? all_dq[t][e] : dq[t][e]);
+          k_out.store(row0 + e, row0 + e < left, GROUPED ? all_dk[t][e] : dr[t][e]);
+        }
+      }
+    }
+    __syncthreads();
+    if (wave == 0) {                                       // sums from each token to the chunk's end
+      float write = dwrite[lane], from = dtotal[lane];
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) write += __shfl_xor(write, m, 64);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const float other = __shfl_down(from, d, 64);
+        if (lane + d < 64) from += other;
+      }
+      const float across = carry == 0.f ? 0.f : carry * ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+      const float d = gate.counts && !gate.starts ? from + (write + across) : 0.f;
+      if (lane < left) delta_put_gate(p.dlog_decay, ((long long)b * p.T + t0 + lane) * p.HV + hv, p.decay_dtype, d);
+    }
+  }
+}
+
+template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hipStream_t s) {
+  const int total = (a.columns + 63) / 64 * a.B * a.HV;
+  hipLaunchKernelGGL((delta_backward_kernel<IO, KS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(kDeltaThreads), 0, s, a);
+  int rc = check_launch("gated_delta_bwd");
+  if (rc) return rc;
+  const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));
+  if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kDeltaThreads), 0, s, a);
+  else hipLaunchKernelGGL((delta_grads_kernel<IO, KS, false>), grid, dim3(kDeltaThreads), 0, s, a);
+  return check_launch("gated_delta_bwd gradients");
+}
+
+int delta_launch_backward(const DeltaArgs& a, int dtype, hipStream_t s) {
+  switch ((a.K + 31) / 32) {
+#define RGLRU_DELTA(KS) case KS: return dtype == RGLRU_BF16 ? delta_backward<__bf16, KS>(a, s) : delta_backward<float, KS>(a, s)
+    RGLRU_DELTA(1);
+    RGLRU_DELTA(2);
+    RGLRU_DELTA(3);
+    RGLRU_DELTA(4);
+#undef RGLRU_DELTA
+  }
+  return fail(RGLRU_E_UNSUPPORTED, "gated_delta_bwd: key size %d", a.K);
+}
+
+}  // namespace rglru

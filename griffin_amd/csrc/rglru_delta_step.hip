@@ -1,0 +1,263 @@
+// Gated delta rule, one token a row with the state updated in place, and the C entry points of all its kernels.
+
+#include <hip/hip_runtime.h>
+
+#include <cstring>
+
+#include "rglru_delta.h"
+#include "rglru_host.h"
+
+namespace rglru {
+
+int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s);
+int delta_launch_backward(const DeltaArgs& a, int dtype, hipStream_t s);
+
+struct DeltaStepArgs {
+  const void *q, *k, *v, *log_decay, *beta;
+  const unsigned char* flags;
+  float* state;
+  void* out;
+  int H, HV, K, V, groups, decay_dtype, beta_dtype;
+  float scale;
+};
+
+// A workgroup takes the rows of LC * N columns of one head's state through its registers: read once, written once.  With r = S k and
+// s = S q of the state before the token, the state after it is a S + k u, u = beta (v - a r), and the output scale (a s + (q . k) u), so
+// both sums over the key run before anything is written.
+template <typename IO, int LC, int N> __global__ __launch_bounds__(kDeltaThreads) void delta_step_kernel(DeltaStepArgs p) {
+  typedef float vec __attribute__((ext_vector_type(N)));
+  constexpr int RG = kDeltaThreads / LC, ROWS = kDeltaMaxKey / RG, WAVES = kDeltaThreads / 64;
+  __shared__ float parts[2 * WAVES][LC * N];
+  __shared__ float pairs[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lc = tid % LC, rg = tid / LC;
+  const int group = blockIdx.x % (unsigned)p.groups, head = blockIdx.x / (unsigned)p.groups, hv = head % p.HV, b = head / p.HV;
+  const int h = hv / (p.HV / p.H), col = (group * LC + lc) * N;
+  const bool live = col < p.V;
+  const unsigned flag = p.flags ? p.flags[b] : 0u;
+  IO* out = (IO*)p.out + (long long)head * p.V + col;
+  if (flag & 2u) {                                          // a masked token: the state stays as it is
+    if (rg == 0 && live)
+      for (int e = 0; e < N; ++e) out[e] = (IO)0.f;
+    return;
+  }
+  const float g = delta_gate(p.log_decay, head, p.decay_dtype), beta = delta_gate(p.beta, head, p.beta_dtype);
+  const bool fresh = (flag & 1u) || g < kDeltaCut;
+  const float decay = fresh ? 0.f : expf(g);
+  const IO *k = (const IO*)p.k + ((long long)b * p.H + h) * p.K, *q = (const IO*)p.q + ((long long)b * p.H + h) * p.K;
+  float* state = p.state + (long long)head * p.K * p.V + col;
+  vec s[ROWS], read = {}, asked = {};
+  float key[ROWS], pair = 0.f;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = rg + RG * i;
+    s[i] = vec{};
+    if (row < p.K && live && !fresh) s[i] = *reinterpret_cast<const vec*>(state + (long long)row * p.V);
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = rg + RG * i;
+    key[i] = row < p.K ? (float)k[row] : 0.f;
+    const float query = row < p.K ? (float)q[row] : 0.f;
+    pair = fmaf(key[i], query, pair);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      read[e] = fmaf(key[i], s[i][e], read[e]);
+      asked[e] = fmaf(query, s[i][e], asked[e]);
+    }
+  }
+#pragma unroll
+  for (int m = LC; m < 64; m <<= 1) {
+    pair += __shfl_xor(pair, m, 64);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      read[e] += __shfl_xor(read[e], m, 64);
+      asked[e] += __shfl_xor(asked[e], m, 64);
+    }
+  }
+  if (lane < LC) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) parts[wave][lane * N + e] = read[e], parts[WAVES + wave][lane * N + e] = asked[e];
+    if (lane == 0) pairs[wave] = pair;
+  }
+  __syncthreads();
+  if (!live) return;
+  vec change, result;
+  pair = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) pair += pairs[w];
+  const IO* v = (const IO*)p.v + (long long)head * p.V + col;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float r = 0.f, a = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) r += parts[w][lc * N + e], a += parts[WAVES + w][lc * N + e];
+    change[e] = beta * fmaf(-decay, r, (float)v[e]);
+    result[e] = p.scale * fmaf(decay, a, pair * change[e]);
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = rg + RG * i;
+    vec next;
+#pragma unroll
+    for (int e = 0; e < N; ++e) next[e] = fmaf(decay, s[i][e], key[i] * change[e]);
+    if (row < p.K) *reinterpret_cast<vec*>(state + (long long)row * p.V) = next;
+  }
+  if (rg == 0) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = (IO)result[e];
+  }
+}
+
+template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bool vec, hipStream_t s) {
+  auto grid = [&](int columns) {
+    a.groups = (a.V + columns - 1) / columns;
+    return dim3((unsigned)(heads * a.groups));
+  };
+  if (!vec) {
+    const dim3 g = grid(32);
+    hipLaunchKernelGGL((delta_step_kernel<IO, 32, 1>), g, dim3(kDeltaThreads), 0, s, a);
+  } else {
+    const dim3 g = grid(32);
+    hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4>), g, dim3(kDeltaThreads), 0, s, a);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+struct DeltaSizes {
+  int64_t chunks, columns, width;
+  size_t gates, solve, within, states, values, total;      // offsets in the workspace; `total` without states and values if not kept
+  DeltaSizes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, bool keep) {
+    chunks = B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk);
+    columns = (V + 15) / 16 * 16;
+    width = (K + 31) / 32 * 32;
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t square = up((size_t)chunks * 4096 * 4);
+    gates = 0;
+    solve = up((size_t)chunks * kDeltaGates * 4);
+    within = solve + square;
+    states = within + square;
+    values = states + (keep ? up((size_t)chunks * columns * width * 4) : 0);
+    total = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
+  }
+  size_t scratch_values() const { return ((size_t)chunks * columns * width * 4 + 255) & ~(size_t)255; }
+  size_t scratch() const { return scratch_values() + (size_t)chunks * columns * 64 * 4; }
+};
+
+static int delta_check(const char* who, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int decay_dtype, int beta_dtype) {
+  if (B <= 0 || T <= 0 || H <= 0 || HV <= 0 || K <= 0 || V <= 0) return fail(RGLRU_E_ARG, "%s: sizes must be positive", who);
+  if (HV % H) return fail(RGLRU_E_ARG, "%s: %lld value heads do not share %lld key heads evenly", who, (long long)HV, (long long)H);
+  for (int d : {dtype, decay_dtype, beta_dtype})
+    if (d != RGLRU_F32 && d != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown dtype %d", who, d);
+  if (K > kDeltaMaxKey) return fail(RGLRU_E_UNSUPPORTED, "%s: keys of %lld elements, at most %d are covered", who, (long long)K, kDeltaMaxKey);
+  const int64_t most = (int64_t)1 << 30;
+  if (H * K >= most / 256 || HV * V >= most / 256) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens wider than %lld elements", who, (long long)(most / 256));
+  if (T >= (1ll << 30) || B * HV * ((V + 63) / 64) >= most || B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk) >= most)
+    return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
+  return RGLRU_OK;
+}
+
+static bool whole_vectors(const void* p, int64_t b, int64_t t, int64_t h, int64_t width, int dtype) {
+  const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % e == 0 && t % e == 0 && h % e == 0 && width % e == 0;
+}
+
+static int delta_operands(const char* who, DeltaArgs& a, const void* q, const void* k, const void* v, const int64_t* strides, int64_t B, int64_t T,
+                          int64_t H, int64_t HV, int64_t K, int64_t V, int dtype) {
+  const int64_t dense[9] = {T * H * K, H * K, K, T * H * K, H * K, K, T * HV * V, HV * V, V};
+  const int64_t* st = strides ? strides : dense;
+  for (int i = 0; i < 9; ++i)
+    if (st[i] < 0) return fail(RGLRU_E_ARG, "%s: negative stride", who);
+  for (int i = 1; i < 9; i += 3)
+    if (st[i] >= (1ll << 30) / 256) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens %lld elements apart", who, (long long)st[i]);
+  a.q = q, a.k = k, a.v = v;
+  a.q_b = st[0], a.q_t = st[1], a.q_h = st[2], a.k_b = st[3], a.k_t = st[4], a.k_h = st[5], a.v_b = st[6], a.v_t = st[7], a.v_h = st[8];
+  a.B = (int)B, a.T = (int)T, a.H = (int)H, a.HV = (int)HV, a.K = (int)K, a.V = (int)V;
+  a.nC = (int)((T + kDeltaChunk - 1) / kDeltaChunk);
+  a.columns = (int)((V + 15) / 16 * 16);
+  a.vec_q = whole_vectors(q, st[0], st[1], st[2], K, dtype), a.vec_k = whole_vectors(k, st[3], st[4], st[5], K, dtype);
+  return RGLRU_OK;
+}
+
+static void delta_workspace(DeltaArgs& a, void* ws, const DeltaSizes& z, bool keep) {
+  char* base = (char*)ws;
+  a.gates = (float*)(base + z.gates);
+  a.solve = base + z.solve, a.within = base + z.within;
+  if (keep) a.states = base + z.states, a.values = base + z.values;
+}
+
+}  // namespace rglru
+
+using namespace rglru;
+
+extern "C" {
+
+int rglru_hip_gated_delta_max_key_size(void) { return kDeltaMaxKey; }
+
+size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int keep) {
+  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey) return 0;
+  return DeltaSizes(B, T, HV, K, V, keep != 0).total;
+}
+
+size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V) {
+  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey) return 0;
+  return DeltaSizes(B, T, HV, K, V, true).scratch();
+}
+
+int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* log_decay, const void* beta,
+                              const float* h0, const uint8_t* flags, void* out, float* h_last, void* ws, int keep, float scale, int64_t B, int64_t T,
+                              int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int decay_dtype, int beta_dtype, void* stream) {
+  int rc = delta_check("gated_delta_fwd", B, T, H, HV, K, V, dtype, decay_dtype, beta_dtype);
+  if (rc) return rc;
+  if (!q || !k || !v || !log_decay || !beta || !out || !ws) return fail(RGLRU_E_ARG, "gated_delta_fwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "gated_delta_fwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
+  DeltaArgs a;
+  memset(&a, 0, sizeof(a));
+  rc = delta_operands("gated_delta_fwd", a, q, k, v, strides, B, T, H, HV, K, V, dtype);
+  if (rc) return rc;
+  a.log_decay = log_decay, a.beta = beta, a.flags = flags, a.h0 = h0, a.out = out, a.h_last = h_last;
+  a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
+  delta_workspace(a, ws, DeltaSizes(B, T, HV, K, V, keep != 0), keep != 0);
+  return delta_launch_forward(a, keep != 0, dtype, (hipStream_t)stream);
+}
+
+int rglru_hip_gated_delta_bwd(const void* q, const void* k, const int64_t* strides, const void* log_decay, const void* beta, const uint8_t* flags,
+                              const void* dout, const float* dh_last, void* ws, void* scratch, void* dq, void* dk, void* dv, void* dlog_decay,
+                              void* dbeta, float* dh0, float scale, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype,
+                              int decay_dtype, int beta_dtype, void* stream) {
+  int rc = delta_check("gated_delta_bwd", B, T, H, HV, K, V, dtype, decay_dtype, beta_dtype);
+  if (rc) return rc;
+  if (!q || !k || !log_decay || !beta || !dout || !ws || !scratch || !dq || !dk || !dv || !dlog_decay || !dbeta)
+    return fail(RGLRU_E_ARG, "gated_delta_bwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "gated_delta_bwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
+  DeltaArgs a;
+  memset(&a, 0, sizeof(a));
+  rc = delta_operands("gated_delta_bwd", a, q, k, nullptr, strides, B, T, H, HV, K, V, dtype);
+  if (rc) return rc;
+  const DeltaSizes z(B, T, HV, K, V, true);
+  a.log_decay = log_decay, a.beta = beta, a.flags = flags, a.dout = dout, a.dh_last = dh_last;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.dlog_decay = dlog_decay, a.dbeta = dbeta, a.dh0 = dh0;
+  a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
+  delta_workspace(a, ws, z, true);
+  a.dstates = scratch, a.dvalues = (char*)scratch + z.scratch_values();
+  return delta_launch_backward(a, dtype, (hipStream_t)stream);
+}
+
+int rglru_hip_gated_delta_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, float* state,
+                               const uint8_t* flags, void* out, float scale, int64_t B, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype,
+                               int decay_dtype, int beta_dtype, void* stream) {
+  int rc = delta_check("gated_delta_step", B, 1, H, HV, K, V, dtype, decay_dtype, beta_dtype);
+  if (rc) return rc;
+  if (!q || !k || !v || !log_decay || !beta || !state || !out) return fail(RGLRU_E_ARG, "gated_delta_step: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "gated_delta_step: RGLRU_FLAGS_FIRST_RESET is not a flag array");
+  DeltaStepArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q, a.k = k, a.v = v, a.log_decay = log_decay, a.beta = beta, a.state = state, a.flags = flags, a.out = out;
+  a.H = (int)H, a.HV = (int)HV, a.K = (int)K, a.V = (int)V, a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
+  const bool vec = V % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
+  if (dtype == RGLRU_BF16) delta_step<__bf16>(a, B * HV, vec, (hipStream_t)stream);
+  else delta_step<float>(a, B * HV, vec, (hipStream_t)stream);
+  return check_launch("gated_delta_step");
+}
+
+}  // extern "C"

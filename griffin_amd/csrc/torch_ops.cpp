@@ -2139,6 +2139,152 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> block_infer(
   return std::make_tuple(out, h_last, new_conv, last);
 }
 
+// ---- gated delta rule ---------------------------------------------------------------------------------------------
+
+// q, k, v as the kernels read them: the last axis contiguous, the others with strides of their own (parts of one projection go in
+// as they are).
+struct DeltaOperands {
+  Tensor q, k, v, log_decay, beta;
+  int64_t strides[9];
+  int64_t B, T, H, HV, K, V;
+  static Tensor rows(const Tensor& t) {
+    bool plain = t.stride(3) == 1 || t.size(3) == 1;
+    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0;
+    return plain && t.stride(1) < (int64_t(1) << 22) ? t : t.contiguous();
+  }
+  DeltaOperands(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& decay_in, const Tensor& beta_in)
+      : q(rows(q_in)), k(rows(k_in)), v(rows(v_in)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
+    int at = 0;
+    for (const Tensor* t : {&q, &k, &v})
+      for (int i = 0; i < 3; ++i) strides[at++] = t->stride(i);
+    B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), HV = v.size(2), V = v.size(3);
+  }
+};
+
+void check_delta(const char* name, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& beta, int64_t axes) {
+  const char* lead = axes == 4 ? "[batch, sequence, " : "[batch, ";
+  TORCH_CHECK_VALUE(q.dim() == axes && k.sizes() == q.sizes(), name, " expects queries and keys of one shape ", lead, "heads, key size], got ", q.sizes(),
+                    " and ", k.sizes());
+  TORCH_CHECK_VALUE(v.dim() == axes && v.sizes().slice(0, axes - 2) == q.sizes().slice(0, axes - 2), name, " expects values of shape ", lead,
+                    "value heads, value size] beside queries of shape ", q.sizes(), ", got ", v.sizes());
+  TORCH_CHECK_VALUE(log_decay.sizes() == v.sizes().slice(0, axes - 1) && beta.sizes() == log_decay.sizes(), name, " expects log_decay and beta of shape ",
+                    v.sizes().slice(0, axes - 1), ", got ", log_decay.sizes(), " and ", beta.sizes());
+  TORCH_CHECK_VALUE(q.numel() > 0 && v.numel() > 0, name, " does not accept empty batches, sequences or heads");
+  TORCH_CHECK_VALUE(v.size(-2) % q.size(-2) == 0, name, " expects the value heads to be a multiple of the key heads, got ", v.size(-2), " and ", q.size(-2));
+  TORCH_CHECK_TYPE(known(q.scalar_type()) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), name,
+                   " expects queries, keys and values all in float32 or all in bfloat16, got ", q.scalar_type(), ", ", k.scalar_type(), " and ", v.scalar_type());
+  TORCH_CHECK_TYPE(known(log_decay.scalar_type()) && known(beta.scalar_type()), name, " expects log_decay and beta in float32 or bfloat16, got ",
+                   log_decay.scalar_type(), " and ", beta.scalar_type());
+}
+
+struct DeltaResult {
+  Tensor out, h_last, kept;
+};
+
+DeltaResult delta_forward(const DeltaOperands& o, const Tensor& h0_in, const Tensor& flags, double scale, bool keep) {
+  DeltaResult r;
+  const auto dtype = o.q.scalar_type();
+  Tensor h0 = as(h0_in, at::kFloat);
+  r.out = fresh({o.B, o.T, o.HV, o.V}, dtype, o.q);
+  r.h_last = fresh({o.B, o.HV, o.K, o.V}, at::kFloat, o.q);
+  const size_t size = rglru_hip_gated_delta_workspace_bytes(o.B, o.T, o.HV, o.K, o.V, keep ? 1 : 0);
+  TORCH_CHECK_VALUE(size > 0, "hip gated delta rule: keys of ", o.K, " elements, at most ", rglru_hip_gated_delta_max_key_size(), " are covered");
+  r.kept = bytes(size, o.q);
+  check(rglru_hip_gated_delta_fwd(ptr(o.q), ptr(o.k), ptr(o.v), o.strides, ptr(o.log_decay), ptr(o.beta), fptr(h0), bptr(flags), ptr(r.out),
+                                  fptr(r.h_last), ptr(r.kept), keep ? 1 : 0, static_cast<float>(scale), o.B, o.T, o.H, o.HV, o.K, o.V, code_of(dtype),
+                                  code_of(o.log_decay.scalar_type()), code_of(o.beta.scalar_type()), stream_of(o.q)),
+        "rglru_hip_gated_delta_fwd");
+  return r;
+}
+
+struct GatedDelta : torch::autograd::Function<GatedDelta> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& beta,
+                               const MaybeTensor& h0_, const MaybeTensor& flags_, double scale) {
+    Tensor h0 = opt(h0_), flags = opt(flags_);
+    note_arguments(ctx, {true, true, true, true, true, h0.defined()});
+    c10::DeviceGuard guard(q.device());
+    DeltaOperands o(q, k, v, log_decay, beta);
+    DeltaResult r = delta_forward(o, h0, flags, scale, true);
+    ctx->save_for_backward({o.q, o.k, o.log_decay, o.beta, flags, r.kept});
+    ctx->saved_data["scale"] = scale;
+    pack(ctx, {o.HV, o.V, type_or_none(h0)});
+    ctx->set_materialize_grads(false);
+    return {r.out, r.h_last};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    auto saved = ctx->get_saved_variables();
+    auto m = unpack(ctx);
+    const Tensor &q = saved[0], &k = saved[1], &log_decay = saved[2], &beta = saved[3], &flags = saved[4], &kept = saved[5];
+    Tensor dq, dk, dv, dlog_decay, dbeta, dh0;
+    {
+      at::NoGradGuard no_grad;
+      c10::DeviceGuard guard(q.device());
+      const auto dtype = q.scalar_type();
+      const int64_t B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), HV = m[0], V = m[1];
+      int64_t strides[9];
+      for (int i = 0; i < 3; ++i) strides[i] = q.stride(i), strides[3 + i] = k.stride(i), strides[6 + i] = 0;
+      Tensor dout = grads[0].defined() ? as(grads[0], dtype) : at::zeros({B, T, HV, V}, q.options());
+      Tensor dh_last = as(grads[1], at::kFloat);
+      dq = fresh({B, T, H, K}, dtype, q), dk = fresh({B, T, H, K}, dtype, q), dv = fresh({B, T, HV, V}, dtype, q);
+      dlog_decay = fresh_like(log_decay), dbeta = fresh_like(beta);
+      if (Needs(ctx)(5)) dh0 = fresh({B, HV, K, V}, at::kFloat, q);
+      Tensor scratch = bytes(rglru_hip_gated_delta_scratch_bytes(B, T, HV, K, V), q);
+      check(rglru_hip_gated_delta_bwd(ptr(q), ptr(k), strides, ptr(log_decay), ptr(beta), bptr(flags), ptr(dout), fptr(dh_last), ptr(kept), ptr(scratch),
+                                      ptr(dq), ptr(dk), ptr(dv), ptr(dlog_decay), ptr(dbeta), fptr(dh0),
+                                      static_cast<float>(ctx->saved_data["scale"].toDouble()), B, T, H, HV, K, V, code_of(dtype),
+                                      code_of(log_decay.scalar_type()), code_of(beta.scalar_type()), stream_of(q)),
+            "rglru_hip_gated_delta_bwd");
+      if (dh0.defined() && type_at(m, 2) != at::kFloat) dh0 = dh0.to(type_at(m, 2));
+    }
+    return once({dq, dk, dv, dlog_decay, dbeta, dh0, Tensor(), Tensor()});
+  }
+};
+
+std::tuple<Tensor, Tensor> gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& beta,
+                                       const MaybeTensor& h0_, const MaybeTensor& flags_, double scale) {
+  const char* name = "hip gated delta rule";
+  Tensor h0 = opt(h0_), flags = opt(flags_);
+  require_gpu(name, {&q, &k, &v, &log_decay, &beta, &h0, &flags});
+  require_device_of(name, q, {&k, &v, &log_decay, &beta, &h0, &flags});
+  check_delta(name, q, k, v, log_decay, beta, 4);
+  TORCH_CHECK_VALUE(!h0.defined() || (h0.dim() == 4 && h0.size(0) == q.size(0) && h0.size(1) == v.size(2) && h0.size(2) == q.size(3) && h0.size(3) == v.size(3)),
+                    "initial state must have shape (", q.size(0), ", ", v.size(2), ", ", q.size(3), ", ", v.size(3), ")");
+  TORCH_CHECK_VALUE(!flags.defined() || (flags.dim() == 2 && flags.size(0) == q.size(0) && flags.size(1) == q.size(1)), "token masks must have shape (",
+                    q.size(0), ", ", q.size(1), ")");
+  flags = token_bytes(flags, q.size(0) * q.size(1));
+  if (wants_grad({&q, &k, &v, &log_decay, &beta, &h0})) {
+    auto out = GatedDelta::apply(q, k, v, log_decay, beta, maybe(h0), maybe(flags), scale);
+    return {out[0], out[1]};
+  }
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(q.device());
+  DeltaResult r = delta_forward(DeltaOperands(q, k, v, log_decay, beta), h0, flags, scale, false);
+  return {r.out, r.h_last};
+}
+
+Tensor gated_delta_step(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& decay_in, const Tensor& beta_in, const Tensor& state,
+                        const MaybeTensor& flags_, double scale) {
+  const char* name = "hip gated delta rule step";
+  Tensor flags = opt(flags_);
+  require_gpu(name, {&q_in, &k_in, &v_in, &decay_in, &beta_in, &state, &flags});
+  require_device_of(name, q_in, {&k_in, &v_in, &decay_in, &beta_in, &state, &flags});
+  check_delta(name, q_in, k_in, v_in, decay_in, beta_in, 3);
+  const int64_t B = q_in.size(0), H = q_in.size(1), K = q_in.size(2), HV = v_in.size(1), V = v_in.size(2);
+  TORCH_CHECK_VALUE(state.dim() == 4 && state.size(0) == B && state.size(1) == HV && state.size(2) == K && state.size(3) == V &&
+                        state.scalar_type() == at::kFloat && state.is_contiguous(),
+                    "step expects a contiguous fp32 state of shape (", B, ", ", HV, ", ", K, ", ", V, ")");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()), name, " updates its state in place and has no gradient; the state requires one");
+  flags = token_bytes(flags, B);
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(q_in.device());
+  Tensor q = q_in.contiguous(), k = k_in.contiguous(), v = v_in.contiguous(), log_decay = decay_in.contiguous(), beta = beta_in.contiguous();
+  Tensor out = fresh({B, HV, V}, v.scalar_type(), v);
+  check(rglru_hip_gated_delta_step(ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(beta), fptr(state), bptr(flags), ptr(out), static_cast<float>(scale), B, H,
+                                   HV, K, V, code_of(v.scalar_type()), code_of(log_decay.scalar_type()), code_of(beta.scalar_type()), stream_of(v)),
+        "rglru_hip_gated_delta_step");
+  return out;
+}
+
 // ---- RMSNorm (griffin/griffin.py:68-80) ---------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> rmsnorm_forward(const Tensor& x_in, const Tensor& g, double eps, bool need_inv) {
@@ -2269,5 +2415,7 @@ PYBIND11_MODULE(_native, m) {
   EXPORT(block_train_packed);
   EXPORT(block_infer);
   EXPORT(rmsnorm);
+  EXPORT(gated_delta);
+  EXPORT(gated_delta_step);
 #undef EXPORT
 }

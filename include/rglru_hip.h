@@ -55,7 +55,7 @@
 extern "C" {
 #endif
 
-#define RGLRU_ABI_VERSION 24
+#define RGLRU_ABI_VERSION 25
 
 enum { RGLRU_F32 = 0, RGLRU_BF16 = 1 };
 
@@ -368,6 +368,37 @@ size_t rglru_hip_rmsnorm_scratch_bytes(int64_t rows, int64_t D);
 int rglru_hip_rmsnorm_bwd(const void* x, const void* g, const float* inv, const void* dy, void* scratch,
                           void* dx, void* dg, int64_t rows, int64_t D, int dtype, int vec_dtype, int grad_dtype,
                           void* stream);
+
+/* ---- gated delta rule: a gated recurrence with a matrix for a state (no counterpart in the reference) ------------------
+ *   S_t = a_t (I - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T,   o_t = scale S_t^T q_t,   a_t = exp(log_decay_t)
+ * q, k [B, T, H, K] and v, out [B, T, HV, V] in `dtype`; log_decay [B, T, HV] in `decay_dtype`, beta [B, T, HV] in `beta_dtype`;
+ * states [B, HV, K, V] fp32.  HV is a multiple of H: value head h reads key head h / (HV / H).  K is at most
+ * rglru_hip_gated_delta_max_key_size(); V is free.  Log decays are meant to be at most 0; one below -1e4 (minus infinity among them)
+ * discards the history as a reset does.  Unit keys and beta in [0, 2] keep the recurrence from growing.
+ *   strides  NULL (everything dense), or nine counts of elements in HOST memory: batch, token and head stride of q, of k, of v
+ *            (non-negative; the last axis is contiguous).  out and all gradients are dense.
+ *   flags    [B, T] or NULL: a reset discards the history in front of its token; an inactive token leaves the state as it is, gives
+ *            zeros, takes part in no gradient, and nothing it holds is read.  A reset of an inactive token does not count.
+ *   h0, h_last, dh_last, dh0 may be NULL.
+ *   ws       rglru_hip_gated_delta_workspace_bytes(.., keep) bytes, 16-byte aligned.  With keep != 0 the forward call leaves there what
+ *            the backward call needs, which changes none of it: any number of backward calls may follow.
+ *   scratch  rglru_hip_gated_delta_scratch_bytes(..) bytes of the backward call's own, 16-byte aligned.
+ * Tokens are taken in chunks of 64: a NaN or an infinity in an active token may reach every output of its chunk.
+ * The step takes one token a row (no T axis, everything dense) and updates `state` in place; inactive rows keep theirs. */
+int rglru_hip_gated_delta_max_key_size(void);
+size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int keep);
+size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V);
+int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* log_decay,
+                              const void* beta, const float* h0, const uint8_t* flags, void* out, float* h_last, void* ws, int keep,
+                              float scale, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype,
+                              int decay_dtype, int beta_dtype, void* stream);
+int rglru_hip_gated_delta_bwd(const void* q, const void* k, const int64_t* strides, const void* log_decay, const void* beta,
+                              const uint8_t* flags, const void* dout, const float* dh_last, void* ws, void* scratch, void* dq,
+                              void* dk, void* dv, void* dlog_decay, void* dbeta, float* dh0, float scale, int64_t B, int64_t T,
+                              int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int decay_dtype, int beta_dtype, void* stream);
+int rglru_hip_gated_delta_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta, float* state,
+                               const uint8_t* flags, void* out, float scale, int64_t B, int64_t H, int64_t HV, int64_t K, int64_t V,
+                               int dtype, int decay_dtype, int beta_dtype, void* stream);
 
 /* Column sums of x[rows, D] (dtype) into out[D] (out_dtype), fp32 accumulation in a fixed order: the
  * bias gradient of the block's three Linear layers (griffin/griffin.py:379-389; autograd of

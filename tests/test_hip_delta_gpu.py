@@ -1,0 +1,305 @@
+"""The gated delta rule on the GPU against its definition, token by token in 64 bits."""
+
+import pytest
+import torch
+
+from griffin_amd import hip_gated_delta, hip_gated_delta_step
+from tests.helpers import rel_err
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("q", "k", "v", "log_decay", "beta", "h0")
+BF16, F32 = torch.bfloat16, torch.float32
+# Largest deviation over largest value.  fp32: sums of up to 128 products, each off by 2^-24, through two products in a row for a
+# result and four for a gradient.  bf16: a result is rounded once, 2^-8; what is computed before enters the products
+# to 2^-17, through up to eight of them in a row, which also bounds the fp32 states of bf16 operands.
+OUT = {F32: 2 ** -16, BF16: 2 ** -8 + 2 ** -14}
+GRAD = {F32: 2 ** -15, BF16: 2 ** -8 + 2 ** -13}
+STATE = {F32: 2 ** -16, BF16: 2 ** -14}
+STATE_GRAD = {F32: 2 ** -15, BF16: 2 ** -13}
+
+
+def recurrence(q, k, v, log_decay, beta, h0, scale, reset=None, active=None):
+    """o and the final state, from the definition (any float type, autograd works)."""
+    B, T, H, K = q.shape
+    HV, V = v.shape[2:]
+    of = torch.arange(HV) // (HV // H)
+    q, k = q[:, :, of], k[:, :, of]
+    state = q.new_zeros(B, HV, K, V) if h0 is None else h0
+    rows = []
+    for t in range(T):
+        kept = state * log_decay[:, t].exp()[..., None, None]
+        if reset is not None:
+            kept = torch.where(reset[:, t, None, None, None], torch.zeros_like(kept), kept)
+        error = v[:, t] - (kept * k[:, t, :, :, None]).sum(2)
+        new = kept + k[:, t, :, :, None] * (beta[:, t, :, None] * error)[:, :, None]
+        out = scale * (new * q[:, t, :, :, None]).sum(2)
+        if active is not None:
+            live = active[:, t, None, None]
+            new = torch.where(live[..., None], new, state)
+            out = torch.where(live, out, torch.zeros_like(out))
+        state = new
+        rows.append(out)
+    return torch.stack(rows, 1), state
+
+
+def make(B, T, H, HV, K, V, dtype=F32, carried=True, seed=0, slow=False):
+    gen = torch.Generator().manual_seed(seed)
+    normal = lambda *shape: torch.randn(*shape, generator=gen)
+    unit = lambda t: t / t.norm(dim=-1, keepdim=True)
+    made = {
+        "q": unit(normal(B, T, H, K)), "k": unit(normal(B, T, H, K) + 0.3), "v": normal(B, T, HV, V),
+        "log_decay": -torch.nn.functional.softplus(normal(B, T, HV) - (6 if slow else 2)), "beta": torch.sigmoid(normal(B, T, HV)),
+    }
+    made = {name: t.to(dtype) for name, t in made.items()}
+    made["h0"] = 0.5 * normal(B, HV, K, V) if carried else None
+    made["up"], made["up_state"] = normal(B, T, HV, V).to(dtype), 0.2 * normal(B, HV, K, V)
+    return made
+
+
+def masks(B, T, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    reset = torch.rand(B, T, generator=gen) < 4.0 / T
+    lengths = torch.randint(1, T + 1, (B,), generator=gen)
+    return reset, torch.arange(T)[None] < lengths[:, None]
+
+
+def run(fn, case, reset, active, device, dtype=None, scale=None):
+    leaves = [None if case[n] is None else case[n].to(device=device, dtype=dtype or case[n].dtype).requires_grad_(True) for n in NAMES]
+    put = lambda t: None if t is None else t.to(device)
+    scale = case["q"].shape[-1] ** -0.5 if scale is None else scale
+    out, last = fn(*leaves, scale, put(reset), put(active))
+    wrt = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad([out, last], wrt, [case["up"].to(out), case["up_state"].to(last)])
+    return out.detach(), last.detach(), dict(zip([n for n, t in zip(NAMES, leaves) if t is not None], grads))
+
+
+def check(case, reset=None, active=None, scale=None):
+    dtype = case["q"].dtype
+    want, want_last, want_grads = run(recurrence, case, reset, active, "cpu", torch.float64, scale)
+    got, last, grads = run(hip_gated_delta, case, reset, active, "cuda", None, scale)
+    torch.cuda.synchronize()
+    # as fp32 numbers: exp(-20000) is 2^-28853 in 64 bits and 0 in any result, whose smallest number is 2^-149
+    want, want_last, want_grads = want.float(), want_last.float(), {n: t.float() for n, t in want_grads.items()}
+    assert got.dtype == dtype and last.dtype == F32
+    errors = {"o": rel_err(got, want) / OUT[dtype], "state": rel_err(last, want_last) / STATE[dtype]}
+    for name in grads:
+        assert grads[name].dtype == case[name].dtype and grads[name].shape == case[name].shape
+        errors["d" + name] = rel_err(grads[name], want_grads[name]) / (STATE_GRAD if name == "h0" else GRAD)[dtype]
+    assert all(e <= 1 for e in errors.values()), errors
+
+
+SHAPES = [
+    # B, T, H, HV, K, V: one token; one chunk; a token more; several chunks; odd sizes; shared key heads
+    (1, 1, 1, 1, 8, 8),
+    (2, 64, 2, 2, 32, 32),
+    (2, 65, 1, 3, 40, 24),
+    (1, 200, 2, 4, 128, 128),
+    (3, 130, 2, 2, 96, 80),
+    (1, 63, 1, 1, 128, 20),
+    (2, 150, 1, 2, 100, 33),
+    (1, 300, 1, 1, 64, 144),
+    (1, 129, 1, 1, 1, 1),
+    (1, 90, 3, 3, 17, 65),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_whole_sequences(shape, dtype):
+    check(make(*shape, dtype=dtype, carried=shape[1] % 2 == 0))
+
+
+@pytest.mark.parametrize("shape", [(3, 130, 2, 2, 96, 80), (4, 77, 1, 2, 64, 32), (2, 200, 2, 2, 128, 64)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_packed_documents_and_padding(shape, dtype):
+    reset, active = masks(*shape[:2])
+    case = make(*shape, dtype=dtype)
+    check(case, reset, active)
+    check(case, reset, None)
+    check(case, None, active)
+
+
+def test_every_token_a_document():
+    check(make(2, 70, 1, 1, 32, 32), torch.ones(2, 70, dtype=torch.bool), None)
+
+
+def test_masks_with_holes_and_rows_without_tokens():
+    gen = torch.Generator().manual_seed(5)
+    active = torch.rand(4, 140, generator=gen) < 0.5
+    active[1] = False
+    active[2, :64] = False
+    reset = torch.rand(4, 140, generator=gen) < 0.1
+    for dtype in (F32, BF16):
+        check(make(4, 140, 1, 2, 64, 48, dtype=dtype), reset, active)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_masked_tokens_may_hold_anything(dtype):
+    reset, active = masks(3, 130, seed=4)
+    case = make(3, 130, 2, 4, 64, 64, dtype=dtype)
+    clean = run(hip_gated_delta, case, reset, active, "cuda")
+    for name in ("q", "k", "v", "log_decay", "beta", "up"):
+        case[name] = case[name].clone()
+        case[name][~active] = float("nan") if name != "log_decay" else float("inf")
+    dirty = run(hip_gated_delta, case, reset, active, "cuda")
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for name in NAMES:
+        assert torch.equal(clean[2][name], dirty[2][name]), name
+        if name != "h0":
+            assert not dirty[2][name][~active.cuda()].any()
+    assert not dirty[0][~active.cuda()].any()
+
+
+def test_a_decay_of_nothing_is_a_reset():
+    case = make(2, 100, 1, 2, 32, 32)
+    reset = torch.zeros(2, 100, dtype=torch.bool)
+    reset[:, 10] = reset[0, 64] = reset[1, 99] = True
+    want = run(hip_gated_delta, case, reset, None, "cuda")
+    case["log_decay"] = case["log_decay"].masked_fill(reset[..., None], -float("inf"))
+    got = run(hip_gated_delta, case, None, None, "cuda")
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for name in NAMES:
+        assert torch.equal(got[2][name], want[2][name]), name
+
+
+def test_decays_that_are_thousands_apart_in_a_chunk():
+    """The running sum reaches thousands, where 32 bits no longer hold the differences between neighbours."""
+    case = make(1, 128, 1, 1, 32, 32)
+    case["log_decay"][:, ::2] = -300.0
+    check(case)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_slow_decay_over_many_chunks(dtype):
+    check(make(1, 700, 1, 1, 64, 64, dtype=dtype, slow=True))
+
+
+def test_gates_in_another_type_than_the_activations():
+    case = make(2, 100, 1, 2, 64, 64, dtype=BF16)
+    case["log_decay"], case["beta"] = case["log_decay"].float(), case["beta"].float()
+    check(case)
+    case["beta"] = case["beta"].to(BF16)
+    check(case)
+
+
+def test_scale_is_a_factor_of_the_output():
+    check(make(1, 80, 1, 1, 32, 32), scale=0.75)
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_parts_of_one_projection_are_read_in_place(dtype, offset):
+    B, T, H, HV, K, V = 2, 100, 2, 4, 32, 24
+    case = make(B, T, H, HV, K, V, dtype=dtype, carried=False)
+    flat = torch.cat([case[n].reshape(B, T, -1) for n in "qkv"], -1)
+    wide = torch.zeros(B, T, flat.shape[-1] + 2 * offset + 8, dtype=dtype)
+    wide[..., offset:offset + flat.shape[-1]] = flat
+    wide = wide.cuda().requires_grad_(True)
+    q, k, v = wide[..., offset:offset + flat.shape[-1]].split([H * K, H * K, HV * V], -1)
+    q, k, v = q.view(B, T, H, K), k.view(B, T, H, K), v.view(B, T, HV, V)
+    gates = [case[n].cuda() for n in ("log_decay", "beta")]
+    out, _ = hip_gated_delta(q, k, v, *gates)
+    want, _ = hip_gated_delta(*(case[n].cuda() for n in NAMES[:5]))
+    assert torch.equal(out, want)
+    (grad,) = torch.autograd.grad(out, wide, case["up"].cuda())
+    dense = run(hip_gated_delta, dict(case, up_state=torch.zeros(B, HV, K, V)), None, None, "cuda")[2]
+    assert torch.equal(grad[..., offset:offset + flat.shape[-1]], torch.cat([dense[n].reshape(B, T, -1) for n in "qkv"], -1))
+
+
+def test_pieces_with_a_carried_state_are_the_whole():
+    case = {n: None if t is None else t.cuda() for n, t in make(2, 230, 1, 2, 64, 64).items()}
+    reset, active = (m.cuda() for m in masks(2, 230, seed=9))
+    operands = [case[n] for n in NAMES[:5]]
+    whole, last = hip_gated_delta(*operands, case["h0"], reset_mask=reset, active_mask=active)
+    state, rows = case["h0"], []
+    for a, b in ((0, 1), (1, 64), (64, 65), (65, 200), (200, 230)):
+        out, state = hip_gated_delta(*(t[:, a:b] for t in operands), state, reset_mask=reset[:, a:b], active_mask=active[:, a:b])
+        rows.append(out)
+    assert rel_err(torch.cat(rows, 1), whole) <= 2 * OUT[F32] and rel_err(state, last) <= 2 * STATE[F32]
+
+
+@pytest.mark.parametrize("shape", [(3, 2, 4, 64, 64), (2, 1, 1, 128, 128), (5, 2, 2, 40, 33), (1, 1, 3, 7, 1), (2, 4, 4, 128, 200)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_single_tokens(shape, dtype):
+    B, H, HV, K, V = shape
+    T = 12
+    case = make(B, T, H, HV, K, V, dtype=dtype)
+    gen = torch.Generator().manual_seed(7)
+    reset, active = torch.rand(B, T, generator=gen) < 0.2, torch.rand(B, T, generator=gen) < 0.8
+    want, want_last = recurrence(*(case[n].double() for n in NAMES), K ** -0.5, reset, active)
+    state = case["h0"].cuda()
+    flags = (reset.to(torch.uint8) + 2 * (~active).to(torch.uint8)).cuda()
+    outs = []
+    for t in range(T):
+        before = state.clone()
+        outs.append(hip_gated_delta_step(*(case[n][:, t].cuda() for n in NAMES[:5]), state, flags=flags[:, t]))
+        idle = ~active[:, t].cuda()
+        assert torch.equal(state[idle], before[idle])
+    assert rel_err(torch.stack(outs, 1), want) <= OUT[dtype]
+    assert rel_err(state, want_last) <= 2 ** -16                # fp32 throughout, whatever the operands' type
+
+
+def test_steps_behind_a_prompt():
+    """A prompt in one call, then token by token, as generation runs it."""
+    case = {n: None if t is None else t.cuda() for n, t in make(2, 80, 2, 4, 128, 64, dtype=BF16, carried=False).items()}
+    operands = [case[n] for n in NAMES[:5]]
+    whole, last = hip_gated_delta(*operands)
+    _, state = hip_gated_delta(*(t[:, :70] for t in operands))
+    outs = [hip_gated_delta_step(*(t[:, i] for t in operands), state) for i in range(70, 80)]
+    assert rel_err(torch.stack(outs, 1), whole[:, 70:]) <= 2 * OUT[BF16] and rel_err(state, last) <= 2 * STATE[BF16]
+
+
+def test_gradients_are_differences():
+    """Central differences of the fp32 operator itself along random directions: h = 2^-6 leaves h^2 = 2^-12 of the third
+    derivative and 2^-16 / h = 2^-10 of the results' own deviation."""
+    case = make(1, 70, 1, 2, 16, 16)
+    leaves = [case[n].cuda().requires_grad_(True) for n in NAMES]
+    up, up_state = case["up"].cuda(), case["up_state"].cuda()
+
+    def value(args):
+        out, last = hip_gated_delta(*args)
+        return ((out.double() * up.double()).sum() + (last.double() * up_state.double()).sum())
+
+    grads = torch.autograd.grad(value(leaves), leaves)
+    gen = torch.Generator().manual_seed(2)
+    for i, (leaf, grad) in enumerate(zip(leaves, grads)):
+        way = torch.randn(leaf.shape, generator=gen).cuda()
+        way = way / way.norm()
+        h = 2.0 ** -6
+        with torch.no_grad():
+            moved = [value([t if j != i else t + s * h * way for j, t in enumerate(leaves)]) for s in (1, -1)]
+        difference = float((moved[0] - moved[1]) / (2 * h))
+        along = float((grad.double() * way.double()).sum())
+        assert abs(difference - along) <= 2 ** -8 * float(grad.double().norm()), NAMES[i]
+
+
+def test_only_the_state_or_only_the_output_is_used():
+    case = make(2, 100, 1, 1, 32, 32)
+    leaves = [case[n].cuda().requires_grad_(True) for n in NAMES]
+    full = run(hip_gated_delta, case, None, None, "cuda")[2]
+    out, last = hip_gated_delta(*leaves)
+    first = torch.autograd.grad(out, leaves, case["up"].cuda(), retain_graph=True)
+    second = torch.autograd.grad(last, leaves, case["up_state"].cuda())
+    for name, a, b in zip(NAMES, first, second):
+        assert rel_err(a + b, full[name]) <= 2 * GRAD[F32], name
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(hip_gated_delta(*leaves)[0].sum(), leaves, create_graph=True)[0].sum().backward()
+
+
+def test_other_stream_than_the_tensors():
+    case = make(2, 100, 2, 2, 64, 64, dtype=BF16)
+    want = run(hip_gated_delta, case, None, None, "cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = run(hip_gated_delta, case, None, None, "cuda")
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and all(torch.equal(got[2][n], want[2][n]) for n in NAMES)
+
+
+def test_results_repeat_bit_for_bit():
+    case = make(2, 300, 2, 4, 128, 64, dtype=BF16)
+    first, second = (run(hip_gated_delta, case, None, None, "cuda") for _ in range(2))
+    assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
+    assert all(torch.equal(first[2][n], second[2][n]) for n in NAMES)
