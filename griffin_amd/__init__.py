@@ -12,7 +12,7 @@ from .hip_scan import (
     set_chain_forward,
     set_reproducible,
 )
-from .hip_block_ops import (hip_block_forward, hip_causal_conv, hip_causal_conv_padded, hip_gelu_gate, hip_linear,
+from .hip_block_ops import (hip_block_forward, hip_causal_conv, hip_causal_conv_padded, hip_gelu_gate, hip_group_norm, hip_linear,
                             hip_linear_pair, hip_rmsnorm)
 from .hip_delta import hip_gated_delta, hip_gated_delta_step
 from .modules import (
@@ -36,6 +36,7 @@ __all__ = [
     "hip_gated_delta",
     "hip_gated_delta_step",
     "hip_gelu_gate",
+    "hip_group_norm",
     "hip_linear",
     "hip_linear_pair",
     "hip_rmsnorm",

@@ -79,6 +79,9 @@ _SIGNATURES = {
     "rglru_hip_gated_delta_fwd": (ctypes.c_int, [_P] * 11 + [ctypes.c_int, ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_bwd": (ctypes.c_int, [_P] * 16 + [ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_step": (ctypes.c_int, [_P] * 8 + [ctypes.c_float] + [_I] * 5 + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_group_norm_scratch_bytes": (ctypes.c_size_t, [_I] * 4 + [ctypes.c_int]),
+    "rglru_hip_group_norm_fwd": (ctypes.c_int, [_P] * 6 + [_I] * 4 + [ctypes.c_float] + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_group_norm_bwd": (ctypes.c_int, [_P] * 9 + [_I] * 4 + [ctypes.c_int] * 4 + [_P]),
     "rglru_hip_linear_splits": (ctypes.c_int64, [ctypes.c_int, _I, _I, _I, ctypes.c_int, ctypes.c_int]),
     "rglru_hip_linear": (ctypes.c_int, [ctypes.c_int, _P, _P, _I, _P, _P, _I] + [_P] * 5 + [_I, _P, _P, _I, _I, _I, ctypes.c_int, _P]),
     "rglru_hip_sums": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, _P]),

@@ -2139,6 +2139,95 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> block_infer(
   return std::make_tuple(out, h_last, new_conv, last);
 }
 
+// ---- group norm with an activation, channels last --------------------------------------------------------------------
+
+struct GroupNormShape {
+  int64_t N, L, C, G;
+};
+
+// Parameters in the type that both share; without one of them the other's.
+struct GroupNormParams {
+  Tensor weight, bias;
+  int vec;
+  GroupNormParams(const Tensor& w, const Tensor& b, at::ScalarType dtype) {
+    auto v = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : dtype;
+    if ((b.defined() && b.scalar_type() != v) || !known(v)) v = at::kFloat;
+    weight = as(w, v), bias = as(b, v);
+    vec = code_of(v);
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_forward(const Tensor& x_in, const GroupNormParams& p, const GroupNormShape& z, double eps,
+                                                      int64_t activation, bool need_stats) {
+  c10::DeviceGuard guard(x_in.device());
+  Tensor x = aligned(x_in);
+  Tensor y = fresh_like(x), stats = need_stats ? fresh({z.N, z.G, 2}, at::kFloat, x) : Tensor();
+  if (x.numel() == 0) return {x, y, stats};
+  Tensor scratch = bytes(rglru_hip_group_norm_scratch_bytes(z.N, z.L, z.C, z.G, 0), x);
+  check(rglru_hip_group_norm_fwd(ptr(x), ptr(p.weight), ptr(p.bias), ptr(y), fptr(stats), ptr(scratch), z.N, z.L, z.C, z.G, static_cast<float>(eps),
+                                 static_cast<int>(activation), code_of(x.scalar_type()), p.vec, stream_of(x)), "rglru_hip_group_norm_fwd");
+  return {x, y, stats};
+}
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const MaybeTensor& weight_, const MaybeTensor& bias_, int64_t N, int64_t L, int64_t G,
+                        double eps, int64_t activation) {
+    Tensor weight = opt(weight_), bias = opt(bias_);
+    note_arguments(ctx, {true, weight.defined(), bias.defined()});
+    const GroupNormShape z{N, L, x_in.size(-1), G};
+    GroupNormParams p(weight, bias, x_in.scalar_type());
+    auto [x, y, stats] = group_norm_forward(x_in, p, z, eps, activation, true);
+    ctx->save_for_backward({x, p.weight, p.bias, stats});
+    pack(ctx, {N, L, G, activation, type_or_none(weight), type_or_none(bias), p.vec});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    auto s = ctx->get_saved_variables();
+    auto m = unpack(ctx);
+    const Tensor &x = s[0], &weight = s[1], &bias = s[2], &stats = s[3];
+    Tensor dx, dw, db;
+    {
+      at::NoGradGuard no_grad;
+      c10::DeviceGuard guard(x.device());
+      Needs needs(ctx);
+      Tensor dy = aligned(as(grads[0], x.scalar_type()));
+      const int64_t C = x.size(-1);
+      dx = fresh_like(x);
+      const auto gt = m[6] == RGLRU_BF16 ? at::kBFloat16 : at::kFloat;
+      if (needs(1)) dw = fresh({C}, gt, x);
+      if (needs(2)) db = fresh({C}, gt, x);
+      if (x.numel() > 0) {
+        Tensor scratch = bytes(rglru_hip_group_norm_scratch_bytes(m[0], m[1], C, m[2], 1), x);
+        check(rglru_hip_group_norm_bwd(ptr(x), ptr(weight), ptr(bias), fptr(stats), ptr(dy), ptr(scratch), ptr(dx), ptr(dw), ptr(db), m[0], m[1], C, m[2],
+                                       static_cast<int>(m[3]), code_of(x.scalar_type()), static_cast<int>(m[6]), static_cast<int>(m[6]), stream_of(x)),
+              "rglru_hip_group_norm_bwd");
+      } else {
+        if (dw.defined()) dw.zero_();
+        if (db.defined()) db.zero_();
+      }
+      if (dw.defined()) dw = dw.to(type_at(m, 4));
+      if (db.defined()) db = db.to(type_at(m, 5));
+    }
+    return once({dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight_, const MaybeTensor& bias_, double eps, int64_t activation) {
+  Tensor weight = opt(weight_), bias = opt(bias_);
+  require_gpu("hip_group_norm", {&x, &weight, &bias});
+  require_device_of("hip_group_norm", x, {&weight, &bias});
+  TORCH_CHECK_VALUE(x.dim() >= 2, "hip_group_norm expects [batch, ..., channels], got ", x.sizes());
+  const int64_t C = x.size(-1);
+  TORCH_CHECK_VALUE(groups > 0 && C % groups == 0 && C > 0, "hip_group_norm expects channels in whole groups, got ", C, " channels and ", groups, " groups");
+  for (const Tensor* t : {&weight, &bias})
+    TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 1 && t->numel() == C), "hip_group_norm expects parameters of shape [", C, "], got ", t->sizes());
+  TORCH_CHECK_TYPE(known(x.scalar_type()), "hip_group_norm supports float32 and bfloat16, got ", x.scalar_type());
+  const int64_t N = x.size(0), L = x.numel() == 0 ? 1 : x.numel() / (N * C);
+  if (wants_grad({&x, &weight, &bias})) return GroupNorm::apply(x, maybe(weight), maybe(bias), N, L, groups, eps, activation);
+  at::NoGradGuard no_grad;
+  return std::get<1>(group_norm_forward(x, GroupNormParams(weight, bias, x.scalar_type()), {N, L, C, groups}, eps, activation, false));
+}
+
 // ---- gated delta rule ---------------------------------------------------------------------------------------------
 
 // q, k, v as the kernels read them: the last axis contiguous, the others with strides of their own (parts of one projection go in
@@ -2415,6 +2504,7 @@ PYBIND11_MODULE(_native, m) {
   EXPORT(block_train_packed);
   EXPORT(block_infer);
   EXPORT(rmsnorm);
+  EXPORT(group_norm);
   EXPORT(gated_delta);
   EXPORT(gated_delta_step);
 #undef EXPORT

@@ -243,3 +243,19 @@ def rmsnorm_max_width(dtype: torch.dtype, aligned: bool = True) -> int:
 def hip_rmsnorm(x: Tensor, g: Tensor, eps: float = 1e-6) -> Tensor:
     """``x * rsqrt(mean(x^2, -1) + eps) * (1 + g)`` (griffin/griffin.py:68-80), differentiable in x and g."""
     return _lib.native().rmsnorm(x, g, eps)
+
+
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}               # RGLRU_ACT_* of the C ABI
+
+
+def hip_group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,
+                   activation: str | None = None) -> Tensor:
+    """``act((x - mean) * rsqrt(var + eps) * weight + bias)`` over channels-last features [N, ..., C]; mean and variance are those
+    of a row's positions (the axes in between) and the C / groups channels of a group.  [N, C] has one position: with a group a
+    head, the norm of a recurrence's heads token by token (``hip_group_norm(o.reshape(-1, heads * width), heads, ...)``).
+
+    ``weight``, ``bias`` [C] or None; ``activation``: None, "silu" or "gelu" (the tanh form).  float32 or bfloat16, sums in fp32.
+    Differentiable (first order) in x, weight and bias."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"hip_group_norm knows the activations None, 'silu' and 'gelu', got {activation!r}")
+    return _lib.native().group_norm(x, groups, weight, bias, eps, _ACTIVATIONS[activation])

@@ -400,6 +400,22 @@ int rglru_hip_gated_delta_step(const void* q, const void* k, const void* v, cons
                                const uint8_t* flags, void* out, float scale, int64_t B, int64_t H, int64_t HV, int64_t K, int64_t V,
                                int dtype, int decay_dtype, int beta_dtype, void* stream);
 
+/* ---- group norm with an activation, channels last (no counterpart in the reference) ----------------------------------------
+ *   y = act((x - mean) rsqrt(var + eps) weight + bias),   mean, var over the L positions and C / G channels of a (row, group)
+ * x, y, dy, dx [N, L, C] dense in `dtype`; weight, bias [C] in `vec_dtype`, each may be NULL (1 and 0).  L = 1 normalises every row's
+ * groups by themselves: the heads of a recurrence's output, token by token.
+ *   stats    [N, G, 2] fp32, mean and rsqrt(var + eps): written by the forward call (may be NULL there), read by the backward call
+ *   scratch  rglru_hip_group_norm_scratch_bytes(N, L, C, G, backward) bytes, 16-byte aligned, of each call's own
+ *   dweight, dbias [C] in `grad_dtype`, each may be NULL
+ * Sums are fp32, in a fixed order. */
+enum { RGLRU_ACT_NONE = 0, RGLRU_ACT_SILU = 1, RGLRU_ACT_GELU = 2 /* the tanh form */ };
+size_t rglru_hip_group_norm_scratch_bytes(int64_t N, int64_t L, int64_t C, int64_t G, int backward);
+int rglru_hip_group_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, void* scratch, int64_t N,
+                             int64_t L, int64_t C, int64_t G, float eps, int activation, int dtype, int vec_dtype, void* stream);
+int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias, const float* stats, const void* dy, void* scratch,
+                             void* dx, void* dweight, void* dbias, int64_t N, int64_t L, int64_t C, int64_t G, int activation,
+                             int dtype, int vec_dtype, int grad_dtype, void* stream);
+
 /* Column sums of x[rows, D] (dtype) into out[D] (out_dtype), fp32 accumulation in a fixed order: the
  * bias gradient of the block's three Linear layers (griffin/griffin.py:379-389; autograd of
  * `nn.Linear`: db = sum over tokens of dy), which the caller's BLAS library leaves to a generic reduction.
