@@ -13,17 +13,19 @@
 #pragma once
 
 #include "rglru_device.h"
+#include "rglru_host.h"
 
 namespace rglru {
 
 constexpr int kDeltaChunk = 64;              // tokens of a chunk
 constexpr int kDeltaThreads = 256;
 constexpr int kDeltaMaxKey = 128;            // widest key that the kernels take
-constexpr int kDeltaGates = 136;             // floats per chunk of the gate record: rho[64], write[64], 64 bits of "token counts", padding
+constexpr int kDeltaGates = 136;             // floats per chunk of the gate record: rho[64], w[64], 64 bits that say which tokens count, padding
 constexpr float kDeltaCut = -1e4f;           // a log decay below this discards the history (exp of it is 0 in any type)
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <typename IO> struct Mx;
 
@@ -39,9 +41,15 @@ template <> struct Mx<__bf16> {
   // nearest bf16, and the nearest to what is left: off by at most 2^-9 2^-9 of the value
   static RGLRU_DEVICE void halves(f32x4 v, bf16x4& hi, bf16x4& lo) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) hi[e] = (__bf16)v[e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) lo[e] = (__bf16)(v[e] - (float)hi[e]);
+    for (int e = 0; e < 4; e += 2) {
+      const f32x2 pair = {v[e], v[e + 1]};
+      const bf16x2 h = __builtin_convertvector(pair, bf16x2);
+      const unsigned bits = __builtin_bit_cast(unsigned, h);
+      const f32x2 rest = {v[e] - __uint_as_float(bits << 16), v[e + 1] - __uint_as_float(bits & 0xffff0000u)};
+      const bf16x2 l = __builtin_convertvector(rest, bf16x2);
+      hi[e] = h[0], hi[e + 1] = h[1];
+      lo[e] = l[0], lo[e + 1] = l[1];
+    }
   }
   static RGLRU_DEVICE Wide wide(f32x4 a, f32x4 b) {
     bf16x4 ah, al, bh, bl;
@@ -162,7 +170,7 @@ struct DeltaArgs {
   long long q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
   int B, T, H, HV, K, V, nC, columns;       // columns: V in whole tiles of 16
   int decay_dtype, beta_dtype;
-  int vec_q, vec_k;                         // rows of q and k can be read as 16-byte vectors
+  int width;                                // of the rows of q and k as the kernels read them: K in whole 16-byte vectors
   float scale;
 };
 
@@ -207,18 +215,18 @@ RGLRU_DEVICE ChunkGates chunk_gates(const DeltaArgs& p, int b, int hv, int n, in
   return r;
 }
 
-// Rows of keys or queries of a chunk as an LDS tile, zeros where a token does not count or the tile is wider than the key.
-// The vectors are requested into registers and put down later, so that a whole chunk's work lies between the two.
+// Rows of keys, queries or upstream gradients of a chunk as an LDS tile, zeros where a token does not count or the tile is wider than
+// the row.  The vectors are requested into registers and put down later.
 template <typename IO, int COLS, int THREADS> struct KeyRows {
   typedef Tile<IO, COLS> T;
   static constexpr int N = kDeltaChunk * T::U / THREADS;   // vectors a thread
   i32x4 v[N];
-  RGLRU_DEVICE void request(const IO* rows, long long stride, int width, int left, unsigned long long counts, bool vec, int tid) {
+  RGLRU_DEVICE void request(const IO* rows, long long stride, int width, unsigned long long counts, bool vec, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = tid + i * THREADS, row = at / T::U, col = at % T::U * T::E;
       v[i] = i32x4{0, 0, 0, 0};
-      if (row < left && ((counts >> row) & 1) && col < width) {
+      if (((counts >> row) & 1) && col < width) {
         const IO* src = rows + (long long)row * stride + col;
         if (vec) {
           v[i] = *reinterpret_cast<const i32x4*>(src);
@@ -263,16 +271,135 @@ template <typename IO, int ROWS, int COLS, int THREADS> struct MatrixRows {
   }
 };
 
-// One element of a [tokens, columns] tensor a lane: rows 16 mt + 4 g + e of the chunk, one column.
-template <typename IO> struct ColumnIo {
-  rsrc_t rows;
-  unsigned row_bytes, col_bytes;
-  RGLRU_DEVICE ColumnIo(const IO* base, long long stride, int col, bool live)
-      : rows(make_rsrc(base, 0x40000000u)), row_bytes((unsigned)(stride * (long long)sizeof(IO))), col_bytes(live ? (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange) {}
-  RGLRU_DEVICE unsigned at(int row, bool ok) const { return ok && col_bytes != kOutOfRange ? (unsigned)row * row_bytes + col_bytes : kOutOfRange; }
-  RGLRU_DEVICE float load(int row, bool ok) const { return BufIo<IO>::load(rows, at(row, ok), 0); }
-  RGLRU_DEVICE void store(int row, bool ok, float v) const { BufIo<IO>::store((IO)v, rows, at(row, ok), 0); }
+RGLRU_DEVICE i32x4 delta_rsrc(const void* base, unsigned bytes) {
+  const unsigned long long at = (unsigned long long)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)at);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(at >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00020000;
+  return r;
+}
+RGLRU_DEVICE unsigned lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const __attribute__((address_space(3))) char*)p);
+}
+// Sixteen bytes a lane from memory to LDS, once or four times `STEP` bytes apart there; the wave's lanes lie one behind the other from
+// `lds` on, offsets past the descriptor's extent give zeros.  The compiler does not count these loads: whoever reads the tile waits for all
+// of the wave's (and for the other waves' at a barrier).  The wait states in front are for a descriptor that a vector instruction has
+// just written (a uniform value, or one that was put aside).
+RGLRU_DEVICE void memory_to_lds(i32x4 r, unsigned off, unsigned lds) {
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+}
+template <int STEP> RGLRU_DEVICE void memory_to_lds(i32x4 r, unsigned off0, unsigned off1, unsigned off2, unsigned off3, unsigned lds) {
+  asm volatile(
+      "s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds" ::"s"(lds),
+      "v"(off0), "v"(off1), "v"(off2), "v"(off3), "s"(r), "n"(STEP)
+      : "memory", "m0", "scc");
+}
+RGLRU_DEVICE void wait_for_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A row-major matrix on its way into an LDS tile.
+template <typename IO, int ROWS, int COLS, int THREADS> struct TileLoad {
+  typedef Tile<IO, COLS> T;
+  static constexpr int kBytes = ROWS * COLS * (int)sizeof(IO), N = ROWS * T::U / THREADS;
+  static_assert(N * THREADS == ROWS * T::U, "whole vectors a thread");
+  unsigned off[N];
+  RGLRU_DEVICE void setup(int tid, long long stride, int width) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = tid + i * THREADS, row = at / T::U, col = ((at % T::U) ^ ((row >> T::kShift) & T::kMask)) * T::E;
+      off[i] = col < width ? (unsigned)row * (unsigned)(stride * (int)sizeof(IO)) + (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange;
+    }
+  }
+  // bytes from the first element to the end of the last of `rows` rows
+  static RGLRU_DEVICE unsigned extent(long long stride, int width, int rows) {
+    rows = rows < ROWS ? rows : ROWS;
+    return rows > 0 ? (unsigned)((rows - 1) * stride + width) * (unsigned)sizeof(IO) : 0u;
+  }
+  RGLRU_DEVICE void request(i32x4 r, unsigned lds, int wave) const {
+    constexpr int STEP = THREADS * 16;
+    lds += (unsigned)wave * 1024u;
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) memory_to_lds<STEP>(r, off[i], off[i + 1], off[i + 2], off[i + 3], lds + (unsigned)(i * STEP));
+#pragma unroll
+    for (int i = N / 4 * 4; i < N; ++i) memory_to_lds(r, off[i], lds + (unsigned)(i * STEP));
+  }
 };
+
+// One element of a [tokens, columns] tensor a lane: rows 16 mt + 4 g + e of a chunk, one column.  Rows past the `rows` there are read
+// as zeros and not written.
+template <typename IO> struct ColumnIo {
+  rsrc_t rsrc;
+  unsigned row_bytes, first;
+  RGLRU_DEVICE ColumnIo(const IO* base, long long stride, int rows, int width, int col, bool live, int g)
+      : rsrc(make_rsrc(base, (unsigned)(((rows < kDeltaChunk ? rows : kDeltaChunk) - 1) * stride + width) * (unsigned)sizeof(IO))),
+        row_bytes((unsigned)(stride * (long long)sizeof(IO))),
+        first(live ? (unsigned)(4 * g) * row_bytes + (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange) {}
+  // the offset of a lane without a column stays out of range: at most 64 rows of 2^22 elements are added to it, modulo 2^32
+  RGLRU_DEVICE unsigned at(int mt, int e) const { return first == kOutOfRange ? kOutOfRange : first + (unsigned)(16 * mt + e) * row_bytes; }
+  // as it lies in memory, so that nothing waits for it before it is used
+  static RGLRU_DEVICE float value(int raw) { return sizeof(IO) == 2 ? __uint_as_float((unsigned)raw << 16) : __uint_as_float((unsigned)raw); }
+  RGLRU_DEVICE int raw(int mt, int e) const {
+    if constexpr (sizeof(IO) == 2) return (int)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(mt, e), 0, 0);
+    else return (int)__builtin_amdgcn_raw_buffer_load_b32(rsrc, at(mt, e), 0, 0);
+  }
+  RGLRU_DEVICE void store(int mt, int e, float v) const { BufIo<IO>::store((IO)v, rsrc, at(mt, e), 0); }
+};
+
+// What a walk along the chunks has in LDS of one chunk, and how it gets there.  Two of them where they fit: the next chunk's is
+// filled while this one's is worked on.
+template <typename IO, int KS, int THREADS, bool OUT> struct ChunkTiles {
+  static constexpr int DK = 32 * KS, PL = Mx<IO>::kPlanes;
+  typedef TileLoad<IO, 64, DK, THREADS> KeyLoad;
+  typedef TileLoad<IO, PL * 64, 64, THREADS> SquareLoad;
+  static constexpr int kKeys = 0, kSolve = KeyLoad::kBytes, kQueries = kSolve + SquareLoad::kBytes,
+                       kWithin = kQueries + (OUT ? KeyLoad::kBytes : 0), kRecord = kWithin + (OUT ? SquareLoad::kBytes : 0),
+                       kBytes = kRecord + 1024;             // the record: one vector a lane of one wave
+  static constexpr int kStages = 2 * kBytes <= 160 * 1024 ? 2 : 1;
+  KeyLoad k, q;
+  SquareLoad square;
+  unsigned record;
+  RGLRU_DEVICE void setup(const DeltaArgs& p, int tid) {
+    k.setup(tid, p.k_t, p.width);
+    if constexpr (OUT) q.setup(tid, p.q_t, p.width);
+    square.setup(tid, 64, 64);
+    record = (tid & 63) * 16 < kDeltaGates * 4 ? (unsigned)(tid & 63) * 16u : kOutOfRange;
+  }
+  RGLRU_DEVICE void request(const DeltaArgs& p, long long chunk, int n, int b, int h, unsigned lds, int wave) const {
+    const int t0 = n * kDeltaChunk, left = p.T - t0;
+    const i32x4 rk = delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left));
+    const i32x4 rs = delta_rsrc((const IO*)p.solve + chunk * (4096 * PL), SquareLoad::kBytes);
+    const i32x4 rq = delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, OUT ? KeyLoad::extent(p.q_t, p.width, left) : 0u);
+    const i32x4 rw = delta_rsrc((const IO*)p.within + chunk * (4096 * PL), SquareLoad::kBytes);
+    const i32x4 rr = delta_rsrc(p.gates + chunk * kDeltaGates, kDeltaGates * 4);
+    k.request(rk, lds + kKeys, wave);
+    square.request(rs, lds + kSolve, wave);
+    if constexpr (OUT) {
+      q.request(rq, lds + kQueries, wave);
+      square.request(rw, lds + kWithin, wave);
+    }
+    if (wave == 0) memory_to_lds(rr, record, lds + kRecord);
+  }
+  // zeros for the rows of tokens that do not count
+  static RGLRU_DEVICE void clear_rows(unsigned char* stage, unsigned long long counts, int tid) {
+    for (int at = tid; at < 64 * KeyLoad::T::U; at += THREADS) {
+      const int row = at / KeyLoad::T::U;
+      if ((counts >> row) & 1) continue;
+      *reinterpret_cast<i32x4*>(stage + kKeys + at * 16) = i32x4{0, 0, 0, 0};
+      if constexpr (OUT) *reinterpret_cast<i32x4*>(stage + kQueries + at * 16) = i32x4{0, 0, 0, 0};
+    }
+  }
+};
+RGLRU_DEVICE unsigned long long counts_of(const float* record) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(__float_as_uint(record[128])), hi = __builtin_amdgcn_readfirstlane(__float_as_uint(record[129]));
+  return (unsigned long long)lo | (unsigned long long)hi << 32;
+}
+
+// Whether a walk's workgroups are of two waves instead of four: where those of four leave compute units without one.
+inline bool delta_narrow(const DeltaArgs& a) { return (long long)(a.columns + 63) / 64 * a.B * a.HV < num_compute_units(); }
 
 // XCDs take workgroups round-robin; each gets a contiguous run of the work, so that neighbours share its L2.  -1: none left.
 RGLRU_DEVICE int xcd_order(int block, int total) {

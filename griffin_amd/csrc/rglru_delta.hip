@@ -56,13 +56,13 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long chunk = blockIdx.x;
   const int n = (int)(chunk % p.nC), head = (int)(chunk / p.nC), hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
-  const int t0 = n * kDeltaChunk, left = p.T - t0;
+  const int t0 = n * kDeltaChunk;
   const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
   const unsigned long long counts = __ballot(gate.counts);
   {
     KeyRows<IO, DK, kDeltaThreads> k, q;
-    k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
-    q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
+    k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, true, tid);
+    q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, true, tid);
     if (wave == 0) {
       total[lane] = gate.total;
       beta[lane] = gate.beta;
@@ -130,25 +130,59 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
 }
 
 // The walk along the chunks.  SAVE: what the backward pass needs is left behind; OUT: the outputs are wanted.
-template <typename IO, int KS, bool SAVE, bool OUT>
-__global__ __launch_bounds__(kDeltaThreads) void delta_forward_kernel(DeltaArgs p) {
+// A chunk's results are stored in front of the next one's requests: behind them, the wait for the requests would be one for the stores.
+template <typename IO, int KS, int WAVES, bool SAVE, bool OUT>
+__global__ __launch_bounds__(64 * WAVES, 1) void delta_forward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
-  constexpr int DK = 32 * KS, PL = M::kPlanes;
+  constexpr int DK = 32 * KS, PL = M::kPlanes, THREADS = 64 * WAVES, COLUMNS = 16 * WAVES;
   typedef Tile<IO, DK> Keys;
   typedef Tile<IO, 64> Square;
-  __shared__ __attribute__((aligned(16))) IO keys[64 * DK], queries[OUT ? 64 * DK : 8], solve[PL * 4096], within[OUT ? PL * 4096 : 8];
-  __shared__ __attribute__((aligned(16))) float gates[kDeltaGates];
+  typedef ChunkTiles<IO, KS, THREADS, OUT> Tiles;
+  constexpr int STAGES = Tiles::kStages;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * Tiles::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = (p.columns + 63) >> 6, total = groups * p.B * p.HV;
+  const int groups = (p.columns + COLUMNS - 1) / COLUMNS, total = groups * p.B * p.HV;
   const int work = xcd_order(blockIdx.x, total);
   if (work < 0) return;
   const int group = work % groups, head = work / groups, hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
-  const int col = group * 64 + wave * 16 + c;
-  const bool mine = group * 64 + wave * 16 < p.columns, live = mine && col < p.V;
+  const int col = group * COLUMNS + wave * 16 + c;
+  const bool mine = group * COLUMNS + wave * 16 < p.columns, live = mine && col < p.V;
+  const long long first = (long long)head * p.nC;
+  const unsigned lds0 = lds_address(lds);
 
-  f32x4 state[2 * KS];
+  Tiles tiles;
+  tiles.setup(p, tid);
+  f32x4 state[2 * KS], o[4], z[4];
+  int v[4][4];
+  auto request = [&](int n, int stage) {
+    tiles.request(p, first + n, n, b, h, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
+    const int t0 = n * kDeltaChunk;
+    const ColumnIo<IO> values((const IO*)p.v + b * p.v_b + t0 * p.v_t + hv * p.v_h, p.v_t, p.T - t0, p.V, col, live, g);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[mt][e] = values.raw(mt, e);
+  };
+  auto put = [&](int n) {                                  // results of chunk n
+    if constexpr (SAVE) {
+      if (mine) {
+        IO* at = (IO*)p.values + ((first + n) * PL * p.columns + col) * 64;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, z[mt]);
+      }
+    }
+    if constexpr (OUT) {
+      const int t0 = n * kDeltaChunk;
+      const ColumnIo<IO> out((const IO*)p.out + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out.store(mt, e, o[mt][e]);
+    }
+  };
+  request(0, 0);
 #pragma unroll
   for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
@@ -156,122 +190,117 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_forward_kernel(DeltaArgs 
       const int row = 16 * t + 4 * g + e;
       state[t][e] = p.h0 && live && row < p.K ? p.h0[((long long)head * p.K + row) * p.V + col] : 0.f;
     }
-
-  KeyRows<IO, DK, kDeltaThreads> next_k, next_q;
-  MatrixRows<IO, 64, 64, kDeltaThreads> next_solve, next_within;
-  float next_gate = 0.f;
-  const long long first = (long long)head * p.nC;
-  auto request = [&](int n) {
-    const long long chunk = first + n;
-    const float* record = p.gates + chunk * kDeltaGates;
-    const unsigned long long counts = (unsigned long long)__float_as_uint(record[128]) | (unsigned long long)__float_as_uint(record[129]) << 32;
-    const int t0 = n * kDeltaChunk, left = p.T - t0;
-    next_k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
-    next_solve.request((const IO*)p.solve + chunk * (4096 * PL), 4096, 64, tid);
-    if constexpr (OUT) {
-      next_q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
-      next_within.request((const IO*)p.within + chunk * (4096 * PL), 4096, 64, tid);
-    }
-    if (tid < kDeltaGates) next_gate = record[tid];
-  };
-  request(0);
+  wait_for_all();
   for (int n = 0; n < p.nC; ++n) {
-    const long long chunk = first + n;
-    const int t0 = n * kDeltaChunk, left = p.T - t0;
-    if (n) __syncthreads();                                // the tiles of the chunk before have been read
-    next_k.put(keys, tid);
-    next_solve.put(solve, tid);
-    if constexpr (OUT) next_q.put(queries, tid), next_within.put(within, tid);
-    if (tid < kDeltaGates) gates[tid] = next_gate;
-    __syncthreads();
-    if (n + 1 < p.nC) request(n + 1);
-    if (!mine) continue;
-    const unsigned long long counts = (unsigned long long)__float_as_uint(gates[128]) | (unsigned long long)__float_as_uint(gates[129]) << 32;
-    const ColumnIo<IO> values((const IO*)p.v + b * p.v_b + t0 * p.v_t + hv * p.v_h, p.v_t, col, live);
-    f32x4 r[4], rho[4];
+    const int stage = STAGES == 2 ? n & 1 : 0;
+    unsigned char* tile = lds + stage * Tiles::kBytes;
+    const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
+             *within = (const IO*)(tile + Tiles::kWithin);
+    const float* record = (const float*)(tile + Tiles::kRecord);
+    const unsigned long long counts = counts_of(record);
+    f32x4 r[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = 16 * mt + 4 * g + e;
-        r[mt][e] = values.load(row, (counts >> row) & 1);
-      }
+      for (int e = 0; e < 4; ++e) r[mt][e] = ColumnIo<IO>::value(v[mt][e]);
+    if (counts != ~0ull) {
+      Tiles::clear_rows(tile, counts, tid);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(gates + 16 * mt + 4 * g);
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[mt][e] = (counts >> (16 * mt + 4 * g + e)) & 1 ? r[mt][e] : 0.f;
+      lds_barrier();
+    }
     Wide s[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) s[ks] = M::wide(state[2 * ks], state[2 * ks + 1]);
+    if (n) put(n - 1);
     if constexpr (SAVE) {
-      IO* at = (IO*)p.states + (chunk * PL * p.columns + col) * DK;
+      if (mine) {
+        IO* at = (IO*)p.states + ((first + n) * PL * p.columns + col) * DK;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, state[t]);
+        for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, state[t]);
+      }
     }
-    // R = V - rho K S
-    {
+    if (STAGES == 2 && n + 1 < p.nC) request(n + 1, stage ^ 1);
+    if (mine) {
+      f32x4 rho[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(record + 16 * mt + 4 * g);
+      const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
+      // R = V - rho K S; where nothing is carried into a document, nothing of it is read either, whatever it is
       f32x4 acc[4] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) acc[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), s[ks], acc[mt]);
+      if (carry == 0.f) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mt][e] = rho[mt][e] == 0.f ? 0.f : acc[mt][e];
+      }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[mt][e] = rho[mt][e] == 0.f ? r[mt][e] : fmaf(-rho[mt][e], acc[mt][e], r[mt][e]);
-    }
-    // Z = T R
-    f32x4 z[4] = {};
-    {
-      const Wide rw[2] = {M::wide(r[0], r[1]), M::wide(r[2], r[3])};
+        for (int e = 0; e < 4; ++e) r[mt][e] = fmaf(-rho[mt][e], acc[mt][e], r[mt][e]);
+      // Z = T R
+      {
+        const Wide rw[2] = {M::wide(r[0], r[1]), M::wide(r[2], r[3])};
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int mt = 0; mt < 4; ++mt) z[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int mt = 2 * ks; mt < 4; ++mt) z[mt] = M::ww(Square::wide_down_rows(solve, 4096, 32 * ks, 16 * mt, lane), rw[ks], z[mt]);
-    }
-    if constexpr (SAVE) {
-      IO* at = (IO*)p.values + (chunk * PL * p.columns + col) * 64;
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, z[mt]);
-    }
-    if constexpr (OUT) {
-      const Wide zw[2] = {M::wide(z[0], z[1]), M::wide(z[2], z[3])};
-      f32x4 o[4] = {};
+          for (int mt = 2 * ks; mt < 4; ++mt) z[mt] = M::ww(Square::wide_down_rows(solve, 4096, 32 * ks, 16 * mt, lane), rw[ks], z[mt]);
+      }
+      // S' = rho_63 S + K^T (w Z)
+      {
+        f32x4 wz[4];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int mt = 0; mt < 4; ++mt) wz[mt] = z[mt] * *reinterpret_cast<const f32x4*>(record + 64 + 16 * mt + 4 * g);
+        const Wide zw[2] = {M::wide(wz[0], wz[1]), M::wide(wz[2], wz[3])};
+        if (carry == 0.f) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) o[mt] = M::ew(Keys::along_row(queries, 16 * mt + c, 32 * ks, g), s[ks], o[mt]);
+          for (int t = 0; t < 2 * KS; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][e] = rho[mt][e] == 0.f ? 0.f : o[mt][e] * (p.scale * rho[mt][e]);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int mt = 2 * ks; mt < 4; ++mt) o[mt] = M::ww(Square::wide_down_rows(within, 4096, 32 * ks, 16 * mt, lane), zw[ks], o[mt]);
-      const ColumnIo<IO> out((const IO*)p.out + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, col, live);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 16 * mt + 4 * g + e;
-          out.store(row, row < left, o[mt][e]);
+          for (int t = 0; t < 2 * KS; ++t) state[t] *= carry;
         }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int t = 0; t < 2 * KS; ++t) state[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), zw[ks], state[t]);
+      }
+      if constexpr (OUT) {
+        const Wide zw[2] = {M::wide(z[0], z[1]), M::wide(z[2], z[3])};
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) o[mt] = M::ew(Keys::along_row(queries, 16 * mt + c, 32 * ks, g), s[ks], o[mt]);
+        if (carry == 0.f) {
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][e] = rho[mt][e] == 0.f ? 0.f : o[mt][e];
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[mt] *= rho[mt] * p.scale;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int mt = 2 * ks; mt < 4; ++mt) o[mt] = M::ww(Square::wide_down_rows(within, 4096, 32 * ks, 16 * mt, lane), zw[ks], o[mt]);
+      }
     }
-    // S' = rho_63 S + K^T (w Z)
-    {
-      const float carry = gates[63];
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) z[mt] *= *reinterpret_cast<const f32x4*>(gates + 64 + 16 * mt + 4 * g);
-      const Wide zw[2] = {M::wide(z[0], z[1]), M::wide(z[2], z[3])};
-#pragma unroll
-      for (int t = 0; t < 2 * KS; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) state[t][e] = carry == 0.f ? 0.f : carry * state[t][e];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) state[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), zw[ks], state[t]);
+    if (STAGES == 1 && n + 1 < p.nC) {
+      lds_barrier();                                       // the tiles have been read
+      request(n + 1, 0);
     }
+    wait_for_all();
   }
+  put(p.nC - 1);
   if (p.h_last && live) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
@@ -283,15 +312,37 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_forward_kernel(DeltaArgs 
   }
 }
 
+template <typename IO, int KS, int WAVES> static void delta_walk_forward(const DeltaArgs& a, bool save, hipStream_t s) {
+  const int total = (a.columns + 16 * WAVES - 1) / (16 * WAVES) * a.B * a.HV;
+  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(64 * WAVES);
+  if (save) hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, true, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, false, true>), grid, block, 0, s, a);
+}
+
 template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool save, hipStream_t s) {
   hipLaunchKernelGGL((delta_prepare_kernel<IO, KS>), dim3((unsigned)((long long)a.B * a.HV * a.nC)), dim3(kDeltaThreads), 0, s, a);
   int rc = check_launch("gated_delta_fwd prepare");
   if (rc) return rc;
-  const int total = (a.columns + 63) / 64 * a.B * a.HV;
-  const dim3 grid((unsigned)((total + 7) / 8 * 8));
-  if (save) hipLaunchKernelGGL((delta_forward_kernel<IO, KS, true, true>), grid, dim3(kDeltaThreads), 0, s, a);
-  else hipLaunchKernelGGL((delta_forward_kernel<IO, KS, false, true>), grid, dim3(kDeltaThreads), 0, s, a);
+  if (delta_narrow(a)) delta_walk_forward<IO, KS, 2>(a, save, s);
+  else delta_walk_forward<IO, KS, 4>(a, save, s);
   return check_launch("gated_delta_fwd");
+}
+
+// Keys that are no whole 16-byte vectors, as rows that are, zeros behind them.
+template <typename IO> __global__ __launch_bounds__(256) void delta_pad_kernel(DeltaArgs p, IO* q, IO* k) {
+  const long long rows = (long long)p.B * p.T * p.H, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= rows * p.width) return;
+  const long long row = i / p.width;
+  const int col = (int)(i % p.width), h = (int)(row % p.H);
+  const long long token = row / p.H, b = token / p.T, t = token % p.T;
+  q[i] = col < p.K ? ((const IO*)p.q)[b * p.q_b + t * p.q_t + h * p.q_h + col] : (IO)0.f;
+  k[i] = col < p.K ? ((const IO*)p.k)[b * p.k_b + t * p.k_t + h * p.k_h + col] : (IO)0.f;
+}
+int delta_launch_pad(const DeltaArgs& a, void* q, void* k, int dtype, hipStream_t s) {
+  const long long n = (long long)a.B * a.T * a.H * a.width;
+  if (dtype == RGLRU_BF16) hipLaunchKernelGGL((delta_pad_kernel<__bf16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, (__bf16*)q, (__bf16*)k);
+  else hipLaunchKernelGGL((delta_pad_kernel<float>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, (float*)q, (float*)k);
+  return check_launch("gated_delta_fwd keys");
 }
 
 int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s) {

@@ -19,25 +19,55 @@
 
 namespace rglru {
 
-template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void delta_backward_kernel(DeltaArgs p) {
+template <typename IO, int KS, int WAVES> __global__ __launch_bounds__(64 * WAVES, 1) void delta_backward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
-  constexpr int DK = 32 * KS, PL = M::kPlanes;
+  constexpr int DK = 32 * KS, PL = M::kPlanes, THREADS = 64 * WAVES, COLUMNS = 16 * WAVES;
   typedef Tile<IO, DK> Keys;
   typedef Tile<IO, 64> Square;
-  __shared__ __attribute__((aligned(16))) IO keys[64 * DK], queries[64 * DK], solve[PL * 4096], within[PL * 4096];
-  __shared__ __attribute__((aligned(16))) float gates[kDeltaGates];
+  typedef ChunkTiles<IO, KS, THREADS, true> Tiles;
+  constexpr int STAGES = Tiles::kStages;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * Tiles::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = (p.columns + 63) >> 6, total = groups * p.B * p.HV;
+  const int groups = (p.columns + COLUMNS - 1) / COLUMNS, total = groups * p.B * p.HV;
   const int work = xcd_order(blockIdx.x, total);
   if (work < 0) return;
   const int group = work % groups, head = work / groups, hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
-  const int col = group * 64 + wave * 16 + c;
-  const bool mine = group * 64 + wave * 16 < p.columns, live = mine && col < p.V;
+  const int col = group * COLUMNS + wave * 16 + c;
+  const bool mine = group * COLUMNS + wave * 16 < p.columns, live = mine && col < p.V;
+  const long long first = (long long)head * p.nC;
+  const unsigned lds0 = lds_address(lds);
 
-  f32x4 dstate[2 * KS];
+  Tiles tiles;
+  tiles.setup(p, tid);
+  f32x4 dstate[2 * KS], y[4];
+  int up_raw[4][4];
+  auto request = [&](int n, int stage) {
+    tiles.request(p, first + n, n, b, h, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
+    const int t0 = n * kDeltaChunk;
+    const ColumnIo<IO> ups((const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) up_raw[mt][e] = ups.raw(mt, e);
+  };
+  auto put = [&](int n) {                                  // results of chunk n
+    if (mine) {
+      IO* at = (IO*)p.dvalues + ((first + n) * PL * p.columns + col) * 64;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, y[mt]);
+    }
+    const int t0 = n * kDeltaChunk;
+    const ColumnIo<IO> out((const IO*)p.dv + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out.store(mt, e, y[mt][e]);
+  };
+  const int last = p.nC - 1;
+  request(last, 0);
 #pragma unroll
   for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
@@ -45,111 +75,74 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
       const int row = 16 * t + 4 * g + e;
       dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
     }
-
-  KeyRows<IO, DK, kDeltaThreads> next_k, next_q;
-  MatrixRows<IO, 64, 64, kDeltaThreads> next_solve, next_within;
-  float next_gate = 0.f;
-  const long long first = (long long)head * p.nC;
-  auto request = [&](int n) {
-    const long long chunk = first + n;
-    const float* record = p.gates + chunk * kDeltaGates;
-    const unsigned long long counts = (unsigned long long)__float_as_uint(record[128]) | (unsigned long long)__float_as_uint(record[129]) << 32;
-    const int t0 = n * kDeltaChunk, left = p.T - t0;
-    next_k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
-    next_q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
-    next_solve.request((const IO*)p.solve + chunk * (4096 * PL), 4096, 64, tid);
-    next_within.request((const IO*)p.within + chunk * (4096 * PL), 4096, 64, tid);
-    if (tid < kDeltaGates) next_gate = record[tid];
-  };
-  request(p.nC - 1);
-  for (int n = p.nC - 1; n >= 0; --n) {
-    const long long chunk = first + n;
-    const int t0 = n * kDeltaChunk, left = p.T - t0;
-    if (n != p.nC - 1) __syncthreads();                    // the tiles of the chunk behind have been read
-    next_k.put(keys, tid);
-    next_q.put(queries, tid);
-    next_solve.put(solve, tid);
-    next_within.put(within, tid);
-    if (tid < kDeltaGates) gates[tid] = next_gate;
-    __syncthreads();
-    if (n > 0) request(n - 1);
-    if (!mine) continue;
-    const unsigned long long counts = (unsigned long long)__float_as_uint(gates[128]) | (unsigned long long)__float_as_uint(gates[129]) << 32;
-    const ColumnIo<IO> ups((const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, col, live);
-    f32x4 up[4], rho[4];
+  wait_for_all();
+  for (int n = last; n >= 0; --n) {
+    const int stage = STAGES == 2 ? (last - n) & 1 : 0;
+    unsigned char* tile = lds + stage * Tiles::kBytes;
+    const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
+             *within = (const IO*)(tile + Tiles::kWithin);
+    const float* record = (const float*)(tile + Tiles::kRecord);
+    const unsigned long long counts = counts_of(record);
+    f32x4 up[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = 16 * mt + 4 * g + e;
-        up[mt][e] = ups.load(row, (counts >> row) & 1);
-      }
+      for (int e = 0; e < 4; ++e) up[mt][e] = ColumnIo<IO>::value(up_raw[mt][e]);
+    if (counts != ~0ull) {
+      Tiles::clear_rows(tile, counts, tid);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(gates + 16 * mt + 4 * g);
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) up[mt][e] = (counts >> (16 * mt + 4 * g + e)) & 1 ? up[mt][e] : 0.f;
+      lds_barrier();
+    }
     Wide d[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) d[ks] = M::wide(dstate[2 * ks], dstate[2 * ks + 1]);
-    {
-      IO* at = (IO*)p.dstates + (chunk * PL * p.columns + col) * DK;
+    if (n != last) put(n + 1);
+    if (mine) {
+      IO* at = (IO*)p.dstates + ((first + n) * PL * p.columns + col) * DK;
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, dstate[t]);
     }
-    // dZ = P^T dO + w K dS'
-    f32x4 dz[4] = {};
+    if (STAGES == 2 && n > 0) request(n - 1, stage ^ 1);
+    if (mine) {
+      f32x4 rho[4];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(record + 16 * mt + 4 * g);
+      const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
+      // dZ = P^T dO + w K dS'
+      f32x4 dz[4] = {};
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) dz[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), d[ks], dz[mt]);
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(gates + 64 + 16 * mt + 4 * g);
+        for (int mt = 0; mt < 4; ++mt) dz[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), d[ks], dz[mt]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dz[mt][e] = w[e] == 0.f ? 0.f : w[e] * dz[mt][e];
-    }
-    {
-      const Frag uf[2] = {M::exact(up[0], up[1]), M::exact(up[2], up[3])};
+      for (int mt = 0; mt < 4; ++mt) dz[mt] *= *reinterpret_cast<const f32x4*>(record + 64 + 16 * mt + 4 * g);
+      {
+        const Frag uf[2] = {M::exact(up[0], up[1]), M::exact(up[2], up[3])};
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int mt = 0; mt < 2 * ks + 2; ++mt) dz[mt] = M::we(Square::wide_along_row(within, 4096, 16 * mt + c, 32 * ks, g), uf[ks], dz[mt]);
-    }
-    // Y = T^T dZ
-    f32x4 y[4] = {};
-    {
-      const Wide zw[2] = {M::wide(dz[0], dz[1]), M::wide(dz[2], dz[3])};
+          for (int mt = 0; mt < 2 * ks + 2; ++mt) dz[mt] = M::we(Square::wide_along_row(within, 4096, 16 * mt + c, 32 * ks, g), uf[ks], dz[mt]);
+      }
+      // Y = T^T dZ
+      {
+        const Wide zw[2] = {M::wide(dz[0], dz[1]), M::wide(dz[2], dz[3])};
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int mt = 0; mt < 2 * ks + 2; ++mt) y[mt] = M::ww(Square::wide_along_row(solve, 4096, 16 * mt + c, 32 * ks, g), zw[ks], y[mt]);
-    }
-    {
-      IO* at = (IO*)p.dvalues + (chunk * PL * p.columns + col) * 64;
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, y[mt]);
-      const ColumnIo<IO> out((const IO*)p.dv + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, col, live);
+          for (int mt = 0; mt < 2 * ks + 2; ++mt) y[mt] = M::ww(Square::wide_along_row(solve, 4096, 16 * mt + c, 32 * ks, g), zw[ks], y[mt]);
+      }
+      // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y)
+      f32x4 ry[4];
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int mt = 0; mt < 4; ++mt) ry[mt] = -rho[mt] * y[mt], up[mt] *= rho[mt] * p.scale;
+      const Wide uw[2] = {M::wide(up[0], up[1]), M::wide(up[2], up[3])}, yw[2] = {M::wide(ry[0], ry[1]), M::wide(ry[2], ry[3])};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 16 * mt + 4 * g + e;
-          out.store(row, row < left, y[mt][e]);
-        }
-    }
-    // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y)
-    {
-      const float carry = gates[63];
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          up[mt][e] *= p.scale * rho[mt][e];
-          y[mt][e] *= -rho[mt][e];
-        }
-      const Wide uw[2] = {M::wide(up[0], up[1]), M::wide(up[2], up[3])}, yw[2] = {M::wide(y[0], y[1]), M::wide(y[2], y[3])};
-#pragma unroll
-      for (int t = 0; t < 2 * KS; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dstate[t][e] = carry == 0.f ? 0.f : carry * dstate[t][e];
+      for (int t = 0; t < 2 * KS; ++t) dstate[t] *= carry;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -158,7 +151,13 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
           dstate[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), yw[ks], dstate[t]);
         }
     }
+    if (STAGES == 1 && n > 0) {
+      lds_barrier();                                       // the tiles have been read
+      request(n - 1, 0);
+    }
+    wait_for_all();
   }
+  put(0);
   if (p.dh0 && live) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
@@ -207,8 +206,8 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
     const float carry = gate.segments == 0 ? expf((float)gate.end) : 0.f;
     if (s == 0) {
       KeyRows<IO, DK, kDeltaThreads> k, q;
-      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.K, left, counts, p.vec_k, tid);
-      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.K, left, counts, p.vec_q, tid);
+      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, true, tid);
+      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, true, tid);
       k.put(keys, tid);
       q.put(queries, tid);
     } else {
@@ -229,7 +228,7 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
       KeyRows<IO, CB, kDeltaThreads> up;
       MatrixRows<IO, CB, 64, kDeltaThreads> z, y;
       MatrixRows<IO, CB, DK, kDeltaThreads> st, ds;
-      up.request(ups + c0, (long long)p.HV * p.V, p.V - c0, left, counts, vec_up, tid);
+      up.request(ups + c0, (long long)p.HV * p.V, p.V - c0, counts, vec_up, tid);
       z.request((const IO*)p.values + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
       y.request((const IO*)p.dvalues + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
       st.request((const IO*)p.states + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
@@ -354,11 +353,12 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
       const long long stride = (long long)p.H * p.K, base = ((long long)b * p.T + t0) * stride + (long long)h * p.K;
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) {
-        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, 16 * t + c, 16 * t + c < p.K), k_out((const IO*)p.dk + base, stride, 16 * t + c, 16 * t + c < p.K);
+        const bool live = 16 * t + c < p.K;
+        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, left, p.K, 16 * t + c, live, g), k_out((const IO*)p.dk + base, stride, left, p.K, 16 * t + c, live, g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          q_out.store(row0 + e, row0 + e < left, GROUPED ? all_dq[t][e] : dq[t][e]);
-          k_out.store(row0 + e, row0 + e < left, GROUPED ? all_dk[t][e] : dr[t][e]);
+          q_out.store(wave, e, GROUPED ? all_dq[t][e] : dq[t][e]);
+          k_out.store(wave, e, GROUPED ? all_dk[t][e] : dr[t][e]);
         }
       }
     }
@@ -380,8 +380,10 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
 }
 
 template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hipStream_t s) {
-  const int total = (a.columns + 63) / 64 * a.B * a.HV;
-  hipLaunchKernelGGL((delta_backward_kernel<IO, KS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(kDeltaThreads), 0, s, a);
+  const int waves = delta_narrow(a) ? 2 : 4, total = (a.columns + 16 * waves - 1) / (16 * waves) * a.B * a.HV;
+  const dim3 walk((unsigned)((total + 7) / 8 * 8)), block(64 * waves);
+  if (waves == 2) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 2>), walk, block, 0, s, a);
+  else hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4>), walk, block, 0, s, a);
   int rc = check_launch("gated_delta_bwd");
   if (rc) return rc;
   const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));

@@ -10,6 +10,7 @@
 namespace rglru {
 
 int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s);
+int delta_launch_pad(const DeltaArgs& a, void* q, void* k, int dtype, hipStream_t s);
 int delta_launch_backward(const DeltaArgs& a, int dtype, hipStream_t s);
 
 struct DeltaStepArgs {
@@ -125,9 +126,11 @@ template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bo
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 struct DeltaSizes {
-  int64_t chunks, columns, width;
-  size_t gates, solve, within, states, values, total;      // offsets in the workspace; `total` without states and values if not kept
-  DeltaSizes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, bool keep) {
+  int64_t chunks, columns, width, row;                     // row: elements of a key as the kernels read it
+  size_t gates, solve, within, q, k, states, values, total;  // offsets in the workspace; q and k: room where keys have to be padded
+  DeltaSizes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, bool keep) {
+    const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
+    row = (K + e - 1) / e * e;
     chunks = B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk);
     columns = (V + 15) / 16 * 16;
     width = (K + 31) / 32 * 32;
@@ -136,7 +139,10 @@ struct DeltaSizes {
     gates = 0;
     solve = up((size_t)chunks * kDeltaGates * 4);
     within = solve + square;
-    states = within + square;
+    const size_t padded = row != K ? up((size_t)(B * T * H * row) * (16 / e)) : 0;
+    q = within + square;
+    k = q + padded;
+    states = k + padded;
     values = states + (keep ? up((size_t)chunks * columns * width * 4) : 0);
     total = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
   }
@@ -151,19 +157,17 @@ static int delta_check(const char* who, int64_t B, int64_t T, int64_t H, int64_t
     if (d != RGLRU_F32 && d != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown dtype %d", who, d);
   if (K > kDeltaMaxKey) return fail(RGLRU_E_UNSUPPORTED, "%s: keys of %lld elements, at most %d are covered", who, (long long)K, kDeltaMaxKey);
   const int64_t most = (int64_t)1 << 30;
+  if (B * T * H >= (1ll << 38) / kDeltaMaxKey) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   if (H * K >= most / 256 || HV * V >= most / 256) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens wider than %lld elements", who, (long long)(most / 256));
   if (T >= (1ll << 30) || B * HV * ((V + 63) / 64) >= most || B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk) >= most)
     return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   return RGLRU_OK;
 }
 
-static bool whole_vectors(const void* p, int64_t b, int64_t t, int64_t h, int64_t width, int dtype) {
-  const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % e == 0 && t % e == 0 && h % e == 0 && width % e == 0;
-}
-
-static int delta_operands(const char* who, DeltaArgs& a, const void* q, const void* k, const void* v, const int64_t* strides, int64_t B, int64_t T,
-                          int64_t H, int64_t HV, int64_t K, int64_t V, int dtype) {
+// Sizes, strides and the parts of the workspace.  Keys that are no whole vectors are read from their padded copies, which the
+// forward call makes.
+static int delta_operands(const char* who, DeltaArgs& a, const void* q, const void* k, const void* v, const int64_t* strides, void* ws, bool keep,
+                          int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype) {
   const int64_t dense[9] = {T * H * K, H * K, K, T * H * K, H * K, K, T * HV * V, HV * V, V};
   const int64_t* st = strides ? strides : dense;
   for (int i = 0; i < 9; ++i)
@@ -175,15 +179,21 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   a.B = (int)B, a.T = (int)T, a.H = (int)H, a.HV = (int)HV, a.K = (int)K, a.V = (int)V;
   a.nC = (int)((T + kDeltaChunk - 1) / kDeltaChunk);
   a.columns = (int)((V + 15) / 16 * 16);
-  a.vec_q = whole_vectors(q, st[0], st[1], st[2], K, dtype), a.vec_k = whole_vectors(k, st[3], st[4], st[5], K, dtype);
-  return RGLRU_OK;
-}
-
-static void delta_workspace(DeltaArgs& a, void* ws, const DeltaSizes& z, bool keep) {
+  const DeltaSizes z(B, T, H, HV, K, V, dtype, keep);
+  a.width = (int)z.row;
+  const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
+  bool whole = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0;
+  for (int i = 0; i < 6; ++i) whole = whole && st[i] % e == 0;
+  if (z.row == K && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of queries and keys must be 16-byte aligned", who);
   char* base = (char*)ws;
   a.gates = (float*)(base + z.gates);
   a.solve = base + z.solve, a.within = base + z.within;
   if (keep) a.states = base + z.states, a.values = base + z.values;
+  return RGLRU_OK;
+}
+static void delta_padded(DeltaArgs& a, void* ws, const DeltaSizes& z) {
+  a.q = (char*)ws + z.q, a.k = (char*)ws + z.k;
+  a.q_h = a.k_h = a.width, a.q_t = a.k_t = (long long)a.H * a.width, a.q_b = a.k_b = a.T * a.q_t;
 }
 
 }  // namespace rglru
@@ -194,14 +204,14 @@ extern "C" {
 
 int rglru_hip_gated_delta_max_key_size(void) { return kDeltaMaxKey; }
 
-size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int keep) {
-  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey) return 0;
-  return DeltaSizes(B, T, HV, K, V, keep != 0).total;
+size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int keep) {
+  if (B <= 0 || T <= 0 || H <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey || (dtype != RGLRU_F32 && dtype != RGLRU_BF16)) return 0;
+  return DeltaSizes(B, T, H, HV, K, V, dtype, keep != 0).total;
 }
 
 size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V) {
   if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey) return 0;
-  return DeltaSizes(B, T, HV, K, V, true).scratch();
+  return DeltaSizes(B, T, 1, HV, K, V, RGLRU_F32, true).scratch();
 }
 
 int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* log_decay, const void* beta,
@@ -213,11 +223,16 @@ int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const
   if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "gated_delta_fwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   DeltaArgs a;
   memset(&a, 0, sizeof(a));
-  rc = delta_operands("gated_delta_fwd", a, q, k, v, strides, B, T, H, HV, K, V, dtype);
+  rc = delta_operands("gated_delta_fwd", a, q, k, v, strides, ws, keep != 0, B, T, H, HV, K, V, dtype);
   if (rc) return rc;
   a.log_decay = log_decay, a.beta = beta, a.flags = flags, a.h0 = h0, a.out = out, a.h_last = h_last;
   a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
-  delta_workspace(a, ws, DeltaSizes(B, T, HV, K, V, keep != 0), keep != 0);
+  if (a.width != a.K) {
+    const DeltaSizes z(B, T, H, HV, K, V, dtype, keep != 0);
+    rc = delta_launch_pad(a, (char*)ws + z.q, (char*)ws + z.k, dtype, (hipStream_t)stream);
+    if (rc) return rc;
+    delta_padded(a, ws, z);
+  }
   return delta_launch_forward(a, keep != 0, dtype, (hipStream_t)stream);
 }
 
@@ -232,13 +247,13 @@ int rglru_hip_gated_delta_bwd(const void* q, const void* k, const int64_t* strid
   if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "gated_delta_bwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   DeltaArgs a;
   memset(&a, 0, sizeof(a));
-  rc = delta_operands("gated_delta_bwd", a, q, k, nullptr, strides, B, T, H, HV, K, V, dtype);
+  rc = delta_operands("gated_delta_bwd", a, q, k, nullptr, strides, ws, true, B, T, H, HV, K, V, dtype);
   if (rc) return rc;
-  const DeltaSizes z(B, T, HV, K, V, true);
+  const DeltaSizes z(B, T, H, HV, K, V, dtype, true);
+  if (a.width != a.K) delta_padded(a, ws, z);
   a.log_decay = log_decay, a.beta = beta, a.flags = flags, a.dout = dout, a.dh_last = dh_last;
   a.dq = dq, a.dk = dk, a.dv = dv, a.dlog_decay = dlog_decay, a.dbeta = dbeta, a.dh0 = dh0;
   a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
-  delta_workspace(a, ws, z, true);
   a.dstates = scratch, a.dvalues = (char*)scratch + z.scratch_values();
   return delta_launch_backward(a, dtype, (hipStream_t)stream);
 }

@@ -2236,13 +2236,16 @@ struct DeltaOperands {
   Tensor q, k, v, log_decay, beta;
   int64_t strides[9];
   int64_t B, T, H, HV, K, V;
-  static Tensor rows(const Tensor& t) {
+  // whole: rows of whole 16-byte vectors have to lie on their boundaries
+  static Tensor rows(const Tensor& t, bool whole) {
+    const int64_t e = 16 / t.element_size();
     bool plain = t.stride(3) == 1 || t.size(3) == 1;
-    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0;
-    return plain && t.stride(1) < (int64_t(1) << 22) ? t : t.contiguous();
+    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0 && (!whole || t.size(3) % e != 0 || t.stride(i) % e == 0);
+    if (whole && t.size(3) % e == 0) plain = plain && is_aligned(t);
+    return plain && t.stride(1) < (int64_t(1) << 22) ? t : whole ? aligned(t) : t.contiguous();
   }
   DeltaOperands(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& decay_in, const Tensor& beta_in)
-      : q(rows(q_in)), k(rows(k_in)), v(rows(v_in)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
+      : q(rows(q_in, true)), k(rows(k_in, true)), v(rows(v_in, false)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
     int at = 0;
     for (const Tensor* t : {&q, &k, &v})
       for (int i = 0; i < 3; ++i) strides[at++] = t->stride(i);
@@ -2276,7 +2279,7 @@ DeltaResult delta_forward(const DeltaOperands& o, const Tensor& h0_in, const Ten
   Tensor h0 = as(h0_in, at::kFloat);
   r.out = fresh({o.B, o.T, o.HV, o.V}, dtype, o.q);
   r.h_last = fresh({o.B, o.HV, o.K, o.V}, at::kFloat, o.q);
-  const size_t size = rglru_hip_gated_delta_workspace_bytes(o.B, o.T, o.HV, o.K, o.V, keep ? 1 : 0);
+  const size_t size = rglru_hip_gated_delta_workspace_bytes(o.B, o.T, o.H, o.HV, o.K, o.V, code_of(dtype), keep ? 1 : 0);
   TORCH_CHECK_VALUE(size > 0, "hip gated delta rule: keys of ", o.K, " elements, at most ", rglru_hip_gated_delta_max_key_size(), " are covered");
   r.kept = bytes(size, o.q);
   check(rglru_hip_gated_delta_fwd(ptr(o.q), ptr(o.k), ptr(o.v), o.strides, ptr(o.log_decay), ptr(o.beta), fptr(h0), bptr(flags), ptr(r.out),
