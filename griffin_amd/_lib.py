@@ -75,7 +75,7 @@ _SIGNATURES = {
     "rglru_hip_rmsnorm_bwd": (ctypes.c_int, [_P] * 7 + [_I, _I, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P]),
     "rglru_hip_gated_delta_max_key_size": (ctypes.c_int, []),
     "rglru_hip_gated_delta_workspace_bytes": (ctypes.c_size_t, [_I] * 6 + [ctypes.c_int] * 2),
-    "rglru_hip_gated_delta_scratch_bytes": (ctypes.c_size_t, [_I] * 5),
+    "rglru_hip_gated_delta_scratch_bytes": (ctypes.c_size_t, [_I] * 5 + [ctypes.c_int]),
     "rglru_hip_gated_delta_fwd": (ctypes.c_int, [_P] * 11 + [ctypes.c_int, ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_bwd": (ctypes.c_int, [_P] * 16 + [ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_step": (ctypes.c_int, [_P] * 8 + [ctypes.c_float] + [_I] * 5 + [ctypes.c_int] * 3 + [_P]),

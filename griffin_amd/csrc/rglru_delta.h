@@ -2,10 +2,10 @@
 // tiles or straight from the accumulators of the product before.
 //
 // An accumulator tile of v_mfma_f32_16x16 gives lane (c = lane % 16, g = lane / 16) the rows 4 g .. 4 g + 3 of column c.  The
-// B operand of the next product wants lane (c, g) to hold eight contraction indices of column c, and a contraction may run over
-// its indices in any order that both operands share: with the order 4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3 of 32 indices, two
-// accumulator tiles ARE that operand.  So a wave that owns 16 columns of the state takes it from product to product in its
-// registers; LDS holds only what comes from memory, and every A operand is read in that order.
+// B operand of the next product wants lane (c, g) to hold the contraction indices 8 g .. 8 g + 7 of 32 for column c.  Which index a
+// tile's row stands for is free: with row 4 g + e of the tiles 2 p and 2 p + 1 standing for 32 p + 8 g + e and 32 p + 8 g + 4 + e (tile_index),
+// the two tiles ARE that operand.  So a wave that owns 16 columns of the state takes it from product to product in its
+// registers; LDS holds only what comes from memory, sixteen bytes a lane and read.
 //
 // bf16 storage: keys, queries and upstream gradients are exact matrix operands; what is computed (state, solved values, the
 // chunk's triangular matrices) enters as the sum of two bf16 numbers, 2^-17 relative, because one bf16 number would round the
@@ -38,14 +38,40 @@ template <> struct Mx<__bf16> {
   static RGLRU_DEVICE f32x4 we(const Wide& a, const Frag& b, f32x4 acc) { return mma(a.lo, b, mma(a.hi, b, acc)); }
   static RGLRU_DEVICE f32x4 ww(const Wide& a, const Wide& b, f32x4 acc) { return mma(a.lo, b.hi, mma(a.hi, b.lo, mma(a.hi, b.hi, acc))); }
   static RGLRU_DEVICE f32x4 ee(const Frag& a, const Frag& b, f32x4 acc) { return mma(a, b, acc); }
-  // nearest bf16, and the nearest to what is left: off by at most 2^-9 2^-9 of the value
+  // acc[i] += a[i] b with the parts of an fp32 operand one after the other: products that follow each other do not wait for each other
+  template <int N> static RGLRU_DEVICE void ew(f32x4 (&acc)[N], const Frag (&a)[N], const Wide& b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = mma(a[i], b.hi, acc[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = mma(a[i], b.lo, acc[i]);
+  }
+  template <int FROM, int TO, int N> static RGLRU_DEVICE void we(f32x4 (&acc)[N], const Wide (&a)[N], const Frag& b) {
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) acc[i] = mma(a[i].hi, b, acc[i]);
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) acc[i] = mma(a[i].lo, b, acc[i]);
+  }
+  template <int FROM, int TO, int N> static RGLRU_DEVICE void ww(f32x4 (&acc)[N], const Wide (&a)[N], const Wide& b) {
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) acc[i] = mma(a[i].hi, b.hi, acc[i]);
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) acc[i] = mma(a[i].hi, b.lo, acc[i]);
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) acc[i] = mma(a[i].lo, b.hi, acc[i]);
+  }
+  // nearest bf16, and the nearest to what is left: off by at most 2^-9 2^-9 of the value.  The rest comes from the value and the
+  // product of the pair with (-1, 0) or (0, -1), one instruction where taking the pair apart is two (a chunk converts 80 values a lane:
+  // backward walk of B8 T2048 H8 of 128 223 -> 210 us).
   static RGLRU_DEVICE void halves(f32x4 v, bf16x4& hi, bf16x4& lo) {
+    // from registers: as an inline constant of this instruction -1 means another pair
+    unsigned lower = 0x0000bf80u, upper = 0xbf800000u;
+    asm("" : "+s"(lower), "+s"(upper));
+    const bf16x2 first = __builtin_bit_cast(bf16x2, lower), second = __builtin_bit_cast(bf16x2, upper);
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
       const f32x2 pair = {v[e], v[e + 1]};
       const bf16x2 h = __builtin_convertvector(pair, bf16x2);
-      const unsigned bits = __builtin_bit_cast(unsigned, h);
-      const f32x2 rest = {v[e] - __uint_as_float(bits << 16), v[e + 1] - __uint_as_float(bits & 0xffff0000u)};
+      const f32x2 rest = {__builtin_amdgcn_fdot2_f32_bf16(h, first, v[e], false), __builtin_amdgcn_fdot2_f32_bf16(h, second, v[e + 1], false)};
       const bf16x2 l = __builtin_convertvector(rest, bf16x2);
       hi[e] = h[0], hi[e + 1] = h[1];
       lo[e] = l[0], lo[e + 1] = l[1];
@@ -65,6 +91,10 @@ template <> struct Mx<__bf16> {
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = (__bf16)a[e], f[4 + e] = (__bf16)b[e];
     return f;
+  }
+  static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = (float)f[e], b[e] = (float)f[4 + e];
   }
   // four consecutive elements of an fp32 matrix, kept in two planes `plane` elements apart
   static RGLRU_DEVICE void put(__bf16* at, long long plane, f32x4 v) {
@@ -90,67 +120,79 @@ template <> struct Mx<float> {
   static RGLRU_DEVICE f32x4 we(const Wide& a, const Frag& b, f32x4 acc) { return mma(a, b, acc); }
   static RGLRU_DEVICE f32x4 ww(const Wide& a, const Wide& b, f32x4 acc) { return mma(a, b, acc); }
   static RGLRU_DEVICE f32x4 ee(const Frag& a, const Frag& b, f32x4 acc) { return mma(a, b, acc); }
+  template <int FROM, int TO, int N> static RGLRU_DEVICE void ww(f32x4 (&acc)[N], const Frag (&a)[N], const Frag& b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = FROM; i < TO; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i].lo[e], b.lo[e], acc[i], 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = FROM; i < TO; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i].hi[e], b.hi[e], acc[i], 0, 0, 0);
+  }
+  template <int FROM, int TO, int N> static RGLRU_DEVICE void we(f32x4 (&acc)[N], const Frag (&a)[N], const Frag& b) { ww<FROM, TO>(acc, a, b); }
+  template <int N> static RGLRU_DEVICE void ew(f32x4 (&acc)[N], const Frag (&a)[N], const Frag& b) { ww<0, N>(acc, a, b); }
   static RGLRU_DEVICE Wide wide(f32x4 a, f32x4 b) { return {a, b}; }
   static RGLRU_DEVICE Frag exact(f32x4 a, f32x4 b) { return {a, b}; }
+  static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) { a = f.lo, b = f.hi; }
   static RGLRU_DEVICE void put(float* at, long long, f32x4 v) { *reinterpret_cast<f32x4*>(at) = v; }
 };
 
-constexpr int delta_pow2_divisor(int n, int most) {
-  int p = 1;
-  while (p < most && n % (2 * p) == 0) p *= 2;
-  return p;
-}
-constexpr int delta_bank_period(int row_bytes) {           // rows after which a column lies in the same bank again, as a shift
-  int s = 0;
-  while (s < 2 && (row_bytes << s) % 256 != 0) ++s;
-  return s;
-}
+// The index that row m of accumulator tile t stands for (see above).
+RGLRU_DEVICE int tile_index(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
 
-// A row-major [rows][COLS] tile in LDS.  Its 16-byte units are exchanged within a row by a pattern of the row, so that sixteen
-// rows of one column (what one operand read touches) spread over all banks without padding.
+// A row-major [rows][COLS] tile in LDS.  Its 16-byte units are exchanged within a row by a pattern of the row, so that what eight lanes read
+// at a time (one unit of eight rows, of 0 .. 7 or of 0 .. 3 and 8 .. 11) lies in all 32 banks.
 template <typename IO, int COLS> struct Tile {
   typedef Mx<IO> M;
   typedef typename M::Frag Frag;
   typedef typename M::Wide Wide;
   static constexpr int E = 16 / (int)sizeof(IO), U = COLS / E;
-  static constexpr int kShift = delta_bank_period(COLS * (int)sizeof(IO)), kMask = delta_pow2_divisor(U, 16) - 1;
-  static RGLRU_DEVICE int unit(int row, int u) { return row * COLS + ((u ^ ((row >> kShift) & kMask)) * E); }
-  static RGLRU_DEVICE int at(int row, int col) { return unit(row, col / E) + col % E; }
-  // A (or B) operand whose contraction runs along a row: indices k0 .. k0 + 31 of row `row`
-  static RGLRU_DEVICE Frag along_row(const IO* t, int row, int k0, int g) {
-    const IO *a = t + at(row, k0 + 4 * g), *b = t + at(row, k0 + 16 + 4 * g);
-    if constexpr (sizeof(IO) == 2) {
-      const bf16x4 lo = *reinterpret_cast<const bf16x4*>(a), hi = *reinterpret_cast<const bf16x4*>(b);
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    } else {
-      return {*reinterpret_cast<const f32x4*>(a), *reinterpret_cast<const f32x4*>(b)};
-    }
+  static_assert(U % 4 == 0, "units are exchanged in fours or eights");
+  static RGLRU_DEVICE int pattern(int row) {
+    const int odd = ((row >> 2) ^ (row >> 3)) & 1;
+    return COLS * (int)sizeof(IO) % 128 == 0 ? (row & 3) << 1 | odd : (row & 2) | odd;   // rows of 64 (mod 128) bytes alternate by themselves
   }
-  // ... runs down the rows: rows k0 .. k0 + 31 of column col0 + c
-  static RGLRU_DEVICE Frag down_rows(const IO* t, int k0, int col0, int lane) {
+  static RGLRU_DEVICE int unit(int row, int u) { return row * COLS + (u ^ pattern(row)) * E; }
+  static RGLRU_DEVICE int at(int row, int col) { return unit(row, col / E) + col % E; }
+  // operand whose contraction runs along a row: indices k0 .. k0 + 31 of row `row`
+  static RGLRU_DEVICE Frag along_row(const IO* t, int row, int k0, int g) {
+    if constexpr (sizeof(IO) == 2) return *reinterpret_cast<const bf16x8*>(t + at(row, k0 + 8 * g));
+    else return {*reinterpret_cast<const f32x4*>(t + at(row, k0 + 8 * g)), *reinterpret_cast<const f32x4*>(t + at(row, k0 + 8 * g + 4))};
+  }
+  // ... runs down the rows: rows k0 .. k0 + 31 of column col0 + step (c / 4) + c % 4
+  static RGLRU_DEVICE Frag down_rows(const IO* t, int k0, int col0, int step, int lane) {
     const int c = lane & 15, g = lane >> 4;
     if constexpr (sizeof(IO) == 2) {
-      // ds_read_b64_tr_b16: lane i of sixteen names row i / 4, columns 4 (i % 4) .. + 3 and receives column i, rows 0 .. 3
+      // ds_read_b64_tr_b16: lane i of sixteen names row i / 4, four columns of block i % 4 and receives column i, rows 0 .. 3
       typedef __attribute__((address_space(3))) bf16x4_lds* lds_ptr_t;
-      const int row = k0 + 4 * g + (c >> 2), col = col0 + 4 * (c & 3);
+      const int row = k0 + 8 * g + (c >> 2), col = col0 + step * (c & 3);
       const bf16x4_lds lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr_t)(t + at(row, col)));
-      const bf16x4_lds hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr_t)(t + at(row + 16, col)));
+      const bf16x4_lds hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr_t)(t + at(row + 4, col)));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
+      const int col = col0 + step * (c >> 2) + (c & 3);
       Frag f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f.lo[e] = t[at(k0 + 4 * g + e, col0 + c)], f.hi[e] = t[at(k0 + 16 + 4 * g + e, col0 + c)];
+      for (int e = 0; e < 4; ++e) f.lo[e] = t[at(k0 + 8 * g + e, col)], f.hi[e] = t[at(k0 + 8 * g + 4 + e, col)];
       return f;
     }
   }
-  // the same for an fp32 matrix; its second plane lies `plane` elements behind the first
+  // the same for accumulator tile t of what comes out, and for sixteen columns in their order
+  static RGLRU_DEVICE Frag down_rows_tile(const IO* x, int k0, int t, int lane) { return down_rows(x, k0, 32 * (t >> 1) + 4 * (t & 1), 8, lane); }
+  static RGLRU_DEVICE Frag down_rows(const IO* x, int k0, int col0, int lane) { return down_rows(x, k0, col0, 4, lane); }
+  // an fp32 matrix, whose second plane lies `plane` elements behind the first
   static RGLRU_DEVICE Wide wide_along_row(const IO* t, int plane, int row, int k0, int g) {
     if constexpr (sizeof(IO) == 2) return {along_row(t, row, k0, g), along_row(t + plane, row, k0, g)};
     else return along_row(t, row, k0, g);
   }
-  static RGLRU_DEVICE Wide wide_down_rows(const IO* t, int plane, int k0, int col0, int lane) {
-    if constexpr (sizeof(IO) == 2) return {down_rows(t, k0, col0, lane), down_rows(t + plane, k0, col0, lane)};
-    else return down_rows(t, k0, col0, lane);
+  static RGLRU_DEVICE Wide wide_down_rows_tile(const IO* x, int plane, int k0, int t, int lane) {
+    if constexpr (sizeof(IO) == 2) return {down_rows_tile(x, k0, t, lane), down_rows_tile(x + plane, k0, t, lane)};
+    else return down_rows_tile(x, k0, t, lane);
+  }
+  static RGLRU_DEVICE Wide wide_down_rows(const IO* x, int plane, int k0, int col0, int lane) {
+    if constexpr (sizeof(IO) == 2) return {down_rows(x, k0, col0, lane), down_rows(x + plane, k0, col0, lane)};
+    else return down_rows(x, k0, col0, lane);
   }
 };
 
@@ -167,10 +209,17 @@ struct DeltaArgs {
   float* gates;                      // [chunks][kDeltaGates]
   void *states, *values;             // [chunks][dv][dk], [chunks][dv][64]: state in front of a chunk, solved values (both transposed)
   void *dstates, *dvalues;           // the same of the backward pass: gradient behind a chunk, gradient of the values
+  // A sequence in several segments of `length` chunks that are walked side by side: [heads][segments][columns][padded K] and, for
+  // `through`, [heads][segments][padded K in][padded K out]
+  float *local, *edges;              // what a segment adds to the state (or its gradient); the state a segment starts from
+  void* through;                     // what a segment makes of the state it starts from, as an operand
+  int segments, length;
   long long q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
   int B, T, H, HV, K, V, nC, columns;       // columns: V in whole tiles of 16
   int decay_dtype, beta_dtype;
   int width;                                // of the rows of q and k as the kernels read them: K in whole 16-byte vectors
+  int value_width;                          // the same of v and dout
+  long long up_b, up_t, up_h;               // strides of dout as the kernels read it
   float scale;
 };
 
@@ -221,22 +270,12 @@ template <typename IO, int COLS, int THREADS> struct KeyRows {
   typedef Tile<IO, COLS> T;
   static constexpr int N = kDeltaChunk * T::U / THREADS;   // vectors a thread
   i32x4 v[N];
-  RGLRU_DEVICE void request(const IO* rows, long long stride, int width, unsigned long long counts, bool vec, int tid) {
+  RGLRU_DEVICE void request(const IO* rows, long long stride, int width, unsigned long long counts, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = tid + i * THREADS, row = at / T::U, col = at % T::U * T::E;
       v[i] = i32x4{0, 0, 0, 0};
-      if (((counts >> row) & 1) && col < width) {
-        const IO* src = rows + (long long)row * stride + col;
-        if (vec) {
-          v[i] = *reinterpret_cast<const i32x4*>(src);
-        } else {
-          IO e[T::E];
-#pragma unroll
-          for (int j = 0; j < T::E; ++j) e[j] = col + j < width ? src[j] : (IO)0.0f;
-          __builtin_memcpy(&v[i], e, 16);
-        }
-      }
+      if (((counts >> row) & 1) && col < width) v[i] = *reinterpret_cast<const i32x4*>(rows + (long long)row * stride + col);
     }
   }
   RGLRU_DEVICE void put(IO* tile, int tid) const {
@@ -304,13 +343,13 @@ RGLRU_DEVICE void wait_for_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n
 // A row-major matrix on its way into an LDS tile.
 template <typename IO, int ROWS, int COLS, int THREADS> struct TileLoad {
   typedef Tile<IO, COLS> T;
-  static constexpr int kBytes = ROWS * COLS * (int)sizeof(IO), N = ROWS * T::U / THREADS;
-  static_assert(N * THREADS == ROWS * T::U, "whole vectors a thread");
+  static constexpr int kBytes = ROWS * COLS * (int)sizeof(IO), kUnits = ROWS * T::U, kWhole = kUnits / THREADS, N = (kUnits + THREADS - 1) / THREADS;
+  static_assert(kUnits % 64 == 0, "whole waves");
   unsigned off[N];
   RGLRU_DEVICE void setup(int tid, long long stride, int width) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS, row = at / T::U, col = ((at % T::U) ^ ((row >> T::kShift) & T::kMask)) * T::E;
+      const int at = tid + i * THREADS, row = at / T::U, col = ((at % T::U) ^ T::pattern(row)) * T::E;
       off[i] = col < width ? (unsigned)row * (unsigned)(stride * (int)sizeof(IO)) + (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange;
     }
   }
@@ -323,60 +362,75 @@ template <typename IO, int ROWS, int COLS, int THREADS> struct TileLoad {
     constexpr int STEP = THREADS * 16;
     lds += (unsigned)wave * 1024u;
 #pragma unroll
-    for (int i = 0; i + 4 <= N; i += 4) memory_to_lds<STEP>(r, off[i], off[i + 1], off[i + 2], off[i + 3], lds + (unsigned)(i * STEP));
+    for (int i = 0; i + 4 <= kWhole; i += 4) memory_to_lds<STEP>(r, off[i], off[i + 1], off[i + 2], off[i + 3], lds + (unsigned)(i * STEP));
 #pragma unroll
-    for (int i = N / 4 * 4; i < N; ++i) memory_to_lds(r, off[i], lds + (unsigned)(i * STEP));
+    for (int i = kWhole / 4 * 4; i < N; ++i)
+      if (i < kWhole || i * THREADS + wave * 64 < kUnits) memory_to_lds(r, off[i], lds + (unsigned)(i * STEP));
   }
 };
 
-// One element of a [tokens, columns] tensor a lane: rows 16 mt + 4 g + e of a chunk, one column.  Rows past the `rows` there are read
-// as zeros and not written.
+// A chunk's rows of a [tokens, columns] tensor, a lane's column.  Only a lane's own offset is checked against the descriptor's extent,
+// so rows go into the scalar offset where the chunk is whole, else into the lane's: those past the end are not written.
 template <typename IO> struct ColumnIo {
   rsrc_t rsrc;
   unsigned row_bytes, first;
-  RGLRU_DEVICE ColumnIo(const IO* base, long long stride, int rows, int width, int col, bool live, int g)
+  bool whole;
+  // lane_row: the first of the lane's rows
+  RGLRU_DEVICE ColumnIo(const IO* base, long long stride, int rows, int width, int col, bool live, int lane_row)
       : rsrc(make_rsrc(base, (unsigned)(((rows < kDeltaChunk ? rows : kDeltaChunk) - 1) * stride + width) * (unsigned)sizeof(IO))),
         row_bytes((unsigned)(stride * (long long)sizeof(IO))),
-        first(live ? (unsigned)(4 * g) * row_bytes + (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange) {}
-  // the offset of a lane without a column stays out of range: at most 64 rows of 2^22 elements are added to it, modulo 2^32
-  RGLRU_DEVICE unsigned at(int mt, int e) const { return first == kOutOfRange ? kOutOfRange : first + (unsigned)(16 * mt + e) * row_bytes; }
-  // as it lies in memory, so that nothing waits for it before it is used
-  static RGLRU_DEVICE float value(int raw) { return sizeof(IO) == 2 ? __uint_as_float((unsigned)raw << 16) : __uint_as_float((unsigned)raw); }
-  RGLRU_DEVICE int raw(int mt, int e) const {
-    if constexpr (sizeof(IO) == 2) return (int)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(mt, e), 0, 0);
-    else return (int)__builtin_amdgcn_raw_buffer_load_b32(rsrc, at(mt, e), 0, 0);
+        first(live ? (unsigned)lane_row * row_bytes + (unsigned)col * (unsigned)sizeof(IO) : kOutOfRange), whole(rows >= kDeltaChunk) {}
+  RGLRU_DEVICE unsigned at(int row) const { return first == kOutOfRange ? kOutOfRange : first + (unsigned)row * row_bytes; }
+  // four accumulator tiles of rows; the lane's first row is 8 g
+  static RGLRU_DEVICE int tile_row(int i) { return 32 * (i >> 3) + 4 * ((i >> 2) & 1) + (i & 3); }
+  RGLRU_DEVICE void store(int row, float v) const { BufIo<IO>::store((IO)v, rsrc, at(row), 0); }
+  RGLRU_DEVICE void store(const f32x4 (&v)[4]) const {
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) BufIo<IO>::store((IO)v[i / 4][i % 4], rsrc, first, (unsigned)tile_row(i) * row_bytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) BufIo<IO>::store((IO)v[i / 4][i % 4], rsrc, at(tile_row(i)), 0);
+    }
   }
-  RGLRU_DEVICE void store(int mt, int e, float v) const { BufIo<IO>::store((IO)v, rsrc, at(mt, e), 0); }
 };
 
-// What a walk along the chunks has in LDS of one chunk, and how it gets there.  Two of them where they fit: the next chunk's is
-// filled while this one's is worked on.
-template <typename IO, int KS, int THREADS, bool OUT> struct ChunkTiles {
-  static constexpr int DK = 32 * KS, PL = Mx<IO>::kPlanes;
+// What a walk along the chunks has in LDS of one chunk, and how it gets there: keys, queries, T, P, the gate record, and `COLUMNS` columns of
+// the values or the upstream gradients.
+template <typename IO, int KS, int WAVES, bool OUT> struct ChunkTiles {
+  static constexpr int DK = 32 * KS, PL = Mx<IO>::kPlanes, THREADS = 64 * WAVES, COLUMNS = 16 * WAVES;
   typedef TileLoad<IO, 64, DK, THREADS> KeyLoad;
   typedef TileLoad<IO, PL * 64, 64, THREADS> SquareLoad;
-  static constexpr int kKeys = 0, kSolve = KeyLoad::kBytes, kQueries = kSolve + SquareLoad::kBytes,
+  typedef TileLoad<IO, 64, COLUMNS, THREADS> ValueLoad;
+  static constexpr int kKeys = 0, kSolve = KeyLoad::kBytes, kValues = kSolve + SquareLoad::kBytes, kQueries = kValues + ValueLoad::kBytes,
                        kWithin = kQueries + (OUT ? KeyLoad::kBytes : 0), kRecord = kWithin + (OUT ? SquareLoad::kBytes : 0),
                        kBytes = kRecord + 1024;             // the record: one vector a lane of one wave
-  static constexpr int kStages = 2 * kBytes <= 160 * 1024 ? 2 : 1;
   KeyLoad k, q;
   SquareLoad square;
+  ValueLoad value;
   unsigned record;
-  RGLRU_DEVICE void setup(const DeltaArgs& p, int tid) {
+  long long value_stride;
+  int value_width;
+  RGLRU_DEVICE void setup(const DeltaArgs& p, int tid, long long stride, int width) {
     k.setup(tid, p.k_t, p.width);
     if constexpr (OUT) q.setup(tid, p.q_t, p.width);
     square.setup(tid, 64, 64);
+    value_stride = stride, value_width = width < COLUMNS ? width : COLUMNS;
+    value.setup(tid, stride, width);
     record = (tid & 63) * 16 < kDeltaGates * 4 ? (unsigned)(tid & 63) * 16u : kOutOfRange;
   }
-  RGLRU_DEVICE void request(const DeltaArgs& p, long long chunk, int n, int b, int h, unsigned lds, int wave) const {
+  // `values`: the chunk's first row, at the group's first column
+  RGLRU_DEVICE void request(const DeltaArgs& p, long long chunk, int n, int b, int h, const IO* values, unsigned lds, int wave) const {
     const int t0 = n * kDeltaChunk, left = p.T - t0;
     const i32x4 rk = delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left));
     const i32x4 rs = delta_rsrc((const IO*)p.solve + chunk * (4096 * PL), SquareLoad::kBytes);
     const i32x4 rq = delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, OUT ? KeyLoad::extent(p.q_t, p.width, left) : 0u);
     const i32x4 rw = delta_rsrc((const IO*)p.within + chunk * (4096 * PL), SquareLoad::kBytes);
+    const i32x4 rv = delta_rsrc(values, ValueLoad::extent(value_stride, value_width, left));
     const i32x4 rr = delta_rsrc(p.gates + chunk * kDeltaGates, kDeltaGates * 4);
     k.request(rk, lds + kKeys, wave);
     square.request(rs, lds + kSolve, wave);
+    if (value_width > 0) value.request(rv, lds + kValues, wave);
     if constexpr (OUT) {
       q.request(rq, lds + kQueries, wave);
       square.request(rw, lds + kWithin, wave);
@@ -384,22 +438,52 @@ template <typename IO, int KS, int THREADS, bool OUT> struct ChunkTiles {
     if (wave == 0) memory_to_lds(rr, record, lds + kRecord);
   }
   // zeros for the rows of tokens that do not count
+  template <typename LOAD> static RGLRU_DEVICE void clear(unsigned char* tile, unsigned long long counts, int tid) {
+    for (int at = tid; at < 64 * LOAD::T::U; at += THREADS)
+      if (!((counts >> (at / LOAD::T::U)) & 1)) *reinterpret_cast<i32x4*>(tile + at * 16) = i32x4{0, 0, 0, 0};
+  }
   static RGLRU_DEVICE void clear_rows(unsigned char* stage, unsigned long long counts, int tid) {
-    for (int at = tid; at < 64 * KeyLoad::T::U; at += THREADS) {
-      const int row = at / KeyLoad::T::U;
-      if ((counts >> row) & 1) continue;
-      *reinterpret_cast<i32x4*>(stage + kKeys + at * 16) = i32x4{0, 0, 0, 0};
-      if constexpr (OUT) *reinterpret_cast<i32x4*>(stage + kQueries + at * 16) = i32x4{0, 0, 0, 0};
-    }
+    clear<KeyLoad>(stage + kKeys, counts, tid);
+    clear<ValueLoad>(stage + kValues, counts, tid);
+    if constexpr (OUT) clear<KeyLoad>(stage + kQueries, counts, tid);
   }
 };
+
+// Sixteen columns of 64 tokens that a wave has in its accumulators on their way to memory, through the wave's columns of a value tile:
+// whole vectors of a row a lane.
+template <typename IO, int COLUMNS> struct WaveRows {
+  typedef Tile<IO, COLUMNS> T;
+  static constexpr int VECTORS = 16 / T::E, N = 64 * VECTORS / 64;       // vectors of a row; of a lane
+  i32x4 v[N];
+  RGLRU_DEVICE void turn(IO* tile, const f32x4 (&x)[4], int wave, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tile[T::at(tile_index(i / 4, 4 * g + i % 4), 16 * wave + c)] = (IO)x[i / 4][i % 4];
+    wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const i32x4*>(tile + T::at((i * 64 + lane) / VECTORS, 16 * wave + lane % VECTORS * T::E));
+  }
+  // rows: that are there; width: of the tensor
+  RGLRU_DEVICE void store(IO* base, long long stride, int rows, int width, int col, int lane) const {
+    const rsrc_t r = make_rsrc(base, (unsigned)(((rows < kDeltaChunk ? rows : kDeltaChunk) - 1) * stride + width) * (unsigned)sizeof(IO));
+    const int at = col + lane % VECTORS * T::E;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      buf_store_b128(v[i], r, at < width ? ((unsigned)((i * 64 + lane) / VECTORS) * (unsigned)stride + (unsigned)at) * (unsigned)sizeof(IO) : kOutOfRange);
+  }
+};
+
+// A chunk's products come in phases; the operands of the next one are requested in front of each.  The scheduler keeps to that: by itself
+// it requests those of all phases at once and runs out of registers.
+RGLRU_DEVICE void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+// Four rows of each of the tiles 2 p and 2 p + 1 from an array of 64 numbers.
+RGLRU_DEVICE f32x4 tile_rows(const float* a, int mt, int g) { return *reinterpret_cast<const f32x4*>(a + 32 * (mt >> 1) + 8 * g + 4 * (mt & 1)); }
+
 RGLRU_DEVICE unsigned long long counts_of(const float* record) {
   const unsigned lo = __builtin_amdgcn_readfirstlane(__float_as_uint(record[128])), hi = __builtin_amdgcn_readfirstlane(__float_as_uint(record[129]));
   return (unsigned long long)lo | (unsigned long long)hi << 32;
 }
-
-// Whether a walk's workgroups are of two waves instead of four: where those of four leave compute units without one.
-inline bool delta_narrow(const DeltaArgs& a) { return (long long)(a.columns + 63) / 64 * a.B * a.HV < num_compute_units(); }
 
 // XCDs take workgroups round-robin; each gets a contiguous run of the work, so that neighbours share its L2.  -1: none left.
 RGLRU_DEVICE int xcd_order(int block, int total) {

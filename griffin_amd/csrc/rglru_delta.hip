@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
+#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
@@ -61,8 +62,8 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   const unsigned long long counts = __ballot(gate.counts);
   {
     KeyRows<IO, DK, kDeltaThreads> k, q;
-    k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, true, tid);
-    q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, true, tid);
+    k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, tid);
+    q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, tid);
     if (wave == 0) {
       total[lane] = gate.total;
       beta[lane] = gate.beta;
@@ -129,220 +130,261 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   for (int it = 0; it < 4; ++it) M::put(solve + (16 * wave + c) * 64 + 16 * it + 4 * g, 4096, column[it]);
 }
 
-// The walk along the chunks.  SAVE: what the backward pass needs is left behind; OUT: the outputs are wanted.
-// A chunk's results are stored in front of the next one's requests: behind them, the wait for the requests would be one for the stores.
-template <typename IO, int KS, int WAVES, bool SAVE, bool OUT>
-__global__ __launch_bounds__(64 * WAVES, 1) void delta_forward_kernel(DeltaArgs p) {
+// The walk along a segment's chunks.  SAVE: what the backward pass needs is left behind.  !OUT: what the segment does to the state, without
+// outputs: column groups behind those of the values walk the columns of the unit matrix, with values of nothing.
+// STAGES 2: the next chunk's tiles are requested in front of this one's products, and a chunk's results are stored in front of the
+// next one's requests (behind them, the wait for the requests would be one for the stores).  STAGES 1: two workgroups share a
+// compute unit, one computes while the other waits.
+template <typename IO, int KS, int WAVES, int STAGES, bool SAVE, bool OUT>
+__global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void delta_forward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
+  typedef typename M::Frag Frag;
   constexpr int DK = 32 * KS, PL = M::kPlanes, THREADS = 64 * WAVES, COLUMNS = 16 * WAVES;
   typedef Tile<IO, DK> Keys;
   typedef Tile<IO, 64> Square;
-  typedef ChunkTiles<IO, KS, THREADS, OUT> Tiles;
-  constexpr int STAGES = Tiles::kStages;
+  typedef Tile<IO, COLUMNS> Values;
+  typedef ChunkTiles<IO, KS, WAVES, OUT> Tiles;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * Tiles::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = (p.columns + COLUMNS - 1) / COLUMNS, total = groups * p.B * p.HV;
-  const int work = xcd_order(blockIdx.x, total);
+  const int value_groups = (p.columns + COLUMNS - 1) / COLUMNS, groups = value_groups + (OUT ? 0 : (DK + COLUMNS - 1) / COLUMNS);
+  const int work = xcd_order(blockIdx.x, groups * p.segments * p.B * p.HV);
   if (work < 0) return;
-  const int group = work % groups, head = work / groups, hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
-  const int col = group * COLUMNS + wave * 16 + c;
-  const bool mine = group * COLUMNS + wave * 16 < p.columns, live = mine && col < p.V;
+  const int group = work % groups, segment = work / groups % p.segments, head = work / groups / p.segments;
+  const int hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
+  const bool unit = !OUT && group >= value_groups;
+  if (!OUT && !unit && segment == p.segments - 1) return;                // nothing starts behind the last segment
+  const int col = (unit ? group - value_groups : group) * COLUMNS + wave * 16 + c, width = unit ? DK : p.columns;
+  const bool mine = col - c < width, live = mine && (unit || col < p.V);
+  const int begin = segment * p.length, end = begin + p.length < p.nC ? begin + p.length : p.nC;
   const long long first = (long long)head * p.nC;
   const unsigned lds0 = lds_address(lds);
 
   Tiles tiles;
-  tiles.setup(p, tid);
+  tiles.setup(p, tid, p.v_t, unit ? 0 : p.value_width - group * COLUMNS);
+  const IO* const values = (const IO*)p.v + b * p.v_b + hv * p.v_h + group * COLUMNS;
+  const bool vectors = p.value_width == p.V;
   f32x4 state[2 * KS], o[4], z[4];
-  int v[4][4];
+  WaveRows<IO, COLUMNS> rows_out;
   auto request = [&](int n, int stage) {
-    tiles.request(p, first + n, n, b, h, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
-    const int t0 = n * kDeltaChunk;
-    const ColumnIo<IO> values((const IO*)p.v + b * p.v_b + t0 * p.v_t + hv * p.v_h, p.v_t, p.T - t0, p.V, col, live, g);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[mt][e] = values.raw(mt, e);
+    tiles.request(p, first + n, n, b, h, values + (long long)n * kDeltaChunk * p.v_t, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
   };
   auto put = [&](int n) {                                  // results of chunk n
     if constexpr (SAVE) {
       if (mine) {
         IO* at = (IO*)p.values + ((first + n) * PL * p.columns + col) * 64;
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, z[mt]);
+        for (int mt = 0; mt < 4; ++mt) M::put(at + tile_index(mt, 4 * g), (long long)p.columns * 64, z[mt]);
       }
     }
     if constexpr (OUT) {
       const int t0 = n * kDeltaChunk;
-      const ColumnIo<IO> out((const IO*)p.out + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out.store(mt, e, o[mt][e]);
+      const long long stride = (long long)p.HV * p.V;
+      IO* at = (IO*)p.out + (((long long)b * p.T + t0) * p.HV + hv) * p.V;
+      if (vectors) {
+        if (mine) rows_out.store(at, stride, p.T - t0, p.V, col - c, lane);
+      } else {
+        ColumnIo<IO>(at, stride, p.T - t0, p.V, col, live, 8 * g).store(o);
+      }
     }
   };
-  request(0, 0);
+  request(begin, 0);
+  if (!OUT) {
 #pragma unroll
-  for (int t = 0; t < 2 * KS; ++t)
+    for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = 16 * t + 4 * g + e;
-      state[t][e] = p.h0 && live && row < p.K ? p.h0[((long long)head * p.K + row) * p.V + col] : 0.f;
-    }
+      for (int e = 0; e < 4; ++e) state[t][e] = unit && tile_index(t, 4 * g + e) == col ? 1.f : 0.f;
+  } else if (p.segments > 1) {
+    const float* at = p.edges + (((long long)head * p.segments + segment) * p.columns + (mine ? col : 0)) * DK;
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) state[t] = *reinterpret_cast<const f32x4*>(at + tile_index(t, 4 * g));
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = tile_index(t, 4 * g + e);
+        state[t][e] = p.h0 && live && row < p.K ? p.h0[((long long)head * p.K + row) * p.V + col] : 0.f;
+      }
+  }
   wait_for_all();
-  for (int n = 0; n < p.nC; ++n) {
-    const int stage = STAGES == 2 ? n & 1 : 0;
+  for (int n = begin; n < end; ++n) {
+    const int stage = STAGES == 2 ? (n - begin) & 1 : 0;
     unsigned char* tile = lds + stage * Tiles::kBytes;
     const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
              *within = (const IO*)(tile + Tiles::kWithin);
     const float* record = (const float*)(tile + Tiles::kRecord);
     const unsigned long long counts = counts_of(record);
-    f32x4 r[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[mt][e] = ColumnIo<IO>::value(v[mt][e]);
     if (counts != ~0ull) {
       Tiles::clear_rows(tile, counts, tid);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[mt][e] = (counts >> (16 * mt + 4 * g + e)) & 1 ? r[mt][e] : 0.f;
       lds_barrier();
     }
-    Wide s[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s[ks] = M::wide(state[2 * ks], state[2 * ks + 1]);
-    if (n) put(n - 1);
+    if (STAGES == 2 && n > begin) put(n - 1);
     if constexpr (SAVE) {
       if (mine) {
         IO* at = (IO*)p.states + ((first + n) * PL * p.columns + col) * DK;
 #pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, state[t]);
+        for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), (long long)p.columns * DK, state[t]);
       }
     }
-    if (STAGES == 2 && n + 1 < p.nC) request(n + 1, stage ^ 1);
+    if (STAGES == 2 && n + 1 < end) request(n + 1, stage ^ 1);
     if (mine) {
-      f32x4 rho[4];
+      Frag ka[2][4], qa[2][4], kt[2][2 * KS];
+      Wide ta[2][4];
+      auto rows = [&](const IO* x, int ks, Frag (&a)[4]) {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(record + 16 * mt + 4 * g);
+        for (int mt = 0; mt < 4; ++mt) a[mt] = Keys::along_row(x, tile_index(mt, c), 32 * ks, g);
+      };
+      auto square = [&](const IO* x, int ks, Wide (&a)[4]) {             // lower triangular: rows in front of the columns are zeros
+#pragma unroll
+        for (int mt = 2 * ks; mt < 4; ++mt) a[mt] = Square::wide_down_rows_tile(x, 4096, 32 * ks, mt, lane);
+      };
+      auto turned = [&](int ks, Frag (&a)[2 * KS]) {
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) a[t] = Keys::down_rows_tile(keys, 32 * ks, t, lane);
+      };
+      phase();
+      rows(keys, 0, ka[0]);
+      if constexpr (OUT) rows(queries, 0, qa[0]);
+      f32x4 rho[4], r[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g), r[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      IO* const value_tile = (IO*)(tile + Tiles::kValues);
+      if (OUT || !unit) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) M::apart(Values::down_rows(value_tile, 32 * ks, 16 * wave, lane), r[2 * ks], r[2 * ks + 1]);
+      }
       const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
-      // R = V - rho K S; where nothing is carried into a document, nothing of it is read either, whatever it is
+      // K S and Q S (o) side by side: a tile of the state becomes an operand once
       f32x4 acc[4] = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int mt = 0; mt < 4; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) acc[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), s[ks], acc[mt]);
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) {
+          rows(keys, ks + 1, ka[(ks + 1) & 1]);
+          if constexpr (OUT) rows(queries, ks + 1, qa[(ks + 1) & 1]);
+        } else {
+          square(solve, 0, ta[0]);
+        }
+        phase();
+        const Wide s = M::wide(state[2 * ks], state[2 * ks + 1]);
+        M::ew(acc, ka[ks & 1], s);
+        if constexpr (OUT) M::ew(o, qa[ks & 1], s);
+        phase();
+      }
+      square(solve, 1, ta[1]);
+      phase();
+      // where nothing is carried into a document, nothing of it is read either, whatever it is
       if (carry == 0.f) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[mt][e] = rho[mt][e] == 0.f ? 0.f : acc[mt][e];
+          for (int e = 0; e < 4; ++e) acc[mt][e] = rho[mt][e] == 0.f ? 0.f : acc[mt][e], o[mt][e] = rho[mt][e] == 0.f ? 0.f : o[mt][e];
       }
+      // Z = T R, R = V - rho K S
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[mt][e] = fmaf(-rho[mt][e], acc[mt][e], r[mt][e]);
-      // Z = T R
-      {
-        const Wide rw[2] = {M::wide(r[0], r[1]), M::wide(r[2], r[3])};
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) z[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int mt = 2 * ks; mt < 4; ++mt) z[mt] = M::ww(Square::wide_down_rows(solve, 4096, 32 * ks, 16 * mt, lane), rw[ks], z[mt]);
+        if constexpr (OUT) o[mt] *= rho[mt] * p.scale;
+        z[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
+      M::template ww<0, 4>(z, ta[0], M::wide(r[0], r[1]));
+      phase();
+      turned(0, kt[0]);
+      phase();
+      M::template ww<2, 4>(z, ta[1], M::wide(r[2], r[3]));
+      phase();
+      turned(1, kt[1]);
+      if constexpr (OUT) square(within, 0, ta[0]);
+      phase();
       // S' = rho_63 S + K^T (w Z)
-      {
-        f32x4 wz[4];
+      if (carry == 0.f) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) wz[mt] = z[mt] * *reinterpret_cast<const f32x4*>(record + 64 + 16 * mt + 4 * g);
-        const Wide zw[2] = {M::wide(wz[0], wz[1]), M::wide(wz[2], wz[3])};
-        if (carry == 0.f) {
+        for (int t = 0; t < 2 * KS; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      } else {
 #pragma unroll
-          for (int t = 0; t < 2 * KS; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        } else {
-#pragma unroll
-          for (int t = 0; t < 2 * KS; ++t) state[t] *= carry;
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int t = 0; t < 2 * KS; ++t) state[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), zw[ks], state[t]);
+        for (int t = 0; t < 2 * KS; ++t) state[t] *= carry;
       }
+      M::ew(state, kt[0], M::wide(z[0] * tile_rows(record + 64, 0, g), z[1] * tile_rows(record + 64, 1, g)));
+      phase();
+      if constexpr (OUT) square(within, 1, ta[1]);
+      phase();
+      M::ew(state, kt[1], M::wide(z[2] * tile_rows(record + 64, 2, g), z[3] * tile_rows(record + 64, 3, g)));
       if constexpr (OUT) {
-        const Wide zw[2] = {M::wide(z[0], z[1]), M::wide(z[2], z[3])};
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt) o[mt] = M::ew(Keys::along_row(queries, 16 * mt + c, 32 * ks, g), s[ks], o[mt]);
-        if (carry == 0.f) {
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][e] = rho[mt][e] == 0.f ? 0.f : o[mt][e];
-        }
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) o[mt] *= rho[mt] * p.scale;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int mt = 2 * ks; mt < 4; ++mt) o[mt] = M::ww(Square::wide_down_rows(within, 4096, 32 * ks, 16 * mt, lane), zw[ks], o[mt]);
+        phase();
+        M::template ww<0, 4>(o, ta[0], M::wide(z[0], z[1]));
+        M::template ww<2, 4>(o, ta[1], M::wide(z[2], z[3]));
+        if (vectors) rows_out.turn(value_tile, o, wave, lane);
       }
+      phase();
     }
-    if (STAGES == 1 && n + 1 < p.nC) {
+    if constexpr (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
-      request(n + 1, 0);
+      if (n + 1 < end) request(n + 1, 0);
+      put(n);
     }
     wait_for_all();
   }
-  put(p.nC - 1);
-  if (p.h_last && live) {
+  if (STAGES == 2) put(end - 1);
+  if (!OUT) {
+    if (mine && unit) {
+      IO* at = (IO*)p.through + (((long long)head * p.segments + segment) * PL * DK + col) * DK;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), DK * DK, state[t]);
+    } else if (mine) {
+      float* at = p.local + (((long long)head * p.segments + segment) * p.columns + col) * DK;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) *reinterpret_cast<f32x4*>(at + tile_index(t, 4 * g)) = state[t];
+    }
+  } else if (p.h_last && live && end == p.nC) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * t + 4 * g + e;
+        const int row = tile_index(t, 4 * g + e);
         if (row < p.K) p.h_last[((long long)head * p.K + row) * p.V + col] = state[t][e];
       }
   }
 }
 
-template <typename IO, int KS, int WAVES> static void delta_walk_forward(const DeltaArgs& a, bool save, hipStream_t s) {
-  const int total = (a.columns + 16 * WAVES - 1) / (16 * WAVES) * a.B * a.HV;
+template <typename IO, int KS, int WAVES, int STAGES> static void delta_walk_forward(const DeltaArgs& a, bool save, hipStream_t s) {
+  const int total = (a.columns + 16 * WAVES - 1) / (16 * WAVES) * a.segments * a.B * a.HV;
   const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(64 * WAVES);
-  if (save) hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, true, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, false, true>), grid, block, 0, s, a);
+  if (save) hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, true, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, false, true>), grid, block, 0, s, a);
 }
 
 template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool save, hipStream_t s) {
   hipLaunchKernelGGL((delta_prepare_kernel<IO, KS>), dim3((unsigned)((long long)a.B * a.HV * a.nC)), dim3(kDeltaThreads), 0, s, a);
   int rc = check_launch("gated_delta_fwd prepare");
   if (rc) return rc;
-  if (delta_narrow(a)) delta_walk_forward<IO, KS, 2>(a, save, s);
-  else delta_walk_forward<IO, KS, 4>(a, save, s);
+  const char* w = getenv("DELTA_WAVES");
+  const int waves = w ? atoi(w) : 2;
+  if constexpr (sizeof(IO) == 2) {
+  if (waves == 2) delta_walk_forward<IO, KS, 2, 2>(a, save, s);
+  else if (waves == 4) delta_walk_forward<IO, KS, 4, 1>(a, save, s);
+  else delta_walk_forward<IO, KS, 4, 2>(a, save, s);
+  } else delta_walk_forward<IO, KS, 4, 1>(a, save, s);
   return check_launch("gated_delta_fwd");
 }
 
-// Keys that are no whole 16-byte vectors, as rows that are, zeros behind them.
-template <typename IO> __global__ __launch_bounds__(256) void delta_pad_kernel(DeltaArgs p, IO* q, IO* k) {
-  const long long rows = (long long)p.B * p.T * p.H, i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= rows * p.width) return;
-  const long long row = i / p.width;
-  const int col = (int)(i % p.width), h = (int)(row % p.H);
-  const long long token = row / p.H, b = token / p.T, t = token % p.T;
-  q[i] = col < p.K ? ((const IO*)p.q)[b * p.q_b + t * p.q_t + h * p.q_h + col] : (IO)0.f;
-  k[i] = col < p.K ? ((const IO*)p.k)[b * p.k_b + t * p.k_t + h * p.k_h + col] : (IO)0.f;
+// Rows [B, T, H, K] that are no whole 16-byte vectors, as dense ones that are, zeros behind them.
+template <typename IO> __global__ __launch_bounds__(256) void delta_pad_kernel(const IO* src, IO* dst, long long rows, int T, int H, int K, int width, long long b_s, long long t_s, long long h_s) {
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= rows * width) return;
+  const long long row = i / width, token = row / H;
+  const int col = (int)(i % width);
+  dst[i] = col < K ? src[token / T * b_s + token % T * t_s + row % H * h_s + col] : (IO)0.f;
 }
-int delta_launch_pad(const DeltaArgs& a, void* q, void* k, int dtype, hipStream_t s) {
-  const long long n = (long long)a.B * a.T * a.H * a.width;
-  if (dtype == RGLRU_BF16) hipLaunchKernelGGL((delta_pad_kernel<__bf16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, (__bf16*)q, (__bf16*)k);
-  else hipLaunchKernelGGL((delta_pad_kernel<float>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, (float*)q, (float*)k);
-  return check_launch("gated_delta_fwd keys");
+int delta_launch_pad(const void* src, void* dst, int B, int T, int H, int K, int width, long long b_s, long long t_s, long long h_s, int dtype, hipStream_t s) {
+  const long long rows = (long long)B * T * H;
+  const dim3 grid((unsigned)((rows * width + 255) / 256));
+  if (dtype == RGLRU_BF16) hipLaunchKernelGGL((delta_pad_kernel<__bf16>), grid, dim3(256), 0, s, (const __bf16*)src, (__bf16*)dst, rows, T, H, K, width, b_s, t_s, h_s);
+  else hipLaunchKernelGGL((delta_pad_kernel<float>), grid, dim3(256), 0, s, (const float*)src, (float*)dst, rows, T, H, K, width, b_s, t_s, h_s);
+  return check_launch("gated_delta rows");
 }
 
 int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s) {

@@ -13,21 +13,23 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
+#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
 
 namespace rglru {
 
-template <typename IO, int KS, int WAVES> __global__ __launch_bounds__(64 * WAVES, 1) void delta_backward_kernel(DeltaArgs p) {
+template <typename IO, int KS, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void delta_backward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
   constexpr int DK = 32 * KS, PL = M::kPlanes, THREADS = 64 * WAVES, COLUMNS = 16 * WAVES;
   typedef Tile<IO, DK> Keys;
   typedef Tile<IO, 64> Square;
-  typedef ChunkTiles<IO, KS, THREADS, true> Tiles;
-  constexpr int STAGES = Tiles::kStages;
+  typedef Tile<IO, COLUMNS> Values;
+  typedef ChunkTiles<IO, KS, WAVES, true> Tiles;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * Tiles::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -41,30 +43,28 @@ template <typename IO, int KS, int WAVES> __global__ __launch_bounds__(64 * WAVE
   const unsigned lds0 = lds_address(lds);
 
   Tiles tiles;
-  tiles.setup(p, tid);
+  tiles.setup(p, tid, p.up_t, p.value_width - group * COLUMNS);
+  const IO* const ups = (const IO*)p.dout + b * p.up_b + hv * p.up_h + group * COLUMNS;
+  const bool vectors = p.value_width == p.V;
   f32x4 dstate[2 * KS], y[4];
-  int up_raw[4][4];
+  WaveRows<IO, COLUMNS> rows_out;
   auto request = [&](int n, int stage) {
-    tiles.request(p, first + n, n, b, h, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
-    const int t0 = n * kDeltaChunk;
-    const ColumnIo<IO> ups((const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) up_raw[mt][e] = ups.raw(mt, e);
+    tiles.request(p, first + n, n, b, h, ups + (long long)n * kDeltaChunk * p.up_t, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
   };
   auto put = [&](int n) {                                  // results of chunk n
     if (mine) {
       IO* at = (IO*)p.dvalues + ((first + n) * PL * p.columns + col) * 64;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) M::put(at + 16 * mt + 4 * g, (long long)p.columns * 64, y[mt]);
+      for (int mt = 0; mt < 4; ++mt) M::put(at + tile_index(mt, 4 * g), (long long)p.columns * 64, y[mt]);
     }
     const int t0 = n * kDeltaChunk;
-    const ColumnIo<IO> out((const IO*)p.dv + (((long long)b * p.T + t0) * p.HV + hv) * p.V, (long long)p.HV * p.V, p.T - t0, p.V, col, live, g);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out.store(mt, e, y[mt][e]);
+    const long long stride = (long long)p.HV * p.V;
+    IO* at = (IO*)p.dv + (((long long)b * p.T + t0) * p.HV + hv) * p.V;
+    if (vectors) {
+      if (mine) rows_out.store(at, stride, p.T - t0, p.V, col - c, lane);
+    } else {
+      ColumnIo<IO>(at, stride, p.T - t0, p.V, col, live, 8 * g).store(y);
+    }
   };
   const int last = p.nC - 1;
   request(last, 0);
@@ -72,7 +72,7 @@ template <typename IO, int KS, int WAVES> __global__ __launch_bounds__(64 * WAVE
   for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 16 * t + 4 * g + e;
+      const int row = tile_index(t, 4 * g + e);
       dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
     }
   wait_for_all();
@@ -83,87 +83,103 @@ template <typename IO, int KS, int WAVES> __global__ __launch_bounds__(64 * WAVE
              *within = (const IO*)(tile + Tiles::kWithin);
     const float* record = (const float*)(tile + Tiles::kRecord);
     const unsigned long long counts = counts_of(record);
-    f32x4 up[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) up[mt][e] = ColumnIo<IO>::value(up_raw[mt][e]);
     if (counts != ~0ull) {
       Tiles::clear_rows(tile, counts, tid);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) up[mt][e] = (counts >> (16 * mt + 4 * g + e)) & 1 ? up[mt][e] : 0.f;
       lds_barrier();
     }
-    Wide d[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) d[ks] = M::wide(dstate[2 * ks], dstate[2 * ks + 1]);
-    if (n != last) put(n + 1);
+    if (STAGES == 2 && n != last) put(n + 1);
     if (mine) {
       IO* at = (IO*)p.dstates + ((first + n) * PL * p.columns + col) * DK;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) M::put(at + 16 * t + 4 * g, (long long)p.columns * DK, dstate[t]);
+      for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), (long long)p.columns * DK, dstate[t]);
     }
     if (STAGES == 2 && n > 0) request(n - 1, stage ^ 1);
     if (mine) {
-      f32x4 rho[4];
+      Frag ka[2][4], kt[2][2 * KS], uf[2];
+      Wide ta[2][4];
+      auto rows = [&](int ks, Frag (&a)[4]) {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) rho[mt] = *reinterpret_cast<const f32x4*>(record + 16 * mt + 4 * g);
+        for (int mt = 0; mt < 4; ++mt) a[mt] = Keys::along_row(keys, tile_index(mt, c), 32 * ks, g);
+      };
+      auto square = [&](const IO* x, int ks, Wide (&a)[4]) {             // upper triangular: rows behind the columns are zeros
+#pragma unroll
+        for (int mt = 0; mt < 2 * ks + 2; ++mt) a[mt] = Square::wide_along_row(x, 4096, tile_index(mt, c), 32 * ks, g);
+      };
+      auto turned = [&](const IO* x, int ks, Frag (&a)[2 * KS]) {
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) a[t] = Keys::down_rows_tile(x, 32 * ks, t, lane);
+      };
+      phase();
+      rows(0, ka[0]);
+      f32x4 rho[4], up[4];
+      IO* const up_tile = (IO*)(tile + Tiles::kValues);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) uf[ks] = Values::down_rows(up_tile, 32 * ks, 16 * wave, lane);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g);
       const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
       // dZ = P^T dO + w K dS'
       f32x4 dz[4] = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) dz[mt] = M::ew(Keys::along_row(keys, 16 * mt + c, 32 * ks, g), d[ks], dz[mt]);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) dz[mt] *= *reinterpret_cast<const f32x4*>(record + 64 + 16 * mt + 4 * g);
-      {
-        const Frag uf[2] = {M::exact(up[0], up[1]), M::exact(up[2], up[3])};
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int mt = 0; mt < 2 * ks + 2; ++mt) dz[mt] = M::we(Square::wide_along_row(within, 4096, 16 * mt + c, 32 * ks, g), uf[ks], dz[mt]);
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) rows(ks + 1, ka[(ks + 1) & 1]);
+        else square(within, 0, ta[0]);
+        phase();
+        M::ew(dz, ka[ks & 1], M::wide(dstate[2 * ks], dstate[2 * ks + 1]));
+        phase();
       }
-      // Y = T^T dZ
-      {
-        const Wide zw[2] = {M::wide(dz[0], dz[1]), M::wide(dz[2], dz[3])};
+      square(within, 1, ta[1]);
+      M::apart(uf[0], up[0], up[1]);
+      M::apart(uf[1], up[2], up[3]);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int mt = 0; mt < 2 * ks + 2; ++mt) y[mt] = M::ww(Square::wide_along_row(solve, 4096, 16 * mt + c, 32 * ks, g), zw[ks], y[mt]);
-      }
-      // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y)
-      f32x4 ry[4];
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) ry[mt] = -rho[mt] * y[mt], up[mt] *= rho[mt] * p.scale;
-      const Wide uw[2] = {M::wide(up[0], up[1]), M::wide(up[2], up[3])}, yw[2] = {M::wide(ry[0], ry[1]), M::wide(ry[2], ry[3])};
+      for (int mt = 0; mt < 4; ++mt) dz[mt] *= tile_rows(record + 64, mt, g), up[mt] *= rho[mt] * p.scale;
+      phase();
+      M::template we<0, 2>(dz, ta[0], uf[0]);
+      phase();
+      square(solve, 0, ta[0]);
+      turned(queries, 0, kt[0]);
+      phase();
+      M::template we<0, 4>(dz, ta[1], uf[1]);
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) dstate[t] *= carry;
+      phase();
+      square(solve, 1, ta[1]);
+      phase();
+      // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y),  Y = T^T dZ
+      M::ew(dstate, kt[0], M::wide(up[0], up[1]));
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) {
-          dstate[t] = M::ew(Keys::down_rows(queries, 32 * ks, 16 * t, lane), uw[ks], dstate[t]);
-          dstate[t] = M::ew(Keys::down_rows(keys, 32 * ks, 16 * t, lane), yw[ks], dstate[t]);
-        }
+      for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      M::template ww<0, 2>(y, ta[0], M::wide(dz[0], dz[1]));
+      phase();
+      turned(queries, 1, kt[1]);
+      phase();
+      M::template ww<0, 4>(y, ta[1], M::wide(dz[2], dz[3]));
+      phase();
+      turned(keys, 0, kt[0]);
+      phase();
+      M::ew(dstate, kt[1], M::wide(up[2], up[3]));
+      phase();
+      turned(keys, 1, kt[1]);
+      phase();
+      M::ew(dstate, kt[0], M::wide(-rho[0] * y[0], -rho[1] * y[1]));
+      M::ew(dstate, kt[1], M::wide(-rho[2] * y[2], -rho[3] * y[3]));
+      if (vectors) rows_out.turn(up_tile, y, wave, lane);
+      phase();
     }
-    if (STAGES == 1 && n > 0) {
+    if (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
-      request(n - 1, 0);
+      if (n > 0) request(n - 1, 0);
+      put(n);
     }
     wait_for_all();
   }
-  put(0);
+  if (STAGES == 2) put(0);
   if (p.dh0 && live) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * t + 4 * g + e;
+        const int row = tile_index(t, 4 * g + e);
         if (row < p.K) p.dh0[((long long)head * p.K + row) * p.V + col] = dstate[t][e];
       }
   }
@@ -206,8 +222,8 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
     const float carry = gate.segments == 0 ? expf((float)gate.end) : 0.f;
     if (s == 0) {
       KeyRows<IO, DK, kDeltaThreads> k, q;
-      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, true, tid);
-      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, true, tid);
+      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, tid);
+      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, tid);
       k.put(keys, tid);
       q.put(queries, tid);
     } else {
@@ -221,14 +237,13 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
     }
     f32x4 dq[2 * KS] = {}, dr[2 * KS] = {}, dw[2 * KS] = {}, n1[4] = {}, n2[4] = {};
     float carried = 0.f;                                   // <S, dS'>
-    const IO* ups = (const IO*)p.dout + (((long long)b * p.T + t0) * p.HV + hv) * p.V;
-    const bool vec_up = ((long long)p.V * sizeof(IO)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dout) % 16 == 0;
+    const IO* ups = (const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h;
     for (int c0 = 0; c0 < p.columns; c0 += CB) {
       const int rows = p.columns - c0 < CB ? p.columns - c0 : CB;
       KeyRows<IO, CB, kDeltaThreads> up;
       MatrixRows<IO, CB, 64, kDeltaThreads> z, y;
       MatrixRows<IO, CB, DK, kDeltaThreads> st, ds;
-      up.request(ups + c0, (long long)p.HV * p.V, p.V - c0, counts, vec_up, tid);
+      up.request(ups + c0, p.up_t, p.value_width - c0, counts, tid);
       z.request((const IO*)p.values + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
       y.request((const IO*)p.dvalues + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
       st.request((const IO*)p.states + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
@@ -354,11 +369,11 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) {
         const bool live = 16 * t + c < p.K;
-        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, left, p.K, 16 * t + c, live, g), k_out((const IO*)p.dk + base, stride, left, p.K, 16 * t + c, live, g);
+        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, left, p.K, 16 * t + c, live, 4 * g), k_out((const IO*)p.dk + base, stride, left, p.K, 16 * t + c, live, 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          q_out.store(wave, e, GROUPED ? all_dq[t][e] : dq[t][e]);
-          k_out.store(wave, e, GROUPED ? all_dk[t][e] : dr[t][e]);
+          q_out.store(16 * wave + e, GROUPED ? all_dq[t][e] : dq[t][e]);
+          k_out.store(16 * wave + e, GROUPED ? all_dk[t][e] : dr[t][e]);
         }
       }
     }
@@ -380,10 +395,13 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
 }
 
 template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hipStream_t s) {
-  const int waves = delta_narrow(a) ? 2 : 4, total = (a.columns + 16 * waves - 1) / (16 * waves) * a.B * a.HV;
+  const char* w = getenv("DELTA_WAVES");
+  const int kind = sizeof(IO) == 4 ? 4 : w ? atoi(w) : 2, waves = kind == 2 ? 2 : 4, total = (a.columns + 16 * waves - 1) / (16 * waves) * a.B * a.HV;
   const dim3 walk((unsigned)((total + 7) / 8 * 8)), block(64 * waves);
-  if (waves == 2) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 2>), walk, block, 0, s, a);
-  else hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4>), walk, block, 0, s, a);
+  if constexpr (sizeof(IO) == 4) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 1>), walk, block, 0, s, a);
+  else if (kind == 2) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 2, 2>), walk, block, 0, s, a);
+  else if (kind == 4) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 1>), walk, block, 0, s, a);
+  else hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 2>), walk, block, 0, s, a);
   int rc = check_launch("gated_delta_bwd");
   if (rc) return rc;
   const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));

@@ -10,7 +10,7 @@
 namespace rglru {
 
 int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s);
-int delta_launch_pad(const DeltaArgs& a, void* q, void* k, int dtype, hipStream_t s);
+int delta_launch_pad(const void* src, void* dst, int B, int T, int H, int K, int width, long long b_s, long long t_s, long long h_s, int dtype, hipStream_t s);
 int delta_launch_backward(const DeltaArgs& a, int dtype, hipStream_t s);
 
 struct DeltaStepArgs {
@@ -126,11 +126,12 @@ template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bo
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 struct DeltaSizes {
-  int64_t chunks, columns, width, row;                     // row: elements of a key as the kernels read it
-  size_t gates, solve, within, q, k, states, values, total;  // offsets in the workspace; q and k: room where keys have to be padded
+  int64_t chunks, columns, width, row, value_row;          // rows: elements of a key and of a value as the kernels read them
+  size_t gates, solve, within, q, k, v, states, values, total;  // offsets in the workspace; q, k, v: room where rows have to be padded
+  size_t padded_v;
   DeltaSizes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, bool keep) {
     const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
-    row = (K + e - 1) / e * e;
+    row = (K + e - 1) / e * e, value_row = (V + e - 1) / e * e;
     chunks = B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk);
     columns = (V + 15) / 16 * 16;
     width = (K + 31) / 32 * 32;
@@ -142,12 +143,15 @@ struct DeltaSizes {
     const size_t padded = row != K ? up((size_t)(B * T * H * row) * (16 / e)) : 0;
     q = within + square;
     k = q + padded;
-    states = k + padded;
+    v = k + padded;
+    padded_v = value_row != V ? up((size_t)(B * T * HV * value_row) * (16 / e)) : 0;
+    states = v + padded_v;
     values = states + (keep ? up((size_t)chunks * columns * width * 4) : 0);
     total = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
   }
   size_t scratch_values() const { return ((size_t)chunks * columns * width * 4 + 255) & ~(size_t)255; }
-  size_t scratch() const { return scratch_values() + (size_t)chunks * columns * 64 * 4; }
+  size_t scratch_up() const { return scratch_values() + (((size_t)chunks * columns * 64 * 4 + 255) & ~(size_t)255); }
+  size_t scratch() const { return scratch_up() + padded_v; }
 };
 
 static int delta_check(const char* who, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int decay_dtype, int beta_dtype) {
@@ -157,15 +161,14 @@ static int delta_check(const char* who, int64_t B, int64_t T, int64_t H, int64_t
     if (d != RGLRU_F32 && d != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown dtype %d", who, d);
   if (K > kDeltaMaxKey) return fail(RGLRU_E_UNSUPPORTED, "%s: keys of %lld elements, at most %d are covered", who, (long long)K, kDeltaMaxKey);
   const int64_t most = (int64_t)1 << 30;
-  if (B * T * H >= (1ll << 38) / kDeltaMaxKey) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
+  if (B * T * H >= (1ll << 38) / kDeltaMaxKey || B * T * HV >= (1ll << 38) / (V + 8)) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   if (H * K >= most / 256 || HV * V >= most / 256) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens wider than %lld elements", who, (long long)(most / 256));
   if (T >= (1ll << 30) || B * HV * ((V + 63) / 64) >= most || B * HV * ((T + kDeltaChunk - 1) / kDeltaChunk) >= most)
     return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   return RGLRU_OK;
 }
 
-// Sizes, strides and the parts of the workspace.  Keys that are no whole vectors are read from their padded copies, which the
-// forward call makes.
+// Sizes, strides and the parts of the workspace.
 static int delta_operands(const char* who, DeltaArgs& a, const void* q, const void* k, const void* v, const int64_t* strides, void* ws, bool keep,
                           int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype) {
   const int64_t dense[9] = {T * H * K, H * K, K, T * H * K, H * K, K, T * HV * V, HV * V, V};
@@ -180,17 +183,22 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   a.nC = (int)((T + kDeltaChunk - 1) / kDeltaChunk);
   a.columns = (int)((V + 15) / 16 * 16);
   const DeltaSizes z(B, T, H, HV, K, V, dtype, keep);
-  a.width = (int)z.row;
+  a.width = (int)z.row, a.value_width = (int)z.value_row;
   const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
   bool whole = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0;
   for (int i = 0; i < 6; ++i) whole = whole && st[i] % e == 0;
   if (z.row == K && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of queries and keys must be 16-byte aligned", who);
+  whole = reinterpret_cast<uintptr_t>(v) % 16 == 0;
+  for (int i = 6; i < 9; ++i) whole = whole && st[i] % e == 0;
+  if (v && z.value_row == V && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of values must be 16-byte aligned", who);
+  a.segments = 1, a.length = a.nC;
   char* base = (char*)ws;
   a.gates = (float*)(base + z.gates);
   a.solve = base + z.solve, a.within = base + z.within;
   if (keep) a.states = base + z.states, a.values = base + z.values;
   return RGLRU_OK;
 }
+// Queries and keys that are no whole vectors are read from padded copies, which the forward call makes.
 static void delta_padded(DeltaArgs& a, void* ws, const DeltaSizes& z) {
   a.q = (char*)ws + z.q, a.k = (char*)ws + z.k;
   a.q_h = a.k_h = a.width, a.q_t = a.k_t = (long long)a.H * a.width, a.q_b = a.k_b = a.T * a.q_t;
@@ -209,9 +217,9 @@ size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, in
   return DeltaSizes(B, T, H, HV, K, V, dtype, keep != 0).total;
 }
 
-size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V) {
-  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey) return 0;
-  return DeltaSizes(B, T, 1, HV, K, V, RGLRU_F32, true).scratch();
+size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int dtype) {
+  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || K > kDeltaMaxKey || (dtype != RGLRU_F32 && dtype != RGLRU_BF16)) return 0;
+  return DeltaSizes(B, T, 1, HV, K, V, dtype, true).scratch();
 }
 
 int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* log_decay, const void* beta,
@@ -227,11 +235,19 @@ int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const
   if (rc) return rc;
   a.log_decay = log_decay, a.beta = beta, a.flags = flags, a.h0 = h0, a.out = out, a.h_last = h_last;
   a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
+  const DeltaSizes z(B, T, H, HV, K, V, dtype, keep != 0);
+  char* base = (char*)ws;
   if (a.width != a.K) {
-    const DeltaSizes z(B, T, H, HV, K, V, dtype, keep != 0);
-    rc = delta_launch_pad(a, (char*)ws + z.q, (char*)ws + z.k, dtype, (hipStream_t)stream);
+    rc = delta_launch_pad(q, base + z.q, a.B, a.T, a.H, a.K, a.width, a.q_b, a.q_t, a.q_h, dtype, (hipStream_t)stream);
+    if (!rc) rc = delta_launch_pad(k, base + z.k, a.B, a.T, a.H, a.K, a.width, a.k_b, a.k_t, a.k_h, dtype, (hipStream_t)stream);
     if (rc) return rc;
     delta_padded(a, ws, z);
+  }
+  if (a.value_width != a.V) {
+    rc = delta_launch_pad(v, base + z.v, a.B, a.T, a.HV, a.V, a.value_width, a.v_b, a.v_t, a.v_h, dtype, (hipStream_t)stream);
+    if (rc) return rc;
+    a.v = base + z.v;
+    a.v_h = a.value_width, a.v_t = (long long)a.HV * a.value_width, a.v_b = a.T * a.v_t;
   }
   return delta_launch_forward(a, keep != 0, dtype, (hipStream_t)stream);
 }
@@ -255,6 +271,15 @@ int rglru_hip_gated_delta_bwd(const void* q, const void* k, const int64_t* strid
   a.dq = dq, a.dk = dk, a.dv = dv, a.dlog_decay = dlog_decay, a.dbeta = dbeta, a.dh0 = dh0;
   a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
   a.dstates = scratch, a.dvalues = (char*)scratch + z.scratch_values();
+  if (a.value_width != a.V) {
+    void* up = (char*)scratch + z.scratch_up();
+    rc = delta_launch_pad(dout, up, a.B, a.T, a.HV, a.V, a.value_width, T * HV * V, HV * V, V, dtype, (hipStream_t)stream);
+    if (rc) return rc;
+    a.dout = up;
+  } else if (reinterpret_cast<uintptr_t>(dout) % 16 != 0) {
+    return fail(RGLRU_E_UNSUPPORTED, "gated_delta_bwd: dout must be 16-byte aligned");
+  }
+  a.up_h = a.value_width, a.up_t = (long long)a.HV * a.value_width, a.up_b = a.T * a.up_t;
   return delta_launch_backward(a, dtype, (hipStream_t)stream);
 }
 

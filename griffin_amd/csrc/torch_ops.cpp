@@ -2236,16 +2236,16 @@ struct DeltaOperands {
   Tensor q, k, v, log_decay, beta;
   int64_t strides[9];
   int64_t B, T, H, HV, K, V;
-  // whole: rows of whole 16-byte vectors have to lie on their boundaries
-  static Tensor rows(const Tensor& t, bool whole) {
+  // rows of whole 16-byte vectors have to lie on their boundaries
+  static Tensor rows(const Tensor& t) {
     const int64_t e = 16 / t.element_size();
-    bool plain = t.stride(3) == 1 || t.size(3) == 1;
-    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0 && (!whole || t.size(3) % e != 0 || t.stride(i) % e == 0);
-    if (whole && t.size(3) % e == 0) plain = plain && is_aligned(t);
-    return plain && t.stride(1) < (int64_t(1) << 22) ? t : whole ? aligned(t) : t.contiguous();
+    const bool whole = t.size(3) % e == 0;
+    bool plain = (t.stride(3) == 1 || t.size(3) == 1) && (!whole || is_aligned(t));
+    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0 && (!whole || t.stride(i) % e == 0);
+    return plain && t.stride(1) < (int64_t(1) << 22) ? t : aligned(t);
   }
   DeltaOperands(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& decay_in, const Tensor& beta_in)
-      : q(rows(q_in, true)), k(rows(k_in, true)), v(rows(v_in, false)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
+      : q(rows(q_in)), k(rows(k_in)), v(rows(v_in)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
     int at = 0;
     for (const Tensor* t : {&q, &k, &v})
       for (int i = 0; i < 3; ++i) strides[at++] = t->stride(i);
@@ -2315,12 +2315,12 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
       const int64_t B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), HV = m[0], V = m[1];
       int64_t strides[9];
       for (int i = 0; i < 3; ++i) strides[i] = q.stride(i), strides[3 + i] = k.stride(i), strides[6 + i] = 0;
-      Tensor dout = grads[0].defined() ? as(grads[0], dtype) : at::zeros({B, T, HV, V}, q.options());
+      Tensor dout = grads[0].defined() ? aligned(as(grads[0], dtype)) : at::zeros({B, T, HV, V}, q.options());
       Tensor dh_last = as(grads[1], at::kFloat);
       dq = fresh({B, T, H, K}, dtype, q), dk = fresh({B, T, H, K}, dtype, q), dv = fresh({B, T, HV, V}, dtype, q);
       dlog_decay = fresh_like(log_decay), dbeta = fresh_like(beta);
       if (Needs(ctx)(5)) dh0 = fresh({B, HV, K, V}, at::kFloat, q);
-      Tensor scratch = bytes(rglru_hip_gated_delta_scratch_bytes(B, T, HV, K, V), q);
+      Tensor scratch = bytes(rglru_hip_gated_delta_scratch_bytes(B, T, HV, K, V, code_of(dtype)), q);
       check(rglru_hip_gated_delta_bwd(ptr(q), ptr(k), strides, ptr(log_decay), ptr(beta), bptr(flags), ptr(dout), fptr(dh_last), ptr(kept), ptr(scratch),
                                       ptr(dq), ptr(dk), ptr(dv), ptr(dlog_decay), ptr(dbeta), fptr(dh0),
                                       static_cast<float>(ctx->saved_data["scale"].toDouble()), B, T, H, HV, K, V, code_of(dtype),

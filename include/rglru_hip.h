@@ -376,8 +376,8 @@ int rglru_hip_rmsnorm_bwd(const void* x, const void* g, const float* inv, const 
  * rglru_hip_gated_delta_max_key_size(); V is free.  Log decays are meant to be at most 0; one below -1e4 (minus infinity among them)
  * discards the history as a reset does.  Unit keys and beta in [0, 2] keep the recurrence from growing.
  *   strides  NULL (everything dense), or nine counts of elements in HOST memory: batch, token and head stride of q, of k, of v
- *            (non-negative; the last axis is contiguous).  out and all gradients are dense.  Where K is a whole number of
- *            16-byte vectors, rows of q and k lie on 16-byte boundaries; other keys are padded by a copy in ws.
+ *            (non-negative; the last axis is contiguous).  out and all gradients are dense.  Where K (V) is a whole number
+ *            of 16-byte vectors, the rows of q and k (v; dout) lie on 16-byte boundaries; others are padded by a copy in ws.
  *   flags    [B, T] or NULL: a reset discards the history in front of its token; an inactive token leaves the state as it is, gives
  *            zeros, takes part in no gradient, and nothing it holds is read.  A reset of an inactive token does not count.
  *   h0, h_last, dh_last, dh0 may be NULL.
@@ -388,7 +388,7 @@ int rglru_hip_rmsnorm_bwd(const void* x, const void* g, const float* inv, const 
  * The step takes one token a row (no T axis, everything dense) and updates `state` in place; inactive rows keep theirs. */
 int rglru_hip_gated_delta_max_key_size(void);
 size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int keep);
-size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V);
+size_t rglru_hip_gated_delta_scratch_bytes(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int dtype);
 int rglru_hip_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* log_decay,
                               const void* beta, const float* h0, const uint8_t* flags, void* out, float* h_last, void* ws, int keep,
                               float scale, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype,
