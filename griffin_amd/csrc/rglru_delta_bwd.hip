@@ -192,151 +192,187 @@ RGLRU_DEVICE float sixteen_sum(float v) {
   return v;
 }
 
-// Gradients of queries, keys and gates of one chunk and key head.  A wave owns 16 tokens.  The contractions over the value
-// columns take 32 of them at a time through LDS; N1 and N2 go through LDS once, where the columns lay.
-template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDeltaThreads) void delta_grads_kernel(DeltaArgs p) {
+// Gradients of queries, keys and gates of one chunk and key head.  Eight waves: four times 16 tokens, by two halves of the key's
+// columns; the first half's waves make N1, the second half's N2.  The contractions over the value columns take 32 of them at a time
+// through LDS, the next 32 on their way there where two fit; N1 and N2 go through LDS once, where the columns lay.
+constexpr int kGradThreads = 512;
+template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradThreads, 2) void delta_grads_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
-  constexpr int DK = 32 * KS, PL = M::kPlanes, CB = 32;
+  constexpr int DK = 32 * KS, PL = M::kPlanes, CB = 32, THREADS = kGradThreads;
   typedef Tile<IO, DK> Keys;
   typedef Tile<IO, 64> Square;
   typedef Tile<IO, CB> Ups;
-  constexpr int kUp = 0, kValues = kUp + 64 * CB, kDValues = kValues + PL * CB * 64, kStates = kDValues + PL * CB * 64,
-                kDStates = kStates + PL * CB * DK, kColumns = kDStates + PL * CB * DK, kPairs = 2 * PL * 4096;
-  __shared__ __attribute__((aligned(16))) IO keys[64 * DK], queries[64 * DK], area[kColumns > kPairs ? kColumns : kPairs];
+  typedef TileLoad<IO, 64, DK, THREADS> KeyLoad;
+  typedef TileLoad<IO, 64, CB, THREADS> UpLoad;
+  typedef TileLoad<IO, CB, 64, THREADS> ValueLoad;          // one plane
+  typedef TileLoad<IO, CB, DK, THREADS> StateLoad;
+  constexpr int kUp = 0, kValues = kUp + UpLoad::kBytes, kDValues = kValues + PL * ValueLoad::kBytes, kStates = kDValues + PL * ValueLoad::kBytes,
+                kDStates = kStates + PL * StateLoad::kBytes, kStage = kDStates + PL * StateLoad::kBytes, kPairs = 2 * PL * 4096 * (int)sizeof(IO);
+  constexpr int STAGES = 2 * kStage + 2 * KeyLoad::kBytes + 4096 <= 160 * 1024 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * KeyLoad::kBytes + (STAGES * kStage > kPairs ? STAGES * kStage : kPairs)];
   __shared__ double total[64];
-  __shared__ float beta[64], to_end[64], dtotal[64], dwrite[64], sums[4];
+  __shared__ float beta[64], to_end[64], reads[2][64], writes[2][64], leaves[2][64], sums[8];
   __shared__ int segment[64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
   const int n = (int)(blockIdx.x % (unsigned)p.nC), bh = (int)(blockIdx.x / (unsigned)p.nC), h = bh % p.H, b = bh / p.H;
-  const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H, row0 = 16 * wave + 4 * g;
-  f32x4 all_dq[GROUPED ? 2 * KS : 1] = {}, all_dk[GROUPED ? 2 * KS : 1] = {};
+  const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H, row0 = 16 * block + 4 * g;
+  IO *const keys = (IO*)lds, *const queries = (IO*)(lds + KeyLoad::kBytes), *const area = (IO*)(lds + 2 * KeyLoad::kBytes);
+  const unsigned lds0 = lds_address(lds);
+  f32x4 all_dq[KS] = {}, all_dk[KS] = {};                   // over the value heads that share the key head
+  UpLoad up_load;
+  ValueLoad value_load;
+  StateLoad state_load;
+  up_load.setup(tid, p.up_t, p.value_width);
+  value_load.setup(tid, 64, 64);
+  state_load.setup(tid, DK, DK);
 
   for (int s = 0; s < share; ++s) {
     const int hv = h * share + s, head = b * p.HV + hv;
     const long long chunk = (long long)head * p.nC + n;
+    auto request = [&](int c0, int stage) {
+      const int there = p.columns - c0;                     // columns of the values from here on
+      const unsigned to = lds0 + 2 * KeyLoad::kBytes + (unsigned)(stage * kStage);
+      const int width = p.value_width - c0;
+      up_load.request(delta_rsrc((const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h + c0, width < CB ? UpLoad::extent(p.up_t, width, left) : UpLoad::extent(p.up_t, CB, left)),
+                      to + kUp, wave);
+#pragma unroll
+      for (int plane = 0; plane < PL; ++plane) {
+        const long long at = (chunk * PL + plane) * p.columns + c0;
+        value_load.request(delta_rsrc((const IO*)p.values + at * 64, ValueLoad::extent(64, 64, there)), to + kValues + plane * ValueLoad::kBytes, wave);
+        value_load.request(delta_rsrc((const IO*)p.dvalues + at * 64, ValueLoad::extent(64, 64, there)), to + kDValues + plane * ValueLoad::kBytes, wave);
+        state_load.request(delta_rsrc((const IO*)p.states + at * DK, StateLoad::extent(DK, DK, there)), to + kStates + plane * StateLoad::kBytes, wave);
+        state_load.request(delta_rsrc((const IO*)p.dstates + at * DK, StateLoad::extent(DK, DK, there)), to + kDStates + plane * StateLoad::kBytes, wave);
+      }
+    };
+    if (s > 0) __syncthreads();                             // the head before is through with the shared arrays
+    if (s == 0) {
+      KeyLoad k;
+      k.setup(tid, p.k_t, p.width);
+      k.request(delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left)), lds0, wave);
+      k.setup(tid, p.q_t, p.width);
+      k.request(delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, KeyLoad::extent(p.q_t, p.width, left)), lds0 + KeyLoad::kBytes, wave);
+    }
+    request(0, 0);
     const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
     const unsigned long long counts = __ballot(gate.counts);
     const float carry = gate.segments == 0 ? expf((float)gate.end) : 0.f;
-    if (s == 0) {
-      KeyRows<IO, DK, kDeltaThreads> k, q;
-      k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, tid);
-      q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, tid);
-      k.put(keys, tid);
-      q.put(queries, tid);
-    } else {
-      __syncthreads();                                     // the head before is through with the shared arrays
-    }
     if (wave == 0) {
       total[lane] = gate.total;
       beta[lane] = gate.beta;
       segment[lane] = gate.segment;
       to_end[lane] = gate.segment == gate.segments ? expf((float)(gate.end - gate.total)) : 0.f;
     }
-    f32x4 dq[2 * KS] = {}, dr[2 * KS] = {}, dw[2 * KS] = {}, n1[4] = {}, n2[4] = {};
+    f32x4 dq[KS] = {}, dr[KS] = {}, dw[KS] = {}, pairs[4] = {};
     float carried = 0.f;                                   // <S, dS'>
-    const IO* ups = (const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h;
+    wait_for_all();
     for (int c0 = 0; c0 < p.columns; c0 += CB) {
-      const int rows = p.columns - c0 < CB ? p.columns - c0 : CB;
-      KeyRows<IO, CB, kDeltaThreads> up;
-      MatrixRows<IO, CB, 64, kDeltaThreads> z, y;
-      MatrixRows<IO, CB, DK, kDeltaThreads> st, ds;
-      up.request(ups + c0, p.up_t, p.value_width - c0, counts, tid);
-      z.request((const IO*)p.values + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
-      y.request((const IO*)p.dvalues + (chunk * PL * p.columns + c0) * 64, (long long)p.columns * 64, rows, tid);
-      st.request((const IO*)p.states + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
-      ds.request((const IO*)p.dstates + (chunk * PL * p.columns + c0) * DK, (long long)p.columns * DK, rows, tid);
-      __syncthreads();                                     // the columns before have been read
-      up.put(area + kUp, tid);
-      z.put(area + kValues, tid);
-      y.put(area + kDValues, tid);
-      st.put(area + kStates, tid);
-      ds.put(area + kDStates, tid);
-      __syncthreads();
-      const Frag uf = Ups::along_row(area + kUp, 16 * wave + c, 0, g);
-      const Wide zf = Square::wide_down_rows(area + kValues, CB * 64, 0, 16 * wave, lane);
-      const Wide yf = Square::wide_down_rows(area + kDValues, CB * 64, 0, 16 * wave, lane);
+      const int stage = STAGES == 2 ? (c0 / CB) & 1 : 0;
+      unsigned char* tile = lds + 2 * KeyLoad::kBytes + stage * kStage;
+      if (counts != ~0ull) {                               // zeros for the rows of tokens that do not count
+        for (int at = tid; at < 64 * Ups::U; at += THREADS)
+          if (!((counts >> (at / Ups::U)) & 1)) *reinterpret_cast<i32x4*>(tile + kUp + at * 16) = i32x4{0, 0, 0, 0};
+        if (s == 0 && c0 == 0)
+          for (int at = tid; at < 64 * Keys::U; at += THREADS)
+            if (!((counts >> (at / Keys::U)) & 1)) {
+              *reinterpret_cast<i32x4*>((unsigned char*)keys + at * 16) = i32x4{0, 0, 0, 0};
+              *reinterpret_cast<i32x4*>((unsigned char*)queries + at * 16) = i32x4{0, 0, 0, 0};
+            }
+        lds_barrier();
+      }
+      if (STAGES == 2 && c0 + CB < p.columns) request(c0 + CB, stage ^ 1);
+      const IO *ups = (const IO*)(tile + kUp), *values = (const IO*)(tile + kValues), *dvalues = (const IO*)(tile + kDValues),
+               *states = (const IO*)(tile + kStates), *dstates = (const IO*)(tile + kDStates);
+      const Frag uf = Ups::along_row(ups, 16 * block + c, 0, g);
+      const Wide zf = Square::wide_down_rows(values, CB * 64, 0, 16 * block, lane);
+      const Wide yf = Square::wide_down_rows(dvalues, CB * 64, 0, 16 * block, lane);
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
-        if (jt <= wave) {
-          const Wide zj = Square::wide_down_rows(area + kValues, CB * 64, 0, 16 * jt, lane);
-          n1[jt] = M::ew(uf, zj, n1[jt]);
-          n2[jt] = M::ww(yf, zj, n2[jt]);
+        if (jt <= block) {
+          const Wide zj = Square::wide_down_rows(values, CB * 64, 0, 16 * jt, lane);
+          pairs[jt] = half == 0 ? M::ew(uf, zj, pairs[jt]) : M::ww(yf, zj, pairs[jt]);
         }
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        const Wide sf = Keys::wide_down_rows(area + kStates, CB * DK, 0, 16 * t, lane);
-        const Wide df = Keys::wide_down_rows(area + kDStates, CB * DK, 0, 16 * t, lane);
+      for (int t = 0; t < KS; ++t) {
+        const Wide sf = Keys::wide_down_rows(states, CB * DK, 0, 16 * (half * KS + t), lane);
+        const Wide df = Keys::wide_down_rows(dstates, CB * DK, 0, 16 * (half * KS + t), lane);
         dq[t] = M::ew(uf, sf, dq[t]);
         dr[t] = M::ww(yf, sf, dr[t]);
         dw[t] = M::ww(zf, df, dw[t]);
+        phase();
       }
-      for (int i = tid; i < CB * DK; i += kDeltaThreads) {
-        if constexpr (PL == 2) carried = fmaf((float)area[kStates + i] + (float)area[kStates + CB * DK + i], (float)area[kDStates + i] + (float)area[kDStates + CB * DK + i], carried);
-        else carried = fmaf((float)area[kStates + i], (float)area[kDStates + i], carried);
+      for (int at = tid; at < CB * Keys::U; at += THREADS) {
+        typedef IO Unit __attribute__((ext_vector_type(Keys::E)));
+        const Unit a = *reinterpret_cast<const Unit*>(states + at * Keys::E), d = *reinterpret_cast<const Unit*>(dstates + at * Keys::E);
+        if constexpr (PL == 2) {
+          const Unit al = *reinterpret_cast<const Unit*>(states + CB * DK + at * Keys::E), dl = *reinterpret_cast<const Unit*>(dstates + CB * DK + at * Keys::E);
+#pragma unroll
+          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], carried);
+        } else {
+#pragma unroll
+          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e], (float)d[e], carried);
+        }
       }
+      if (STAGES == 1 && c0 + CB < p.columns) {
+        lds_barrier();                                     // the columns have been read
+        request(c0 + CB, 0);
+      }
+      wait_for_all();
     }
     // the factors of what reads the carried state and of what is left for the next chunk; the decays of the pairs
-    float dk_written[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = row0 + e;
       const float rho = segment[i] == 0 ? expf((float)total[i]) : 0.f, end = to_end[i];
       float dot = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
+      for (int t = 0; t < KS; ++t) {
         dq[t][e] *= p.scale * rho;
         dr[t][e] *= -rho;
         dw[t][e] *= end;
-        dot = fmaf(dw[t][e], (float)keys[Keys::at(i, 16 * t + c)], dot);
+        dot = fmaf(dw[t][e], (float)keys[Keys::at(i, 16 * (half * KS + t) + c)], dot);
       }
-      dk_written[e] = beta[i] * sixteen_sum(dot);
+      dot = sixteen_sum(dot);
+      if (c == 0) leaves[half][i] = beta[i] * dot;
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt) {
         const int j = 16 * jt + c;
-        const bool joined = i >= j && segment[i] == segment[j];
+        const bool joined = i >= j + half && segment[i] == segment[j];   // N2: strictly in front
         const float d = joined ? expf((float)(total[i] - total[j])) : 0.f;
-        n1[jt][e] = joined ? p.scale * d * n1[jt][e] : 0.f;
-        n2[jt][e] = joined && i > j ? -d * n2[jt][e] : 0.f;
+        pairs[jt][e] = joined ? (half == 0 ? p.scale * d : -d) * pairs[jt][e] : 0.f;
       }
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) carried += __shfl_xor(carried, m, 64);
-    __syncthreads();                                       // the last columns have been read
+    if (lane == 0) sums[wave] = carried;
     auto put_pairs = [&](bool strengths) {                 // kept [j][i]; blocks above the diagonal that a product touches are zeros
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
-        if (jt <= (wave | 1)) {
-          const float f = strengths ? beta[16 * jt + c] : 1.f;
-          const int at = Square::at(16 * jt + c, row0);
-          M::put(area + at, 4096, n1[jt] * f);
-          M::put(area + PL * 4096 + at, 4096, n2[jt] * f);
-        }
+        if (jt <= (block | 1)) M::put(area + half * PL * 4096 + Square::at(16 * jt + c, row0), 4096, pairs[jt] * (strengths ? beta[16 * jt + c] : 1.f));
     };
     put_pairs(false);
-    if (lane == 0) sums[wave] = carried;
     __syncthreads();
     // F = N1^T Q + N2^T K + ...: pairs in which the wave's tokens are the written ones
-    for (int ks = wave >> 1; ks < 2; ++ks) {
-      const Wide a = Square::wide_along_row(area, 4096, 16 * wave + c, 32 * ks, g);
-      const Wide a2 = Square::wide_along_row(area + PL * 4096, 4096, 16 * wave + c, 32 * ks, g);
+    for (int ks = block >> 1; ks < 2; ++ks) {
+      const Wide a = Square::wide_along_row(area, 4096, 16 * block + c, 32 * ks, g);
+      const Wide a2 = Square::wide_along_row(area + PL * 4096, 4096, 16 * block + c, 32 * ks, g);
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        dw[t] = M::we(a, Keys::down_rows(queries, 32 * ks, 16 * t, lane), dw[t]);
-        dw[t] = M::we(a2, Keys::down_rows(keys, 32 * ks, 16 * t, lane), dw[t]);
+      for (int t = 0; t < KS; ++t) {
+        dw[t] = M::we(a, Keys::down_rows(queries, 32 * ks, 16 * (half * KS + t), lane), dw[t]);
+        dw[t] = M::we(a2, Keys::down_rows(keys, 32 * ks, 16 * (half * KS + t), lane), dw[t]);
       }
     }
     __syncthreads();
     put_pairs(true);
     __syncthreads();
-    for (int ks = 0; ks <= (wave >> 1); ++ks) {
-      const Wide a = Square::wide_down_rows(area, 4096, 32 * ks, 16 * wave, lane);
-      const Wide a2 = Square::wide_down_rows(area + PL * 4096, 4096, 32 * ks, 16 * wave, lane);
+    for (int ks = 0; ks <= (block >> 1); ++ks) {
+      const Wide a = Square::wide_down_rows(area, 4096, 32 * ks, 16 * block, lane);
+      const Wide a2 = Square::wide_down_rows(area + PL * 4096, 4096, 32 * ks, 16 * block, lane);
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        const Frag kf = Keys::down_rows(keys, 32 * ks, 16 * t, lane);
+      for (int t = 0; t < KS; ++t) {
+        const Frag kf = Keys::down_rows(keys, 32 * ks, 16 * (half * KS + t), lane);
         dq[t] = M::we(a, kf, dq[t]);
         dr[t] = M::we(a2, kf, dr[t]);
       }
@@ -346,40 +382,23 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
       const int i = row0 + e;
       float read = 0.f, written = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        const float k = (float)keys[Keys::at(i, 16 * t + c)], q = (float)queries[Keys::at(i, 16 * t + c)];
+      for (int t = 0; t < KS; ++t) {
+        const int at = Keys::at(i, 16 * (half * KS + t) + c);
+        const float k = (float)keys[at], q = (float)queries[at];
         read = fmaf(q, dq[t][e], fmaf(k, dr[t][e], read));
         written = fmaf(k, dw[t][e], written);
+        dr[t][e] = fmaf(beta[i], dw[t][e], dr[t][e]);
+        all_dq[t][e] = GROUPED ? all_dq[t][e] + dq[t][e] : dq[t][e];
+        all_dk[t][e] = GROUPED ? all_dk[t][e] + dr[t][e] : dr[t][e];
       }
       read = sixteen_sum(read);
       written = sixteen_sum(written);
-      if (c == 0) {
-        dtotal[i] = read - beta[i] * written;
-        dwrite[i] = dk_written[e];
-        if (i < left) delta_put_gate(p.dbeta, ((long long)b * p.T + t0 + i) * p.HV + hv, p.beta_dtype, written);
-      }
-#pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        dr[t][e] = fmaf(beta[i], dw[t][e], dr[t][e]);
-        if constexpr (GROUPED) all_dq[t][e] += dq[t][e], all_dk[t][e] += dr[t][e];
-      }
-    }
-    if (!GROUPED || s == share - 1) {
-      const long long stride = (long long)p.H * p.K, base = ((long long)b * p.T + t0) * stride + (long long)h * p.K;
-#pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) {
-        const bool live = 16 * t + c < p.K;
-        const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, left, p.K, 16 * t + c, live, 4 * g), k_out((const IO*)p.dk + base, stride, left, p.K, 16 * t + c, live, 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q_out.store(16 * wave + e, GROUPED ? all_dq[t][e] : dq[t][e]);
-          k_out.store(16 * wave + e, GROUPED ? all_dk[t][e] : dr[t][e]);
-        }
-      }
+      if (c == 0) reads[half][i] = read, writes[half][i] = written;
     }
     __syncthreads();
     if (wave == 0) {                                       // sums from each token to the chunk's end
-      float write = dwrite[lane], from = dtotal[lane];
+      const float written = writes[0][lane] + writes[1][lane];
+      float write = leaves[0][lane] + leaves[1][lane], from = (reads[0][lane] + reads[1][lane]) - beta[lane] * written;
 #pragma unroll
       for (int m = 32; m >= 1; m >>= 1) write += __shfl_xor(write, m, 64);
 #pragma unroll
@@ -387,9 +406,46 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kDelta
         const float other = __shfl_down(from, d, 64);
         if (lane + d < 64) from += other;
       }
-      const float across = carry == 0.f ? 0.f : carry * ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+      float across = 0.f;
+#pragma unroll
+      for (int w = 0; w < THREADS / 64; ++w) across += sums[w];
+      across = carry == 0.f ? 0.f : carry * across;
       const float d = gate.counts && !gate.starts ? from + (write + across) : 0.f;
-      if (lane < left) delta_put_gate(p.dlog_decay, ((long long)b * p.T + t0 + lane) * p.HV + hv, p.decay_dtype, d);
+      const long long at = ((long long)b * p.T + t0 + lane) * p.HV + hv;
+      if (lane < left) {
+        delta_put_gate(p.dlog_decay, at, p.decay_dtype, d);
+        delta_put_gate(p.dbeta, at, p.beta_dtype, written);
+      }
+    }
+  }
+  const long long stride = (long long)p.H * p.K, base = ((long long)b * p.T + t0) * stride + (long long)h * p.K;
+  if (p.width == p.K) {                                     // through the tiles of queries and keys, which all waves are through with
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = Keys::at(row0 + e, 16 * (half * KS + t) + c);
+        queries[at] = (IO)all_dq[t][e];
+        keys[at] = (IO)all_dk[t][e];
+      }
+    __syncthreads();
+    for (int at = tid; at < 64 * Keys::U; at += THREADS) {
+      const int row = at / Keys::U, u = at % Keys::U;
+      if (row >= left || u * Keys::E >= p.K) continue;
+      const long long to = base + row * stride + u * Keys::E;
+      *reinterpret_cast<i32x4*>((IO*)p.dq + to) = *reinterpret_cast<const i32x4*>(queries + Keys::unit(row, u));
+      *reinterpret_cast<i32x4*>((IO*)p.dk + to) = *reinterpret_cast<const i32x4*>(keys + Keys::unit(row, u));
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      const int col = 16 * (half * KS + t) + c;
+      const ColumnIo<IO> q_out((const IO*)p.dq + base, stride, left, p.K, col, col < p.K, 4 * g), k_out((const IO*)p.dk + base, stride, left, p.K, col, col < p.K, 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        q_out.store(16 * block + e, all_dq[t][e]);
+        k_out.store(16 * block + e, all_dk[t][e]);
+      }
     }
   }
 }
@@ -405,8 +461,8 @@ template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hip
   int rc = check_launch("gated_delta_bwd");
   if (rc) return rc;
   const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));
-  if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kDeltaThreads), 0, s, a);
-  else hipLaunchKernelGGL((delta_grads_kernel<IO, KS, false>), grid, dim3(kDeltaThreads), 0, s, a);
+  if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kGradThreads), 0, s, a);
+  else hipLaunchKernelGGL((delta_grads_kernel<IO, KS, false>), grid, dim3(kGradThreads), 0, s, a);
   return check_launch("gated_delta_bwd gradients");
 }
 
