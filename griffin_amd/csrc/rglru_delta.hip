@@ -154,7 +154,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
   const int group = work % groups, segment = work / groups % p.segments, head = work / groups / p.segments;
   const int hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
   const bool unit = !OUT && group >= value_groups;
-  if (!OUT && !unit && segment == p.segments - 1) return;                // nothing starts behind the last segment
+  // nothing starts behind the last segment; what it makes of its state is for the backward pass
+  if (!OUT && segment == p.segments - 1 && !(unit && p.states)) return;
   const int col = (unit ? group - value_groups : group) * COLUMNS + wave * 16 + c, width = unit ? DK : p.columns;
   const bool mine = col - c < width, live = mine && (unit || col < p.V);
   const int begin = segment * p.length, end = begin + p.length < p.nC ? begin + p.length : p.nC;
@@ -350,25 +351,98 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
   }
 }
 
-template <typename IO, int KS, int WAVES, int STAGES> static void delta_walk_forward(const DeltaArgs& a, bool save, hipStream_t s) {
-  const int total = (a.columns + 16 * WAVES - 1) / (16 * WAVES) * a.segments * a.B * a.HV;
+// The states that segments start from: S' = L + M S with what a segment adds (`local`) and makes of its state (`through`, [in][out]).
+// BACKWARD: the gradients behind the segments, dS = L + M^T dS'.  A wave owns 16 columns again; M goes to LDS a segment ahead.
+template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDeltaThreads) void delta_join_kernel(DeltaArgs p) {
+  typedef Mx<IO> M;
+  typedef typename M::Wide Wide;
+  constexpr int DK = 32 * KS, PL = M::kPlanes;
+  typedef Tile<IO, DK> Square;
+  typedef TileLoad<IO, PL * DK, DK, kDeltaThreads> Load;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * Load::kBytes];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = (p.columns + 63) / 64, group = (int)(blockIdx.x % (unsigned)groups), head = (int)(blockIdx.x / (unsigned)groups);
+  const int col = group * 64 + wave * 16 + c;
+  const bool mine = col - c < p.columns, live = col < p.V;
+  const unsigned lds0 = lds_address(lds);
+  const int from = BACKWARD ? p.segments - 1 : 0, to = BACKWARD ? 0 : p.segments - 1, step = BACKWARD ? -1 : 1;
+  const float* first = BACKWARD ? p.dh_last : p.h0;
+  Load load;
+  load.setup(tid, DK, DK);
+  auto request = [&](int s, int stage) {
+    load.request(delta_rsrc((const IO*)p.through + ((long long)head * p.segments + s) * (PL * DK * DK), Load::kBytes), lds0 + (unsigned)(stage * Load::kBytes), wave);
+  };
+  f32x4 state[2 * KS];
+  request(from, 0);
+#pragma unroll
+  for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = tile_index(t, 4 * g + e);
+      state[t][e] = first && live && row < p.K ? first[((long long)head * p.K + row) * p.V + col] : 0.f;
+    }
+  for (int s = from;; s += step) {
+    const long long at = (((long long)head * p.segments + s) * p.columns + (mine ? col : 0)) * DK;
+    if (mine) {
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) *reinterpret_cast<f32x4*>(p.edges + at + tile_index(t, 4 * g)) = state[t];
+    }
+    if (s == to) break;
+    const int stage = (s - from) & 1;
+    f32x4 next[2 * KS];
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) next[t] = *reinterpret_cast<const f32x4*>(p.local + at + tile_index(t, 4 * g));
+    wait_for_all();
+    if (s + step != to) request(s + step, stage ^ 1);
+    const IO* through = (const IO*)(lds + stage * Load::kBytes);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const Wide x = M::wide(state[2 * ks], state[2 * ks + 1]);
+      Wide a[2 * KS];
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t)
+        a[t] = BACKWARD ? Square::wide_along_row(through, DK * DK, tile_index(t, c), 32 * ks, g) : Square::wide_down_rows_tile(through, DK * DK, 32 * ks, t, lane);
+      M::template ww<0, 2 * KS>(next, a, x);
+      phase();
+    }
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) state[t] = next[t];
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // a request that nothing was read of
+}
+template <typename IO, int KS> int delta_join(const DeltaArgs& a, bool backward, hipStream_t s) {
+  const dim3 grid((unsigned)((a.columns + 63) / 64 * a.B * a.HV));
+  if (backward) hipLaunchKernelGGL((delta_join_kernel<IO, KS, true>), grid, dim3(kDeltaThreads), 0, s, a);
+  else hipLaunchKernelGGL((delta_join_kernel<IO, KS, false>), grid, dim3(kDeltaThreads), 0, s, a);
+  return check_launch("gated_delta segments");
+}
+
+template <typename IO, int KS, int WAVES, int STAGES, bool SAVE, bool OUT> static int delta_walk(const DeltaArgs& a, hipStream_t s) {
+  const int width = 16 * WAVES, groups = (a.columns + width - 1) / width + (OUT ? 0 : (32 * KS + width - 1) / width);
+  const long long total = (long long)groups * a.segments * a.B * a.HV;
   const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(64 * WAVES);
-  if (save) hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, true, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, false, true>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, SAVE, OUT>), grid, block, 0, s, a);
+  return check_launch("gated_delta_fwd");
 }
 
 template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool save, hipStream_t s) {
   hipLaunchKernelGGL((delta_prepare_kernel<IO, KS>), dim3((unsigned)((long long)a.B * a.HV * a.nC)), dim3(kDeltaThreads), 0, s, a);
   int rc = check_launch("gated_delta_fwd prepare");
   if (rc) return rc;
+  constexpr bool kTwo = sizeof(IO) == 2;                    // two chunks' tiles fit the LDS
   const char* w = getenv("DELTA_WAVES");
   const int waves = w ? atoi(w) : 2;
-  if constexpr (sizeof(IO) == 2) {
-  if (waves == 2) delta_walk_forward<IO, KS, 2, 2>(a, save, s);
-  else if (waves == 4) delta_walk_forward<IO, KS, 4, 1>(a, save, s);
-  else delta_walk_forward<IO, KS, 4, 2>(a, save, s);
-  } else delta_walk_forward<IO, KS, 4, 1>(a, save, s);
-  return check_launch("gated_delta_fwd");
+  if (a.segments > 1) {
+    const char* l = getenv("DELTA_LOCAL");
+    if (l && atoi(l) == 2) rc = delta_walk<IO, KS, 4, kTwo ? 2 : 1, false, false>(a, s);
+    else rc = delta_walk<IO, KS, 4, 1, false, false>(a, s);
+    if (!rc) rc = delta_join<IO, KS>(a, false, s);
+    if (rc) return rc;
+  }
+  if (kTwo && waves == 2) return save ? delta_walk<IO, KS, 2, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 2, kTwo ? 2 : 1, false, true>(a, s);
+  if (kTwo && waves == 4) return save ? delta_walk<IO, KS, 4, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 4, kTwo ? 2 : 1, false, true>(a, s);
+  return save ? delta_walk<IO, KS, 4, 1, true, true>(a, s) : delta_walk<IO, KS, 4, 1, false, true>(a, s);
 }
 
 // Rows [B, T, H, K] that are no whole 16-byte vectors, as dense ones that are, zeros behind them.
@@ -385,6 +459,18 @@ int delta_launch_pad(const void* src, void* dst, int B, int T, int H, int K, int
   if (dtype == RGLRU_BF16) hipLaunchKernelGGL((delta_pad_kernel<__bf16>), grid, dim3(256), 0, s, (const __bf16*)src, (__bf16*)dst, rows, T, H, K, width, b_s, t_s, h_s);
   else hipLaunchKernelGGL((delta_pad_kernel<float>), grid, dim3(256), 0, s, (const float*)src, (float*)dst, rows, T, H, K, width, b_s, t_s, h_s);
   return check_launch("gated_delta rows");
+}
+
+int delta_launch_join(const DeltaArgs& a, int dtype, hipStream_t s) {
+  switch ((a.K + 31) / 32) {
+#define RGLRU_DELTA(KS) case KS: return dtype == RGLRU_BF16 ? delta_join<__bf16, KS>(a, true, s) : delta_join<float, KS>(a, true, s)
+    RGLRU_DELTA(1);
+    RGLRU_DELTA(2);
+    RGLRU_DELTA(3);
+    RGLRU_DELTA(4);
+#undef RGLRU_DELTA
+  }
+  return fail(RGLRU_E_UNSUPPORTED, "gated_delta_bwd: key size %d", a.K);
 }
 
 int delta_launch_forward(const DeltaArgs& a, bool save, int dtype, hipStream_t s) {

@@ -20,7 +20,8 @@
 
 namespace rglru {
 
-template <typename IO, int KS, int WAVES, int STAGES>
+// LOCAL: what a segment adds to the gradient of the state, from nothing behind it; nothing else is written.
+template <typename IO, int KS, int WAVES, int STAGES, bool LOCAL>
 __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void delta_backward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
@@ -34,9 +35,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = (p.columns + COLUMNS - 1) / COLUMNS, total = groups * p.B * p.HV;
-  const int work = xcd_order(blockIdx.x, total);
+  const int work = xcd_order(blockIdx.x, total * p.segments);
   if (work < 0) return;
-  const int group = work % groups, head = work / groups, hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
+  const int group = work % groups, segment = work / groups % p.segments, head = work / groups / p.segments;
+  const int hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
+  if (LOCAL && segment == 0) return;                        // nothing ends in front of the first segment
   const int col = group * COLUMNS + wave * 16 + c;
   const bool mine = group * COLUMNS + wave * 16 < p.columns, live = mine && col < p.V;
   const long long first = (long long)head * p.nC;
@@ -66,8 +69,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       ColumnIo<IO>(at, stride, p.T - t0, p.V, col, live, 8 * g).store(y);
     }
   };
-  const int last = p.nC - 1;
+  const int begin = segment * p.length, last = (begin + p.length < p.nC ? begin + p.length : p.nC) - 1;
   request(last, 0);
+  if (LOCAL) {
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) dstate[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  } else if (p.segments > 1) {
+    const float* at = p.edges + (((long long)head * p.segments + segment) * p.columns + (mine ? col : 0)) * DK;
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) dstate[t] = *reinterpret_cast<const f32x4*>(at + tile_index(t, 4 * g));
+  } else {
 #pragma unroll
   for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
@@ -75,8 +86,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       const int row = tile_index(t, 4 * g + e);
       dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
     }
+  }
   wait_for_all();
-  for (int n = last; n >= 0; --n) {
+  for (int n = last; n >= begin; --n) {
     const int stage = STAGES == 2 ? (last - n) & 1 : 0;
     unsigned char* tile = lds + stage * Tiles::kBytes;
     const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
@@ -87,13 +99,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       Tiles::clear_rows(tile, counts, tid);
       lds_barrier();
     }
-    if (STAGES == 2 && n != last) put(n + 1);
-    if (mine) {
+    if (STAGES == 2 && !LOCAL && n != last) put(n + 1);
+    if (mine && !LOCAL) {
       IO* at = (IO*)p.dstates + ((first + n) * PL * p.columns + col) * DK;
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), (long long)p.columns * DK, dstate[t]);
     }
-    if (STAGES == 2 && n > 0) request(n - 1, stage ^ 1);
+    if (STAGES == 2 && n > begin) request(n - 1, stage ^ 1);
     if (mine) {
       Frag ka[2][4], kt[2][2 * KS], uf[2];
       Wide ta[2][4];
@@ -163,18 +175,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       phase();
       M::ew(dstate, kt[0], M::wide(-rho[0] * y[0], -rho[1] * y[1]));
       M::ew(dstate, kt[1], M::wide(-rho[2] * y[2], -rho[3] * y[3]));
-      if (vectors) rows_out.turn(up_tile, y, wave, lane);
+      if (vectors && !LOCAL) rows_out.turn(up_tile, y, wave, lane);
       phase();
     }
     if (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
-      if (n > 0) request(n - 1, 0);
-      put(n);
+      if (n > begin) request(n - 1, 0);
+      if (!LOCAL) put(n);
     }
     wait_for_all();
   }
-  if (STAGES == 2) put(0);
-  if (p.dh0 && live) {
+  if (STAGES == 2 && !LOCAL) put(begin);
+  if (LOCAL) {
+    if (mine) {
+      float* at = p.local + (((long long)head * p.segments + segment) * p.columns + col) * DK;
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t) *reinterpret_cast<f32x4*>(at + tile_index(t, 4 * g)) = dstate[t];
+    }
+  } else if (p.dh0 && live && begin == 0) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
@@ -450,15 +468,26 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
   }
 }
 
+int delta_launch_join(const DeltaArgs& a, int dtype, hipStream_t s);
+
+template <typename IO, int KS, int WAVES, int STAGES, bool LOCAL> static int delta_walk_back(const DeltaArgs& a, hipStream_t s) {
+  const long long total = (long long)((a.columns + 16 * WAVES - 1) / (16 * WAVES)) * a.segments * a.B * a.HV;
+  hipLaunchKernelGGL((delta_backward_kernel<IO, KS, WAVES, STAGES, LOCAL>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WAVES), 0, s, a);
+  return check_launch("gated_delta_bwd");
+}
+
 template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hipStream_t s) {
+  constexpr bool kTwo = sizeof(IO) == 2;                    // two chunks' tiles fit the LDS
   const char* w = getenv("DELTA_WAVES");
-  const int kind = sizeof(IO) == 4 ? 4 : w ? atoi(w) : 2, waves = kind == 2 ? 2 : 4, total = (a.columns + 16 * waves - 1) / (16 * waves) * a.B * a.HV;
-  const dim3 walk((unsigned)((total + 7) / 8 * 8)), block(64 * waves);
-  if constexpr (sizeof(IO) == 4) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 1>), walk, block, 0, s, a);
-  else if (kind == 2) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 2, 2>), walk, block, 0, s, a);
-  else if (kind == 4) hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 1>), walk, block, 0, s, a);
-  else hipLaunchKernelGGL((delta_backward_kernel<IO, KS, 4, 2>), walk, block, 0, s, a);
-  int rc = check_launch("gated_delta_bwd");
+  const int waves = w ? atoi(w) : 2;
+  int rc = RGLRU_OK;
+  if (a.segments > 1) {
+    rc = delta_walk_back<IO, KS, 4, kTwo ? 2 : 1, true>(a, s);
+    if (!rc) rc = delta_launch_join(a, kTwo ? RGLRU_BF16 : RGLRU_F32, s);
+    if (rc) return rc;
+  }
+  if (kTwo && waves == 2) rc = delta_walk_back<IO, KS, 2, kTwo ? 2 : 1, false>(a, s);
+  else rc = delta_walk_back<IO, KS, 4, kTwo ? 2 : 1, false>(a, s);
   if (rc) return rc;
   const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));
   if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kGradThreads), 0, s, a);

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
+#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
@@ -125,10 +126,20 @@ template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bo
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
+// Segments of `length` chunks that a sequence is walked in side by side.
+static void delta_segments(int64_t heads, int64_t columns, int64_t nC, int64_t width, int64_t& segments, int64_t& length) {
+  const char* e = getenv("DELTA_SEGMENTS");
+  segments = e ? atoi(e) : 1;
+  if (segments > nC) segments = nC;
+  length = (nC + segments - 1) / segments;
+  segments = (nC + length - 1) / length;
+}
+
 struct DeltaSizes {
   int64_t chunks, columns, width, row, value_row;          // rows: elements of a key and of a value as the kernels read them
   size_t gates, solve, within, q, k, v, states, values, total;  // offsets in the workspace; q, k, v: room where rows have to be padded
-  size_t padded_v;
+  size_t padded_v, through, local, edges, segment_states;
+  int64_t segments, length;
   DeltaSizes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, bool keep) {
     const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
     row = (K + e - 1) / e * e, value_row = (V + e - 1) / e * e;
@@ -147,11 +158,17 @@ struct DeltaSizes {
     padded_v = value_row != V ? up((size_t)(B * T * HV * value_row) * (16 / e)) : 0;
     states = v + padded_v;
     values = states + (keep ? up((size_t)chunks * columns * width * 4) : 0);
-    total = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
+    through = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
+    delta_segments(B * HV, columns, (T + kDeltaChunk - 1) / kDeltaChunk, width, segments, length);
+    segment_states = segments > 1 ? up((size_t)(B * HV * segments * columns * width) * 4) : 0;
+    local = through + (segments > 1 ? up((size_t)(B * HV * segments * width * width) * 4) : 0);
+    edges = local + segment_states;
+    total = edges + segment_states;
   }
   size_t scratch_values() const { return ((size_t)chunks * columns * width * 4 + 255) & ~(size_t)255; }
   size_t scratch_up() const { return scratch_values() + (((size_t)chunks * columns * 64 * 4 + 255) & ~(size_t)255); }
-  size_t scratch() const { return scratch_up() + padded_v; }
+  size_t scratch_local() const { return scratch_up() + padded_v; }
+  size_t scratch() const { return scratch_local() + 2 * segment_states; }
 };
 
 static int delta_check(const char* who, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int decay_dtype, int beta_dtype) {
@@ -191,8 +208,9 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   whole = reinterpret_cast<uintptr_t>(v) % 16 == 0;
   for (int i = 6; i < 9; ++i) whole = whole && st[i] % e == 0;
   if (v && z.value_row == V && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of values must be 16-byte aligned", who);
-  a.segments = 1, a.length = a.nC;
+  a.segments = (int)z.segments, a.length = (int)z.length;
   char* base = (char*)ws;
+  a.through = base + z.through, a.local = (float*)(base + z.local), a.edges = (float*)(base + z.edges);
   a.gates = (float*)(base + z.gates);
   a.solve = base + z.solve, a.within = base + z.within;
   if (keep) a.states = base + z.states, a.values = base + z.values;
@@ -271,6 +289,7 @@ int rglru_hip_gated_delta_bwd(const void* q, const void* k, const int64_t* strid
   a.dq = dq, a.dk = dk, a.dv = dv, a.dlog_decay = dlog_decay, a.dbeta = dbeta, a.dh0 = dh0;
   a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
   a.dstates = scratch, a.dvalues = (char*)scratch + z.scratch_values();
+  a.local = (float*)((char*)scratch + z.scratch_local()), a.edges = (float*)((char*)scratch + z.scratch_local() + z.segment_states);
   if (a.value_width != a.V) {
     void* up = (char*)scratch + z.scratch_up();
     rc = delta_launch_pad(dout, up, a.B, a.T, a.HV, a.V, a.value_width, T * HV * V, HV * V, V, dtype, (hipStream_t)stream);
