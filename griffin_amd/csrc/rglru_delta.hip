@@ -231,31 +231,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
     }
     if (STAGES == 2 && n + 1 < end) request(n + 1, stage ^ 1);
     if (mine) {
-      Frag ka[2][4], qa[2][4], kt[2][2 * KS];
-      Wide ta[2][4];
-      auto rows = [&](const IO* x, int ks, Frag (&a)[4]) {
+      // operands of the next phase are requested in front of a phase's products, or at its start where another workgroup's
+      // products fill the wait and the registers are for two
+      constexpr int D = STAGES == 2 ? 2 : 1;
+      Frag ka[D][4], qa[D][4], kt[D][2 * KS];
+      Wide ta[D][4];
+      auto rows = [&](int ks) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) a[mt] = Keys::along_row(x, tile_index(mt, c), 32 * ks, g);
+        for (int mt = 0; mt < 4; ++mt) {
+          ka[ks % D][mt] = Keys::along_row(keys, tile_index(mt, c), 32 * ks, g);
+          if constexpr (OUT) qa[ks % D][mt] = Keys::along_row(queries, tile_index(mt, c), 32 * ks, g);
+        }
       };
-      auto square = [&](const IO* x, int ks, Wide (&a)[4]) {             // lower triangular: rows in front of the columns are zeros
+      auto square = [&](const IO* x, int ks) {             // lower triangular: rows in front of the columns are zeros
 #pragma unroll
-        for (int mt = 2 * ks; mt < 4; ++mt) a[mt] = Square::wide_down_rows_tile(x, 4096, 32 * ks, mt, lane);
+        for (int mt = 2 * ks; mt < 4; ++mt) ta[ks % D][mt] = Square::wide_down_rows_tile(x, 4096, 32 * ks, mt, lane);
       };
-      auto turned = [&](int ks, Frag (&a)[2 * KS]) {
+      auto turned = [&](int ks) {
 #pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) a[t] = Keys::down_rows_tile(keys, 32 * ks, t, lane);
+        for (int t = 0; t < 2 * KS; ++t) kt[ks % D][t] = Keys::down_rows_tile(keys, 32 * ks, t, lane);
       };
       phase();
-      rows(keys, 0, ka[0]);
-      if constexpr (OUT) rows(queries, 0, qa[0]);
+      if (D == 2) rows(0);
       f32x4 rho[4], r[4];
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g), r[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g);
       IO* const value_tile = (IO*)(tile + Tiles::kValues);
-      if (OUT || !unit) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) M::apart(Values::down_rows(value_tile, 32 * ks, 16 * wave, lane), r[2 * ks], r[2 * ks + 1]);
-      }
       const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
       // K S and Q S (o) side by side: a tile of the state becomes an operand once
       f32x4 acc[4] = {};
@@ -263,19 +264,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       for (int mt = 0; mt < 4; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks + 1 < KS) {
-          rows(keys, ks + 1, ka[(ks + 1) & 1]);
-          if constexpr (OUT) rows(queries, ks + 1, qa[(ks + 1) & 1]);
-        } else {
-          square(solve, 0, ta[0]);
-        }
+        if (D == 1) rows(ks);
+        else if (ks + 1 < KS) rows(ks + 1);
+        else square(solve, 0);
         phase();
         const Wide s = M::wide(state[2 * ks], state[2 * ks + 1]);
-        M::ew(acc, ka[ks & 1], s);
-        if constexpr (OUT) M::ew(o, qa[ks & 1], s);
+        M::ew(acc, ka[ks % D], s);
+        if constexpr (OUT) M::ew(o, qa[ks % D], s);
         phase();
       }
-      square(solve, 1, ta[1]);
+      square(solve, D - 1);
+      if (OUT || !unit) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) M::apart(Values::down_rows(value_tile, 32 * ks, 16 * wave, lane), r[2 * ks], r[2 * ks + 1]);
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) r[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
       phase();
       // where nothing is carried into a document, nothing of it is read either, whatever it is
       if (carry == 0.f) {
@@ -294,12 +299,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       }
       M::template ww<0, 4>(z, ta[0], M::wide(r[0], r[1]));
       phase();
-      turned(0, kt[0]);
+      if (D == 2) turned(0);
+      else square(solve, 1);
       phase();
-      M::template ww<2, 4>(z, ta[1], M::wide(r[2], r[3]));
+      M::template ww<2, 4>(z, ta[1 % D], M::wide(r[2], r[3]));
       phase();
-      turned(1, kt[1]);
-      if constexpr (OUT) square(within, 0, ta[0]);
+      turned(D - 1);
+      if (OUT && D == 2) square(within, 0);
       phase();
       // S' = rho_63 S + K^T (w Z)
       if (carry == 0.f) {
@@ -311,13 +317,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       }
       M::ew(state, kt[0], M::wide(z[0] * tile_rows(record + 64, 0, g), z[1] * tile_rows(record + 64, 1, g)));
       phase();
-      if constexpr (OUT) square(within, 1, ta[1]);
+      if (D == 1) turned(1);
+      else if (OUT) square(within, 1);
       phase();
-      M::ew(state, kt[1], M::wide(z[2] * tile_rows(record + 64, 2, g), z[3] * tile_rows(record + 64, 3, g)));
+      M::ew(state, kt[1 % D], M::wide(z[2] * tile_rows(record + 64, 2, g), z[3] * tile_rows(record + 64, 3, g)));
       if constexpr (OUT) {
         phase();
+        if (D == 1) square(within, 0);
         M::template ww<0, 4>(o, ta[0], M::wide(z[0], z[1]));
-        M::template ww<2, 4>(o, ta[1], M::wide(z[2], z[3]));
+        if (D == 1) phase(), square(within, 1);
+        M::template ww<2, 4>(o, ta[1 % D], M::wide(z[2], z[3]));
         if (vectors) rows_out.turn(value_tile, o, wave, lane);
       }
       phase();
@@ -373,8 +382,14 @@ template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDelt
   auto request = [&](int s, int stage) {
     load.request(delta_rsrc((const IO*)p.through + ((long long)head * p.segments + s) * (PL * DK * DK), Load::kBytes), lds0 + (unsigned)(stage * Load::kBytes), wave);
   };
-  f32x4 state[2 * KS];
+  f32x4 state[2 * KS], next[2 * KS];
+  auto added = [&](int s) {
+    const float* at = p.local + (((long long)head * p.segments + s) * p.columns + (mine ? col : 0)) * DK;
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) next[t] = *reinterpret_cast<const f32x4*>(at + tile_index(t, 4 * g));
+  };
   request(from, 0);
+  added(from);
 #pragma unroll
   for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
@@ -383,18 +398,18 @@ template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDelt
       state[t][e] = first && live && row < p.K ? first[((long long)head * p.K + row) * p.V + col] : 0.f;
     }
   for (int s = from;; s += step) {
-    const long long at = (((long long)head * p.segments + s) * p.columns + (mine ? col : 0)) * DK;
     if (mine) {
+      float* at = p.edges + (((long long)head * p.segments + s) * p.columns + col) * DK;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) *reinterpret_cast<f32x4*>(p.edges + at + tile_index(t, 4 * g)) = state[t];
+      for (int t = 0; t < 2 * KS; ++t) *reinterpret_cast<f32x4*>(at + tile_index(t, 4 * g)) = state[t];
     }
     if (s == to) break;
     const int stage = (s - from) & 1;
-    f32x4 next[2 * KS];
-#pragma unroll
-    for (int t = 0; t < 2 * KS; ++t) next[t] = *reinterpret_cast<const f32x4*>(p.local + at + tile_index(t, 4 * g));
+    f32x4 sum[2 * KS];
     wait_for_all();
-    if (s + step != to) request(s + step, stage ^ 1);
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) sum[t] = next[t];
+    if (s + step != to) request(s + step, stage ^ 1), added(s + step);
     const IO* through = (const IO*)(lds + stage * Load::kBytes);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -403,13 +418,12 @@ template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDelt
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t)
         a[t] = BACKWARD ? Square::wide_along_row(through, DK * DK, tile_index(t, c), 32 * ks, g) : Square::wide_down_rows_tile(through, DK * DK, 32 * ks, t, lane);
-      M::template ww<0, 2 * KS>(next, a, x);
+      M::template ww<0, 2 * KS>(sum, a, x);
       phase();
     }
 #pragma unroll
-    for (int t = 0; t < 2 * KS; ++t) state[t] = next[t];
+    for (int t = 0; t < 2 * KS; ++t) state[t] = sum[t];
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // a request that nothing was read of
 }
 template <typename IO, int KS> int delta_join(const DeltaArgs& a, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)((a.columns + 63) / 64 * a.B * a.HV));
