@@ -10,7 +10,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
-#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
@@ -43,13 +42,18 @@ template <int J> RGLRU_DEVICE void delta_solve_column(const float* low, const fl
   }
 }
 
-// T, P and the gate record of one chunk and value head.
+// T, P and the gate record of one chunk and value head.  A wave owns 16 rows of both; its operands come straight from memory (a row's
+// 64 bytes a quarter of the wave), so that four workgroups and more share a compute unit: what one of them does is short, and one
+// after the other.
 template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void delta_prepare_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
-  constexpr int DK = 32 * KS;
-  typedef Tile<IO, DK> Keys;
-  __shared__ __attribute__((aligned(16))) IO keys[kDeltaChunk * DK], queries[kDeltaChunk * DK];
-  __shared__ __attribute__((aligned(16))) float low[64 * kLowStride], inv[64 * kInvStride];
+  typedef typename M::Frag Frag;
+  typedef Tile<IO, 64> Square;
+  constexpr int PL = M::kPlanes;
+  // A, and T in its place once it has been read; P
+  __shared__ __attribute__((aligned(16))) unsigned char area[64 * kLowStride * 4], squares[16384];
+  __shared__ __attribute__((aligned(16))) float inv[64 * kInvStride];
+  float* const low = (float*)area;
   __shared__ double total[64];
   __shared__ float beta[64];
   __shared__ int segment[64];
@@ -57,51 +61,69 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long chunk = blockIdx.x;
   const int n = (int)(chunk % p.nC), head = (int)(chunk / p.nC), hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
-  const int t0 = n * kDeltaChunk;
+  const int t0 = n * kDeltaChunk, left = p.T - t0;
+  const IO *keys = (const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, *queries = (const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h;
+  auto rows = [&](const IO* base, long long stride, int row, Frag (&f)[KS]) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      i32x4 v[sizeof(IO) / 2] = {};
+      const int col = 32 * ks + 8 * g;
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(IO) / 2; ++i)
+        if (row < left && col + i * 4 < p.width) v[i] = *reinterpret_cast<const i32x4*>(base + row * stride + col + i * 4);
+      __builtin_memcpy(&f[ks], v, sizeof(Frag));
+    }
+  };
+  auto mask = [&](Frag (&f)[KS], bool counts) {              // whatever a masked token holds
+    if (!counts) __builtin_memset(&f, 0, sizeof(f));
+  };
+  Frag ki[KS], qi[KS], kj[KS];
+  rows(keys, p.k_t, 16 * wave + c, ki);
+  rows(queries, p.q_t, 16 * wave + c, qi);
   const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
   const unsigned long long counts = __ballot(gate.counts);
-  {
-    KeyRows<IO, DK, kDeltaThreads> k, q;
-    k.request((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, p.k_t, p.width, counts, tid);
-    q.request((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, p.q_t, p.width, counts, tid);
-    if (wave == 0) {
-      total[lane] = gate.total;
-      beta[lane] = gate.beta;
-      segment[lane] = gate.segment;
-      float* record = p.gates + chunk * kDeltaGates;
-      record[lane] = gate.segment == 0 ? expf((float)gate.total) : 0.f;
-      record[64 + lane] = gate.segment == gate.segments ? gate.beta * expf((float)(gate.end - gate.total)) : 0.f;
-      if (lane < 2) record[128 + lane] = __uint_as_float((unsigned)(counts >> (32 * lane)));
-    }
-    k.put(keys, tid);
-    q.put(queries, tid);
+  if (wave == 0) {
+    total[lane] = gate.total;
+    beta[lane] = gate.beta;
+    segment[lane] = gate.segment;
+    float* record = p.gates + chunk * kDeltaGates;
+    record[lane] = gate.segment == 0 ? expf((float)gate.total) : 0.f;
+    record[64 + lane] = gate.segment == gate.segments ? gate.beta * expf((float)(gate.end - gate.total)) : 0.f;
+    if (lane < 2) record[128 + lane] = __uint_as_float((unsigned)(counts >> (32 * lane)));
   }
+  mask(ki, (counts >> (16 * wave + c)) & 1);
+  mask(qi, (counts >> (16 * wave + c)) & 1);
   __syncthreads();
   const int i0 = 16 * wave + 4 * g;                        // first of the lane's four rows
-  IO* within = (IO*)p.within + chunk * (4096 * M::kPlanes);
+  double total_i[4];
+  int segment_i[4];
 #pragma unroll
+  for (int e = 0; e < 4; ++e) total_i[e] = total[i0 + e], segment_i[e] = segment[i0 + e];
   for (int jt = 0; jt < 4; ++jt) {
     const int j = 16 * jt + c;
     f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
     if (jt <= wave) {
+      rows(keys, p.k_t, j, kj);
+      mask(kj, (counts >> j) & 1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const auto at_j = Keys::along_row(keys, j, 32 * ks, g);
-        kk = M::ee(Keys::along_row(keys, 16 * wave + c, 32 * ks, g), at_j, kk);
-        qk = M::ee(Keys::along_row(queries, 16 * wave + c, 32 * ks, g), at_j, qk);
+        kk = M::ee(ki[ks], kj[ks], kk);
+        qk = M::ee(qi[ks], kj[ks], qk);
       }
+      const double total_j = total[j];
+      const float beta_j = beta[j];
+      const int segment_j = segment[j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = i0 + e;
-        const bool joined = i >= j && segment[i] == segment[j];
-        const float d = joined ? beta[j] * expf((float)(total[i] - total[j])) : 0.f;
+        const bool joined = i >= j && segment_i[e] == segment_j;
+        const float d = joined ? beta_j * expf((float)(total_i[e] - total_j)) : 0.f;
         kk[e] = joined && i > j ? d * kk[e] : 0.f;
         qk[e] = joined ? p.scale * d * qk[e] : 0.f;
+        low[i * kLowStride + j] = kk[e];
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) low[(i0 + e) * kLowStride + j] = kk[e];
     }
-    M::put(within + j * 64 + i0, 4096, qk);
+    M::put((IO*)squares + Square::at(j, i0), 4096, qk);
   }
   wave_lds_fence();
   // inverse of the wave's diagonal block by substitution, a column a lane (the four quarters do the same)
@@ -111,7 +133,12 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
     for (int i = 0; i < 16; ++i) {
       float s = i == c ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) s = fmaf(-low[(16 * wave + i) * kLowStride + 16 * wave + j], x[j], s);
+      for (int j0 = 0; j0 < i; j0 += 4) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(low + (16 * wave + i) * kLowStride + 16 * wave + j0);
+#pragma unroll
+        for (int j = j0; j < j0 + 4; ++j)
+          if (j < i) s = fmaf(-a[j - j0], x[j], s);
+      }
       x[i] = s;
     }
     if (lane < 16) {
@@ -125,9 +152,18 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   else if (wave == 1) delta_solve_column<1>(low, inv, lane, column);
   else if (wave == 2) delta_solve_column<2>(low, inv, lane, column);
   else delta_solve_column<3>(low, inv, lane, column);
-  IO* solve = (IO*)p.solve + chunk * (4096 * M::kPlanes);
+  __syncthreads();
 #pragma unroll
-  for (int it = 0; it < 4; ++it) M::put(solve + (16 * wave + c) * 64 + 16 * it + 4 * g, 4096, column[it]);
+  for (int it = 0; it < 4; ++it) M::put((IO*)area + Square::at(16 * wave + c, 16 * it + 4 * g), 4096, column[it]);
+  __syncthreads();
+  // whole rows at a time
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = tid + i * kDeltaThreads, row = at / Square::U, u = at % Square::U;
+    const long long to = chunk * (4096 * PL) + row * 64 + u * Square::E;
+    *reinterpret_cast<i32x4*>((IO*)p.solve + to) = *reinterpret_cast<const i32x4*>((const IO*)area + Square::unit(row, u));
+    *reinterpret_cast<i32x4*>((IO*)p.within + to) = *reinterpret_cast<const i32x4*>((const IO*)squares + Square::unit(row, u));
+  }
 }
 
 // The walk along a segment's chunks.  SAVE: what the backward pass needs is left behind.  !OUT: what the segment does to the state, without
@@ -445,17 +481,12 @@ template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool
   int rc = check_launch("gated_delta_fwd prepare");
   if (rc) return rc;
   constexpr bool kTwo = sizeof(IO) == 2;                    // two chunks' tiles fit the LDS
-  const char* w = getenv("DELTA_WAVES");
-  const int waves = w ? atoi(w) : 2;
   if (a.segments > 1) {
-    const char* l = getenv("DELTA_LOCAL");
-    if (l && atoi(l) == 2) rc = delta_walk<IO, KS, 4, kTwo ? 2 : 1, false, false>(a, s);
-    else rc = delta_walk<IO, KS, 4, 1, false, false>(a, s);
+    rc = delta_walk<IO, KS, 4, 1, false, false>(a, s);
     if (!rc) rc = delta_join<IO, KS>(a, false, s);
     if (rc) return rc;
   }
-  if (kTwo && waves == 2) return save ? delta_walk<IO, KS, 2, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 2, kTwo ? 2 : 1, false, true>(a, s);
-  if (kTwo && waves == 4) return save ? delta_walk<IO, KS, 4, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 4, kTwo ? 2 : 1, false, true>(a, s);
+  if (delta_narrow(a, kTwo)) return save ? delta_walk<IO, KS, 2, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 2, kTwo ? 2 : 1, false, true>(a, s);
   return save ? delta_walk<IO, KS, 4, 1, true, true>(a, s) : delta_walk<IO, KS, 4, 1, false, true>(a, s);
 }
 

@@ -13,7 +13,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
-#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
@@ -107,26 +106,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
     }
     if (STAGES == 2 && n > begin) request(n - 1, stage ^ 1);
     if (mine) {
-      Frag ka[2][4], kt[2][2 * KS], uf[2];
-      Wide ta[2][4];
-      auto rows = [&](int ks, Frag (&a)[4]) {
+      // operands of the next phase are requested in front of a phase's products, or at its start (as in the forward walk)
+      constexpr int D = STAGES == 2 ? 2 : 1;
+      Frag ka[D][4], kt[D][2 * KS], uf[2];
+      Wide ta[D][4];
+      auto rows = [&](int ks) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) a[mt] = Keys::along_row(keys, tile_index(mt, c), 32 * ks, g);
+        for (int mt = 0; mt < 4; ++mt) ka[ks % D][mt] = Keys::along_row(keys, tile_index(mt, c), 32 * ks, g);
       };
-      auto square = [&](const IO* x, int ks, Wide (&a)[4]) {             // upper triangular: rows behind the columns are zeros
+      auto square = [&](const IO* x, int ks) {             // upper triangular: rows behind the columns are zeros
 #pragma unroll
-        for (int mt = 0; mt < 2 * ks + 2; ++mt) a[mt] = Square::wide_along_row(x, 4096, tile_index(mt, c), 32 * ks, g);
+        for (int mt = 0; mt < 2 * ks + 2; ++mt) ta[ks % D][mt] = Square::wide_along_row(x, 4096, tile_index(mt, c), 32 * ks, g);
       };
-      auto turned = [&](const IO* x, int ks, Frag (&a)[2 * KS]) {
+      auto turned = [&](const IO* x, int ks) {
 #pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) a[t] = Keys::down_rows_tile(x, 32 * ks, t, lane);
+        for (int t = 0; t < 2 * KS; ++t) kt[ks % D][t] = Keys::down_rows_tile(x, 32 * ks, t, lane);
       };
       phase();
-      rows(0, ka[0]);
+      if (D == 2) rows(0);
       f32x4 rho[4], up[4];
       IO* const up_tile = (IO*)(tile + Tiles::kValues);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) uf[ks] = Values::down_rows(up_tile, 32 * ks, 16 * wave, lane);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g);
       const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
@@ -134,28 +133,33 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       f32x4 dz[4] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks + 1 < KS) rows(ks + 1, ka[(ks + 1) & 1]);
-        else square(within, 0, ta[0]);
+        if (D == 1) rows(ks);
+        else if (ks + 1 < KS) rows(ks + 1);
+        else square(within, 0);
         phase();
-        M::ew(dz, ka[ks & 1], M::wide(dstate[2 * ks], dstate[2 * ks + 1]));
+        M::ew(dz, ka[ks % D], M::wide(dstate[2 * ks], dstate[2 * ks + 1]));
         phase();
       }
-      square(within, 1, ta[1]);
-      M::apart(uf[0], up[0], up[1]);
-      M::apart(uf[1], up[2], up[3]);
+      square(within, D - 1);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        uf[ks] = Values::down_rows(up_tile, 32 * ks, 16 * wave, lane);
+        M::apart(uf[ks], up[2 * ks], up[2 * ks + 1]);
+      }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) dz[mt] *= tile_rows(record + 64, mt, g), up[mt] *= rho[mt] * p.scale;
       phase();
       M::template we<0, 2>(dz, ta[0], uf[0]);
       phase();
-      square(solve, 0, ta[0]);
-      turned(queries, 0, kt[0]);
+      if (D == 2) square(solve, 0), turned(queries, 0);
+      else square(within, 1);
       phase();
-      M::template we<0, 4>(dz, ta[1], uf[1]);
+      M::template we<0, 4>(dz, ta[1 % D], uf[1]);
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) dstate[t] *= carry;
       phase();
-      square(solve, 1, ta[1]);
+      if (D == 2) square(solve, 1);
+      else square(solve, 0), turned(queries, 0);
       phase();
       // dS = rho_63 dS' + Q^T (scale rho dO) - K^T (rho Y),  Y = T^T dZ
       M::ew(dstate, kt[0], M::wide(up[0], up[1]));
@@ -163,18 +167,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
       M::template ww<0, 2>(y, ta[0], M::wide(dz[0], dz[1]));
       phase();
-      turned(queries, 1, kt[1]);
+      if (D == 1) square(solve, 1);
+      turned(queries, 1);
       phase();
-      M::template ww<0, 4>(y, ta[1], M::wide(dz[2], dz[3]));
+      M::template ww<0, 4>(y, ta[1 % D], M::wide(dz[2], dz[3]));
       phase();
-      turned(keys, 0, kt[0]);
+      if (D == 2) turned(keys, 0);
       phase();
-      M::ew(dstate, kt[1], M::wide(up[2], up[3]));
+      M::ew(dstate, kt[1 % D], M::wide(up[2], up[3]));
       phase();
-      turned(keys, 1, kt[1]);
+      turned(keys, D - 1);
       phase();
       M::ew(dstate, kt[0], M::wide(-rho[0] * y[0], -rho[1] * y[1]));
-      M::ew(dstate, kt[1], M::wide(-rho[2] * y[2], -rho[3] * y[3]));
+      if (D == 1) phase(), turned(keys, 1);
+      M::ew(dstate, kt[1 % D], M::wide(-rho[2] * y[2], -rho[3] * y[3]));
       if (vectors && !LOCAL) rows_out.turn(up_tile, y, wave, lane);
       phase();
     }
@@ -478,16 +484,13 @@ template <typename IO, int KS, int WAVES, int STAGES, bool LOCAL> static int del
 
 template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hipStream_t s) {
   constexpr bool kTwo = sizeof(IO) == 2;                    // two chunks' tiles fit the LDS
-  const char* w = getenv("DELTA_WAVES");
-  const int waves = w ? atoi(w) : 2;
   int rc = RGLRU_OK;
   if (a.segments > 1) {
-    rc = delta_walk_back<IO, KS, 4, kTwo ? 2 : 1, true>(a, s);
+    rc = delta_walk_back<IO, KS, 4, 1, true>(a, s);
     if (!rc) rc = delta_launch_join(a, kTwo ? RGLRU_BF16 : RGLRU_F32, s);
     if (rc) return rc;
   }
-  if (kTwo && waves == 2) rc = delta_walk_back<IO, KS, 2, kTwo ? 2 : 1, false>(a, s);
-  else rc = delta_walk_back<IO, KS, 4, kTwo ? 2 : 1, false>(a, s);
+  rc = delta_narrow(a, kTwo) ? delta_walk_back<IO, KS, 2, kTwo ? 2 : 1, false>(a, s) : delta_walk_back<IO, KS, 4, 1, false>(a, s);
   if (rc) return rc;
   const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));
   if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kGradThreads), 0, s, a);

@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
-#include <cstdlib>
 
 #include "rglru_delta.h"
 #include "rglru_host.h"
@@ -126,11 +125,35 @@ template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bo
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-// Segments of `length` chunks that a sequence is walked in side by side.
-static void delta_segments(int64_t heads, int64_t columns, int64_t nC, int64_t width, int64_t& segments, int64_t& length) {
-  const char* e = getenv("DELTA_SEGMENTS");
-  segments = e ? atoi(e) : 1;
-  if (segments > nC) segments = nC;
+// Segments of `length` chunks that a sequence is walked in side by side.  One walk takes as long as its chunks, however many compute units
+// stand idle; in segments, all of them are walked twice (what a segment adds to the state and what it makes of it, 128 further
+// columns; then the outputs from the joined states).  The number is the one with the least time by what launches of both kinds measure, us a
+// chunk of a round of workgroups (bf16, keys and values of 128; it is their ratios that decide, also for other sizes).
+static int64_t delta_best_segments(int64_t heads, int64_t columns, int64_t width, int64_t nC, bool two, bool keep) {
+  const int64_t cus = num_compute_units(), groups = (columns + 63) / 64, units = (width + 63) / 64;
+  auto rounds = [&](int64_t n, double alone, double shared) {  // one workgroup a compute unit, or two that share it
+    if (n <= cus) return alone;
+    return two ? (double)((n + 2 * cus - 1) / (2 * cus)) * shared : (double)((n + cus - 1) / cus) * alone;
+  };
+  int64_t best = 1;
+  double least = 0.;
+  for (int64_t s = 1; s <= nC && s <= 64; ++s) {
+    const int64_t length = (nC + s - 1) / s;
+    if (s > 1 && (nC + length - 1) / length != s) continue;
+    double us = rounds(heads * groups * s, keep ? 6.5 : 4.8, keep ? 12. : 7.);
+    if (s == 1 && two && heads * ((columns + 31) / 32) <= cus) us = keep ? 5. : 4.;
+    if (keep) us *= 2.;                                      // the backward walk takes about as long
+    if (s > 1) {
+      us += rounds(heads * (groups * (s - 1) + units * (keep ? s : s - 1)), 3.2, 4.3);
+      if (keep) us += rounds(heads * groups * (s - 1), 3.8, 5.5);
+    }
+    us = us * (double)length + (s > 1 ? 4. * (double)s * (keep ? 2. : 1.) + 5. : 0.);
+    if (s == 1 || us < 0.9 * least || (best > 1 && us < least)) best = s, least = us;
+  }
+  return best;
+}
+static void delta_segments(int64_t heads, int64_t columns, int64_t nC, int64_t width, int dtype, bool keep, int64_t& segments, int64_t& length) {
+  segments = delta_best_segments(heads, columns, width, nC, dtype == RGLRU_BF16, keep);
   length = (nC + segments - 1) / segments;
   segments = (nC + length - 1) / length;
 }
@@ -159,7 +182,7 @@ struct DeltaSizes {
     states = v + padded_v;
     values = states + (keep ? up((size_t)chunks * columns * width * 4) : 0);
     through = values + (keep ? up((size_t)chunks * columns * 64 * 4) : 0);
-    delta_segments(B * HV, columns, (T + kDeltaChunk - 1) / kDeltaChunk, width, segments, length);
+    delta_segments(B * HV, columns, (T + kDeltaChunk - 1) / kDeltaChunk, width, dtype, keep, segments, length);
     segment_states = segments > 1 ? up((size_t)(B * HV * segments * columns * width) * 4) : 0;
     local = through + (segments > 1 ? up((size_t)(B * HV * segments * width * width) * 4) : 0);
     edges = local + segment_states;

@@ -175,6 +175,20 @@ def test_slow_decay_over_many_chunks(dtype):
     check(make(1, 700, 1, 1, 64, 64, dtype=dtype, slow=True))
 
 
+@pytest.mark.parametrize("shape", [(1, 1500, 1, 2, 64, 48), (2, 1100, 1, 1, 128, 20), (1, 1290, 1, 1, 20, 100)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_long_sequences_of_few_heads(shape, dtype):
+    """Walked in segments side by side, which are joined; slow decay carries the state across them."""
+    check(make(*shape, dtype=dtype, slow=True))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_long_packed_sequences_of_few_heads(dtype):
+    reset, active = masks(2, 1300, seed=3)
+    active[0, 600:700] = False
+    check(make(2, 1300, 1, 2, 64, 32, dtype=dtype, slow=True), reset, active)
+
+
 def test_gates_in_another_type_than_the_activations():
     case = make(2, 100, 1, 2, 64, 64, dtype=BF16)
     case["log_decay"], case["beta"] = case["log_decay"].float(), case["beta"].float()
