@@ -141,17 +141,22 @@ template <> struct Mx<float> {
 // The index that row m of accumulator tile t stands for (see above).
 RGLRU_DEVICE int tile_index(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
 
-// A row-major [rows][COLS] tile in LDS.  Its 16-byte units are exchanged within a row by a pattern of the row, so that what eight lanes read
-// at a time (one unit of eight rows, of 0 .. 7 or of 0 .. 3 and 8 .. 11) lies in all 32 banks.
+// A row-major [rows][COLS] tile in LDS.  Its 16-byte units are exchanged within a row by a pattern of the row.  LDS has 64 banks of
+// 4 bytes; a read of 16 bytes a lane takes 4 cycles where the lanes that are served together lie in all of them.  Which lanes
+// those are was found by timing all patterns that are linear in a row's lowest four bits: these are the simplest of those that every
+// read below is at full rate with (4.6 .. 5.4 cycles a read with four waves reading, 8.1 .. 16 with the units as they come).
 template <typename IO, int COLS> struct Tile {
   typedef Mx<IO> M;
   typedef typename M::Frag Frag;
   typedef typename M::Wide Wide;
   static constexpr int E = 16 / (int)sizeof(IO), U = COLS / E;
-  static_assert(U % 4 == 0, "units are exchanged in fours or eights");
+  static_assert(U % (COLS * (int)sizeof(IO) % 256 == 0 ? 16 : COLS * (int)sizeof(IO) % 128 == 0 ? 8 : 4) == 0, "units are exchanged in fours, eights or sixteens");
   static RGLRU_DEVICE int pattern(int row) {
-    const int odd = ((row >> 2) ^ (row >> 3)) & 1;
-    return COLS * (int)sizeof(IO) % 128 == 0 ? (row & 3) << 1 | odd : (row & 2) | odd;   // rows of 64 (mod 128) bytes alternate by themselves
+    constexpr int bytes = COLS * (int)sizeof(IO), low = sizeof(IO) == 2 ? 1 : 0;
+    const int r0 = row & 1, r1 = row >> 1 & 1, r3 = row >> 3 & 1;
+    if constexpr (bytes % 256 == 0) return r0 << low | r3 << 2 | r1 << 3;
+    else if constexpr (bytes % 128 == 0) return sizeof(IO) == 2 ? r1 << 1 | r3 << 2 : r3 | r1 << 2;
+    else return r3 << low;
   }
   static RGLRU_DEVICE int unit(int row, int u) { return row * COLS + (u ^ pattern(row)) * E; }
   static RGLRU_DEVICE int at(int row, int col) { return unit(row, col / E) + col % E; }
@@ -263,52 +268,6 @@ RGLRU_DEVICE ChunkGates chunk_gates(const DeltaArgs& p, int b, int hv, int n, in
   r.end = __shfl(sum, 63, 64);
   return r;
 }
-
-// Rows of keys, queries or upstream gradients of a chunk as an LDS tile, zeros where a token does not count or the tile is wider than
-// the row.  The vectors are requested into registers and put down later.
-template <typename IO, int COLS, int THREADS> struct KeyRows {
-  typedef Tile<IO, COLS> T;
-  static constexpr int N = kDeltaChunk * T::U / THREADS;   // vectors a thread
-  i32x4 v[N];
-  RGLRU_DEVICE void request(const IO* rows, long long stride, int width, unsigned long long counts, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS, row = at / T::U, col = at % T::U * T::E;
-      v[i] = i32x4{0, 0, 0, 0};
-      if (((counts >> row) & 1) && col < width) v[i] = *reinterpret_cast<const i32x4*>(rows + (long long)row * stride + col);
-    }
-  }
-  RGLRU_DEVICE void put(IO* tile, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS;
-      *reinterpret_cast<i32x4*>(tile + T::unit(at / T::U, at % T::U)) = v[i];
-    }
-  }
-};
-
-// Planes of an fp32 matrix [ROWS][COLS] in memory as LDS tiles, one behind the other.
-template <typename IO, int ROWS, int COLS, int THREADS> struct MatrixRows {
-  typedef Tile<IO, COLS> T;
-  static constexpr int kUnits = Mx<IO>::kPlanes * ROWS * T::U, N = (kUnits + THREADS - 1) / THREADS;
-  static_assert(kUnits % THREADS == 0, "whole vectors a thread");
-  i32x4 v[N];
-  // `src`: first plane's first row to take; `plane`: elements from plane to plane; `rows`: rows that are there
-  RGLRU_DEVICE void request(const IO* src, long long plane, int rows, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS, which = at / (ROWS * T::U), row = at / T::U % ROWS, u = at % T::U;
-      v[i] = row < rows ? *reinterpret_cast<const i32x4*>(src + which * plane + (long long)row * COLS + u * T::E) : i32x4{0, 0, 0, 0};
-    }
-  }
-  RGLRU_DEVICE void put(IO* tile, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + i * THREADS, which = at / (ROWS * T::U), row = at / T::U % ROWS, u = at % T::U;
-      *reinterpret_cast<i32x4*>(tile + which * ROWS * COLS + T::unit(row, u)) = v[i];
-    }
-  }
-};
 
 RGLRU_DEVICE i32x4 delta_rsrc(const void* base, unsigned bytes) {
   const unsigned long long at = (unsigned long long)base;
