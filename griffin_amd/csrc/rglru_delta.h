@@ -103,6 +103,11 @@ template <> struct Mx<__bf16> {
     *reinterpret_cast<bf16x4*>(at) = hi;
     *reinterpret_cast<bf16x4*>(at + plane) = lo;
   }
+  // the eight consecutive elements that an operand holds; `at` and `plane` in bytes
+  static RGLRU_DEVICE void put(rsrc_t r, unsigned at, unsigned plane, const Wide& w) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, w.hi), r, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, w.lo), r, at, plane, 0);
+  }
 };
 
 template <> struct Mx<float> {
@@ -136,6 +141,10 @@ template <> struct Mx<float> {
   static RGLRU_DEVICE Frag exact(f32x4 a, f32x4 b) { return {a, b}; }
   static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) { a = f.lo, b = f.hi; }
   static RGLRU_DEVICE void put(float* at, long long, f32x4 v) { *reinterpret_cast<f32x4*>(at) = v; }
+  static RGLRU_DEVICE void put(rsrc_t r, unsigned at, unsigned, const Wide& w) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, w.lo), r, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, w.hi), r, at + 16, 0, 0);
+  }
 };
 
 // The index that row m of accumulator tile t stands for (see above).
@@ -368,33 +377,38 @@ template <typename IO, int KS, int WAVES, bool OUT> struct ChunkTiles {
   SquareLoad square;
   ValueLoad value;
   unsigned record;
+  const IO *keys, *queries, *values, *solve, *within;      // of the chunk that is requested next
+  const float* gates;
   long long value_stride;
-  int value_width;
-  RGLRU_DEVICE void setup(const DeltaArgs& p, int tid, long long stride, int width) {
+  int value_width, left, step;
+  // From chunk n of a sequence on (`chunk` of all), forwards or backwards; first_values: the sequence's first row at the group's first column
+  RGLRU_DEVICE void setup(const DeltaArgs& p, int tid, const IO* first_values, long long stride, int width, long long chunk, int n, int b, int h, int step_) {
     k.setup(tid, p.k_t, p.width);
     if constexpr (OUT) q.setup(tid, p.q_t, p.width);
     square.setup(tid, 64, 64);
     value_stride = stride, value_width = width < COLUMNS ? width : COLUMNS;
     value.setup(tid, stride, width);
     record = (tid & 63) * 16 < kDeltaGates * 4 ? (unsigned)(tid & 63) * 16u : kOutOfRange;
+    const long long t0 = (long long)n * kDeltaChunk;
+    keys = (const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h;
+    queries = (const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h;
+    values = first_values + t0 * stride;
+    solve = (const IO*)p.solve + chunk * (4096 * PL);
+    within = (const IO*)p.within + chunk * (4096 * PL);
+    gates = p.gates + chunk * kDeltaGates;
+    left = p.T - (int)t0, step = step_;
   }
-  // `values`: the chunk's first row, at the group's first column
-  RGLRU_DEVICE void request(const DeltaArgs& p, long long chunk, int n, int b, int h, const IO* values, unsigned lds, int wave) const {
-    const int t0 = n * kDeltaChunk, left = p.T - t0;
-    const i32x4 rk = delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left));
-    const i32x4 rs = delta_rsrc((const IO*)p.solve + chunk * (4096 * PL), SquareLoad::kBytes);
-    const i32x4 rq = delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, OUT ? KeyLoad::extent(p.q_t, p.width, left) : 0u);
-    const i32x4 rw = delta_rsrc((const IO*)p.within + chunk * (4096 * PL), SquareLoad::kBytes);
-    const i32x4 rv = delta_rsrc(values, ValueLoad::extent(value_stride, value_width, left));
-    const i32x4 rr = delta_rsrc(p.gates + chunk * kDeltaGates, kDeltaGates * 4);
-    k.request(rk, lds + kKeys, wave);
-    square.request(rs, lds + kSolve, wave);
-    if (value_width > 0) value.request(rv, lds + kValues, wave);
+  RGLRU_DEVICE void request(const DeltaArgs& p, unsigned lds, int wave) {
+    k.request(delta_rsrc(keys, KeyLoad::extent(p.k_t, p.width, left)), lds + kKeys, wave);
+    square.request(delta_rsrc(solve, SquareLoad::kBytes), lds + kSolve, wave);
+    if (value_width > 0) value.request(delta_rsrc(values, ValueLoad::extent(value_stride, value_width, left)), lds + kValues, wave);
     if constexpr (OUT) {
-      q.request(rq, lds + kQueries, wave);
-      square.request(rw, lds + kWithin, wave);
+      q.request(delta_rsrc(queries, KeyLoad::extent(p.q_t, p.width, left)), lds + kQueries, wave);
+      square.request(delta_rsrc(within, SquareLoad::kBytes), lds + kWithin, wave);
     }
-    if (wave == 0) memory_to_lds(rr, record, lds + kRecord);
+    if (wave == 0) memory_to_lds(delta_rsrc(gates, kDeltaGates * 4), record, lds + kRecord);
+    keys += step * kDeltaChunk * p.k_t, queries += step * kDeltaChunk * p.q_t, values += step * kDeltaChunk * value_stride;
+    solve += step * 4096 * PL, within += step * 4096 * PL, gates += step * kDeltaGates, left -= step * kDeltaChunk;
   }
   // zeros for the rows of tokens that do not count
   template <typename LOAD> static RGLRU_DEVICE void clear(unsigned char* tile, unsigned long long counts, int tid) {

@@ -172,7 +172,7 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
 // next one's requests (behind them, the wait for the requests would be one for the stores).  STAGES 1: two workgroups share a
 // compute unit, one computes while the other waits.
 template <typename IO, int KS, int WAVES, int STAGES, bool SAVE, bool OUT>
-__global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void delta_forward_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof(IO) <= 8 ? 2 : 1) void delta_forward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
@@ -199,20 +199,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
   const unsigned lds0 = lds_address(lds);
 
   Tiles tiles;
-  tiles.setup(p, tid, p.v_t, unit ? 0 : p.value_width - group * COLUMNS);
-  const IO* const values = (const IO*)p.v + b * p.v_b + hv * p.v_h + group * COLUMNS;
+  tiles.setup(p, tid, (const IO*)p.v + b * p.v_b + hv * p.v_h + group * COLUMNS, p.v_t, unit ? 0 : p.value_width - group * COLUMNS, first + begin,
+              begin, b, h, 1);
   const bool vectors = p.value_width == p.V;
   f32x4 state[2 * KS], o[4], z[4];
+  Wide zw[2];
   WaveRows<IO, COLUMNS> rows_out;
-  auto request = [&](int n, int stage) {
-    tiles.request(p, first + n, n, b, h, values + (long long)n * kDeltaChunk * p.v_t, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
+  auto request = [&](int stage) { tiles.request(p, lds0 + (unsigned)(stage * Tiles::kBytes), wave); };
+  // a chunk's matrix of `rows` elements a column, by eight of a column a lane
+  const unsigned plane_bytes = (unsigned)p.columns * (unsigned)sizeof(IO);
+  auto matrix = [&](void* base, int n, int rows) {
+    return make_rsrc((IO*)base + (first + n) * PL * p.columns * rows, PL * plane_bytes * (unsigned)rows);
   };
   auto put = [&](int n) {                                  // results of chunk n
     if constexpr (SAVE) {
       if (mine) {
-        IO* at = (IO*)p.values + ((first + n) * PL * p.columns + col) * 64;
+        const rsrc_t r = matrix(p.values, n, 64);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) M::put(at + tile_index(mt, 4 * g), (long long)p.columns * 64, z[mt]);
+        for (int ks = 0; ks < 2; ++ks) M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, zw[ks]);
       }
     }
     if constexpr (OUT) {
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       }
     }
   };
-  request(begin, 0);
+  request(0);
   if (!OUT) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t)
@@ -258,14 +262,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       lds_barrier();
     }
     if (STAGES == 2 && n > begin) put(n - 1);
-    if constexpr (SAVE) {
-      if (mine) {
-        IO* at = (IO*)p.states + ((first + n) * PL * p.columns + col) * DK;
-#pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), (long long)p.columns * DK, state[t]);
-      }
-    }
-    if (STAGES == 2 && n + 1 < end) request(n + 1, stage ^ 1);
+    if (STAGES == 2 && n + 1 < end) request(stage ^ 1);
     if (mine) {
       // operands of the next phase are requested in front of a phase's products, or at its start where another workgroup's
       // products fill the wait and the registers are for two
@@ -298,6 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       f32x4 acc[4] = {};
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const rsrc_t saved = matrix(p.states, n, SAVE ? DK : 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if (D == 1) rows(ks);
@@ -307,6 +305,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
         const Wide s = M::wide(state[2 * ks], state[2 * ks + 1]);
         M::ew(acc, ka[ks % D], s);
         if constexpr (OUT) M::ew(o, qa[ks % D], s);
+        if constexpr (SAVE) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, s);
         phase();
       }
       square(solve, D - 1);
@@ -360,16 +359,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       if constexpr (OUT) {
         phase();
         if (D == 1) square(within, 0);
-        M::template ww<0, 4>(o, ta[0], M::wide(z[0], z[1]));
+        zw[0] = M::wide(z[0], z[1]), zw[1] = M::wide(z[2], z[3]);
+        M::template ww<0, 4>(o, ta[0], zw[0]);
         if (D == 1) phase(), square(within, 1);
-        M::template ww<2, 4>(o, ta[1 % D], M::wide(z[2], z[3]));
+        M::template ww<2, 4>(o, ta[1 % D], zw[1]);
         if (vectors) rows_out.turn(value_tile, o, wave, lane);
       }
       phase();
     }
     if constexpr (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
-      if (n + 1 < end) request(n + 1, 0);
+      if (n + 1 < end) request(0);
       put(n);
     }
     wait_for_all();

@@ -21,7 +21,7 @@ namespace rglru {
 
 // LOCAL: what a segment adds to the gradient of the state, from nothing behind it; nothing else is written.
 template <typename IO, int KS, int WAVES, int STAGES, bool LOCAL>
-__global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void delta_backward_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof(IO) <= 8 ? 2 : 1) void delta_backward_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
@@ -44,20 +44,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
   const long long first = (long long)head * p.nC;
   const unsigned lds0 = lds_address(lds);
 
+  const int begin = segment * p.length, last = (begin + p.length < p.nC ? begin + p.length : p.nC) - 1;
   Tiles tiles;
-  tiles.setup(p, tid, p.up_t, p.value_width - group * COLUMNS);
-  const IO* const ups = (const IO*)p.dout + b * p.up_b + hv * p.up_h + group * COLUMNS;
+  tiles.setup(p, tid, (const IO*)p.dout + b * p.up_b + hv * p.up_h + group * COLUMNS, p.up_t, p.value_width - group * COLUMNS, first + last, last, b, h, -1);
   const bool vectors = p.value_width == p.V;
   f32x4 dstate[2 * KS], y[4];
   WaveRows<IO, COLUMNS> rows_out;
-  auto request = [&](int n, int stage) {
-    tiles.request(p, first + n, n, b, h, ups + (long long)n * kDeltaChunk * p.up_t, lds0 + (unsigned)(stage * Tiles::kBytes), wave);
+  auto request = [&](int stage) { tiles.request(p, lds0 + (unsigned)(stage * Tiles::kBytes), wave); };
+  // a chunk's matrix of `rows` elements a column, by eight of a column a lane
+  const unsigned plane_bytes = (unsigned)p.columns * (unsigned)sizeof(IO);
+  auto matrix = [&](void* base, int n, int rows) {
+    return make_rsrc((IO*)base + (first + n) * PL * p.columns * rows, PL * plane_bytes * (unsigned)rows);
   };
   auto put = [&](int n) {                                  // results of chunk n
     if (mine) {
-      IO* at = (IO*)p.dvalues + ((first + n) * PL * p.columns + col) * 64;
+      const rsrc_t r = matrix(p.dvalues, n, 64);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) M::put(at + tile_index(mt, 4 * g), (long long)p.columns * 64, y[mt]);
+      for (int ks = 0; ks < 2; ++ks)
+        M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, M::wide(y[2 * ks], y[2 * ks + 1]));
     }
     const int t0 = n * kDeltaChunk;
     const long long stride = (long long)p.HV * p.V;
@@ -68,8 +72,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       ColumnIo<IO>(at, stride, p.T - t0, p.V, col, live, 8 * g).store(y);
     }
   };
-  const int begin = segment * p.length, last = (begin + p.length < p.nC ? begin + p.length : p.nC) - 1;
-  request(last, 0);
+  request(0);
   if (LOCAL) {
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t) dstate[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -99,12 +102,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       lds_barrier();
     }
     if (STAGES == 2 && !LOCAL && n != last) put(n + 1);
-    if (mine && !LOCAL) {
-      IO* at = (IO*)p.dstates + ((first + n) * PL * p.columns + col) * DK;
-#pragma unroll
-      for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), (long long)p.columns * DK, dstate[t]);
-    }
-    if (STAGES == 2 && n > begin) request(n - 1, stage ^ 1);
+    if (STAGES == 2 && n > begin) request(stage ^ 1);
     if (mine) {
       // operands of the next phase are requested in front of a phase's products, or at its start (as in the forward walk)
       constexpr int D = STAGES == 2 ? 2 : 1;
@@ -131,13 +129,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
       const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
       // dZ = P^T dO + w K dS'
       f32x4 dz[4] = {};
+      const rsrc_t saved = matrix(p.dstates, n, LOCAL ? 0 : DK);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if (D == 1) rows(ks);
         else if (ks + 1 < KS) rows(ks + 1);
         else square(within, 0);
         phase();
-        M::ew(dz, ka[ks % D], M::wide(dstate[2 * ks], dstate[2 * ks + 1]));
+        const Wide d = M::wide(dstate[2 * ks], dstate[2 * ks + 1]);
+        M::ew(dz, ka[ks % D], d);
+        if constexpr (!LOCAL) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, d);
         phase();
       }
       square(within, D - 1);
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES * (3 - STAGES) >= 8 ? 2 : 1) void
     }
     if (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
-      if (n > begin) request(n - 1, 0);
+      if (n > begin) request(0);
       if (!LOCAL) put(n);
     }
     wait_for_all();
