@@ -195,6 +195,21 @@ template <typename IO, int COLS> struct Tile {
   // the same for accumulator tile t of what comes out, and for sixteen columns in their order
   static RGLRU_DEVICE Frag down_rows_tile(const IO* x, int k0, int t, int lane) { return down_rows(x, k0, 32 * (t >> 1) + 4 * (t & 1), 8, lane); }
   static RGLRU_DEVICE Frag down_rows(const IO* x, int k0, int col0, int lane) { return down_rows(x, k0, col0, 4, lane); }
+  // the elements that an accumulator tile's lanes hold: rows row0 + 4 g .. + 3 of column col0 + c
+  static RGLRU_DEVICE f32x4 accumulator_tile(const IO* t, int row0, int col0, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    f32x4 v;
+    if constexpr (sizeof(IO) == 2) {
+      typedef __attribute__((address_space(3))) bf16x4_lds* lds_ptr_t;
+      const bf16x4_lds x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr_t)(t + at(row0 + 4 * g + (c >> 2), col0 + 4 * (c & 3))));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (float)x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = t[at(row0 + 4 * g + e, col0 + c)];
+    }
+    return v;
+  }
   // an fp32 matrix, whose second plane lies `plane` elements behind the first
   static RGLRU_DEVICE Wide wide_along_row(const IO* t, int plane, int row, int k0, int g) {
     if constexpr (sizeof(IO) == 2) return {along_row(t, row, k0, g), along_row(t + plane, row, k0, g)};

@@ -210,10 +210,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
   }
 }
 
-// Sum over the sixteen columns of an accumulator row.
+// Sum over the sixteen columns of an accumulator row: the lanes of a row of sixteen turn by 8, 4, 2 and 1.
 RGLRU_DEVICE float sixteen_sum(float v) {
-#pragma unroll
-  for (int m = 8; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x124, 0xf, 0xf, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x122, 0xf, 0xf, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x121, 0xf, 0xf, true));
   return v;
 }
 
@@ -221,7 +223,9 @@ RGLRU_DEVICE float sixteen_sum(float v) {
 // columns; the first half's waves make N1, the second half's N2.  The contractions over the value columns take 32 of them at a time
 // through LDS, the next 32 on their way there where two fit; N1 and N2 go through LDS once, where the columns lay.
 constexpr int kGradThreads = 512;
-template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradThreads, 2) void delta_grads_kernel(DeltaArgs p) {
+template <typename IO, bool GROUPED> constexpr bool kGradShared = (sizeof(IO) == 2) && !GROUPED;
+template <typename IO, int KS, bool GROUPED>
+__global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) void delta_grads_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
   typedef typename M::Frag Frag;
@@ -234,16 +238,16 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
   typedef TileLoad<IO, CB, 64, THREADS> ValueLoad;          // one plane
   typedef TileLoad<IO, CB, DK, THREADS> StateLoad;
   constexpr int kUp = 0, kValues = kUp + UpLoad::kBytes, kDValues = kValues + PL * ValueLoad::kBytes, kStates = kDValues + PL * ValueLoad::kBytes,
-                kDStates = kStates + PL * StateLoad::kBytes, kStage = kDStates + PL * StateLoad::kBytes, kPairs = 2 * PL * 4096 * (int)sizeof(IO);
-  constexpr int STAGES = 2 * kStage + 2 * KeyLoad::kBytes + 4096 <= 160 * 1024 ? 2 : 1;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * KeyLoad::kBytes + (STAGES * kStage > kPairs ? STAGES * kStage : kPairs)];
+                kDStates = kStates + PL * StateLoad::kBytes, kStage = kDStates + PL * StateLoad::kBytes, kRows = 2 * KeyLoad::kBytes + 2 * PL * 4096 * (int)sizeof(IO);
+  constexpr int STAGES = 2 * kStage + 4096 <= (kGradShared<IO, GROUPED> ? 80 : 160) * 1024 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * kStage > kRows ? STAGES * kStage : kRows];
   __shared__ double total[64];
   __shared__ float beta[64], to_end[64], reads[2][64], writes[2][64], leaves[2][64], sums[8];
   __shared__ int segment[64];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
   const int n = (int)(blockIdx.x % (unsigned)p.nC), bh = (int)(blockIdx.x / (unsigned)p.nC), h = bh % p.H, b = bh / p.H;
-  const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H, row0 = 16 * block + 4 * g;
+  const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H;
   IO *const keys = (IO*)lds, *const queries = (IO*)(lds + KeyLoad::kBytes), *const area = (IO*)(lds + 2 * KeyLoad::kBytes);
   const unsigned lds0 = lds_address(lds);
   f32x4 all_dq[KS] = {}, all_dk[KS] = {};                   // over the value heads that share the key head
@@ -254,12 +258,16 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
   value_load.setup(tid, 64, 64);
   state_load.setup(tid, DK, DK);
 
-  for (int s = 0; s < share; ++s) {
+  for (int s = 0; s < (GROUPED ? share : 1); ++s) {
+    // no address that hangs on the lane is kept from head to head: there are more of them than registers
+    int lane = tid & 63;
+    if (GROUPED) asm("" : "+v"(lane) : "s"(s));
+    const int c = lane & 15, g = lane >> 4, row0 = 16 * block + 4 * g;
     const int hv = h * share + s, head = b * p.HV + hv;
     const long long chunk = (long long)head * p.nC + n;
     auto request = [&](int c0, int stage) {
       const int there = p.columns - c0;                     // columns of the values from here on
-      const unsigned to = lds0 + 2 * KeyLoad::kBytes + (unsigned)(stage * kStage);
+      const unsigned to = lds0 + (unsigned)(stage * kStage);
       const int width = p.value_width - c0;
       up_load.request(delta_rsrc((const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h + c0, width < CB ? UpLoad::extent(p.up_t, width, left) : UpLoad::extent(p.up_t, CB, left)),
                       to + kUp, wave);
@@ -273,13 +281,6 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
       }
     };
     if (s > 0) __syncthreads();                             // the head before is through with the shared arrays
-    if (s == 0) {
-      KeyLoad k;
-      k.setup(tid, p.k_t, p.width);
-      k.request(delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left)), lds0, wave);
-      k.setup(tid, p.q_t, p.width);
-      k.request(delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, KeyLoad::extent(p.q_t, p.width, left)), lds0 + KeyLoad::kBytes, wave);
-    }
     request(0, 0);
     const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
     const unsigned long long counts = __ballot(gate.counts);
@@ -295,16 +296,10 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
     wait_for_all();
     for (int c0 = 0; c0 < p.columns; c0 += CB) {
       const int stage = STAGES == 2 ? (c0 / CB) & 1 : 0;
-      unsigned char* tile = lds + 2 * KeyLoad::kBytes + stage * kStage;
+      unsigned char* tile = lds + stage * kStage;
       if (counts != ~0ull) {                               // zeros for the rows of tokens that do not count
         for (int at = tid; at < 64 * Ups::U; at += THREADS)
           if (!((counts >> (at / Ups::U)) & 1)) *reinterpret_cast<i32x4*>(tile + kUp + at * 16) = i32x4{0, 0, 0, 0};
-        if (s == 0 && c0 == 0)
-          for (int at = tid; at < 64 * Keys::U; at += THREADS)
-            if (!((counts >> (at / Keys::U)) & 1)) {
-              *reinterpret_cast<i32x4*>((unsigned char*)keys + at * 16) = i32x4{0, 0, 0, 0};
-              *reinterpret_cast<i32x4*>((unsigned char*)queries + at * 16) = i32x4{0, 0, 0, 0};
-            }
         lds_barrier();
       }
       if (STAGES == 2 && c0 + CB < p.columns) request(c0 + CB, stage ^ 1);
@@ -318,6 +313,7 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
         if (jt <= block) {
           const Wide zj = Square::wide_down_rows(values, CB * 64, 0, 16 * jt, lane);
           pairs[jt] = half == 0 ? M::ew(uf, zj, pairs[jt]) : M::ww(yf, zj, pairs[jt]);
+          phase();
         }
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
@@ -344,28 +340,29 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
         lds_barrier();                                     // the columns have been read
         request(c0 + CB, 0);
       }
-      wait_for_all();
+      if (c0 + CB < p.columns) wait_for_all();
+    }
+    lds_barrier();
+    {
+      KeyLoad k;
+      k.setup(tid, p.k_t, p.width);
+      k.request(delta_rsrc((const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, KeyLoad::extent(p.k_t, p.width, left)), lds0, wave);
+      k.setup(tid, p.q_t, p.width);
+      k.request(delta_rsrc((const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h, KeyLoad::extent(p.q_t, p.width, left)), lds0 + KeyLoad::kBytes, wave);
     }
     // the factors of what reads the carried state and of what is left for the next chunk; the decays of the pairs
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = row0 + e;
       const float rho = segment[i] == 0 ? expf((float)total[i]) : 0.f, end = to_end[i];
-      float dot = 0.f;
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        dq[t][e] *= p.scale * rho;
-        dr[t][e] *= -rho;
-        dw[t][e] *= end;
-        dot = fmaf(dw[t][e], (float)keys[Keys::at(i, 16 * (half * KS + t) + c)], dot);
-      }
-      dot = sixteen_sum(dot);
-      if (c == 0) leaves[half][i] = beta[i] * dot;
+      for (int t = 0; t < KS; ++t) dq[t][e] *= p.scale * rho, dr[t][e] *= -rho, dw[t][e] *= end;
+      phase();
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt) {
         const int j = 16 * jt + c;
         const bool joined = i >= j + half && segment[i] == segment[j];   // N2: strictly in front
-        const float d = joined ? expf((float)(total[i] - total[j])) : 0.f;
+        const float d = expf(joined ? (float)(total[i] - total[j]) : 0.f);
         pairs[jt][e] = joined ? (half == 0 ? p.scale * d : -d) * pairs[jt][e] : 0.f;
       }
     }
@@ -378,7 +375,25 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
         if (jt <= (block | 1)) M::put(area + half * PL * 4096 + Square::at(16 * jt + c, row0), 4096, pairs[jt] * (strengths ? beta[16 * jt + c] : 1.f));
     };
     put_pairs(false);
-    __syncthreads();
+    wait_for_all();
+    if (counts != ~0ull) {
+      for (int at = tid; at < 64 * Keys::U; at += THREADS)
+        if (!((counts >> (at / Keys::U)) & 1)) {
+          *reinterpret_cast<i32x4*>((unsigned char*)keys + at * 16) = i32x4{0, 0, 0, 0};
+          *reinterpret_cast<i32x4*>((unsigned char*)queries + at * 16) = i32x4{0, 0, 0, 0};
+        }
+      lds_barrier();
+    }
+    {
+      f32x4 dot = {};
+#pragma unroll
+      for (int t = 0; t < KS; ++t) dot += dw[t] * Keys::accumulator_tile(keys, 16 * block, 16 * (half * KS + t), lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float sum = sixteen_sum(dot[e]);
+        if (c == 0) leaves[half][row0 + e] = beta[row0 + e] * sum;
+      }
+    }
     // F = N1^T Q + N2^T K + ...: pairs in which the wave's tokens are the written ones
     for (int ks = block >> 1; ks < 2; ++ks) {
       const Wide a = Square::wide_along_row(area, 4096, 16 * block + c, 32 * ks, g);
@@ -387,6 +402,7 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
       for (int t = 0; t < KS; ++t) {
         dw[t] = M::we(a, Keys::down_rows(queries, 32 * ks, 16 * (half * KS + t), lane), dw[t]);
         dw[t] = M::we(a2, Keys::down_rows(keys, 32 * ks, 16 * (half * KS + t), lane), dw[t]);
+        phase();
       }
     }
     __syncthreads();
@@ -400,25 +416,25 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
         const Frag kf = Keys::down_rows(keys, 32 * ks, 16 * (half * KS + t), lane);
         dq[t] = M::we(a, kf, dq[t]);
         dr[t] = M::we(a2, kf, dr[t]);
+        phase();
       }
+    }
+    f32x4 read = {}, written = {}, strength;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) strength[e] = beta[row0 + e];
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      const f32x4 k = Keys::accumulator_tile(keys, 16 * block, 16 * (half * KS + t), lane);
+      read += Keys::accumulator_tile(queries, 16 * block, 16 * (half * KS + t), lane) * dq[t] + k * dr[t];
+      written += k * dw[t];
+      dr[t] += strength * dw[t];
+      all_dq[t] = GROUPED ? all_dq[t] + dq[t] : dq[t];
+      all_dk[t] = GROUPED ? all_dk[t] + dr[t] : dr[t];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = row0 + e;
-      float read = 0.f, written = 0.f;
-#pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        const int at = Keys::at(i, 16 * (half * KS + t) + c);
-        const float k = (float)keys[at], q = (float)queries[at];
-        read = fmaf(q, dq[t][e], fmaf(k, dr[t][e], read));
-        written = fmaf(k, dw[t][e], written);
-        dr[t][e] = fmaf(beta[i], dw[t][e], dr[t][e]);
-        all_dq[t][e] = GROUPED ? all_dq[t][e] + dq[t][e] : dq[t][e];
-        all_dk[t][e] = GROUPED ? all_dk[t][e] + dr[t][e] : dr[t][e];
-      }
-      read = sixteen_sum(read);
-      written = sixteen_sum(written);
-      if (c == 0) reads[half][i] = read, writes[half][i] = written;
+      const float from = sixteen_sum(read[e]), back = sixteen_sum(written[e]);
+      if (c == 0) reads[half][row0 + e] = from, writes[half][row0 + e] = back;
     }
     __syncthreads();
     if (wave == 0) {                                       // sums from each token to the chunk's end
@@ -443,6 +459,7 @@ template <typename IO, int KS, bool GROUPED> __global__ __launch_bounds__(kGradT
       }
     }
   }
+  const int c = tid & 15, g = (tid & 63) >> 4, row0 = 16 * block + 4 * g;
   const long long stride = (long long)p.H * p.K, base = ((long long)b * p.T + t0) * stride + (long long)h * p.K;
   if (p.width == p.K) {                                     // through the tiles of queries and keys, which all waves are through with
 #pragma unroll
