@@ -401,6 +401,9 @@ template <typename IO, int KS, int WAVES, bool OUT> struct ChunkTiles {
     k.setup(tid, p.k_t, p.width);
     if constexpr (OUT) q.setup(tid, p.q_t, p.width);
     square.setup(tid, 64, 64);
+#pragma unroll
+    for (int i = 0; i < SquareLoad::N; ++i)                 // the quarter above the diagonal is neither written nor used
+      if ((square.off[i] / (64 * (unsigned)sizeof(IO)) & 32) && (square.off[i] & (32 * (unsigned)sizeof(IO)))== 0) square.off[i] = kOutOfRange;
     value_stride = stride, value_width = width < COLUMNS ? width : COLUMNS;
     value.setup(tid, stride, width);
     record = (tid & 63) * 16 < kDeltaGates * 4 ? (unsigned)(tid & 63) * 16u : kOutOfRange;
@@ -484,5 +487,7 @@ RGLRU_DEVICE int xcd_order(int block, int total) {
   const int per = (total + 7) >> 3, at = (block & 7) * per + (block >> 3);
   return (block >> 3) < per && at < total ? at : -1;
 }
+
+inline dim3 xcd_grid(long long total) { return dim3((unsigned)((total + 7) / 8 * 8)); }
 
 }  // namespace rglru

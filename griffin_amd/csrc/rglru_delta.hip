@@ -43,15 +43,15 @@ template <int J> RGLRU_DEVICE void delta_solve_column(const float* low, const fl
 }
 
 // T, P and the gate record of one chunk and value head.  A wave owns 16 rows of both; its operands come straight from memory (a row's
-// 64 bytes a quarter of the wave), so that four workgroups and more share a compute unit: what one of them does is short, and one
-// after the other.
-template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void delta_prepare_kernel(DeltaArgs p) {
+// 64 bytes a quarter of the wave) and T and P take turns in LDS, so that five workgroups share a compute unit: what one of them does
+// is short, and one after the other.
+template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads, sizeof(IO) == 2 ? 5 : 3) void delta_prepare_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Frag Frag;
   typedef Tile<IO, 64> Square;
   constexpr int PL = M::kPlanes;
-  // A, and T in its place once it has been read; P
-  __shared__ __attribute__((aligned(16))) unsigned char area[64 * kLowStride * 4], squares[16384];
+  // A, T in its place once it has been read, P behind that
+  __shared__ __attribute__((aligned(16))) unsigned char area[64 * kLowStride * 4];
   __shared__ __attribute__((aligned(16))) float inv[64 * kInvStride];
   float* const low = (float*)area;
   __shared__ double total[64];
@@ -59,8 +59,11 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   __shared__ int segment[64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const long long chunk = blockIdx.x;
-  const int n = (int)(chunk % p.nC), head = (int)(chunk / p.nC), hv = head % p.HV, b = head / p.HV, h = hv / (p.HV / p.H);
+  // the heads of a chunk side by side: what they read lies side by side
+  const int work = xcd_order(blockIdx.x, p.nC * p.B * p.HV);
+  if (work < 0) return;
+  const int hv = work % p.HV, n = work / p.HV % p.nC, b = work / p.HV / p.nC, h = hv / (p.HV / p.H);
+  const long long chunk = ((long long)b * p.HV + hv) * p.nC + n;
   const int t0 = n * kDeltaChunk, left = p.T - t0;
   const IO *keys = (const IO*)p.k + b * p.k_b + t0 * p.k_t + h * p.k_h, *queries = (const IO*)p.q + b * p.q_b + t0 * p.q_t + h * p.q_h;
   auto rows = [&](const IO* base, long long stride, int row, Frag (&f)[KS]) {
@@ -99,10 +102,12 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   int segment_i[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) total_i[e] = total[i0 + e], segment_i[e] = segment[i0 + e];
+  f32x4 within[4] = {};
+#pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
     const int j = 16 * jt + c;
-    f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
     if (jt <= wave) {
+      f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
       rows(keys, p.k_t, j, kj);
       mask(kj, (counts >> j) & 1);
 #pragma unroll
@@ -119,11 +124,11 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
         const bool joined = i >= j && segment_i[e] == segment_j;
         const float d = beta_j * expf(joined ? (float)(total_i[e] - total_j) : 0.f);
         kk[e] = joined && i > j ? d * kk[e] : 0.f;
-        qk[e] = joined ? p.scale * d * qk[e] : 0.f;
+        within[jt][e] = joined ? p.scale * d * qk[e] : 0.f;
         low[i * kLowStride + j] = kk[e];
       }
     }
-    M::put((IO*)squares + Square::at(j, i0), 4096, qk);
+    phase();
   }
   wave_lds_fence();
   // inverse of the wave's diagonal block by substitution, a column a lane (the four quarters do the same)
@@ -152,18 +157,24 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads) void 
   else if (wave == 1) delta_solve_column<1>(low, inv, lane, column);
   else if (wave == 2) delta_solve_column<2>(low, inv, lane, column);
   else delta_solve_column<3>(low, inv, lane, column);
+  // whole rows at a time; the quarter above the diagonal is not read by anyone
+  auto rows_out = [&](IO* to) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = tid + i * kDeltaThreads, row = at / Square::U, u = at % Square::U;
+      if ((row & 32) && u < Square::U / 2) continue;
+      *reinterpret_cast<i32x4*>(to + chunk * (4096 * PL) + row * 64 + u * Square::E) = *reinterpret_cast<const i32x4*>((const IO*)area + Square::unit(row, u));
+    }
+    __syncthreads();
+  };
   __syncthreads();
 #pragma unroll
   for (int it = 0; it < 4; ++it) M::put((IO*)area + Square::at(16 * wave + c, 16 * it + 4 * g), 4096, column[it]);
-  __syncthreads();
-  // whole rows at a time
+  rows_out((IO*)p.solve);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = tid + i * kDeltaThreads, row = at / Square::U, u = at % Square::U;
-    const long long to = chunk * (4096 * PL) + row * 64 + u * Square::E;
-    *reinterpret_cast<i32x4*>((IO*)p.solve + to) = *reinterpret_cast<const i32x4*>((const IO*)area + Square::unit(row, u));
-    *reinterpret_cast<i32x4*>((IO*)p.within + to) = *reinterpret_cast<const i32x4*>((const IO*)squares + Square::unit(row, u));
-  }
+  for (int jt = 0; jt < 4; ++jt) M::put((IO*)area + Square::at(16 * jt + c, i0), 4096, within[jt]);
+  rows_out((IO*)p.within);
 }
 
 // The walk along a segment's chunks.  SAVE: what the backward pass needs is left behind.  !OUT: what the segment does to the state, without
@@ -471,13 +482,12 @@ template <typename IO, int KS> int delta_join(const DeltaArgs& a, bool backward,
 template <typename IO, int KS, int WAVES, int STAGES, bool SAVE, bool OUT> static int delta_walk(const DeltaArgs& a, hipStream_t s) {
   const int width = 16 * WAVES, groups = (a.columns + width - 1) / width + (OUT ? 0 : (32 * KS + width - 1) / width);
   const long long total = (long long)groups * a.segments * a.B * a.HV;
-  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(64 * WAVES);
-  hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, SAVE, OUT>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((delta_forward_kernel<IO, KS, WAVES, STAGES, SAVE, OUT>), xcd_grid(total), dim3(64 * WAVES), 0, s, a);
   return check_launch("gated_delta_fwd");
 }
 
 template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool save, hipStream_t s) {
-  hipLaunchKernelGGL((delta_prepare_kernel<IO, KS>), dim3((unsigned)((long long)a.B * a.HV * a.nC)), dim3(kDeltaThreads), 0, s, a);
+  hipLaunchKernelGGL((delta_prepare_kernel<IO, KS>), xcd_grid((long long)a.B * a.HV * a.nC), dim3(kDeltaThreads), 0, s, a);
   int rc = check_launch("gated_delta_fwd prepare");
   if (rc) return rc;
   constexpr bool kTwo = sizeof(IO) == 2;                    // two chunks' tiles fit the LDS

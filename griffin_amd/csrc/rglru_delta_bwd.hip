@@ -246,7 +246,10 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
   __shared__ int segment[64];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
-  const int n = (int)(blockIdx.x % (unsigned)p.nC), bh = (int)(blockIdx.x / (unsigned)p.nC), h = bh % p.H, b = bh / p.H;
+  // the heads of a chunk side by side: what they read and write lies side by side
+  const int work = xcd_order(blockIdx.x, p.nC * p.B * p.H);
+  if (work < 0) return;
+  const int h = work % p.H, n = work / p.H % p.nC, b = work / p.H / p.nC;
   const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H;
   IO *const keys = (IO*)lds, *const queries = (IO*)(lds + KeyLoad::kBytes), *const area = (IO*)(lds + 2 * KeyLoad::kBytes);
   const unsigned lds0 = lds_address(lds);
@@ -496,7 +499,7 @@ int delta_launch_join(const DeltaArgs& a, int dtype, hipStream_t s);
 
 template <typename IO, int KS, int WAVES, int STAGES, bool LOCAL> static int delta_walk_back(const DeltaArgs& a, hipStream_t s) {
   const long long total = (long long)((a.columns + 16 * WAVES - 1) / (16 * WAVES)) * a.segments * a.B * a.HV;
-  hipLaunchKernelGGL((delta_backward_kernel<IO, KS, WAVES, STAGES, LOCAL>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WAVES), 0, s, a);
+  hipLaunchKernelGGL((delta_backward_kernel<IO, KS, WAVES, STAGES, LOCAL>), xcd_grid(total), dim3(64 * WAVES), 0, s, a);
   return check_launch("gated_delta_bwd");
 }
 
@@ -510,7 +513,7 @@ template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hip
   }
   rc = delta_narrow(a, kTwo) ? delta_walk_back<IO, KS, 2, kTwo ? 2 : 1, false>(a, s) : delta_walk_back<IO, KS, 4, 1, false>(a, s);
   if (rc) return rc;
-  const dim3 grid((unsigned)((long long)a.B * a.H * a.nC));
+  const dim3 grid = xcd_grid((long long)a.B * a.H * a.nC);
   if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kGradThreads), 0, s, a);
   else hipLaunchKernelGGL((delta_grads_kernel<IO, KS, false>), grid, dim3(kGradThreads), 0, s, a);
   return check_launch("gated_delta_bwd gradients");
