@@ -122,7 +122,7 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads, sizeo
       for (int e = 0; e < 4; ++e) {
         const int i = i0 + e;
         const bool joined = i >= j && segment_i[e] == segment_j;
-        const float d = beta_j * expf(joined ? (float)(total_i[e] - total_j) : 0.f);
+        const float d = beta_j * __expf(joined ? (float)(total_i[e] - total_j) : 0.f);
         kk[e] = joined && i > j ? d * kk[e] : 0.f;
         within[jt][e] = joined ? p.scale * d * qk[e] : 0.f;
         low[i * kLowStride + j] = kk[e];

@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
       for (int jt = 0; jt < 4; ++jt) {
         const int j = 16 * jt + c;
         const bool joined = i >= j + half && segment[i] == segment[j];   // N2: strictly in front
-        const float d = expf(joined ? (float)(total[i] - total[j]) : 0.f);
+        const float d = __expf(joined ? (float)(total[i] - total[j]) : 0.f);
         pairs[jt][e] = joined ? (half == 0 ? p.scale * d : -d) * pairs[jt][e] : 0.f;
       }
     }
