@@ -50,16 +50,36 @@ template <typename IO, int V> struct Run {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = (float)r[e];
   }
-  static RGLRU_DEVICE void store(void* p, long long at, const float (&v)[V]) {
-    Raw r;
+  // Written through: whole 128-byte lines
+  static RGLRU_DEVICE void store(rsrc_t r, unsigned at, const float (&v)[V]) {
+    if constexpr (V > 1) {
+      Raw raw;
 #pragma unroll
-    for (int e = 0; e < V; ++e) r[e] = (IO)v[e];
-    *reinterpret_cast<Raw*>((IO*)p + at) = r;
+      for (int e = 0; e < V; ++e) raw[e] = (IO)v[e];
+      buf_store_b128<kWriteThrough>(__builtin_bit_cast(i32x4, raw), r, at * (unsigned)sizeof(IO));
+    } else {
+      BufIo<IO>::store((IO)v[0], r, at * (unsigned)sizeof(IO), 0);
+    }
   }
+  static RGLRU_DEVICE rsrc_t rows(void* p, long long at) { return make_rsrc((IO*)p + at, 0xfffffff0u); }
 };
 
-// V parameters from channel c on; `absent` without a tensor.
+// V parameters from channel c on (a multiple of V); `absent` without a tensor.
 template <int V> RGLRU_DEVICE void group_params(const void* p, int c, int dtype, float absent, float (&out)[V]) {
+  if (V > 1 && p != nullptr && ((unsigned long long)p & 15) == 0) {  // by vectors where the tensor lies on their boundaries
+    typedef __bf16 Half __attribute__((ext_vector_type(V)));
+    typedef float Full __attribute__((ext_vector_type(V)));
+    if (dtype == 1) {
+      const Half h = *reinterpret_cast<const Half*>((const __bf16*)p + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = (float)h[e];
+    } else {
+      const Full f = *reinterpret_cast<const Full*>((const float*)p + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = f[e];
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < V; ++e) out[e] = p == nullptr ? absent : dtype == 1 ? (float)((const __bf16*)p)[c + e] : ((const float*)p)[c + e];
 }
@@ -75,8 +95,17 @@ RGLRU_DEVICE float group_slope(float v, int activation) {
   return activation == RGLRU_ACT_GELU ? gelu_tanh_parts(v).dgelu : 1.f;
 }
 
+// Sum over runs of `lanes` lanes (a power of two).  Within sixteen lanes by data-parallel moves: once the lanes of a quad (of eight)
+// hold one number, mirroring eight (sixteen) lanes brings the other half's.
+template <int CONTROL> RGLRU_DEVICE float lane_move(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
 RGLRU_DEVICE float lanes_sum(float v, int lanes) {
-  for (int m = lanes >> 1; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  if (lanes >= 2) v += lane_move<0xb1>(v);                  // quad: 1 0 3 2
+  if (lanes >= 4) v += lane_move<0x4e>(v);                  // quad: 2 3 0 1
+  if (lanes >= 8) v += lane_move<0x141>(v);                 // eight lanes mirrored
+  if (lanes >= 16) v += lane_move<0x140>(v);                // sixteen lanes mirrored
+  for (int m = 16; m < lanes; m <<= 1) v += __shfl_xor(v, m, 64);
   return v;
 }
 
@@ -85,25 +114,20 @@ RGLRU_DEVICE float lanes_sum(float v, int lanes) {
 // G, so a lane keeps its channels, whose parameter gradients it adds up in registers.
 template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_bounds__(kGroupThreads) void group_norm_rows_kernel(GroupArgs p) {
   typedef Run<IO, V> R;
-  const int lane = threadIdx.x & 63, wave = blockIdx.x * (kGroupThreads / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kGroupThreads / 64) + (threadIdx.x >> 6));
   if (wave >= p.waves) return;
   const int runs = 64 / p.lanes, l = lane % p.lanes, first = wave * runs + lane / p.lanes;
+  const unsigned here = (unsigned)(lane / p.lanes * p.Cg);   // from the wave's first run on
   const long long round = (long long)p.waves * runs;
   const int c0 = first % p.G * p.Cg;
-  float w[SLOTS][V], b[SLOTS][V], dw[BACKWARD ? SLOTS : 1][V], db[BACKWARD ? SLOTS : 1][V];
   bool has[SLOTS];
 #pragma unroll
-  for (int s = 0; s < SLOTS; ++s) {
-    has[s] = l + p.lanes * s < p.width;
-    const int c = has[s] ? c0 + (l + p.lanes * s) * V : 0;
-    group_params<V>(p.weight, c, p.vec_dtype, 1.f, w[s]);
-    group_params<V>(p.bias, c, p.vec_dtype, 0.f, b[s]);
-    if constexpr (BACKWARD)
-#pragma unroll
-      for (int e = 0; e < V; ++e) dw[s][e] = db[s][e] = 0.f;
-  }
+  for (int s = 0; s < SLOTS; ++s) has[s] = l + p.lanes * s < p.width;
   typename R::Raw next[SLOTS], next_up[SLOTS];
+  float next_mean = 0.f, next_rstd = 0.f;
   auto request = [&](long long run) {
+    if constexpr (BACKWARD)
+      if (run < p.rows) next_mean = p.stats[2 * run], next_rstd = p.stats[2 * run + 1];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const bool ok = run < p.rows && has[s];
@@ -117,13 +141,25 @@ template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_boun
     }
   };
   request(first);
-  for (long long run = first; run - lane / p.lanes < p.rows; run += round) {
+  float w[SLOTS][V], b[SLOTS][V], dw[BACKWARD ? SLOTS : 1][V], db[BACKWARD ? SLOTS : 1][V];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    const int c = has[s] ? c0 + (l + p.lanes * s) * V : 0;
+    group_params<V>(p.weight, c, p.vec_dtype, 1.f, w[s]);
+    group_params<V>(p.bias, c, p.vec_dtype, 0.f, b[s]);
+    if constexpr (BACKWARD)
+#pragma unroll
+      for (int e = 0; e < V; ++e) dw[s][e] = db[s][e] = 0.f;
+  }
+  for (long long start = (long long)wave * runs; start < p.rows; start += round) {
+    const long long run = start + lane / p.lanes;
     float x[SLOTS][V], up[BACKWARD ? SLOTS : 1][V];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       R::unpack(next[s], x[s]);
       if constexpr (BACKWARD) R::unpack(next_up[s], up[s]);
     }
+    const float mean_there = next_mean, rstd_there = next_rstd;
     request(run + round);
     const bool live = run < p.rows;
     if constexpr (!BACKWARD) {
@@ -146,10 +182,10 @@ template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_boun
       for (int s = 0; s < SLOTS; ++s) {
 #pragma unroll
         for (int e = 0; e < V; ++e) x[s][e] = group_act(fmaf(x[s][e] * rstd, w[s][e], b[s][e]), p.activation);
-        if (live && has[s]) R::store(p.y, run * p.Cg + (l + p.lanes * s) * V, x[s]);
+        if (live && has[s]) R::store(R::rows(p.y, start * p.Cg), here + (unsigned)((l + p.lanes * s) * V), x[s]);
       }
     } else {
-      const float mean = live ? p.stats[2 * run] : 0.f, rstd = live ? p.stats[2 * run + 1] : 0.f;
+      const float mean = mean_there, rstd = rstd_there;
       float m1 = 0.f, m2 = 0.f;
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s)
@@ -168,7 +204,7 @@ template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_boun
       for (int s = 0; s < SLOTS; ++s) {
 #pragma unroll
         for (int e = 0; e < V; ++e) x[s][e] = rstd * (up[s][e] - fmaf(x[s][e], m2, m1));
-        if (live && has[s]) R::store(p.dx, run * p.Cg + (l + p.lanes * s) * V, x[s]);
+        if (live && has[s]) R::store(R::rows(p.dx, start * p.Cg), here + (unsigned)((l + p.lanes * s) * V), x[s]);
       }
     }
   }
@@ -289,6 +325,7 @@ RGLRU_DEVICE void group_statistics(const GroupArgs& p, const GroupPlace& g, floa
   for (int i = threadIdx.x >> 3; i < g.groups; i += kGroupThreads / 8) {
     const long long group = (long long)g.n * p.G + g.first_group + i;
     Moments m = {0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int e = sub; e < entries; e += 8) {
       const float* at = p.entries + (group * entries + e) * 3;
       m = join(m, {at[0], at[1], at[2]});
@@ -303,31 +340,52 @@ RGLRU_DEVICE void group_statistics(const GroupArgs& p, const GroupPlace& g, floa
   }
 }
 
+// A thread's next U vectors of its column, on their way while the ones before are worked on (and, the first, while the statistics and the
+// parameters are read).  Zeros behind the chunk.
+template <typename IO, int V, int U> struct GroupAhead {
+  typedef Run<IO, V> R;
+  typename R::Raw next[U];
+  RGLRU_DEVICE void request(const GroupArgs& p, const GroupPlace& g, const void* from, int l0) {
+    const long long base = (long long)g.n * p.L * p.C + g.c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int l = l0 + g.line + u * p.lines;
+      next[u] = typename R::Raw{};
+      if (g.live && l < g.to) next[u] = R::request(from, base + (long long)l * p.C);
+    }
+  }
+  RGLRU_DEVICE void take(float (&v)[U][V]) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) R::unpack(next[u], v[u]);
+  }
+};
+
 template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void group_norm_apply_kernel(GroupArgs p) {
   typedef Run<IO, V> R;
   constexpr int U = 4;
   __shared__ float mean[kGroupThreads], rstd[kGroupThreads];
   const GroupPlace g = group_place<V>(p);
+  GroupAhead<IO, V, U> x;
+  x.request(p, g, p.x, g.from);
+  float w[V], b[V];
+  group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
+  group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
   group_statistics(p, g, mean, rstd);
   __syncthreads();
   if (!g.live) return;
   const int mine = p.per_group > 1 ? 0 : g.col / p.width;
   const float mu = mean[mine], rs = rstd[mine];
-  float w[V], b[V];
-  group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
-  group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
-  const long long base = (long long)g.n * p.L * p.C + g.c;
-  for (int l = g.from + g.line; l < g.to; l += U * p.lines) {
+  for (int l0 = g.from; l0 < g.to; l0 += U * p.lines) {
+    const rsrc_t to = R::rows(p.y, ((long long)g.n * p.L + l0) * p.C);
     float v[U][V];
+    x.take(v);
+    x.request(p, g, p.x, l0 + U * p.lines);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (l + u * p.lines < g.to) R::load(p.x, base + (long long)(l + u * p.lines) * p.C, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (l + u * p.lines < g.to) {
+      if (l0 + g.line + u * p.lines < g.to) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[u][e] = group_act(fmaf((v[u][e] - mu) * rs, w[e], b[e]), p.activation);
-        R::store(p.y, base + (long long)(l + u * p.lines) * p.C, v[u]);
+        R::store(to, (unsigned)((g.line + u * p.lines) * p.C + g.c), v[u]);
       }
   }
 }
@@ -335,12 +393,13 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
 struct TwoSums { float a, b; };
 
 template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void group_norm_sums_kernel(GroupArgs p) {
-  typedef Run<IO, V> R;
-  constexpr int U = 2;
+  constexpr int U = 4;
   __shared__ TwoSums shared[kGroupThreads];
   __shared__ float lines[2][kGroupThreads * V];
   const GroupPlace g = group_place<V>(p);
-  const long long base = (long long)g.n * p.L * p.C + g.c;
+  GroupAhead<IO, V, U> next_x, next_up;
+  next_x.request(p, g, p.x, g.from);
+  next_up.request(p, g, p.dy, g.from);
   float w[V], dw[V], db[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
@@ -350,17 +409,15 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
     const float mu = p.stats[2 * group], rs = p.stats[2 * group + 1];
     group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
     group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
-    for (int l = g.from + g.line; l < g.to; l += U * p.lines) {
+    for (int l0 = g.from; l0 < g.to; l0 += U * p.lines) {
       float x[U][V], up[U][V];
+      next_x.take(x);
+      next_up.take(up);
+      next_x.request(p, g, p.x, l0 + U * p.lines);
+      next_up.request(p, g, p.dy, l0 + U * p.lines);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (l + u * p.lines < g.to) {
-          R::load(p.x, base + (long long)(l + u * p.lines) * p.C, x[u]);
-          R::load(p.dy, base + (long long)(l + u * p.lines) * p.C, up[u]);
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (l + u * p.lines < g.to)
+        if (l0 + g.line + u * p.lines < g.to)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float xhat = (x[u][e] - mu) * rs, t = up[u][e] * group_slope(fmaf(xhat, w[e], b[e]), p.activation);
@@ -402,13 +459,22 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
 
 template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void group_norm_dx_kernel(GroupArgs p) {
   typedef Run<IO, V> R;
-  constexpr int U = 2;
+  constexpr int U = 4;
   __shared__ float first[kGroupThreads], second[kGroupThreads];
   const GroupPlace g = group_place<V>(p);
+  GroupAhead<IO, V, U> next_x, next_up;
+  next_x.request(p, g, p.x, g.from);
+  next_up.request(p, g, p.dy, g.from);
+  const long long own = (long long)g.n * p.G + g.c / p.Cg;
+  const float mu = p.stats[2 * own], rs = p.stats[2 * own + 1];
+  float w[V], b[V];
+  group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
+  group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
   const int entries = p.chunks * p.per_group, sub = threadIdx.x & 7;
   for (int i = threadIdx.x >> 3; i < g.groups; i += kGroupThreads / 8) {
     const long long group = (long long)g.n * p.G + g.first_group + i;
     float a = 0.f, b = 0.f;
+#pragma unroll 4
     for (int e = sub; e < entries; e += 8) a += p.entries[(group * entries + e) * 2], b += p.entries[(group * entries + e) * 2 + 1];
 #pragma unroll
     for (int d = 4; d >= 1; d >>= 1) a += __shfl_down(a, d, 8), b += __shfl_down(b, d, 8);
@@ -418,28 +484,22 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
   if (!g.live) return;
   const int mine = p.per_group > 1 ? 0 : g.col / p.width;
   const float m1 = first[mine], m2 = second[mine];
-  const long long group = (long long)g.n * p.G + g.c / p.Cg, base = (long long)g.n * p.L * p.C + g.c;
-  const float mu = p.stats[2 * group], rs = p.stats[2 * group + 1];
-  float w[V], b[V];
-  group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
-  group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
-  for (int l = g.from + g.line; l < g.to; l += U * p.lines) {
+  for (int l0 = g.from; l0 < g.to; l0 += U * p.lines) {
+    const rsrc_t to = R::rows(p.dx, ((long long)g.n * p.L + l0) * p.C);
     float x[U][V], up[U][V];
+    next_x.take(x);
+    next_up.take(up);
+    next_x.request(p, g, p.x, l0 + U * p.lines);
+    next_up.request(p, g, p.dy, l0 + U * p.lines);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (l + u * p.lines < g.to) {
-        R::load(p.x, base + (long long)(l + u * p.lines) * p.C, x[u]);
-        R::load(p.dy, base + (long long)(l + u * p.lines) * p.C, up[u]);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (l + u * p.lines < g.to) {
+      if (l0 + g.line + u * p.lines < g.to) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float xhat = (x[u][e] - mu) * rs, t = up[u][e] * group_slope(fmaf(xhat, w[e], b[e]), p.activation);
           x[u][e] = rs * (fmaf(t, w[e], -m1) - xhat * m2);
         }
-        R::store(p.dx, base + (long long)(l + u * p.lines) * p.C, x[u]);
+        R::store(to, (unsigned)((g.line + u * p.lines) * p.C + g.c), x[u]);
       }
   }
 }
@@ -461,7 +521,7 @@ struct GroupPlan {
   int V, slots;
   int64_t sets, entries;                                    // partial parameter gradients; entries of a group
 };
-static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64_t G, int V) {
+static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64_t G, int V, bool backward) {
   GroupPlan plan;
   memset(&plan, 0, sizeof(plan));
   a.N = (int)N, a.L = (int)L, a.C = (int)C, a.G = (int)G, a.Cg = (int)(C / G), a.width = a.Cg / V;
@@ -476,7 +536,7 @@ static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64
     const int64_t runs = 64 / a.lanes;
     int64_t step = G;                                       // waves whose runs are a multiple of G
     for (int64_t r = runs; r > 1 && step % 2 == 0; r /= 2) step /= 2;
-    const int64_t all = (a.rows + runs - 1) / runs, most = (int64_t)num_compute_units() * 8;
+    const int64_t all = (a.rows + runs - 1) / runs, most = (int64_t)num_compute_units() * (backward ? 8 : 16);
     int64_t waves = all < most ? all : most;
     waves = (waves + step - 1) / step * step;
     a.waves = (int)waves;
@@ -488,7 +548,7 @@ static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64
   a.per_group = (a.width + a.columns - 1) / a.columns;
   a.blocks = a.per_group > 1 ? (int)(G * a.per_group) : (int)((C / V + a.columns - 1) / a.columns);
   a.lines = kGroupThreads / a.columns;
-  const int64_t wanted = (4 * (int64_t)num_compute_units() + N * a.blocks - 1) / (N * a.blocks), most = (L + 8 * a.lines - 1) / (8 * a.lines);
+  const int64_t wanted = (2 * (int64_t)num_compute_units() + N * a.blocks - 1) / (N * a.blocks), most = (L + 8 * a.lines - 1) / (8 * a.lines);
   int64_t chunks = wanted < most ? wanted : most;
   if (chunks < 1) chunks = 1;
   a.chunk = (int)((L + chunks - 1) / chunks);
@@ -551,7 +611,7 @@ size_t rglru_hip_group_norm_scratch_bytes(int64_t N, int64_t L, int64_t C, int64
     if ((C / G) % v) continue;
     GroupArgs a;
     memset(&a, 0, sizeof(a));
-    const GroupPlan plan = group_plan(a, N, L, C, G, v);
+    const GroupPlan plan = group_plan(a, N, L, C, G, v, backward != 0);
     const size_t n = group_entries_bytes(a, plan, backward != 0) + (backward ? 2 * group_up((size_t)plan.sets * C * 4) : 0);
     if (n > most) most = n;
   }
@@ -565,7 +625,7 @@ int rglru_hip_group_norm_fwd(const void* x, const void* weight, const void* bias
   if (!x || !y || !scratch) return fail(RGLRU_E_ARG, "group_norm_fwd: null pointer");
   GroupArgs a;
   memset(&a, 0, sizeof(a));
-  const GroupPlan plan = group_plan(a, N, L, C, G, group_vector(C / G, dtype, {x, y}));
+  const GroupPlan plan = group_plan(a, N, L, C, G, group_vector(C / G, dtype, {x, y}), false);
   a.x = x, a.weight = weight, a.bias = bias, a.y = y, a.stats = stats, a.entries = (float*)scratch;
   a.eps = eps, a.activation = activation, a.vec_dtype = vec_dtype;
   hipStream_t s = (hipStream_t)stream;
@@ -590,7 +650,7 @@ int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias
   if (!x || !stats || !dy || !scratch || !dx) return fail(RGLRU_E_ARG, "group_norm_bwd: null pointer");
   GroupArgs a;
   memset(&a, 0, sizeof(a));
-  const GroupPlan plan = group_plan(a, N, L, C, G, group_vector(C / G, dtype, {x, dy, dx}));
+  const GroupPlan plan = group_plan(a, N, L, C, G, group_vector(C / G, dtype, {x, dy, dx}), true);
   a.x = x, a.weight = weight, a.bias = bias, a.dy = dy, a.dx = dx, a.stats = const_cast<float*>(stats), a.entries = (float*)scratch;
   a.activation = activation, a.vec_dtype = vec_dtype;
   const bool params = dweight || dbias;
