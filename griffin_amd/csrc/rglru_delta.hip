@@ -219,6 +219,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
   auto request = [&](int stage) { tiles.request(p, lds0 + (unsigned)(stage * Tiles::kBytes), wave); };
   // a chunk's matrix of `rows` elements a column, by eight of a column a lane
   const unsigned plane_bytes = (unsigned)p.columns * (unsigned)sizeof(IO);
+  const bool past = p.past != 0;
   auto matrix = [&](void* base, int n, int rows) {
     return make_rsrc((IO*)base + (first + n) * PL * p.columns * rows, PL * plane_bytes * (unsigned)rows);
   };
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       if (mine) {
         const rsrc_t r = matrix(p.values, n, 64);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, zw[ks]);
+        for (int ks = 0; ks < 2; ++ks) M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, zw[ks], past);
       }
     }
     if constexpr (OUT) {
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
         const Wide s = M::wide(state[2 * ks], state[2 * ks + 1]);
         M::ew(acc, ka[ks % D], s);
         if constexpr (OUT) M::ew(o, qa[ks % D], s);
-        if constexpr (SAVE) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, s);
+        if constexpr (SAVE) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, s, past);
         phase();
       }
       square(solve, D - 1);

@@ -53,6 +53,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
   auto request = [&](int stage) { tiles.request(p, lds0 + (unsigned)(stage * Tiles::kBytes), wave); };
   // a chunk's matrix of `rows` elements a column, by eight of a column a lane
   const unsigned plane_bytes = (unsigned)p.columns * (unsigned)sizeof(IO);
+  const bool past = p.past != 0;
   auto matrix = [&](void* base, int n, int rows) {
     return make_rsrc((IO*)base + (first + n) * PL * p.columns * rows, PL * plane_bytes * (unsigned)rows);
   };
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       const rsrc_t r = matrix(p.dvalues, n, 64);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
-        M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, M::wide(y[2 * ks], y[2 * ks + 1]));
+        M::put(r, (unsigned)(col * 64 + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * 64, M::wide(y[2 * ks], y[2 * ks + 1]), past);
     }
     const int t0 = n * kDeltaChunk;
     const long long stride = (long long)p.HV * p.V;
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
         phase();
         const Wide d = M::wide(dstate[2 * ks], dstate[2 * ks + 1]);
         M::ew(dz, ka[ks % D], d);
-        if constexpr (!LOCAL) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, d);
+        if constexpr (!LOCAL) M::put(saved, (unsigned)(col * DK + 32 * ks + 8 * g) * (unsigned)sizeof(IO), plane_bytes * DK, d, past);
         phase();
       }
       square(within, D - 1);

@@ -232,6 +232,7 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   for (int i = 6; i < 9; ++i) whole = whole && st[i] % e == 0;
   if (v && z.value_row == V && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of values must be 16-byte aligned", who);
   a.segments = (int)z.segments, a.length = (int)z.length;
+  a.past = z.chunks * z.columns * (z.width + 64) * 4 > kCachedBytes;
   char* base = (char*)ws;
   a.through = base + z.through, a.local = (float*)(base + z.local), a.edges = (float*)(base + z.edges);
   a.gates = (float*)(base + z.gates);
