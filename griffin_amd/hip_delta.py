@@ -8,11 +8,9 @@ counterpart.  There is no CPU fallback here: the operators raise when the librar
 
 from __future__ import annotations
 
-import torch
 from torch import Tensor
 
 from . import _lib
-from .hip_scan import pack_flags
 
 
 def _scale(scale: float | None, q: Tensor) -> float:
@@ -40,8 +38,9 @@ def hip_gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Te
     for name, mask in (("reset_mask", reset_mask), ("active_mask", active_mask)):
         if mask is not None and mask.shape != q.shape[:2]:
             raise ValueError(f"{name} must have shape {tuple(q.shape[:2])}, got {tuple(mask.shape)}")
-    reset_mask, active_mask = (None if m is None else m.to(device=q.device, dtype=torch.bool) for m in (reset_mask, active_mask))
-    return native.gated_delta(q, k, v, log_decay, beta, h0, pack_flags(reset_mask, active_mask), _scale(scale, q))
+    reset_mask, active_mask = (None if m is None else m.to(device=q.device) for m in (reset_mask, active_mask))
+    flags = None if reset_mask is None and active_mask is None else native.pack_flags(reset_mask, active_mask)
+    return native.gated_delta(q, k, v, log_decay, beta, h0, flags, _scale(scale, q))
 
 
 def hip_gated_delta_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor, state: Tensor,

@@ -1,5 +1,9 @@
 """The gated delta rule on the GPU against its definition, token by token in 64 bits."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -317,3 +321,51 @@ def test_results_repeat_bit_for_bit():
     first, second = (run(hip_gated_delta, case, None, None, "cuda") for _ in range(2))
     assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
     assert all(torch.equal(first[2][n], second[2][n]) for n in NAMES)
+
+
+def test_a_state_that_is_carried_by_itself():
+    """Sequences of one token, of masked tokens alone, and of nothing but the carried state."""
+    case = make(2, 1, 1, 2, 32, 32)
+    check(case)
+    check(case, None, torch.zeros(2, 1, dtype=torch.bool))
+    case = make(1, 130, 1, 1, 32, 32)
+    check(case, None, torch.zeros(1, 130, dtype=torch.bool))
+
+
+def test_a_reset_mask_that_is_written_between_calls():
+    case = make(1, 100, 1, 1, 32, 32, carried=False)
+    operands = [case[n].cuda() for n in NAMES[:5]]
+    reset = torch.zeros(1, 100, dtype=torch.bool, device="cuda")
+    plain, none = hip_gated_delta(*operands, reset_mask=reset), hip_gated_delta(*operands)
+    assert torch.equal(plain[0], none[0])
+    reset[0, 50] = True
+    got, last = hip_gated_delta(*operands, reset_mask=reset)
+    want, want_last = recurrence(*(t.cpu().double() for t in operands), None, 32 ** -0.5, reset.cpu())
+    assert rel_err(got, want) <= OUT[F32] and rel_err(last, want_last) <= STATE[F32]
+    with torch.inference_mode():
+        made = reset.clone()
+    leaves = [t.requires_grad_(True) for t in operands]
+    torch.autograd.grad(hip_gated_delta(*leaves, reset_mask=made)[0].sum(), leaves)
+
+
+def test_two_calls_at_once():
+    """On two streams, in segments and not: nothing is shared."""
+    cases = [make(1, 1500, 1, 1, 128, 64, dtype=BF16, seed=7), make(2, 300, 2, 4, 64, 64, dtype=BF16, seed=8)]
+    want = [run(hip_gated_delta, case, None, None, "cuda") for case in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(run(hip_gated_delta, case, None, None, "cuda"))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(a[2][n], b[2][n]) for n in NAMES)
+
+
+def test_captures():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    child = subprocess.run([sys.executable, "-u", "-m", "tests.capture_operators_child"], cwd=root, capture_output=True, text=True, timeout=100)
+    print(child.stdout + child.stderr[-2000:], flush=True)
+    assert child.returncode == 0
