@@ -369,3 +369,26 @@ def test_captures():
     child = subprocess.run([sys.executable, "-u", "-m", "tests.capture_operators_child"], cwd=root, capture_output=True, text=True, timeout=100)
     print(child.stdout + child.stderr[-2000:], flush=True)
     assert child.returncode == 0
+
+
+def test_states_that_go_past_the_caches():
+    """Large batches, whose states are not kept in the caches, against the same rows in parts."""
+    B, H, K, V = 260, 8, 128, 128                              # 130 MiB of state
+    gen = torch.Generator("cuda").manual_seed(3)
+    normal = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")
+    q, k = (torch.nn.functional.normalize(normal(B, H, K), dim=-1).bfloat16() for _ in range(2))
+    rest = [normal(B, H, V).bfloat16(), -normal(B, H).abs(), normal(B, H).sigmoid()]
+    flags = (torch.arange(B, device="cuda") % 5 == 0).to(torch.uint8)
+    state = normal(B, H, K, V)
+    parts = [[t[i : i + 65].clone() for t in (q, k, *rest, state, flags)] for i in range(0, B, 65)]
+    out = hip_gated_delta_step(q, k, *rest, state, flags=flags)
+    want = torch.cat([hip_gated_delta_step(*part[:6], flags=part[6]) for part in parts])
+    assert torch.equal(out, want) and torch.equal(state, torch.cat([part[5] for part in parts]))
+
+    case = make(8, 1100, 12, 12, 128, 128, dtype=BF16)        # 162 MiB of states and values
+    whole = run(hip_gated_delta, case, None, None, "cuda")
+    halves = [run(hip_gated_delta, {n: t[i : i + 4] for n, t in case.items()}, None, None, "cuda") for i in (0, 4)]
+    assert rel_err(whole[0], torch.cat([h[0] for h in halves])) <= 2 * OUT[BF16]
+    assert rel_err(whole[1], torch.cat([h[1] for h in halves])) <= 2 * STATE[BF16]
+    for name in NAMES:
+        assert rel_err(whole[2][name], torch.cat([h[2][name] for h in halves])) <= 2 * GRAD[BF16], name
