@@ -392,3 +392,24 @@ def test_states_that_go_past_the_caches():
     assert rel_err(whole[1], torch.cat([h[1] for h in halves])) <= 2 * STATE[BF16]
     for name in NAMES:
         assert rel_err(whole[2][name], torch.cat([h[2][name] for h in halves])) <= 2 * GRAD[BF16], name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_broadcast_operands_and_gradients(dtype):
+    """Operands that one number stands for along an axis, gradients that autograd hands over without memory of their own."""
+    case = make(2, 90, 2, 2, 32, 48, dtype=dtype)
+    case["q"] = case["q"][:, :1, :1]                           # one query for all tokens and heads
+    case["beta"] = case["beta"][:1, :1, :1]
+
+    def results(fn, device, to):
+        leaves = [case[n].to(device=device, dtype=to or case[n].dtype).requires_grad_(True) for n in NAMES]
+        q, k, v, log_decay, beta, h0 = leaves
+        out, last = fn(q.expand(2, 90, 2, 32), k, v, log_decay, beta.expand(2, 90, 2), h0)
+        return [out.detach(), last.detach(), *torch.autograd.grad(out.float().sum() + last.sum() if to is None else out.sum() + last.sum(), leaves)]
+
+    want = results(lambda *t: recurrence(*t, 32 ** -0.5), "cpu", torch.float64)
+    got = results(hip_gated_delta, "cuda", None)
+    # a broadcast input's gradient is the sum of up to 360 of those of its uses, which cancel by less than sixteen to one
+    for name, g, w in zip(("o", "state", *NAMES), got, want):
+        limit = OUT[dtype] if name == "o" else STATE[dtype] if name == "state" else (16 if name in ("q", "beta") else 1) * GRAD[dtype]
+        assert rel_err(g, w) <= limit, (name, rel_err(g, w))

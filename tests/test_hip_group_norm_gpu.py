@@ -166,3 +166,18 @@ def test_heads_of_a_recurrence(dtype):
     assert rel_err(got, want) <= 3 * steps
     for name, a, b in zip(("q", "k", "v", "log_decay", "beta", "weight", "bias", "gate"), got_grads, want_grads):
         assert rel_err(a, b) <= 6 * steps, name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(20, 64), (2, 70, 64)], ids=str)
+def test_parameters_off_a_vector_boundary(shape, dtype):
+    """... give what the same numbers on one give, bit for bit."""
+    x, weight, bias, up = (t.cuda() for t in make(shape, dtype=dtype))
+    results = []
+    for offset in (0, 1):
+        room = torch.zeros(2, shape[-1] + offset, dtype=dtype, device="cuda")
+        room[0, offset:], room[1, offset:] = weight, bias
+        leaves = [x.clone().requires_grad_(True), *(row[offset:].detach().requires_grad_(True) for row in room)]
+        out = hip_group_norm(leaves[0], 4, leaves[1], leaves[2], activation="silu")
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, up)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
