@@ -6,7 +6,13 @@
 //
 // One position (the heads' norm behind a recurrence: every token on its own): a group is a run of C / G elements, which 4 to 64
 // lanes hold in registers.  Everything is read once and written once.
-// Many positions: the positions are cut into chunks, one kernel leaves each chunk's sums, the next joins them and writes.
+// 16384 rows of 1024 in 8 groups (bf16): 14 us forward, 29 + 5 backward, where the bytes take 13 and 20 at the rate of a large copy.
+// The backward pass keeps half as many waves: each leaves a set of partial parameter gradients (16 waves a compute unit instead of
+// 8: 35 + 9 instead of 37 + 5 us at the time).
+// Many positions: the positions are cut into chunks, two workgroups a compute unit, one kernel leaves each chunk's sums, the next joins
+// them and writes (four a compute unit: more sums to join, 25.6 -> 26.4 and 21.3 -> 22.4 us for the two that write).  8 rows of 2048 x 1024: 10 + 17 us
+// forward, 22 + 26 + 4 backward.  Bound by memory and by the chain in front of it; the first vectors are requested before
+// the sums are joined (apply 21 -> 17 us).
 // All sums are fp32.  Variances come from deviations from a mean (of the run, or of the batch of values a thread holds) and are joined
 // with the difference of the means, never from a difference of squares.
 
