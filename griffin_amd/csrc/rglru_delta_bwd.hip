@@ -86,12 +86,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
     for (int t = 0; t < 2 * KS; ++t) dstate[t] = *reinterpret_cast<const f32x4*>(at + tile_index(t, 4 * g));
   } else {
 #pragma unroll
-  for (int t = 0; t < 2 * KS; ++t)
+    for (int t = 0; t < 2 * KS; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = tile_index(t, 4 * g + e);
-      dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
-    }
+      for (int e = 0; e < 4; ++e) {
+        const int row = tile_index(t, 4 * g + e);
+        dstate[t][e] = p.dh_last && live && row < p.K ? p.dh_last[((long long)head * p.K + row) * p.V + col] : 0.f;
+      }
   }
   wait_for_all();
   for (int n = last; n >= begin; --n) {

@@ -32,6 +32,10 @@ def hip_gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Te
     that count; the others leave the state as it is, give zeros and receive zero gradients, whatever they hold.  Among the
     active tokens a NaN or an infinity may reach all outputs of its chunk of 64 tokens, and those behind it.
 
+    Products are exact to fp32 for float32 operands and to 2^-17 for what is computed between them from bfloat16 ones, relative to their terms:
+    what the keys of a chunk all but erase (the gradient of ``h0`` behind many parallel keys) is known to that part of what it was, not
+    of what is left.
+
     Differentiable (first order) in q, k, v, log_decay, beta and h0, through both results.
     """
     native = _lib.native()
