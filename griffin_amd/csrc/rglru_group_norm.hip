@@ -574,9 +574,11 @@ static int group_check(const char* who, int64_t N, int64_t L, int64_t C, int64_t
   if (activation != RGLRU_ACT_NONE && activation != RGLRU_ACT_SILU && activation != RGLRU_ACT_GELU) return fail(RGLRU_E_ARG, "%s: unknown activation %d", who, activation);
   for (int d : {dtype, vec_dtype})
     if (d != RGLRU_F32 && d != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown dtype %d", who, d);
-  if (L >= (1ll << 30) || C >= (1ll << 24) || N * G >= (1ll << 30) || N >= (1ll << 30) / C) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
+  if (L >= (1ll << 30) || C >= (1ll << 24) || N >= (1ll << 30) / G) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   return RGLRU_OK;
 }
+
+static bool group_fits(const GroupPlan& plan, const GroupArgs& a) { return plan.rows || (int64_t)a.N * a.blocks < (1ll << 31) / a.chunks; }
 
 static int group_vector(int64_t Cg, int dtype, std::initializer_list<const void*> tensors) {
   const int v = dtype == RGLRU_BF16 ? 8 : 4;
@@ -635,6 +637,7 @@ int rglru_hip_group_norm_fwd(const void* x, const void* weight, const void* bias
   a.x = x, a.weight = weight, a.bias = bias, a.y = y, a.stats = stats, a.entries = (float*)scratch;
   a.eps = eps, a.activation = activation, a.vec_dtype = vec_dtype;
   hipStream_t s = (hipStream_t)stream;
+  if (!group_fits(plan, a)) return fail(RGLRU_E_UNSUPPORTED, "group_norm_fwd: too large for one launch");
   if (plan.rows) {
     group_rows<false>(a, plan, dtype, s);
     return check_launch("group_norm_fwd");
@@ -665,6 +668,7 @@ int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias
     a.dbias = (float*)((char*)a.dweight + group_up((size_t)plan.sets * C * 4));
   }
   hipStream_t s = (hipStream_t)stream;
+  if (!group_fits(plan, a)) return fail(RGLRU_E_UNSUPPORTED, "group_norm_bwd: too large for one launch");
   if (plan.rows) {
     group_rows<true>(a, plan, dtype, s);
     rc = check_launch("group_norm_bwd");

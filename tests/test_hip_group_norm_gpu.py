@@ -181,3 +181,15 @@ def test_parameters_off_a_vector_boundary(shape, dtype):
         out = hip_group_norm(leaves[0], 4, leaves[1], leaves[2], activation="silu")
         results.append([out.detach(), *torch.autograd.grad(out, leaves, up)])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_more_than_two_to_the_31_elements():
+    """... whose offsets pass 32 bits: the last rows by themselves give the same."""
+    rows, channels = (1 << 21) + 3, 1024
+    x = torch.empty(rows, channels, dtype=BF16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1)).requires_grad_(True)
+    out = hip_group_norm(x, 8)
+    (grad,) = torch.autograd.grad(out, x, torch.ones((), dtype=BF16, device="cuda").expand_as(out) * out.detach())
+    last = x.detach()[-64:].clone().requires_grad_(True)
+    want = hip_group_norm(last, 8)
+    (want_grad,) = torch.autograd.grad(want, last, want.detach())
+    assert torch.equal(out[-64:], want) and torch.equal(grad[-64:], want_grad)

@@ -119,6 +119,9 @@ def norm_bwd(lib, sizes=(2, 3, 8, 2), activation=0, types=(F32, F32, F32), stats
     (lambda lib: norm_fwd(lib, scratch=None), ARG, b"null"),
     (lambda lib: norm_fwd(lib, sizes=(2, 1 << 30, 8, 2)), UNSUPPORTED, b"too large"),
     (lambda lib: norm_fwd(lib, sizes=(2, 3, 1 << 24, 2)), UNSUPPORTED, b"too large"),
+    (lambda lib: norm_fwd(lib, sizes=(1 << 27, 1, 64, 8)), UNSUPPORTED, b"too large"),
+    (lambda lib: norm_fwd(lib, sizes=(1 << 28, 8, 8192, 1)), UNSUPPORTED, b"too large"),
+    (lambda lib: norm_bwd(lib, sizes=(1 << 28, 8, 8192, 1)), UNSUPPORTED, b"too large"),
     (lambda lib: norm_bwd(lib, sizes=(2, 3, 8, 5)), ARG, b"sizes"),
     (lambda lib: norm_bwd(lib, stats=None), ARG, b"null"),
     (lambda lib: norm_bwd(lib, types=(F32, F32, 6)), ARG, b"dtype"),
