@@ -413,3 +413,25 @@ def test_broadcast_operands_and_gradients(dtype):
     for name, g, w in zip(("o", "state", *NAMES), got, want):
         limit = OUT[dtype] if name == "o" else STATE[dtype] if name == "state" else (16 if name in ("q", "beta") else 1) * GRAD[dtype]
         assert rel_err(g, w) <= limit, (name, rel_err(g, w))
+
+
+def test_offsets_that_pass_32_bits():
+    """A prompt of more than 2^31 elements a tensor and a state of as many: the ends by themselves give the same."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    normal = lambda *shape, by=1.0: torch.empty(*shape, dtype=BF16, device="cuda").normal_(generator=gen).mul_(by)
+    T, H, K, tail = (1 << 19) + 128, 32, 128, 128
+    q, k, v = normal(1, T, H, K, by=K ** -0.5), normal(1, T, H, K, by=0.8 * K ** -0.5), normal(1, T, H, K)
+    decay, beta = -normal(1, T, H).abs_(), normal(1, T, H).sigmoid_()
+    out, last = hip_gated_delta(q, k, v, decay, beta)
+    front = [t[:, : T - tail] for t in (q, k, v, decay, beta)]
+    _, state = hip_gated_delta(*front)
+    want, want_last = hip_gated_delta(*(t[:, T - tail :] for t in (q, k, v, decay, beta)), state)
+    assert rel_err(out[:, T - tail :], want) <= 2 * OUT[BF16] and rel_err(last, want_last) <= 2 * STATE[BF16]
+    del q, k, v, out, front
+
+    B, H = 16500, 8
+    state = torch.empty(B, H, K, K, device="cuda").normal_(generator=gen)
+    token = [normal(B, H, K, by=K ** -0.5), normal(B, H, K, by=K ** -0.5), normal(B, H, K), -normal(B, H).abs_(), normal(B, H).sigmoid_()]
+    end = state[-4:].clone()
+    out = hip_gated_delta_step(*token, state)
+    assert torch.equal(out[-4:], hip_gated_delta_step(*(t[-4:] for t in token), end)) and torch.equal(state[-4:], end)
