@@ -92,12 +92,6 @@ template <> struct Mx<__bf16> {
     w.lo = __builtin_shufflevector(al, bl, 0, 1, 2, 3, 4, 5, 6, 7);
     return w;
   }
-  static RGLRU_DEVICE Frag exact(f32x4 a, f32x4 b) {
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = (__bf16)a[e], f[4 + e] = (__bf16)b[e];
-    return f;
-  }
   static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] = (float)f[e], b[e] = (float)f[4 + e];
@@ -150,7 +144,6 @@ template <> struct Mx<float> {
   template <int FROM, int TO, int N> static RGLRU_DEVICE void we(f32x4 (&acc)[N], const Frag (&a)[N], const Frag& b) { ww<FROM, TO>(acc, a, b); }
   template <int N> static RGLRU_DEVICE void ew(f32x4 (&acc)[N], const Frag (&a)[N], const Frag& b) { ww<0, N>(acc, a, b); }
   static RGLRU_DEVICE Wide wide(f32x4 a, f32x4 b) { return {a, b}; }
-  static RGLRU_DEVICE Frag exact(f32x4 a, f32x4 b) { return {a, b}; }
   static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) { a = f.lo, b = f.hi; }
   static RGLRU_DEVICE void put(float* at, long long, f32x4 v) { *reinterpret_cast<f32x4*>(at) = v; }
   static RGLRU_DEVICE void put(rsrc_t r, unsigned at, unsigned, const Wide& w, bool past) {
