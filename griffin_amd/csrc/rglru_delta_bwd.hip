@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * kStage > kRows ? STAGES * kStage : kRows];
   __shared__ double total[64];
   __shared__ float beta[64], to_end[64], reads[2][64], writes[2][64], leaves[2][64], sums[8];
-  __shared__ int segment[64];
+  __shared__ int segment[64], held[8];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
   // the heads of a chunk side by side: what they read and write lies side by side
@@ -302,6 +302,7 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     }
     f32x4 dq[KS] = {}, dr[KS] = {}, dw[KS] = {}, pairs[4] = {};
     float carried = 0.f;                                   // <S, dS'>
+    bool some = false;                                     // S is not all zeros
     wait_for_all();
     for (int c0 = 0; c0 < p.columns; c0 += CB) {
       const int stage = STAGES == 2 ? (c0 / CB) & 1 : 0;
@@ -339,10 +340,13 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
         if constexpr (PL == 2) {
           const Unit al = *reinterpret_cast<const Unit*>(states + CB * DK + at * Keys::E), dl = *reinterpret_cast<const Unit*>(dstates + CB * DK + at * Keys::E);
 #pragma unroll
-          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], carried);
+          for (int e = 0; e < Keys::E; ++e) {
+            carried = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], carried);
+            some = some || !((float)a[e] == 0.f);
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e], (float)d[e], carried);
+          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e], (float)d[e], carried), some = some || !((float)a[e] == 0.f);
         }
       }
       if (STAGES == 1 && c0 + CB < p.columns) {
@@ -377,7 +381,8 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) carried += __shfl_xor(carried, m, 64);
-    if (lane == 0) sums[wave] = carried;
+    const bool wave_some = __ballot(some) != 0;
+    if (lane == 0) sums[wave] = carried, held[wave] = wave_some;
     auto put_pairs = [&](bool strengths) {                 // kept [j][i]; blocks above the diagonal that a product touches are zeros
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
@@ -457,10 +462,13 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
         if (lane + d < 64) from += other;
       }
       float across = 0.f;
+      int history = 0;
 #pragma unroll
-      for (int w = 0; w < THREADS / 64; ++w) across += sums[w];
+      for (int w = 0; w < THREADS / 64; ++w) across += sums[w], history |= held[w];
       across = carry == 0.f ? 0.f : carry * across;
-      const float d = gate.counts && !gate.starts ? from + (write + across) : 0.f;
+      // a first token has nothing to decay: zero, and not what is left of sums that cancel
+      const bool first = history == 0 && (counts & ((1ull << lane) - 1)) == 0;
+      const float d = gate.counts && !gate.starts && !first ? from + (write + across) : 0.f;
       const long long at = ((long long)b * p.T + t0 + lane) * p.HV + hv;
       if (lane < left) {
         delta_put_gate(p.dlog_decay, at, p.decay_dtype, d);

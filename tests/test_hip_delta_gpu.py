@@ -435,3 +435,17 @@ def test_offsets_that_pass_32_bits():
     end = state[-4:].clone()
     out = hip_gated_delta_step(*token, state)
     assert torch.equal(out[-4:], hip_gated_delta_step(*(t[-4:] for t in token), end)) and torch.equal(state[-4:], end)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape, skipped", [((2, 1, 1, 2, 40, 33), 0), ((1, 1, 2, 2, 128, 128), 0), ((1, 71, 1, 1, 64, 64), 70), ((2, 200, 1, 1, 64, 64), 150)], ids=str)
+def test_a_first_token_has_nothing_to_decay(shape, skipped, dtype):
+    """The gradient of its log decay is zero, not a rounding: without a state in front, and behind padding."""
+    case = make(*shape, dtype=dtype, carried=False)
+    active = (torch.arange(shape[1]) >= skipped).expand(shape[0], -1) if skipped else None
+    _, _, grads = run(hip_gated_delta, case, None, active, "cuda")
+    assert grads["log_decay"][:, : skipped + 1].abs().max() == 0
+    check(case, None, active)
+    if shape[1] == 1:
+        carried = make(*shape, dtype=dtype)
+        assert run(hip_gated_delta, carried, None, None, "cuda")[2]["log_decay"].abs().min() > 0
