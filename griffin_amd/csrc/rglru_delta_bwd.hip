@@ -260,10 +260,8 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
   IO *const keys = (IO*)lds, *const queries = (IO*)(lds + KeyLoad::kBytes), *const area = (IO*)(lds + 2 * KeyLoad::kBytes);
   const unsigned lds0 = lds_address(lds);
   f32x4 all_dq[KS] = {}, all_dk[KS] = {};                   // over the value heads that share the key head
-  UpLoad up_load;
   ValueLoad value_load;
   StateLoad state_load;
-  up_load.setup(tid, p.up_t, p.value_width);
   value_load.setup(tid, 64, 64);
   state_load.setup(tid, DK, DK);
 
@@ -277,9 +275,11 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     auto request = [&](int c0, int stage) {
       const int there = p.columns - c0;                     // columns of the values from here on
       const unsigned to = lds0 + (unsigned)(stage * kStage);
-      const int width = p.value_width - c0;
-      up_load.request(delta_rsrc((const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h + c0, width < CB ? UpLoad::extent(p.up_t, width, left) : UpLoad::extent(p.up_t, CB, left)),
-                      to + kUp, wave);
+      // zeros past the value's last column: what lies there are other heads' and other tokens' gradients, whatever they hold
+      const int width = p.value_width - c0 < CB ? p.value_width - c0 : CB;
+      UpLoad up_load;
+      up_load.setup(tid, p.up_t, width);
+      up_load.request(delta_rsrc((const IO*)p.dout + b * p.up_b + t0 * p.up_t + hv * p.up_h + c0, UpLoad::extent(p.up_t, width, left)), to + kUp, wave);
 #pragma unroll
       for (int plane = 0; plane < PL; ++plane) {
         const long long at = (chunk * PL + plane) * p.columns + c0;

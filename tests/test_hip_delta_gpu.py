@@ -449,3 +449,43 @@ def test_a_first_token_has_nothing_to_decay(shape, skipped, dtype):
     if shape[1] == 1:
         carried = make(*shape, dtype=dtype)
         assert run(hip_gated_delta, carried, None, None, "cuda")[2]["log_decay"].abs().min() > 0
+
+
+@pytest.mark.parametrize("V", [40, 48, 80])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_masked_tokens_may_hold_anything_beside_any_width(V, dtype):
+    """Behind the last columns of a value lie the next head's and, behind the last head, the next token's."""
+    reset, active = masks(3, 130, seed=4)
+    active[0] = torch.arange(130) < 37                          # padding behind the middle of a chunk
+    case = make(3, 130, 2, 4, 64, V, dtype=dtype)
+    clean = run(hip_gated_delta, case, reset, active, "cuda")
+    for name in ("q", "k", "v", "log_decay", "beta", "up"):
+        case[name] = case[name].clone()
+        case[name][~active] = float("nan") if name != "log_decay" else float("inf")
+    dirty = run(hip_gated_delta, case, reset, active, "cuda")
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for name in NAMES:
+        assert torch.equal(clean[2][name], dirty[2][name]), name
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (2, 4)], ids=str)
+@pytest.mark.parametrize("V", [33, 40, 48, 80])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_heads_keep_their_gradients_whatever_others_receive(V, dtype, heads):
+    case = make(2, 70, *heads, 64, V, dtype=dtype)
+    share = heads[1] // heads[0]
+    clean = run(hip_gated_delta, case, None, None, "cuda")[2]
+    for value in (float("inf"), float("nan")):
+        for spoilt in range(2):                                 # the value heads of one key head
+            of = slice(spoilt * share, (spoilt + 1) * share)
+            case["up"] = case["up"].clone()
+            kept = case["up"].clone()
+            case["up"][:, :, of] = value
+            got = run(hip_gated_delta, case, None, None, "cuda")[2]
+            case["up"] = kept
+            rest = slice((1 - spoilt) * share, (2 - spoilt) * share)
+            for name in NAMES:
+                axis = 1 if name == "h0" else 2
+                one = slice(1 - spoilt, 2 - spoilt) if name in ("q", "k") else rest
+                picked = [t[(slice(None),) * axis + (one,)] for t in (got[name], clean[name])]
+                assert torch.equal(*picked), name
