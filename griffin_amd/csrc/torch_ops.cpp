@@ -2236,19 +2236,23 @@ struct DeltaOperands {
   Tensor q, k, v, log_decay, beta;
   int64_t strides[9];
   int64_t B, T, H, HV, K, V;
+  // where batch, tokens and heads lie; an axis of one element has no distance, whatever its tensor says
+  static void distances(const Tensor& t, int64_t* to) {
+    for (int i = 0; i < 3; ++i) to[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
   // rows of whole 16-byte vectors have to lie on their boundaries
   static Tensor rows(const Tensor& t) {
     const int64_t e = 16 / t.element_size();
     const bool whole = t.size(3) % e == 0;
     bool plain = (t.stride(3) == 1 || t.size(3) == 1) && (!whole || is_aligned(t));
-    for (int i = 0; i < 3; ++i) plain = plain && t.stride(i) >= 0 && (!whole || t.stride(i) % e == 0);
-    return plain && t.stride(1) < (int64_t(1) << 22) ? t : aligned(t);
+    int64_t at[3];
+    distances(t, at);
+    for (int i = 0; i < 3; ++i) plain = plain && at[i] >= 0 && (!whole || at[i] % e == 0);
+    return plain && at[1] < (int64_t(1) << 22) ? t : aligned(t);
   }
   DeltaOperands(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& decay_in, const Tensor& beta_in)
       : q(rows(q_in)), k(rows(k_in)), v(rows(v_in)), log_decay(decay_in.contiguous()), beta(beta_in.contiguous()) {
-    int at = 0;
-    for (const Tensor* t : {&q, &k, &v})
-      for (int i = 0; i < 3; ++i) strides[at++] = t->stride(i);
+    distances(q, strides), distances(k, strides + 3), distances(v, strides + 6);
     B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), HV = v.size(2), V = v.size(3);
   }
 };
@@ -2313,8 +2317,8 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
       c10::DeviceGuard guard(q.device());
       const auto dtype = q.scalar_type();
       const int64_t B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), HV = m[0], V = m[1];
-      int64_t strides[9];
-      for (int i = 0; i < 3; ++i) strides[i] = q.stride(i), strides[3 + i] = k.stride(i), strides[6 + i] = 0;
+      int64_t strides[9] = {};
+      DeltaOperands::distances(q, strides), DeltaOperands::distances(k, strides + 3);
       Tensor dout = grads[0].defined() ? aligned(as(grads[0], dtype)) : at::zeros({B, T, HV, V}, q.options());
       Tensor dh_last = as(grads[1], at::kFloat);
       dq = fresh({B, T, H, K}, dtype, q), dk = fresh({B, T, H, K}, dtype, q), dv = fresh({B, T, HV, V}, dtype, q);

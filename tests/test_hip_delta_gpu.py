@@ -489,3 +489,32 @@ def test_heads_keep_their_gradients_whatever_others_receive(V, dtype, heads):
                 one = slice(1 - spoilt, 2 - spoilt) if name in ("q", "k") else rest
                 picked = [t[(slice(None),) * axis + (one,)] for t in (got[name], clean[name])]
                 assert torch.equal(*picked), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_axes_of_one_element_may_have_any_stride(dtype):
+    """A token of one row out of a projection whose rows are no whole vectors; tokens of a long way apart, of which there is one."""
+    H, HV, K, V = 2, 4, 32, 24
+    width = 2 * H * K + HV * V
+    gen = torch.Generator().manual_seed(3)
+    rows = torch.randn(1, 9, width + 2, generator=gen).to(dtype).cuda()
+    gates = [-torch.rand(1, 1, HV, generator=gen).cuda(), torch.rand(1, 1, HV, generator=gen).cuda()]
+
+    def both(views):
+        results = []
+        for operands in (views, [t.clone(memory_format=torch.contiguous_format) for t in views]):
+            leaves = [t.detach().requires_grad_(True) for t in operands]
+            batch = leaves[0].shape[0]
+            out, last = hip_gated_delta(*leaves, *(g.expand(batch, 1, HV) for g in gates))
+            results.append([out, last, *torch.autograd.grad(out.sum() + last.sum(), leaves)])
+            with torch.no_grad():
+                results[-1].append(hip_gated_delta(*leaves, *(g.expand(batch, 1, HV) for g in gates))[0])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+    for token in range(9):
+        q, k, v = rows[:, token : token + 1, :width].split([H * K, H * K, HV * V], -1)
+        both([q.view(1, 1, H, K), k.view(1, 1, H, K), v.view(1, 1, HV, V)])
+    far = torch.randn(2 * 2 * H * K + 2 * HV * V, generator=gen).to(dtype).cuda()
+    parts = far.split([2 * H * K, 2 * H * K, 2 * HV * V])
+    both([t.as_strided((2, 1, heads, size), (heads * size, 1 << 23, size, 1), t.storage_offset())
+          for t, heads, size in zip(parts, (H, H, HV), (K, K, V))])
