@@ -20,7 +20,8 @@ namespace rglru {
 constexpr int kDeltaChunk = 64;              // tokens of a chunk
 constexpr int kDeltaThreads = 256;
 constexpr int kDeltaMaxKey = 128;            // widest key that the kernels take
-constexpr int kDeltaGates = 136;             // floats per chunk of the gate record: rho[64], w[64], 64 bits that say which tokens count, padding
+// Floats per chunk of the gate record: rho[64], w[64] (zeros for tokens that do not count), four words of facts (ChunkFacts), padding
+constexpr int kDeltaGates = 136;
 constexpr float kDeltaCut = -1e4f;           // a log decay below this discards the history (exp of it is 0 in any type)
 
 // States and solved values of a whole pass that the caches would not hold until they are read again are not kept there (`past` below:
@@ -253,6 +254,7 @@ struct DeltaArgs {
   // `through`, [heads][segments][padded K in][padded K out]
   float *local, *edges;              // what a segment adds to the state (or its gradient); the state a segment starts from
   void* through;                     // what a segment makes of the state it starts from, as an operand
+  int* cut;                          // [heads][segments]: whether a segment leaves nothing of that state
   int segments, length, past;
   long long q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
   int B, T, H, HV, K, V, nC, columns;       // columns: V in whole tiles of 16
@@ -482,10 +484,21 @@ RGLRU_DEVICE void phase() { __builtin_amdgcn_sched_barrier(0); }
 // Four rows of each of the tiles 2 p and 2 p + 1 from an array of 64 numbers.
 RGLRU_DEVICE f32x4 tile_rows(const float* a, int mt, int g) { return *reinterpret_cast<const f32x4*>(a + 32 * (mt >> 1) + 8 * g + 4 * (mt & 1)); }
 
-RGLRU_DEVICE unsigned long long counts_of(const float* record) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane(__float_as_uint(record[128])), hi = __builtin_amdgcn_readfirstlane(__float_as_uint(record[129]));
-  return (unsigned long long)lo | (unsigned long long)hi << 32;
-}
+// What a gate record says about its chunk.  Where the first token that counts starts a document (`fresh`), the chunk reads nothing of the state
+// in front of it and hands no gradient back; where no token counts, both pass by.  Whatever they hold: a factor of zero would keep a NaN.
+struct ChunkFacts {
+  unsigned long long counts;         // tokens that count, a bit each
+  bool fresh, plain;                 // plain: all of them count, and not fresh
+  float carry;                       // what the chunk leaves of the state in front of it
+  RGLRU_DEVICE explicit ChunkFacts(const float* record) {
+    const f32x4 words = *reinterpret_cast<const f32x4*>(record + 128);
+    const unsigned lo = __builtin_amdgcn_readfirstlane(__float_as_uint(words[0])), hi = __builtin_amdgcn_readfirstlane(__float_as_uint(words[1]));
+    counts = (unsigned long long)lo | (unsigned long long)hi << 32;
+    fresh = __builtin_amdgcn_readfirstlane(__float_as_uint(words[2])) != 0;
+    carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(words[3])));
+    plain = counts == ~0ull && !fresh;
+  }
+};
 
 // Whether a walk's workgroups are of two waves with two chunks' tiles in LDS (`two`: they fit) instead of four waves with one: where there
 // are so few that each has a compute unit to itself and the time a chunk takes is all that counts.

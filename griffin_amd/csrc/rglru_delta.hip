@@ -90,15 +90,17 @@ template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads, sizeo
   rows(keys, p.k_t, 16 * wave + c, ki);
   rows(queries, p.q_t, 16 * wave + c, qi);
   const ChunkGates gate = chunk_gates(p, b, hv, n, lane);
-  const unsigned long long counts = __ballot(gate.counts);
+  const unsigned long long counts = __ballot(gate.counts), starts = __ballot(gate.starts);
   if (wave == 0) {
     total[lane] = gate.total;
     beta[lane] = gate.beta;
     segment[lane] = gate.segment;
     float* record = p.gates + chunk * kDeltaGates;
-    record[lane] = gate.segment == 0 ? expf((float)gate.total) : 0.f;
+    record[lane] = gate.counts && gate.segment == 0 ? expf((float)gate.total) : 0.f;
     record[64 + lane] = gate.segment == gate.segments ? gate.beta * expf((float)(gate.end - gate.total)) : 0.f;
     if (lane < 2) record[128 + lane] = __uint_as_float((unsigned)(counts >> (32 * lane)));
+    if (lane == 2) record[130] = (starts & (0 - counts) & counts) != 0 ? 1.f : 0.f;
+    if (lane == 3) record[131] = gate.segments == 0 ? expf((float)gate.end) : 0.f;
   }
   mask(ki, (counts >> (16 * wave + c)) & 1);
   mask(qi, (counts >> (16 * wave + c)) & 1);
@@ -222,6 +224,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
   tiles.setup(p, tid, (const IO*)p.v + b * p.v_b + hv * p.v_h + group * COLUMNS, p.v_t, unit ? 0 : p.value_width - group * COLUMNS, first + begin,
               begin, b, h, 1);
   const bool vectors = p.value_width == p.V;
+  bool cut = false;                                        // some chunk leaves nothing of the state
   f32x4 state[2 * KS], o[4], z[4];
   Wide zw[2];
   WaveRows<IO, COLUMNS> rows_out;
@@ -277,9 +280,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
     const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
              *within = (const IO*)(tile + Tiles::kWithin);
     const float* record = (const float*)(tile + Tiles::kRecord);
-    const unsigned long long counts = counts_of(record);
-    if (counts != ~0ull) {
-      Tiles::clear_rows(tile, counts, tid);
+    const ChunkFacts facts(record);
+    const float carry = facts.carry;
+    if (!OUT) cut = cut || carry == 0.f;
+    if (!facts.plain) {
+      if (facts.fresh) {
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      Tiles::clear_rows(tile, facts.counts, tid);
       lds_barrier();
     }
     if (STAGES == 2 && n > begin) put(n - 1);
@@ -311,7 +320,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g);
       IO* const value_tile = (IO*)(tile + Tiles::kValues);
-      const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
       // K S and Q S (o) side by side: a tile of the state becomes an operand once
       f32x4 acc[4] = {};
 #pragma unroll
@@ -338,8 +346,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
         for (int mt = 0; mt < 4; ++mt) r[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       phase();
-      // where nothing is carried into a document, nothing of it is read either, whatever it is
-      if (carry == 0.f) {
+      // what a masked token would read, whatever it is
+      if (!facts.plain) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -364,13 +372,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       if (OUT && D == 2) square(within, 0);
       phase();
       // S' = rho_63 S + K^T (w Z)
-      if (carry == 0.f) {
 #pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) state[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) state[t] *= carry;
-      }
+      for (int t = 0; t < 2 * KS; ++t) state[t] *= carry;
       M::ew(state, kt[0], M::wide(z[0] * tile_rows(record + 64, 0, g), z[1] * tile_rows(record + 64, 1, g)));
       phase();
       if (D == 1) turned(1);
@@ -401,6 +404,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       IO* at = (IO*)p.through + (((long long)head * p.segments + segment) * PL * DK + col) * DK;
 #pragma unroll
       for (int t = 0; t < 2 * KS; ++t) M::put(at + tile_index(t, 4 * g), DK * DK, state[t]);
+      if (group == value_groups && tid == 0) p.cut[(long long)head * p.segments + segment] = cut;
     } else if (mine) {
       float* at = p.local + (((long long)head * p.segments + segment) * p.columns + col) * DK;
 #pragma unroll
@@ -418,7 +422,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
 }
 
 // The states that segments start from: S' = L + M S with what a segment adds (`local`) and makes of its state (`through`, [in][out]).
-// BACKWARD: the gradients behind the segments, dS = L + M^T dS'.  A wave owns 16 columns again; M goes to LDS a segment ahead.
+// BACKWARD: the gradients behind the segments, dS = L + M^T dS'.  A wave owns 16 columns again; M goes to LDS a segment ahead.  Where a
+// segment leaves nothing of its state (`cut`: a document starts in it), S' = L without the product, whatever S holds.
 template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDeltaThreads) void delta_join_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Wide Wide;
@@ -440,7 +445,9 @@ template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDelt
     load.request(delta_rsrc((const IO*)p.through + ((long long)head * p.segments + s) * (PL * DK * DK), Load::kBytes), lds0 + (unsigned)(stage * Load::kBytes), wave);
   };
   f32x4 state[2 * KS], next[2 * KS];
+  int next_cut = 0;
   auto added = [&](int s) {
+    next_cut = p.cut[(long long)head * p.segments + s];
     const float* at = p.local + (((long long)head * p.segments + s) * p.columns + (mine ? col : 0)) * DK;
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t) next[t] = *reinterpret_cast<const f32x4*>(at + tile_index(t, 4 * g));
@@ -466,17 +473,20 @@ template <typename IO, int KS, bool BACKWARD> __global__ __launch_bounds__(kDelt
     wait_for_all();
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t) sum[t] = next[t];
+    const bool passes = __builtin_amdgcn_readfirstlane(next_cut) == 0;
     if (s + step != to) request(s + step, stage ^ 1), added(s + step);
     const IO* through = (const IO*)(lds + stage * Load::kBytes);
+    if (passes) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const Wide x = M::wide(state[2 * ks], state[2 * ks + 1]);
-      Wide a[2 * KS];
+      for (int ks = 0; ks < KS; ++ks) {
+        const Wide x = M::wide(state[2 * ks], state[2 * ks + 1]);
+        Wide a[2 * KS];
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t)
-        a[t] = BACKWARD ? Square::wide_along_row(through, DK * DK, tile_index(t, c), 32 * ks, g) : Square::wide_down_rows_tile(through, DK * DK, 32 * ks, t, lane);
-      M::template ww<0, 2 * KS>(sum, a, x);
-      phase();
+        for (int t = 0; t < 2 * KS; ++t)
+          a[t] = BACKWARD ? Square::wide_along_row(through, DK * DK, tile_index(t, c), 32 * ks, g) : Square::wide_down_rows_tile(through, DK * DK, 32 * ks, t, lane);
+        M::template ww<0, 2 * KS>(sum, a, x);
+        phase();
+      }
     }
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t) state[t] = sum[t];

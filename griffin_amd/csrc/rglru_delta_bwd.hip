@@ -100,9 +100,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
     const IO *keys = (const IO*)(tile + Tiles::kKeys), *queries = (const IO*)(tile + Tiles::kQueries), *solve = (const IO*)(tile + Tiles::kSolve),
              *within = (const IO*)(tile + Tiles::kWithin);
     const float* record = (const float*)(tile + Tiles::kRecord);
-    const unsigned long long counts = counts_of(record);
-    if (counts != ~0ull) {
-      Tiles::clear_rows(tile, counts, tid);
+    const ChunkFacts facts(record);
+    const float carry = facts.carry;
+    if (!facts.plain) {
+      Tiles::clear_rows(tile, facts.counts, tid);
       lds_barrier();
     }
     if (STAGES == 2 && !LOCAL && n != last) put(n + 1);
@@ -130,7 +131,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       IO* const up_tile = (IO*)(tile + Tiles::kValues);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) rho[mt] = tile_rows(record, mt, g);
-      const float carry = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(record[63])));
       // dZ = P^T dO + w K dS'
       f32x4 dz[4] = {};
       const rsrc_t saved = matrix(p.dstates, n, LOCAL ? 0 : DK);
@@ -150,6 +150,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       for (int ks = 0; ks < 2; ++ks) {
         uf[ks] = Values::down_rows(up_tile, 32 * ks, 16 * wave, lane);
         M::apart(uf[ks], up[2 * ks], up[2 * ks + 1]);
+      }
+      // what a masked token would receive, whatever it is
+      if (!facts.plain) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          const f32x4 w = tile_rows(record + 64, mt, g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dz[mt][e] = w[e] == 0.f ? 0.f : dz[mt][e];
+        }
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) dz[mt] *= tile_rows(record + 64, mt, g), up[mt] *= rho[mt] * p.scale;
@@ -188,6 +197,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
       M::ew(dstate, kt[1 % D], M::wide(-rho[2] * y[2], -rho[3] * y[3]));
       if (vectors && !LOCAL) rows_out.turn(up_tile, y, wave, lane);
       phase();
+      if (facts.fresh) {
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) dstate[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
     }
     if (STAGES == 1) {
       lds_barrier();                                       // the tiles have been read
@@ -257,6 +270,21 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
   if (work < 0) return;
   const int h = work % p.H, n = work / p.H % p.nC, b = work / p.H / p.nC;
   const int t0 = n * kDeltaChunk, left = p.T - t0, share = p.HV / p.H;
+  if (p.flags) {                                            // no token counts: zeros, whatever state and gradient pass by
+    const int t = t0 + (tid & 63);
+    if (__ballot(t < p.T && !(p.flags[(long long)b * p.T + (t < p.T ? t : 0)] & 2u)) == 0) {
+      const int rows = left < kDeltaChunk ? left : kDeltaChunk;
+      for (int row = wave; row < rows; row += THREADS / 64) {
+        const long long token = (long long)b * p.T + t0 + row;
+        for (int i = tid & 63; i < p.K; i += 64) ((IO*)p.dq)[(token * p.H + h) * p.K + i] = ((IO*)p.dk)[(token * p.H + h) * p.K + i] = (IO)0.f;
+        for (int s = tid & 63; s < share; s += 64) {
+          delta_put_gate(p.dlog_decay, token * p.HV + h * share + s, p.decay_dtype, 0.f);
+          delta_put_gate(p.dbeta, token * p.HV + h * share + s, p.beta_dtype, 0.f);
+        }
+      }
+      return;
+    }
+  }
   IO *const keys = (IO*)lds, *const queries = (IO*)(lds + KeyLoad::kBytes), *const area = (IO*)(lds + 2 * KeyLoad::kBytes);
   const unsigned lds0 = lds_address(lds);
   f32x4 all_dq[KS] = {}, all_dk[KS] = {};                   // over the value heads that share the key head

@@ -172,7 +172,7 @@ static void delta_segments(int64_t heads, int64_t columns, int64_t nC, int64_t w
 struct DeltaSizes {
   int64_t chunks, columns, width, row, value_row;          // rows: elements of a key and of a value as the kernels read them
   size_t gates, solve, within, q, k, v, states, values, total;  // offsets in the workspace; q, k, v: room where rows have to be padded
-  size_t padded_v, through, local, edges, segment_states;
+  size_t padded_v, through, local, edges, cut, segment_states;
   int64_t segments, length;
   DeltaSizes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, bool keep) {
     const int64_t e = dtype == RGLRU_BF16 ? 8 : 4;
@@ -197,7 +197,8 @@ struct DeltaSizes {
     segment_states = segments > 1 ? up((size_t)(B * HV * segments * columns * width) * 4) : 0;
     local = through + (segments > 1 ? up((size_t)(B * HV * segments * width * width) * 4) : 0);
     edges = local + segment_states;
-    total = edges + segment_states;
+    cut = edges + segment_states;
+    total = cut + (segments > 1 ? up((size_t)(B * HV * segments) * sizeof(int)) : 0);
   }
   size_t scratch_values() const { return ((size_t)chunks * columns * width * 4 + 255) & ~(size_t)255; }
   size_t scratch_up() const { return scratch_values() + (((size_t)chunks * columns * 64 * 4 + 255) & ~(size_t)255); }
@@ -245,7 +246,7 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   a.segments = (int)z.segments, a.length = (int)z.length;
   a.past = z.chunks * z.columns * (z.width + 64) * 4 > kCachedBytes;
   char* base = (char*)ws;
-  a.through = base + z.through, a.local = (float*)(base + z.local), a.edges = (float*)(base + z.edges);
+  a.through = base + z.through, a.local = (float*)(base + z.local), a.edges = (float*)(base + z.edges), a.cut = (int*)(base + z.cut);
   a.gates = (float*)(base + z.gates);
   a.solve = base + z.solve, a.within = base + z.within;
   if (keep) a.states = base + z.states, a.values = base + z.values;

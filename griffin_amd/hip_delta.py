@@ -30,7 +30,9 @@ def hip_gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Te
 
     ``reset_mask`` [B, T]: tokens that start a document (the history in front of them is discarded).  ``active_mask`` [B, T]: tokens
     that count; the others leave the state as it is, give zeros and receive zero gradients, whatever they hold.  Among the
-    active tokens a NaN or an infinity may reach all outputs of its chunk of 64 tokens, and those behind it.
+    active tokens a NaN or an infinity may reach all outputs of its chunk of 64 tokens and those behind it, in gradients those in front
+    of it.  Where the first active token of a chunk starts a document, the chunk takes nothing from what lies in front of it, a
+    state of NaN included, and hands no gradient on to it.
 
     Products are exact to fp32 for float32 operands and to 2^-17 for what is computed between them from bfloat16 ones, relative to their terms:
     what the keys of a chunk all but erase (the gradient of ``h0`` behind many parallel keys) is known to that part of what it was, not

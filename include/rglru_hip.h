@@ -384,7 +384,8 @@ int rglru_hip_rmsnorm_bwd(const void* x, const void* g, const float* inv, const 
  *   ws       rglru_hip_gated_delta_workspace_bytes(.., keep) bytes, 16-byte aligned.  With keep != 0 the forward call leaves there what
  *            the backward call needs, which changes none of it: any number of backward calls may follow.
  *   scratch  rglru_hip_gated_delta_scratch_bytes(..) bytes of the backward call's own, 16-byte aligned.
- * Tokens are taken in chunks of 64: a NaN or an infinity in an active token may reach every output of its chunk.
+ * Tokens are taken in chunks of 64: a NaN or an infinity in an active token may reach every output of its chunk and behind it (gradients:
+ * in front of it).  Where the first active token of a chunk is a reset, nothing crosses, whatever it is: a state that holds NaN, a gradient.
  * The step takes one token a row (no T axis, everything dense) and updates `state` in place; inactive rows keep theirs. */
 int rglru_hip_gated_delta_max_key_size(void);
 size_t rglru_hip_gated_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int dtype, int keep);

@@ -518,3 +518,62 @@ def test_axes_of_one_element_may_have_any_stride(dtype):
     parts = far.split([2 * H * K, 2 * H * K, 2 * HV * V])
     both([t.as_strided((2, 1, heads, size), (heads * size, 1 << 23, size, 1), t.storage_offset())
           for t, heads, size in zip(parts, (H, H, HV), (K, K, V))])
+
+
+@pytest.mark.parametrize("skipped", [0, 5, 64, 70])
+@pytest.mark.parametrize("shape", [(2, 130, 1, 2, 64, 48), (1, 300, 2, 2, 128, 64), (1, 1500, 1, 1, 64, 40)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_a_first_document_discards_whatever_state_there_is(shape, skipped, dtype):
+    """A recycled state in front of a document start, padding between them or not, walked in one or in segments."""
+    case = make(*shape, dtype=dtype)
+    B, T = shape[:2]
+    active = (torch.arange(T) >= skipped).expand(B, T) if skipped else None
+    reset = torch.zeros(B, T, dtype=torch.bool)
+    reset[:, skipped] = True
+    case["h0"] = torch.zeros_like(case["h0"])
+    want = run(hip_gated_delta, case, reset, active, "cuda")
+    for value in (float("nan"), float("inf")):
+        case["h0"] = torch.full_like(case["h0"], value)
+        got = run(hip_gated_delta, case, reset, active, "cuda")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for name in NAMES:
+            assert torch.equal(got[2][name], want[2][name]), name
+        with torch.no_grad():
+            put = lambda t: None if t is None else t.cuda()
+            out, last = hip_gated_delta(*(case[n].cuda() for n in NAMES), reset_mask=put(reset), active_mask=put(active))
+            assert rel_err(out, want[0]) <= 2 * OUT[dtype] and rel_err(last, want[1]) <= 2 * STATE[dtype]
+
+
+@pytest.mark.parametrize("shape, start", [((2, 190, 1, 2, 64, 48), 64), ((1, 1500, 1, 1, 64, 40), 704), ((1, 1500, 1, 1, 128, 64), 128)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_chunks_in_front_of_a_document_receive_nothing_from_it(shape, start, dtype):
+    """A document that starts a chunk: its gradients, whatever they are, end there."""
+    case = make(*shape, dtype=dtype)
+    reset = torch.zeros(*shape[:2], dtype=torch.bool)
+    reset[:, start] = True
+    want = run(hip_gated_delta, case, reset, None, "cuda")[2]
+    for value in (float("nan"), float("inf")):
+        case["up"] = case["up"].clone()
+        case["up"][:, start:] = value
+        case["up_state"] = torch.full_like(case["up_state"], value)
+        got = run(hip_gated_delta, case, reset, None, "cuda")[2]
+        assert torch.equal(got["h0"], want["h0"])
+        for name in NAMES[:5]:
+            assert torch.equal(got[name][:, :start], want[name][:, :start]), name
+
+
+@pytest.mark.parametrize("shape", [(2, 130, 1, 2, 64, 48), (1, 1500, 1, 1, 64, 40)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_rows_without_tokens_keep_whatever_state_they_have(shape, dtype):
+    case = make(*shape, dtype=dtype)
+    active = torch.zeros(*shape[:2], dtype=torch.bool)
+    for value in (None, float("nan"), float("inf")):
+        if value is not None:
+            case["h0"] = torch.full_like(case["h0"], value)
+        out, last, grads = run(hip_gated_delta, case, None, active, "cuda")
+        assert not out.any() and all(not grads[name].any() for name in NAMES[:5])
+        assert rel_err(grads["h0"], case["up_state"]) <= STATE_GRAD[dtype]
+        assert rel_err(last, case["h0"]) <= STATE[dtype] if value is None else not last.isfinite().any()
+    case["up_state"] = torch.full_like(case["up_state"], float("nan"))
+    grads = run(hip_gated_delta, case, None, active, "cuda")[2]
+    assert all(not grads[name].any() for name in NAMES[:5]) and grads["h0"].isnan().all()
