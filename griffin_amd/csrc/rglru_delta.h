@@ -104,6 +104,10 @@ template <> struct Mx<__bf16> {
     *reinterpret_cast<bf16x4*>(at) = hi;
     *reinterpret_cast<bf16x4*>(at + plane) = lo;
   }
+  static RGLRU_DEVICE f32x4 get(const __bf16* at, long long plane) {
+    const bf16x4 hi = *reinterpret_cast<const bf16x4*>(at), lo = *reinterpret_cast<const bf16x4*>(at + plane);
+    return f32x4{(float)hi[0] + (float)lo[0], (float)hi[1] + (float)lo[1], (float)hi[2] + (float)lo[2], (float)hi[3] + (float)lo[3]};
+  }
   // the eight consecutive elements that an operand holds; `at` and `plane` in bytes
   static RGLRU_DEVICE void put(rsrc_t r, unsigned at, unsigned plane, const Wide& w, bool past) {
     const i32x4 hi = __builtin_bit_cast(i32x4, w.hi), lo = __builtin_bit_cast(i32x4, w.lo);
@@ -147,6 +151,7 @@ template <> struct Mx<float> {
   static RGLRU_DEVICE Wide wide(f32x4 a, f32x4 b) { return {a, b}; }
   static RGLRU_DEVICE void apart(const Frag& f, f32x4& a, f32x4& b) { a = f.lo, b = f.hi; }
   static RGLRU_DEVICE void put(float* at, long long, f32x4 v) { *reinterpret_cast<f32x4*>(at) = v; }
+  static RGLRU_DEVICE f32x4 get(const float* at, long long) { return *reinterpret_cast<const f32x4*>(at); }
   static RGLRU_DEVICE void put(rsrc_t r, unsigned at, unsigned, const Wide& w, bool past) {
     const i32x4 first = __builtin_bit_cast(i32x4, w.lo), second = __builtin_bit_cast(i32x4, w.hi);
     if (past) {

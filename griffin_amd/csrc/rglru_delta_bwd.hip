@@ -5,10 +5,13 @@
 //   N1 = scale tril(D . dO Z^T)      N2 = -stril(D . Y Z^T)
 //   dQ = scale rho dO S^T + (N1 beta) K          dK = E + beta F,  dbeta = k . F
 //   E  = -rho Y S^T + (N2 beta) K                F  = N1^T Q + N2^T K + e^(G_63 - G) Z dS'^T
-//   dG = q . dQ + k . E - beta dbeta             dlog_decay_t = sum of dG from t on + rho_63 <S, dS'> + sum over j of beta_j k_j . (last term of F)_j
-// (a factor e^(G_i) goes with everything that token i reads, e^(-G_j) with everything that token j writes, so the gradients of the
-// running log decay are products that are there already).  The first kernel walks back along the chunks with dS' as the
-// forward pass walks with S; the second one has no order: a workgroup a chunk and key head, which adds up its value heads.
+//   dlog_decay_t = sum over i >= t of (scale rho q dO S^T - rho k Y S^T)_i + rho_63 <S, dS'> + sum over j < t of beta_j k_j . e^(G_63 - G_j) (Z dS'^T)_j
+//                  + sum over i >= t > j of beta_j (N1_ij q_i + N2_ij k_i) . k_j
+// (everything that decays by token t: what is read behind it of what was written in front of it.  Sums over all that a token reads less all that it
+// writes would be the same, but their common terms do not cancel to the last bit: what little crosses a strong decay would drown in them, and a
+// document's gradient in its neighbours'.  The price is the products of all keys with queries and keys once more: 8 us of the step below.)
+// The first kernel walks back along the chunks with dS' as the forward pass walks with S; the second one has no order: a workgroup a chunk and
+// key head, which adds up its value heads.
 // B8 T2048, 8 heads of 128 x 128 in bf16: 157 + 156 us.  The walk is bound like the forward one.  The second kernel reads what both walks left,
 // 490 MB, and takes 112 us with its loads alone, 58 with its products over the columns alone: it is bound by memory in front and by
 // what each workgroup does behind its last column, where nothing is loaded.
@@ -236,6 +239,26 @@ RGLRU_DEVICE float sixteen_sum(float v) {
   return v;
 }
 
+// Sum over the lanes in front, of the same sixteen.
+template <int N> RGLRU_DEVICE float sixteen_shift(float v) {  // N lanes up, zeros behind
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x110 | N, 0xf, 0xf, true));
+}
+RGLRU_DEVICE float sixteen_in_front(float v) {
+  v = sixteen_shift<1>(v);
+  v += sixteen_shift<1>(v);
+  v += sixteen_shift<2>(v);
+  v += sixteen_shift<4>(v);
+  v += sixteen_shift<8>(v);
+  return v;
+}
+// Sum over the four lanes of a column: rows of sixteen exchanged in pairs, then halves of the wave.
+RGLRU_DEVICE float four_rows_sum(float v) {
+  const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+}
+
 // Gradients of queries, keys and gates of one chunk and key head.  Eight waves: four times 16 tokens, by two halves of the key's
 // columns; the first half's waves make N1, the second half's N2.  The contractions over the value columns take 32 of them at a time
 // through LDS, the next 32 on their way there where two fit; queries, keys, N1 and N2 come where the columns lay.
@@ -258,11 +281,11 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
   typedef TileLoad<IO, CB, DK, THREADS> StateLoad;
   constexpr int kUp = 0, kValues = kUp + UpLoad::kBytes, kDValues = kValues + PL * ValueLoad::kBytes, kStates = kDValues + PL * ValueLoad::kBytes,
                 kDStates = kStates + PL * StateLoad::kBytes, kStage = kDStates + PL * StateLoad::kBytes, kRows = 2 * KeyLoad::kBytes + 2 * PL * 4096 * (int)sizeof(IO);
-  constexpr int STAGES = 2 * kStage + 4096 <= (kGradShared<IO, GROUPED> ? 80 : 160) * 1024 ? 2 : 1;
+  constexpr int STAGES = 2 * kStage + 6144 <= (kGradShared<IO, GROUPED> ? 80 : 160) * 1024 ? 2 : 1;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * kStage > kRows ? STAGES * kStage : kRows];
   __shared__ double total[64];
-  __shared__ float beta[64], to_end[64], reads[2][64], writes[2][64], leaves[2][64], sums[8];
-  __shared__ int segment[64], held[8];
+  __shared__ float beta[64], to_end[64], reads[2][64], writes[2][64], leaves[2][64], sums[8], crossing[2][64], columns_of[8][48];
+  __shared__ int segment[64];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
   // the heads of a chunk side by side: what they read and write lies side by side
@@ -330,7 +353,6 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     }
     f32x4 dq[KS] = {}, dr[KS] = {}, dw[KS] = {}, pairs[4] = {};
     float carried = 0.f;                                   // <S, dS'>
-    bool some = false;                                     // S is not all zeros
     wait_for_all();
     for (int c0 = 0; c0 < p.columns; c0 += CB) {
       const int stage = STAGES == 2 ? (c0 / CB) & 1 : 0;
@@ -370,11 +392,10 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
 #pragma unroll
           for (int e = 0; e < Keys::E; ++e) {
             carried = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], carried);
-            some = some || !((float)a[e] == 0.f);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e], (float)d[e], carried), some = some || !((float)a[e] == 0.f);
+          for (int e = 0; e < Keys::E; ++e) carried = fmaf((float)a[e], (float)d[e], carried);
         }
       }
       if (STAGES == 1 && c0 + CB < p.columns) {
@@ -409,8 +430,7 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) carried += __shfl_xor(carried, m, 64);
-    const bool wave_some = __ballot(some) != 0;
-    if (lane == 0) sums[wave] = carried, held[wave] = wave_some;
+    if (lane == 0) sums[wave] = carried;
     auto put_pairs = [&](bool strengths) {                 // kept [j][i]; blocks above the diagonal that a product touches are zeros
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
@@ -427,14 +447,23 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
       lds_barrier();
     }
     {
-      f32x4 dot = {};
+      int lane = tid & 63;                                 // addresses anew: there are no registers to keep them in
+      asm("" : "+v"(lane) : "s"(n));
+      const int c = lane & 15, g = lane >> 4, row0 = 16 * block + 4 * g;
+      f32x4 read = {}, dot = {};                           // of the state in front of the chunk; of the one behind it
 #pragma unroll
-      for (int t = 0; t < KS; ++t) dot += dw[t] * Keys::accumulator_tile(keys, 16 * block, 16 * (half * KS + t), lane);
+      for (int t = 0; t < KS; ++t) {
+        const f32x4 k = Keys::accumulator_tile(keys, 16 * block, 16 * (half * KS + t), lane);
+        read += Keys::accumulator_tile(queries, 16 * block, 16 * (half * KS + t), lane) * dq[t] + k * dr[t];
+        dot += dw[t] * k;
+        phase();
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float sum = sixteen_sum(dot[e]);
-        if (c == 0) leaves[half][row0 + e] = beta[row0 + e] * sum;
+        const float from = sixteen_sum(read[e]), sum = sixteen_sum(dot[e]);
+        if (c == 0) reads[half][row0 + e] = from, leaves[half][row0 + e] = beta[row0 + e] * sum;
       }
+      phase();
     }
     // F = N1^T Q + N2^T K + ...: pairs in which the wave's tokens are the written ones
     for (int ks = block >> 1; ks < 2; ++ks) {
@@ -461,13 +490,12 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
         phase();
       }
     }
-    f32x4 read = {}, written = {}, strength;
+    f32x4 written = {}, strength;
 #pragma unroll
     for (int e = 0; e < 4; ++e) strength[e] = beta[row0 + e];
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
       const f32x4 k = Keys::accumulator_tile(keys, 16 * block, 16 * (half * KS + t), lane);
-      read += Keys::accumulator_tile(queries, 16 * block, 16 * (half * KS + t), lane) * dq[t] + k * dr[t];
       written += k * dw[t];
       dr[t] += strength * dw[t];
       all_dq[t] = GROUPED ? all_dq[t] + dq[t] : dq[t];
@@ -475,28 +503,74 @@ __global__ __launch_bounds__(kGradThreads, (kGradShared<IO, GROUPED>) ? 4 : 2) v
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float from = sixteen_sum(read[e]), back = sixteen_sum(written[e]);
-      if (c == 0) reads[half][row0 + e] = from, writes[half][row0 + e] = back;
+      const float back = sixteen_sum(written[e]);
+      if (c == 0) writes[half][row0 + e] = back;
+    }
+    // pairs across each token: N1 with q_i . k_j, N2 with k_i . k_j; the wave reads what it has put there itself.  Of its sixteen rows, for its
+    // own sixteen tokens t the sums over i >= t as a product with a triangle of ones, then over j < t; for tokens in front of them
+    // all rows, column by column, and the sums over j < t.
+    {
+      int lane = tid & 63;
+      asm("" : "+v"(lane) : "s"(n));
+      const int c = lane & 15, g = lane >> 4, row0 = 16 * block + 4 * g;
+      float earlier = 0.f;
+      f32x4 before = {}, own = {};                         // columns in front of the wave's tokens, added up; its own
+      const IO* const rows = half == 0 ? queries : keys;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+        if (jt <= block) {
+          f32x4 w = {};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) w = M::ee(Keys::along_row(rows, 16 * block + c, 32 * ks, g), Keys::along_row(keys, 16 * jt + c, 32 * ks, g), w);
+          const f32x4 pair = M::get(area + half * PL * 4096 + Square::at(16 * jt + c, row0), 4096);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pair[e] == 0.f ? 0.f : pair[e] * w[e];
+          if (jt < block) {
+            before += w;
+            const float sum = four_rows_sum((w[0] + w[1]) + (w[2] + w[3]));
+            const float in_front = sixteen_in_front(sum);
+            if (g == 0) columns_of[wave][16 * jt + c] = earlier + in_front;
+            earlier += sixteen_sum(sum);
+          } else {
+            own = w;
+          }
+          phase();
+        }
+      f32x4 in_front = {}, among = {};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float one = 4 * g + e >= c ? 1.f : 0.f;
+        in_front = __builtin_amdgcn_mfma_f32_16x16x4f32(one, before[e], in_front, 0, 0, 0);
+        among = __builtin_amdgcn_mfma_f32_16x16x4f32(one, own[e], among, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float sum = sixteen_sum(in_front[e] + (c < 4 * g + e ? among[e] : 0.f));
+        if (c == 0) crossing[half][row0 + e] = sum;
+      }
+      phase();
     }
     __syncthreads();
-    if (wave == 0) {                                       // sums from each token to the chunk's end
+    if (wave == 0) {                                       // what crosses each token
       const float written = writes[0][lane] + writes[1][lane];
-      float write = leaves[0][lane] + leaves[1][lane], from = (reads[0][lane] + reads[1][lane]) - beta[lane] * written;
-#pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) write += __shfl_xor(write, m, 64);
+      // read from the token on; written in front of it: for the state behind the chunk, for tokens of the second, third and last sixteen
+      float from = reads[0][lane] + reads[1][lane], to = leaves[0][lane] + leaves[1][lane];
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const float other = __shfl_down(from, d, 64);
         if (lane + d < 64) from += other;
+        const float before = __shfl_up(to, d, 64);
+        if (lane >= d) to += before;
       }
-      float across = 0.f;
-      int history = 0;
+      to = __shfl_up(to, 1, 64);
+      float across = 0.f, pairs_across = (crossing[0][lane] + crossing[1][lane]) + (lane > 0 ? to : 0.f);
 #pragma unroll
-      for (int w = 0; w < THREADS / 64; ++w) across += sums[w], history |= held[w];
+      for (int w = 0; w < THREADS / 64; ++w) across += sums[w];
       across = carry == 0.f ? 0.f : carry * across;
-      // a first token has nothing to decay: zero, and not what is left of sums that cancel
-      const bool first = history == 0 && (counts & ((1ull << lane) - 1)) == 0;
-      const float d = gate.counts && !gate.starts && !first ? from + (write + across) : 0.f;
+#pragma unroll
+      for (int i = 1; i < 4; ++i)
+        if (lane < 16 * i) pairs_across += columns_of[i][lane] + columns_of[4 + i][lane];
+      const float d = gate.counts && !gate.starts ? from + (across + pairs_across) : 0.f;
       const long long at = ((long long)b * p.T + t0 + lane) * p.HV + hv;
       if (lane < left) {
         delta_put_gate(p.dlog_decay, at, p.decay_dtype, d);

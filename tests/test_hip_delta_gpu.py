@@ -577,3 +577,51 @@ def test_rows_without_tokens_keep_whatever_state_they_have(shape, dtype):
     case["up_state"] = torch.full_like(case["up_state"], float("nan"))
     grads = run(hip_gated_delta, case, None, active, "cuda")[2]
     assert all(not grads[name].any() for name in NAMES[:5]) and grads["h0"].isnan().all()
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (1, 3)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_documents_of_a_chunk_do_not_share_decay_gradients(dtype, heads):
+    """A document without an upstream gradient has none of its decays, to the last bit."""
+    T, starts = 128, (20, 41, 100)
+    case = make(2, T, *heads, 64, 48, dtype=dtype)
+    reset = torch.zeros(2, T, dtype=torch.bool)
+    reset[:, list(starts)] = True
+    whole, state = case["up"], case["up_state"]
+    edges = (0, *starts, T)
+    for a, b in zip(edges, edges[1:]):
+        case["up"] = whole.clone()
+        case["up"][:, a:b] = 0
+        case["up_state"] = state if b < T else torch.zeros_like(state)
+        grad = run(hip_gated_delta, case, reset, None, "cuda")[2]["log_decay"]
+        assert not grad[:, a:b].any(), (a, b)
+        assert grad.any()
+        check(case, reset)
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (1, 2)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_decay_gradients_where_little_is_left(dtype, heads):
+    """Decays of e^-12 a token: what crosses a token is the write of the one in front of it, 2^-17 of what the tokens exchange with
+    themselves.  A token's gradient is the product of the state that it keeps with that state's gradient and known to what those are
+    known to (STATE, STATE_GRAD) of their norms' product, and to its own rounding."""
+    case = make(2, 100, *heads, 64, 48, dtype=dtype)
+    case["log_decay"] = (case["log_decay"].float() - 12.0).to(dtype)
+    leaves = {n: case[n].double().requires_grad_(n == "log_decay") for n in NAMES}
+    B, T, H, K = case["q"].shape
+    of = torch.arange(heads[1]) // (heads[1] // heads[0])
+    q, k = leaves["q"][:, :, of], leaves["k"][:, :, of]
+    state, outs, kept = leaves["h0"], [], []
+    for t in range(T):
+        kept.append(state * leaves["log_decay"][:, t].exp()[..., None, None])
+        kept[-1].retain_grad()
+        error = leaves["v"][:, t] - (kept[-1] * k[:, t, :, :, None]).sum(2)
+        state = kept[-1] + k[:, t, :, :, None] * (leaves["beta"][:, t, :, None] * error)[:, :, None]
+        outs.append(K ** -0.5 * (state * q[:, t, :, :, None]).sum(2))
+    ((torch.stack(outs, 1) * case["up"].double()).sum() + (state * case["up_state"].double()).sum()).backward()
+    norm = lambda t: t.square().sum((-1, -2)).sqrt()
+    product = torch.stack([norm(s.detach()) * norm(s.grad) for s in kept], 1)
+    want = leaves["log_decay"].grad
+    got = run(hip_gated_delta, case, None, None, "cuda")[2]["log_decay"].cpu().double()
+    limit = (STATE[dtype] + STATE_GRAD[dtype]) * product + (2 ** -8 if dtype == BF16 else 2 ** -24) * want.abs()
+    assert ((got - want).abs() / limit).max() <= 1, float(((got - want).abs() / limit).max())
