@@ -40,6 +40,7 @@ struct GroupArgs {
   int Cg, width;                              // channels of a group; in vectors
   int columns, lines, blocks, per_group;      // many positions: vector columns of a workgroup, positions at a time, column blocks, blocks a group
   int chunks, chunk;                          // chunks of positions, positions in one
+  int rows_apart;                             // many positions: the kernel of the sums goes on rows_apart further
   int lanes, waves;                           // one position: lanes a run, waves of the launch
   float eps, inv_count;
 };
@@ -230,8 +231,11 @@ template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_boun
 }
 
 // ---- many positions -------------------------------------------------------------------------------------------------
-// A workgroup takes a chunk of positions of one row and a block of vector columns: whole groups where 256 vectors hold one, else
+// A workgroup takes a chunk of positions of a row and a block of vector columns: whole groups where 256 vectors hold one, else
 // a part of one group.  Thread (column, line): one vector of every lines-th position.
+// Most workgroups a compute unit of the kernel of the sums: it goes on to further rows and adds their parameter gradients up, of which each workgroup
+// leaves one set.  A million rows of 2 x 64: 33 MiB of scratch instead of 544 and 12.1 ms a training step instead of 19.6.
+constexpr int kGroupSums = 8;
 struct GroupPlace {
   int n, chunk, block, first_group, groups, part;            // groups of the block; part of the group where it is one
   int col, line, c;                                         // c: first channel
@@ -402,20 +406,23 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
   constexpr int U = 4;
   __shared__ TwoSums shared[kGroupThreads];
   __shared__ float lines[2][kGroupThreads * V];
-  const GroupPlace g = group_place<V>(p);
+  GroupPlace g = group_place<V>(p);
   GroupAhead<IO, V, U> next_x, next_up;
   next_x.request(p, g, p.x, g.from);
   next_up.request(p, g, p.dy, g.from);
-  float w[V], dw[V], db[V];
+  float w[V], b[V], all_dw[V], all_db[V];                   // over the workgroup's rows
+  group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
+  group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
 #pragma unroll
-  for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
-  if (g.live) {
-    float b[V];
+  for (int e = 0; e < V; ++e) all_dw[e] = all_db[e] = 0.f;
+  const int row0 = g.n;
+  while (true) {
+    float dw[V], db[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
     const long long group = (long long)g.n * p.G + g.c / p.Cg;
     const float mu = p.stats[2 * group], rs = p.stats[2 * group + 1];
-    group_params<V>(p.weight, g.c, p.vec_dtype, 1.f, w);
-    group_params<V>(p.bias, g.c, p.vec_dtype, 0.f, b);
-    for (int l0 = g.from; l0 < g.to; l0 += U * p.lines) {
+    for (int l0 = g.from; g.live && l0 < g.to; l0 += U * p.lines) {
       float x[U][V], up[U][V];
       next_x.take(x);
       next_up.take(up);
@@ -431,34 +438,39 @@ template <typename IO, int V> __global__ __launch_bounds__(kGroupThreads) void g
             dw[e] = fmaf(t, xhat, dw[e]);
           }
     }
-  } else {
+    TwoSums s = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < V; ++e) w[e] = 0.f;
+    for (int e = 0; e < V; ++e) {
+      s.a = fmaf(w[e], db[e], s.a);
+      s.b = fmaf(w[e], dw[e], s.b);
+      all_dw[e] += dw[e], all_db[e] += db[e];
+    }
+    const int n = g.n;
+    g.n += p.rows_apart;
+    const bool more = g.n < p.N;
+    if (more) next_x.request(p, g, p.x, g.from), next_up.request(p, g, p.dy, g.from);
+    s = group_join(s, TwoSums{0.f, 0.f}, p, g, shared, [](const TwoSums& a, const TwoSums& b) { return TwoSums{a.a + b.a, a.b + b.b}; });
+    const int width = p.per_group > 1 ? p.columns : p.width;
+    if (g.line == 0 && g.col % width == 0 && g.live) {
+      const long long entries = (long long)p.chunks * p.per_group;
+      float* out = p.entries + (((long long)n * p.G + g.first_group + g.col / width) * entries + (long long)g.chunk * p.per_group + g.part) * 2;
+      out[0] = s.a, out[1] = s.b;
+    }
+    if (!more) break;
   }
-  TwoSums s = {0.f, 0.f};
+  if (!p.dweight) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    s.a = fmaf(w[e], db[e], s.a);
-    s.b = fmaf(w[e], dw[e], s.b);
-    lines[0][threadIdx.x * V + e] = dw[e];
-    lines[1][threadIdx.x * V + e] = db[e];
-  }
-  s = group_join(s, TwoSums{0.f, 0.f}, p, g, shared, [](const TwoSums& a, const TwoSums& b) { return TwoSums{a.a + b.a, a.b + b.b}; });
-  const int width = p.per_group > 1 ? p.columns : p.width;
-  if (g.line == 0 && g.col % width == 0 && g.live) {
-    const long long entries = (long long)p.chunks * p.per_group;
-    float* out = p.entries + (((long long)g.n * p.G + g.first_group + g.col / width) * entries + (long long)g.chunk * p.per_group + g.part) * 2;
-    out[0] = s.a, out[1] = s.b;
-  }
-  if (p.dweight && g.line == 0 && g.live) {
-    const long long at = ((long long)g.n * p.chunks + g.chunk) * p.C + g.c;
+  for (int e = 0; e < V; ++e) lines[0][threadIdx.x * V + e] = all_dw[e], lines[1][threadIdx.x * V + e] = all_db[e];
+  __syncthreads();
+  if (g.line == 0 && g.live) {
+    const long long at = ((long long)row0 * p.chunks + g.chunk) * p.C + g.c;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       for (int i = 1; i < p.lines; ++i) {
-        dw[e] += lines[0][(i * p.columns + g.col) * V + e];
-        db[e] += lines[1][(i * p.columns + g.col) * V + e];
+        all_dw[e] += lines[0][(i * p.columns + g.col) * V + e];
+        all_db[e] += lines[1][(i * p.columns + g.col) * V + e];
       }
-      p.dweight[at + e] = dw[e], p.dbias[at + e] = db[e];
+      p.dweight[at + e] = all_dw[e], p.dbias[at + e] = all_db[e];
     }
   }
 }
@@ -526,6 +538,7 @@ struct GroupPlan {
   bool rows;                                                // one position, runs that fit the registers
   int V, slots;
   int64_t sets, entries;                                    // partial parameter gradients; entries of a group
+  int64_t sum_rows;                                         // many positions: rows that the kernel of the sums takes side by side
 };
 static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64_t G, int V, bool backward) {
   GroupPlan plan;
@@ -559,7 +572,9 @@ static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64
   if (chunks < 1) chunks = 1;
   a.chunk = (int)((L + chunks - 1) / chunks);
   a.chunks = (int)((L + a.chunk - 1) / a.chunk);
-  plan.sets = N * a.chunks;
+  const int64_t each = (int64_t)a.chunks * a.blocks, most_sums = (int64_t)num_compute_units() * kGroupSums;
+  plan.sum_rows = each >= most_sums ? 1 : N < most_sums / each ? N : most_sums / each;
+  plan.sets = plan.sum_rows * a.chunks;
   plan.entries = (int64_t)a.chunks * a.per_group;
   return plan;
 }
@@ -673,8 +688,9 @@ int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias
     group_rows<true>(a, plan, dtype, s);
     rc = check_launch("group_norm_bwd");
   } else {
-    const dim3 grid((unsigned)(N * a.chunks * a.blocks));
-    RGLRU_GROUP_LAUNCH(group_norm_sums_kernel, dtype, plan.V, grid, s, a);
+    a.rows_apart = (int)plan.sum_rows;
+    const dim3 sum_grid((unsigned)(plan.sum_rows * a.chunks * a.blocks)), grid((unsigned)(N * a.chunks * a.blocks));
+    RGLRU_GROUP_LAUNCH(group_norm_sums_kernel, dtype, plan.V, sum_grid, s, a);
     rc = check_launch("group_norm_bwd sums");
     if (rc) return rc;
     RGLRU_GROUP_LAUNCH(group_norm_dx_kernel, dtype, plan.V, grid, s, a);

@@ -193,3 +193,18 @@ def test_more_than_two_to_the_31_elements():
     want = hip_group_norm(last, 8)
     (want_grad,) = torch.autograd.grad(want, last, want.detach())
     assert torch.equal(out[-64:], want) and torch.equal(grad[-64:], want_grad)
+
+
+def test_sums_over_many_short_rows():
+    """Gradients of the parameters over a million positions in rows of two.  A thread adds up 147 rows, a workgroup its lines and the last
+    sum 2048 sets in 32 runs of 64: half a step of 2^-24 for each of fewer than 300 additions, all of them to one side for equal terms."""
+    x, weight, bias, up = make((300000, 2, 8))
+    up = torch.full_like(up, 1.1)
+    got = run(hip_group_norm, (x, weight, bias, up), 2, 1e-5, None, "cuda")
+    want = run(definition, (x, weight, bias, up), 2, 1e-5, None, "cpu", torch.float64)
+    assert rel_err(got[3], want[3]) <= 2 ** -16, rel_err(got[3], want[3])
+    # a weight's gradient cancels: its terms are 1.1 times xhat, of deviation 1
+    assert float((got[2].cpu().double() - want[2]).abs().max()) <= 2 ** -16 * 1.1 * 600000
+    assert rel_err(got[1], want[1]) <= 2 ** -12 and rel_err(got[0], want[0]) <= TOLERANCE[F32]
+    case = make((40000, 3, 24), BF16)
+    check(case, 3, "silu")

@@ -194,3 +194,8 @@ def swapped(index, tensor):
 def test_tensors_that_do_not_fit(error, call):
     with pytest.raises(error):
         call()
+
+
+def test_partial_gradients_of_many_short_rows_do_not_outgrow_them(lib):
+    x = 2 * (1 << 20) * 2 * 64                                                  # a million rows of 2 x 64 in bf16
+    assert lib.rglru_hip_group_norm_scratch_bytes(1 << 20, 2, 64, 4, 1) <= x // 4
