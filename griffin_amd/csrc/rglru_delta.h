@@ -22,6 +22,7 @@ constexpr int kDeltaThreads = 256;
 constexpr int kDeltaMaxKey = 128;            // widest key that the kernels take
 // Floats per chunk of the gate record: rho[64], w[64] (zeros for tokens that do not count), four words of facts (ChunkFacts), padding
 constexpr int kDeltaGates = 136;
+constexpr int kDeltaGrid = (1 << 24) - 8;    // most workgroups of 256 threads in a launch, whose threads have to stay below 2^32 (rounded up for the XCDs)
 constexpr float kDeltaCut = -1e4f;           // a log decay below this discards the history (exp of it is 0 in any type)
 
 // States and solved values of a whole pass that the caches would not hold until they are read again are not kept there (`past` below:

@@ -522,15 +522,15 @@ template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool
 
 // Rows [B, T, H, K] that are no whole 16-byte vectors, as dense ones that are, zeros behind them.
 template <typename IO> __global__ __launch_bounds__(256) void delta_pad_kernel(const IO* src, IO* dst, long long rows, int T, int H, int K, int width, long long b_s, long long t_s, long long h_s) {
-  const long long i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= rows * width) return;
-  const long long row = i / width, token = row / H;
-  const int col = (int)(i % width);
-  dst[i] = col < K ? src[token / T * b_s + token % T * t_s + row % H * h_s + col] : (IO)0.f;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * width; i += gridDim.x * 256ll) {
+    const long long row = i / width, token = row / H;
+    const int col = (int)(i % width);
+    dst[i] = col < K ? src[token / T * b_s + token % T * t_s + row % H * h_s + col] : (IO)0.f;
+  }
 }
 int delta_launch_pad(const void* src, void* dst, int B, int T, int H, int K, int width, long long b_s, long long t_s, long long h_s, int dtype, hipStream_t s) {
-  const long long rows = (long long)B * T * H;
-  const dim3 grid((unsigned)((rows * width + 255) / 256));
+  const long long rows = (long long)B * T * H, blocks = (rows * width + 255) / 256;
+  const dim3 grid((unsigned)(blocks < kDeltaGrid ? blocks : kDeltaGrid));
   if (dtype == RGLRU_BF16) hipLaunchKernelGGL((delta_pad_kernel<__bf16>), grid, dim3(256), 0, s, (const __bf16*)src, (__bf16*)dst, rows, T, H, K, width, b_s, t_s, h_s);
   else hipLaunchKernelGGL((delta_pad_kernel<float>), grid, dim3(256), 0, s, (const float*)src, (float*)dst, rows, T, H, K, width, b_s, t_s, h_s);
   return check_launch("gated_delta rows");

@@ -123,15 +123,26 @@ template <typename IO, int LC, int N, bool PAST> __global__ __launch_bounds__(kD
   }
 }
 
-template <typename IO> static void delta_step(DeltaStepArgs a, int64_t heads, bool vec, hipStream_t s) {
-  auto grid = [&](int columns) {
-    a.groups = (a.V + columns - 1) / columns;
-    return dim3((unsigned)(heads * a.groups));
-  };
-  const dim3 g = grid(32), block(kDeltaThreads);
-  if (!vec) hipLaunchKernelGGL((delta_step_kernel<IO, 32, 1, false>), g, block, 0, s, a);
-  else if ((long long)heads * a.K * a.V * 4 < kCachedBytes) hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, false>), g, block, 0, s, a);
-  else hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, true>), g, block, 0, s, a);
+// One launch, or several where there are more rows than one holds.
+template <typename IO> static int delta_step(DeltaStepArgs a, int64_t B, bool vec, hipStream_t s) {
+  const int64_t heads = B * a.HV, bytes = heads * a.K * a.V * 4;
+  a.groups = (a.V + 31) / 32;
+  const int64_t fit = (kDeltaGrid - 1) / ((int64_t)a.HV * a.groups), each = fit < B ? fit : B;
+  auto moved = [](const void* p, int64_t elements, int dtype) { return (const char*)p + elements * (dtype == RGLRU_BF16 ? 2 : 4); };
+  const int dtype = sizeof(IO) == 2 ? RGLRU_BF16 : RGLRU_F32;
+  for (int64_t row = 0; row < B; row += each) {
+    const dim3 grid((unsigned)((B - row < each ? B - row : each) * a.HV * a.groups)), block(kDeltaThreads);
+    if (!vec) hipLaunchKernelGGL((delta_step_kernel<IO, 32, 1, false>), grid, block, 0, s, a);
+    else if (bytes < kCachedBytes) hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, true>), grid, block, 0, s, a);
+    const int rc = check_launch("gated_delta_step");
+    if (rc) return rc;
+    a.q = moved(a.q, each * a.H * a.K, dtype), a.k = moved(a.k, each * a.H * a.K, dtype), a.v = moved(a.v, each * a.HV * a.V, dtype);
+    a.out = (void*)moved(a.out, each * a.HV * a.V, dtype), a.state += each * a.HV * a.K * a.V;
+    a.log_decay = moved(a.log_decay, each * a.HV, a.decay_dtype), a.beta = moved(a.beta, each * a.HV, a.beta_dtype);
+    if (a.flags) a.flags += each;
+  }
+  return RGLRU_OK;
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -243,6 +254,8 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   whole = reinterpret_cast<uintptr_t>(v) % 16 == 0;
   for (int i = 6; i < 9; ++i) whole = whole && st[i] % e == 0;
   if (v && z.value_row == V && !whole) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of values must be 16-byte aligned", who);
+  if (B * HV * ((V + 63) / 64) >= kDeltaGrid || z.chunks >= kDeltaGrid || (keep && z.chunks >= kDeltaGrid / 2))
+    return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   a.segments = (int)z.segments, a.length = (int)z.length;
   a.past = z.chunks * z.columns * (z.width + 64) * 4 > kCachedBytes;
   char* base = (char*)ws;
@@ -350,9 +363,7 @@ int rglru_hip_gated_delta_step(const void* q, const void* k, const void* v, cons
   a.q = q, a.k = k, a.v = v, a.log_decay = log_decay, a.beta = beta, a.state = state, a.flags = flags, a.out = out;
   a.H = (int)H, a.HV = (int)HV, a.K = (int)K, a.V = (int)V, a.decay_dtype = decay_dtype, a.beta_dtype = beta_dtype, a.scale = scale;
   const bool vec = V % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
-  if (dtype == RGLRU_BF16) delta_step<__bf16>(a, B * HV, vec, (hipStream_t)stream);
-  else delta_step<float>(a, B * HV, vec, (hipStream_t)stream);
-  return check_launch("gated_delta_step");
+  return dtype == RGLRU_BF16 ? delta_step<__bf16>(a, B, vec, (hipStream_t)stream) : delta_step<float>(a, B, vec, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -40,7 +40,7 @@ struct GroupArgs {
   int Cg, width;                              // channels of a group; in vectors
   int columns, lines, blocks, per_group;      // many positions: vector columns of a workgroup, positions at a time, column blocks, blocks a group
   int chunks, chunk;                          // chunks of positions, positions in one
-  int rows_apart;                             // many positions: the kernel of the sums goes on rows_apart further
+  int row0, rows_apart;                       // many positions: first row of the launch; the kernel of the sums goes on rows_apart further
   int lanes, waves;                           // one position: lanes a run, waves of the launch
   float eps, inv_count;
 };
@@ -233,6 +233,7 @@ template <typename IO, int V, int SLOTS, bool BACKWARD> __global__ __launch_boun
 // ---- many positions -------------------------------------------------------------------------------------------------
 // A workgroup takes a chunk of positions of a row and a block of vector columns: whole groups where 256 vectors hold one, else
 // a part of one group.  Thread (column, line): one vector of every lines-th position.
+constexpr int kGroupGrid = 1 << 22;           // most workgroups of a launch; further rows take another one
 // Most workgroups a compute unit of the kernel of the sums: it goes on to further rows and adds their parameter gradients up, of which each workgroup
 // leaves one set.  A million rows of 2 x 64: 33 MiB of scratch instead of 544 and 12.1 ms a training step instead of 19.6.
 constexpr int kGroupSums = 8;
@@ -246,7 +247,7 @@ template <int V> RGLRU_DEVICE GroupPlace group_place(const GroupArgs& p) {
   GroupPlace g;
   long long i = blockIdx.x;
   g.block = (int)(i % p.blocks), i /= p.blocks;
-  g.chunk = (int)(i % p.chunks), g.n = (int)(i / p.chunks);
+  g.chunk = (int)(i % p.chunks), g.n = p.row0 + (int)(i / p.chunks);
   g.part = p.per_group > 1 ? g.block % p.per_group : 0;
   const int each = p.per_group > 1 ? 1 : p.columns / p.width;
   g.first_group = p.per_group > 1 ? g.block / p.per_group : g.block * each;
@@ -538,7 +539,7 @@ struct GroupPlan {
   bool rows;                                                // one position, runs that fit the registers
   int V, slots;
   int64_t sets, entries;                                    // partial parameter gradients; entries of a group
-  int64_t sum_rows;                                         // many positions: rows that the kernel of the sums takes side by side
+  int64_t rows_side_by_side, sum_rows;                      // many positions: rows of a launch; of the kernel of the sums
 };
 static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64_t G, int V, bool backward) {
   GroupPlan plan;
@@ -572,8 +573,10 @@ static GroupPlan group_plan(GroupArgs& a, int64_t N, int64_t L, int64_t C, int64
   if (chunks < 1) chunks = 1;
   a.chunk = (int)((L + chunks - 1) / chunks);
   a.chunks = (int)((L + a.chunk - 1) / a.chunk);
-  const int64_t each = (int64_t)a.chunks * a.blocks, most_sums = (int64_t)num_compute_units() * kGroupSums;
-  plan.sum_rows = each >= most_sums ? 1 : N < most_sums / each ? N : most_sums / each;
+  const int64_t each = (int64_t)a.chunks * a.blocks;
+  auto rows = [&](int64_t workgroups) { return each >= workgroups ? 1 : N < workgroups / each ? N : workgroups / each; };
+  plan.rows_side_by_side = rows(kGroupGrid);
+  plan.sum_rows = rows((int64_t)num_compute_units() * kGroupSums);
   plan.sets = plan.sum_rows * a.chunks;
   plan.entries = (int64_t)a.chunks * a.per_group;
   return plan;
@@ -589,11 +592,9 @@ static int group_check(const char* who, int64_t N, int64_t L, int64_t C, int64_t
   if (activation != RGLRU_ACT_NONE && activation != RGLRU_ACT_SILU && activation != RGLRU_ACT_GELU) return fail(RGLRU_E_ARG, "%s: unknown activation %d", who, activation);
   for (int d : {dtype, vec_dtype})
     if (d != RGLRU_F32 && d != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown dtype %d", who, d);
-  if (L >= (1ll << 30) || C >= (1ll << 24) || N >= (1ll << 30) / G) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
+  if (L >= (1ll << 30) || C >= (1ll << 24) || N >= (1ll << 30) / G || N >= (1ll << 38) / (L * C)) return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   return RGLRU_OK;
 }
-
-static bool group_fits(const GroupPlan& plan, const GroupArgs& a) { return plan.rows || (int64_t)a.N * a.blocks < (1ll << 31) / a.chunks; }
 
 static int group_vector(int64_t Cg, int dtype, std::initializer_list<const void*> tensors) {
   const int v = dtype == RGLRU_BF16 ? 8 : 4;
@@ -613,6 +614,18 @@ template <bool BACKWARD> static void group_rows(const GroupArgs& a, const GroupP
   if (dtype == RGLRU_BF16) { if (plan.V > 1) RGLRU_GROUP_ROWS(__bf16, 8); else RGLRU_GROUP_ROWS(__bf16, 1); }
   else { if (plan.V > 1) RGLRU_GROUP_ROWS(float, 4); else RGLRU_GROUP_ROWS(float, 1); }
 #undef RGLRU_GROUP_ROWS
+}
+
+// One launch, or several where there are more rows than one holds.
+template <typename LAUNCH> static int group_rows_launches(GroupArgs a, const GroupPlan& plan, const char* what, LAUNCH launch) {
+  for (int64_t row = 0; row < a.N; row += plan.rows_side_by_side) {
+    const int64_t rows = a.N - row < plan.rows_side_by_side ? a.N - row : plan.rows_side_by_side;
+    a.row0 = (int)row;
+    launch(a, dim3((unsigned)(rows * a.chunks * a.blocks)));
+    const int rc = check_launch(what);
+    if (rc) return rc;
+  }
+  return RGLRU_OK;
 }
 
 #define RGLRU_GROUP_LAUNCH(KERNEL, dtype, V, grid, s, a)                                                                          \
@@ -652,17 +665,13 @@ int rglru_hip_group_norm_fwd(const void* x, const void* weight, const void* bias
   a.x = x, a.weight = weight, a.bias = bias, a.y = y, a.stats = stats, a.entries = (float*)scratch;
   a.eps = eps, a.activation = activation, a.vec_dtype = vec_dtype;
   hipStream_t s = (hipStream_t)stream;
-  if (!group_fits(plan, a)) return fail(RGLRU_E_UNSUPPORTED, "group_norm_fwd: too large for one launch");
   if (plan.rows) {
     group_rows<false>(a, plan, dtype, s);
     return check_launch("group_norm_fwd");
   }
-  const dim3 grid((unsigned)(N * a.chunks * a.blocks));
-  RGLRU_GROUP_LAUNCH(group_norm_moments_kernel, dtype, plan.V, grid, s, a);
-  rc = check_launch("group_norm_fwd moments");
+  rc = group_rows_launches(a, plan, "group_norm_fwd moments", [&](const GroupArgs& a, dim3 grid) { RGLRU_GROUP_LAUNCH(group_norm_moments_kernel, dtype, plan.V, grid, s, a); });
   if (rc) return rc;
-  RGLRU_GROUP_LAUNCH(group_norm_apply_kernel, dtype, plan.V, grid, s, a);
-  return check_launch("group_norm_fwd");
+  return group_rows_launches(a, plan, "group_norm_fwd", [&](const GroupArgs& a, dim3 grid) { RGLRU_GROUP_LAUNCH(group_norm_apply_kernel, dtype, plan.V, grid, s, a); });
 }
 
 int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias, const float* stats, const void* dy, void* scratch, void* dx,
@@ -683,18 +692,16 @@ int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias
     a.dbias = (float*)((char*)a.dweight + group_up((size_t)plan.sets * C * 4));
   }
   hipStream_t s = (hipStream_t)stream;
-  if (!group_fits(plan, a)) return fail(RGLRU_E_UNSUPPORTED, "group_norm_bwd: too large for one launch");
   if (plan.rows) {
     group_rows<true>(a, plan, dtype, s);
     rc = check_launch("group_norm_bwd");
   } else {
     a.rows_apart = (int)plan.sum_rows;
-    const dim3 sum_grid((unsigned)(plan.sum_rows * a.chunks * a.blocks)), grid((unsigned)(N * a.chunks * a.blocks));
-    RGLRU_GROUP_LAUNCH(group_norm_sums_kernel, dtype, plan.V, sum_grid, s, a);
+    const dim3 grid((unsigned)(plan.sum_rows * a.chunks * a.blocks));
+    RGLRU_GROUP_LAUNCH(group_norm_sums_kernel, dtype, plan.V, grid, s, a);
     rc = check_launch("group_norm_bwd sums");
     if (rc) return rc;
-    RGLRU_GROUP_LAUNCH(group_norm_dx_kernel, dtype, plan.V, grid, s, a);
-    rc = check_launch("group_norm_bwd");
+    rc = group_rows_launches(a, plan, "group_norm_bwd", [&](const GroupArgs& a, dim3 grid) { RGLRU_GROUP_LAUNCH(group_norm_dx_kernel, dtype, plan.V, grid, s, a); });
   }
   if (rc || !params) return rc;
   SumJob jobs[2];

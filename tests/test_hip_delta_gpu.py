@@ -625,3 +625,37 @@ def test_decay_gradients_where_little_is_left(dtype, heads):
     got = run(hip_gated_delta, case, None, None, "cuda")[2]["log_decay"].cpu().double()
     limit = (STATE[dtype] + STATE_GRAD[dtype]) * product + (2 ** -8 if dtype == BF16 else 2 ** -24) * want.abs()
     assert ((got - want).abs() / limit).max() <= 1, float(((got - want).abs() / limit).max())
+
+
+def test_more_rows_than_a_launch_holds():
+    """Single tokens of 2^23 rows, two workgroups each, against the step written out; keys of more than 2^32 elements in rows of whole vectors."""
+    B, K, V = (1 << 23) + 5, 2, 33
+    gen = torch.Generator("cuda").manual_seed(6)
+    normal = lambda *shape: torch.empty(*shape, dtype=BF16, device="cuda").normal_(generator=gen)
+    q, k, v, decay, beta = normal(B, 1, K), normal(B, 1, K), normal(B, 1, V), -normal(B, 1).abs_(), normal(B, 1).sigmoid_()
+    state = torch.empty(B, 1, K, V, device="cuda").normal_(generator=gen)
+    flags = (torch.arange(B, device="cuda") % 3).to(torch.uint8)
+    for at in (slice(0, 1000), slice(B - 1000, B)):
+        kept = state[at].double()
+        out = hip_gated_delta_step(*(t[at] for t in (q, k, v, decay, beta)), state[at].clone(), flags=flags[at])
+        qd, kd, vd = (t[at].double() for t in (q, k, v))
+        kept = kept * torch.where(flags[at] == 1, 0.0, decay[at, 0].double().exp())[:, None, None, None]
+        change = beta[at].double()[..., None] * (vd - (kept * kd[..., None]).sum(2))
+        want = K ** -0.5 * ((kept + kd[..., None] * change[:, :, None]) * qd[..., None]).sum(2)
+        assert rel_err(out, torch.where(flags[at] == 2, 0.0, want.movedim(0, -1)).movedim(-1, 0)) <= OUT[BF16]
+    ends = [(at, state[at].clone()) for at in (slice(0, 1000), slice((1 << 23) - 500, B))]
+    out = hip_gated_delta_step(q, k, v, decay, beta, state, flags=flags)
+    for at, end in ends:
+        assert torch.equal(out[at], hip_gated_delta_step(*(t[at] for t in (q, k, v, decay, beta)), end, flags=flags[at]))
+        assert torch.equal(state[at], end)
+    del state, out, q, k, v
+
+    T, H, K, V = (1 << 20) + 64, 40, 100, 8
+    q = normal(1, T, H, K).mul_(0.1)
+    k, v, decay, beta = q.flip(-1), normal(1, T, H, V), normal(1, T, H).abs_().add_(1).neg_(), normal(1, T, H).sigmoid_()
+    with torch.no_grad():
+        out, last = hip_gated_delta(q, k, v, decay, beta)
+    # decays of at least e^-1 a token: what is 128 tokens back is gone; three heads by the definition
+    tail = [t[:, -192:, :3].double() for t in (q, k, v, decay, beta)]
+    want, want_last = recurrence(*(t.cpu() for t in tail), None, K ** -0.5)
+    assert rel_err(out[:, -64:, :3], want[:, -64:]) <= OUT[BF16] and rel_err(last[:, :3], want_last) <= STATE[BF16]

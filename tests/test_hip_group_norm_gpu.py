@@ -208,3 +208,27 @@ def test_sums_over_many_short_rows():
     assert rel_err(got[1], want[1]) <= 2 ** -12 and rel_err(got[0], want[0]) <= TOLERANCE[F32]
     case = make((40000, 3, 24), BF16)
     check(case, 3, "silu")
+
+
+def test_more_rows_than_a_launch_holds():
+    """2^24 rows of two positions: the ends and sums against the definition in 64 bits."""
+    rows, C, groups = (1 << 24) + 3, 8, 2
+    gen = torch.Generator("cuda").manual_seed(4)
+    x, up = (torch.empty(rows, 2, C, dtype=BF16, device="cuda").normal_(generator=gen) for _ in range(2))
+    weight, bias = (t.to(BF16).cuda() for t in make((2, C))[1:3])
+    leaves = [t.requires_grad_(True) for t in (x, weight, bias)]
+    out = hip_group_norm(x, groups, weight, bias, 1e-2, "silu")
+    got = torch.autograd.grad(out, leaves, up)
+    sums = [torch.zeros(C, dtype=torch.float64, device="cuda") for _ in range(2)]
+    for at in range(0, rows, 1 << 20):
+        part = [t[at : at + (1 << 20)].detach().double() if t.dim() == 3 else t.detach().double() for t in leaves]
+        part = [t.requires_grad_(True) for t in part]
+        want = definition(part[0], groups, *part[1:], 1e-2, "silu")
+        grads = torch.autograd.grad(want, part, up[at : at + (1 << 20)].double())
+        if at in (0, rows - rows % (1 << 20)):
+            assert rel_err(out[at : at + (1 << 20)], want) <= TOLERANCE[BF16] and rel_err(got[0][at : at + (1 << 20)], grads[0]) <= TOLERANCE[BF16]
+        for total, g in zip(sums, grads[1:]):
+            total += g
+    # terms of up to about 1 that cancel to their square root: 2^-16 of their number beside the rounding of the result
+    for g, total in zip(got[1:], sums):
+        assert ((g.double() - total).abs() <= 2 ** -8 * total.abs() + 2 ** -16 * 2 * rows).all()

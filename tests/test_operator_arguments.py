@@ -199,3 +199,15 @@ def test_tensors_that_do_not_fit(error, call):
 def test_partial_gradients_of_many_short_rows_do_not_outgrow_them(lib):
     x = 2 * (1 << 20) * 2 * 64                                                  # a million rows of 2 x 64 in bf16
     assert lib.rglru_hip_group_norm_scratch_bytes(1 << 20, 2, 64, 4, 1) <= x // 4
+
+
+@pytest.mark.parametrize("call", [
+    lambda lib: fwd(lib, sizes=(1 << 20, 1, 1, 1, 1, 1024)),                    # 2^24 workgroups of 64 columns
+    lambda lib: fwd(lib, sizes=(1 << 24, 1, 1, 1, 8, 8)),                       # ... of a chunk
+    lambda lib: bwd(lib, sizes=(1 << 23, 1, 1, 1, 8, 8)),                       # 2^23 of twice the threads
+    lambda lib: norm_fwd(lib, sizes=(1 << 24, 1 << 10, 64, 4)),                 # more than any card holds
+    lambda lib: norm_bwd(lib, sizes=(1 << 24, 1 << 10, 64, 4)),
+])
+def test_launches_of_too_many_threads_are_refused(lib, call):
+    assert call(lib) == UNSUPPORTED
+    assert b"too large" in lib.rglru_hip_last_error()
