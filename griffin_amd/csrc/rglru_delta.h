@@ -506,11 +506,9 @@ struct ChunkFacts {
   }
 };
 
-// Whether a walk's workgroups are of two waves with two chunks' tiles in LDS (`two`: they fit) instead of four waves with one: where there
+// Whether a walk's workgroups are of two waves with two chunks' tiles in LDS (they fit in bf16 only) instead of four waves with one: where there
 // are so few that each has a compute unit to itself and the time a chunk takes is all that counts.
-inline bool delta_narrow(const DeltaArgs& a, bool two) {
-  return two && a.segments == 1 && (long long)((a.columns + 31) / 32) * a.B * a.HV <= num_compute_units();
-}
+inline bool delta_narrow(const DeltaArgs& a) { return a.segments == 1 && (long long)((a.columns + 31) / 32) * a.B * a.HV <= num_compute_units(); }
 
 // XCDs take workgroups round-robin; each gets a contiguous run of the work, so that neighbours share its L2.  -1: none left.
 RGLRU_DEVICE int xcd_order(int block, int total) {

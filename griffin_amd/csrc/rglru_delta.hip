@@ -516,7 +516,8 @@ template <typename IO, int KS> static int delta_forward(const DeltaArgs& a, bool
     if (!rc) rc = delta_join<IO, KS>(a, false, s);
     if (rc) return rc;
   }
-  if (delta_narrow(a, kTwo)) return save ? delta_walk<IO, KS, 2, kTwo ? 2 : 1, true, true>(a, s) : delta_walk<IO, KS, 2, kTwo ? 2 : 1, false, true>(a, s);
+  if constexpr (kTwo)
+    if (delta_narrow(a)) return save ? delta_walk<IO, KS, 2, 2, true, true>(a, s) : delta_walk<IO, KS, 2, 2, false, true>(a, s);
   return save ? delta_walk<IO, KS, 4, 1, true, true>(a, s) : delta_walk<IO, KS, 4, 1, false, true>(a, s);
 }
 

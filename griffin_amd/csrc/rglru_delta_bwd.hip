@@ -627,7 +627,12 @@ template <typename IO, int KS> static int delta_backward(const DeltaArgs& a, hip
     if (!rc) rc = delta_launch_join(a, kTwo ? RGLRU_BF16 : RGLRU_F32, s);
     if (rc) return rc;
   }
-  rc = delta_narrow(a, kTwo) ? delta_walk_back<IO, KS, 2, kTwo ? 2 : 1, false>(a, s) : delta_walk_back<IO, KS, 4, 1, false>(a, s);
+  bool narrow = false;
+  if constexpr (kTwo) {
+    narrow = delta_narrow(a);
+    if (narrow) rc = delta_walk_back<IO, KS, 2, 2, false>(a, s);
+  }
+  if (!narrow) rc = delta_walk_back<IO, KS, 4, 1, false>(a, s);
   if (rc) return rc;
   const dim3 grid = xcd_grid((long long)a.B * a.H * a.nC);
   if (a.HV > a.H) hipLaunchKernelGGL((delta_grads_kernel<IO, KS, true>), grid, dim3(kGradThreads), 0, s, a);
