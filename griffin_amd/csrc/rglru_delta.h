@@ -25,11 +25,13 @@ constexpr int kDeltaGates = 136;
 constexpr int kDeltaGrid = (1 << 24) - 8;    // most workgroups of 256 threads in a launch, whose threads have to stay below 2^32 (rounded up for the XCDs)
 constexpr float kDeltaCut = -1e4f;           // a log decay below this discards the history (exp of it is 0 in any type)
 
-// States and solved values of a whole pass that the caches would not hold until they are read again are not kept there (`past` below:
-// more than half of the 256 MiB of the last cache).  Training step of B8 T2048 H8 of 128 (192 MiB a pass) 495 -> 475 us; B1 T8192 H8 (96 MiB)
-// would take 391 instead of 383.
+// What a pass leaves for the next one goes past the caches (`past`: stores without a place in the last one, of 256 MiB) in walks of two waves, where
+// it fills more than half of that cache and not more than all of it: training steps of 8 heads of 128 x 128, us with and without, by MiB a walk:
+//   B5 T2048 (120) 382 : 384, B6 (144) 427 : 438, B7 (168) 459 : 473, B8 (192) 487 : 501, B8 T2560 (240) 610 : 616, B8 T2816 (264) 690 : 682, B8 T4096 (384)
+//   1032 : 994; B4 T2048 (96) 324 : 320.
+// Walks of four waves lose at every size: B16 T1024 (192) 438 : 411, B12 T2048 (288) 727 : 674, in segments B4 T4096 (192) 596 : 569.
 constexpr int kPastCaches = 2;
-constexpr long long kCachedBytes = 128ll << 20;
+constexpr long long kLastCache = 256ll << 20;
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

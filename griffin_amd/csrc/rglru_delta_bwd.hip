@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && STAGES * KS * (int)sizeof
   auto request = [&](int stage) { tiles.request(p, lds0 + (unsigned)(stage * Tiles::kBytes), wave); };
   // a chunk's matrix of `rows` elements a column, by eight of a column a lane
   const unsigned plane_bytes = (unsigned)p.columns * (unsigned)sizeof(IO);
-  const bool past = p.past != 0;
+  const bool past = WAVES == 2 && p.past != 0;
   auto matrix = [&](void* base, int n, int rows) {
     return make_rsrc((IO*)base + (first + n) * PL * p.columns * rows, PL * plane_bytes * (unsigned)rows);
   };

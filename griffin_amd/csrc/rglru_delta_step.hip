@@ -29,9 +29,10 @@ struct DeltaStepArgs {
 //   Eight lanes of four columns and 32 row groups: a wave reads eight rows' whole 128-byte lines, and enough workgroups are there to fill the
 //   device from 16 rows of 8 heads on.  Whole rows of 128 columns a wave take 7.1 us there instead of 6.0, and 38.7 instead of 29.6 for 256 x 16
 //   heads of 64 x 64, whose rows they leave half empty.
-//   PAST: a state of half the last cache or more goes past it, since nothing of it would be there by the next token (states of other
-//   layers in between): 61.6 -> 53.7 us; 512 rows of 20 heads 280 -> 252.  Below that, a state that is all there is stays cached: 64 rows
-//   of 8 heads 13.8 us either way.
+//   PAST: states of 16 MiB or more go past the caches; by the next token the states of other layers have been there.  us a token past them and
+//   through them, by MiB of state: twelve layers in turn 8.1 : 11.9 (16), 15.3 : 20.7 (32), 28.3 : 34.2 (64), 51 : 60 (128), 99 : 117 (256); one state over and
+//   over 7.4 : 7.5 (16), 25.9 : 28.4 (64), 49.9 : 48.4 (128), 72.9 : 68.4 (192), 98 : 104 (256).  Below that 6.0 : 6.5 (8) and 4.9 : 5.2 (4) in
+//   turn, but 7.0 : 5.9 over and over (37 rows of 12 heads of 72 x 40, 5 MiB).
 template <typename IO, int LC, int N, bool PAST> __global__ __launch_bounds__(kDeltaThreads) void delta_step_kernel(DeltaStepArgs p) {
   typedef float vec __attribute__((ext_vector_type(N)));
   constexpr int RG = kDeltaThreads / LC, ROWS = kDeltaMaxKey / RG, WAVES = kDeltaThreads / 64;
@@ -125,7 +126,7 @@ template <typename IO, int LC, int N, bool PAST> __global__ __launch_bounds__(kD
 
 // One launch, or several where there are more rows than one holds.
 template <typename IO> static int delta_step(DeltaStepArgs a, int64_t B, bool vec, hipStream_t s) {
-  const int64_t heads = B * a.HV, bytes = heads * a.K * a.V * 4;
+  const bool past = B * a.HV * a.K * a.V >= (16ll << 20) / 4;
   a.groups = (a.V + 31) / 32;
   const int64_t fit = (kDeltaGrid - 1) / ((int64_t)a.HV * a.groups), each = fit < B ? fit : B;
   auto moved = [](const void* p, int64_t elements, int dtype) { return (const char*)p + elements * (dtype == RGLRU_BF16 ? 2 : 4); };
@@ -133,7 +134,7 @@ template <typename IO> static int delta_step(DeltaStepArgs a, int64_t B, bool ve
   for (int64_t row = 0; row < B; row += each) {
     const dim3 grid((unsigned)((B - row < each ? B - row : each) * a.HV * a.groups)), block(kDeltaThreads);
     if (!vec) hipLaunchKernelGGL((delta_step_kernel<IO, 32, 1, false>), grid, block, 0, s, a);
-    else if (bytes < kCachedBytes) hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, false>), grid, block, 0, s, a);
+    else if (!past) hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, false>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((delta_step_kernel<IO, 8, 4, true>), grid, block, 0, s, a);
     const int rc = check_launch("gated_delta_step");
     if (rc) return rc;
@@ -150,7 +151,9 @@ template <typename IO> static int delta_step(DeltaStepArgs a, int64_t B, bool ve
 // Segments of `length` chunks that a sequence is walked in side by side.  One walk takes as long as its chunks, however many compute units
 // stand idle; in segments, all of them are walked twice (what a segment adds to the state and what it makes of it, 128 further
 // columns; then the outputs from the joined states).  The number is the one with the least time by what launches of both kinds measure, us a
-// chunk of a round of workgroups (bf16, keys and values of 128; it is their ratios that decide, also for other sizes).
+// chunk of a round of workgroups (bf16, keys and values of 128; it is their ratios that decide, also for other sizes and fp32).  Against the best of
+// twelve numbers tried, of seven shapes with and without gradients (B1 T2048 H4 of 64 x 64 to B1 T32768 H4 of 128 x 128): bf16 within 5 %, fp32 within
+// 10 %, but for prefills of B3 T777 H8 of 96 x 80, which it leaves whole: 57 us instead of 52, 133 instead of 107.
 static int64_t delta_best_segments(int64_t heads, int64_t columns, int64_t width, int64_t nC, bool two, bool keep) {
   const int64_t cus = num_compute_units(), groups = (columns + 63) / 64, units = (width + 63) / 64;
   auto rounds = [&](int64_t n, double alone, double shared) {  // one workgroup a compute unit, or two that share it
@@ -257,7 +260,8 @@ static int delta_operands(const char* who, DeltaArgs& a, const void* q, const vo
   if (B * HV * ((V + 63) / 64) >= kDeltaGrid || z.chunks >= kDeltaGrid || (keep && z.chunks >= kDeltaGrid / 2))
     return fail(RGLRU_E_UNSUPPORTED, "%s: too large for one launch", who);
   a.segments = (int)z.segments, a.length = (int)z.length;
-  a.past = z.chunks * z.columns * (z.width + 64) * 4 > kCachedBytes;
+  const long long kept = z.chunks * z.columns * (z.width + 64) * 4;
+  a.past = kept > kLastCache / 2 && kept <= kLastCache;
   char* base = (char*)ws;
   a.through = base + z.through, a.local = (float*)(base + z.local), a.edges = (float*)(base + z.edges), a.cut = (int*)(base + z.cut);
   a.gates = (float*)(base + z.gates);

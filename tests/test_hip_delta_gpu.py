@@ -659,3 +659,30 @@ def test_more_rows_than_a_launch_holds():
     tail = [t[:, -192:, :3].double() for t in (q, k, v, decay, beta)]
     want, want_last = recurrence(*(t.cpu() for t in tail), None, K ** -0.5)
     assert rel_err(out[:, -64:, :3], want[:, -64:]) <= OUT[BF16] and rel_err(last[:, :3], want_last) <= STATE[BF16]
+
+
+def test_large_passes_against_the_definition():
+    """Sizes whose states go past the caches, of walks of two waves and of four: a row and its gradients by the definition."""
+    for shape, row in (((8, 1408, 8, 8, 128, 128), 3), ((10, 1100, 8, 8, 128, 128), 9)):
+        case = make(*shape, dtype=BF16)
+        out, last, grads = run(hip_gated_delta, case, None, None, "cuda")
+        one = {n: t[row : row + 1] for n, t in case.items()}
+        want, want_last, want_grads = run(recurrence, one, None, None, "cuda", torch.float64)
+        assert rel_err(out[row : row + 1], want) <= OUT[BF16] and rel_err(last[row : row + 1], want_last) <= STATE[BF16]
+        for name in NAMES:
+            assert rel_err(grads[name][row : row + 1], want_grads[name]) <= (STATE_GRAD if name == "h0" else GRAD)[BF16], name
+
+
+def test_large_steps_against_the_definition():
+    B, H, HV, K, V = 512, 4, 8, 128, 128                       # 256 MiB of state
+    gen = torch.Generator("cuda").manual_seed(8)
+    normal = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")
+    q, k = (torch.nn.functional.normalize(normal(B, H, K), dim=-1).bfloat16() for _ in range(2))
+    v, decay, beta = normal(B, HV, V).bfloat16(), -normal(B, HV).abs(), normal(B, HV).sigmoid()
+    state = normal(B, HV, K, V)
+    of = torch.arange(HV, device="cuda") // (HV // H)
+    kept = state.double() * decay.double().exp()[..., None, None]
+    keys, queries = k.double()[:, of], q.double()[:, of]
+    new = kept + keys[..., None] * (beta.double()[..., None] * (v.double() - (kept * keys[..., None]).sum(2)))[:, :, None]
+    out = hip_gated_delta_step(q, k, v, decay, beta, state)
+    assert rel_err(out, K ** -0.5 * (new * queries[..., None]).sum(2)) <= OUT[BF16] and rel_err(state, new) <= 2 ** -16
