@@ -686,3 +686,30 @@ def test_large_steps_against_the_definition():
     new = kept + keys[..., None] * (beta.double()[..., None] * (v.double() - (kept * keys[..., None]).sum(2)))[:, :, None]
     out = hip_gated_delta_step(q, k, v, decay, beta, state)
     assert rel_err(out, K ** -0.5 * (new * queries[..., None]).sum(2)) <= OUT[BF16] and rel_err(state, new) <= 2 ** -16
+
+
+def test_the_end_of_a_long_prompt_against_the_definition():
+    """More than 2^31 elements a tensor; decays of at least e^-1 a token leave nothing of what is 128 tokens back."""
+    T, H, K, heads = (1 << 19) + 128, 32, 128, 4
+    gen = torch.Generator("cuda").manual_seed(9)
+    normal = lambda *shape, by=1.0: torch.empty(*shape, dtype=BF16, device="cuda").normal_(generator=gen).mul_(by)
+    operands = [normal(1, T, H, K, by=K ** -0.5), normal(1, T, H, K, by=0.8 * K ** -0.5), normal(1, T, H, K),
+                -normal(1, T, H).abs_().add_(1), normal(1, T, H).sigmoid_()]
+    out, last = hip_gated_delta(*operands)
+    tail = [t[:, -192:, -heads:].double().cpu() for t in operands]
+    want, want_last = recurrence(*tail, None, K ** -0.5)
+    assert rel_err(out[:, -64:, -heads:], want[:, -64:]) <= OUT[BF16] and rel_err(last[:, -heads:], want_last) <= STATE[BF16]
+
+
+@pytest.mark.parametrize("T", [63, 200])
+def test_what_parallel_keys_all_but_erase(T):
+    """Keys of one element are parallel: a chunk erases nearly all of a state's gradient, whose terms are the upstream gradients of all tokens.
+    Of those it is known to what a gradient of bf16 operands is (STATE_GRAD), not of the little that is left."""
+    case = make(1, T, 1, 2, 1, 48, dtype=BF16, slow=True)
+    _, _, want = run(recurrence, case, None, None, "cpu", torch.float64)
+    _, _, grads = run(hip_gated_delta, case, None, None, "cuda")
+    # a token hands on its query times its upstream gradient, both keys of one; what they erase of it comes back in the products
+    q, up = case["q"].double(), case["up"].double()
+    terms = (q[..., 0].abs().repeat(1, 1, 2)[..., None] * up.abs()).sum(1) + case["up_state"].double().abs()[:, :, 0]
+    assert float(want["h0"].abs().max()) < 2 ** -4 * float(terms.max())
+    assert ((grads["h0"].cpu().double() - want["h0"])[:, :, 0].abs() <= STATE_GRAD[BF16] * terms).all()
