@@ -10,8 +10,8 @@
 // states joined along the segments, the outputs from these.
 //
 // Chunks of 64: the products within a chunk grow with its length (64 x 64 x 128 twice), those with the state do not, and
-// the tiles of two chunks fit the LDS.  B8 T2048, 8 heads of 128 x 128 in bf16, saving for the backward pass: 42 + 156 us, against 97 for
-// the 500 MB of both kernels at the rate of a large copy.  One sequence of 32768 tokens and 20 heads: 180 + 310 + 42 + 300 us, against 385 for 1.97 GB.
+// the tiles of two chunks fit the LDS.  B8 T2048, 8 heads of 128 x 128 in bf16, saving for the backward pass: 43 + 155 us, against 97 for
+// the 500 MB of both kernels at the rate of a large copy.  One sequence of 32768 tokens and 20 heads: 179 + 310 + 43 + 300 us, against 385 for 1.97 GB.
 
 #include <hip/hip_runtime.h>
 
@@ -50,7 +50,7 @@ template <int J> RGLRU_DEVICE void delta_solve_column(const float* low, const fl
 
 // T, P and the gate record of one chunk and value head.  A wave owns 16 rows of both; its operands come straight from memory (a row's
 // 64 bytes a quarter of the wave) and T and P take turns in LDS, so that five workgroups share a compute unit: what one of them does
-// is short, and one after the other.
+// is short, and one after the other.  (Keys of 128 in bf16 put one register aside in scratch for it.)
 template <typename IO, int KS> __global__ __launch_bounds__(kDeltaThreads, sizeof(IO) == 2 ? 5 : 3) void delta_prepare_kernel(DeltaArgs p) {
   typedef Mx<IO> M;
   typedef typename M::Frag Frag;

@@ -12,7 +12,7 @@
 // document's gradient in its neighbours'.  The price is the products of all keys with queries and keys once more: 8 us of the step below.)
 // The first kernel walks back along the chunks with dS' as the forward pass walks with S; the second one has no order: a workgroup a chunk and
 // key head, which adds up its value heads.
-// B8 T2048, 8 heads of 128 x 128 in bf16: 157 + 156 us.  The walk is bound like the forward one.  The second kernel reads what both walks left,
+// B8 T2048, 8 heads of 128 x 128 in bf16: 151 + 164 us.  The walk is bound like the forward one.  The second kernel reads what both walks left,
 // 490 MB, and takes 112 us with its loads alone, 58 with its products over the columns alone: it is bound by memory in front and by
 // what each workgroup does behind its last column, where nothing is loaded.
 
@@ -262,8 +262,9 @@ RGLRU_DEVICE float four_rows_sum(float v) {
 // Gradients of queries, keys and gates of one chunk and key head.  Eight waves: four times 16 tokens, by two halves of the key's
 // columns; the first half's waves make N1, the second half's N2.  The contractions over the value columns take 32 of them at a time
 // through LDS, the next 32 on their way there where two fit; queries, keys, N1 and N2 come where the columns lay.
-// Two workgroups share a compute unit in bf16 (kGradShared; one alone: 195 us instead of 176 at B8 T2048 H8 of 128); fp32 operands and
-// the sums over value heads need the registers of one.
+// Two workgroups share a compute unit in bf16 (kGradShared; one alone: 195 us instead of 176 at B8 T2048 H8 of 128 at the time); fp32 operands and
+// the sums over value heads need the registers of one.  Keys of 128 in bf16 put 22 registers aside in scratch for it (96 elements: 6), and so
+// does fp32 with value heads that share keys of 128 (13).
 constexpr int kGradThreads = 512;
 template <typename IO, bool GROUPED> constexpr bool kGradShared = (sizeof(IO) == 2) && !GROUPED;
 template <typename IO, int KS, bool GROUPED>
