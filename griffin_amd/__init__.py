@@ -12,9 +12,10 @@ from .hip_scan import (
     set_chain_forward,
     set_reproducible,
 )
-from .hip_block_ops import (hip_block_forward, hip_causal_conv, hip_causal_conv_padded, hip_gelu_gate, hip_group_norm, hip_linear,
+from .hip_block_ops import (hip_add_rmsnorm, hip_add_rmsnorm_quantised, hip_block_forward, hip_causal_conv, hip_causal_conv_padded, hip_gelu_gate, hip_group_norm, hip_linear,
                             hip_linear_pair, hip_rmsnorm)
 from .hip_delta import hip_gated_delta, hip_gated_delta_step
+from .hip_selective import hip_selective_scan, hip_selective_step, hip_short_conv, hip_short_conv_step
 from .modules import (
     BlockDiagonalLinear,
     RG_LRU,
@@ -30,6 +31,8 @@ __all__ = [
     "RMSNorm",
     "RecurrentBlock",
     "RecurrentBlockCache",
+    "hip_add_rmsnorm",
+    "hip_add_rmsnorm_quantised",
     "hip_block_forward",
     "hip_causal_conv",
     "hip_causal_conv_padded",
@@ -46,6 +49,10 @@ __all__ = [
     "hip_rglru_steps",
     "hip_scan_available",
     "hip_scan_is_usable",
+    "hip_selective_scan",
+    "hip_selective_step",
+    "hip_short_conv",
+    "hip_short_conv_step",
     "set_chain_forward",
     "set_reproducible",
 ]

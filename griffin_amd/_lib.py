@@ -14,7 +14,7 @@ RGLRU_BF16 = 1
 FLAG_RESET = 1
 FLAG_INACTIVE = 2
 CHUNK = 32
-ABI_VERSION = 25
+ABI_VERSION = 26
 PATH_PORTABLE, PATH_FAST_TILED, PATH_FAST_CHAIN, PATH_WIDE, PATH_PRE = range(5)
 PATH_NAMES = ("portable", "fast_tiled", "fast_chain", "wide", "pre")
 
@@ -79,6 +79,21 @@ _SIGNATURES = {
     "rglru_hip_gated_delta_fwd": (ctypes.c_int, [_P] * 11 + [ctypes.c_int, ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_bwd": (ctypes.c_int, [_P] * 16 + [ctypes.c_float] + [_I] * 6 + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_gated_delta_step": (ctypes.c_int, [_P] * 8 + [ctypes.c_float] + [_I] * 5 + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_selective_max_states": (ctypes.c_int, []),
+    "rglru_hip_selective_workspace_bytes": (ctypes.c_size_t, [_I] * 5 + [ctypes.c_int]),
+    "rglru_hip_selective_scratch_bytes": (ctypes.c_size_t, [_I] * 5),
+    "rglru_hip_selective_fwd": (ctypes.c_int, [_P] * 14 + [ctypes.c_int] * 2 + [_I] * 5 + [ctypes.c_int, _P]),
+    "rglru_hip_selective_bwd": (ctypes.c_int, [_P] * 23 + [ctypes.c_int] + [_I] * 5 + [ctypes.c_int, _P]),
+    "rglru_hip_selective_step": (ctypes.c_int, [_P] * 12 + [ctypes.c_int] + [_I] * 4 + [ctypes.c_int, _P]),
+    "rglru_hip_short_conv_scratch_bytes": (ctypes.c_size_t, [_I] * 4),
+    "rglru_hip_short_conv_fwd": (ctypes.c_int, [_P, _I, _I] + [_P] * 6 + [ctypes.c_int] + [_I] * 4 + [ctypes.c_int] * 2 + [_P]),
+    "rglru_hip_short_conv_bwd": (ctypes.c_int, [_P, _I, _I] + [_P] * 10 + [ctypes.c_int] + [_I] * 4 + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_short_conv_step": (ctypes.c_int, [_P, _I] + [_P] * 5 + [ctypes.c_int] + [_I] * 3 + [ctypes.c_int] * 2 + [_P]),
+    "rglru_hip_add_rmsnorm_max_width": (ctypes.c_int, []),
+    "rglru_hip_add_rmsnorm_fwd": (ctypes.c_int, [_P] * 6 + [_I] * 2 + [ctypes.c_float] + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_add_rmsnorm_quantised": (ctypes.c_int, [_P] * 6 + [_I] * 2 + [ctypes.c_float] + [ctypes.c_int] * 3 + [_P]),
+    "rglru_hip_add_rmsnorm_scratch_bytes": (ctypes.c_size_t, [_I] * 2),
+    "rglru_hip_add_rmsnorm_bwd": (ctypes.c_int, [_P] * 9 + [_I] * 2 + [ctypes.c_int] * 4 + [_P]),
     "rglru_hip_group_norm_scratch_bytes": (ctypes.c_size_t, [_I] * 4 + [ctypes.c_int]),
     "rglru_hip_group_norm_fwd": (ctypes.c_int, [_P] * 6 + [_I] * 4 + [ctypes.c_float] + [ctypes.c_int] * 3 + [_P]),
     "rglru_hip_group_norm_bwd": (ctypes.c_int, [_P] * 9 + [_I] * 4 + [ctypes.c_int] * 4 + [_P]),

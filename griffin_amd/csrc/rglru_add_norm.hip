@@ -1,0 +1,398 @@
+// Root-mean-square norm with the residual's addition in front of it, in one pass over a row:
+//   s = x + r (rounded to r's type: the stream that goes on),  y = s inv (1 + g),  inv = 1 / sqrt(mean(s^2) + eps)
+// with rows of y in the type of x, or in 8 bits (e4m3) with one scale a row, y = q scale, for a product in 8 bits.  Reverse mode, with upstream
+// gradients dy and ds:
+//   d = ds + inv (w dy - s inv^2 mean(w dy s)),  w = 1 + g,  for both addends;  dg = sum over rows of dy s inv
+// The statistics are those of the stored s, which the backward pass reads again.  A row is held in registers by one wave, by four or sixteen where it
+// is wider than 1024 or 4096 elements: at most sixteen elements a lane; nothing is read twice.  Bound by memory.
+
+#include <hip/hip_runtime.h>
+
+#include <cstring>
+
+#include "rglru_device.h"
+#include "rglru_host.h"
+#include "rglru_sums.h"
+
+namespace rglru {
+
+constexpr int kAddMaxWidth = 16384;
+constexpr int add_threads(int waves) { return waves > 4 ? 64 * waves : 256; }
+constexpr float kByteMost = 448.f;            // largest number of e4m3
+constexpr float kByteLeast = 7.8886090522101181e-31f;   // 2^-100: rows no larger than that have this for their largest value
+
+struct AddArgs {
+  const void *x, *r, *g, *dy, *ds;            // r, ds: or null
+  const float* inv_in;
+  void *sum, *y, *dx, *dr;                    // sum: or null; dx, dr: one of them may be null
+  float *inv, *scale, *partial;               // inv: or null
+  long long rows;
+  int D, nvec, vec_dtype;
+  float eps;
+};
+
+// A row's vectors by buffers that end with the row: what lies behind it reads as zeros and is not written.
+template <typename T, int V> struct AddRow {
+  static constexpr int kWords = V * (int)sizeof(T) / 4;     // 0: one bf16
+  typedef T Raw __attribute__((ext_vector_type(V)));
+  static RGLRU_DEVICE rsrc_t row(const void* p, long long row, int D, bool there) {
+    return make_rsrc((const T*)p + row * D, there ? (unsigned)D * (unsigned)sizeof(T) : 0u);
+  }
+  static RGLRU_DEVICE Raw request(rsrc_t r, int vec) {
+    const unsigned off = (unsigned)(vec * V) * (unsigned)sizeof(T);
+    if constexpr (kWords == 0) return __builtin_bit_cast(Raw, (short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+    else if constexpr (kWords == 1) return __builtin_bit_cast(Raw, (int)__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else if constexpr (kWords == 2) return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    else if constexpr (kWords == 4) return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    else {
+      struct { i32x4 lo, hi; } both;
+      both.lo = buf_load_frag<i32x4>(r, off); both.hi = buf_load_frag<i32x4>(r, off + 16);
+      return __builtin_bit_cast(Raw, both);
+    }
+  }
+  static RGLRU_DEVICE void store(rsrc_t r, int vec, const float (&v)[V]) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const unsigned off = (unsigned)(vec * V) * (unsigned)sizeof(T);
+    Raw raw;
+#pragma unroll
+    for (int e = 0; e < V; ++e) raw[e] = (T)v[e];
+    if constexpr (kWords == 0) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, raw), r, off, 0, 0);
+    else if constexpr (kWords == 1) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, raw), r, off, 0, 0);
+    else if constexpr (kWords == 2) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, raw), r, off, 0, 0);
+    else if constexpr (kWords == 4) buf_store_b128(__builtin_bit_cast(i32x4, raw), r, off);
+    else {
+      struct Both { i32x4 lo, hi; };
+      const Both both = __builtin_bit_cast(Both, raw);
+      buf_store_b128(both.lo, r, off); buf_store_b128(both.hi, r, off + 16);
+    }
+  }
+};
+
+RGLRU_DEVICE float add_wave_sum(float v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+RGLRU_DEVICE float add_wave_max(float v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+  return v;
+}
+// Over the WAVES waves of a row; `turn` takes one of two places, so that one barrier is enough.
+template <int WAVES, bool MOST> RGLRU_DEVICE float add_row_all(float v, float (*mem)[16], int turn) {
+  v = MOST ? add_wave_max(v) : add_wave_sum(v);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) mem[turn][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = mem[turn][0];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) v = MOST ? fmaxf(v, mem[turn][k]) : v + mem[turn][k];
+  }
+  return v;
+}
+
+// 1 + g of a lane's vectors.
+template <int V> RGLRU_DEVICE void add_scale(const AddArgs& p, int first, bool ok, float (&w)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    w[e] = !ok ? 0.f : 1.f + (p.vec_dtype == RGLRU_BF16 ? (float)((const __bf16*)p.g)[first + e] : ((const float*)p.g)[first + e]);
+}
+
+template <typename XT, typename RT, int V, int SLOTS, int WAVES, bool BYTES> __global__ __launch_bounds__(add_threads(WAVES)) void add_norm_kernel(AddArgs p) {
+  __shared__ float mem[4][16];
+  constexpr int LANES = 64 * WAVES, kAddThreads = add_threads(WAVES);
+  const int l = threadIdx.x % LANES;
+  const long long step = (long long)gridDim.x * (kAddThreads / LANES);
+  float w[SLOTS][V];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) add_scale<V>(p, (l + LANES * s) * V, l + LANES * s < p.nvec, w[s]);
+  const float inv_d = 1.f / (float)p.D;
+  typename AddRow<XT, V>::Raw next_x[SLOTS];
+  typename AddRow<RT, V>::Raw next_r[SLOTS];
+  auto request = [&](long long row) {
+    const rsrc_t rx = AddRow<XT, V>::row(p.x, row, p.D, row < p.rows), rr = AddRow<RT, V>::row(p.r, row, p.D, row < p.rows && p.r);
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      next_x[s] = AddRow<XT, V>::request(rx, l + LANES * s);
+      next_r[s] = AddRow<RT, V>::request(rr, l + LANES * s);
+    }
+  };
+  long long row = (long long)blockIdx.x * (kAddThreads / LANES) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / LANES);
+  request(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    float v[SLOTS][V], acc = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[s][e] = (float)next_x[s][e];
+        if (p.r) v[s][e] = (float)(RT)(v[s][e] + (float)next_r[s][e]);
+        acc = fmaf(v[s][e], v[s][e], acc);
+      }
+    request(row + step);
+    if (p.sum) {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) AddRow<RT, V>::store(AddRow<RT, V>::row(p.sum, row, p.D, true), l + LANES * s, v[s]);
+    }
+    const float inv = __builtin_amdgcn_rsqf(fmaf(add_row_all<WAVES, false>(acc, mem, turn), inv_d, p.eps));
+    if (p.inv && l == 0) p.inv[row] = inv;
+    float most = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[s][e] *= inv * w[s][e];
+        if (BYTES) most = fmaxf(most, fabsf(v[s][e]));
+      }
+    if constexpr (BYTES) {
+      most = fmaxf(add_row_all<WAVES, true>(most, mem, 2 + turn), kByteLeast);
+      const float up = kByteMost / most;
+      if (l == 0) p.scale[row] = most / kByteMost;
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) {
+        const bool ok = l + LANES * s < p.nvec;
+        unsigned char* out = (unsigned char*)p.y + row * p.D + (long long)(l + LANES * s) * V;
+        if constexpr (V >= 4) {
+          unsigned word[V / 4];
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][e] * up, v[s][e + 1] * up, 0, false);
+            word[e / 4] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][e + 2] * up, v[s][e + 3] * up, q, true);
+          }
+          if (ok) {
+#pragma unroll
+            for (int e = 0; e < V / 4; ++e) reinterpret_cast<unsigned*>(out)[e] = word[e];
+          }
+        } else {
+          if (ok) out[0] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(v[s][0] * up, 0.f, 0, false);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) AddRow<XT, V>::store(AddRow<XT, V>::row(p.y, row, p.D, true), l + LANES * s, v[s]);
+    }
+  }
+}
+
+template <typename XT, typename RT, int V, int SLOTS, int WAVES> __global__ __launch_bounds__(add_threads(WAVES)) void add_norm_bwd_kernel(AddArgs p) {
+  __shared__ float mem[4][16];
+  constexpr int LANES = 64 * WAVES, kAddThreads = add_threads(WAVES);
+  const int l = threadIdx.x % LANES;
+  const long long step = (long long)gridDim.x * (kAddThreads / LANES);
+  // sixteen waves leave a lane 128 registers: the scale is read again for every row, and the next row is not asked for ahead
+  constexpr bool AHEAD = WAVES < 16;
+  float dg[SLOTS][V], w[AHEAD ? SLOTS : 1][V];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    if constexpr (AHEAD) add_scale<V>(p, (l + LANES * s) * V, l + LANES * s < p.nvec, w[s]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) dg[s][e] = 0.f;
+  }
+  const float inv_d = 1.f / (float)p.D;
+  typename AddRow<RT, V>::Raw next_s[SLOTS], next_u[SLOTS];
+  typename AddRow<XT, V>::Raw next_d[SLOTS];
+  float next_inv = 0.f;
+  auto request = [&](long long row) {
+    next_inv = row < p.rows ? p.inv_in[row] : 0.f;
+    const rsrc_t rs = AddRow<RT, V>::row(p.sum, row, p.D, row < p.rows), rd = AddRow<XT, V>::row(p.dy, row, p.D, row < p.rows);
+    const rsrc_t ru = AddRow<RT, V>::row(p.ds, row, p.D, row < p.rows && p.ds);
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      next_s[s] = AddRow<RT, V>::request(rs, l + LANES * s);
+      next_d[s] = AddRow<XT, V>::request(rd, l + LANES * s);
+      next_u[s] = AddRow<RT, V>::request(ru, l + LANES * s);
+    }
+  };
+  long long row = (long long)blockIdx.x * (kAddThreads / LANES) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / LANES);
+  if (AHEAD) request(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    if (!AHEAD) request(row);
+    float v[SLOTS][V], d[SLOTS][V], u[SLOTS][V], dot = 0.f;
+    const float inv = next_inv;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      float again[V];
+      if constexpr (!AHEAD) add_scale<V>(p, (l + LANES * s) * V, l + LANES * s < p.nvec, again);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[s][e] = (float)next_s[s][e];
+        d[s][e] = (float)next_d[s][e];
+        u[s][e] = (float)next_u[s][e];
+        dg[s][e] = fmaf(d[s][e] * inv, v[s][e], dg[s][e]);
+        d[s][e] *= AHEAD ? w[AHEAD ? s : 0][e] : again[e];
+        dot = fmaf(d[s][e], v[s][e], dot);
+      }
+    }
+    if (AHEAD) request(row + step);
+    const float k = add_row_all<WAVES, false>(dot, mem, turn) * inv_d * inv * inv;
+    const rsrc_t rx = AddRow<XT, V>::row(p.dx, row, p.D, p.dx != nullptr), rr = AddRow<RT, V>::row(p.dr, row, p.D, p.dr != nullptr);
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[s][e] = fmaf(inv, fmaf(-k, v[s][e], d[s][e]), u[s][e]);
+      if (p.dx) AddRow<XT, V>::store(rx, l + LANES * s, d[s]);
+      if (p.dr) AddRow<RT, V>::store(rr, l + LANES * s, d[s]);
+    }
+  }
+  if (!p.partial) return;
+  if constexpr (LANES == kAddThreads) {
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) AddRow<float, V>::store(AddRow<float, V>::row(p.partial, blockIdx.x, p.D, true), l + LANES * s, dg[s]);
+    return;
+  }
+  // the workgroup's waves add up in LDS, one after the other
+  __shared__ float red[LANES == kAddThreads ? 1 : SLOTS * LANES * V];
+  for (int turn = 0; turn < kAddThreads / LANES; ++turn) {
+    if ((int)(threadIdx.x / LANES) == turn) {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float& to = red[(e * SLOTS + s) * LANES + l];
+          to = turn ? to + dg[s][e] : dg[s][e];
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < p.D; i += kAddThreads) {
+    const int vec = i / V, e = i - vec * V;
+    p.partial[(long long)blockIdx.x * p.D + i] = red[(e * SLOTS + vec / LANES) * LANES + vec % LANES];
+  }
+}
+
+static __global__ __launch_bounds__(256) void add_sums_kernel(SumJob j) {
+  __shared__ float red[8][32];
+  run_sum_job(j, (int)blockIdx.x, red);
+}
+
+// How a row lies in registers: waves and vectors a lane.
+struct AddShape { int v, nvec, waves, slots; };
+static AddShape add_shape(int64_t D, int dtype, bool whole) {
+  AddShape z;
+  z.v = whole ? (dtype == RGLRU_BF16 ? 8 : 4) : 1;
+  z.nvec = (int)(D / z.v);
+  z.waves = D <= 1024 ? 1 : D <= 4096 ? 4 : 16;
+  const int each = (z.nvec + 64 * z.waves - 1) / (64 * z.waves);
+  z.slots = 1;
+  while (z.slots < each) z.slots *= 2;
+  return z;
+}
+
+static int add_grid(int64_t rows, int waves, int per_unit) {
+  const long long each = waves == 1 ? 4 : 1, blocks = (rows + each - 1) / each, cap = (long long)num_compute_units() * per_unit;
+  return (int)(blocks < cap ? blocks : cap);
+}
+
+static int add_check(const char* who, int64_t rows, int64_t D, int dtype, int residual_dtype, int vec_dtype, std::initializer_list<const void*> ptrs, AddShape* z) {
+  for (int t : {dtype, residual_dtype})
+    if (t != RGLRU_F32 && t != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: dtype must be RGLRU_F32 or RGLRU_BF16, got %d", who, t);
+  if (vec_dtype != RGLRU_F32 && vec_dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown parameter dtype %d", who, vec_dtype);
+  if (rows <= 0 || D <= 0) return fail(RGLRU_E_ARG, "%s: sizes rows=%lld D=%lld", who, (long long)rows, (long long)D);
+  bool whole = D % (dtype == RGLRU_BF16 ? 8 : 4) == 0;
+  for (const void* q : ptrs) whole = whole && (uintptr_t)q % 16 == 0;
+  if (D > kAddMaxWidth) return fail(RGLRU_E_UNSUPPORTED, "%s: rows of %lld elements exceed the supported %d", who, (long long)D, kAddMaxWidth);
+  if (rows >= (1ll << 40) / D) return fail(RGLRU_E_UNSUPPORTED, "%s: tensor too large", who);
+  *z = add_shape(D, dtype, whole);
+  return RGLRU_OK;
+}
+
+// The compiled shapes: whole vectors of 8 (bf16 x) or 4 (fp32 x), and single elements.
+#define RGLRU_ADD_ONE(KERNEL, XT, RT, V, SLOTS, WAVES, ...) \
+  hipLaunchKernelGGL((KERNEL<XT, RT, V, SLOTS, WAVES __VA_ARGS__>), grid, dim3(add_threads(WAVES)), 0, (hipStream_t)stream, a)
+#define RGLRU_ADD_SLOTS(KERNEL, XT, RT, V, WAVES, ...)                                                          \
+  do {                                                                                                         \
+    if (z.slots * V <= 8) RGLRU_ADD_ONE(KERNEL, XT, RT, V, 8 / V, WAVES, __VA_ARGS__);                          \
+    else RGLRU_ADD_ONE(KERNEL, XT, RT, V, 16 / V, WAVES, __VA_ARGS__);                                          \
+  } while (0)
+#define RGLRU_ADD_TYPES(KERNEL, XT, RT, FULL, ...)                                                              \
+  do {                                                                                                         \
+    if (z.v == 1) {                                                                                            \
+      if (z.waves == 1) RGLRU_ADD_SLOTS(KERNEL, XT, RT, 1, 1, __VA_ARGS__);                                     \
+      else if (z.waves == 4) RGLRU_ADD_ONE(KERNEL, XT, RT, 1, 16, 4, __VA_ARGS__);                              \
+      else RGLRU_ADD_ONE(KERNEL, XT, RT, 1, 16, 16, __VA_ARGS__);                                               \
+    } else if (z.waves == 1) {                                                                                 \
+      RGLRU_ADD_SLOTS(KERNEL, XT, RT, FULL, 1, __VA_ARGS__);                                                    \
+    } else if (z.waves == 4) {                                                                                 \
+      RGLRU_ADD_SLOTS(KERNEL, XT, RT, FULL, 4, __VA_ARGS__);                                                    \
+    } else {                                                                                                   \
+      RGLRU_ADD_SLOTS(KERNEL, XT, RT, FULL, 16, __VA_ARGS__);                                                   \
+    }                                                                                                          \
+  } while (0)
+#define RGLRU_ADD_LAUNCH(KERNEL, ...)                                                                           \
+  do {                                                                                                         \
+    if (dtype == RGLRU_BF16) {                                                                                 \
+      if (residual_dtype == RGLRU_BF16) RGLRU_ADD_TYPES(KERNEL, __bf16, __bf16, 8, __VA_ARGS__);                \
+      else RGLRU_ADD_TYPES(KERNEL, __bf16, float, 8, __VA_ARGS__);                                              \
+    } else {                                                                                                   \
+      if (residual_dtype == RGLRU_BF16) RGLRU_ADD_TYPES(KERNEL, float, __bf16, 4, __VA_ARGS__);                 \
+      else RGLRU_ADD_TYPES(KERNEL, float, float, 4, __VA_ARGS__);                                               \
+    }                                                                                                          \
+  } while (0)
+#define RGLRU_COMMA ,
+
+}  // namespace rglru
+
+using namespace rglru;
+
+extern "C" {
+
+int rglru_hip_add_rmsnorm_max_width(void) { return kAddMaxWidth; }
+
+int rglru_hip_add_rmsnorm_fwd(const void* x, const void* residual, const void* g, void* sum, void* y, float* inv, int64_t rows, int64_t D, float eps,
+                              int dtype, int residual_dtype, int vec_dtype, void* stream) {
+  if (!x || !residual || !g || !sum || !y) return fail(RGLRU_E_ARG, "add_rmsnorm_fwd: null pointer");
+  AddShape z;
+  int rc = add_check("add_rmsnorm_fwd", rows, D, dtype, residual_dtype, vec_dtype, {x, residual, sum, y}, &z);
+  if (rc) return rc;
+  AddArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x; a.r = residual; a.g = g; a.sum = sum; a.y = y; a.inv = inv; a.rows = rows; a.D = (int)D; a.nvec = z.nvec; a.vec_dtype = vec_dtype; a.eps = eps;
+  const dim3 grid((unsigned)add_grid(rows, z.waves, 8));
+  RGLRU_ADD_LAUNCH(add_norm_kernel, RGLRU_COMMA false);
+  return check_launch("add_rmsnorm_fwd");
+}
+
+int rglru_hip_add_rmsnorm_quantised(const void* x, const void* residual, const void* g, void* sum, void* q, float* scale, int64_t rows, int64_t D, float eps,
+                                    int dtype, int residual_dtype, int vec_dtype, void* stream) {
+  if (!x || !g || !q || !scale || (residual != nullptr) != (sum != nullptr)) return fail(RGLRU_E_ARG, "add_rmsnorm_quantised: null pointer");
+  AddShape z;
+  int rc = add_check("add_rmsnorm_quantised", rows, D, dtype, residual_dtype, vec_dtype, {x, residual, sum, q}, &z);
+  if (rc) return rc;
+  AddArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x; a.r = residual; a.g = g; a.sum = sum; a.y = q; a.scale = scale; a.rows = rows; a.D = (int)D; a.nvec = z.nvec; a.vec_dtype = vec_dtype; a.eps = eps;
+  const dim3 grid((unsigned)add_grid(rows, z.waves, 8));
+  RGLRU_ADD_LAUNCH(add_norm_kernel, RGLRU_COMMA true);
+  return check_launch("add_rmsnorm_quantised");
+}
+
+size_t rglru_hip_add_rmsnorm_scratch_bytes(int64_t rows, int64_t D) {
+  if (rows <= 0 || D <= 0) return 0;
+  return (size_t)add_grid(rows, add_shape(D, RGLRU_F32, false).waves, 4) * (size_t)D * 4;
+}
+
+int rglru_hip_add_rmsnorm_bwd(const void* sum, const void* g, const float* inv, const void* dy, const void* dsum, void* scratch, void* dx, void* dresidual,
+                              void* dg, int64_t rows, int64_t D, int dtype, int residual_dtype, int vec_dtype, int grad_dtype, void* stream) {
+  if (!sum || !g || !inv || !dy || (dg && !scratch)) return fail(RGLRU_E_ARG, "add_rmsnorm_bwd: null pointer");
+  if (grad_dtype != RGLRU_F32 && grad_dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "add_rmsnorm_bwd: unknown gradient dtype %d", grad_dtype);
+  AddShape z;
+  int rc = add_check("add_rmsnorm_bwd", rows, D, dtype, residual_dtype, vec_dtype, {sum, dy, dsum, dx, dresidual}, &z);
+  if (rc) return rc;
+  AddArgs a;
+  memset(&a, 0, sizeof(a));
+  a.sum = const_cast<void*>(sum); a.g = g; a.inv_in = inv; a.dy = dy; a.ds = dsum; a.dx = dx; a.dr = dresidual; a.partial = dg ? (float*)scratch : nullptr;
+  a.rows = rows; a.D = (int)D; a.nvec = z.nvec; a.vec_dtype = vec_dtype;
+  const int blocks = add_grid(rows, z.waves, 4);
+  const dim3 grid((unsigned)blocks);
+  RGLRU_ADD_LAUNCH(add_norm_bwd_kernel, );
+  rc = check_launch("add_rmsnorm_bwd");
+  if (rc || !dg) return rc;
+  SumJob j;
+  memset(&j, 0, sizeof(j));
+  j.src = a.partial; j.dst = dg; j.n = D; j.sets = blocks; j.dst_bf16 = grad_dtype == RGLRU_BF16;
+  plan_sum_job(j);
+  hipLaunchKernelGGL(add_sums_kernel, dim3((unsigned)j.blocks), dim3(256), 0, (hipStream_t)stream, j);
+  return check_launch("add_rmsnorm_bwd sums");
+}
+
+}  // extern "C"

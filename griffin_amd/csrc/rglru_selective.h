@@ -1,0 +1,240 @@
+// Selective state space scan: each channel w carries N numbers, which its token's step size s_t lets decay and which read and write the
+// vectors B_t, C_t of the channel's group,
+//   h_t[n] = exp(s_t A[n]) h_{t-1}[n] + s_t u_t B_t[n],   y_t = sum_n C_t[n] h_t[n] + D u_t,   out_t = y_t silu(z_t),   s_t = softplus(dt_t + bias)
+//
+// A wave owns 16 channels and 16 of their states and walks the tokens in tiles of 16.  Lane (c = lane % 16, j = lane / 16) holds the states
+// 4 j .. 4 j + 3 of channel c, so that
+//   - B and C of a tile are four registers each: lane k of a row of 16 lanes holds token k's elements 4 j .. + 3, and a product takes them from there by
+//     its own operand's row broadcast.  Neither goes through LDS, whose reads of 16 bytes a lane (17 cycles a wave) would be the bound;
+//   - what a token and channel need once (step size, gates, rounding) is computed by one lane each, (c, j) for the tokens 4 q + j, and goes to the other
+//     rows through 2 KB of LDS that belong to the wave: no wave waits for another;
+//   - sums over the states are three adds of registers and two swaps of rows for four tokens.
+// More than 16 states: two or four waves of a workgroup share 16 channels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <utility>
+
+#include "rglru_device.h"
+#include "rglru_host.h"
+
+namespace rglru {
+
+constexpr int kSelThreads = 256;
+constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kSelTile = 16;                  // tokens of a tile; the forward pass keeps the state in front of every tile for the backward pass
+constexpr int kSelLanes = 16;                 // channels of a wave
+constexpr int kSelStates = 16;                // states of a wave
+constexpr int kSelMaxStates = 64;
+constexpr int kSelMaxSegments = 64;
+constexpr unsigned kSelRange = 0x7fffff00u;   // bytes of a tile's buffers; kOutOfRange lies outside
+
+struct SelArgs {
+  const void *u, *dt, *z, *Bm, *Cm, *dout;    // z: or null
+  const float *A, *D, *bias, *h0, *dh_last;   // D, bias, h0, dh_last: or null
+  const unsigned char* flags;                 // or null
+  void *y, *du, *ddt, *dz;
+  float *h_last, *dh0;
+  float* kept;                                // [B][tiles][W][N]: states in front of tiles, or null
+  float* ends;                                // [B][S][W][N]: what a segment leaves of a state (a gradient) of zeros
+  float* sums;                                // [B][S][W][2]: a segment's sum of step sizes; whether a document starts in it
+  float *dB, *dC;                             // [sets][B][T][G][N], a set for each workgroup of a group
+  float *dA, *dD, *dbias;                     // [B][S][W][N], [B][S][W]
+  long long sub, sut, sdb, sdt, szb, szt, sBb, sBt, sBg, sCb, sCt, sCg;  // elements between batch rows, tokens and groups
+  int B, T, W, N, G, Wg;                      // Wg: channels of a group
+  int per_group;                              // workgroups of a group's channels
+  int S, tiles, seg_tiles;                    // segments, tiles of a sequence and of a segment
+  int softplus, vector;                       // vector: rows of B and C go by whole vectors of four elements
+};
+
+// A place of the walk: what all lanes of a wave share.
+struct SelPlace {
+  int b, seg, g, set, slab, cg;
+};
+template <int SLABS> RGLRU_DEVICE SelPlace sel_place(const SelArgs& p) {
+  SelPlace r;
+  unsigned i = blockIdx.x;
+  r.set = (int)(i % (unsigned)p.per_group); i /= (unsigned)p.per_group;
+  r.g = (int)(i % (unsigned)p.G); i /= (unsigned)p.G;
+  r.seg = (int)(i % (unsigned)p.S);
+  r.b = (int)(i / (unsigned)p.S);
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  r.slab = wave % SLABS;
+  r.cg = (r.set * kSelWaves + wave) / SLABS;
+  return r;
+}
+
+template <int CONTROL> RGLRU_DEVICE float sel_move(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
+// Lane K of every row of 16 lanes, for the whole row.
+template <int K> RGLRU_DEVICE float row_bcast(float v) { return sel_move<0x150 + K>(v); }
+
+// a's two lower rows beside b's two lower rows, and the upper ones: the sum of the two holds a's sum over row pairs in the lower half, b's in the upper.
+RGLRU_DEVICE float halves_sum(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+RGLRU_DEVICE float rows_sum(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+// Sums over the four rows of v[0 .. 3]: row j receives that of v[j].
+RGLRU_DEVICE float four_rows_sum(const float (&v)[4]) { return rows_sum(halves_sum(v[0], v[2]), halves_sum(v[1], v[3])); }
+RGLRU_DEVICE float all_rows_sum(float v) {
+  const float h = halves_sum(v, v);
+  return rows_sum(h, h);
+}
+
+// Sums over the 16 lanes of a row of v[token][i]: lane 8 t1 + 4 t0 + 2 i1 + i0 of a row receives that of v[2 t1 + t0][2 i1 + i0].  Each step sends half of
+// what a lane holds to the lane that keeps it.
+RGLRU_DEVICE float lanes_scatter_sum(const float (&v)[4][4], int lane) {
+  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+  float r[2][4], q[4], s[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[t][i] = (b3 ? v[2 + t][i] : v[t][i]) + sel_move<0x128>(b3 ? v[t][i] : v[2 + t][i]);   // eight lanes on
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = (b2 ? r[1][i] : r[0][i]) + sel_move<0x141>(b2 ? r[0][i] : r[1][i]);                // eight lanes mirrored
+#pragma unroll
+  for (int i = 0; i < 2; ++i) s[i] = (b1 ? q[2 + i] : q[i]) + sel_move<0x4e>(b1 ? q[i] : q[2 + i]);
+  return (b0 ? s[1] : s[0]) + sel_move<0xb1>(b0 ? s[0] : s[1]);
+}
+
+// Writes of some lanes of a wave before reads of others: LDS serves a wave in order, so only the compiler has to keep it.
+RGLRU_DEVICE void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// softplus and its slope.  log(1 + e), e = exp(-|x|) in (0, 1], is 2 artanh(e / (2 + e)) by its series: 1.4e-8 relative at e = 1, and exact where
+// 1 + e would round e away.
+struct SelRate { float s, slope; };
+RGLRU_DEVICE SelRate sel_rate(float x, bool soft) {
+  SelRate r;
+  if (!soft) { r.s = x; r.slope = 1.f; return r; }
+  const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
+  const float v = e * __builtin_amdgcn_rcpf(2.f + e), v2 = v * v;
+  float q = 1.f / 13.f;
+  q = fmaf(q, v2, 1.f / 11.f);
+  q = fmaf(q, v2, 1.f / 9.f);
+  q = fmaf(q, v2, 1.f / 7.f);
+  q = fmaf(q, v2, 1.f / 5.f);
+  q = fmaf(q, v2, 1.f / 3.f);
+  q = fmaf(q, v2, 1.f);
+  r.s = fmaxf(x, 0.f) + 2.f * v * q;
+  r.slope = (x >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+  return r;
+}
+
+// Tokens t0 + 4 q + j (q = 0 .. 3) of one operand, a channel a lane.
+template <typename IO> struct SelStream {
+  float v[4];
+  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int c, int left, bool ok, int j) {
+    const rsrc_t r = make_rsrc((const IO*)base + at, kSelRange);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int t = 4 * q + j;
+      v[q] = BufIo<IO>::load(r, ok && t < left ? ((unsigned)t * stride + (unsigned)c) * (unsigned)sizeof(IO) : kOutOfRange, 0);
+    }
+  }
+};
+template <typename IO> RGLRU_DEVICE void sel_store(const float (&v)[4], void* base, long long at, unsigned stride, int c, int left, bool ok, int j) {
+  const rsrc_t r = make_rsrc((IO*)base + at, kSelRange);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int t = 4 * q + j;
+    BufIo<IO>::store((IO)v[q], r, ok && t < left ? ((unsigned)t * stride + (unsigned)c) * (unsigned)sizeof(IO) : kOutOfRange, 0);
+  }
+}
+
+// Elements n0 .. n0 + 3 of token t0 + lane % 16 of B or C.
+template <typename IO> struct SelVector {
+  float v[4];
+  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int n0, int N, int left, int k, bool vector) {
+    const rsrc_t r = make_rsrc((const IO*)base + at, kSelRange);
+    const unsigned off = ((unsigned)k * stride + (unsigned)n0) * (unsigned)sizeof(IO);
+    if (vector) {
+      const unsigned o = k < left && n0 < N ? off : kOutOfRange;
+      if constexpr (sizeof(IO) == 2) {
+        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        v[0] = __uint_as_float(w[0] << 16); v[1] = __uint_as_float(w[0] & 0xffff0000u);
+        v[2] = __uint_as_float(w[1] << 16); v[3] = __uint_as_float(w[1] & 0xffff0000u);
+      } else {
+        const f32x4 w = buf_load_frag<f32x4>(r, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = w[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = BufIo<IO>::load(r, k < left && n0 + i < N ? off + (unsigned)(i * sizeof(IO)) : kOutOfRange, 0);
+    }
+  }
+};
+
+// Four states of a lane, at p + n0 .. (rows of N).
+RGLRU_DEVICE void sel_load_states(const float* p, long long row, int n0, int N, bool ok, float (&v)[4]) {
+  const float* at = p + row * N + n0;
+  if (ok && n0 + 4 <= N && ((uintptr_t)at & 15) == 0) {
+    const f32x4 w = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ok && n0 + i < N ? at[i] : 0.f;
+  }
+}
+RGLRU_DEVICE void sel_store_states(float* p, long long row, int n0, int N, bool ok, const float (&v)[4]) {
+  float* at = p + row * N + n0;
+  if (ok && n0 + 4 <= N && ((uintptr_t)at & 15) == 0) {
+    *reinterpret_cast<f32x4*>(at) = (f32x4){v[0], v[1], v[2], v[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (ok && n0 + i < N) at[i] = v[i];
+  }
+}
+
+// The masks of a tile's tokens, the same in all lanes: bit k is token t0 + k's.  Tokens behind the sequence's end are inactive.
+struct SelMasks { unsigned live, starts; };
+template <bool MASKED> RGLRU_DEVICE SelMasks sel_masks(const unsigned char* flags, long long at, int left, int lane) {
+  SelMasks m;
+  m.starts = 0;
+  if constexpr (MASKED) {
+    const int k = lane & 15;
+    const unsigned f = k < left ? flags[at + k] : 2u;
+    m.live = (unsigned)__ballot(!(f & 2u)) & 0xffffu;
+    m.starts = (unsigned)__ballot((f & 3u) == 1u) & 0xffffu;
+  } else {
+    m.live = left >= 16 ? 0xffffu : (1u << left) - 1u;
+  }
+  return m;
+}
+
+// Calls f with the constants 0 .. N - 1.
+template <typename F, int... K> RGLRU_DEVICE void sel_each(F&& f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
+template <int N, typename F> RGLRU_DEVICE void sel_each(F&& f) { sel_each(f, std::make_integer_sequence<int, N>{}); }
+
+// What the segments in front (behind, for gradients) of this one leave of the state that enters the first (last) of them: a few dozen at most, each
+// multiplies by exp(A sum) unless a document starts in it.
+template <bool REVERSE> RGLRU_DEVICE void sel_join(const SelArgs& p, const SelPlace& at, int w, int n0, bool ok, const float (&a2)[4], float (&h)[4]) {
+  const int count = REVERSE ? p.S - 1 - at.seg : at.seg;
+  for (int r = 0; r < count; ++r) {
+    const long long row = ((long long)at.b * p.S + (REVERSE ? p.S - 1 - r : r)) * p.W + w;
+    float e[4];
+    sel_load_states(p.ends, row, n0, p.N, ok, e);
+    const float sum = ok ? p.sums[2 * row] : 0.f;
+    const bool cut = ok && p.sums[2 * row + 1] != 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = cut ? e[i] : fmaf(__builtin_amdgcn_exp2f(a2[i] * sum), h[i], e[i]);
+  }
+}
+
+int sel_launch_forward(const SelArgs& a, int dtype, hipStream_t s);
+int sel_launch_backward(const SelArgs& a, void* dB, void* dC, float* dA, float* dD, float* dbias, int dtype, hipStream_t s);
+
+}  // namespace rglru

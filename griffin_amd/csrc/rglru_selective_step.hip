@@ -1,0 +1,195 @@
+// Selective state space scan, one token a row with the state updated in place, and the C entry points of all its kernels.
+
+#include <hip/hip_runtime.h>
+
+#include <cstring>
+
+#include "rglru_selective.h"
+
+namespace rglru {
+
+struct SelStepArgs {
+  const void *u, *dt, *z, *Bm, *Cm;
+  const float *A, *D, *bias;
+  const unsigned char* flags;
+  float* state;
+  void* y;
+  long long su, sdt, sz, sBb, sBg, sCb, sCg;
+  int B, W, N, Wg, lanes, softplus;
+};
+
+// Four states a lane, N / 4 lanes (a power of two) a channel: the state is read and written once, in whole vectors, one behind the other.
+template <typename IO> __global__ __launch_bounds__(kSelThreads) void sel_step_kernel(SelStepArgs p) {
+  const long long item = (long long)blockIdx.x * kSelThreads + threadIdx.x;
+  const long long channel = item / p.lanes;
+  const int l = (int)(item % p.lanes), n0 = 4 * l;
+  const bool there = channel < (long long)p.B * p.W;
+  const int b = there ? (int)(channel / p.W) : 0, w = there ? (int)(channel - (long long)b * p.W) : 0, g = w / p.Wg;
+  const unsigned flag = p.flags ? p.flags[b] : 0u;
+  const bool live = !(flag & 2u);
+  const long long row = (long long)b * p.W + w;
+  float a[4], h[4], y = 0.f;
+  sel_load_states(p.state, row, n0, p.N, there && flag == 0u, h);
+  sel_load_states(p.A, w, n0, p.N, there, a);
+  const float u = (float)((const IO*)p.u)[b * p.su + w];
+  const float s = sel_rate((float)((const IO*)p.dt)[b * p.sdt + w] + (p.bias ? p.bias[w] : 0.f), p.softplus).s, su = s * u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool has = n0 + i < p.N;
+    const float vb = has ? (float)((const IO*)p.Bm)[b * p.sBb + g * p.sBg + n0 + i] : 0.f;
+    const float vc = has ? (float)((const IO*)p.Cm)[b * p.sCb + g * p.sCg + n0 + i] : 0.f;
+    h[i] = fmaf(__builtin_amdgcn_exp2f(a[i] * kLog2e * s), h[i], vb * su);
+    y = fmaf(vc, h[i], y);
+  }
+  for (int m = 1; m < p.lanes; m <<= 1) y += __shfl_xor(y, m, 64);
+  if (!there) return;
+  if (live) sel_store_states(p.state, row, n0, p.N, true, h);
+  if (l == 0) {
+    if (p.D) y = fmaf(p.D[w], u, y);
+    if (p.z) {
+      const float z = (float)((const IO*)p.z)[b * p.sz + w];
+      y *= z * sigmoid_fast(z);
+    }
+    ((IO*)p.y)[row] = (IO)(live ? y : 0.f);
+  }
+}
+
+static size_t sel_bytes(long long floats) { return ((size_t)floats * 4 + 255) & ~(size_t)255; }
+
+// Segments of a sequence.  One workgroup a compute unit leaves each SIMD one wave, which issues at half the rate that two reach; but a sequence in
+// segments is walked twice.
+static int sel_segments(int64_t B, int64_t G, int64_t per_group, int64_t tiles) {
+  const long long wgs = B * G * per_group, units = num_compute_units();
+  if (wgs >= units) return 1;
+  long long s = 2 * units / wgs;
+  if (s > tiles / 4) s = tiles / 4;
+  if (s > kSelMaxSegments) s = kSelMaxSegments;
+  if (s < 2) return 1;
+  const long long each = (tiles + s - 1) / s;
+  return (int)((tiles + each - 1) / each);
+}
+
+static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N) {
+  if (B <= 0 || T <= 0 || W <= 0 || G <= 0 || N <= 0 || W % G || N > kSelMaxStates || W >= (1 << 22) || T >= (1ll << 31) - 64 || B >= (1ll << 31)) return false;
+  const int slabs = N <= 16 ? 1 : N <= 32 ? 2 : 4;
+  a->B = (int)B; a->T = (int)T; a->W = (int)W; a->N = (int)N; a->G = (int)G; a->Wg = (int)(W / G);
+  a->per_group = (int)((((W / G) + kSelLanes - 1) / kSelLanes * slabs + kSelWaves - 1) / kSelWaves);
+  a->tiles = (int)((T + kSelTile - 1) / kSelTile);
+  if (B * G * a->per_group >= (1ll << 24)) return false;
+  a->S = sel_segments(B, G, a->per_group, a->tiles);
+  a->seg_tiles = (a->tiles + a->S - 1) / a->S;
+  return B * (long long)a->S * G * a->per_group < (1ll << 24);
+}
+
+static int sel_check(const char* who, SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype) {
+  if (dtype != RGLRU_F32 && dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: dtype must be RGLRU_F32 or RGLRU_BF16, got %d", who, dtype);
+  if (B <= 0 || T <= 0 || W <= 0 || G <= 0 || N <= 0 || W % G)
+    return fail(RGLRU_E_ARG, "%s: sizes B=%lld T=%lld W=%lld G=%lld N=%lld", who, (long long)B, (long long)T, (long long)W, (long long)G, (long long)N);
+  if (N > kSelMaxStates) return fail(RGLRU_E_UNSUPPORTED, "%s: %lld states a channel exceed the supported %d", who, (long long)N, kSelMaxStates);
+  memset(a, 0, sizeof(*a));
+  if (!sel_plan(a, B, T, W, G, N)) return fail(RGLRU_E_UNSUPPORTED, "%s: tensor too large", who);
+  return RGLRU_OK;
+}
+
+// Distances between batch rows, tokens and groups: of u, dt, z (two each), B, C (three each).
+static int sel_strides(const char* who, SelArgs* a, const int64_t* s, int dtype) {
+  const int64_t tokens[5] = {s[1], s[3], s[5], s[7], s[10]};
+  for (int64_t t : tokens)
+    if (t < 0 || t >= (1 << 22)) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens %lld elements apart", who, (long long)t);
+  a->sub = s[0]; a->sut = s[1]; a->sdb = s[2]; a->sdt = s[3]; a->szb = s[4]; a->szt = s[5];
+  a->sBb = s[6]; a->sBt = s[7]; a->sBg = s[8]; a->sCb = s[9]; a->sCt = s[10]; a->sCg = s[11];
+  bool whole = a->N % 4 == 0;
+  for (int i = 6; i < 12; ++i) whole = whole && s[i] % 4 == 0;
+  const uintptr_t boundary = dtype == RGLRU_BF16 ? 8 : 16;
+  a->vector = whole && (uintptr_t)a->Bm % boundary == 0 && (uintptr_t)a->Cm % boundary == 0;
+  return RGLRU_OK;
+}
+
+}  // namespace rglru
+
+using namespace rglru;
+
+extern "C" {
+
+int rglru_hip_selective_max_states(void) { return kSelMaxStates; }
+
+size_t rglru_hip_selective_workspace_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int keep) {
+  SelArgs a;
+  if (!sel_plan(&a, B, T, W, G, N)) return 0;
+  size_t n = keep ? sel_bytes((long long)B * a.tiles * W * N) : 0;
+  if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
+  return n + 256;
+}
+
+size_t rglru_hip_selective_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N) {
+  SelArgs a;
+  if (!sel_plan(&a, B, T, W, G, N)) return 0;
+  size_t n = 2 * sel_bytes((long long)a.per_group * B * T * G * N) + sel_bytes((long long)B * a.S * W * N) + 2 * sel_bytes((long long)B * a.S * W);
+  if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
+  return n;
+}
+
+int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                            const float* D, const float* bias, const float* h0, const uint8_t* flags, void* y, float* h_last, void* ws, int keep,
+                            int softplus, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream) {
+  SelArgs a;
+  int rc = sel_check("selective_fwd", &a, B, T, W, G, N, dtype);
+  if (rc) return rc;
+  if (!u || !dt || !Bm || !Cm || !strides || !A || !y || !h_last || !ws) return fail(RGLRU_E_ARG, "selective_fwd: null pointer");
+  a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.A = A; a.D = D; a.bias = bias; a.h0 = h0; a.flags = flags; a.y = y; a.h_last = h_last;
+  a.softplus = softplus;
+  rc = sel_strides("selective_fwd", &a, strides, dtype);
+  if (rc) return rc;
+  char* at = (char*)ws;
+  if (keep) { a.kept = (float*)at; at += sel_bytes((long long)B * a.tiles * W * N); }
+  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + sel_bytes((long long)B * a.S * W * N)); }
+  return sel_launch_forward(a, dtype, (hipStream_t)stream);
+}
+
+int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                            const float* D, const float* bias, const uint8_t* flags, const void* dout, const float* dh_last, const void* ws, void* scratch,
+                            void* du, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* dbias, float* dh0, int softplus, int64_t B,
+                            int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream) {
+  SelArgs a;
+  int rc = sel_check("selective_bwd", &a, B, T, W, G, N, dtype);
+  if (rc) return rc;
+  if (!u || !dt || !Bm || !Cm || !strides || !A || !dout || !ws || !scratch || !du || !ddt || (z && !dz) || !dB || !dC)
+    return fail(RGLRU_E_ARG, "selective_bwd: null pointer");
+  a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.A = A; a.D = D; a.bias = bias; a.flags = flags; a.dout = dout; a.dh_last = dh_last;
+  a.du = du; a.ddt = ddt; a.dz = dz; a.dh0 = dh0; a.softplus = softplus;
+  rc = sel_strides("selective_bwd", &a, strides, dtype);
+  if (rc) return rc;
+  a.kept = (float*)const_cast<void*>(ws);
+  char* at = (char*)scratch;
+  const size_t vectors = sel_bytes((long long)a.per_group * B * T * G * N), states = sel_bytes((long long)B * a.S * W * N), rows = sel_bytes((long long)B * a.S * W);
+  a.dB = (float*)at; at += vectors;
+  a.dC = (float*)at; at += vectors;
+  a.dA = (float*)at; at += states;
+  a.dD = (float*)at; at += rows;
+  a.dbias = (float*)at; at += rows;
+  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + states); }
+  return sel_launch_backward(a, dB, dC, dA, dD, dbias, dtype, (hipStream_t)stream);
+}
+
+int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                             const float* D, const float* bias, const uint8_t* flags, float* state, void* y, int softplus, int64_t B, int64_t W, int64_t G,
+                             int64_t N, int dtype, void* stream) {
+  SelArgs a;
+  int rc = sel_check("selective_step", &a, B, 1, W, G, N, dtype);
+  if (rc) return rc;
+  if (!u || !dt || !Bm || !Cm || !strides || !A || !state || !y) return fail(RGLRU_E_ARG, "selective_step: null pointer");
+  SelStepArgs p;
+  memset(&p, 0, sizeof(p));
+  p.u = u; p.dt = dt; p.z = z; p.Bm = Bm; p.Cm = Cm; p.A = A; p.D = D; p.bias = bias; p.flags = flags; p.state = state; p.y = y;
+  p.su = strides[0]; p.sdt = strides[1]; p.sz = strides[2]; p.sBb = strides[3]; p.sBg = strides[4]; p.sCb = strides[5]; p.sCg = strides[6];
+  p.B = (int)B; p.W = (int)W; p.N = (int)N; p.Wg = (int)(W / G); p.softplus = softplus;
+  p.lanes = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
+  const long long blocks = (B * W * p.lanes + kSelThreads - 1) / kSelThreads;
+  if (blocks >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "selective_step: tensor too large");
+  const dim3 grid((unsigned)blocks), block(kSelThreads);
+  if (dtype == RGLRU_BF16) hipLaunchKernelGGL((sel_step_kernel<__bf16>), grid, block, 0, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL((sel_step_kernel<float>), grid, block, 0, (hipStream_t)stream, p);
+  return check_launch("selective_step");
+}
+
+}  // extern "C"

@@ -2381,6 +2381,409 @@ Tensor gated_delta_step(const Tensor& q_in, const Tensor& k_in, const Tensor& v_
   return out;
 }
 
+// ---- selective state space scan -----------------------------------------------------------------------------------
+
+// u, dt, z, B and C as the kernels read them: the last axis contiguous, the others with strides of their own (parts of one projection go in as they are).
+struct SelectiveOperands {
+  Tensor u, dt, z, B, C, A, D, bias;
+  int64_t strides[12];
+  // an axis of one element has no distance, whatever its tensor says
+  static int64_t distance(const Tensor& t, int64_t axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); }
+  static Tensor rows(const Tensor& t, int64_t token_axis) {
+    if (!t.defined()) return t;
+    const bool plain = t.stride(-1) == 1 || t.size(-1) == 1;
+    return plain && (token_axis < 0 || distance(t, token_axis) < (int64_t(1) << 22)) ? t : t.contiguous();
+  }
+  SelectiveOperands(const Tensor& u_in, const Tensor& dt_in, const Tensor& z_in, const Tensor& B_in, const Tensor& C_in, const Tensor& A_in,
+                    const Tensor& D_in, const Tensor& bias_in, bool sequence)
+      : u(rows(u_in, sequence ? 1 : -1)), dt(rows(dt_in, sequence ? 1 : -1)), z(rows(z_in, sequence ? 1 : -1)), B(rows(B_in, sequence ? 1 : -1)),
+        C(rows(C_in, sequence ? 1 : -1)), A(as(A_in, at::kFloat)), D(as(D_in, at::kFloat)), bias(as(bias_in, at::kFloat)) {
+    distances(sequence);
+  }
+  SelectiveOperands(const variable_list& s) : u(s[0]), dt(s[1]), z(s[2]), B(s[3]), C(s[4]), A(s[5]), D(s[6]), bias(s[7]) { distances(true); }
+  void distances(bool sequence) {
+    int at = 0;
+    for (const Tensor* t : {&u, &dt, &z})
+      for (int64_t axis = 0; axis < (sequence ? 2 : 1); ++axis) strides[at++] = t->defined() ? distance(*t, axis) : 0;
+    for (const Tensor* t : {&B, &C})
+      for (int64_t axis = 0; axis < (sequence ? 3 : 2); ++axis) strides[at++] = distance(*t, axis);
+  }
+};
+
+void check_selective(const char* name, const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& D, const Tensor& z,
+                     const Tensor& bias, int64_t axes) {
+  const char* lead = axes == 3 ? "[batch, sequence, " : "[batch, ";
+  TORCH_CHECK_VALUE(u.dim() == axes && dt.sizes() == u.sizes() && (!z.defined() || z.sizes() == u.sizes()), name, " expects u, dt and z of one shape ", lead,
+                    "width], got ", u.sizes(), ", ", dt.sizes(), " and ", z.defined() ? z.sizes() : u.sizes());
+  TORCH_CHECK_VALUE(B.dim() == axes + 1 && C.sizes() == B.sizes() && B.sizes().slice(0, axes - 1) == u.sizes().slice(0, axes - 1), name,
+                    " expects B and C of one shape ", lead, "groups, states] beside u of shape ", u.sizes(), ", got ", B.sizes(), " and ", C.sizes());
+  TORCH_CHECK_VALUE(A.dim() == 2 && A.size(0) == u.size(-1) && A.size(1) == B.size(-1), name, " expects A of shape [", u.size(-1), ", ", B.size(-1), "], got ",
+                    A.sizes());
+  for (const Tensor* t : {&D, &bias})
+    TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 1 && t->size(0) == u.size(-1)), name, " expects D and dt_bias of shape [", u.size(-1), "], got ", t->sizes());
+  TORCH_CHECK_VALUE(u.numel() > 0 && B.numel() > 0, name, " does not accept empty batches, sequences, widths or states");
+  TORCH_CHECK_VALUE(u.size(-1) % B.size(-2) == 0, name, " expects the width to be a multiple of the groups, got ", u.size(-1), " and ", B.size(-2));
+  TORCH_CHECK_VALUE(B.size(-1) <= rglru_hip_selective_max_states(), name, ": ", B.size(-1), " states a channel, at most ", rglru_hip_selective_max_states(),
+                    " are covered");
+  TORCH_CHECK_TYPE(known(u.scalar_type()) && dt.scalar_type() == u.scalar_type() && B.scalar_type() == u.scalar_type() && C.scalar_type() == u.scalar_type() &&
+                       (!z.defined() || z.scalar_type() == u.scalar_type()),
+                   name, " expects u, dt, z, B and C all in float32 or all in bfloat16, got ", u.scalar_type(), ", ", dt.scalar_type(), ", ",
+                   z.defined() ? z.scalar_type() : u.scalar_type(), ", ", B.scalar_type(), " and ", C.scalar_type());
+  for (const Tensor* t : {&A, &D, &bias})
+    TORCH_CHECK_TYPE(!t->defined() || known(t->scalar_type()), name, " expects A, D and dt_bias in float32 or bfloat16, got ", t->scalar_type());
+}
+
+struct SelectiveResult {
+  Tensor y, h_last, kept;
+};
+
+SelectiveResult selective_forward(const SelectiveOperands& o, const Tensor& h0_in, const Tensor& flags, bool softplus, bool keep) {
+  SelectiveResult r;
+  const int64_t B = o.u.size(0), T = o.u.size(1), W = o.u.size(2), G = o.B.size(2), N = o.B.size(3);
+  Tensor h0 = as(h0_in, at::kFloat);
+  const size_t size = rglru_hip_selective_workspace_bytes(B, T, W, G, N, keep ? 1 : 0);
+  TORCH_CHECK_VALUE(size > 0, "hip selective scan: tensor too large");
+  r.y = fresh({B, T, W}, o.u.scalar_type(), o.u);
+  r.h_last = fresh({B, W, N}, at::kFloat, o.u);
+  r.kept = bytes(size, o.u);
+  check(rglru_hip_selective_fwd(ptr(o.u), ptr(o.dt), ptr(o.z), ptr(o.B), ptr(o.C), o.strides, fptr(o.A), fptr(o.D), fptr(o.bias), fptr(h0), bptr(flags),
+                                ptr(r.y), fptr(r.h_last), ptr(r.kept), keep ? 1 : 0, softplus ? 1 : 0, B, T, W, G, N, code_of(o.u.scalar_type()),
+                                stream_of(o.u)),
+        "rglru_hip_selective_fwd");
+  return r;
+}
+
+struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                               const MaybeTensor& D_, const MaybeTensor& z_, const MaybeTensor& bias_, const MaybeTensor& h0_, const MaybeTensor& flags_,
+                               bool softplus) {
+    Tensor D = opt(D_), z = opt(z_), bias = opt(bias_), h0 = opt(h0_), flags = opt(flags_);
+    note_arguments(ctx, {true, true, true, true, true, D.defined(), z.defined(), bias.defined(), h0.defined()});
+    c10::DeviceGuard guard(u.device());
+    SelectiveOperands o(u, dt, z, B, C, A, D, bias, true);
+    SelectiveResult r = selective_forward(o, h0, flags, softplus, true);
+    ctx->save_for_backward({o.u, o.dt, o.z, o.B, o.C, o.A, o.D, o.bias, flags, r.kept});
+    pack(ctx, {softplus, type_or_none(A), type_or_none(D), type_or_none(bias), type_or_none(h0)});
+    ctx->set_materialize_grads(false);
+    return {r.y, r.h_last};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    auto saved = ctx->get_saved_variables();
+    auto m = unpack(ctx);
+    Tensor du, ddt, dA, dB, dC, dD, dz, dbias, dh0;
+    {
+      at::NoGradGuard no_grad;
+      SelectiveOperands o(saved);
+      const Tensor &flags = saved[8], &kept = saved[9];
+      c10::DeviceGuard guard(o.u.device());
+      Needs needs(ctx);
+      const auto dtype = o.u.scalar_type();
+      const int64_t B = o.u.size(0), T = o.u.size(1), W = o.u.size(2), G = o.B.size(2), N = o.B.size(3);
+      Tensor dout = grads[0].defined() ? as(grads[0], dtype) : at::zeros({B, T, W}, o.u.options());
+      Tensor dh_last = as(grads[1], at::kFloat);
+      du = fresh({B, T, W}, dtype, o.u), ddt = fresh({B, T, W}, dtype, o.u);
+      dB = fresh({B, T, G, N}, dtype, o.u), dC = fresh({B, T, G, N}, dtype, o.u);
+      if (o.z.defined()) dz = fresh({B, T, W}, dtype, o.u);
+      if (needs(2)) dA = fresh({W, N}, at::kFloat, o.u);
+      if (needs(5)) dD = fresh({W}, at::kFloat, o.u);
+      if (needs(7)) dbias = fresh({W}, at::kFloat, o.u);
+      if (needs(8)) dh0 = fresh({B, W, N}, at::kFloat, o.u);
+      Tensor scratch = bytes(rglru_hip_selective_scratch_bytes(B, T, W, G, N), o.u);
+      check(rglru_hip_selective_bwd(ptr(o.u), ptr(o.dt), ptr(o.z), ptr(o.B), ptr(o.C), o.strides, fptr(o.A), fptr(o.D), fptr(o.bias), bptr(flags), ptr(dout),
+                                    fptr(dh_last), ptr(kept), ptr(scratch), ptr(du), ptr(ddt), ptr(dz), ptr(dB), ptr(dC), fptr(dA), fptr(dD), fptr(dbias),
+                                    fptr(dh0), static_cast<int>(m[0]), B, T, W, G, N, code_of(dtype), stream_of(o.u)),
+            "rglru_hip_selective_bwd");
+      if (dA.defined()) dA = dA.to(type_at(m, 1));
+      if (dD.defined()) dD = dD.to(type_at(m, 2));
+      if (dbias.defined()) dbias = dbias.to(type_at(m, 3));
+      if (dh0.defined()) dh0 = dh0.to(type_at(m, 4));
+    }
+    return once({du, ddt, dA, dB, dC, dD, dz, dbias, dh0, Tensor(), Tensor()});
+  }
+};
+
+std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const MaybeTensor& D_,
+                                          const MaybeTensor& z_, const MaybeTensor& bias_, const MaybeTensor& h0_, const MaybeTensor& flags_, bool softplus) {
+  const char* name = "hip selective scan";
+  Tensor D = opt(D_), z = opt(z_), bias = opt(bias_), h0 = opt(h0_), flags = opt(flags_);
+  require_gpu(name, {&u, &dt, &A, &B, &C, &D, &z, &bias, &h0, &flags});
+  require_device_of(name, u, {&dt, &A, &B, &C, &D, &z, &bias, &h0, &flags});
+  check_selective(name, u, dt, A, B, C, D, z, bias, 3);
+  TORCH_CHECK_VALUE(!h0.defined() || (h0.dim() == 3 && h0.size(0) == u.size(0) && h0.size(1) == u.size(2) && h0.size(2) == B.size(3)),
+                    "initial state must have shape (", u.size(0), ", ", u.size(2), ", ", B.size(3), ")");
+  TORCH_CHECK_TYPE(!h0.defined() || known(h0.scalar_type()), name, " expects an initial state in float32 or bfloat16, got ", h0.scalar_type());
+  TORCH_CHECK_VALUE(!flags.defined() || (flags.dim() == 2 && flags.size(0) == u.size(0) && flags.size(1) == u.size(1)), "token masks must have shape (",
+                    u.size(0), ", ", u.size(1), ")");
+  flags = token_bytes(flags, u.size(0) * u.size(1));
+  if (wants_grad({&u, &dt, &A, &B, &C, &D, &z, &bias, &h0})) {
+    auto out = SelectiveScan::apply(u, dt, A, B, C, maybe(D), maybe(z), maybe(bias), maybe(h0), maybe(flags), softplus);
+    return {out[0], out[1]};
+  }
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(u.device());
+  SelectiveResult r = selective_forward(SelectiveOperands(u, dt, z, B, C, A, D, bias, true), h0, flags, softplus, false);
+  return {r.y, r.h_last};
+}
+
+Tensor selective_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& state, const MaybeTensor& D_,
+                      const MaybeTensor& z_, const MaybeTensor& bias_, const MaybeTensor& flags_, bool softplus) {
+  const char* name = "hip selective scan step";
+  Tensor D = opt(D_), z = opt(z_), bias = opt(bias_), flags = opt(flags_);
+  require_gpu(name, {&u, &dt, &A, &B, &C, &state, &D, &z, &bias, &flags});
+  require_device_of(name, u, {&dt, &A, &B, &C, &state, &D, &z, &bias, &flags});
+  check_selective(name, u, dt, A, B, C, D, z, bias, 2);
+  const int64_t rows = u.size(0), W = u.size(1), G = B.size(1), N = B.size(2);
+  TORCH_CHECK_VALUE(state.dim() == 3 && state.size(0) == rows && state.size(1) == W && state.size(2) == N && state.scalar_type() == at::kFloat &&
+                        state.is_contiguous(),
+                    "step expects a contiguous fp32 state of shape (", rows, ", ", W, ", ", N, ")");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()), name, " updates its state in place and has no gradient; the state requires one");
+  flags = token_bytes(flags, rows);
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(u.device());
+  SelectiveOperands o(u, dt, z, B, C, A, D, bias, false);
+  Tensor y = fresh({rows, W}, u.scalar_type(), u);
+  check(rglru_hip_selective_step(ptr(o.u), ptr(o.dt), ptr(o.z), ptr(o.B), ptr(o.C), o.strides, fptr(o.A), fptr(o.D), fptr(o.bias), bptr(flags), fptr(state),
+                                 ptr(y), softplus ? 1 : 0, rows, W, G, N, code_of(u.scalar_type()), stream_of(u)),
+        "rglru_hip_selective_step");
+  return y;
+}
+
+// ---- short causal convolution with an activation --------------------------------------------------------------------
+
+void check_short_conv(const char* name, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t axes) {
+  TORCH_CHECK_VALUE(x.dim() == axes && x.numel() > 0, name, " expects a non-empty input of shape ", axes == 3 ? "[batch, sequence, width]" : "[batch, width]",
+                    ", got ", x.sizes());
+  const int64_t W = x.size(-1);
+  TORCH_CHECK_VALUE(weight.dim() == 3 && weight.size(0) == W && weight.size(1) == 1 && weight.size(2) >= 1, name,
+                    " expects the weight of a depthwise Conv1d, [", W, ", 1, kernel_size], got ", weight.sizes());
+  TORCH_CHECK_VALUE(weight.size(2) <= rglru_hip_conv_max_kernel_size(), name, ": kernel size ", weight.size(2), ", at most ", rglru_hip_conv_max_kernel_size(),
+                    " is covered");
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == W), name, " expects a bias of shape [", W, "], got ", bias.sizes());
+  TORCH_CHECK_TYPE(known(x.scalar_type()), name, " supports float32 and bfloat16, got ", x.scalar_type());
+}
+
+struct ShortConvOperands {
+  Tensor x, taps, bias, state;
+  int64_t batch, token;
+  ShortConvOperands(const Tensor& x_in, const Tensor& weight, const Tensor& b, const Tensor& st) {
+    x = x_in.stride(2) == 1 || x_in.size(2) == 1 ? x_in : x_in.contiguous();
+    taps = operand(weight, x.scalar_type());
+    bias = as(b, taps.scalar_type());
+    state = weight.size(2) == 1 ? Tensor() : as(st, x.scalar_type());
+    distances();
+  }
+  ShortConvOperands(const variable_list& s) : x(s[0]), taps(s[1]), bias(s[2]), state(s[3]) { distances(); }
+  void distances() { batch = x.size(0) == 1 ? 0 : x.stride(0), token = x.size(1) == 1 ? 0 : x.stride(1); }
+};
+
+std::tuple<Tensor, Tensor> short_conv_forward(const ShortConvOperands& o, const Tensor& flags, int64_t activation, bool need_state) {
+  const int64_t B = o.x.size(0), T = o.x.size(1), W = o.x.size(2), K = o.taps.size(2);
+  Tensor y = fresh({B, T, W}, o.x.scalar_type(), o.x), window = need_state ? fresh({B, K - 1, W}, o.x.scalar_type(), o.x) : Tensor();
+  check(rglru_hip_short_conv_fwd(ptr(o.x), o.batch, o.token, ptr(o.state), ptr(o.taps), ptr(o.bias), bptr(flags), ptr(y),
+                                 need_state && K > 1 ? ptr(window) : nullptr, static_cast<int>(activation), B, T, W, K, code_of(o.x.scalar_type()),
+                                 code_of(o.taps.scalar_type()), stream_of(o.x)),
+        "rglru_hip_short_conv_fwd");
+  return {y, window};
+}
+
+struct ShortConv : torch::autograd::Function<ShortConv> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, const MaybeTensor& state_,
+                               const MaybeTensor& flags_, int64_t activation, bool need_state) {
+    Tensor bias = opt(bias_), state = opt(state_), flags = opt(flags_);
+    note_arguments(ctx, {true, true, bias.defined(), state.defined()});
+    c10::DeviceGuard guard(x.device());
+    ShortConvOperands o(x, weight, bias, state);
+    auto [y, window] = short_conv_forward(o, flags, activation, need_state);
+    ctx->save_for_backward({o.x, o.taps, o.bias, o.state, flags});
+    pack(ctx, {activation, type_or_none(weight), type_or_none(bias), type_or_none(state)});
+    ctx->set_materialize_grads(false);
+    if (!need_state) return {y};
+    ctx->mark_non_differentiable({window});
+    return {y, window};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    if (!grads[0].defined()) return variable_list(7);
+    auto saved = ctx->get_saved_variables();
+    auto m = unpack(ctx);
+    Tensor dx, dweight, dbias, dstate;
+    {
+      at::NoGradGuard no_grad;
+      ShortConvOperands o(saved);
+      const Tensor& flags = saved[4];
+      c10::DeviceGuard guard(o.x.device());
+      Needs needs(ctx);
+      const int64_t B = o.x.size(0), T = o.x.size(1), W = o.x.size(2), K = o.taps.size(2);
+      const auto dtype = o.x.scalar_type(), gt = o.taps.scalar_type();
+      Tensor dy = aligned(as(grads[0], dtype));
+      dx = fresh({B, T, W}, dtype, o.x);
+      if (needs(1)) dweight = fresh({W, 1, K}, gt, o.x);
+      if (needs(2)) dbias = fresh({W}, gt, o.x);
+      if (needs(3)) dstate = fresh({B, K - 1, W}, dtype, o.x);
+      Tensor scratch = bytes(rglru_hip_short_conv_scratch_bytes(B, T, W, K), o.x);
+      check(rglru_hip_short_conv_bwd(ptr(o.x), o.batch, o.token, ptr(o.state), ptr(o.taps), ptr(o.bias), bptr(flags), ptr(dy), ptr(scratch), ptr(dx),
+                                     K > 1 ? ptr(dstate) : nullptr, ptr(dweight), ptr(dbias), static_cast<int>(m[0]), B, T, W, K, code_of(dtype),
+                                     code_of(gt), code_of(gt), stream_of(o.x)),
+            "rglru_hip_short_conv_bwd");
+      if (dweight.defined()) dweight = dweight.to(type_at(m, 1));
+      if (dbias.defined()) dbias = dbias.to(type_at(m, 2));
+      if (dstate.defined()) dstate = dstate.to(type_at(m, 3));
+    }
+    return once({dx, dweight, dbias, dstate, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+std::tuple<Tensor, MaybeTensor> short_conv(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, const MaybeTensor& state_, const MaybeTensor& flags_,
+                                           int64_t activation, bool need_state) {
+  const char* name = "hip_short_conv";
+  Tensor bias = opt(bias_), state = opt(state_), flags = opt(flags_);
+  require_gpu(name, {&x, &weight, &bias, &state, &flags});
+  require_device_of(name, x, {&weight, &bias, &state, &flags});
+  check_short_conv(name, x, weight, bias, 3);
+  TORCH_CHECK_VALUE(!state.defined() || (state.dim() == 3 && state.size(0) == x.size(0) && state.size(1) == weight.size(2) - 1 && state.size(2) == x.size(2)),
+                    name, " expects a state of shape [", x.size(0), ", ", weight.size(2) - 1, ", ", x.size(2), "], got ", state.sizes());
+  TORCH_CHECK_VALUE(!flags.defined() || (flags.dim() == 2 && flags.size(0) == x.size(0) && flags.size(1) == x.size(1)), "token masks must have shape (",
+                    x.size(0), ", ", x.size(1), ")");
+  flags = token_bytes(flags, x.size(0) * x.size(1));
+  if (wants_grad({&x, &weight, &bias, &state})) {
+    auto out = ShortConv::apply(x, weight, maybe(bias), maybe(state), maybe(flags), activation, need_state);
+    return {out[0], need_state ? MaybeTensor(out[1]) : MaybeTensor()};
+  }
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(x.device());
+  auto [y, window] = short_conv_forward(ShortConvOperands(x, weight, bias, state), flags, activation, need_state);
+  return {y, maybe(window)};
+}
+
+Tensor short_conv_step(const Tensor& x_in, const Tensor& weight, const MaybeTensor& bias_, const Tensor& state, const MaybeTensor& flags_, int64_t activation) {
+  const char* name = "hip_short_conv_step";
+  Tensor bias = opt(bias_), flags = opt(flags_);
+  require_gpu(name, {&x_in, &weight, &bias, &state, &flags});
+  require_device_of(name, x_in, {&weight, &bias, &state, &flags});
+  check_short_conv(name, x_in, weight, bias, 2);
+  const int64_t B = x_in.size(0), W = x_in.size(1), K = weight.size(2);
+  TORCH_CHECK_VALUE(state.dim() == 3 && state.size(0) == B && state.size(1) == K - 1 && state.size(2) == W && state.scalar_type() == x_in.scalar_type() &&
+                        state.is_contiguous(),
+                    name, " expects a contiguous state of shape (", B, ", ", K - 1, ", ", W, ") in the type of the input");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && state.requires_grad()), name, " updates its state in place and has no gradient; the state requires one");
+  flags = token_bytes(flags, B);
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(x_in.device());
+  Tensor x = x_in.stride(1) == 1 || W == 1 ? x_in : x_in.contiguous();
+  Tensor taps = operand(weight, x.scalar_type()), shift = as(bias, taps.scalar_type());
+  Tensor y = fresh({B, W}, x.scalar_type(), x);
+  check(rglru_hip_short_conv_step(ptr(x), B == 1 ? 0 : x.stride(0), ptr(taps), ptr(shift), bptr(flags), K > 1 ? ptr(state) : nullptr, ptr(y),
+                                  static_cast<int>(activation), B, W, K, code_of(x.scalar_type()), code_of(taps.scalar_type()), stream_of(x)),
+        "rglru_hip_short_conv_step");
+  return y;
+}
+
+// ---- root-mean-square norm with the residual's addition -------------------------------------------------------------
+
+void check_add_rmsnorm(const char* name, const Tensor& x, const Tensor& residual, const Tensor& g) {
+  require_gpu(name, {&x, &residual, &g});
+  require_device_of(name, x, {&residual, &g});
+  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x.sizes(), name, " expects x and the residual of one shape, got ", x.sizes(), " and ",
+                    residual.sizes());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && g.dim() == 1 && x.size(-1) == g.numel(), name, " expects a scale of shape [",
+                    x.dim() >= 1 ? x.size(-1) : 0, "], got ", g.sizes());
+  TORCH_CHECK_VALUE(x.size(-1) <= rglru_hip_add_rmsnorm_max_width(), name, ": rows of ", x.size(-1), " elements, at most ", rglru_hip_add_rmsnorm_max_width(),
+                    " are covered");
+  TORCH_CHECK_TYPE(known(x.scalar_type()) && (!residual.defined() || known(residual.scalar_type())), name, " supports float32 and bfloat16, got ",
+                   x.scalar_type(), " and ", residual.defined() ? residual.scalar_type() : x.scalar_type());
+}
+
+struct AddRmsNormResult {
+  Tensor y, sum, scale, inv;
+};
+
+AddRmsNormResult add_rmsnorm_forward(const Tensor& x_in, const Tensor& residual_in, const Tensor& g, double eps, bool need_inv) {
+  AddRmsNormResult r;
+  Tensor x = aligned(x_in), residual = aligned(residual_in);
+  r.scale = operand(g, x.scalar_type());
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  r.y = fresh_like(x), r.sum = fresh_like(residual);
+  if (need_inv) r.inv = fresh({rows}, at::kFloat, x);
+  if (rows > 0)
+    check(rglru_hip_add_rmsnorm_fwd(ptr(x), ptr(residual), ptr(r.scale), ptr(r.sum), ptr(r.y), fptr(r.inv), rows, D, static_cast<float>(eps),
+                                    code_of(x.scalar_type()), code_of(residual.scalar_type()), code_of(r.scale.scalar_type()), stream_of(x)),
+          "rglru_hip_add_rmsnorm_fwd");
+  return r;
+}
+
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& g, double eps) {
+    c10::DeviceGuard guard(x.device());
+    AddRmsNormResult r = add_rmsnorm_forward(x, residual, g, eps, true);
+    ctx->save_for_backward({r.sum, r.scale, r.inv});
+    pack(ctx, {type_or_none(x), type_or_none(g)});
+    ctx->set_materialize_grads(false);
+    return {r.y, r.sum};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    auto s = ctx->get_saved_variables();
+    auto m = unpack(ctx);
+    const Tensor &sum = s[0], &scale = s[1], &inv = s[2];
+    Tensor dx, dresidual, dg;
+    {
+      at::NoGradGuard no_grad;
+      c10::DeviceGuard guard(sum.device());
+      const auto dtype = type_at(m, 0), stream_type = sum.scalar_type(), gt = scale.scalar_type();
+      const int64_t D = sum.size(-1), rows = sum.numel() / D;
+      const bool need_x = ctx->needs_input_grad(0), need_r = ctx->needs_input_grad(1);
+      Tensor dy = grads[0].defined() ? aligned(as(grads[0], dtype)) : at::zeros(sum.sizes(), sum.options().dtype(dtype));
+      Tensor dsum = grads[1].defined() ? aligned(as(grads[1], stream_type)) : Tensor();
+      if (need_r) dresidual = fresh_like(sum);
+      // one type: the two gradients are one tensor, as those of an addition are
+      if (need_x && !(need_r && dtype == stream_type)) dx = fresh(sum.sizes(), dtype, sum);
+      if (ctx->needs_input_grad(2)) dg = fresh({D}, gt, sum);
+      if (rows > 0) {
+        Tensor scratch = dg.defined() ? bytes(rglru_hip_add_rmsnorm_scratch_bytes(rows, D), sum) : Tensor();
+        check(rglru_hip_add_rmsnorm_bwd(ptr(sum), ptr(scale), fptr(inv), ptr(dy), ptr(dsum), ptr(scratch), ptr(dx), ptr(dresidual), ptr(dg), rows, D,
+                                        code_of(dtype), code_of(stream_type), code_of(gt), code_of(gt), stream_of(sum)),
+              "rglru_hip_add_rmsnorm_bwd");
+      } else if (dg.defined()) {
+        dg.zero_();
+      }
+      if (need_x && !dx.defined()) dx = dresidual;
+      if (dg.defined()) dg = dg.to(type_at(m, 1));
+    }
+    return once({dx, dresidual, dg, Tensor()});
+  }
+};
+
+std::tuple<Tensor, Tensor> add_rmsnorm(const Tensor& x, const Tensor& residual, const Tensor& g, double eps) {
+  check_add_rmsnorm("hip_add_rmsnorm", x, residual, g);
+  if (wants_grad({&x, &residual, &g})) {
+    auto out = AddRmsNorm::apply(x, residual, g, eps);
+    return {out[0], out[1]};
+  }
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(x.device());
+  AddRmsNormResult r = add_rmsnorm_forward(x, residual, g, eps, false);
+  return {r.y, r.sum};
+}
+
+std::tuple<Tensor, Tensor, MaybeTensor> add_rmsnorm_quantised(const Tensor& x_in, const MaybeTensor& residual_, const Tensor& g, double eps) {
+  const char* name = "hip_add_rmsnorm_quantised";
+  Tensor residual_in = opt(residual_);
+  check_add_rmsnorm(name, x_in, residual_in, g);
+  TORCH_CHECK(!wants_grad({&x_in, &residual_in, &g}), name, " has no gradient; an operand requires one");
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(x_in.device());
+  Tensor x = aligned(x_in), residual = residual_in.defined() ? aligned(residual_in) : Tensor(), scale = operand(g, x.scalar_type());
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  auto sizes = x.sizes().vec();
+  Tensor q = fresh(sizes, at::kFloat8_e4m3fn, x), sum = residual.defined() ? fresh_like(residual) : Tensor();
+  sizes.back() = 1;
+  Tensor scales = fresh(sizes, at::kFloat, x);
+  if (rows > 0)
+    check(rglru_hip_add_rmsnorm_quantised(ptr(x), ptr(residual), ptr(scale), ptr(sum), ptr(q), fptr(scales), rows, D, static_cast<float>(eps),
+                                          code_of(x.scalar_type()), code_of(residual.defined() ? residual.scalar_type() : x.scalar_type()),
+                                          code_of(scale.scalar_type()), stream_of(x)),
+          "rglru_hip_add_rmsnorm_quantised");
+  return {q, scales, maybe(sum)};
+}
+
 // ---- RMSNorm (griffin/griffin.py:68-80) ---------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> rmsnorm_forward(const Tensor& x_in, const Tensor& g, double eps, bool need_inv) {
@@ -2514,5 +2917,11 @@ PYBIND11_MODULE(_native, m) {
   EXPORT(group_norm);
   EXPORT(gated_delta);
   EXPORT(gated_delta_step);
+  EXPORT(selective_scan);
+  EXPORT(selective_step);
+  EXPORT(short_conv);
+  EXPORT(short_conv_step);
+  EXPORT(add_rmsnorm);
+  EXPORT(add_rmsnorm_quantised);
 #undef EXPORT
 }

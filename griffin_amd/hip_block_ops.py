@@ -245,6 +245,22 @@ def hip_rmsnorm(x: Tensor, g: Tensor, eps: float = 1e-6) -> Tensor:
     return _lib.native().rmsnorm(x, g, eps)
 
 
+
+def hip_add_rmsnorm(x: Tensor, residual: Tensor, g: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """``hip_rmsnorm`` of the residual stream with ``x`` added to it, in one pass: returns ``(y in x.dtype, x + residual in residual.dtype)``.
+
+    ``x`` and ``residual`` [..., D] of one shape (D up to 16384), float32 or bfloat16 each: a stream in float32 keeps its precision beside bfloat16 layers.
+    The statistics are those of the sum as it is stored.  Differentiable (first order) in x, residual and g, through both results."""
+    return _lib.native().add_rmsnorm(x, residual, g, eps)
+
+
+def hip_add_rmsnorm_quantised(x: Tensor, residual: Tensor | None, g: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor | None]:
+    """``hip_add_rmsnorm`` with rows in 8 bits for a product in 8 bits, without gradients: returns ``(q [..., D] in float8_e4m3fn, scale [..., 1] in
+    float32, x + residual)`` with ``y = q * scale``, ``scale`` the largest ``|y|`` of the row (at least 2^-100) over 448.  Without a residual, the norm of x
+    (and None for the sum).  A row with a NaN is NaN."""
+    return _lib.native().add_rmsnorm_quantised(x, residual, g, eps)
+
+
 _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}               # RGLRU_ACT_* of the C ABI
 
 

@@ -55,7 +55,7 @@
 extern "C" {
 #endif
 
-#define RGLRU_ABI_VERSION 25
+#define RGLRU_ABI_VERSION 26
 
 enum { RGLRU_F32 = 0, RGLRU_BF16 = 1 };
 
@@ -417,6 +417,67 @@ int rglru_hip_group_norm_fwd(const void* x, const void* weight, const void* bias
 int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias, const float* stats, const void* dy, void* scratch,
                              void* dx, void* dweight, void* dbias, int64_t N, int64_t L, int64_t C, int64_t G, int activation,
                              int dtype, int vec_dtype, int grad_dtype, void* stream);
+
+/* ---- selective state space scan (no counterpart in the reference) ------------------------------------------------------------
+ * Each channel w carries N numbers; B, C are its group's (channel w reads group w / (W / G)), a document start discards what lies in front of it:
+ *   s_t = softplus(dt_t + bias) (softplus 0: dt_t + bias),  h_t[n] = exp(s_t A[n]) h_{t-1}[n] + s_t u_t B_t[n]
+ *   y_t = (sum over n of C_t[n] h_t[n] + D u_t) silu(z_t)          (z NULL: without the gate; D, bias NULL: zeros)
+ * u, dt, z [B, T, W] and B, C [B, T, G, N] in `dtype`, their last axes contiguous; `strides`: elements between u's batch rows and tokens, dt's, z's,
+ * then B's batch rows, tokens and groups and C's (tokens less than 2^22 elements apart).  y, dout and all gradients dense.  A [W, N], D, bias [W], states
+ * [B, W, N] fp32.  `flags`: one byte a token or NULL, bit 0 = starts a document, bit 1 = inactive: the state stays, the output and the token's gradients are
+ * zero, whatever it holds.  N up to rglru_hip_selective_max_states().
+ *   ws       rglru_hip_selective_workspace_bytes(..., keep) bytes, 16-byte aligned: with `keep` the state in front of every 16 tokens, which the backward call
+ *            reads and leaves as it is
+ *   scratch  rglru_hip_selective_scratch_bytes(...) bytes, 16-byte aligned, of each backward call's own
+ *   dA, dD, dbias, dh0 may be NULL, dz where z is; dh_last NULL: zeros
+ * rglru_hip_selective_step: one token a row, u, dt, z [B, W], B, C [B, G, N], strides: u's rows, dt's, z's, B's rows and groups, C's; `state` is updated in place.
+ * Sums are fp32 in a fixed order; how many segments a sequence is walked in depends on the sizes and the number of compute units only. */
+int rglru_hip_selective_max_states(void);
+size_t rglru_hip_selective_workspace_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int keep);
+size_t rglru_hip_selective_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N);
+int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                            const float* D, const float* bias, const float* h0, const uint8_t* flags, void* y, float* h_last, void* ws, int keep,
+                            int softplus, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream);
+int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                            const float* D, const float* bias, const uint8_t* flags, const void* dout, const float* dh_last, const void* ws, void* scratch,
+                            void* du, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* dbias, float* dh0, int softplus, int64_t B,
+                            int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream);
+int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const int64_t* strides, const float* A,
+                             const float* D, const float* bias, const uint8_t* flags, float* state, void* y, int softplus, int64_t B, int64_t W,
+                             int64_t G, int64_t N, int dtype, void* stream);
+
+/* ---- short causal depthwise convolution with an activation (no counterpart in the reference) -----------------------------------
+ *   y_t = act(bias + sum over j < K of taps[w][K - 1 - j] x_{t - j}),  t - j counting the active tokens of t's document
+ * x [B, T, W] in `dtype`, batch rows x_batch and tokens x_token elements apart; y, dy, dx dense; state, new_state, dstate [B, K - 1, W]: the inputs in front
+ * of the first token (NULL: zeros) and behind the last one, the newest last; taps [W][K], bias [W] or NULL in `vec_dtype`; `flags` as above; K up to 4;
+ * activation RGLRU_ACT_NONE or RGLRU_ACT_SILU.
+ *   scratch  rglru_hip_short_conv_scratch_bytes(B, T, W, K) bytes, of each backward call's own;  dtaps [W][K], dbias [W] in `grad_dtype`
+ *   new_state, dstate, dtaps, dbias may be NULL
+ * rglru_hip_short_conv_step: one token a row, x [B, W], `state` updated in place. */
+size_t rglru_hip_short_conv_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_t K);
+int rglru_hip_short_conv_fwd(const void* x, int64_t x_batch, int64_t x_token, const void* state, const void* taps, const void* bias, const uint8_t* flags,
+                             void* y, void* new_state, int activation, int64_t B, int64_t T, int64_t W, int64_t K, int dtype, int vec_dtype, void* stream);
+int rglru_hip_short_conv_bwd(const void* x, int64_t x_batch, int64_t x_token, const void* state, const void* taps, const void* bias, const uint8_t* flags,
+                             const void* dy, void* scratch, void* dx, void* dstate, void* dtaps, void* dbias, int activation, int64_t B, int64_t T,
+                             int64_t W, int64_t K, int dtype, int vec_dtype, int grad_dtype, void* stream);
+int rglru_hip_short_conv_step(const void* x, int64_t x_batch, const void* taps, const void* bias, const uint8_t* flags, void* state, void* y,
+                              int activation, int64_t B, int64_t W, int64_t K, int dtype, int vec_dtype, void* stream);
+
+/* ---- root-mean-square norm with the residual's addition (no counterpart in the reference) --------------------------------------
+ *   sum = x + residual (rounded to the residual's type),  y = sum rsqrt(mean(sum^2) + eps) (1 + g)      over rows of D elements, dense
+ * x, y, dy, dx in `dtype`, residual, sum, dsum, dresidual in `residual_dtype`, g [D] in `vec_dtype`; inv [rows] fp32 (NULL without a backward call);
+ * D up to rglru_hip_add_rmsnorm_max_width().
+ * rglru_hip_add_rmsnorm_quantised: y = q scale, q[rows, D] in e4m3, scale[rows] = max(largest |y| of the row, 2^-100) / 448; residual and sum NULL together:
+ * the norm of x.
+ * Backward: dsum NULL = zeros; dx, dresidual (the same numbers in the two types) and dg may be NULL; scratch rglru_hip_add_rmsnorm_scratch_bytes(rows, D). */
+int rglru_hip_add_rmsnorm_max_width(void);
+int rglru_hip_add_rmsnorm_fwd(const void* x, const void* residual, const void* g, void* sum, void* y, float* inv, int64_t rows, int64_t D, float eps,
+                              int dtype, int residual_dtype, int vec_dtype, void* stream);
+int rglru_hip_add_rmsnorm_quantised(const void* x, const void* residual, const void* g, void* sum, void* q, float* scale, int64_t rows, int64_t D, float eps,
+                                    int dtype, int residual_dtype, int vec_dtype, void* stream);
+size_t rglru_hip_add_rmsnorm_scratch_bytes(int64_t rows, int64_t D);
+int rglru_hip_add_rmsnorm_bwd(const void* sum, const void* g, const float* inv, const void* dy, const void* dsum, void* scratch, void* dx, void* dresidual,
+                              void* dg, int64_t rows, int64_t D, int dtype, int residual_dtype, int vec_dtype, int grad_dtype, void* stream);
 
 /* Column sums of x[rows, D] (dtype) into out[D] (out_dtype), fp32 accumulation in a fixed order: the
  * bias gradient of the block's three Linear layers (griffin/griffin.py:379-389; autograd of

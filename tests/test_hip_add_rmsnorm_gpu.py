@@ -1,0 +1,155 @@
+"""The norm with the residual's addition on the GPU, its gradients and its rows in 8 bits, against the definition in 64 bits."""
+
+import pytest
+import torch
+
+from griffin_amd import hip_add_rmsnorm, hip_add_rmsnorm_quantised, hip_rmsnorm
+from tests.helpers import rel_err
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {F32: 2 ** -24, BF16: 2 ** -8}
+EPS = 1e-6
+SHAPES = [(1, 1), (3, 8), (5, 63), (2, 3, 64), (700, 128), (33, 520), (9, 1000), (7, 1024), (6, 1032), (5, 1500), (4, 2560), (3, 4096), (2, 4104), (2, 6001),
+          (2, 16384)]
+TYPES = [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)]
+
+
+def make(shape, dtype, residual, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    normal = lambda *s: torch.randn(*s, generator=gen)
+    return [normal(*shape).to(dtype), (3 * normal(*shape)).to(residual), (0.3 * normal(shape[-1])).to(dtype)], [normal(*shape).to(dtype), normal(*shape).to(residual)]
+
+
+def reference(x, r, g, eps=EPS):
+    """The sum as it is stored, and the norm of that."""
+    total = x.double() + (0 if r is None else r.double())
+    stored = total.to(total.dtype if r is None else r.dtype).double()
+    return stored * (stored.square().mean(-1, keepdim=True) + eps).rsqrt() * (1 + g.double()), stored
+
+
+def sum_steps(shape):
+    """fp32 sums of a row: sixteen terms a lane in a row, ten joins; a rounding each."""
+    return 64 * 2 ** -24
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype, residual", TYPES, ids=["f32", "bf16", "bf16+f32", "f32+bf16"])
+def test_norm_and_gradients(shape, dtype, residual):
+    leaves, ups = make(shape, dtype, residual)
+    leaves = [t.cuda().requires_grad_(True) for t in leaves]
+    y, total = hip_add_rmsnorm(*leaves, EPS)
+    grads = torch.autograd.grad([y, total], leaves, [t.cuda() for t in ups])
+    torch.cuda.synchronize()
+    assert y.dtype == dtype and total.dtype == residual
+    assert torch.equal(total.cpu(), (leaves[0].detach().float() + leaves[1].detach().float()).to(residual).cpu())
+    want, stored = reference(*(t.detach().cpu() for t in leaves))
+    assert rel_err(y, want) <= HALF_STEP[dtype] + sum_steps(shape)
+    s, g = stored.requires_grad_(True), leaves[2].detach().double().cpu().requires_grad_(True)
+    out = s * (s.square().mean(-1, keepdim=True) + EPS).rsqrt() * (1 + g)
+    ds, dg = torch.autograd.grad([out, s], [s, g], [t.double() for t in ups])
+    rows = stored.numel() // shape[-1]
+    # through both sums of a row; a scale's gradient adds up the rows, fp32 sums in runs
+    assert rel_err(grads[0], ds) <= HALF_STEP[dtype] + 2 * sum_steps(shape) and rel_err(grads[1], ds) <= HALF_STEP[residual] + 2 * sum_steps(shape)
+    assert rel_err(grads[2], dg) <= HALF_STEP[dtype] + 2 * sum_steps(shape) + rows * 2 ** -24
+    for got, leaf in zip(grads, leaves):
+        assert got.dtype == leaf.dtype and got.shape == leaf.shape
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype, residual", [*TYPES, (BF16, None), (F32, None)], ids=["f32", "bf16", "bf16+f32", "f32+bf16", "bf16 alone", "f32 alone"])
+def test_rows_in_bytes(shape, dtype, residual):
+    (x, r, g), _ = make(shape, dtype, residual or dtype, seed=3)
+    r = None if residual is None else r.cuda()
+    q, scale, total = hip_add_rmsnorm_quantised(x.cuda(), r, g.cuda(), EPS)
+    torch.cuda.synchronize()
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape and scale.shape == (*shape[:-1], 1) and scale.dtype == F32
+    want, stored = reference(x, None if r is None else r.cpu(), g)
+    assert total is None if r is None else torch.equal(total.cpu().double(), stored)
+    wanted_scale = want.abs().amax(-1, keepdim=True) / 448
+    assert ((scale.cpu().double() - wanted_scale) / wanted_scale).abs().max() <= sum_steps(shape) + 4 * 2 ** -24
+    # half a step of e4m3: 2^-4 of the value, 2^-10 of the scale below its smallest normal number; and what is off before that
+    back = q.cpu().to(F32).double() * scale.cpu().double()
+    assert ((back - want).abs() <= (2 ** -4 + 2 * sum_steps(shape)) * want.abs() + (2 ** -10 * 1.001) * wanted_scale).all()
+
+
+def test_sum_is_that_of_the_norm_alone():
+    (x, r, g), _ = make((40, 1024), BF16, BF16)
+    y, total = hip_add_rmsnorm(x.cuda(), r.cuda(), g.cuda())
+    # the same numbers through another kernel: sums in another order, rounded once each
+    assert rel_err(y, hip_rmsnorm(total, g.cuda())) <= 2 * HALF_STEP[BF16]
+
+
+def test_rows_of_zeros_and_of_what_is_not_a_number():
+    x = torch.zeros(6, 64)
+    x[1] = float("nan")
+    x[2, 5] = float("inf")
+    x[3] = 1e-38
+    x[4] = 3e38
+    x[5] = torch.linspace(-1, 1, 64)
+    g = torch.zeros(64)
+    y, total = hip_add_rmsnorm(x.cuda(), torch.zeros(6, 64).cuda(), g.cuda())
+    assert (y[0] == 0).all() and y[1].isnan().all() and y[2, 5].isnan() and torch.equal(total.cpu().nan_to_num(), x.nan_to_num())
+    q, scale, _ = hip_add_rmsnorm_quantised(x.cuda(), None, g.cuda())
+    back = q.to(F32) * scale
+    assert (back[0] == 0).all() and abs(float(scale[0]) * 448 * 2.0 ** 100 - 1) <= 2 ** -23
+    assert back[1].isnan().all() and back[2, 5].isnan()
+    assert torch.isfinite(back[[3, 5]]).all() and not q[3].to(F32).isnan().any()
+
+
+def test_one_result_and_one_operand():
+    leaves, ups = make((9, 256), BF16, F32)
+    leaves, ups = [t.cuda().requires_grad_(True) for t in leaves], [t.cuda() for t in ups]
+    y, total = hip_add_rmsnorm(*leaves)
+    whole = torch.autograd.grad([y, total], leaves, [ups[0], torch.zeros_like(total)], retain_graph=True)
+    alone = torch.autograd.grad(y, leaves, ups[0], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(whole, alone))
+    for i in range(3):
+        assert torch.equal(torch.autograd.grad(y, leaves[i], ups[0], retain_graph=True)[0], alone[i])
+    through = torch.autograd.grad(total, leaves, ups[1], retain_graph=True)
+    assert torch.equal(through[0], ups[1].to(BF16)) and torch.equal(through[1], ups[1]) and (through[2] == 0).all()
+    # leaves that share a gradient do not share its memory
+    a, b = (torch.randn(4, 64, device="cuda", requires_grad=True) for _ in range(2))
+    hip_add_rmsnorm(a, b, torch.zeros(64, device="cuda"))[0].sum().backward()
+    a.grad.add_(1)
+    assert not torch.equal(a.grad, b.grad)
+
+
+def test_gradients_against_differences():
+    leaves, ups = make((5, 200), F32, F32)
+    leaves, ups = [t.cuda().requires_grad_(True) for t in leaves], [t.cuda() for t in ups]
+    grads = torch.autograd.grad(hip_add_rmsnorm(*leaves), leaves, ups)
+    gen = torch.Generator().manual_seed(1)
+    for i in range(3):
+        way = torch.randn(leaves[i].shape, generator=gen).cuda()
+        moved = lambda e: [t.detach() + (e * way if j == i else 0) for j, t in enumerate(leaves)]
+        value = lambda e: sum((o.double() * u.double()).sum() for o, u in zip(hip_add_rmsnorm(*moved(e)), ups))
+        slope, size = (value(2.0 ** -8) - value(-2.0 ** -8)) * 2 ** 7, float((grads[i] * way).abs().sum())
+        assert abs(float(slope) - float((grads[i].double() * way.double()).sum())) < 2e-3 * size
+
+
+def test_views_are_taken():
+    wide = torch.randn(10, 130, device="cuda")
+    x, r, g = wide[:, 1:65], wide[:, 65:129], torch.zeros(64, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(hip_add_rmsnorm(x, r, g), hip_add_rmsnorm(x.contiguous(), r.contiguous(), g)))
+    empty = hip_add_rmsnorm(torch.zeros(0, 64, device="cuda"), torch.zeros(0, 64, device="cuda"), g)
+    assert empty[0].shape == empty[1].shape == (0, 64)
+    assert hip_add_rmsnorm_quantised(torch.zeros(0, 64, device="cuda"), None, g)[1].shape == (0, 1)
+
+
+@pytest.mark.parametrize("error, call", [
+    (ValueError, lambda x, g: hip_add_rmsnorm(x, x[:3], g)),
+    (ValueError, lambda x, g: hip_add_rmsnorm(x, x, g[:5])),
+    (ValueError, lambda x, g: hip_add_rmsnorm(torch.zeros(1, 16385, device="cuda"), torch.zeros(1, 16385, device="cuda"), torch.zeros(16385, device="cuda"))),
+    (TypeError, lambda x, g: hip_add_rmsnorm(x.half(), x, g)),
+    (TypeError, lambda x, g: hip_add_rmsnorm(x, x.double(), g)),
+    (RuntimeError, lambda x, g: hip_add_rmsnorm(x, x.cpu(), g)),
+    (RuntimeError, lambda x, g: hip_add_rmsnorm(x, x, g.cpu())),
+    (ValueError, lambda x, g: hip_add_rmsnorm_quantised(x, None, g[:5])),
+    (TypeError, lambda x, g: hip_add_rmsnorm_quantised(x.half(), None, g)),
+    (RuntimeError, lambda x, g: hip_add_rmsnorm_quantised(x.requires_grad_(), None, g)),
+])
+def test_tensors_that_do_not_fit(error, call):
+    with pytest.raises(error):
+        call(torch.zeros(4, 64, device="cuda"), torch.zeros(64, device="cuda"))

@@ -1,0 +1,636 @@
+"""The selective state space scan and its short convolution on the GPU against their definitions, token by token in 64 bits."""
+
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from griffin_amd import hip_add_rmsnorm, hip_linear, hip_selective_scan, hip_selective_step, hip_short_conv, hip_short_conv_step
+from tests.helpers import rel_err
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("u", "dt", "A", "B", "C", "D", "z", "dt_bias", "h0")
+BF16, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {F32: 2 ** -24, BF16: 2 ** -8}
+
+
+def bound(dtype, steps, grad=False):
+    """Largest deviation over largest value.  A step multiplies the state by a decay that is off by two units of exp2 and one of its argument and rounds
+    its sum: 4 half steps of fp32 a token, and sums whose terms cancel to a quarter of them.  A gradient goes through two such walks and
+    one more sum over states.  The result is rounded once."""
+    walk = (4 * steps + 64) * 2 ** -24
+    return HALF_STEP[dtype] + (4 if grad else 1) * walk
+
+
+def softplus(x):
+    return torch.where(x > 0, x, torch.zeros_like(x)) + torch.log1p(torch.exp(-x.abs()))
+
+
+def recurrence(u, dt, A, B, C, D, z, dt_bias, h0, soft=True, reset=None, active=None):
+    """y and the final state, from the definition (any float type, autograd works)."""
+    batch, steps, width = u.shape
+    of = torch.arange(width) // (width // B.shape[2])
+    s = dt if dt_bias is None else dt + dt_bias
+    s = softplus(s) if soft else s
+    h = u.new_zeros(batch, width, A.shape[1]) if h0 is None else h0
+    rows = []
+    for t in range(steps):
+        decay = torch.exp(s[:, t, :, None] * A)
+        kept = decay * h
+        if reset is not None:
+            kept = torch.where(reset[:, t, None, None], torch.zeros_like(kept), kept)
+        new = kept + (s[:, t] * u[:, t])[..., None] * B[:, t, of]
+        y = (new * C[:, t, of]).sum(-1)
+        if D is not None:
+            y = y + D * u[:, t]
+        if z is not None:
+            y = y * z[:, t] * torch.sigmoid(z[:, t])
+        if active is not None:
+            new = torch.where(active[:, t, None, None], new, h)
+            y = torch.where(active[:, t, None], y, torch.zeros_like(y))
+        h = new
+        rows.append(y)
+    return torch.stack(rows, 1), h
+
+
+def make(batch, steps, width, groups, states, dtype=F32, gated=True, skip=True, bias=True, carried=True, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    normal = lambda *shape: torch.randn(*shape, generator=gen)
+    rate = 0.001 * 100 ** torch.rand(width, generator=gen)
+    made = {
+        "u": normal(batch, steps, width).to(dtype), "dt": (0.7 * normal(batch, steps, width) - (0 if bias else 3)).to(dtype),
+        "A": -torch.arange(1, states + 1) * torch.exp(0.1 * normal(width, states)),
+        "B": normal(batch, steps, groups, states).to(dtype), "C": normal(batch, steps, groups, states).to(dtype),
+        "D": 1 + 0.1 * normal(width) if skip else None, "z": normal(batch, steps, width).to(dtype) if gated else None,
+        "dt_bias": rate + torch.log(-torch.expm1(-rate)) if bias else None, "h0": 0.3 * normal(batch, width, states) if carried else None,
+        "up": normal(batch, steps, width).to(dtype), "up_state": 0.2 * normal(batch, width, states),
+    }
+    return made
+
+
+def masks(batch, steps, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    reset = torch.rand(batch, steps, generator=gen) < 4.0 / steps
+    lengths = torch.randint(1, steps + 1, (batch,), generator=gen)
+    return reset, torch.arange(steps)[None] < lengths[:, None]
+
+
+def holes(batch, steps, seed=5):
+    gen = torch.Generator().manual_seed(seed)
+    active = torch.rand(batch, steps, generator=gen) < 0.5
+    active[0] = False
+    active[-1, : steps // 2] = False
+    return torch.rand(batch, steps, generator=gen) < 0.1, active
+
+
+def put(t):
+    return None if t is None else t.cuda()
+
+
+def scan(*leaves, soft=True, reset=None, active=None):
+    return hip_selective_scan(*leaves, softplus=soft, reset_mask=put(reset), active_mask=put(active))
+
+
+def run(fn, case, device, dtype=None, **how):
+    leaves = [None if case[n] is None else case[n].detach().to(device=device, dtype=dtype or case[n].dtype).requires_grad_(True) for n in NAMES]
+    y, last = fn(*leaves, **how)
+    wrt = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad([y, last], wrt, [case["up"].to(y), case["up_state"].to(last)])
+    return y.detach(), last.detach(), dict(zip([n for n, t in zip(NAMES, leaves) if t is not None], grads))
+
+
+def check(case, **how):
+    dtype, steps = case["u"].dtype, case["u"].shape[1]
+    want, want_last, want_grads = run(recurrence, case, "cpu", torch.float64, **how)
+    got, last, grads = run(scan, case, "cuda", **how)
+    torch.cuda.synchronize()
+    assert got.dtype == dtype and last.dtype == F32
+    errors = {"y": rel_err(got, want) / bound(dtype, steps), "state": rel_err(last, want_last) / bound(F32, steps)}
+    for name in grads:
+        assert grads[name].dtype == case[name].dtype and grads[name].shape == case[name].shape
+        errors["d" + name] = rel_err(grads[name], want_grads[name]) / bound(case[name].dtype, steps, True)
+    assert all(e <= 1 for e in errors.values()), errors
+
+
+SHAPES = [
+    # batch, steps, width, groups, states: one token; a tile; a token more; several tiles; odd sizes; groups; more states than a wave holds
+    (1, 1, 16, 1, 16),
+    (2, 16, 64, 1, 16),
+    (2, 17, 80, 1, 16),
+    (3, 130, 36, 2, 12),
+    (1, 65, 1, 1, 1),
+    (2, 50, 7, 7, 5),
+    (2, 40, 24, 1, 32),
+    (1, 33, 70, 2, 64),
+    (2, 35, 33, 1, 47),
+    (1, 20, 130, 1, 8),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_whole_sequences(shape, dtype):
+    check(make(*shape, dtype=dtype, carried=shape[1] % 2 == 0))
+
+
+@pytest.mark.parametrize("shape", [(3, 130, 36, 2, 12), (4, 77, 20, 1, 16), (2, 61, 18, 1, 40)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_packed_documents_and_padding(shape, dtype):
+    reset, active = masks(*shape[:2])
+    case = make(*shape, dtype=dtype)
+    check(case, reset=reset, active=active)
+    check(case, reset=reset)
+    check(case, active=active)
+
+
+def test_masks_with_holes_and_rows_without_tokens():
+    for dtype, states in ((F32, 16), (BF16, 10), (F32, 33)):
+        reset, active = holes(4, 90)
+        check(make(4, 90, 20, 1, states, dtype=dtype), reset=reset, active=active)
+
+
+def test_every_token_a_document():
+    check(make(2, 37, 20, 1, 16), reset=torch.ones(2, 37, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("absent", [("D",), ("z",), ("dt_bias",), ("h0",), ("D", "z", "dt_bias", "h0")], ids="-".join)
+def test_optional_operands(absent):
+    for dtype in (F32, BF16):
+        check(make(2, 45, 20, 1, 16, dtype=dtype, gated="z" not in absent, skip="D" not in absent, bias="dt_bias" not in absent, carried="h0" not in absent))
+
+
+@pytest.mark.parametrize("shape", [(1, 700, 20, 1, 16), (2, 600, 32, 2, 16), (1, 512, 20, 1, 33)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_sequences_in_segments(shape, dtype):
+    """Few channels: the sequence is walked in segments that are joined."""
+    case = make(*shape, dtype=dtype)
+    check(case)
+    gen = torch.Generator().manual_seed(3)
+    reset = torch.rand(shape[0], shape[1], generator=gen) < 0.004
+    active = torch.arange(shape[1])[None] < torch.tensor([shape[1] - 130, shape[1]])[:shape[0], None]
+    check(case, reset=reset, active=active)
+
+
+def test_step_sizes_as_they_are():
+    case = make(2, 40, 20, 1, 16)
+    case["dt"], case["dt_bias"] = case["dt"].abs() * 0.1, None
+    check(case, soft=False)
+
+
+def test_small_and_large_step_sizes():
+    """softplus of -80 is 1.8e-35, of 60 is 60: a step that forgets everything, steps that change nothing."""
+    case = make(2, 64, 20, 1, 16, bias=False)
+    gen = torch.Generator().manual_seed(8)
+    case["dt"] = torch.rand(2, 64, 20, generator=gen) * 140 - 80
+    check(case)
+
+
+def test_small_step_sizes_keep_their_digits():
+    """softplus(-16) is 1.1e-7, less than a half step of 1: the series does not lose it in 1 + e."""
+    gen = torch.Generator().manual_seed(9)
+    dt = -torch.rand(1, 16, 64, generator=gen) * 14 - 4
+    ones = torch.ones(1, 16, 64)
+    vectors = torch.zeros(1, 16, 1, 1)
+    vectors[:, 0] = 1
+    A = -torch.zeros(64, 1)
+    # h_0 = s_0 u_0 B_0 and no decay: the final state is the first token's step size
+    _, last = hip_selective_scan(ones.cuda(), dt.cuda(), A.cuda(), vectors.cuda(), torch.ones(1, 16, 1, 1).cuda())
+    want = softplus(dt[:, 0].double())[..., None]
+    # exp2, two reciprocals and a dozen sums: 16 half steps, and the argument of exp, up to 18 log2(e), rounded once
+    assert ((last.cpu().double() - want) / want).abs().max() < (16 + 26 * 2) * 2 ** -24
+
+
+def test_masked_tokens_may_hold_anything():
+    bad = [float("nan"), float("inf"), -float("inf")]
+    for dtype, states in ((F32, 16), (BF16, 20)):
+        reset, active = holes(4, 90)
+        case = make(4, 90, 20, 1, states, dtype=dtype)
+        dirty = {k: v if v is None else v.clone() for k, v in case.items()}
+        for name in ("u", "dt", "B", "C", "z", "up"):
+            for i, value in enumerate(bad):
+                dirty[name][~active & (torch.arange(90)[None] % 3 == i)] = value
+        want = run(scan, case, "cuda", reset=reset, active=active)
+        got = run(scan, dirty, "cuda", reset=reset, active=active)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for name in got[2]:
+            assert torch.equal(got[2][name], want[2][name]), name
+        for name in ("u", "dt", "B", "C", "z"):
+            assert (got[2][name][~active.cuda()] == 0).all(), name
+        assert (got[0][~active.cuda()] == 0).all()
+
+
+def test_a_document_start_discards_whatever_there_was():
+    for steps in (40, 700):                                  # in one walk, in segments
+        case = make(1, steps, 20, 1, 16)
+        reset = torch.zeros(1, steps, dtype=torch.bool)
+        reset[0, steps // 2] = True
+        case["up_state"] = torch.zeros_like(case["up_state"])
+        want = run(scan, case, "cuda", reset=reset)
+        dirty = dict(case, h0=torch.full_like(case["h0"], float("nan")))
+        dirty["up"] = case["up"].clone()
+        got = run(scan, dirty, "cuda", reset=reset)
+        assert torch.equal(got[0][:, steps // 2:], want[0][:, steps // 2:]) and torch.equal(got[1], want[1])
+        for name in ("u", "dt", "B", "C", "z"):
+            assert torch.equal(got[2][name][:, steps // 2 + 1:], want[2][name][:, steps // 2 + 1:]), name
+
+
+def test_pieces_and_single_tokens_give_the_whole():
+    reset, active = masks(3, 75)
+    for dtype, states, groups in ((F32, 16, 1), (BF16, 6, 2), (BF16, 48, 1)):
+        case = make(3, 75, 22, groups, states, dtype=dtype)
+        args = {n: put(case[n]) for n in NAMES}
+        whole, last = hip_selective_scan(**args, reset_mask=reset.cuda(), active_mask=active.cuda())
+        state, pieces = args["h0"], []
+        part = lambda a, b: {n: t[:, a:b] if n in ("u", "dt", "B", "C", "z") else t for n, t in args.items()}
+        for a, b in ((0, 16), (16, 17), (17, 50), (50, 75)):
+            y, state = hip_selective_scan(**dict(part(a, b), h0=state), reset_mask=reset[:, a:b].cuda(), active_mask=active[:, a:b].cuda())
+            pieces.append(y)
+        # the same tokens through the same states: the bound of both walks
+        assert rel_err(torch.cat(pieces, 1), whole) <= 2 * bound(dtype, 75) and rel_err(state, last) <= 2 * bound(F32, 75)
+        flags = (reset.to(torch.uint8) + 2 * (~active).to(torch.uint8)).cuda()
+        state, rows = args["h0"].clone(), []
+        for t in range(75):
+            at = state.data_ptr()
+            rows.append(hip_selective_step(args["u"][:, t], args["dt"][:, t], args["A"], args["B"][:, t], args["C"][:, t], state, args["D"], args["z"][:, t],
+                                           args["dt_bias"], flags=flags[:, t]))
+            assert state.data_ptr() == at
+        assert rel_err(torch.stack(rows, 1), whole) <= 2 * bound(dtype, 75) and rel_err(state, last) <= 2 * bound(F32, 75)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_parts_of_one_projection(dtype):
+    """Views with strides of their own, on and off vector boundaries, broadcast over tokens or rows: the results of dense copies, bit for bit."""
+    gen = torch.Generator().manual_seed(4)
+    for offset, states, groups, width in ((0, 16, 1, 40), (1, 16, 2, 40), (8, 12, 1, 33), (3, 40, 1, 20)):
+        wide = torch.randn(2, 50, 2 * width + offset, generator=gen).to(dtype).cuda()
+        one = torch.randn(2, 50, offset + 2 * groups * states, generator=gen).to(dtype).cuda()
+        case = {n: put(t) for n, t in make(2, 50, width, groups, states, dtype=dtype).items()}
+        case["u"], case["z"] = wide[..., offset:offset + width], wide[..., offset + width:]
+        case["B"] = one[..., offset:offset + groups * states].unflatten(-1, (groups, states))
+        case["C"] = one[..., offset + groups * states:].unflatten(-1, (groups, states))
+        case["dt"] = case["dt"][:, :1].expand(-1, 50, -1)
+        views = run(hip_selective_scan, case, "cuda")
+        dense = run(hip_selective_scan, {n: t.contiguous() for n, t in case.items()}, "cuda")
+        assert torch.equal(views[0], dense[0]) and torch.equal(views[1], dense[1])
+        for name in views[2]:
+            assert torch.equal(views[2][name], dense[2][name]), name
+        y = [hip_selective_step(*(f(case[n][:, 3]) if n not in ("A",) else case[n] for n in ("u", "dt", "A", "B", "C")), case["h0"].clone(), case["D"],
+                                f(case["z"][:, 3]), case["dt_bias"]) for f in (lambda t: t, torch.Tensor.contiguous)]
+        assert torch.equal(*y)
+
+
+def test_gradients_of_parameters_in_half_precision_and_of_one_output():
+    case = make(2, 40, 20, 1, 16, dtype=BF16)
+    half = {n: (t.bfloat16() if n in ("A", "D", "dt_bias", "h0") else t) for n, t in case.items()}
+    full = {n: (t.float() if n in ("A", "D", "dt_bias", "h0") else t) for n, t in half.items()}
+    got, want = run(scan, half, "cuda"), run(scan, full, "cuda")
+    assert torch.equal(got[0], want[0])
+    for name in ("A", "D", "dt_bias", "h0"):
+        assert got[2][name].dtype == BF16 and torch.equal(got[2][name], want[2][name].bfloat16())
+    leaves = [put(case[n]).requires_grad_(True) for n in NAMES]
+    y, last = hip_selective_scan(*leaves)
+    alone = torch.autograd.grad(last, leaves, put(case["up_state"]), retain_graph=True)
+    none = torch.autograd.grad([y, last], leaves, [torch.zeros_like(y), put(case["up_state"])])
+    assert all(torch.equal(a, b) for a, b in zip(alone, none))
+
+
+def test_gradients_against_differences():
+    """The slope along a random direction, from results 2 eps apart: an error of eps^2 and of the results' rounding over eps."""
+    case = {n: put(t) for n, t in make(2, 37, 20, 1, 16).items()}
+    gen = torch.Generator().manual_seed(6)
+    _, _, grads = run(hip_selective_scan, case, "cuda")
+    value = lambda c: sum((o.double() * up.double()).sum() for o, up in zip(hip_selective_scan(*(c[n] for n in NAMES)), (c["up"], c["up_state"])))
+    for name in NAMES:
+        way = torch.randn(case[name].shape, generator=gen).cuda()
+        way = way / way.norm() * case[name].norm()
+        eps = 2.0 ** -9
+        slope = (value(dict(case, **{name: case[name] + eps * way})) - value(dict(case, **{name: case[name] - eps * way}))) / (2 * eps)
+        size = float((grads[name].double() * way.double()).abs().sum())
+        assert abs(float(slope) - float((grads[name].double() * way.double()).sum())) < 2e-3 * size, name
+
+
+def test_results_repeat_bit_for_bit_and_on_another_stream():
+    for shape in ((2, 300, 70, 1, 16), (1, 900, 20, 1, 16), (2, 60, 36, 1, 40)):
+        case = {n: put(t) for n, t in make(*shape, dtype=BF16).items()}
+        first = run(hip_selective_scan, case, "cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = run(hip_selective_scan, case, "cuda")
+        side.synchronize()
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+        assert all(torch.equal(first[2][n], again[2][n]) for n in first[2])
+
+
+def test_masks_written_after_the_call_do_not_reach_the_gradients():
+    case = make(2, 60, 20, 1, 16)
+    reset, active = (m.cuda() for m in masks(2, 60))
+    want = run(scan, case, "cuda", reset=reset, active=active)
+    leaves = [put(case[n]).requires_grad_(True) for n in NAMES]
+    y, last = hip_selective_scan(*leaves, reset_mask=reset, active_mask=active)
+    reset.fill_(True), active.fill_(False)
+    grads = torch.autograd.grad([y, last], leaves, [put(case["up"]), put(case["up_state"])])
+    assert all(torch.equal(a, want[2][n]) for a, n in zip(grads, NAMES))
+
+
+def test_backward_twice_from_one_forward():
+    case = make(1, 300, 20, 1, 16)
+    leaves = [put(case[n]).requires_grad_(True) for n in NAMES]
+    y, last = hip_selective_scan(*leaves)
+    ups = [put(case["up"]), put(case["up_state"])]
+    first = torch.autograd.grad([y, last], leaves, ups, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad([y, last], leaves, ups)))
+
+
+def test_step_leaves_idle_rows_alone():
+    case = {n: put(t) for n, t in make(5, 1, 20, 1, 16).items()}
+    state = case["h0"].clone()
+    state[1] = float("nan")
+    state[3] = float("nan")
+    before = state.clone()
+    flags = torch.tensor([0, 2, 3, 1, 0], dtype=torch.uint8, device="cuda")
+    for name in ("u", "dt", "B", "C", "z"):
+        case[name][1:3] = float("nan")
+    y = hip_selective_step(*(case[n][:, 0] if n != "A" else case[n] for n in ("u", "dt", "A", "B", "C")), state, case["D"], case["z"][:, 0], case["dt_bias"],
+                           flags=flags)
+    assert torch.equal(state[1:3].view(torch.int32), before[1:3].view(torch.int32)) and (y[1:3] == 0).all()
+    assert torch.isfinite(state[[0, 3, 4]]).all() and torch.isfinite(y).all()
+
+
+# ---- the short convolution ---------------------------------------------------------------------------------------------
+
+def convolution(x, weight, bias, state, silu, reset=None, active=None):
+    """y and the window behind the last token, from the definition."""
+    back = weight.shape[2] - 1
+    window = x.new_zeros(x.shape[0], back, x.shape[2]) if state is None else state
+    rows = []
+    for t in range(x.shape[1]):
+        old = window if reset is None else torch.where(reset[:, t, None, None], torch.zeros_like(window), window)
+        now = torch.cat((old, x[:, t, None]), 1)
+        y = (now * weight[:, 0].T).sum(1) + (0 if bias is None else bias)
+        y = y * torch.sigmoid(y) if silu else y
+        if active is not None:
+            y = torch.where(active[:, t, None], y, torch.zeros_like(y))
+            window = torch.where(active[:, t, None, None], now[:, 1:], window)
+        else:
+            window = now[:, 1:]
+        rows.append(y)
+    return torch.stack(rows, 1), window
+
+
+def make_conv(batch, steps, width, taps, dtype=F32, bias=True, carried=True, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    normal = lambda *shape: torch.randn(*shape, generator=gen).to(dtype)
+    return {"x": normal(batch, steps, width), "weight": normal(width, 1, taps), "bias": normal(width) if bias else None,
+            "state": normal(batch, taps - 1, width) if carried else None, "up": normal(batch, steps, width)}
+
+
+def check_conv(case, silu=True, reset=None, active=None):
+    dtype, names = case["x"].dtype, ("x", "weight", "bias", "state")
+    leaves = [None if case[n] is None else case[n].double().requires_grad_(True) for n in names]
+    want, want_window = convolution(*leaves, silu, reset, active)
+    wrt = [t for t in leaves if t is not None]
+    want_grads = torch.autograd.grad(want, wrt, case["up"].double(), allow_unused=True, materialize_grads=True)
+    leaves = [None if case[n] is None else case[n].cuda().requires_grad_(True) for n in names]
+    got, window = hip_short_conv(*leaves, "silu" if silu else None, put(reset), put(active))
+    grads = torch.autograd.grad(got, [t for t in leaves if t is not None], case["up"].cuda())
+    torch.cuda.synchronize()
+    # five products and sums, the activation's exp and reciprocal, rounded once; weights' sums over all tokens in runs of 16
+    tokens = case["x"].shape[0] * case["x"].shape[1]
+    assert rel_err(got, want) <= HALF_STEP[dtype] + 2 ** -20
+    assert torch.equal(window.cpu().double(), want_window)
+    for n, g, w in zip([n for n in names if case[n] is not None], grads, want_grads):
+        assert g.dtype == dtype and g.shape == w.shape
+        assert not w.numel() or rel_err(g, w) <= HALF_STEP[dtype] + 2 ** -19 + tokens * 2 ** -24, n
+
+
+CONV_SHAPES = [(1, 1, 8, 4), (2, 15, 16, 4), (2, 16, 16, 3), (3, 17, 24, 2), (2, 33, 7, 4), (1, 300, 40, 4), (2, 140, 300, 4), (2, 20, 12, 1), (4, 3, 260, 4)]
+
+
+@pytest.mark.parametrize("shape", CONV_SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_short_convolutions(shape, dtype):
+    check_conv(make_conv(*shape, dtype=dtype))
+    check_conv(make_conv(*shape, dtype=dtype, bias=False, carried=False), silu=False)
+
+
+@pytest.mark.parametrize("shape", [(3, 130, 36, 4), (4, 77, 20, 3), (2, 61, 8, 2), (2, 40, 16, 1)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_short_convolutions_of_documents(shape, dtype):
+    reset, active = masks(*shape[:2])
+    case = make_conv(*shape, dtype=dtype)
+    check_conv(case, reset=reset, active=active)
+    check_conv(case, reset=reset)
+    check_conv(case, active=active)
+    check_conv(case, active=active.flip(1))                  # padding in front
+    check_conv(case, reset=torch.ones_like(reset))
+    reset, active = holes(*shape[:2])
+    check_conv(case, reset=reset, active=active)
+    sparse = torch.zeros_like(active)
+    sparse[:, ::37] = True
+    check_conv(case, active=sparse)
+
+
+def test_short_convolution_of_views_and_dirty_padding():
+    gen = torch.Generator().manual_seed(2)
+    for offset, width in ((0, 32), (1, 32), (8, 30)):
+        wide = torch.randn(2, 50, 2 * width + offset, generator=gen).bfloat16().cuda()
+        case = make_conv(2, 50, width, 4, dtype=BF16)
+        args = [wide[..., offset:offset + width], *(case[n].cuda() for n in ("weight", "bias", "state"))]
+        got, want = hip_short_conv(*args, "silu"), hip_short_conv(args[0].contiguous(), *args[1:], "silu")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    reset, active = (m.cuda() for m in holes(4, 90))
+    case = {n: t.cuda() for n, t in make_conv(4, 90, 24, 4).items()}
+    dirty = dict(case, x=case["x"].clone(), up=case["up"].clone())
+    dirty["x"][~active] = float("nan")
+    dirty["up"][~active] = float("inf")
+    results = []
+    for c in (case, dirty):
+        leaves = [c[n].clone().requires_grad_(True) for n in ("x", "weight", "bias", "state")]
+        y, window = hip_short_conv(*leaves, "silu", reset, active)
+        results.append([y.detach(), window, *torch.autograd.grad(y, leaves, c["up"])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert (results[0][2][~active] == 0).all()
+
+
+def test_short_convolution_by_pieces_and_tokens():
+    reset, active = masks(3, 60)
+    for dtype, taps in ((F32, 4), (BF16, 3), (BF16, 1)):
+        case = {n: t.cuda() for n, t in make_conv(3, 60, 40, taps, dtype=dtype).items()}
+        whole, window = hip_short_conv(*(case[n] for n in ("x", "weight", "bias", "state")), "silu", reset.cuda(), active.cuda())
+        state, rows = case["state"], []
+        for a, b in ((0, 1), (1, 18), (18, 20), (20, 60)):
+            y, state = hip_short_conv(case["x"][:, a:b], case["weight"], case["bias"], state, "silu", reset[:, a:b].cuda(), active[:, a:b].cuda())
+            rows.append(y)
+        assert torch.equal(torch.cat(rows, 1), whole) and torch.equal(state, window)
+        flags = (reset.to(torch.uint8) + 2 * (~active).to(torch.uint8)).cuda()
+        state = case["state"].clone()
+        rows = [hip_short_conv_step(case["x"][:, t], case["weight"], case["bias"], state, "silu", flags[:, t]) for t in range(60)]
+        # the taps are added in another order: half a step of the result, and of fp32 sums
+        assert rel_err(torch.stack(rows, 1), whole) <= 2 * HALF_STEP[dtype] + 2 ** -20 and torch.equal(state, window)
+        assert hip_short_conv(case["x"], case["weight"], need_state=False)[1] is None
+
+
+# ---- as they are used ----------------------------------------------------------------------------------------------------
+
+class Mixer(torch.nn.Module):
+    """A block around a selective state space: norm with the residual's addition, projection, short convolution, scan with its gate, projection."""
+
+    def __init__(self, dim, width, states, rank, dtype):
+        super().__init__()
+        normal = lambda *shape: torch.nn.Parameter((torch.randn(*shape) * shape[-1] ** -0.5).to(dtype))
+        self.rank, self.states, self.width = rank, states, width
+        self.g = torch.nn.Parameter(torch.zeros(dim, dtype=dtype))
+        self.project, self.conv, self.conv_bias = normal(2 * width, dim), normal(width, 1, 4), torch.nn.Parameter(torch.zeros(width, dtype=dtype))
+        self.select, self.rates, self.out = normal(rank + 2 * states, width), normal(width, rank), normal(dim, width)
+        self.log_A = torch.nn.Parameter(torch.arange(1, states + 1).float().log().repeat(width, 1))
+        self.D, self.dt_bias = torch.nn.Parameter(torch.ones(width)), torch.nn.Parameter(torch.full((width,), -3.0))
+
+    def forward(self, x, stream, reset=None, active=None, cache=None):
+        y, stream = hip_add_rmsnorm(x, stream, self.g)
+        inner, gate = hip_linear(y, self.project, None).split(self.width, -1)
+        window, state = (None, None) if cache is None else cache
+        inner, window = hip_short_conv(inner, self.conv, self.conv_bias, window, "silu", reset, active)
+        dt, B, C = hip_linear(inner, self.select, None).split([self.rank, self.states, self.states], -1)
+        y, state = hip_selective_scan(inner, hip_linear(dt.contiguous(), self.rates, None), -self.log_A.exp(), B[:, :, None], C[:, :, None], self.D, gate,
+                                      self.dt_bias, state, reset_mask=reset, active_mask=active)
+        return hip_linear(y, self.out, None), stream, (window, state)
+
+    def step(self, x, stream, window, state, flags=None):
+        y, stream = hip_add_rmsnorm(x, stream, self.g)
+        inner, gate = hip_linear(y, self.project, None).split(self.width, -1)
+        inner = hip_short_conv_step(inner, self.conv, self.conv_bias, window, "silu", flags)
+        dt, B, C = hip_linear(inner, self.select, None).split([self.rank, self.states, self.states], -1)
+        y = hip_selective_step(inner, hip_linear(dt.contiguous(), self.rates, None), -self.log_A.exp(), B[:, None], C[:, None], state, self.D, gate,
+                               self.dt_bias, flags=flags)
+        return hip_linear(y, self.out, None), stream
+
+
+def reference_mixer(m, x, stream, reset, active):
+    p = {n: t.detach().double().cpu().requires_grad_(True) for n, t in m.named_parameters()}
+    total = x + stream
+    y = total * (total.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * (1 + p["g"])
+    inner, gate = (y @ p["project"].T).split(m.width, -1)
+    inner, _ = convolution(inner, p["conv"], p["conv_bias"], None, True, reset, active)
+    dt, B, C = (inner @ p["select"].T).split([m.rank, m.states, m.states], -1)
+    y, _ = recurrence(inner, dt @ p["rates"].T, -p["log_A"].exp(), B[:, :, None], C[:, :, None], p["D"], gate, p["dt_bias"], None, reset=reset, active=active)
+    return y @ p["out"].T, total, p
+
+
+def test_a_block_of_them_trains():
+    torch.manual_seed(0)
+    m = Mixer(32, 48, 16, 8, F32).cuda()
+    x, stream, up = torch.randn(3, 70, 32), torch.randn(3, 70, 32), torch.randn(2, 3, 70, 32)
+    reset, active = masks(3, 70)
+    a, b = x.cuda().requires_grad_(True), stream.cuda().requires_grad_(True)
+    out, total, _ = m(a, b, reset.cuda(), active.cuda())
+    names, params = zip(*m.named_parameters())
+    grads = torch.autograd.grad([out, total], [a, b, *params], list(up.cuda()))
+    x64, stream64 = x.double().requires_grad_(True), stream.double().requires_grad_(True)
+    want, want_total, p = reference_mixer(m, x64, stream64, reset, active)
+    want_grads = torch.autograd.grad([want, want_total], [x64, stream64, *(p[n] for n in names)], list(up.double()))
+    # four products of up to 64 terms on the way, each term off by 2^-24 of its size: 2^-16 for the results, four times that for gradients through all of them
+    assert rel_err(out, want) <= 2 ** -16 + bound(F32, 70) and rel_err(total, want_total) <= 2 ** -23
+    for n, g, w in zip(("x", "stream", *names), grads, want_grads):
+        assert rel_err(g, w) <= 2 ** -14 + bound(F32, 70, True), n
+
+
+def test_a_block_of_them_answers():
+    """A prompt, then single tokens, against the whole sequence."""
+    torch.manual_seed(1)
+    for dtype in (F32, BF16):
+        m = Mixer(32, 48, 16, 8, dtype).cuda()
+        x, stream = torch.randn(3, 40, 32).to(dtype).cuda(), torch.randn(3, 40, 32).cuda()
+        with torch.no_grad():
+            whole, _, (window, state) = m(x, stream)
+            first, _, (w, h) = m(x[:, :30], stream[:, :30])
+            rows = [first]
+            for t in range(30, 40):
+                out, _ = m.step(x[:, t], stream[:, t], w, h)
+                rows.append(out[:, None])
+        # every layer's result may fall on another side of a rounding: five of them, half a step each side
+        assert rel_err(torch.cat(rows, 1), whole) <= 10 * HALF_STEP[dtype] + 2 * bound(F32, 40)
+        assert rel_err(h, state) <= 10 * HALF_STEP[dtype] + 2 * bound(F32, 40) and rel_err(w, window) <= 4 * HALF_STEP[dtype] + 2 ** -18
+
+
+def test_captured_graphs():
+    child = os.path.join(os.path.dirname(__file__), "capture_selective_child.py")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    ran = subprocess.run([sys.executable, "-u", child], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=110)
+    assert ran.returncode == 0, ran.stdout[-2000:] + ran.stderr[-2000:]
+
+
+# ---- refusals ----------------------------------------------------------------------------------------------------------------
+
+def swapped(name, change, step=False):
+    case = {n: put(t) for n, t in make(2, 5, 12, 2, 4).items()}
+    if step:
+        case = {n: t[:, 0] if n in ("u", "dt", "B", "C", "z") else t for n, t in case.items()}
+    case[name] = change(case[name])
+    return [case[n] for n in NAMES]
+
+
+def steps_of(name=None, change=None, **more):
+    leaves = dict(zip(NAMES, swapped(name or "u", change or (lambda t: t), True)))
+    state = more.pop("state", leaves["h0"])
+    return hip_selective_step(*(leaves[n] for n in ("u", "dt", "A", "B", "C")), state, leaves["D"], leaves["z"], leaves["dt_bias"], **more)
+
+
+def conv_of(name=None, change=None, **more):
+    case = {n: put(t) for n, t in make_conv(2, 5, 8, 4).items()}
+    if name:
+        case[name] = change(case[name])
+    return hip_short_conv(*(case[n] for n in ("x", "weight", "bias", "state")), **more)
+
+
+def conv_step_of(name=None, change=None, **more):
+    case = {n: put(t) for n, t in make_conv(2, 1, 8, 4).items()}
+    case["x"] = case["x"][:, 0]
+    if name:
+        case[name] = change(case[name])
+    return hip_short_conv_step(*(case[n] for n in ("x", "weight", "bias", "state")), **more)
+
+
+@pytest.mark.parametrize("error, call", [
+    (ValueError, lambda: hip_selective_scan(*swapped("dt", lambda t: t[..., :6]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("z", lambda t: t[:, :4]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("B", lambda t: t[..., :3]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("C", lambda t: t[:, :, :1]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("A", lambda t: t.T.contiguous()))),
+    (ValueError, lambda: hip_selective_scan(*swapped("D", lambda t: t[:5]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("dt_bias", lambda t: t[:, None]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("h0", lambda t: t[:1]))),
+    (ValueError, lambda: hip_selective_scan(*(t[:0] if t.dim() > 2 else t for t in swapped("u", lambda t: t)))),
+    (ValueError, lambda: hip_selective_scan(*(put(t) for t in list(make(1, 3, 10, 3, 4).values())[:5]))),
+    (ValueError, lambda: hip_selective_scan(*(put(t) for t in list(make(1, 3, 10, 1, 65).values())[:5]))),
+    (ValueError, lambda: hip_selective_scan(*swapped("u", lambda t: t), reset_mask=torch.zeros(2, 4, dtype=torch.bool))),
+    (TypeError, lambda: hip_selective_scan(*swapped("u", lambda t: t.bfloat16()))),
+    (TypeError, lambda: hip_selective_scan(*swapped("A", lambda t: t.half()))),
+    (TypeError, lambda: hip_selective_scan(*swapped("h0", lambda t: t.double()))),
+    (RuntimeError, lambda: hip_selective_scan(*swapped("B", lambda t: t.cpu()))),
+    (ValueError, lambda: steps_of("u", lambda t: t[:1])),
+    (ValueError, lambda: steps_of(state=torch.zeros(2, 4, 12, device="cuda"))),
+    (ValueError, lambda: steps_of(state=torch.zeros(2, 4, 12, device="cuda").mT)),
+    (ValueError, lambda: steps_of(state=torch.zeros(2, 12, 4, device="cuda").bfloat16())),
+    (ValueError, lambda: steps_of(flags=torch.zeros(3, dtype=torch.uint8, device="cuda"))),
+    (RuntimeError, lambda: steps_of(state=torch.zeros(2, 12, 4, device="cuda").requires_grad_())),
+    (ValueError, lambda: conv_of("weight", lambda t: t[:, 0])),
+    (ValueError, lambda: conv_of("weight", lambda t: torch.cat((t, t), 2))),
+    (ValueError, lambda: conv_of("bias", lambda t: t[:3])),
+    (ValueError, lambda: conv_of("state", lambda t: t[:, :2])),
+    (ValueError, lambda: conv_of("x", lambda t: t[:, :0])),
+    (ValueError, lambda: conv_of(activation="gelu")),
+    (ValueError, lambda: conv_of(active_mask=torch.ones(2, 6, dtype=torch.bool))),
+    (TypeError, lambda: conv_of("x", lambda t: t.half())),
+    (RuntimeError, lambda: conv_of("weight", lambda t: t.cpu())),
+    (ValueError, lambda: conv_step_of("state", lambda t: t.bfloat16())),
+    (ValueError, lambda: conv_step_of("state", lambda t: t.transpose(0, 1))),
+    (ValueError, lambda: conv_step_of(flags=torch.zeros(1, dtype=torch.uint8, device="cuda"))),
+    (RuntimeError, lambda: conv_step_of("state", lambda t: t.requires_grad_())),
+])
+def test_tensors_that_do_not_fit(error, call):
+    with pytest.raises(error):
+        call()

@@ -1,0 +1,156 @@
+"""What the selective scan, its convolution and the norm with the residual's addition refuse, without a GPU: the C entry points check before they launch."""
+
+import ctypes
+import os
+
+import pytest
+import torch
+
+from griffin_amd import (_lib, hip_add_rmsnorm, hip_add_rmsnorm_quantised, hip_selective_scan, hip_selective_step, hip_short_conv,
+                         hip_short_conv_step)
+
+F32, BF16, ARG, UNSUPPORTED = _lib.RGLRU_F32, _lib.RGLRU_BF16, 1, 2
+FAKE = ctypes.c_void_p(256)                                  # never dereferenced: the checks come first
+STRIDES = (ctypes.c_int64 * 12)(*[64, 8] * 3, *[64, 8, 4] * 2)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        from griffin_amd import build
+
+        build.build()
+    return _lib.load()
+
+
+def scan_fwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, u=FAKE, ws=FAKE, strides=STRIDES):
+    return lib.rglru_hip_selective_fwd(u, FAKE, None, FAKE, FAKE, strides, FAKE, None, None, None, None, FAKE, FAKE, ws, 0, 1, *sizes, dtype, None)
+
+
+def scan_bwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, z=None, scratch=FAKE):
+    return lib.rglru_hip_selective_bwd(FAKE, FAKE, z, FAKE, FAKE, STRIDES, FAKE, None, None, None, FAKE, None, FAKE, scratch, FAKE, FAKE, None, FAKE, FAKE, None,
+                                       None, None, None, 1, *sizes, dtype, None)
+
+
+def scan_step(lib, sizes=(2, 8, 2, 4), dtype=F32, state=FAKE):
+    return lib.rglru_hip_selective_step(FAKE, FAKE, None, FAKE, FAKE, STRIDES, FAKE, None, None, None, state, FAKE, 1, *sizes, dtype, None)
+
+
+def conv_fwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32), activation=1, x=FAKE):
+    return lib.rglru_hip_short_conv_fwd(x, 40, 8, None, FAKE, None, None, FAKE, None, activation, *sizes, *types, None)
+
+
+def conv_bwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32, F32), activation=1, scratch=FAKE):
+    return lib.rglru_hip_short_conv_bwd(FAKE, 40, 8, None, FAKE, None, None, FAKE, scratch, FAKE, None, None, None, activation, *sizes, *types, None)
+
+
+def conv_step(lib, sizes=(2, 8, 4), types=(F32, F32), state=FAKE):
+    return lib.rglru_hip_short_conv_step(FAKE, 8, FAKE, None, None, state, FAKE, 1, *sizes, *types, None)
+
+
+def norm_fwd(lib, sizes=(3, 8), types=(F32, F32, F32), residual=FAKE):
+    return lib.rglru_hip_add_rmsnorm_fwd(FAKE, residual, FAKE, FAKE, FAKE, None, *sizes, 1e-6, *types, None)
+
+
+def norm_bytes(lib, sizes=(3, 8), types=(F32, F32, F32), residual=FAKE, total=FAKE):
+    return lib.rglru_hip_add_rmsnorm_quantised(FAKE, residual, FAKE, total, FAKE, FAKE, *sizes, 1e-6, *types, None)
+
+
+def norm_bwd(lib, sizes=(3, 8), types=(F32, F32, F32, F32), scratch=FAKE):
+    return lib.rglru_hip_add_rmsnorm_bwd(FAKE, FAKE, FAKE, FAKE, None, scratch, FAKE, FAKE, FAKE, *sizes, *types, None)
+
+
+@pytest.mark.parametrize("call, code, word", [
+    (lambda lib: scan_fwd(lib, sizes=(2, 5, 8, 3, 4)), ARG, b"sizes"),
+    (lambda lib: scan_fwd(lib, sizes=(0, 5, 8, 2, 4)), ARG, b"sizes"),
+    (lambda lib: scan_fwd(lib, sizes=(2, 0, 8, 2, 4)), ARG, b"sizes"),
+    (lambda lib: scan_fwd(lib, sizes=(2, 5, 8, 2, 0)), ARG, b"sizes"),
+    (lambda lib: scan_fwd(lib, sizes=(2, 5, 8, 2, 65)), UNSUPPORTED, b"states"),
+    (lambda lib: scan_fwd(lib, dtype=7), ARG, b"dtype"),
+    (lambda lib: scan_fwd(lib, u=None), ARG, b"null"),
+    (lambda lib: scan_fwd(lib, ws=None), ARG, b"null"),
+    (lambda lib: scan_fwd(lib, strides=(ctypes.c_int64 * 12)(64, 1 << 22, *[64, 8] * 2, *[64, 8, 4] * 2)), UNSUPPORTED, b"apart"),
+    (lambda lib: scan_fwd(lib, strides=(ctypes.c_int64 * 12)(*[64, 8] * 3, 64, -8, 4, 64, 8, 4)), UNSUPPORTED, b"apart"),
+    (lambda lib: scan_fwd(lib, sizes=(1 << 24, 5, 8, 1, 4)), UNSUPPORTED, b"too large"),
+    (lambda lib: scan_fwd(lib, sizes=(2, 1 << 31, 8, 1, 4)), UNSUPPORTED, b"too large"),
+    (lambda lib: scan_fwd(lib, sizes=(2, 5, 1 << 22, 1, 4)), UNSUPPORTED, b"too large"),
+    (lambda lib: scan_bwd(lib, sizes=(2, 5, 8, 3, 4)), ARG, b"sizes"),
+    (lambda lib: scan_bwd(lib, scratch=None), ARG, b"null"),
+    (lambda lib: scan_bwd(lib, z=FAKE), ARG, b"null"),
+    (lambda lib: scan_bwd(lib, dtype=-1), ARG, b"dtype"),
+    (lambda lib: scan_step(lib, sizes=(2, 8, 2, 65)), UNSUPPORTED, b"states"),
+    (lambda lib: scan_step(lib, sizes=(2, 9, 2, 4)), ARG, b"sizes"),
+    (lambda lib: scan_step(lib, state=None), ARG, b"null"),
+    (lambda lib: conv_fwd(lib, sizes=(2, 5, 8, 5)), UNSUPPORTED, b"kernel size"),
+    (lambda lib: conv_fwd(lib, sizes=(2, 5, 8, 0)), UNSUPPORTED, b"kernel size"),
+    (lambda lib: conv_fwd(lib, sizes=(2, 0, 8, 4)), ARG, b"sizes"),
+    (lambda lib: conv_fwd(lib, types=(F32, 3)), ARG, b"parameter dtype"),
+    (lambda lib: conv_fwd(lib, types=(3, F32)), ARG, b"dtype"),
+    (lambda lib: conv_fwd(lib, activation=2), ARG, b"activation"),
+    (lambda lib: conv_fwd(lib, x=None), ARG, b"null"),
+    (lambda lib: conv_fwd(lib, sizes=(1 << 24, 5, 8, 4)), UNSUPPORTED, b"too large"),
+    (lambda lib: conv_bwd(lib, scratch=None), ARG, b"null"),
+    (lambda lib: conv_bwd(lib, types=(F32, F32, 9)), ARG, b"gradient dtype"),
+    (lambda lib: conv_step(lib, state=None), ARG, b"null"),
+    (lambda lib: conv_step(lib, sizes=(0, 8, 4)), ARG, b"sizes"),
+    (lambda lib: norm_fwd(lib, sizes=(3, 16385)), UNSUPPORTED, b"exceed"),
+    (lambda lib: norm_fwd(lib, sizes=(0, 8)), ARG, b"sizes"),
+    (lambda lib: norm_fwd(lib, types=(F32, 5, F32)), ARG, b"dtype"),
+    (lambda lib: norm_fwd(lib, types=(F32, F32, 5)), ARG, b"parameter dtype"),
+    (lambda lib: norm_fwd(lib, residual=None), ARG, b"null"),
+    (lambda lib: norm_fwd(lib, sizes=(1 << 37, 8)), UNSUPPORTED, b"too large"),
+    (lambda lib: norm_bytes(lib, total=None), ARG, b"null"),
+    (lambda lib: norm_bytes(lib, sizes=(3, 16385)), UNSUPPORTED, b"exceed"),
+    (lambda lib: norm_bwd(lib, scratch=None), ARG, b"null"),
+    (lambda lib: norm_bwd(lib, types=(F32, F32, F32, 5)), ARG, b"gradient dtype"),
+])
+def test_calls_are_refused(lib, call, code, word):
+    assert call(lib) == code
+    assert word in lib.rglru_hip_last_error()
+
+
+def test_sizes_of_buffers(lib):
+    size, scratch = lib.rglru_hip_selective_workspace_bytes, lib.rglru_hip_selective_scratch_bytes
+    assert size(2, 5, 8, 3, 4, 1) == size(0, 5, 8, 1, 4, 1) == size(2, 5, 8, 1, 65, 0) == scratch(2, 5, 8, 3, 4) == 0
+    # the state in front of every 16 tokens
+    assert size(8, 2048, 2048, 1, 16, 1) - size(8, 2048, 2048, 1, 16, 0) == 8 * 128 * 2048 * 16 * 4
+    assert scratch(2, 5, 8, 2, 4) > 0
+    assert lib.rglru_hip_short_conv_scratch_bytes(2, 5, 8, 5) == 0 < lib.rglru_hip_short_conv_scratch_bytes(2, 5, 8, 4)
+    assert lib.rglru_hip_add_rmsnorm_scratch_bytes(0, 8) == 0 < lib.rglru_hip_add_rmsnorm_scratch_bytes(3, 8)
+    assert lib.rglru_hip_selective_max_states() == 64 and lib.rglru_hip_add_rmsnorm_max_width() == 16384
+
+
+def operands(B=2, T=5, W=8, G=2, N=4):
+    make = torch.zeros
+    return [make(B, T, W), make(B, T, W), make(W, N), make(B, T, G, N), make(B, T, G, N)]
+
+
+def test_no_fallback_on_the_cpu():
+    u, dt, A, B, C = operands()
+    with pytest.raises(RuntimeError):
+        hip_selective_scan(u, dt, A, B, C)
+    with pytest.raises(RuntimeError):
+        hip_selective_scan(u, dt, A, B, C, active_mask=torch.ones(2, 5, dtype=torch.bool))
+    with pytest.raises(RuntimeError):
+        hip_selective_step(u[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], torch.zeros(2, 8, 4))
+    with pytest.raises(RuntimeError):
+        hip_short_conv(u, torch.zeros(8, 1, 4))
+    with pytest.raises(RuntimeError):
+        hip_short_conv_step(u[:, 0], torch.zeros(8, 1, 4), None, torch.zeros(2, 3, 8))
+    with pytest.raises(RuntimeError):
+        hip_add_rmsnorm(u, u, torch.zeros(8))
+    with pytest.raises(RuntimeError):
+        hip_add_rmsnorm_quantised(u, None, torch.zeros(8))
+
+
+def test_arguments_that_are_wrong_anywhere():
+    u, dt, A, B, C = operands()
+    for name in ("reset_mask", "active_mask"):
+        with pytest.raises(ValueError):
+            hip_selective_scan(u, dt, A, B, C, **{name: torch.ones(2, 4, dtype=torch.bool)})
+        with pytest.raises(ValueError):
+            hip_short_conv(u, torch.zeros(8, 1, 4), **{name: torch.ones(2, 4, dtype=torch.bool)})
+    with pytest.raises(ValueError):
+        hip_short_conv(u, torch.zeros(8, 1, 4), activation="gelu")
+    with pytest.raises(ValueError):
+        hip_short_conv_step(u[:, 0], torch.zeros(8, 1, 4), None, torch.zeros(2, 3, 8), "relu")
