@@ -27,6 +27,7 @@ constexpr int kSelTile = 16;                  // tokens of a tile; the forward p
 constexpr int kSelLanes = 16;                 // channels of a wave
 constexpr int kSelStates = 16;                // states of a wave
 constexpr int kSelMaxStates = 64;
+constexpr int kSelPipe = 2;                   // waves that take a sequence's tiles in turn
 constexpr int kSelMaxSegments = 64;
 constexpr unsigned kSelRange = 0x7fffff00u;   // bytes of a tile's buffers; kOutOfRange lies outside
 
@@ -43,25 +44,32 @@ struct SelArgs {
   float *dA, *dD, *dbias;                     // [B][S][W][N], [B][S][W]
   long long sub, sut, sdb, sdt, szb, szt, sBb, sBt, sBg, sCb, sCt, sCg;  // elements between batch rows, tokens and groups
   int B, T, W, N, G, Wg;                      // Wg: channels of a group
-  int per_group;                              // workgroups of a group's channels
-  int S, tiles, seg_tiles;                    // segments, tiles of a sequence and of a segment
-  int softplus, vector;                       // vector: rows of B and C go by whole vectors of four elements
+  int per_group, pipe_group;                  // workgroups of a group's channels: one wave, or kSelPipe waves to 16 of them (and states)
+  int S, tiles, seg_tiles;                    // segments, tiles of a sequence and of a segment (of the pass)
+  int softplus, whole;                        // whole: rows of B, C and the states are whole vectors of four elements
 };
 
 // A place of the walk: what all lanes of a wave share.
 struct SelPlace {
-  int b, seg, g, set, slab, cg;
+  int b, seg, g, set, slab, turn, cg;
 };
-template <int SLABS> RGLRU_DEVICE SelPlace sel_place(const SelArgs& p) {
+// Workgroups go round the 8 XCDs in turn: those of neighbouring channels, which share lines of memory, are given to one of them.
+RGLRU_DEVICE unsigned sel_block() {
+  const unsigned n = gridDim.x, whole = n / 8 * 8, i = blockIdx.x;
+  return i < whole ? i % 8 * (n / 8) + i / 8 : i;
+}
+// SLABS waves of a workgroup share channels, by their states; PIPE teams of them, by tiles in turn.
+template <int SLABS, int PIPE> RGLRU_DEVICE SelPlace sel_place(const SelArgs& p) {
   SelPlace r;
-  unsigned i = blockIdx.x;
+  unsigned i = sel_block();
   r.set = (int)(i % (unsigned)p.per_group); i /= (unsigned)p.per_group;
   r.g = (int)(i % (unsigned)p.G); i /= (unsigned)p.G;
   r.seg = (int)(i % (unsigned)p.S);
   r.b = (int)(i / (unsigned)p.S);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   r.slab = wave % SLABS;
-  r.cg = (r.set * kSelWaves + wave) / SLABS;
+  r.turn = wave / SLABS % PIPE;
+  r.cg = (r.set * kSelWaves + wave) / (SLABS * PIPE);
   return r;
 }
 
@@ -115,7 +123,6 @@ RGLRU_DEVICE void wave_order() {
 struct SelRate { float s, slope; };
 RGLRU_DEVICE SelRate sel_rate(float x, bool soft) {
   SelRate r;
-  if (!soft) { r.s = x; r.slope = 1.f; return r; }
   const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
   const float v = e * __builtin_amdgcn_rcpf(2.f + e), v2 = v * v;
   float q = 1.f / 13.f;
@@ -125,62 +132,84 @@ RGLRU_DEVICE SelRate sel_rate(float x, bool soft) {
   q = fmaf(q, v2, 1.f / 5.f);
   q = fmaf(q, v2, 1.f / 3.f);
   q = fmaf(q, v2, 1.f);
-  r.s = fmaxf(x, 0.f) + 2.f * v * q;
-  r.slope = (x >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+  r.s = soft ? fmaxf(x, 0.f) + 2.f * v * q : x;
+  r.slope = soft ? (x >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e) : 1.f;
   return r;
 }
 
-// Tokens t0 + 4 q + j (q = 0 .. 3) of one operand, a channel a lane.
+// One operand of u's shape, a channel a lane: tokens t0 + 4 q + j of a tile (q = 0 .. 3) as they lie in memory, so that nothing waits for them before they
+// are used.  The buffer ends with the tile's last token; lanes without a channel ask behind it.
 template <typename IO> struct SelStream {
-  float v[4];
-  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int c, int left, bool ok, int j) {
-    const rsrc_t r = make_rsrc((const IO*)base + at, kSelRange);
+  int raw[4];
+  static RGLRU_DEVICE unsigned lane_offset(unsigned stride, int w, bool ok, int j) {
+    return ok ? ((unsigned)j * stride + (unsigned)w) * (unsigned)sizeof(IO) : kOutOfRange;
+  }
+  static RGLRU_DEVICE rsrc_t tile(const void* base, long long at, unsigned stride, int left) {
+    return make_rsrc((const IO*)base + at, stride ? (unsigned)left * stride * (unsigned)sizeof(IO) : kSelRange);
+  }
+  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int left, unsigned lane) {
+    const rsrc_t r = tile(base, at, stride, left);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int t = 4 * q + j;
-      v[q] = BufIo<IO>::load(r, ok && t < left ? ((unsigned)t * stride + (unsigned)c) * (unsigned)sizeof(IO) : kOutOfRange, 0);
+      const unsigned off = lane + (unsigned)q * 4u * stride * (unsigned)sizeof(IO);
+      if constexpr (sizeof(IO) == 2) raw[q] = (int)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+      else raw[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
     }
   }
+  RGLRU_DEVICE float operator[](int q) const { return __builtin_bit_cast(float, sizeof(IO) == 2 ? raw[q] << 16 : raw[q]); }
 };
-template <typename IO> RGLRU_DEVICE void sel_store(const float (&v)[4], void* base, long long at, unsigned stride, int c, int left, bool ok, int j) {
-  const rsrc_t r = make_rsrc((IO*)base + at, kSelRange);
+template <typename IO> RGLRU_DEVICE void sel_store(const float (&v)[4], void* base, long long at, unsigned stride, int left, unsigned lane) {
+  const rsrc_t r = SelStream<IO>::tile(base, at, stride, left);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int t = 4 * q + j;
-    BufIo<IO>::store((IO)v[q], r, ok && t < left ? ((unsigned)t * stride + (unsigned)c) * (unsigned)sizeof(IO) : kOutOfRange, 0);
-  }
+  for (int q = 0; q < 4; ++q) BufIo<IO>::store((IO)v[q], r, lane + (unsigned)q * 4u * stride * (unsigned)sizeof(IO), 0);
 }
 
-// Elements n0 .. n0 + 3 of token t0 + lane % 16 of B or C.
-template <typename IO> struct SelVector {
-  float v[4];
-  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int n0, int N, int left, int k, bool vector) {
+// Elements n0 .. n0 + 3 of token t0 + lane % 16 of B or C, as they lie in memory.
+template <typename IO, bool WHOLE> struct SelVector {
+  int raw[4];
+  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int n0, int N, int left, int k) {
     const rsrc_t r = make_rsrc((const IO*)base + at, kSelRange);
-    const unsigned off = ((unsigned)k * stride + (unsigned)n0) * (unsigned)sizeof(IO);
-    if (vector) {
-      const unsigned o = k < left && n0 < N ? off : kOutOfRange;
+    const unsigned off = k < left ? ((unsigned)k * stride + (unsigned)n0) * (unsigned)sizeof(IO) : kOutOfRange;
+    if constexpr (WHOLE) {
+      const unsigned o = n0 < N ? off : kOutOfRange;
       if constexpr (sizeof(IO) == 2) {
-        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
-        v[0] = __uint_as_float(w[0] << 16); v[1] = __uint_as_float(w[0] & 0xffff0000u);
-        v[2] = __uint_as_float(w[1] << 16); v[3] = __uint_as_float(w[1] & 0xffff0000u);
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        const i32x2 w = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        raw[0] = w[0]; raw[1] = w[1];
       } else {
-        const f32x4 w = buf_load_frag<f32x4>(r, o);
+        const i32x4 w = buf_load_frag<i32x4>(r, o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = w[i];
+        for (int i = 0; i < 4; ++i) raw[i] = w[i];
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = BufIo<IO>::load(r, k < left && n0 + i < N ? off + (unsigned)(i * sizeof(IO)) : kOutOfRange, 0);
+      for (int i = 0; i < 4; ++i) {
+        const unsigned o = n0 + i < N ? off + (unsigned)(i * sizeof(IO)) : kOutOfRange;
+        if constexpr (sizeof(IO) == 2) raw[i] = (int)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+        else raw[i] = (int)__builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      }
+    }
+  }
+  RGLRU_DEVICE void get(float (&v)[4], bool live) const {
+    if constexpr (sizeof(IO) == 2 && WHOLE) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[2 * i] = live ? __uint_as_float((unsigned)raw[i] << 16) : 0.f;
+        v[2 * i + 1] = live ? __uint_as_float((unsigned)raw[i] & 0xffff0000u) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = live ? __builtin_bit_cast(float, sizeof(IO) == 2 ? raw[i] << 16 : raw[i]) : 0.f;
     }
   }
 };
 
-// Four states of a lane, at p + n0 .. (rows of N).
-RGLRU_DEVICE void sel_load_states(const float* p, long long row, int n0, int N, bool ok, float (&v)[4]) {
+// Four states of a lane, n0 .. n0 + 3 of a row of N.  `whole`: rows are whole vectors on 16-byte boundaries.
+RGLRU_DEVICE void sel_load_states(const float* p, long long row, int n0, int N, bool ok, bool whole, float (&v)[4]) {
   const float* at = p + row * N + n0;
-  if (ok && n0 + 4 <= N && ((uintptr_t)at & 15) == 0) {
-    const f32x4 w = *reinterpret_cast<const f32x4*>(at);
+  if (whole) {
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    if (ok && n0 < N) w = *reinterpret_cast<const f32x4*>(at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = w[i];
   } else {
@@ -188,16 +217,44 @@ RGLRU_DEVICE void sel_load_states(const float* p, long long row, int n0, int N, 
     for (int i = 0; i < 4; ++i) v[i] = ok && n0 + i < N ? at[i] : 0.f;
   }
 }
-RGLRU_DEVICE void sel_store_states(float* p, long long row, int n0, int N, bool ok, const float (&v)[4]) {
+RGLRU_DEVICE void sel_store_states(float* p, long long row, int n0, int N, bool ok, bool whole, const float (&v)[4]) {
   float* at = p + row * N + n0;
-  if (ok && n0 + 4 <= N && ((uintptr_t)at & 15) == 0) {
-    *reinterpret_cast<f32x4*>(at) = (f32x4){v[0], v[1], v[2], v[3]};
+  if (whole) {
+    if (ok && n0 < N) *reinterpret_cast<f32x4*>(at) = (f32x4){v[0], v[1], v[2], v[3]};
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (ok && n0 + i < N) at[i] = v[i];
   }
 }
+
+// The same of rows that begin at `rows`, `count` of them, by a buffer: nothing branches, and what lies outside is dropped.
+template <bool WHOLE> struct SelStates {
+  int raw[4];
+  static RGLRU_DEVICE unsigned lane_offset(int w, int n0, int N, bool ok) { return ok && n0 < N ? ((unsigned)w * (unsigned)N + (unsigned)n0) * 4u : kOutOfRange; }
+  static RGLRU_DEVICE rsrc_t rows(const float* p, long long at, int count, int N) { return make_rsrc(p + at * N, p ? (unsigned)count * (unsigned)N * 4u : 0u); }
+  RGLRU_DEVICE void load(rsrc_t r, unsigned lane, int n0, int N) {
+    if constexpr (WHOLE) {
+      const i32x4 w = buf_load_frag<i32x4>(r, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = (int)__builtin_amdgcn_raw_buffer_load_b32(r, n0 + i < N ? lane + 4u * i : kOutOfRange, 0, 0);
+    }
+  }
+  static RGLRU_DEVICE void store(rsrc_t r, unsigned lane, int n0, int N, const float (&v)[4]) {
+    if constexpr (WHOLE) {
+      buf_store_b128(__builtin_bit_cast(i32x4, (f32x4){v[0], v[1], v[2], v[3]}), r, lane);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, v[i]), r, n0 + i < N ? lane + 4u * i : kOutOfRange, 0, 0);
+    }
+  }
+};
+
+// Has the compiler make `v` here, and not where it is used.
+RGLRU_DEVICE void sel_made(float& v) { asm volatile("" : "+v"(v)); }
 
 // The masks of a tile's tokens, the same in all lanes: bit k is token t0 + k's.  Tokens behind the sequence's end are inactive.
 struct SelMasks { unsigned live, starts; };
@@ -226,7 +283,7 @@ template <bool REVERSE> RGLRU_DEVICE void sel_join(const SelArgs& p, const SelPl
   for (int r = 0; r < count; ++r) {
     const long long row = ((long long)at.b * p.S + (REVERSE ? p.S - 1 - r : r)) * p.W + w;
     float e[4];
-    sel_load_states(p.ends, row, n0, p.N, ok, e);
+    sel_load_states(p.ends, row, n0, p.N, ok, p.whole, e);
     const float sum = ok ? p.sums[2 * row] : 0.f;
     const bool cut = ok && p.sums[2 * row + 1] != 0.f;
 #pragma unroll

@@ -8,38 +8,30 @@
 
 namespace rglru {
 
-// SUMMARY: what a segment leaves of a state of zeros and its sum of step sizes.  Otherwise outputs, the last state and, for a backward pass, the state
-// in front of every tile.
-template <typename IO, int SLABS, bool MASKED, bool SUMMARY> __global__ __launch_bounds__(kSelThreads) void sel_forward_kernel(SelArgs p) {
+// What a segment leaves of a state of zeros, and its sum of step sizes.
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_summary_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
-  __shared__ float parts[SLABS > 1 && !SUMMARY ? 2 : 1][SLABS > 1 && !SUMMARY ? kSelWaves : 1][4][64];
-  const SelPlace at = sel_place<SLABS>(p);
-  if (SUMMARY && at.seg == p.S - 1) return;                 // nothing asks what the last one leaves
+  const SelPlace at = sel_place<SLABS, 1>(p);
+  if (at.seg == p.S - 1) return;                            // nothing asks what the last one leaves
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
   const int w = at.g * p.Wg + (ok ? in_group : 0);
   const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
   float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-  sel_load_states(p.A, w, n0, p.N, ok, a2);
+  sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
-  const float bias = ok && p.bias ? p.bias[w] : 0.f, skip = ok && p.D ? p.D[w] : 0.f;
-  if constexpr (!SUMMARY) {
-    if (p.h0) sel_load_states(p.h0, (long long)at.b * p.W + w, n0, p.N, ok, h);
-    sel_join<false>(p, at, w, n0, ok, a2, h);
-  }
-  SelStream<IO> next_u, next_dt, next_z;
-  SelVector<IO> next_B, next_C;
-  const bool gated = !SUMMARY && p.z != nullptr;
+  const float bias = ok && p.bias ? p.bias[w] : 0.f;
+  const unsigned lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j), lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
+  SelStream<IO> next_u, next_dt;
+  SelVector<IO, WHOLE> next_B;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, w, left, ok, j);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, w, left, ok, j);
-    if (gated) next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, w, left, ok, j);
-    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c, p.vector);
-    if (!SUMMARY) next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c, p.vector);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
+    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
   };
   request(first);
   float total = 0.f;
@@ -48,48 +40,152 @@ template <typename IO, int SLABS, bool MASKED, bool SUMMARY> __global__ __launch
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
-    float u[4], z[4], B[4], C[4];
+    float B[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool live = (m.live >> (4 * q + j)) & 1u;
-      const float s = live ? sel_rate(next_dt.v[q] + bias, p.softplus).s : 0.f;
-      u[q] = live ? next_u.v[q] : 0.f;
-      z[q] = live && gated ? next_z.v[q] : 0.f;
-      rates[wave][4 * q + j][c] = make_float2(s, s * u[q]);
-      if (SUMMARY) total += s;
+      const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f;
+      rates[wave][4 * q + j][c] = make_float2(s, live ? s * next_u[q] : 0.f);
+      total += s;
     }
-    const bool mine = (m.live >> c) & 1u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      B[i] = mine ? next_B.v[i] : 0.f;
-      C[i] = !SUMMARY && mine ? next_C.v[i] : 0.f;
-    }
+    next_B.get(B, (m.live >> c) & 1u);
     wave_order();
     if (tile + 1 < last) request(tile + 1);
-    if (!SUMMARY && p.kept) sel_store_states(p.kept, ((long long)at.b * p.tiles + tile) * p.W + w, n0, p.N, ok, h);
     if (MASKED) cut = cut || m.starts;
+    sel_each<kSelTile>([&](auto token) {
+      constexpr int t = decltype(token)::value;
+      const float2 rate = rates[wave][t][c];
+      if constexpr (MASKED)
+        if ((m.starts >> t) & 1u) h[0] = h[1] = h[2] = h[3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(a2[i] * rate.x), h[i], row_bcast<t>(B[i]) * rate.y);
+    });
+    wave_order();                                           // the next tile's rates come after these reads
+  }
+  const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
+  sel_store_states(p.ends, row, n0, p.N, ok, WHOLE, h);
+  total = all_rows_sum(total);
+  if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
+}
+
+// Outputs, the last state and, for a backward pass, the state in front of every tile.
+// PIPE waves take a sequence's tiles in turn.  Decays and what is written need no state, so a wave makes those of its tile while the one in front walks; the
+// state then goes through the tile in 16 steps of one multiply-add, and on to the next wave through LDS before anything is made of it.
+template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads, 2) void sel_forward_kernel(SelArgs p) {
+  constexpr int TEAMS = kSelWaves / (SLABS * PIPE);
+  __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
+  __shared__ f32x4 passed[PIPE > 1 ? kSelWaves : 1][64];     // the state in front of a wave's next tile
+  __shared__ int ready[kSelWaves];                           // that tile
+  __shared__ float parts[SLABS > 1 ? 2 : 1][SLABS > 1 ? kSelWaves : 1][4][64];
+  static_assert(TEAMS * SLABS * PIPE == kSelWaves && (SLABS == 1 || PIPE == 1), "waves of a workgroup");
+  const SelPlace at = sel_place<SLABS, PIPE>(p);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, j = lane >> 4;
+  const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
+  const bool ok = in_group < p.Wg;
+  const int w = at.g * p.Wg + (ok ? in_group : 0);
+  const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
+  if constexpr (PIPE > 1) {
+    if (threadIdx.x < kSelWaves) ready[threadIdx.x] = -1;
+    __syncthreads();
+  }
+  float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+  sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
+  const float bias = ok && p.bias ? p.bias[w] : 0.f, skip = ok && p.D ? p.D[w] : 0.f;
+  if (at.turn == 0) {
+    if (p.h0) sel_load_states(p.h0, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
+    sel_join<false>(p, at, w, n0, ok, a2, h);
+  }
+  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
+  const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
+  const unsigned lane_h = SelStates<WHOLE>::lane_offset(w, n0, p.N, ok);
+  const bool gated = p.z != nullptr;
+  const unsigned lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
+  SelStream<IO> next_u, next_dt, next_z;
+  SelVector<IO, WHOLE> next_B, next_C;
+  auto request = [&](int tile) {
+    const long long t0 = (long long)tile * kSelTile;
+    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
+    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
+    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+  };
+  if (first + at.turn < last) request(first + at.turn);
+  for (int tile = first + at.turn; tile < last; tile += PIPE) {
+    const long long t0 = (long long)tile * kSelTile;
+    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
+    float u[4], gate[4], B[4], C[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool live = (m.live >> (4 * q + j)) & 1u;
+      const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f, z = next_z[q];
+      u[q] = live ? next_u[q] : 0.f;
+      gate[q] = gated ? z * sigmoid_fast(z) : 1.f;
+      rates[wave][4 * q + j][c] = make_float2(s, s * u[q]);
+    }
+    next_B.get(B, (m.live >> c) & 1u);
+    next_C.get(C, (m.live >> c) & 1u);
+    wave_order();
+    if (tile + PIPE < last) request(tile + PIPE);
+    float a[kSelTile][4], x[kSelTile][4];
+    sel_each<kSelTile>([&](auto token) {
+      constexpr int t = decltype(token)::value;
+      const float2 rate = rates[wave][t][c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[t][i] = __builtin_amdgcn_exp2f(a2[i] * rate.x);
+        x[t][i] = row_bcast<t>(B[i]) * rate.y;
+        sel_made(a[t][i]), sel_made(x[t][i]);                // in front of the wait
+      }
+    });
+    wave_order();                                           // the next tile's rates come after these reads
+    if constexpr (PIPE > 1) {
+      if (tile > first) {
+        while (__hip_atomic_load(&ready[wave], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) != tile) __builtin_amdgcn_s_sleep(1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        const f32x4 got = passed[wave][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = got[i];
+      }
+    }
+    float before[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) before[i] = h[i];
+    __builtin_amdgcn_s_setprio(3);                          // the other waves wait for what follows
+    sel_each<kSelTile>([&](auto token) {
+      constexpr int t = decltype(token)::value;
+      if constexpr (MASKED)
+        if ((m.starts >> t) & 1u) h[0] = h[1] = h[2] = h[3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[t][i] = h[i] = fmaf(a[t][i], h[i], x[t][i]);
+    });
+    if constexpr (PIPE > 1) {
+      if (tile + 1 < last) {                                // this wave read what the next one leaves there before that one could
+        const int to = at.turn + 1 == PIPE ? wave + 1 - PIPE : wave + 1;
+        passed[to][lane] = (f32x4){h[0], h[1], h[2], h[3]};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __hip_atomic_store(&ready[to], tile + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    SelStates<WHOLE>::store(SelStates<WHOLE>::rows(p.kept, ((long long)at.b * p.tiles + tile) * p.W, p.W, p.N), lane_h, n0, p.N, before);
     float y[4];
     sel_each<4>([&](auto group) {
       float sums[4];
       sel_each<4>([&](auto token) {
         constexpr int t = 4 * decltype(group)::value + decltype(token)::value;
-        const float2 rate = rates[wave][t][c];
-        if constexpr (MASKED)
-          if ((m.starts >> t) & 1u) h[0] = h[1] = h[2] = h[3] = 0.f;
-        float sum = 0.f;
+        float sum = row_bcast<t>(C[0]) * x[t][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = __builtin_amdgcn_exp2f(a2[i] * rate.x);
-          h[i] = fmaf(a, h[i], row_bcast<t>(B[i]) * rate.y);
-          if (!SUMMARY) sum = fmaf(row_bcast<t>(C[i]), h[i], sum);
-        }
+        for (int i = 1; i < 4; ++i) sum += row_bcast<t>(C[i]) * x[t][i];
         sums[decltype(token)::value] = sum;
       });
-      if (!SUMMARY) y[decltype(group)::value] = four_rows_sum(sums);
+      y[decltype(group)::value] = four_rows_sum(sums);
     });
-    wave_order();                                           // the next tile's rates come after these reads
-    if constexpr (SUMMARY) continue;
-    if constexpr (SLABS > 1) {                              // the other states of these channels: each wave takes its share of the tokens
+    if constexpr (SLABS > 1) {                              // the other states of these channels
       float (*mem)[4][64] = parts[tile & 1];
 #pragma unroll
       for (int q = 0; q < 4; ++q) mem[wave][q][lane] = y[q];
@@ -104,34 +200,30 @@ template <typename IO, int SLABS, bool MASKED, bool SUMMARY> __global__ __launch
       }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      y[q] = fmaf(skip, u[q], y[q]);
-      if (gated) y[q] *= z[q] * sigmoid_fast(z[q]);
-      if (!((m.live >> (4 * q + j)) & 1u)) y[q] = 0.f;
-    }
-    if (SLABS == 1 || at.slab == 0)
-      sel_store<IO>(y, p.y, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, w, left, ok, j);
+    for (int q = 0; q < 4; ++q) y[q] = (m.live >> (4 * q + j)) & 1u ? fmaf(skip, u[q], y[q]) * gate[q] : 0.f;
+    if (SLABS == 1 || at.slab == 0) sel_store<IO>(y, p.y, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
   }
-  if constexpr (SUMMARY) {
-    const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
-    sel_store_states(p.ends, row, n0, p.N, ok, h);
-    total = all_rows_sum(total);
-    if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
-  } else if (at.seg == p.S - 1) {
-    sel_store_states(p.h_last, (long long)at.b * p.W + w, n0, p.N, ok, h);
-  }
+  if ((last - 1 - first) % PIPE == at.turn && at.seg == p.S - 1) sel_store_states(p.h_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
 }
 
-template <typename IO, int SLABS, bool MASKED> static void sel_forward_masked(const SelArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.B * (long long)a.S * a.G * a.per_group)), block(kSelThreads);
-  if (a.S > 1) hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, MASKED, true>), grid, block, 0, s, a);
-  hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, MASKED, false>), grid, block, 0, s, a);
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_forward_whole(const SelArgs& a, hipStream_t s) {
+  constexpr int PIPE = SLABS == 1 ? kSelPipe : 1;
+  const dim3 block(kSelThreads);
+  if (a.S > 1)
+    hipLaunchKernelGGL((sel_summary_kernel<IO, SLABS, MASKED, WHOLE>), dim3((unsigned)(a.B * (long long)a.S * a.G * a.per_group)), block, 0, s, a);
+  SelArgs f = a;
+  f.per_group = PIPE > 1 ? a.pipe_group : a.per_group;
+  hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, PIPE, MASKED, WHOLE>), dim3((unsigned)(f.B * (long long)f.S * f.G * f.per_group)), block, 0, s, f);
+}
+template <typename IO, int SLABS> static void sel_forward_slabs(const SelArgs& a, hipStream_t s) {
+  if (a.flags) { if (a.whole) sel_forward_whole<IO, SLABS, true, true>(a, s); else sel_forward_whole<IO, SLABS, true, false>(a, s); }
+  else { if (a.whole) sel_forward_whole<IO, SLABS, false, true>(a, s); else sel_forward_whole<IO, SLABS, false, false>(a, s); }
 }
 template <typename IO> static void sel_forward_typed(const SelArgs& a, hipStream_t s) {
   const int slabs = (a.N + kSelStates - 1) / kSelStates;
-  if (slabs == 1) { if (a.flags) sel_forward_masked<IO, 1, true>(a, s); else sel_forward_masked<IO, 1, false>(a, s); }
-  else if (slabs == 2) { if (a.flags) sel_forward_masked<IO, 2, true>(a, s); else sel_forward_masked<IO, 2, false>(a, s); }
-  else { if (a.flags) sel_forward_masked<IO, 4, true>(a, s); else sel_forward_masked<IO, 4, false>(a, s); }
+  if (slabs == 1) sel_forward_slabs<IO, 1>(a, s);
+  else if (slabs == 2) sel_forward_slabs<IO, 2>(a, s);
+  else sel_forward_slabs<IO, 4>(a, s);
 }
 
 int sel_launch_forward(const SelArgs& a, int dtype, hipStream_t s) {

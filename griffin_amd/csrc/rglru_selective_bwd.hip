@@ -19,9 +19,9 @@ namespace rglru {
 
 // What a segment hands back of a gradient of zeros at its last state.  (Its sums of step sizes and document starts are made again here: the forward
 // pass keeps them only until its own join.)
-template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSelThreads) void sel_reverse_kernel(SelArgs p) {
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_reverse_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
-  const SelPlace at = sel_place<SLABS>(p);
+  const SelPlace at = sel_place<SLABS, 1>(p);
   if (at.seg == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
@@ -29,20 +29,22 @@ template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSel
   const int w = at.g * p.Wg + (ok ? in_group : 0);
   const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
   float a2[4], carry[4] = {0.f, 0.f, 0.f, 0.f};
-  sel_load_states(p.A, w, n0, p.N, ok, a2);
+  sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
   const float bias = ok && p.bias ? p.bias[w] : 0.f;
   const bool gated = p.z != nullptr;
+  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
+  const unsigned lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
   SelStream<IO> next_dt, next_z, next_d;
-  SelVector<IO> next_C;
+  SelVector<IO, WHOLE> next_C;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, w, left, ok, j);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, w, left, ok, j);
-    if (gated) next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, w, left, ok, j);
-    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c, p.vector);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
+    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
   };
   request(last - 1);
   float total = 0.f;
@@ -55,15 +57,13 @@ template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSel
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool live = (m.live >> (4 * q + j)) & 1u;
-      const float s = live ? sel_rate(next_dt.v[q] + bias, p.softplus).s : 0.f;
-      float dy = live ? next_d.v[q] : 0.f;
-      if (gated && live) dy *= next_z.v[q] * sigmoid_fast(next_z.v[q]);
-      rates[wave][4 * q + j][c] = make_float2(s, dy);
+      const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f, z = next_z[q];
+      const float dy = next_d[q] * (gated ? z * sigmoid_fast(z) : 1.f);
+      rates[wave][4 * q + j][c] = make_float2(s, live ? dy : 0.f);
       total += s;
     }
     const bool mine = (m.live >> c) & 1u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) C[i] = mine ? next_C.v[i] : 0.f;
+    next_C.get(C, mine);
     wave_order();
     if (tile > first) request(tile - 1);
     if (MASKED) cut = cut || m.starts;
@@ -71,79 +71,85 @@ template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSel
       constexpr int t = kSelTile - 1 - decltype(token)::value;
       const float2 rate = rates[wave][t][c];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) carry[i] = fmaf(row_bcast<t>(C[i]), rate.y, carry[i]) * __builtin_amdgcn_exp2f(a2[i] * rate.x);
+      for (int i = 0; i < 4; ++i) carry[i] = (row_bcast<t>(C[i]) * rate.y + carry[i]) * __builtin_amdgcn_exp2f(a2[i] * rate.x);
       if constexpr (MASKED)
         if ((m.starts >> t) & 1u) carry[0] = carry[1] = carry[2] = carry[3] = 0.f;
     });
     wave_order();
   }
   const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
-  sel_store_states(p.ends, row, n0, p.N, ok, carry);
+  sel_store_states(p.ends, row, n0, p.N, ok, WHOLE, carry);
   total = all_rows_sum(total);
   if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
 }
 
-template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSelThreads, 1) void sel_backward_kernel(SelArgs p) {
-  __shared__ f32x4 rates[kSelWaves][kSelTile][kSelLanes];   // step size, that times u, dy
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads, 2) void sel_backward_kernel(SelArgs p) {
+  __shared__ f32x4 rates[kSelWaves][kSelTile][kSelLanes];   // step size, that times u, dy, u
+  __shared__ f32x4 gates[kSelWaves][kSelTile][kSelLanes];   // slope of the step size, d silu'(z), sum over the states of C h
+  // what a lane needs once a tile, out of its registers: the state in front of the tile, and its sums over the tiles before
+  __shared__ f32x4 fronts[kSelWaves][64], sum_dA[kSelWaves][64];
+  __shared__ float2 sum_rows[kSelWaves][64];
   __shared__ float vectors[2][2][kSelWaves][4][64];         // dB and dC of a tile, by waves; two tiles in turn
   __shared__ float parts[SLABS > 1 ? 2 : 1][SLABS > 1 ? kSelWaves : 1][3][4][64];
-  const SelPlace at = sel_place<SLABS>(p);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
+  const SelPlace at = sel_place<SLABS, 1>(p);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
   const int w = at.g * p.Wg + (ok ? in_group : 0);
   const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
-  float a2[4], carry[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
-  sel_load_states(p.A, w, n0, p.N, ok, a2);
+  float a2[4], carry[4] = {0.f, 0.f, 0.f, 0.f};
+  sum_dA[wave][lane] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  sum_rows[wave][lane] = make_float2(0.f, 0.f);
+  sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
   const float bias = ok && p.bias ? p.bias[w] : 0.f, skip = ok && p.D ? p.D[w] : 0.f;
-  if (p.dh_last) sel_load_states(p.dh_last, (long long)at.b * p.W + w, n0, p.N, ok, carry);
+  if (p.dh_last) sel_load_states(p.dh_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, carry);
   sel_join<true>(p, at, w, n0, ok, a2, carry);
   const bool gated = p.z != nullptr;
+  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
+  const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j), lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
+  const unsigned lane_h = SelStates<WHOLE>::lane_offset(w, n0, p.N, ok);
+  // what is written for the tile's tokens: one lane a token and channel, of the first slab's waves
+  const unsigned lane_out = SLABS == 1 || at.slab == 0 ? lane_d : kOutOfRange;
   SelStream<IO> next_u, next_dt, next_z, next_d;
-  SelVector<IO> next_B, next_C;
-  float next_h[4];
+  SelVector<IO, WHOLE> next_B, next_C;
+  SelStates<WHOLE> next_h;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, w, left, ok, j);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, w, left, ok, j);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, w, left, ok, j);
-    if (gated) next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, w, left, ok, j);
-    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c, p.vector);
-    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c, p.vector);
-    sel_load_states(p.kept, ((long long)at.b * p.tiles + tile) * p.W + w, n0, p.N, ok, next_h);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
+    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
+    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
+    next_h.load(SelStates<WHOLE>::rows(p.kept, ((long long)at.b * p.tiles + tile) * p.W, p.W, p.N), lane_h, n0, p.N);
   };
   request(last - 1);
   for (int tile = last - 1; tile >= first; --tile) {
-    const long long t0 = (long long)tile * kSelTile;
+    const long long t0 = (long long)tile * kSelTile, place = ((long long)at.b * p.T + t0) * p.W;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
-    float u[4], s[4], slope[4], d[4], z[4], dy[4], B[4], C[4], before[4];
+    float B[4], C[4], before[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool live = (m.live >> (4 * q + j)) & 1u;
-      const SelRate rate = sel_rate(next_dt.v[q] + bias, p.softplus);
-      s[q] = live ? rate.s : 0.f;
-      slope[q] = live ? rate.slope : 0.f;
-      u[q] = live ? next_u.v[q] : 0.f;
-      d[q] = live ? next_d.v[q] : 0.f;
-      z[q] = live && gated ? next_z.v[q] : 0.f;
-      dy[q] = gated ? d[q] * (z[q] * sigmoid_fast(z[q])) : d[q];
-      rates[wave][4 * q + j][c] = (f32x4){s[q], s[q] * u[q], dy[q], 0.f};
+      const SelRate rate = sel_rate(next_dt[q] + bias, p.softplus);
+      const float z = next_z[q], sig = sigmoid_fast(z);
+      const float s = live ? rate.s : 0.f, u = live ? next_u[q] : 0.f, d = live ? next_d[q] : 0.f, slope = live ? rate.slope : 0.f;
+      const float dy = live && gated ? d * z * sig : d, dz = live && gated ? d * (sig * fmaf(z, 1.f - sig, 1.f)) : 0.f;
+      rates[wave][4 * q + j][c] = (f32x4){s, s * u, dy, u};
+      gates[wave][4 * q + j][c] = (f32x4){slope, dz, 0.f, 0.f};
     }
-    const bool mine = (m.live >> c) & 1u;
+    next_B.get(B, (m.live >> c) & 1u);
+    next_C.get(C, (m.live >> c) & 1u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      B[i] = mine ? next_B.v[i] : 0.f;
-      C[i] = mine ? next_C.v[i] : 0.f;
-      before[i] = next_h[i];
-    }
+    for (int i = 0; i < 4; ++i) before[i] = __builtin_bit_cast(float, next_h.raw[i]);
+    fronts[wave][lane] = (f32x4){before[0], before[1], before[2], before[3]};
     wave_order();
-    if (tile > first) request(tile - 1);
     // decays and states of the tile, and y where the gate asks for it
-    float a[kSelTile][4], h[kSelTile][4], y[4];
+    float a[kSelTile][4], h[kSelTile][4];
     sel_each<4>([&](auto group) {
       float sums[4];
       sel_each<4>([&](auto token) {
@@ -156,50 +162,70 @@ template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSel
           if constexpr (MASKED) old = (m.starts >> t) & 1u ? 0.f : old;
           a[t][i] = __builtin_amdgcn_exp2f(a2[i] * rate.x);
           h[t][i] = fmaf(a[t][i], old, row_bcast<t>(B[i]) * rate.y);
-          sum = fmaf(row_bcast<t>(C[i]), h[t][i], sum);
+          sum = i ? sum + row_bcast<t>(C[i]) * h[t][i] : row_bcast<t>(C[i]) * h[t][i];
         }
         sums[decltype(token)::value] = sum;
       });
-      y[decltype(group)::value] = gated ? four_rows_sum(sums) : 0.f;
+      gates[wave][4 * decltype(group)::value + j][c][2] = four_rows_sum(sums);
+      __builtin_amdgcn_sched_barrier(0);
     });
-    float along[4], through[4], tile_dA[4] = {0.f, 0.f, 0.f, 0.f}, tile_dD = 0.f, tile_dbias = 0.f;  // tile by tile: a long sum loses less
+    // other names for B and C: broadcasts of theirs that the way back shared with the way there would each keep a register
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sel_made(B[i]), sel_made(C[i]);
+    float tile_dA[4] = {0.f, 0.f, 0.f, 0.f}, tile_dD = 0.f, tile_dbias = 0.f;  // tile by tile: a long sum loses less
+    // what one lane makes of its tokens' sums
+    auto finish = [&](int q, float along, float through, const float* y_all) {
+      const f32x4 rate = rates[wave][4 * q + j][c], gate = gates[wave][4 * q + j][c];
+      const float ddt = fmaf(rate[3], along, through * kLn2) * gate[0];
+      const bool live = (m.live >> (4 * q + j)) & 1u;
+      const float du = live ? fmaf(rate[0], along, skip * rate[2]) : 0.f, dt_out = live ? ddt : 0.f;
+      tile_dD = fmaf(rate[2], rate[3], tile_dD);
+      tile_dbias += dt_out;
+      const unsigned off = lane_out + (unsigned)q * 4u * (unsigned)p.W * (unsigned)sizeof(IO);
+      BufIo<IO>::store((IO)du, SelStream<IO>::tile(p.du, place, (unsigned)p.W, left), off, 0);
+      BufIo<IO>::store((IO)dt_out, SelStream<IO>::tile(p.ddt, place, (unsigned)p.W, left), off, 0);
+      if (gated) BufIo<IO>::store((IO)(live ? gate[1] * fmaf(skip, rate[3], y_all ? *y_all : gate[2]) : 0.f), SelStream<IO>::tile(p.dz, place, (unsigned)p.W, left), off, 0);
+    };
     sel_each<4>([&](auto back) {
       constexpr int g4 = 3 - decltype(back)::value;
       float dB[4][4], dC[4][4], sum_b[4], sum_a[4];
+      f32x4 front;
+      if constexpr (g4 == 0) front = fronts[wave][lane];
       sel_each<4>([&](auto token) {
         constexpr int k = 3 - decltype(token)::value, t = 4 * g4 + k;
         const f32x4 rate = rates[wave][t][c];
         float sb = 0.f, sa = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float dh = fmaf(row_bcast<t>(C[i]), rate[2], carry[i]);
+          const float dh = row_bcast<t>(C[i]) * rate[2] + carry[i];
           dC[k][i] = rate[2] * h[t][i];
           dB[k][i] = rate[1] * dh;
-          sb = fmaf(row_bcast<t>(B[i]), dh, sb);
-          float old = t ? h[t ? t - 1 : 0][i] : before[i];
+          sb = i ? sb + row_bcast<t>(B[i]) * dh : row_bcast<t>(B[i]) * dh;
           carry[i] = a[t][i] * dh;
+          float q = carry[i] * (t ? h[t ? t - 1 : 0][i] : front[i]);
           if constexpr (MASKED) {
             const bool cut = (m.starts >> t) & 1u;
-            old = cut ? 0.f : old;
+            q = cut ? 0.f : q;
             carry[i] = cut ? 0.f : carry[i];
           }
-          const float q = carry[i] * old;
-          sa = fmaf(a2[i], q, sa);
+          sa = i ? fmaf(a2[i], q, sa) : a2[i] * q;
           tile_dA[i] = fmaf(rate[0], q, tile_dA[i]);
         }
         sum_b[k] = sb;
         sum_a[k] = sa;
       });
-      along[g4] = four_rows_sum(sum_b);
-      through[g4] = four_rows_sum(sum_a);
+      const float along = four_rows_sum(sum_b), through = four_rows_sum(sum_a);
       vectors[tile & 1][0][wave][g4][lane] = lanes_scatter_sum(dB, lane);
       vectors[tile & 1][1][wave][g4][lane] = lanes_scatter_sum(dC, lane);
+      if constexpr (SLABS == 1) {
+        finish(g4, along, through, nullptr);
+      } else {
+        float (*mem)[4][64] = parts[tile & 1][wave];
+        mem[0][g4][lane] = along; mem[1][g4][lane] = through; mem[2][g4][lane] = gates[wave][4 * g4 + j][c][2];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (g4 == 2 && tile > first) request(tile - 1);        // half of the decays and states are through: their registers are free
     });
-    if constexpr (SLABS > 1) {
-      float (*mem)[3][4][64] = parts[tile & 1];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) { mem[wave][0][q][lane] = along[q]; mem[wave][1][q][lane] = through[q]; mem[wave][2][q][lane] = y[q]; }
-    }
     __syncthreads();                                        // the other buffer's readers are past the barrier before
     if constexpr (SLABS > 1) {
       float (*mem)[3][4][64] = parts[tile & 1];
@@ -211,52 +237,36 @@ template <typename IO, int SLABS, bool MASKED> __global__ __launch_bounds__(kSel
         for (int k = 0; k < SLABS; ++k)
 #pragma unroll
           for (int e = 0; e < 3; ++e) x[e] += mem[head + k][e][q][lane];
-        along[q] = x[0]; through[q] = x[1]; y[q] = x[2];
+        finish(q, x[0], x[1], &x[2]);
       }
     }
     // dB and dC of the workgroup's channels: thread (slab, group of tokens, lane as lanes_scatter_sum leaves it)
-    for (int idx = threadIdx.x; idx < 2 * SLABS * 256; idx += kSelThreads) {
-      const int which = idx / (SLABS * 256), slab = idx / 256 % SLABS, q = idx / 64 % 4, l = idx & 63;
-      const int t = 4 * q + 2 * ((l >> 3) & 1) + ((l >> 2) & 1), n = slab * kSelStates + 4 * (l >> 4) + (l & 3);
-      float sum = 0.f;
 #pragma unroll
-      for (int k = slab; k < kSelWaves; k += SLABS) sum += vectors[tile & 1][which][k][q][l];
-      if (t < left && n < p.N) {
-        float* out = (which ? p.dC : p.dB) + ((((long long)at.set * p.B + at.b) * p.T + t0 + t) * p.G + at.g) * p.N + n;
-        *out = (m.live >> t) & 1u ? sum : 0.f;
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int slab = 0; slab < SLABS; ++slab) {
+        const int t = 4 * wave + 2 * ((lane >> 3) & 1) + ((lane >> 2) & 1), n = slab * kSelStates + 4 * (lane >> 4) + (lane & 3);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = slab; k < kSelWaves; k += SLABS) sum += vectors[tile & 1][which][k][wave][lane];
+        const long long row = (((long long)at.set * p.B + at.b) * p.T + t0) * p.G;
+        const rsrc_t r = make_rsrc((which ? p.dC : p.dB) + row * p.N, (unsigned)left * (unsigned)p.G * (unsigned)p.N * 4u);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, (m.live >> t) & 1u ? sum : 0.f), r,
+                                              n < p.N ? (((unsigned)t * (unsigned)p.G + (unsigned)at.g) * (unsigned)p.N + (unsigned)n) * 4u : kOutOfRange, 0, 0);
       }
-    }
-    float du[4], ddt[4], dz[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float ds = fmaf(u[q], along[q], through[q] * kLn2);
-      const bool live = (m.live >> (4 * q + j)) & 1u;
-      ddt[q] = live ? ds * slope[q] : 0.f;
-      du[q] = live ? fmaf(s[q], along[q], skip * dy[q]) : 0.f;
-      tile_dD = fmaf(dy[q], u[q], tile_dD);
-      tile_dbias += ddt[q];
-      if (gated) {
-        const float sig = sigmoid_fast(z[q]);
-        dz[q] = live ? d[q] * fmaf(skip, u[q], y[q]) * sig * fmaf(z[q], 1.f - sig, 1.f) : 0.f;
-      }
-    }
-    dD += tile_dD;
-    dbias += tile_dbias;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dA[i] += tile_dA[i];
-    if (SLABS == 1 || at.slab == 0) {
-      const long long place = ((long long)at.b * p.T + t0) * p.W;
-      sel_store<IO>(du, p.du, place, (unsigned)p.W, w, left, ok, j);
-      sel_store<IO>(ddt, p.ddt, place, (unsigned)p.W, w, left, ok, j);
-      if (gated) sel_store<IO>(dz, p.dz, place, (unsigned)p.W, w, left, ok, j);
-    }
+    sum_dA[wave][lane] += (f32x4){tile_dA[0], tile_dA[1], tile_dA[2], tile_dA[3]};
+    const float2 rows = sum_rows[wave][lane];
+    sum_rows[wave][lane] = make_float2(rows.x + tile_dD, rows.y + tile_dbias);
   }
+  const f32x4 all_dA = sum_dA[wave][lane];
+  const float dA[4] = {all_dA[0], all_dA[1], all_dA[2], all_dA[3]};
+  float dD = sum_rows[wave][lane].x, dbias = sum_rows[wave][lane].y;
   const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
-  sel_store_states(p.dA, row, n0, p.N, ok, dA);
+  sel_store_states(p.dA, row, n0, p.N, ok, WHOLE, dA);
   dD = all_rows_sum(dD);
   dbias = all_rows_sum(dbias);
   if (ok && j == 0 && at.slab == 0) { p.dD[row] = dD; p.dbias[row] = dbias; }
-  if (at.seg == 0 && p.dh0) sel_store_states(p.dh0, (long long)at.b * p.W + w, n0, p.N, ok, carry);
+  if (at.seg == 0 && p.dh0) sel_store_states(p.dh0, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, carry);
 }
 
 // The sums of all partial gradients in one launch.
@@ -271,16 +281,20 @@ static __global__ __launch_bounds__(256) void sel_sums_kernel(SelSums jobs) {
   run_sum_job(jobs.job[i], (int)blockIdx.x - jobs.first[i], red);
 }
 
-template <typename IO, int SLABS, bool MASKED> static void sel_backward_masked(const SelArgs& a, hipStream_t s) {
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_backward_whole(const SelArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * (long long)a.S * a.G * a.per_group)), block(kSelThreads);
-  if (a.S > 1) hipLaunchKernelGGL((sel_reverse_kernel<IO, SLABS, MASKED>), grid, block, 0, s, a);
-  hipLaunchKernelGGL((sel_backward_kernel<IO, SLABS, MASKED>), grid, block, 0, s, a);
+  if (a.S > 1) hipLaunchKernelGGL((sel_reverse_kernel<IO, SLABS, MASKED, WHOLE>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((sel_backward_kernel<IO, SLABS, MASKED, WHOLE>), grid, block, 0, s, a);
+}
+template <typename IO, int SLABS> static void sel_backward_slabs(const SelArgs& a, hipStream_t s) {
+  if (a.flags) { if (a.whole) sel_backward_whole<IO, SLABS, true, true>(a, s); else sel_backward_whole<IO, SLABS, true, false>(a, s); }
+  else { if (a.whole) sel_backward_whole<IO, SLABS, false, true>(a, s); else sel_backward_whole<IO, SLABS, false, false>(a, s); }
 }
 template <typename IO> static void sel_backward_typed(const SelArgs& a, hipStream_t s) {
   const int slabs = (a.N + kSelStates - 1) / kSelStates;
-  if (slabs == 1) { if (a.flags) sel_backward_masked<IO, 1, true>(a, s); else sel_backward_masked<IO, 1, false>(a, s); }
-  else if (slabs == 2) { if (a.flags) sel_backward_masked<IO, 2, true>(a, s); else sel_backward_masked<IO, 2, false>(a, s); }
-  else { if (a.flags) sel_backward_masked<IO, 4, true>(a, s); else sel_backward_masked<IO, 4, false>(a, s); }
+  if (slabs == 1) sel_backward_slabs<IO, 1>(a, s);
+  else if (slabs == 2) sel_backward_slabs<IO, 2>(a, s);
+  else sel_backward_slabs<IO, 4>(a, s);
 }
 
 int sel_launch_backward(const SelArgs& a, void* dB, void* dC, float* dA, float* dD, float* dbias, int dtype, hipStream_t s) {

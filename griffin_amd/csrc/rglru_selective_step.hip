@@ -15,7 +15,7 @@ struct SelStepArgs {
   float* state;
   void* y;
   long long su, sdt, sz, sBb, sBg, sCb, sCg;
-  int B, W, N, Wg, lanes, softplus;
+  int B, W, N, Wg, lanes, softplus, whole;
 };
 
 // Four states a lane, N / 4 lanes (a power of two) a channel: the state is read and written once, in whole vectors, one behind the other.
@@ -29,8 +29,8 @@ template <typename IO> __global__ __launch_bounds__(kSelThreads) void sel_step_k
   const bool live = !(flag & 2u);
   const long long row = (long long)b * p.W + w;
   float a[4], h[4], y = 0.f;
-  sel_load_states(p.state, row, n0, p.N, there && flag == 0u, h);
-  sel_load_states(p.A, w, n0, p.N, there, a);
+  sel_load_states(p.state, row, n0, p.N, there && flag == 0u, p.whole, h);
+  sel_load_states(p.A, w, n0, p.N, there, p.whole, a);
   const float u = (float)((const IO*)p.u)[b * p.su + w];
   const float s = sel_rate((float)((const IO*)p.dt)[b * p.sdt + w] + (p.bias ? p.bias[w] : 0.f), p.softplus).s, su = s * u;
 #pragma unroll
@@ -43,7 +43,7 @@ template <typename IO> __global__ __launch_bounds__(kSelThreads) void sel_step_k
   }
   for (int m = 1; m < p.lanes; m <<= 1) y += __shfl_xor(y, m, 64);
   if (!there) return;
-  if (live) sel_store_states(p.state, row, n0, p.N, true, h);
+  if (live) sel_store_states(p.state, row, n0, p.N, true, p.whole, h);
   if (l == 0) {
     if (p.D) y = fmaf(p.D[w], u, y);
     if (p.z) {
@@ -56,39 +56,53 @@ template <typename IO> __global__ __launch_bounds__(kSelThreads) void sel_step_k
 
 static size_t sel_bytes(long long floats) { return ((size_t)floats * 4 + 255) & ~(size_t)255; }
 
-// Segments of a sequence.  One workgroup a compute unit leaves each SIMD one wave, which issues at half the rate that two reach; but a sequence in
-// segments is walked twice.
-static int sel_segments(int64_t B, int64_t G, int64_t per_group, int64_t tiles) {
-  const long long wgs = B * G * per_group, units = num_compute_units();
-  if (wgs >= units) return 1;
-  long long s = 2 * units / wgs;
-  if (s > tiles / 4) s = tiles / 4;
-  if (s > kSelMaxSegments) s = kSelMaxSegments;
-  if (s < 2) return 1;
-  const long long each = (tiles + s - 1) / s;
-  return (int)((tiles + each - 1) / each);
+// Segments of a sequence, by a time estimate.  A compute unit holds two workgroups at a time; one alone leaves each SIMD one wave, which issues an
+// instruction in 5.3 cycles where two take 6.2 for one each.  Walking in segments adds `again` of the work in all segments but one.
+static int sel_segments(long long wgs, long long tiles, double again) {
+  const long long units = num_compute_units();
+  int best = 1;
+  double least = 0.;
+  for (long long s = 1; s <= kSelMaxSegments && (s == 1 || s <= tiles / 4); ++s) {
+    const long long each = (tiles + s - 1) / s;
+    if ((tiles + each - 1) / each != s) continue;            // the same segments as fewer
+    const long long all = wgs * s, full = all / (2 * units), rest = all - full * 2 * units;
+    const double rounds = 6.2 * (double)full + (rest > units ? 6.2 : rest > 0 ? 5.3 : 0.), time = rounds * (double)each * (1. + again * (double)(s - 1) / (double)s);
+    if (s == 1 || time < 0.97 * least) { best = (int)s; least = time; }
+  }
+  return best;
 }
 
-static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N) {
-  if (B <= 0 || T <= 0 || W <= 0 || G <= 0 || N <= 0 || W % G || N > kSelMaxStates || W >= (1 << 22) || T >= (1ll << 31) - 64 || B >= (1ll << 31)) return false;
+static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, bool backward) {
+  if (B <= 0 || T <= 0 || W <= 0 || G <= 0 || N <= 0 || W % G || N > kSelMaxStates || W >= (1 << 22) || T >= (1ll << 31) - 64 || B >= (1ll << 24)) return false;
   const int slabs = N <= 16 ? 1 : N <= 32 ? 2 : 4;
+  const long long columns = ((W / G) + kSelLanes - 1) / kSelLanes;
   a->B = (int)B; a->T = (int)T; a->W = (int)W; a->N = (int)N; a->G = (int)G; a->Wg = (int)(W / G);
-  a->per_group = (int)((((W / G) + kSelLanes - 1) / kSelLanes * slabs + kSelWaves - 1) / kSelWaves);
+  a->per_group = (int)((columns * slabs + kSelWaves - 1) / kSelWaves);
+  a->pipe_group = slabs > 1 ? a->per_group : (int)((columns * kSelPipe + kSelWaves - 1) / kSelWaves);
   a->tiles = (int)((T + kSelTile - 1) / kSelTile);
-  if (B * G * a->per_group >= (1ll << 24)) return false;
-  a->S = sel_segments(B, G, a->per_group, a->tiles);
+  const long long wgs = B * G * (backward ? a->per_group : a->pipe_group);
+  if (wgs >= (1ll << 24) || (long long)G * N >= (1ll << 22)) return false;
+  // a summary's share of a walk's instructions
+  a->S = sel_segments(wgs, a->tiles, backward ? 0.27 : 0.6);
   a->seg_tiles = (a->tiles + a->S - 1) / a->S;
-  return B * (long long)a->S * G * a->per_group < (1ll << 24);
+  return wgs * a->S < (1ll << 24);
 }
 
-static int sel_check(const char* who, SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype) {
+static int sel_check(const char* who, SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype, bool backward) {
   if (dtype != RGLRU_F32 && dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: dtype must be RGLRU_F32 or RGLRU_BF16, got %d", who, dtype);
   if (B <= 0 || T <= 0 || W <= 0 || G <= 0 || N <= 0 || W % G)
     return fail(RGLRU_E_ARG, "%s: sizes B=%lld T=%lld W=%lld G=%lld N=%lld", who, (long long)B, (long long)T, (long long)W, (long long)G, (long long)N);
   if (N > kSelMaxStates) return fail(RGLRU_E_UNSUPPORTED, "%s: %lld states a channel exceed the supported %d", who, (long long)N, kSelMaxStates);
   memset(a, 0, sizeof(*a));
-  if (!sel_plan(a, B, T, W, G, N)) return fail(RGLRU_E_UNSUPPORTED, "%s: tensor too large", who);
+  if (!sel_plan(a, B, T, W, G, N, backward)) return fail(RGLRU_E_UNSUPPORTED, "%s: tensor too large", who);
   return RGLRU_OK;
+}
+
+// Whether rows of N states are whole vectors on 16-byte boundaries.
+static bool sel_whole(int64_t N, std::initializer_list<const void*> tensors) {
+  bool whole = N % 4 == 0;
+  for (const void* t : tensors) whole = whole && (uintptr_t)t % 16 == 0;
+  return whole;
 }
 
 // Distances between batch rows, tokens and groups: of u, dt, z (two each), B, C (three each).
@@ -98,10 +112,10 @@ static int sel_strides(const char* who, SelArgs* a, const int64_t* s, int dtype)
     if (t < 0 || t >= (1 << 22)) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens %lld elements apart", who, (long long)t);
   a->sub = s[0]; a->sut = s[1]; a->sdb = s[2]; a->sdt = s[3]; a->szb = s[4]; a->szt = s[5];
   a->sBb = s[6]; a->sBt = s[7]; a->sBg = s[8]; a->sCb = s[9]; a->sCt = s[10]; a->sCg = s[11];
-  bool whole = a->N % 4 == 0;
+  bool whole = true;
   for (int i = 6; i < 12; ++i) whole = whole && s[i] % 4 == 0;
   const uintptr_t boundary = dtype == RGLRU_BF16 ? 8 : 16;
-  a->vector = whole && (uintptr_t)a->Bm % boundary == 0 && (uintptr_t)a->Cm % boundary == 0;
+  a->whole = whole && (uintptr_t)a->Bm % boundary == 0 && (uintptr_t)a->Cm % boundary == 0;
   return RGLRU_OK;
 }
 
@@ -115,7 +129,7 @@ int rglru_hip_selective_max_states(void) { return kSelMaxStates; }
 
 size_t rglru_hip_selective_workspace_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int keep) {
   SelArgs a;
-  if (!sel_plan(&a, B, T, W, G, N)) return 0;
+  if (!sel_plan(&a, B, T, W, G, N, false)) return 0;
   size_t n = keep ? sel_bytes((long long)B * a.tiles * W * N) : 0;
   if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
   return n + 256;
@@ -123,7 +137,7 @@ size_t rglru_hip_selective_workspace_bytes(int64_t B, int64_t T, int64_t W, int6
 
 size_t rglru_hip_selective_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_t G, int64_t N) {
   SelArgs a;
-  if (!sel_plan(&a, B, T, W, G, N)) return 0;
+  if (!sel_plan(&a, B, T, W, G, N, true)) return 0;
   size_t n = 2 * sel_bytes((long long)a.per_group * B * T * G * N) + sel_bytes((long long)B * a.S * W * N) + 2 * sel_bytes((long long)B * a.S * W);
   if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
   return n;
@@ -133,7 +147,7 @@ int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const 
                             const float* D, const float* bias, const float* h0, const uint8_t* flags, void* y, float* h_last, void* ws, int keep,
                             int softplus, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream) {
   SelArgs a;
-  int rc = sel_check("selective_fwd", &a, B, T, W, G, N, dtype);
+  int rc = sel_check("selective_fwd", &a, B, T, W, G, N, dtype, false);
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !y || !h_last || !ws) return fail(RGLRU_E_ARG, "selective_fwd: null pointer");
   a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.A = A; a.D = D; a.bias = bias; a.h0 = h0; a.flags = flags; a.y = y; a.h_last = h_last;
@@ -143,6 +157,7 @@ int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const 
   char* at = (char*)ws;
   if (keep) { a.kept = (float*)at; at += sel_bytes((long long)B * a.tiles * W * N); }
   if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + sel_bytes((long long)B * a.S * W * N)); }
+  a.whole = a.whole && sel_whole(N, {A, h0, h_last, ws});
   return sel_launch_forward(a, dtype, (hipStream_t)stream);
 }
 
@@ -151,7 +166,7 @@ int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const 
                             void* du, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* dbias, float* dh0, int softplus, int64_t B,
                             int64_t T, int64_t W, int64_t G, int64_t N, int dtype, void* stream) {
   SelArgs a;
-  int rc = sel_check("selective_bwd", &a, B, T, W, G, N, dtype);
+  int rc = sel_check("selective_bwd", &a, B, T, W, G, N, dtype, true);
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !dout || !ws || !scratch || !du || !ddt || (z && !dz) || !dB || !dC)
     return fail(RGLRU_E_ARG, "selective_bwd: null pointer");
@@ -168,6 +183,7 @@ int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const 
   a.dD = (float*)at; at += rows;
   a.dbias = (float*)at; at += rows;
   if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + states); }
+  a.whole = a.whole && sel_whole(N, {A, dh_last, dh0, ws, scratch});
   return sel_launch_backward(a, dB, dC, dA, dD, dbias, dtype, (hipStream_t)stream);
 }
 
@@ -175,7 +191,7 @@ int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const
                              const float* D, const float* bias, const uint8_t* flags, float* state, void* y, int softplus, int64_t B, int64_t W, int64_t G,
                              int64_t N, int dtype, void* stream) {
   SelArgs a;
-  int rc = sel_check("selective_step", &a, B, 1, W, G, N, dtype);
+  int rc = sel_check("selective_step", &a, B, 1, W, G, N, dtype, false);
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !state || !y) return fail(RGLRU_E_ARG, "selective_step: null pointer");
   SelStepArgs p;
@@ -184,6 +200,7 @@ int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const
   p.su = strides[0]; p.sdt = strides[1]; p.sz = strides[2]; p.sBb = strides[3]; p.sBg = strides[4]; p.sCb = strides[5]; p.sCg = strides[6];
   p.B = (int)B; p.W = (int)W; p.N = (int)N; p.Wg = (int)(W / G); p.softplus = softplus;
   p.lanes = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
+  p.whole = sel_whole(N, {A, state});
   const long long blocks = (B * W * p.lanes + kSelThreads - 1) / kSelThreads;
   if (blocks >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "selective_step: tensor too large");
   const dim3 grid((unsigned)blocks), block(kSelThreads);
