@@ -38,14 +38,14 @@ struct SelArgs {
   void *y, *du, *ddt, *dz;
   float *h_last, *dh0;
   float* kept;                                // [B][tiles][W][N]: states in front of tiles, or null
-  float* ends;                                // [B][S][W][N]: what a segment leaves of a state (a gradient) of zeros
-  float* sums;                                // [B][S][W][2]: a segment's sum of step sizes; whether a document starts in it
+  float* ends;                                // [B][S * parts][W][N]: what a part of a segment leaves of a state (a gradient) of zeros
+  float* sums;                                // [B][S * parts][W][2]: its sum of step sizes; whether a document starts in it
   float *dB, *dC;                             // [sets][B][T][G][N], a set for each workgroup of a group
   float *dA, *dD, *dbias;                     // [B][S][W][N], [B][S][W]
   long long sub, sut, sdb, sdt, szb, szt, sBb, sBt, sBg, sCb, sCt, sCg;  // elements between batch rows, tokens and groups
   int B, T, W, N, G, Wg;                      // Wg: channels of a group
   int per_group, pipe_group;                  // workgroups of a group's channels: one wave, or kSelPipe waves to 16 of them (and states)
-  int S, tiles, seg_tiles;                    // segments, tiles of a sequence and of a segment (of the pass)
+  int S, tiles, seg_tiles, parts;             // segments, tiles of a sequence and of a segment, parts that a segment is summarised in
   int softplus, whole;                        // whole: rows of B, C and the states are whole vectors of four elements
 };
 
@@ -59,13 +59,13 @@ RGLRU_DEVICE unsigned sel_block() {
   return i < whole ? i % 8 * (n / 8) + i / 8 : i;
 }
 // SLABS waves of a workgroup share channels, by their states; PIPE teams of them, by tiles in turn.
-template <int SLABS, int PIPE> RGLRU_DEVICE SelPlace sel_place(const SelArgs& p) {
+template <int SLABS, int PIPE> RGLRU_DEVICE SelPlace sel_place(const SelArgs& p, int segments) {
   SelPlace r;
   unsigned i = sel_block();
   r.set = (int)(i % (unsigned)p.per_group); i /= (unsigned)p.per_group;
   r.g = (int)(i % (unsigned)p.G); i /= (unsigned)p.G;
-  r.seg = (int)(i % (unsigned)p.S);
-  r.b = (int)(i / (unsigned)p.S);
+  r.seg = (int)(i % (unsigned)segments);
+  r.b = (int)(i / (unsigned)segments);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   r.slab = wave % SLABS;
   r.turn = wave / SLABS % PIPE;
@@ -78,6 +78,23 @@ template <int CONTROL> RGLRU_DEVICE float sel_move(float v) {
 }
 // Lane K of every row of 16 lanes, for the whole row.
 template <int K> RGLRU_DEVICE float row_bcast(float v) { return sel_move<0x150 + K>(v); }
+
+// Multiply-adds whose factor is lane T of the row, which the compiler leaves as a move and a multiply-add: v[i] of that lane times x (times x[i], summed up).
+// A lane's register read by another lane has to be two wait states old; the first instruction waits for them, as nothing else would inside an asm block.
+#define RGLRU_BCAST " row_newbcast:%9 row_mask:0xf bank_mask:0xf\n\t"
+template <int T> RGLRU_DEVICE float bcast_dot(const float (&v)[4], const float (&x)[4]) {
+  float r;
+  asm("s_nop 1\n\t"
+      "v_mul_f32_dpp %0, %1, %5" RGLRU_BCAST "v_fmac_f32_dpp %0, %2, %6" RGLRU_BCAST "v_fmac_f32_dpp %0, %3, %7" RGLRU_BCAST "v_fmac_f32_dpp %0, %4, %8" RGLRU_BCAST
+      : "=&v"(r) : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(T));
+  return r;
+}
+template <int T> RGLRU_DEVICE void bcast_fma(float (&sum)[4], const float (&v)[4], float x) {
+  asm("s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %4, %8" RGLRU_BCAST "v_fmac_f32_dpp %1, %5, %8" RGLRU_BCAST "v_fmac_f32_dpp %2, %6, %8" RGLRU_BCAST "v_fmac_f32_dpp %3, %7, %8" RGLRU_BCAST
+      : "+v"(sum[0]), "+v"(sum[1]), "+v"(sum[2]), "+v"(sum[3]) : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(x), "n"(T));
+}
+#undef RGLRU_BCAST
 
 // a's two lower rows beside b's two lower rows, and the upper ones: the sum of the two holds a's sum over row pairs in the lower half, b's in the upper.
 RGLRU_DEVICE float halves_sum(float a, float b) {
@@ -95,21 +112,32 @@ RGLRU_DEVICE float all_rows_sum(float v) {
   return rows_sum(h, h);
 }
 
+// Lanes that lie `move` apart exchange: those in the banks of MASK (four lanes of a row each) receive b's sum of the two, the others a's.  The second
+// addition writes those banks only, which saves the selections.  As above, the sources have to be two wait states old.
+#define RGLRU_PAIR(R, A, B, MOVE, MASK) \
+  "v_add_f32_dpp " R ", " A ", " A " " MOVE " row_mask:0xf bank_mask:0xf\n\tv_add_f32_dpp " R ", " B ", " B " " MOVE " row_mask:0xf bank_mask:" MASK "\n\t"
+
 // Sums over the 16 lanes of a row of v[token][i]: lane 8 t1 + 4 t0 + 2 i1 + i0 of a row receives that of v[2 t1 + t0][2 i1 + i0].  Each step sends half of
 // what a lane holds to the lane that keeps it.
 RGLRU_DEVICE float lanes_scatter_sum(const float (&v)[4][4], int lane) {
-  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+  const bool b1 = lane & 2, b0 = lane & 1;
   float r[2][4], q[4], s[2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[t][i] = (b3 ? v[2 + t][i] : v[t][i]) + sel_move<0x128>(b3 ? v[t][i] : v[2 + t][i]);   // eight lanes on
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = (b2 ? r[1][i] : r[0][i]) + sel_move<0x141>(b2 ? r[0][i] : r[1][i]);                // eight lanes mirrored
+  for (int t = 0; t < 2; ++t)                                // eight lanes on
+    asm("s_nop 1\n\t" RGLRU_PAIR("%0", "%4", "%8", "row_ror:8", "0xc") RGLRU_PAIR("%1", "%5", "%9", "row_ror:8", "0xc")
+            RGLRU_PAIR("%2", "%6", "%10", "row_ror:8", "0xc") RGLRU_PAIR("%3", "%7", "%11", "row_ror:8", "0xc")
+        : "=&v"(r[t][0]), "=&v"(r[t][1]), "=&v"(r[t][2]), "=&v"(r[t][3])
+        : "v"(v[t][0]), "v"(v[t][1]), "v"(v[t][2]), "v"(v[t][3]), "v"(v[2 + t][0]), "v"(v[2 + t][1]), "v"(v[2 + t][2]), "v"(v[2 + t][3]));
+  // eight lanes mirrored
+  asm("s_nop 1\n\t" RGLRU_PAIR("%0", "%4", "%8", "row_half_mirror", "0xa") RGLRU_PAIR("%1", "%5", "%9", "row_half_mirror", "0xa")
+          RGLRU_PAIR("%2", "%6", "%10", "row_half_mirror", "0xa") RGLRU_PAIR("%3", "%7", "%11", "row_half_mirror", "0xa")
+      : "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+      : "v"(r[0][0]), "v"(r[0][1]), "v"(r[0][2]), "v"(r[0][3]), "v"(r[1][0]), "v"(r[1][1]), "v"(r[1][2]), "v"(r[1][3]));
 #pragma unroll
   for (int i = 0; i < 2; ++i) s[i] = (b1 ? q[2 + i] : q[i]) + sel_move<0x4e>(b1 ? q[i] : q[2 + i]);
   return (b0 ? s[1] : s[0]) + sel_move<0xb1>(b0 ? s[0] : s[1]);
 }
+#undef RGLRU_PAIR
 
 // Writes of some lanes of a wave before reads of others: LDS serves a wave in order, so only the compiler has to keep it.
 RGLRU_DEVICE void wave_order() {
@@ -276,19 +304,36 @@ template <bool MASKED> RGLRU_DEVICE SelMasks sel_masks(const unsigned char* flag
 template <typename F, int... K> RGLRU_DEVICE void sel_each(F&& f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
 template <int N, typename F> RGLRU_DEVICE void sel_each(F&& f) { sel_each(f, std::make_integer_sequence<int, N>{}); }
 
-// What the segments in front (behind, for gradients) of this one leave of the state that enters the first (last) of them: a few dozen at most, each
-// multiplies by exp(A sum) unless a document starts in it.
-template <bool REVERSE> RGLRU_DEVICE void sel_join(const SelArgs& p, const SelPlace& at, int w, int n0, bool ok, const float (&a2)[4], float (&h)[4]) {
-  const int count = REVERSE ? p.S - 1 - at.seg : at.seg;
-  for (int r = 0; r < count; ++r) {
-    const long long row = ((long long)at.b * p.S + (REVERSE ? p.S - 1 - r : r)) * p.W + w;
-    float e[4];
-    sel_load_states(p.ends, row, n0, p.N, ok, p.whole, e);
-    const float sum = ok ? p.sums[2 * row] : 0.f;
-    const bool cut = ok && p.sums[2 * row + 1] != 0.f;
+// What the parts of the sequence in front of this segment (behind it, for gradients) leave of the state that enters the first (last) of them: each
+// multiplies by exp(A sum) unless a document starts in it.  Four parts are asked for at a time.
+template <bool REVERSE, bool WHOLE> RGLRU_DEVICE void sel_join(const SelArgs& p, const SelPlace& at, int w, int n0, bool ok, const float (&a2)[4], float (&h)[4]) {
+  const int all = p.S * p.parts, count = (REVERSE ? p.S - 1 - at.seg : at.seg) * p.parts;
+  for (int r0 = 0; r0 < count; r0 += 4) {
+    float e[4][4], sum[4], cut[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = cut ? e[i] : fmaf(__builtin_amdgcn_exp2f(a2[i] * sum), h[i], e[i]);
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k < count ? r0 + k : count - 1;
+      const long long row = ((long long)at.b * all + (REVERSE ? all - 1 - r : r)) * p.W + w;
+      sel_load_states(p.ends, row, n0, p.N, ok, WHOLE, e[k]);
+      sum[k] = p.sums[2 * row];
+      cut[k] = p.sums[2 * row + 1];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (r0 + k < count) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = cut[k] != 0.f ? e[k][i] : fmaf(__builtin_amdgcn_exp2f(a2[i] * sum[k]), h[i], e[k][i]);
+      }
   }
+}
+// The tiles of part r of a segment that ends with tile `last`: some of the last parts may be empty.
+struct SelPart { int first, last; };
+RGLRU_DEVICE SelPart sel_part(const SelArgs& p, int seg, int r) {
+  const int begin = seg * p.seg_tiles, end = begin + p.seg_tiles < p.tiles ? begin + p.seg_tiles : p.tiles, each = (p.seg_tiles + p.parts - 1) / p.parts;
+  SelPart t;
+  t.first = begin + r * each < end ? begin + r * each : end;
+  t.last = t.first + each < end ? t.first + each : end;
+  return t;
 }
 
 int sel_launch_forward(const SelArgs& a, int dtype, hipStream_t s);

@@ -8,16 +8,18 @@
 
 namespace rglru {
 
-// What a segment leaves of a state of zeros, and its sum of step sizes.
+// What a part of a segment leaves of a state of zeros, and its sum of step sizes.
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_summary_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
-  const SelPlace at = sel_place<SLABS, 1>(p);
-  if (at.seg == p.S - 1) return;                            // nothing asks what the last one leaves
+  const SelPlace at = sel_place<SLABS, 1>(p, p.S * p.parts);
+  const int seg = at.seg / p.parts;
+  if (seg == p.S - 1) return;                               // nothing asks what the last one leaves
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
   const int w = at.g * p.Wg + (ok ? in_group : 0);
-  const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
+  const SelPart part = sel_part(p, seg, at.seg % p.parts);
+  const int first = part.first, last = part.last;
   float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
   sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
 #pragma unroll
@@ -33,7 +35,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
     next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
   };
-  request(first);
+  if (first < last) request(first);
   float total = 0.f;
   bool cut = false;
   for (int tile = first; tile < last; ++tile) {
@@ -62,7 +64,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     });
     wave_order();                                           // the next tile's rates come after these reads
   }
-  const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
+  const long long row = ((long long)at.b * p.S * p.parts + at.seg) * p.W + w;
   sel_store_states(p.ends, row, n0, p.N, ok, WHOLE, h);
   total = all_rows_sum(total);
   if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
@@ -78,7 +80,7 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
   __shared__ int ready[kSelWaves];                           // that tile
   __shared__ float parts[SLABS > 1 ? 2 : 1][SLABS > 1 ? kSelWaves : 1][4][64];
   static_assert(TEAMS * SLABS * PIPE == kSelWaves && (SLABS == 1 || PIPE == 1), "waves of a workgroup");
-  const SelPlace at = sel_place<SLABS, PIPE>(p);
+  const SelPlace at = sel_place<SLABS, PIPE>(p, p.S);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
@@ -95,7 +97,7 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
   const float bias = ok && p.bias ? p.bias[w] : 0.f, skip = ok && p.D ? p.D[w] : 0.f;
   if (at.turn == 0) {
     if (p.h0) sel_load_states(p.h0, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
-    sel_join<false>(p, at, w, n0, ok, a2, h);
+    sel_join<false, WHOLE>(p, at, w, n0, ok, a2, h);
   }
   const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
   const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
@@ -178,10 +180,7 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
       float sums[4];
       sel_each<4>([&](auto token) {
         constexpr int t = 4 * decltype(group)::value + decltype(token)::value;
-        float sum = row_bcast<t>(C[0]) * x[t][0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i) sum += row_bcast<t>(C[i]) * x[t][i];
-        sums[decltype(token)::value] = sum;
+        sums[decltype(token)::value] = bcast_dot<t>(C, x[t]);
       });
       y[decltype(group)::value] = four_rows_sum(sums);
     });
@@ -210,7 +209,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_forwa
   constexpr int PIPE = SLABS == 1 ? kSelPipe : 1;
   const dim3 block(kSelThreads);
   if (a.S > 1)
-    hipLaunchKernelGGL((sel_summary_kernel<IO, SLABS, MASKED, WHOLE>), dim3((unsigned)(a.B * (long long)a.S * a.G * a.per_group)), block, 0, s, a);
+    hipLaunchKernelGGL((sel_summary_kernel<IO, SLABS, MASKED, WHOLE>), dim3((unsigned)(a.B * (long long)a.S * a.parts * a.G * a.per_group)), block, 0, s, a);
   SelArgs f = a;
   f.per_group = PIPE > 1 ? a.pipe_group : a.per_group;
   hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, PIPE, MASKED, WHOLE>), dim3((unsigned)(f.B * (long long)f.S * f.G * f.per_group)), block, 0, s, f);

@@ -17,17 +17,19 @@
 
 namespace rglru {
 
-// What a segment hands back of a gradient of zeros at its last state.  (Its sums of step sizes and document starts are made again here: the forward
+// What a part of a segment hands back of a gradient of zeros at its last state.  (Its sums of step sizes and document starts are made again here: the forward
 // pass keeps them only until its own join.)
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_reverse_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
-  const SelPlace at = sel_place<SLABS, 1>(p);
-  if (at.seg == 0) return;
+  const SelPlace at = sel_place<SLABS, 1>(p, p.S * p.parts);
+  const int seg = at.seg / p.parts;
+  if (seg == 0) return;                                     // nothing asks what the first one hands back
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
   const int w = at.g * p.Wg + (ok ? in_group : 0);
-  const int first = at.seg * p.seg_tiles, last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
+  const SelPart part = sel_part(p, seg, at.seg % p.parts);
+  const int first = part.first, last = part.last;
   float a2[4], carry[4] = {0.f, 0.f, 0.f, 0.f};
   sel_load_states(p.A, w, n0, p.N, ok, WHOLE, a2);
 #pragma unroll
@@ -46,7 +48,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
     next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
   };
-  request(last - 1);
+  if (first < last) request(last - 1);
   float total = 0.f;
   bool cut = false;
   for (int tile = last - 1; tile >= first; --tile) {
@@ -70,14 +72,15 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     sel_each<kSelTile>([&](auto token) {
       constexpr int t = kSelTile - 1 - decltype(token)::value;
       const float2 rate = rates[wave][t][c];
+      bcast_fma<t>(carry, C, rate.y);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) carry[i] = (row_bcast<t>(C[i]) * rate.y + carry[i]) * __builtin_amdgcn_exp2f(a2[i] * rate.x);
+      for (int i = 0; i < 4; ++i) carry[i] *= __builtin_amdgcn_exp2f(a2[i] * rate.x);
       if constexpr (MASKED)
         if ((m.starts >> t) & 1u) carry[0] = carry[1] = carry[2] = carry[3] = 0.f;
     });
     wave_order();
   }
-  const long long row = ((long long)at.b * p.S + at.seg) * p.W + w;
+  const long long row = ((long long)at.b * p.S * p.parts + at.seg) * p.W + w;
   sel_store_states(p.ends, row, n0, p.N, ok, WHOLE, carry);
   total = all_rows_sum(total);
   if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
@@ -91,7 +94,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   __shared__ float2 sum_rows[kSelWaves][64];
   __shared__ float vectors[2][2][kSelWaves][4][64];         // dB and dC of a tile, by waves; two tiles in turn
   __shared__ float parts[SLABS > 1 ? 2 : 1][SLABS > 1 ? kSelWaves : 1][3][4][64];
-  const SelPlace at = sel_place<SLABS, 1>(p);
+  const SelPlace at = sel_place<SLABS, 1>(p, p.S);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, j = lane >> 4;
   const int in_group = at.cg * kSelLanes + c, n0 = at.slab * kSelStates + 4 * j;
   const bool ok = in_group < p.Wg;
@@ -105,7 +108,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
   const float bias = ok && p.bias ? p.bias[w] : 0.f, skip = ok && p.D ? p.D[w] : 0.f;
   if (p.dh_last) sel_load_states(p.dh_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, carry);
-  sel_join<true>(p, at, w, n0, ok, a2, carry);
+  sel_join<true, WHOLE>(p, at, w, n0, ok, a2, carry);
   const bool gated = p.z != nullptr;
   const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
   const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j), lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
@@ -155,16 +158,14 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       sel_each<4>([&](auto token) {
         constexpr int t = 4 * decltype(group)::value + decltype(token)::value;
         const float2 rate = *reinterpret_cast<const float2*>(&rates[wave][t][c]);
-        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float old = t ? h[t ? t - 1 : 0][i] : before[i];
           if constexpr (MASKED) old = (m.starts >> t) & 1u ? 0.f : old;
           a[t][i] = __builtin_amdgcn_exp2f(a2[i] * rate.x);
           h[t][i] = fmaf(a[t][i], old, row_bcast<t>(B[i]) * rate.y);
-          sum = i ? sum + row_bcast<t>(C[i]) * h[t][i] : row_bcast<t>(C[i]) * h[t][i];
         }
-        sums[decltype(token)::value] = sum;
+        sums[decltype(token)::value] = bcast_dot<t>(C, h[t]);
       });
       gates[wave][4 * decltype(group)::value + j][c][2] = four_rows_sum(sums);
       __builtin_amdgcn_sched_barrier(0);
@@ -194,14 +195,14 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       sel_each<4>([&](auto token) {
         constexpr int k = 3 - decltype(token)::value, t = 4 * g4 + k;
         const f32x4 rate = rates[wave][t][c];
-        float sb = 0.f, sa = 0.f;
+        float sa = 0.f;
+        bcast_fma<t>(carry, C, rate[2]);                     // the gradient of this token's state
+        sum_b[k] = bcast_dot<t>(B, carry);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float dh = row_bcast<t>(C[i]) * rate[2] + carry[i];
           dC[k][i] = rate[2] * h[t][i];
-          dB[k][i] = rate[1] * dh;
-          sb = i ? sb + row_bcast<t>(B[i]) * dh : row_bcast<t>(B[i]) * dh;
-          carry[i] = a[t][i] * dh;
+          dB[k][i] = rate[1] * carry[i];
+          carry[i] *= a[t][i];
           float q = carry[i] * (t ? h[t ? t - 1 : 0][i] : front[i]);
           if constexpr (MASKED) {
             const bool cut = (m.starts >> t) & 1u;
@@ -211,7 +212,6 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
           sa = i ? fmaf(a2[i], q, sa) : a2[i] * q;
           tile_dA[i] = fmaf(rate[0], q, tile_dA[i]);
         }
-        sum_b[k] = sb;
         sum_a[k] = sa;
       });
       const float along = four_rows_sum(sum_b), through = four_rows_sum(sum_a);
@@ -282,8 +282,9 @@ static __global__ __launch_bounds__(256) void sel_sums_kernel(SelSums jobs) {
 }
 
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_backward_whole(const SelArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.B * (long long)a.S * a.G * a.per_group)), block(kSelThreads);
-  if (a.S > 1) hipLaunchKernelGGL((sel_reverse_kernel<IO, SLABS, MASKED, WHOLE>), grid, block, 0, s, a);
+  const unsigned wgs = (unsigned)(a.B * (long long)a.S * a.G * a.per_group);
+  const dim3 grid(wgs), block(kSelThreads);
+  if (a.S > 1) hipLaunchKernelGGL((sel_reverse_kernel<IO, SLABS, MASKED, WHOLE>), dim3(wgs * (unsigned)a.parts), block, 0, s, a);
   hipLaunchKernelGGL((sel_backward_kernel<IO, SLABS, MASKED, WHOLE>), grid, block, 0, s, a);
 }
 template <typename IO, int SLABS> static void sel_backward_slabs(const SelArgs& a, hipStream_t s) {

@@ -85,7 +85,13 @@ static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int
   // a summary's share of a walk's instructions
   a->S = sel_segments(wgs, a->tiles, backward ? 0.27 : 0.6);
   a->seg_tiles = (a->tiles + a->S - 1) / a->S;
-  return wgs * a->S < (1ll << 24);
+  // the summary is a short walk of few registers, which fills the device with six waves a SIMD
+  const long long summaries = B * G * (long long)a->per_group * (a->S - 1), most = a->seg_tiles / 4;
+  long long parts = summaries > 0 ? 6ll * num_compute_units() / summaries : 1;
+  if (parts > most) parts = most;
+  if (parts > kSelMaxSegments / a->S) parts = kSelMaxSegments / a->S;
+  a->parts = (int)(parts < 1 ? 1 : parts);
+  return B * G * (long long)(a->per_group + a->pipe_group) * a->S * a->parts < (1ll << 24);
 }
 
 static int sel_check(const char* who, SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int64_t N, int dtype, bool backward) {
@@ -131,7 +137,7 @@ size_t rglru_hip_selective_workspace_bytes(int64_t B, int64_t T, int64_t W, int6
   SelArgs a;
   if (!sel_plan(&a, B, T, W, G, N, false)) return 0;
   size_t n = keep ? sel_bytes((long long)B * a.tiles * W * N) : 0;
-  if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
+  if (a.S > 1) n += sel_bytes((long long)B * a.S * a.parts * W * N) + sel_bytes(2ll * B * a.S * a.parts * W);
   return n + 256;
 }
 
@@ -139,7 +145,7 @@ size_t rglru_hip_selective_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_
   SelArgs a;
   if (!sel_plan(&a, B, T, W, G, N, true)) return 0;
   size_t n = 2 * sel_bytes((long long)a.per_group * B * T * G * N) + sel_bytes((long long)B * a.S * W * N) + 2 * sel_bytes((long long)B * a.S * W);
-  if (a.S > 1) n += sel_bytes((long long)B * a.S * W * N) + sel_bytes(2ll * B * a.S * W);
+  if (a.S > 1) n += sel_bytes((long long)B * a.S * a.parts * W * N) + sel_bytes(2ll * B * a.S * a.parts * W);
   return n;
 }
 
@@ -156,7 +162,7 @@ int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const 
   if (rc) return rc;
   char* at = (char*)ws;
   if (keep) { a.kept = (float*)at; at += sel_bytes((long long)B * a.tiles * W * N); }
-  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + sel_bytes((long long)B * a.S * W * N)); }
+  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + sel_bytes((long long)B * a.S * a.parts * W * N)); }
   a.whole = a.whole && sel_whole(N, {A, h0, h_last, ws});
   return sel_launch_forward(a, dtype, (hipStream_t)stream);
 }
@@ -182,7 +188,7 @@ int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const 
   a.dA = (float*)at; at += states;
   a.dD = (float*)at; at += rows;
   a.dbias = (float*)at; at += rows;
-  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + states); }
+  if (a.S > 1) { a.ends = (float*)at; a.sums = (float*)(at + sel_bytes((long long)B * a.S * a.parts * W * N)); }
   a.whole = a.whole && sel_whole(N, {A, dh_last, dh0, ws, scratch});
   return sel_launch_backward(a, dB, dC, dA, dD, dbias, dtype, (hipStream_t)stream);
 }
