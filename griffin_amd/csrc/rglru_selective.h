@@ -27,7 +27,7 @@ constexpr int kSelTile = 16;                  // tokens of a tile; the forward p
 constexpr int kSelLanes = 16;                 // channels of a wave
 constexpr int kSelStates = 16;                // states of a wave
 constexpr int kSelMaxStates = 64;
-constexpr int kSelPipe = 2;                   // waves that take a sequence's tiles in turn
+constexpr int kSelPipe = 4;                   // waves that take a sequence's tiles in turn
 constexpr int kSelMaxSegments = 64;
 constexpr unsigned kSelRange = 0x7fffff00u;   // bytes of a tile's buffers; kOutOfRange lies outside
 
@@ -169,14 +169,18 @@ RGLRU_DEVICE SelRate sel_rate(float x, bool soft) {
 // are used.  The buffer ends with the tile's last token; lanes without a channel ask behind it.
 template <typename IO> struct SelStream {
   int raw[4];
-  static RGLRU_DEVICE unsigned lane_offset(unsigned stride, int w, bool ok, int j) {
-    return ok ? ((unsigned)j * stride + (unsigned)w) * (unsigned)sizeof(IO) : kOutOfRange;
+  // Where the lane's channel lies in a row; its first token's place comes to that (both below 2^24), made where it is used: kept, it would cost a register.
+  static RGLRU_DEVICE unsigned channel(int w, bool ok) { return ok ? (unsigned)w * (unsigned)sizeof(IO) : kOutOfRange; }
+  static RGLRU_DEVICE unsigned first(unsigned channel, unsigned stride, int j) {
+    asm("" : "+v"(j));
+    return channel + __umul24((unsigned)j, stride * (unsigned)sizeof(IO));
   }
   static RGLRU_DEVICE rsrc_t tile(const void* base, long long at, unsigned stride, int left) {
     return make_rsrc((const IO*)base + at, stride ? (unsigned)left * stride * (unsigned)sizeof(IO) : kSelRange);
   }
-  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int left, unsigned lane) {
+  RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int left, unsigned channel, int j) {
     const rsrc_t r = tile(base, at, stride, left);
+    const unsigned lane = first(channel, stride, j);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const unsigned off = lane + (unsigned)q * 4u * stride * (unsigned)sizeof(IO);
@@ -186,8 +190,9 @@ template <typename IO> struct SelStream {
   }
   RGLRU_DEVICE float operator[](int q) const { return __builtin_bit_cast(float, sizeof(IO) == 2 ? raw[q] << 16 : raw[q]); }
 };
-template <typename IO> RGLRU_DEVICE void sel_store(const float (&v)[4], void* base, long long at, unsigned stride, int left, unsigned lane) {
+template <typename IO> RGLRU_DEVICE void sel_store(const float (&v)[4], void* base, long long at, unsigned stride, int left, unsigned channel, int j) {
   const rsrc_t r = SelStream<IO>::tile(base, at, stride, left);
+  const unsigned lane = SelStream<IO>::first(channel, stride, j);
 #pragma unroll
   for (int q = 0; q < 4; ++q) BufIo<IO>::store((IO)v[q], r, lane + (unsigned)q * 4u * stride * (unsigned)sizeof(IO), 0);
 }
@@ -197,6 +202,7 @@ template <typename IO, bool WHOLE> struct SelVector {
   int raw[4];
   RGLRU_DEVICE void load(const void* base, long long at, unsigned stride, int n0, int N, int left, int k) {
     const rsrc_t r = make_rsrc((const IO*)base + at, kSelRange);
+    asm("" : "+v"(k), "+v"(n0));                             // as above
     const unsigned off = k < left ? ((unsigned)k * stride + (unsigned)n0) * (unsigned)sizeof(IO) : kOutOfRange;
     if constexpr (WHOLE) {
       const unsigned o = n0 < N ? off : kOutOfRange;
@@ -282,7 +288,7 @@ template <bool WHOLE> struct SelStates {
 };
 
 // Has the compiler make `v` here, and not where it is used.
-RGLRU_DEVICE void sel_made(float& v) { asm volatile("" : "+v"(v)); }
+RGLRU_DEVICE void sel_made(float& v) { asm("" : "+v"(v)); }
 
 // The masks of a tile's tokens, the same in all lanes: bit k is token t0 + k's.  Tokens behind the sequence's end are inactive.
 struct SelMasks { unsigned live, starts; };

@@ -25,14 +25,14 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
 #pragma unroll
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
   const float bias = ok && p.bias ? p.bias[w] : 0.f;
-  const unsigned lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j), lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
+  const unsigned channel = SelStream<IO>::channel(w, ok);
   SelStream<IO> next_u, next_dt;
   SelVector<IO, WHOLE> next_B;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
     next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
   };
   if (first < last) request(first);
@@ -99,21 +99,19 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
     if (p.h0) sel_load_states(p.h0, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
     sel_join<false, WHOLE>(p, at, w, n0, ok, a2, h);
   }
-  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
-  const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
+  const unsigned channel = SelStream<IO>::channel(w, ok);
   const unsigned lane_h = SelStates<WHOLE>::lane_offset(w, n0, p.N, ok);
   const bool gated = p.z != nullptr;
-  const unsigned lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
   SelStream<IO> next_u, next_dt, next_z;
   SelVector<IO, WHOLE> next_B, next_C;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
     next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
     next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
   };
   if (first + at.turn < last) request(first + at.turn);
   for (int tile = first + at.turn; tile < last; tile += PIPE) {
@@ -199,8 +197,12 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
       }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) y[q] = (m.live >> (4 * q + j)) & 1u ? fmaf(skip, u[q], y[q]) * gate[q] : 0.f;
-    if (SLABS == 1 || at.slab == 0) sel_store<IO>(y, p.y, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
+    for (int q = 0; q < 4; ++q) {
+      float out = fmaf(skip, u[q], y[q]) * gate[q];
+      sel_made(out);                                        // no branch around it
+      y[q] = (m.live >> (4 * q + j)) & 1u ? out : 0.f;
+    }
+    if (SLABS == 1 || at.slab == 0) sel_store<IO>(y, p.y, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
   }
   if ((last - 1 - first) % PIPE == at.turn && at.seg == p.S - 1) sel_store_states(p.h_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
 }

@@ -36,16 +36,15 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   for (int i = 0; i < 4; ++i) a2[i] *= kLog2e;
   const float bias = ok && p.bias ? p.bias[w] : 0.f;
   const bool gated = p.z != nullptr;
-  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j);
-  const unsigned lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
+  const unsigned channel = SelStream<IO>::channel(w, ok);
   SelStream<IO> next_dt, next_z, next_d;
   SelVector<IO, WHOLE> next_C;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
+    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
     next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
   };
   if (first < last) request(last - 1);
@@ -110,21 +109,20 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   if (p.dh_last) sel_load_states(p.dh_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, carry);
   sel_join<true, WHOLE>(p, at, w, n0, ok, a2, carry);
   const bool gated = p.z != nullptr;
-  const unsigned lane_d = SelStream<IO>::lane_offset((unsigned)p.W, w, ok, j), lane_u = SelStream<IO>::lane_offset((unsigned)p.sut, w, ok, j);
-  const unsigned lane_dt = SelStream<IO>::lane_offset((unsigned)p.sdt, w, ok, j), lane_z = SelStream<IO>::lane_offset((unsigned)p.szt, w, ok && gated, j);
+  const unsigned channel = SelStream<IO>::channel(w, ok);
   const unsigned lane_h = SelStates<WHOLE>::lane_offset(w, n0, p.N, ok);
   // what is written for the tile's tokens: one lane a token and channel, of the first slab's waves
-  const unsigned lane_out = SLABS == 1 || at.slab == 0 ? lane_d : kOutOfRange;
+  const unsigned channel_out = SLABS == 1 || at.slab == 0 ? channel : kOutOfRange;
   SelStream<IO> next_u, next_dt, next_z, next_d;
   SelVector<IO, WHOLE> next_B, next_C;
   SelStates<WHOLE> next_h;
   auto request = [&](int tile) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, lane_dt);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, lane_u);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, lane_d);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, lane_z);
+    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
+    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
+    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
+    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
     next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
     next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
     next_h.load(SelStates<WHOLE>::rows(p.kept, ((long long)at.b * p.tiles + tile) * p.W, p.W, p.N), lane_h, n0, p.N);
@@ -182,7 +180,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       const float du = live ? fmaf(rate[0], along, skip * rate[2]) : 0.f, dt_out = live ? ddt : 0.f;
       tile_dD = fmaf(rate[2], rate[3], tile_dD);
       tile_dbias += dt_out;
-      const unsigned off = lane_out + (unsigned)q * 4u * (unsigned)p.W * (unsigned)sizeof(IO);
+      const unsigned off = SelStream<IO>::first(channel_out, (unsigned)p.W, j) + (unsigned)q * 4u * (unsigned)p.W * (unsigned)sizeof(IO);
       BufIo<IO>::store((IO)du, SelStream<IO>::tile(p.du, place, (unsigned)p.W, left), off, 0);
       BufIo<IO>::store((IO)dt_out, SelStream<IO>::tile(p.ddt, place, (unsigned)p.W, left), off, 0);
       if (gated) BufIo<IO>::store((IO)(live ? gate[1] * fmaf(skip, rate[3], y_all ? *y_all : gate[2]) : 0.f), SelStream<IO>::tile(p.dz, place, (unsigned)p.W, left), off, 0);
