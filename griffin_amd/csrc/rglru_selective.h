@@ -287,6 +287,10 @@ template <bool WHOLE> struct SelStates {
   }
 };
 
+// Waits for the loads in front of a loop.  Inside it the loads for the next round are older than the stores of this one, and a wait for them lets the stores be;
+// with loads under way on the path into the loop, the compiler would have every round wait for all.
+RGLRU_DEVICE void sel_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // Has the compiler make `v` here, and not where it is used.
 RGLRU_DEVICE void sel_made(float& v) { asm("" : "+v"(v)); }
 

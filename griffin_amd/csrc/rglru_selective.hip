@@ -36,6 +36,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
   };
   if (first < last) request(first);
+  sel_arrived();
   float total = 0.f;
   bool cut = false;
   for (int tile = first; tile < last; ++tile) {
@@ -114,6 +115,7 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
     next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
   };
   if (first + at.turn < last) request(first + at.turn);
+  sel_arrived();
   for (int tile = first + at.turn; tile < last; tile += PIPE) {
     const long long t0 = (long long)tile * kSelTile;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);

@@ -48,6 +48,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
   };
   if (first < last) request(last - 1);
+  sel_arrived();
   float total = 0.f;
   bool cut = false;
   for (int tile = last - 1; tile >= first; --tile) {
@@ -128,6 +129,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     next_h.load(SelStates<WHOLE>::rows(p.kept, ((long long)at.b * p.tiles + tile) * p.W, p.W, p.N), lane_h, n0, p.N);
   };
   request(last - 1);
+  sel_arrived();
   for (int tile = last - 1; tile >= first; --tile) {
     const long long t0 = (long long)tile * kSelTile, place = ((long long)at.b * p.T + t0) * p.W;
     const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);

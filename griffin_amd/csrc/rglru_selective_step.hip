@@ -15,42 +15,89 @@ struct SelStepArgs {
   float* state;
   void* y;
   long long su, sdt, sz, sBb, sBg, sCb, sCg;
-  int B, W, N, Wg, lanes, softplus, whole;
+  int B, W, N, Wg, lanes, softplus;
 };
 
-// Four states a lane, N / 4 lanes (a power of two) a channel: the state is read and written once, in whole vectors, one behind the other.
-template <typename IO> __global__ __launch_bounds__(kSelThreads) void sel_step_kernel(SelStepArgs p) {
-  const long long item = (long long)blockIdx.x * kSelThreads + threadIdx.x;
-  const long long channel = item / p.lanes;
-  const int l = (int)(item % p.lanes), n0 = 4 * l;
-  const bool there = channel < (long long)p.B * p.W;
-  const int b = there ? (int)(channel / p.W) : 0, w = there ? (int)(channel - (long long)b * p.W) : 0, g = w / p.Wg;
-  const unsigned flag = p.flags ? p.flags[b] : 0u;
-  const bool live = !(flag & 2u);
-  const long long row = (long long)b * p.W + w;
-  float a[4], h[4], y = 0.f;
-  sel_load_states(p.state, row, n0, p.N, there && flag == 0u, p.whole, h);
-  sel_load_states(p.A, w, n0, p.N, there, p.whole, a);
-  const float u = (float)((const IO*)p.u)[b * p.su + w];
-  const float s = sel_rate((float)((const IO*)p.dt)[b * p.sdt + w] + (p.bias ? p.bias[w] : 0.f), p.softplus).s, su = s * u;
+// Four states a lane, N / 4 lanes (a power of two) a channel, so that the state is read and written in whole vectors, one behind the other; a thread takes
+// kSelStepItems such vectors a workgroup's width apart, all of them asked for before the first is used.  Bound by the state's traffic.
+// PAST: states of 16 MiB or more go past the caches: by the next token the states of other layers have been there.
+constexpr int kSelStepItems = 2;
+template <typename IO, bool WHOLE, bool PAST> __global__ __launch_bounds__(kSelThreads) void sel_step_kernel(SelStepArgs p) {
+  typedef IO Four __attribute__((ext_vector_type(4)));
+  const int l = (int)threadIdx.x % p.lanes, n0 = 4 * l;
+  const unsigned channels = (unsigned)kSelThreads / (unsigned)p.lanes;   // of a workgroup's pass
+  float a[kSelStepItems][4], h[kSelStepItems][4], u[kSelStepItems], x[kSelStepItems], z[kSelStepItems], skip[kSelStepItems], vb[kSelStepItems][4], vc[kSelStepItems][4];
+  long long row[kSelStepItems];
+  int where[kSelStepItems];
+  unsigned flag[kSelStepItems];
+  bool there[kSelStepItems];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool has = n0 + i < p.N;
-    const float vb = has ? (float)((const IO*)p.Bm)[b * p.sBb + g * p.sBg + n0 + i] : 0.f;
-    const float vc = has ? (float)((const IO*)p.Cm)[b * p.sCb + g * p.sCg + n0 + i] : 0.f;
-    h[i] = fmaf(__builtin_amdgcn_exp2f(a[i] * kLog2e * s), h[i], vb * su);
-    y = fmaf(vc, h[i], y);
-  }
-  for (int m = 1; m < p.lanes; m <<= 1) y += __shfl_xor(y, m, 64);
-  if (!there) return;
-  if (live) sel_store_states(p.state, row, n0, p.N, true, p.whole, h);
-  if (l == 0) {
-    if (p.D) y = fmaf(p.D[w], u, y);
-    if (p.z) {
-      const float z = (float)((const IO*)p.z)[b * p.sz + w];
-      y *= z * sigmoid_fast(z);
+  for (int k = 0; k < kSelStepItems; ++k) {
+    const long long channel = ((long long)blockIdx.x * kSelStepItems + k) * channels + threadIdx.x / (unsigned)p.lanes;
+    there[k] = channel < (long long)p.B * p.W;
+    row[k] = there[k] ? channel : 0;
+    const unsigned b = (unsigned)(row[k] / p.W);
+    const int w = (int)(row[k] - (long long)b * p.W), g = w / p.Wg;
+    where[k] = w;
+    flag[k] = p.flags ? p.flags[b] : 0u;
+    const float* state = p.state + row[k] * p.N + n0;
+    if constexpr (WHOLE) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f}, d = s;
+      Four fb = {}, fc = {};
+      if (n0 < p.N) {
+        s = PAST ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(state)) : *reinterpret_cast<const f32x4*>(state);
+        d = *reinterpret_cast<const f32x4*>(p.A + (long long)w * p.N + n0);
+        fb = *reinterpret_cast<const Four*>((const IO*)p.Bm + b * p.sBb + g * p.sBg + n0);
+        fc = *reinterpret_cast<const Four*>((const IO*)p.Cm + b * p.sCb + g * p.sCg + n0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { h[k][i] = s[i]; a[k][i] = d[i]; vb[k][i] = (float)fb[i]; vc[k][i] = (float)fc[i]; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool has = n0 + i < p.N;
+        h[k][i] = has ? state[i] : 0.f;
+        a[k][i] = has ? p.A[(long long)w * p.N + n0 + i] : 0.f;
+        vb[k][i] = has ? (float)((const IO*)p.Bm)[b * p.sBb + g * p.sBg + n0 + i] : 0.f;
+        vc[k][i] = has ? (float)((const IO*)p.Cm)[b * p.sCb + g * p.sCg + n0 + i] : 0.f;
+      }
     }
-    ((IO*)p.y)[row] = (IO)(live ? y : 0.f);
+    u[k] = (float)((const IO*)p.u)[b * p.su + w];
+    x[k] = (float)((const IO*)p.dt)[b * p.sdt + w] + (p.bias ? p.bias[w] : 0.f);
+    z[k] = p.z ? (float)((const IO*)p.z)[b * p.sz + w] : 0.f;
+    skip[k] = p.D ? p.D[w] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < kSelStepItems; ++k) {
+    const float s = sel_rate(x[k], p.softplus).s, su = s * u[k];
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float old = flag[k] & 1u ? 0.f : h[k][i];       // whatever a document start discards
+      h[k][i] = fmaf(__builtin_amdgcn_exp2f(a[k][i] * kLog2e * s), old, vb[k][i] * su);
+      y = fmaf(vc[k][i], h[k][i], y);
+    }
+    for (int m = 1; m < p.lanes; m <<= 1) y += __shfl_xor(y, m, 64);
+    if (!there[k]) continue;
+    const bool live = !(flag[k] & 2u);
+    float* state = p.state + row[k] * p.N + n0;
+    if (live) {
+      if constexpr (WHOLE) {
+        const f32x4 out = {h[k][0], h[k][1], h[k][2], h[k][3]};
+        if (n0 < p.N) {
+          if constexpr (PAST) __builtin_nontemporal_store(out, reinterpret_cast<f32x4*>(state)); else *reinterpret_cast<f32x4*>(state) = out;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n0 + i < p.N) state[i] = h[k][i];
+      }
+    }
+    if (l == 0) {
+      y = fmaf(skip[k], u[k], y);
+      if (p.z) y *= z[k] * sigmoid_fast(z[k]);
+      ((IO*)p.y)[row[k]] = (IO)(live ? y : 0.f);
+    }
   }
 }
 
@@ -206,12 +253,22 @@ int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const
   p.su = strides[0]; p.sdt = strides[1]; p.sz = strides[2]; p.sBb = strides[3]; p.sBg = strides[4]; p.sCb = strides[5]; p.sCg = strides[6];
   p.B = (int)B; p.W = (int)W; p.N = (int)N; p.Wg = (int)(W / G); p.softplus = softplus;
   p.lanes = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
-  p.whole = sel_whole(N, {A, state});
-  const long long blocks = (B * W * p.lanes + kSelThreads - 1) / kSelThreads;
+  bool whole = sel_whole(N, {A, state});
+  for (int i = 3; i < 7; ++i) whole = whole && strides[i] % 4 == 0;
+  const uintptr_t boundary = dtype == RGLRU_BF16 ? 8 : 16;
+  whole = whole && (uintptr_t)Bm % boundary == 0 && (uintptr_t)Cm % boundary == 0;
+  const bool past = B * W * N * 4 >= (16ll << 20);
+  const long long each = (long long)kSelStepItems * (kSelThreads / p.lanes), blocks = (B * W + each - 1) / each;
   if (blocks >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "selective_step: tensor too large");
   const dim3 grid((unsigned)blocks), block(kSelThreads);
-  if (dtype == RGLRU_BF16) hipLaunchKernelGGL((sel_step_kernel<__bf16>), grid, block, 0, (hipStream_t)stream, p);
-  else hipLaunchKernelGGL((sel_step_kernel<float>), grid, block, 0, (hipStream_t)stream, p);
+#define RGLRU_STEP_LAUNCH(IO)                                                                                                     \
+  do {                                                                                                                            \
+    if (!whole) hipLaunchKernelGGL((sel_step_kernel<IO, false, false>), grid, block, 0, (hipStream_t)stream, p);                    \
+    else if (past) hipLaunchKernelGGL((sel_step_kernel<IO, true, true>), grid, block, 0, (hipStream_t)stream, p);                   \
+    else hipLaunchKernelGGL((sel_step_kernel<IO, true, false>), grid, block, 0, (hipStream_t)stream, p);                            \
+  } while (0)
+  if (dtype == RGLRU_BF16) RGLRU_STEP_LAUNCH(__bf16); else RGLRU_STEP_LAUNCH(float);
+#undef RGLRU_STEP_LAUNCH
   return check_launch("selective_step");
 }
 

@@ -18,7 +18,8 @@ namespace rglru {
 
 constexpr int kShortThreads = 256;
 constexpr int kShortTaps = 4;
-constexpr int kShortRun = 16;                 // tokens of a run
+constexpr int kShortRun = 16, kShortRunBack = 32;  // tokens of a run, most of one on the way back
+constexpr int kShortBatch = 8, kShortBatchBack = 4;  // tokens asked for at a time
 constexpr int kShortVecs = 32, kShortRuns = kShortThreads / kShortVecs;  // channel vectors and runs of a workgroup
 
 struct ShortArgs {
@@ -27,20 +28,25 @@ struct ShortArgs {
   void *y, *new_state, *dx, *dstate;          // new_state, dstate: or null
   float* partial;                             // [B][run groups][K + 1][W]
   long long sxb, sxt;                         // elements between x's batch rows and tokens
-  int B, T, W, nvec, runs, vec_dtype, activation;
+  int B, T, W, nvec, run, runs, vec_dtype, activation;   // run: tokens of a run
 };
 
 template <typename IO, int V> struct ShortRow {
   typedef IO Raw __attribute__((ext_vector_type(V)));
-  static RGLRU_DEVICE void load(const IO* p, float (&v)[V]) {
+  static RGLRU_DEVICE Raw request(const IO* p) {
     if constexpr (V == 1) {
-      v[0] = (float)*p;
+      Raw r;
+      r[0] = *p;
+      return r;
     } else {
-      const Raw r = *reinterpret_cast<const Raw*>(p);
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = (float)r[e];
+      return *reinterpret_cast<const Raw*>(p);
     }
   }
+  static RGLRU_DEVICE void unpack(const Raw& r, float (&v)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)r[e];
+  }
+  static RGLRU_DEVICE void load(const IO* p, float (&v)[V]) { unpack(request(p), v); }
   static RGLRU_DEVICE void store(IO* p, const float (&v)[V]) {
     if constexpr (V == 1) {
       *p = (IO)v[0];
@@ -53,15 +59,43 @@ template <typename IO, int V> struct ShortRow {
   }
 };
 
-RGLRU_DEVICE float short_param(const void* p, long long i, int dtype) { return dtype == RGLRU_BF16 ? (float)((const __bf16*)p)[i] : ((const float*)p)[i]; }
+// N consecutive parameters, by vectors where they lie on their boundaries: element by element, the taps of eight channels are 32 loads.
+template <typename T, int N> RGLRU_DEVICE void short_params_of(const T* p, float (&out)[N]) {
+  constexpr int E = 16 / (int)sizeof(T);
+  if (N % E == 0 && ((uintptr_t)p & 15) == 0) {
+    typedef T Raw __attribute__((ext_vector_type(E)));
+#pragma unroll
+    for (int q = 0; q < N / E; ++q) {
+      const Raw r = reinterpret_cast<const Raw*>(p)[q];
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[(q * E + e) % N] = (float)r[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = (float)p[e];
+  }
+}
+template <int N> RGLRU_DEVICE void short_params(const void* p, long long first, int dtype, float (&out)[N]) {
+  if (dtype == RGLRU_BF16) short_params_of<__bf16, N>((const __bf16*)p + first, out); else short_params_of<float, N>((const float*)p + first, out);
+}
 
 template <int V, int K> RGLRU_DEVICE void short_taps(const ShortArgs& p, int c0, float (&tap)[K][V], float (&bias)[V]) {
+  float flat[V * K];
+  short_params<V * K>(p.taps, (long long)c0 * K, p.vec_dtype, flat);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    bias[v] = p.bias ? short_param(p.bias, c0 + v, p.vec_dtype) : 0.f;
+    bias[v] = 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) tap[j][v] = short_param(p.taps, (long long)(c0 + v) * K + K - 1 - j, p.vec_dtype);  // by lag
+    for (int j = 0; j < K; ++j) tap[j][v] = flat[v * K + K - 1 - j];  // by lag
   }
+  if (p.bias) short_params<V>(p.bias, c0, p.vec_dtype, bias);
+}
+
+// Whether 32 tokens in a row are inactive.
+RGLRU_DEVICE bool short_idle(const unsigned char* flags) {
+  unsigned long long w[4];
+  __builtin_memcpy(w, flags, 32);
+  return (w[0] & w[1] & w[2] & w[3] & 0x0202020202020202ull) == 0x0202020202020202ull;
 }
 
 // The window in front of token t0: win[j] is the input of lag j + 1, zero in front of the document.  Rows of the carried state stand in front of token 0
@@ -81,12 +115,7 @@ RGLRU_DEVICE void short_window(const ShortArgs& p, int b, int c0, int t0, float 
     if constexpr (MASKED) {
       const unsigned char* flags = p.flags + (long long)b * p.T;
       // past inactive tokens, 32 at a time where there are so many
-      while (open && t >= 31) {
-        unsigned long long w[4];
-        __builtin_memcpy(w, flags + t - 31, 32);
-        if ((w[0] & w[1] & w[2] & w[3] & 0x0202020202020202ull) != 0x0202020202020202ull) break;
-        t -= 32;
-      }
+      while (open && t >= 31 && short_idle(flags + t - 31)) t -= 32;
       while (open && t >= 0 && (flags[t] & 2u)) --t;
       f = open && t >= 0 ? flags[t] : 0u;
     }
@@ -134,33 +163,66 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
   short_window<IO, V, K, MASKED>(p, b, c0, t0, win);
   const IO* x = (const IO*)p.x + b * p.sxb + t0 * p.sxt + c0;
   IO* y = (IO*)p.y + ((long long)b * p.T + t0) * p.W + c0;
-#pragma unroll 8
-  for (int i = 0; i < kShortRun; ++i) {
-    if (i >= n) break;
-    unsigned f = 0;
-    if constexpr (MASKED) f = p.flags[(long long)b * p.T + t0 + i];
-    const bool live = !(f & 2u), start = (f & 3u) == 1u;
-    float cur[V], out[V];
-    ShortRow<IO, V>::load(x + i * p.sxt, cur);
+  const unsigned char* flags = MASKED ? p.flags + (long long)b * p.T + t0 : nullptr;
+  for (int i0 = 0; i0 < n; i0 += kShortBatch) {
+    typename ShortRow<IO, V>::Raw raw[kShortBatch];
+    unsigned f[kShortBatch];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float a = fmaf(cur[v], tap[0][v], bias[v]);
-      if constexpr (MASKED) {
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) win[j][v] = start ? 0.f : win[j][v];
-      }
-#pragma unroll
-      for (int j = K - 2; j >= 0; --j) {
-        a = fmaf(win[j][v], tap[j + 1][v], a);
-        if (!MASKED || live) win[j][v] = j ? win[j ? j - 1 : 0][v] : cur[v];
-      }
-      out[v] = live ? short_act(a, p.activation) : 0.f;
+    for (int k = 0; k < kShortBatch; ++k) {
+      const int i = i0 + k < n ? i0 + k : n - 1;
+      raw[k] = ShortRow<IO, V>::request(x + i * p.sxt);
+      f[k] = MASKED ? flags[i] : 0u;
     }
-    ShortRow<IO, V>::store(y + (long long)i * p.W, out);
+#pragma unroll
+    for (int k = 0; k < kShortBatch; ++k) {
+      const bool there = i0 + k < n, live = there && !(f[k] & 2u), start = live && (f[k] & 1u);
+      float cur[V], out[V];
+      ShortRow<IO, V>::unpack(raw[k], cur);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a = fmaf(cur[v], tap[0][v], bias[v]);
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) win[j][v] = start ? 0.f : win[j][v];
+        }
+#pragma unroll
+        for (int j = K - 2; j >= 0; --j) {
+          a = fmaf(win[j][v], tap[j + 1][v], a);
+          win[j][v] = live ? (j ? win[j ? j - 1 : 0][v] : cur[v]) : win[j][v];
+        }
+        a = short_act(a, p.activation);
+        out[v] = live ? a : 0.f;
+      }
+      if (there) ShortRow<IO, V>::store(y + (long long)(i0 + k) * p.W, out);
+    }
   }
   if (K > 1 && p.new_state && it.run == p.runs - 1) {
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) ShortRow<IO, V>::store((IO*)p.new_state + ((long long)b * (K - 1) + K - 2 - j) * p.W + c0, win[j]);
+  }
+}
+
+// A workgroup's runs add up their parameter gradients in LDS.
+template <int V, int K> RGLRU_DEVICE void short_reduce(const ShortArgs& p, float (&red)[kShortRuns][(K + 1) * V][kShortVecs + 1], const float (&dtap)[K][V],
+                                                       const float (&dbias)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    red[threadIdx.x / kShortVecs][K * V + v][threadIdx.x % kShortVecs] = dbias[v];
+#pragma unroll
+    for (int j = 0; j < K; ++j) red[threadIdx.x / kShortVecs][(K - 1 - j) * V + v][threadIdx.x % kShortVecs] = dtap[j][v];
+  }
+  __syncthreads();
+  const unsigned vec_groups = (unsigned)(p.nvec + kShortVecs - 1) / kShortVecs;
+  float* part = p.partial + (long long)(blockIdx.x / vec_groups) * (K + 1) * p.W;
+  const int first = (int)(blockIdx.x % vec_groups) * kShortVecs;
+  for (int idx = threadIdx.x; idx < (K + 1) * V * kShortVecs; idx += kShortThreads) {
+    const int row = idx / kShortVecs, lv = idx - row * kShortVecs, k = row / V, v = row - k * V, ch = (first + lv) * V + v;
+    if (first + lv < p.nvec) {
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < kShortRuns; ++q) sum += red[q][row][lv];
+      part[(long long)k * p.W + ch] = sum;
+    }
   }
 }
 
@@ -169,7 +231,7 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
 template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(kShortThreads) void short_conv_bwd_kernel(ShortArgs p) {
   __shared__ float red[kShortRuns][(K + 1) * V][kShortVecs + 1];
   const ShortItem it = short_item<V>(p);
-  const int b = it.b, c0 = it.c0, t0 = it.run * kShortRun, t1 = t0 + kShortRun < p.T ? t0 + kShortRun : p.T;
+  const int b = it.b, c0 = it.c0, t0 = it.run * p.run, t1 = t0 + p.run < p.T ? t0 + p.run : p.T;
   float dtap[K][V], dbias[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -203,9 +265,8 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
     }
     place[K - 1] = kNowhere;
     int owned = it.run == 0 && K > 1 ? K - 1 : 0;            // entries that wait for outputs
-    for (int t = t0; t < p.T && (t < t1 || owned > 0); ++t) {
-      unsigned f = 0;
-      if constexpr (MASKED) f = p.flags[(long long)b * p.T + t];
+    const unsigned char* flags = MASKED ? p.flags + (long long)b * p.T : nullptr;
+    auto token = [&](int t, unsigned f, const typename ShortRow<IO, V>::Raw& raw_x, const typename ShortRow<IO, V>::Raw& raw_d) {
       if (MASKED && (f & 2u)) {
         if (t < t1) {
           float none[V];
@@ -213,7 +274,7 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
           for (int v = 0; v < V; ++v) none[v] = 0.f;
           ShortRow<IO, V>::store(dx + (long long)t * p.W, none);
         }
-        continue;
+        return;
       }
       if (MASKED && (f & 1u)) {                              // the document ends: what waits is complete
 #pragma unroll
@@ -224,11 +285,11 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
           for (int v = 0; v < V; ++v) win[j][v] = 0.f;
         }
         owned = 0;
-        if (t >= t1) break;
+        if (t >= t1) return;
       }
       float cur[V], up[V];
-      ShortRow<IO, V>::load(x + t * p.sxt, cur);
-      ShortRow<IO, V>::load(dy + (long long)t * p.W, up);
+      ShortRow<IO, V>::unpack(raw_x, cur);
+      ShortRow<IO, V>::unpack(raw_d, up);
       // shift: entry j becomes lag j
 #pragma unroll
       for (int j = K - 1; j > 0; --j) {
@@ -236,23 +297,22 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
 #pragma unroll
         for (int v = 0; v < V; ++v) grad[j][v] = grad[j - 1][v];
       }
-      place[0] = t < t1 ? t : kNowhere;
-      if (t < t1) ++owned;
+      const bool mine = t < t1;
+      place[0] = mine ? t : kNowhere;
+      if (mine) ++owned;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float a = fmaf(cur[v], tap[0][v], bias[v]);
 #pragma unroll
         for (int j = K - 1; j >= 1; --j) a = fmaf(win[j - 1][v], tap[j][v], a);
-        const float d = up[v] * short_slope(a, p.activation);
+        const float d = up[v] * short_slope(a, p.activation), own = mine ? d : 0.f;
         grad[0][v] = d * tap[0][v];
 #pragma unroll
         for (int j = 1; j < K; ++j) grad[j][v] = fmaf(d, tap[j][v], grad[j][v]);
-        if (t < t1) {
-          dbias[v] += d;
-          dtap[0][v] = fmaf(d, cur[v], dtap[0][v]);
+        dbias[v] += own;
+        dtap[0][v] = fmaf(own, cur[v], dtap[0][v]);
 #pragma unroll
-          for (int j = 1; j < K; ++j) dtap[j][v] = fmaf(d, win[j - 1][v], dtap[j][v]);
-        }
+        for (int j = 1; j < K; ++j) dtap[j][v] = fmaf(own, win[j - 1][v], dtap[j][v]);
 #pragma unroll
         for (int j = K - 2; j >= 0; --j) win[j][v] = j ? win[j ? j - 1 : 0][v] : cur[v];
       }
@@ -261,29 +321,165 @@ template <typename IO, int V, int K, bool MASKED> __global__ __launch_bounds__(k
         place[K - 1] = kNowhere;
         --owned;
       }
+    };
+    typedef typename ShortRow<IO, V>::Raw Raw;
+    for (int u0 = t0; u0 < t1; u0 += kShortBatchBack) {
+      Raw raw_x[kShortBatchBack], raw_d[kShortBatchBack];
+      unsigned f[kShortBatchBack];
+#pragma unroll
+      for (int k = 0; k < kShortBatchBack; ++k) {
+        const int t = u0 + k < t1 ? u0 + k : t1 - 1;
+        raw_x[k] = ShortRow<IO, V>::request(x + t * p.sxt);
+        raw_d[k] = ShortRow<IO, V>::request(dy + (long long)t * p.W);
+        f[k] = MASKED ? flags[t] : 0u;
+      }
+#pragma unroll
+      for (int k = 0; k < kShortBatchBack; ++k)
+        if (u0 + k < t1) token(u0 + k, f[k], raw_x[k], raw_d[k]);
+    }
+    // outputs behind the run
+    for (int t = t1; t < p.T && owned > 0; ++t) {
+      if constexpr (MASKED) {                                // past inactive tokens, 32 at a time where there are so many
+        while (t + 32 <= p.T && short_idle(flags + t)) t += 32;
+        if (t == p.T) break;
+      }
+      token(t, MASKED ? flags[t] : 0u, ShortRow<IO, V>::request(x + t * p.sxt), ShortRow<IO, V>::request(dy + (long long)t * p.W));
     }
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) put(place[j], grad[j]);  // the row ends
   }
+  short_reduce<V, K>(p, red, dtap, dbias);
+}
+
+// ---- every token active, no document starts ---------------------------------------------------------------------------
+// The same walks without a branch: what lies outside a row is asked for behind its buffer's end and comes as zeros, and stores there are dropped.  A buffer begins
+// with the workgroup's first token, so that offsets stay below 2^31 (short_dense).
+template <typename IO, int V> struct ShortBuffer {
+  typedef typename ShortRow<IO, V>::Raw Raw;
+  rsrc_t r;
+  unsigned stride, at;                                       // bytes between tokens; of the lane's channels
+  RGLRU_DEVICE ShortBuffer(const void* base, long long first, long long step, int c0)
+      : r(make_rsrc((const IO*)base + first, base ? 0x7fffff00u : 0u)), stride((unsigned)step * (unsigned)sizeof(IO)), at((unsigned)c0 * (unsigned)sizeof(IO)) {}
+  RGLRU_DEVICE unsigned place(int t, bool ok) const { return ok ? (unsigned)t * stride + at : kOutOfRange; }
+  RGLRU_DEVICE Raw request(int t, bool ok) const {
+    if constexpr (V * sizeof(IO) == 2) return __builtin_bit_cast(Raw, (short)__builtin_amdgcn_raw_buffer_load_b16(r, place(t, ok), 0, 0));
+    else if constexpr (V * sizeof(IO) == 4) return __builtin_bit_cast(Raw, (int)__builtin_amdgcn_raw_buffer_load_b32(r, place(t, ok), 0, 0));
+    else if constexpr (V * sizeof(IO) == 8) return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(r, place(t, ok), 0, 0));
+    else return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(r, place(t, ok), 0, 0));
+  }
+  RGLRU_DEVICE void store(int t, bool ok, const float (&v)[V]) const {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    Raw raw;
+#pragma unroll
+    for (int e = 0; e < V; ++e) raw[e] = (IO)v[e];
+    if constexpr (V * sizeof(IO) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, raw), r, place(t, ok), 0, 0);
+    else if constexpr (V * sizeof(IO) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, raw), r, place(t, ok), 0, 0);
+    else if constexpr (V * sizeof(IO) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, raw), r, place(t, ok), 0, 0);
+    else buf_store_b128(__builtin_bit_cast(i32x4, raw), r, place(t, ok));
+  }
+};
+
+// One token of the forward walk: y of the token, and the window behind it.
+template <int V, int K> RGLRU_DEVICE void short_token(float (&win)[K > 1 ? K - 1 : 1][V], const float (&cur)[V], const float (&tap)[K][V], const float (&bias)[V],
+                                                      float (&pre)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    red[threadIdx.x / kShortVecs][K * V + v][threadIdx.x % kShortVecs] = dbias[v];
+    float a = fmaf(cur[v], tap[0][v], bias[v]);
 #pragma unroll
-    for (int j = 0; j < K; ++j) red[threadIdx.x / kShortVecs][(K - 1 - j) * V + v][threadIdx.x % kShortVecs] = dtap[j][v];
+    for (int j = K - 1; j >= 1; --j) a = fmaf(win[j - 1][v], tap[j][v], a);
+    pre[v] = a;
   }
-  __syncthreads();
-  const unsigned vec_groups = (unsigned)(p.nvec + kShortVecs - 1) / kShortVecs;
-  float* part = p.partial + (long long)(blockIdx.x / vec_groups) * (K + 1) * p.W;
-  const int first = (int)(blockIdx.x % vec_groups) * kShortVecs;
-  for (int idx = threadIdx.x; idx < (K + 1) * V * kShortVecs; idx += kShortThreads) {
-    const int row = idx / kShortVecs, lv = idx - row * kShortVecs, k = row / V, v = row - k * V, ch = (first + lv) * V + v;
-    if (first + lv < p.nvec) {
-      float sum = 0.f;
+}
+template <int V, int K> RGLRU_DEVICE void short_shift(float (&win)[K > 1 ? K - 1 : 1][V], const float (&cur)[V]) {
 #pragma unroll
-      for (int q = 0; q < kShortRuns; ++q) sum += red[q][row][lv];
-      part[(long long)k * p.W + ch] = sum;
+  for (int j = K - 2; j >= 0; --j)
+#pragma unroll
+    for (int v = 0; v < V; ++v) win[j][v] = j ? win[j ? j - 1 : 0][v] : cur[v];
+}
+
+template <typename IO, int V, int K> __global__ __launch_bounds__(kShortThreads) void short_conv_dense_kernel(ShortArgs p) {
+  const ShortItem it = short_item<V>(p);
+  const int b = it.b, c0 = it.c0, g0 = it.group * kShortRuns * kShortRun, t0 = it.run * kShortRun - g0, rows = p.T - g0;   // tokens from the workgroup's first on
+  const ShortBuffer<IO, V> x(p.x, b * p.sxb + (long long)g0 * p.sxt, p.sxt, c0), y(p.y, ((long long)b * p.T + g0) * p.W, p.W, c0);
+  float tap[K][V], bias[V], win[K > 1 ? K - 1 : 1][V];
+  typename ShortRow<IO, V>::Raw raw[kShortRun];
+#pragma unroll
+  for (int i = 0; i < kShortRun; ++i) raw[i] = x.request(t0 + i, it.ok && t0 + i < rows);
+  short_taps<V, K>(p, c0, tap, bias);
+  if (it.ok) short_window<IO, V, K, false>(p, b, c0, g0 + t0, win);
+#pragma unroll
+  for (int i = 0; i < kShortRun; ++i) {
+    float cur[V], out[V];
+    ShortRow<IO, V>::unpack(raw[i], cur);
+    short_token<V, K>(win, cur, tap, bias, out);
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = short_act(out[v], p.activation);
+    y.store(t0 + i, it.ok && t0 + i < rows, out);
+    short_shift<V, K>(win, cur);
+  }
+  if (K > 1 && p.new_state && it.ok && it.run == p.runs - 1) {  // the window behind the last token
+    short_window<IO, V, K, false>(p, b, c0, p.T, win);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) ShortRow<IO, V>::store((IO*)p.new_state + ((long long)b * (K - 1) + K - 2 - j) * p.W + c0, win[j]);
+  }
+}
+
+template <typename IO, int V, int K> __global__ __launch_bounds__(kShortThreads) void short_conv_dense_bwd_kernel(ShortArgs p) {
+  __shared__ float red[kShortRuns][(K + 1) * V][kShortVecs + 1];
+  const ShortItem it = short_item<V>(p);
+  const int b = it.b, c0 = it.c0, g0 = it.group * kShortRuns * p.run, t0 = it.run * p.run - g0, rows = p.T - g0;
+  const int t1 = t0 + p.run < rows ? t0 + p.run : rows;
+  const ShortBuffer<IO, V> x(p.x, b * p.sxb + (long long)g0 * p.sxt, p.sxt, c0), dy(p.dy, ((long long)b * p.T + g0) * p.W, p.W, c0);
+  const ShortBuffer<IO, V> dx(p.dx, ((long long)b * p.T + g0) * p.W, p.W, c0), dstate(p.dstate, (long long)b * (K - 1) * p.W, p.W, c0);
+  float tap[K][V], bias[V], win[K > 1 ? K - 1 : 1][V], grad[K][V], dtap[K][V], dbias[V];
+  short_taps<V, K>(p, c0, tap, bias);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    dbias[v] = 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) { dtap[j][v] = 0.f; grad[j][v] = 0.f; }
+  }
+  if (it.ok) short_window<IO, V, K, false>(p, b, c0, g0 + t0, win);
+  else
+    for (int j = 0; j < K - 1; ++j)
+      for (int v = 0; v < V; ++v) win[j][v] = 0.f;
+  // the run's outputs and the K - 1 behind it, whose upstream gradients are zeros past the row's end
+  typename ShortRow<IO, V>::Raw raw_x[kShortBatchBack], raw_d[kShortBatchBack];
+  auto request = [&](int u0) {
+#pragma unroll
+    for (int k = 0; k < kShortBatchBack; ++k) {
+      raw_x[k] = x.request(u0 + k, it.ok && u0 + k < rows);
+      raw_d[k] = dy.request(u0 + k, it.ok && u0 + k < rows);
+    }
+  };
+  request(t0);
+  for (int u0 = t0; u0 < t0 + p.run + K - 1; u0 += kShortBatchBack) {
+    float cur[kShortBatchBack][V], up[kShortBatchBack][V];
+#pragma unroll
+    for (int k = 0; k < kShortBatchBack; ++k) { ShortRow<IO, V>::unpack(raw_x[k], cur[k]); ShortRow<IO, V>::unpack(raw_d[k], up[k]); }
+    if (u0 + kShortBatchBack < t0 + p.run + K - 1) request(u0 + kShortBatchBack);
+#pragma unroll
+    for (int k = 0; k < kShortBatchBack; ++k) {
+      const int t = u0 + k, done = t - (K - 1);              // the input whose last output this is
+      float pre[V];
+      short_token<V, K>(win, cur[k], tap, bias, pre);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = up[k][v] * short_slope(pre[v], p.activation), own = t < t1 ? d : 0.f;
+#pragma unroll
+        for (int j = K - 1; j >= 1; --j) grad[j][v] = fmaf(d, tap[j][v], grad[j - 1][v]);
+        grad[0][v] = d * tap[0][v];
+        dbias[v] += own;
+        dtap[0][v] = fmaf(own, cur[k][v], dtap[0][v]);
+#pragma unroll
+        for (int j = 1; j < K; ++j) dtap[j][v] = fmaf(own, win[j - 1][v], dtap[j][v]);
+      }
+      dx.store(done, it.ok && done >= t0 && done < t1, grad[K - 1]);
+      if (K > 1 && p.dstate && it.run == 0 && t < K - 1) dstate.store(t, it.ok, grad[K - 1]);  // lag K - 1 of token t is the state's row t
+      short_shift<V, K>(win, cur[k]);
     }
   }
+  short_reduce<V, K>(p, red, dtap, dbias);
 }
 
 template <typename IO, int V, int K> __global__ __launch_bounds__(kShortThreads) void short_conv_step_kernel(ShortArgs p) {
@@ -330,24 +526,39 @@ static __global__ __launch_bounds__(256) void short_sums_kernel(SumJob j) {
 }
 
 static int short_check(const char* who, ShortArgs* a, int64_t B, int64_t T, int64_t W, int64_t K, int64_t sxb, int64_t sxt, int dtype, int vec_dtype,
-                       int activation, std::initializer_list<const void*> rows) {
+                       int activation, int run, std::initializer_list<const void*> rows) {
   if (dtype != RGLRU_F32 && dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: dtype must be RGLRU_F32 or RGLRU_BF16, got %d", who, dtype);
   if (vec_dtype != RGLRU_F32 && vec_dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "%s: unknown parameter dtype %d", who, vec_dtype);
   if (activation != RGLRU_ACT_NONE && activation != RGLRU_ACT_SILU) return fail(RGLRU_E_ARG, "%s: unknown activation %d", who, activation);
   if (B <= 0 || T <= 0 || W <= 0) return fail(RGLRU_E_ARG, "%s: sizes B=%lld T=%lld W=%lld", who, (long long)B, (long long)T, (long long)W);
   if (K < 1 || K > kShortTaps) return fail(RGLRU_E_UNSUPPORTED, "%s: kernel size %lld outside 1..%d", who, (long long)K, kShortTaps);
   memset(a, 0, sizeof(*a));
-  const int v = dtype == RGLRU_BF16 ? 8 : 4;
+  // four channels a thread: in bf16, eight leave three waves a SIMD (34.7 us forward where four take 33.7, B8 T2048 W2048)
+  const int v = 4;
   bool whole = W % v == 0 && sxb % v == 0 && sxt % v == 0;
-  for (const void* q : rows) whole = whole && (uintptr_t)q % 16 == 0;
+  for (const void* q : rows) whole = whole && (uintptr_t)q % (dtype == RGLRU_BF16 ? 8 : 16) == 0;
   if (B >= (1ll << 31) || T >= (1ll << 31) - 64 || W >= (1ll << 31)) return fail(RGLRU_E_UNSUPPORTED, "%s: tensor too large", who);
   a->sxb = sxb; a->sxt = sxt; a->B = (int)B; a->T = (int)T; a->W = (int)W; a->vec_dtype = vec_dtype; a->activation = activation;
   a->nvec = (int)(whole ? W / v : W);
-  a->runs = (int)((T + kShortRun - 1) / kShortRun);
+  a->run = run;
+  a->runs = (int)((T + run - 1) / run);
   return RGLRU_OK;
 }
-static long long short_run_groups(long long T) { return ((T + kShortRun - 1) / kShortRun + kShortRuns - 1) / kShortRuns; }
-static long long short_blocks(const ShortArgs& a) { return a.B * short_run_groups(a.T) * ((a.nvec + kShortVecs - 1) / kShortVecs); }
+static long long short_run_groups(long long runs) { return (runs + kShortRuns - 1) / kShortRuns; }
+static long long short_blocks(const ShortArgs& a) { return a.B * short_run_groups(a.runs) * ((a.nvec + kShortVecs - 1) / kShortVecs); }
+// Tokens of a run on the way back: each run reads the K - 1 tokens around it a second time, short ones fill the device with small tensors.
+static int short_run_back(int64_t B, int64_t T, int64_t W) {
+  int run = kShortRunBack;
+  while (run > 8 && B * short_run_groups((T + run - 1) / run) * ((W + 4 * kShortVecs - 1) / (4 * kShortVecs)) < 2 * num_compute_units()) run /= 2;
+  return run;
+}
+static long long short_sets(int64_t B, int64_t T, int run) { return B * short_run_groups((T + run - 1) / run); }
+
+// Whether the walks without branches take a call: a workgroup's tokens and those around them lie within 2^31 bytes.
+static bool short_dense(const ShortArgs& a, int dtype) {
+  const long long es = dtype == RGLRU_BF16 ? 2 : 4, tokens = kShortRuns * kShortRunBack + 2 * kShortTaps;
+  return !a.flags && a.sxt >= 0 && (a.sxt > a.W ? a.sxt : a.W) * es * tokens < (1ll << 31) - 4096;
+}
 
 #define RGLRU_SHORT_K(KERNEL, IO, V, ...)                                                                                          \
   switch (K) {                                                                                                                     \
@@ -358,7 +569,7 @@ static long long short_blocks(const ShortArgs& a) { return a.B * short_run_group
   }
 #define RGLRU_SHORT_LAUNCH(KERNEL, ...)                                                                                            \
   do {                                                                                                                             \
-    if (dtype == RGLRU_BF16) { if (a.nvec < a.W) { RGLRU_SHORT_K(KERNEL, __bf16, 8, __VA_ARGS__) } else { RGLRU_SHORT_K(KERNEL, __bf16, 1, __VA_ARGS__) } } \
+    if (dtype == RGLRU_BF16) { if (a.nvec < a.W) { RGLRU_SHORT_K(KERNEL, __bf16, 4, __VA_ARGS__) } else { RGLRU_SHORT_K(KERNEL, __bf16, 1, __VA_ARGS__) } } \
     else { if (a.nvec < a.W) { RGLRU_SHORT_K(KERNEL, float, 4, __VA_ARGS__) } else { RGLRU_SHORT_K(KERNEL, float, 1, __VA_ARGS__) } } \
   } while (0)
 #define RGLRU_COMMA ,
@@ -372,36 +583,40 @@ extern "C" {
 int rglru_hip_short_conv_fwd(const void* x, int64_t x_batch, int64_t x_token, const void* state, const void* taps, const void* bias, const uint8_t* flags,
                              void* y, void* new_state, int activation, int64_t B, int64_t T, int64_t W, int64_t K, int dtype, int vec_dtype, void* stream) {
   ShortArgs a;
-  int rc = short_check("short_conv_fwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, {x, state, y, new_state});
+  int rc = short_check("short_conv_fwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, kShortRun, {x, state, y, new_state});
   if (rc) return rc;
   if (!x || !taps || !y) return fail(RGLRU_E_ARG, "short_conv_fwd: null pointer");
   if (short_blocks(a) >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "short_conv_fwd: tensor too large");
   a.x = x; a.state = state; a.taps = taps; a.bias = bias; a.flags = flags; a.y = y; a.new_state = new_state;
   const dim3 grid((unsigned)short_blocks(a));
-  if (flags) RGLRU_SHORT_LAUNCH(short_conv_kernel, RGLRU_COMMA true); else RGLRU_SHORT_LAUNCH(short_conv_kernel, RGLRU_COMMA false);
+  if (flags) RGLRU_SHORT_LAUNCH(short_conv_kernel, RGLRU_COMMA true);
+  else if (short_dense(a, dtype)) RGLRU_SHORT_LAUNCH(short_conv_dense_kernel, );
+  else RGLRU_SHORT_LAUNCH(short_conv_kernel, RGLRU_COMMA false);
   return check_launch("short_conv_fwd");
 }
 
 size_t rglru_hip_short_conv_scratch_bytes(int64_t B, int64_t T, int64_t W, int64_t K) {
   if (B <= 0 || T <= 0 || W <= 0 || K < 1 || K > kShortTaps) return 0;
-  return (size_t)B * (size_t)short_run_groups(T) * (size_t)(K + 1) * (size_t)W * 4;
+  return (size_t)short_sets(B, T, short_run_back(B, T, W)) * (size_t)(K + 1) * (size_t)W * 4;
 }
 
 int rglru_hip_short_conv_bwd(const void* x, int64_t x_batch, int64_t x_token, const void* state, const void* taps, const void* bias, const uint8_t* flags,
                              const void* dy, void* scratch, void* dx, void* dstate, void* dtaps, void* dbias, int activation, int64_t B, int64_t T,
                              int64_t W, int64_t K, int dtype, int vec_dtype, int grad_dtype, void* stream) {
   ShortArgs a;
-  int rc = short_check("short_conv_bwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, {x, state, dy, dx, dstate});
+  int rc = short_check("short_conv_bwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, short_run_back(B, T, W), {x, state, dy, dx, dstate});
   if (rc) return rc;
   if (!x || !taps || !dy || !scratch || !dx) return fail(RGLRU_E_ARG, "short_conv_bwd: null pointer");
   if (grad_dtype != RGLRU_F32 && grad_dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "short_conv_bwd: unknown gradient dtype %d", grad_dtype);
   if (short_blocks(a) >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "short_conv_bwd: tensor too large");
   a.x = x; a.state = state; a.taps = taps; a.bias = bias; a.flags = flags; a.dy = dy; a.dx = dx; a.dstate = dstate; a.partial = (float*)scratch;
   const dim3 grid((unsigned)short_blocks(a));
-  if (flags) RGLRU_SHORT_LAUNCH(short_conv_bwd_kernel, RGLRU_COMMA true); else RGLRU_SHORT_LAUNCH(short_conv_bwd_kernel, RGLRU_COMMA false);
+  if (flags) RGLRU_SHORT_LAUNCH(short_conv_bwd_kernel, RGLRU_COMMA true);
+  else if (short_dense(a, dtype)) RGLRU_SHORT_LAUNCH(short_conv_dense_bwd_kernel, );
+  else RGLRU_SHORT_LAUNCH(short_conv_bwd_kernel, RGLRU_COMMA false);
   rc = check_launch("short_conv_bwd");
   if (rc || (!dtaps && !dbias)) return rc;
-  SumJob j = conv_sum_job(a.partial, dtaps, dbias, W, K, B * short_run_groups(T), grad_dtype);
+  SumJob j = conv_sum_job(a.partial, dtaps, dbias, W, K, short_sets(B, T, a.run), grad_dtype);
   plan_sum_job(j);
   hipLaunchKernelGGL(short_sums_kernel, dim3((unsigned)j.blocks), dim3(256), 0, (hipStream_t)stream, j);
   return check_launch("short_conv_bwd sums");
@@ -410,7 +625,7 @@ int rglru_hip_short_conv_bwd(const void* x, int64_t x_batch, int64_t x_token, co
 int rglru_hip_short_conv_step(const void* x, int64_t x_batch, const void* taps, const void* bias, const uint8_t* flags, void* state, void* y, int activation,
                               int64_t B, int64_t W, int64_t K, int dtype, int vec_dtype, void* stream) {
   ShortArgs a;
-  int rc = short_check("short_conv_step", &a, B, 1, W, K, x_batch, 0, dtype, vec_dtype, activation, {x, state, y});
+  int rc = short_check("short_conv_step", &a, B, 1, W, K, x_batch, 0, dtype, vec_dtype, activation, kShortRun, {x, state, y});
   if (rc) return rc;
   if (!x || !taps || !y || (K > 1 && !state)) return fail(RGLRU_E_ARG, "short_conv_step: null pointer");
   a.x = x; a.taps = taps; a.bias = bias; a.flags = flags; a.y = y; a.new_state = state;

@@ -456,6 +456,11 @@ def test_short_convolution_of_views_and_dirty_padding():
     assert (results[0][2][~active] == 0).all()
 
 
+def test_short_convolution_of_far_apart_tokens():
+    """Rows of so many channels that a run of tokens spans more than 2^31 bytes."""
+    check_conv(make_conv(1, 5, 2100001, 3))
+
+
 def test_short_convolution_by_pieces_and_tokens():
     reset, active = masks(3, 60)
     for dtype, taps in ((F32, 4), (BF16, 3), (BF16, 1)):
