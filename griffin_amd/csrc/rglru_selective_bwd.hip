@@ -168,7 +168,6 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
         sums[decltype(token)::value] = bcast_dot<t>(C, h[t]);
       });
       gates[wave][4 * decltype(group)::value + j][c][2] = four_rows_sum(sums);
-      __builtin_amdgcn_sched_barrier(0);
     });
     // other names for B and C: broadcasts of theirs that the way back shared with the way there would each keep a register
 #pragma unroll
@@ -187,6 +186,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       BufIo<IO>::store((IO)dt_out, SelStream<IO>::tile(p.ddt, place, (unsigned)p.W, left), off, 0);
       if (gated) BufIo<IO>::store((IO)(live ? gate[1] * fmaf(skip, rate[3], y_all ? *y_all : gate[2]) : 0.f), SelStream<IO>::tile(p.dz, place, (unsigned)p.W, left), off, 0);
     };
+    if (tile > first) request(tile - 1);                    // the next tile's, as early as registers allow
     sel_each<4>([&](auto back) {
       constexpr int g4 = 3 - decltype(back)::value;
       float dB[4][4], dC[4][4], sum_b[4], sum_a[4];
@@ -223,8 +223,6 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
         float (*mem)[4][64] = parts[tile & 1][wave];
         mem[0][g4][lane] = along; mem[1][g4][lane] = through; mem[2][g4][lane] = gates[wave][4 * g4 + j][c][2];
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (g4 == 2 && tile > first) request(tile - 1);        // half of the decays and states are through: their registers are free
     });
     __syncthreads();                                        // the other buffer's readers are past the barrier before
     if constexpr (SLABS > 1) {
