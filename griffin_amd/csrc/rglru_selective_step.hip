@@ -103,18 +103,23 @@ template <typename IO, bool WHOLE, bool PAST> __global__ __launch_bounds__(kSelT
 
 static size_t sel_bytes(long long floats) { return ((size_t)floats * 4 + 255) & ~(size_t)255; }
 
-// Segments of a sequence, by a time estimate.  A compute unit holds two workgroups at a time; one alone leaves each SIMD one wave, which issues an
-// instruction in 5.3 cycles where two take 6.2 for one each.  Walking in segments adds `again` of the work in all segments but one.
-static int sel_segments(long long wgs, long long tiles, double again) {
+// Segments of a sequence, by a time estimate in microseconds.  A compute unit holds two workgroups at a time and takes `two` a tile of each with both, `one`
+// with one of them (measured: 0.8 and 0.5 forward, 7.8 and 5.5 back).  In segments, all but one are summarised first: a launch of 6, a tile's summary 1.2 on
+// a SIMD that has no other work and 1.27 / 4 of a unit's time where all have, and 0.25 for each segment that the others are joined from.
+static int sel_segments(long long wgs, long long waves, long long tiles, double two, double one) {
   const long long units = num_compute_units();
   int best = 1;
   double least = 0.;
-  for (long long s = 1; s <= kSelMaxSegments && (s == 1 || s <= tiles / 4); ++s) {
+  for (long long s = 1; s <= kSelMaxSegments && s <= tiles; ++s) {
     const long long each = (tiles + s - 1) / s;
     if ((tiles + each - 1) / each != s) continue;            // the same segments as fewer
     const long long all = wgs * s, full = all / (2 * units), rest = all - full * 2 * units;
-    const double rounds = 6.2 * (double)full + (rest > units ? 6.2 : rest > 0 ? 5.3 : 0.), time = rounds * (double)each * (1. + again * (double)(s - 1) / (double)s);
-    if (s == 1 || time < 0.97 * least) { best = (int)s; least = time; }
+    double time = (double)each * (two * (double)full + (rest > units ? two : rest > 0 ? one : 0.));
+    if (s > 1) {
+      const double filled = 1.27 * (double)(waves * each * (s - 1)) / (4. * (double)units), alone = 1.2 * (double)(each < 4 ? each : 4);
+      time += 6. + 0.25 * (double)s + (filled > alone ? filled : alone);
+    }
+    if (s == 1 || time < least) { best = (int)s; least = time; }
   }
   return best;
 }
@@ -129,12 +134,11 @@ static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int
   a->tiles = (int)((T + kSelTile - 1) / kSelTile);
   const long long wgs = B * G * (backward ? a->per_group : a->pipe_group);
   if (wgs >= (1ll << 24) || (long long)G * N >= (1ll << 22)) return false;
-  // a summary's share of a walk's instructions
-  a->S = sel_segments(wgs, a->tiles, backward ? 0.27 : 0.6);
+  a->S = sel_segments(wgs, B * G * columns * slabs, a->tiles, backward ? 7.8 : 0.8, backward ? 5.5 : 0.5);
   a->seg_tiles = (a->tiles + a->S - 1) / a->S;
-  // the summary is a short walk of few registers, which fills the device with six waves a SIMD
+  // the summary is a short walk of few registers: more and shorter ones until four waves share a SIMD
   const long long summaries = B * G * (long long)a->per_group * (a->S - 1), most = a->seg_tiles / 4;
-  long long parts = summaries > 0 ? 6ll * num_compute_units() / summaries : 1;
+  long long parts = summaries > 0 ? 4ll * num_compute_units() / summaries : 1;
   if (parts > most) parts = most;
   if (parts > kSelMaxSegments / a->S) parts = kSelMaxSegments / a->S;
   a->parts = (int)(parts < 1 ? 1 : parts);
