@@ -167,6 +167,8 @@ static int sel_strides(const char* who, SelArgs* a, const int64_t* s, int dtype)
   const int64_t tokens[5] = {s[1], s[3], s[5], s[7], s[10]};
   for (int64_t t : tokens)
     if (t < 0 || t >= (1 << 22)) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens %lld elements apart", who, (long long)t);
+  for (int i = 0; i < 3; ++i)                                // a tile's buffer ends where the token behind it would begin
+    if (tokens[i] != 0 && tokens[i] < a->W) return fail(RGLRU_E_UNSUPPORTED, "%s: tokens of %d elements lie %lld apart", who, a->W, (long long)tokens[i]);
   a->sub = s[0]; a->sut = s[1]; a->sdb = s[2]; a->sdt = s[3]; a->szb = s[4]; a->szt = s[5];
   a->sBb = s[6]; a->sBt = s[7]; a->sBg = s[8]; a->sCb = s[9]; a->sCt = s[10]; a->sCg = s[11];
   bool whole = true;

@@ -2389,15 +2389,20 @@ struct SelectiveOperands {
   int64_t strides[12];
   // an axis of one element has no distance, whatever its tensor says
   static int64_t distance(const Tensor& t, int64_t axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); }
-  static Tensor rows(const Tensor& t, int64_t token_axis) {
+  // `apart`: tokens that lie less than their width apart overlap, and are copied
+  static Tensor rows(const Tensor& t, bool sequence, bool apart) {
     if (!t.defined()) return t;
-    const bool plain = t.stride(-1) == 1 || t.size(-1) == 1;
-    return plain && (token_axis < 0 || distance(t, token_axis) < (int64_t(1) << 22)) ? t : t.contiguous();
+    bool plain = t.stride(-1) == 1 || t.size(-1) == 1;
+    if (sequence) {
+      const int64_t step = distance(t, 1);
+      plain = plain && step < (int64_t(1) << 22) && (!apart || step == 0 || step >= t.size(-1));
+    }
+    return plain ? t : t.contiguous();
   }
   SelectiveOperands(const Tensor& u_in, const Tensor& dt_in, const Tensor& z_in, const Tensor& B_in, const Tensor& C_in, const Tensor& A_in,
                     const Tensor& D_in, const Tensor& bias_in, bool sequence)
-      : u(rows(u_in, sequence ? 1 : -1)), dt(rows(dt_in, sequence ? 1 : -1)), z(rows(z_in, sequence ? 1 : -1)), B(rows(B_in, sequence ? 1 : -1)),
-        C(rows(C_in, sequence ? 1 : -1)), A(as(A_in, at::kFloat)), D(as(D_in, at::kFloat)), bias(as(bias_in, at::kFloat)) {
+      : u(rows(u_in, sequence, true)), dt(rows(dt_in, sequence, true)), z(rows(z_in, sequence, true)), B(rows(B_in, sequence, false)),
+        C(rows(C_in, sequence, false)), A(as(A_in, at::kFloat)), D(as(D_in, at::kFloat)), bias(as(bias_in, at::kFloat)) {
     distances(sequence);
   }
   SelectiveOperands(const variable_list& s) : u(s[0]), dt(s[1]), z(s[2]), B(s[3]), C(s[4]), A(s[5]), D(s[6]), bias(s[7]) { distances(true); }

@@ -138,6 +138,22 @@ def test_views_are_taken():
     assert hip_add_rmsnorm_quantised(torch.zeros(0, 64, device="cuda"), None, g)[1].shape == (0, 1)
 
 
+def test_more_elements_than_32_bits_address():
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x, r = (torch.empty(300000, 8192, device="cuda", dtype=BF16).normal_(generator=gen) for _ in range(2))
+    g = torch.randn(8192, device="cuda", generator=gen).to(BF16)
+    leaves = [x.requires_grad_(True), r.requires_grad_(True), g]
+    y, total = hip_add_rmsnorm(*leaves)
+    dx, dr = torch.autograd.grad(y, leaves[:2], x.detach())
+    part = [t.detach()[-5:].clone().requires_grad_(True) for t in (x, r)]
+    want, want_total = hip_add_rmsnorm(*part, g)
+    assert torch.equal(y[-5:], want) and torch.equal(total[-5:], want_total)
+    assert torch.equal(dr[-5:], torch.autograd.grad(want, part, part[0].detach())[1]) and torch.equal(dx, dr)
+    q, scale, _ = hip_add_rmsnorm_quantised(x.detach(), r.detach(), g)
+    few = hip_add_rmsnorm_quantised(part[0].detach(), part[1].detach(), g)
+    assert torch.equal(q[-5:].view(torch.uint8), few[0].view(torch.uint8)) and torch.equal(scale[-5:], few[1])
+
+
 @pytest.mark.parametrize("error, call", [
     (ValueError, lambda x, g: hip_add_rmsnorm(x, x[:3], g)),
     (ValueError, lambda x, g: hip_add_rmsnorm(x, x, g[:5])),

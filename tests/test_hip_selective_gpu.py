@@ -282,6 +282,66 @@ def test_parts_of_one_projection(dtype):
         assert torch.equal(*y)
 
 
+def test_tokens_that_overlap():
+    """Windows over one row of numbers: each token lies a few elements behind the one before."""
+    case = {n: put(t) for n, t in make(2, 40, 20, 1, 8).items()}
+    line = torch.randn(2, 400, generator=torch.Generator().manual_seed(1)).cuda()
+    for name in ("u", "dt", "z"):
+        case[name] = line.as_strided((2, 40, 20), (400, 3, 1))
+    for name in ("B", "C"):
+        case[name] = line.as_strided((2, 40, 1, 8), (400, 5, 1, 1))
+    views = run(hip_selective_scan, case, "cuda")
+    dense = run(hip_selective_scan, {n: t.contiguous() for n, t in case.items()}, "cuda")
+    assert torch.equal(views[0], dense[0]) and torch.equal(views[1], dense[1]) and all(torch.equal(views[2][n], dense[2][n]) for n in dense[2])
+    conv = make_conv(2, 40, 20, 4)
+    args = [put(conv[n]) for n in ("weight", "bias", "state")]
+    assert torch.equal(hip_short_conv(case["u"], *args, "silu")[0], hip_short_conv(case["u"].contiguous(), *args, "silu")[0])
+
+
+def test_more_elements_than_32_bits_address():
+    """2.4e9 elements a tensor, more than 2^31 bytes of kept states: the last document alone gives the same."""
+    steps, width, states, tail = 40000, 60000, 4, 20
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    wide = lambda: torch.randn(1, steps, width, device="cuda", dtype=BF16, generator=gen)
+    u, dt = wide(), wide()
+    few = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)
+    A, B, C = -few(width, states).abs(), few(1, steps, 1, states).to(BF16), few(1, steps, 1, states).to(BF16)
+    weight, window = few(width, 1, 4).to(BF16), None
+    reset = torch.zeros(1, steps, dtype=torch.bool, device="cuda")
+    reset[0, -tail] = True
+    leaves = [t.requires_grad_(True) for t in (u, dt, A, B, C)]
+    up = torch.zeros_like(u)
+    up[:, -tail:] = 1
+    y, last = hip_selective_scan(*leaves, reset_mask=reset)
+    grads = torch.autograd.grad(y, leaves, up)
+    part = [t.detach()[:, -tail:].clone().requires_grad_(True) if t.dim() > 2 else t.detach().requires_grad_(True) for t in leaves]
+    want, want_last = hip_selective_scan(*part)
+    want_grads = torch.autograd.grad(want, part, up[:, -tail:])
+    # the same tokens in tiles that begin elsewhere: both within the bound
+    assert rel_err(y[:, -tail:], want) <= 2 * bound(BF16, tail) and rel_err(last, want_last) <= 2 * bound(F32, tail)
+    for i, (g, w) in enumerate(zip(grads, want_grads)):
+        assert rel_err(g[:, -tail:] if g.dim() > 2 else g, w) <= 2 * bound(g.dtype, tail, True), i
+        assert g.dim() == 2 or not g[:, : -tail].any()
+    del y, grads, up
+    out, _ = hip_short_conv(u.detach(), weight, None, window, "silu", reset)
+    tail_out, _ = hip_short_conv(u.detach()[:, -tail:], weight, None, window, "silu")
+    assert torch.equal(out[:, -tail:], tail_out)
+    dense, behind = hip_short_conv(u.detach(), weight)
+    assert torch.equal(dense[:, -tail + 3:], hip_short_conv(u.detach()[:, -tail:], weight)[0][:, 3:]) and torch.equal(behind, u.detach()[:, -3:])
+
+
+def test_states_of_more_elements_than_32_bits_address():
+    rows, width, states = 3000, 12000, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    few = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)
+    state = torch.empty(rows, width, states, device="cuda").normal_(generator=gen)
+    u, dt, A, B, C = few(rows, width), few(rows, width), -few(width, states).abs(), few(rows, 1, states), few(rows, 1, states)
+    last = state[-2:].clone()
+    want = hip_selective_step(u[-2:], dt[-2:], A, B[-2:], C[-2:], last)
+    got = hip_selective_step(u, dt, A, B, C, state)
+    assert torch.equal(got[-2:], want) and torch.equal(state[-2:], last)
+
+
 def test_gradients_of_parameters_in_half_precision_and_of_one_output():
     case = make(2, 40, 20, 1, 16, dtype=BF16)
     half = {n: (t.bfloat16() if n in ("A", "D", "dt_bias", "h0") else t) for n, t in case.items()}

@@ -71,6 +71,7 @@ def norm_bwd(lib, sizes=(3, 8), types=(F32, F32, F32, F32), scratch=FAKE):
     (lambda lib: scan_fwd(lib, ws=None), ARG, b"null"),
     (lambda lib: scan_fwd(lib, strides=(ctypes.c_int64 * 12)(64, 1 << 22, *[64, 8] * 2, *[64, 8, 4] * 2)), UNSUPPORTED, b"apart"),
     (lambda lib: scan_fwd(lib, strides=(ctypes.c_int64 * 12)(*[64, 8] * 3, 64, -8, 4, 64, 8, 4)), UNSUPPORTED, b"apart"),
+    (lambda lib: scan_fwd(lib, strides=(ctypes.c_int64 * 12)(64, 7, *[64, 8] * 2, *[64, 8, 4] * 2)), UNSUPPORTED, b"apart"),
     (lambda lib: scan_fwd(lib, sizes=(1 << 24, 5, 8, 1, 4)), UNSUPPORTED, b"too large"),
     (lambda lib: scan_fwd(lib, sizes=(2, 1 << 31, 8, 1, 4)), UNSUPPORTED, b"too large"),
     (lambda lib: scan_fwd(lib, sizes=(2, 5, 1 << 22, 1, 4)), UNSUPPORTED, b"too large"),
