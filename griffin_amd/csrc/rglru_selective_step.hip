@@ -209,6 +209,7 @@ int rglru_hip_selective_fwd(const void* u, const void* dt, const void* z, const 
   int rc = sel_check("selective_fwd", &a, B, T, W, G, N, dtype, false);
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !y || !h_last || !ws) return fail(RGLRU_E_ARG, "selective_fwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "selective_fwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.A = A; a.D = D; a.bias = bias; a.h0 = h0; a.flags = flags; a.y = y; a.h_last = h_last;
   a.softplus = softplus;
   rc = sel_strides("selective_fwd", &a, strides, dtype);
@@ -229,6 +230,7 @@ int rglru_hip_selective_bwd(const void* u, const void* dt, const void* z, const 
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !dout || !ws || !scratch || !du || !ddt || (z && !dz) || !dB || !dC)
     return fail(RGLRU_E_ARG, "selective_bwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "selective_bwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.A = A; a.D = D; a.bias = bias; a.flags = flags; a.dout = dout; a.dh_last = dh_last;
   a.du = du; a.ddt = ddt; a.dz = dz; a.dh0 = dh0; a.softplus = softplus;
   rc = sel_strides("selective_bwd", &a, strides, dtype);
@@ -253,6 +255,7 @@ int rglru_hip_selective_step(const void* u, const void* dt, const void* z, const
   int rc = sel_check("selective_step", &a, B, 1, W, G, N, dtype, false);
   if (rc) return rc;
   if (!u || !dt || !Bm || !Cm || !strides || !A || !state || !y) return fail(RGLRU_E_ARG, "selective_step: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "selective_step: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   SelStepArgs p;
   memset(&p, 0, sizeof(p));
   p.u = u; p.dt = dt; p.z = z; p.Bm = Bm; p.Cm = Cm; p.A = A; p.D = D; p.bias = bias; p.flags = flags; p.state = state; p.y = y;

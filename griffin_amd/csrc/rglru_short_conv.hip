@@ -586,6 +586,7 @@ int rglru_hip_short_conv_fwd(const void* x, int64_t x_batch, int64_t x_token, co
   int rc = short_check("short_conv_fwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, kShortRun, {x, state, y, new_state});
   if (rc) return rc;
   if (!x || !taps || !y) return fail(RGLRU_E_ARG, "short_conv_fwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "short_conv_fwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   if (short_blocks(a) >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "short_conv_fwd: tensor too large");
   a.x = x; a.state = state; a.taps = taps; a.bias = bias; a.flags = flags; a.y = y; a.new_state = new_state;
   const dim3 grid((unsigned)short_blocks(a));
@@ -607,6 +608,7 @@ int rglru_hip_short_conv_bwd(const void* x, int64_t x_batch, int64_t x_token, co
   int rc = short_check("short_conv_bwd", &a, B, T, W, K, x_batch, x_token, dtype, vec_dtype, activation, short_run_back(B, T, W), {x, state, dy, dx, dstate});
   if (rc) return rc;
   if (!x || !taps || !dy || !scratch || !dx) return fail(RGLRU_E_ARG, "short_conv_bwd: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "short_conv_bwd: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   if (grad_dtype != RGLRU_F32 && grad_dtype != RGLRU_BF16) return fail(RGLRU_E_ARG, "short_conv_bwd: unknown gradient dtype %d", grad_dtype);
   if (short_blocks(a) >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "short_conv_bwd: tensor too large");
   a.x = x; a.state = state; a.taps = taps; a.bias = bias; a.flags = flags; a.dy = dy; a.dx = dx; a.dstate = dstate; a.partial = (float*)scratch;
@@ -628,6 +630,7 @@ int rglru_hip_short_conv_step(const void* x, int64_t x_batch, const void* taps, 
   int rc = short_check("short_conv_step", &a, B, 1, W, K, x_batch, 0, dtype, vec_dtype, activation, kShortRun, {x, state, y});
   if (rc) return rc;
   if (!x || !taps || !y || (K > 1 && !state)) return fail(RGLRU_E_ARG, "short_conv_step: null pointer");
+  if (flags == RGLRU_FLAGS_FIRST_RESET) return fail(RGLRU_E_ARG, "short_conv_step: RGLRU_FLAGS_FIRST_RESET is not a flag array");
   a.x = x; a.taps = taps; a.bias = bias; a.flags = flags; a.y = y; a.new_state = state;
   const long long blocks = (B * (long long)a.nvec + kShortThreads - 1) / kShortThreads;
   if (blocks >= (1ll << 24)) return fail(RGLRU_E_UNSUPPORTED, "short_conv_step: tensor too large");

@@ -424,7 +424,7 @@ int rglru_hip_group_norm_bwd(const void* x, const void* weight, const void* bias
  *   y_t = (sum over n of C_t[n] h_t[n] + D u_t) silu(z_t)          (z NULL: without the gate; D, bias NULL: zeros)
  * u, dt, z [B, T, W] and B, C [B, T, G, N] in `dtype`, their last axes contiguous; `strides`: elements between u's batch rows and tokens, dt's, z's,
  * then B's batch rows, tokens and groups and C's (tokens less than 2^22 elements apart, those of u, dt and z at least W or 0: one token for all).  y, dout and all gradients dense.  A [W, N], D, bias [W], states
- * [B, W, N] fp32.  `flags`: one byte a token or NULL, bit 0 = starts a document, bit 1 = inactive: the state stays, the output and the token's gradients are
+ * [B, W, N] fp32.  `flags`: one byte a token or NULL (not RGLRU_FLAGS_FIRST_RESET), bit 0 = starts a document, bit 1 = inactive: the state stays, the output and the token's gradients are
  * zero, whatever it holds.  N up to rglru_hip_selective_max_states().
  *   ws       rglru_hip_selective_workspace_bytes(..., keep) bytes, 16-byte aligned: with `keep` the state in front of every 16 tokens, which the backward call
  *            reads and leaves as it is

@@ -11,6 +11,7 @@ from griffin_amd import (_lib, hip_add_rmsnorm, hip_add_rmsnorm_quantised, hip_s
 
 F32, BF16, ARG, UNSUPPORTED = _lib.RGLRU_F32, _lib.RGLRU_BF16, 1, 2
 FAKE = ctypes.c_void_p(256)                                  # never dereferenced: the checks come first
+FIRST_RESET = ctypes.c_void_p(1)                             # a sentinel of other entry points, in place of flags
 STRIDES = (ctypes.c_int64 * 12)(*[64, 8] * 3, *[64, 8, 4] * 2)
 
 
@@ -23,29 +24,29 @@ def lib():
     return _lib.load()
 
 
-def scan_fwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, u=FAKE, ws=FAKE, strides=STRIDES):
-    return lib.rglru_hip_selective_fwd(u, FAKE, None, FAKE, FAKE, strides, FAKE, None, None, None, None, FAKE, FAKE, ws, 0, 1, *sizes, dtype, None)
+def scan_fwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, u=FAKE, ws=FAKE, strides=STRIDES, flags=None):
+    return lib.rglru_hip_selective_fwd(u, FAKE, None, FAKE, FAKE, strides, FAKE, None, None, None, flags, FAKE, FAKE, ws, 0, 1, *sizes, dtype, None)
 
 
-def scan_bwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, z=None, scratch=FAKE):
-    return lib.rglru_hip_selective_bwd(FAKE, FAKE, z, FAKE, FAKE, STRIDES, FAKE, None, None, None, FAKE, None, FAKE, scratch, FAKE, FAKE, None, FAKE, FAKE, None,
+def scan_bwd(lib, sizes=(2, 5, 8, 2, 4), dtype=F32, z=None, scratch=FAKE, flags=None):
+    return lib.rglru_hip_selective_bwd(FAKE, FAKE, z, FAKE, FAKE, STRIDES, FAKE, None, None, flags, FAKE, None, FAKE, scratch, FAKE, FAKE, None, FAKE, FAKE, None,
                                        None, None, None, 1, *sizes, dtype, None)
 
 
-def scan_step(lib, sizes=(2, 8, 2, 4), dtype=F32, state=FAKE):
-    return lib.rglru_hip_selective_step(FAKE, FAKE, None, FAKE, FAKE, STRIDES, FAKE, None, None, None, state, FAKE, 1, *sizes, dtype, None)
+def scan_step(lib, sizes=(2, 8, 2, 4), dtype=F32, state=FAKE, flags=None):
+    return lib.rglru_hip_selective_step(FAKE, FAKE, None, FAKE, FAKE, STRIDES, FAKE, None, None, flags, state, FAKE, 1, *sizes, dtype, None)
 
 
-def conv_fwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32), activation=1, x=FAKE):
-    return lib.rglru_hip_short_conv_fwd(x, 40, 8, None, FAKE, None, None, FAKE, None, activation, *sizes, *types, None)
+def conv_fwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32), activation=1, x=FAKE, flags=None):
+    return lib.rglru_hip_short_conv_fwd(x, 40, 8, None, FAKE, None, flags, FAKE, None, activation, *sizes, *types, None)
 
 
-def conv_bwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32, F32), activation=1, scratch=FAKE):
-    return lib.rglru_hip_short_conv_bwd(FAKE, 40, 8, None, FAKE, None, None, FAKE, scratch, FAKE, None, None, None, activation, *sizes, *types, None)
+def conv_bwd(lib, sizes=(2, 5, 8, 4), types=(F32, F32, F32), activation=1, scratch=FAKE, flags=None):
+    return lib.rglru_hip_short_conv_bwd(FAKE, 40, 8, None, FAKE, None, flags, FAKE, scratch, FAKE, None, None, None, activation, *sizes, *types, None)
 
 
-def conv_step(lib, sizes=(2, 8, 4), types=(F32, F32), state=FAKE):
-    return lib.rglru_hip_short_conv_step(FAKE, 8, FAKE, None, None, state, FAKE, 1, *sizes, *types, None)
+def conv_step(lib, sizes=(2, 8, 4), types=(F32, F32), state=FAKE, flags=None):
+    return lib.rglru_hip_short_conv_step(FAKE, 8, FAKE, None, flags, state, FAKE, 1, *sizes, *types, None)
 
 
 def norm_fwd(lib, sizes=(3, 8), types=(F32, F32, F32), residual=FAKE):
@@ -94,6 +95,12 @@ def norm_bwd(lib, sizes=(3, 8), types=(F32, F32, F32, F32), scratch=FAKE):
     (lambda lib: conv_bwd(lib, types=(F32, F32, 9)), ARG, b"gradient dtype"),
     (lambda lib: conv_step(lib, state=None), ARG, b"null"),
     (lambda lib: conv_step(lib, sizes=(0, 8, 4)), ARG, b"sizes"),
+    (lambda lib: scan_fwd(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
+    (lambda lib: scan_bwd(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
+    (lambda lib: scan_step(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
+    (lambda lib: conv_fwd(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
+    (lambda lib: conv_bwd(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
+    (lambda lib: conv_step(lib, flags=FIRST_RESET), ARG, b"FIRST_RESET"),
     (lambda lib: norm_fwd(lib, sizes=(3, 16385)), UNSUPPORTED, b"exceed"),
     (lambda lib: norm_fwd(lib, sizes=(0, 8)), ARG, b"sizes"),
     (lambda lib: norm_fwd(lib, types=(F32, 5, F32)), ARG, b"dtype"),
