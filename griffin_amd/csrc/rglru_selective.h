@@ -165,6 +165,16 @@ RGLRU_DEVICE SelRate sel_rate(float x, bool soft) {
   return r;
 }
 
+// Where a row's operands begin, and what lies in front of a token: with one product of 32 bits a tile and operand, the addresses leave the scalar registers to
+// the masks (made from the batch row for every tile, they took 46 more moves out of spilled ones in the gradient kernel's loop).
+template <typename IO> struct SelRows {
+  const IO *u, *dt, *z, *d, *B, *C;
+  RGLRU_DEVICE SelRows(const SelArgs& p, const SelPlace& at)
+      : u((const IO*)p.u + at.b * p.sub), dt((const IO*)p.dt + at.b * p.sdb), z((const IO*)p.z + at.b * p.szb), d((const IO*)p.dout + (long long)at.b * p.T * p.W),
+        B((const IO*)p.Bm + at.b * p.sBb + at.g * p.sBg), C((const IO*)p.Cm + at.b * p.sCb + at.g * p.sCg) {}
+};
+RGLRU_DEVICE long long sel_tokens(int t0, long long stride) { return (long long)((unsigned long long)(unsigned)t0 * (unsigned)stride); }
+
 // One operand of u's shape, a channel a lane: tokens t0 + 4 q + j of a tile (q = 0 .. 3) as they lie in memory, so that nothing waits for them before they
 // are used.  The buffer ends with the tile's last token; lanes without a channel ask behind it.
 template <typename IO> struct SelStream {

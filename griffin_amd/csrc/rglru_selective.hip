@@ -28,30 +28,29 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   const unsigned channel = SelStream<IO>::channel(w, ok);
   SelStream<IO> next_u, next_dt;
   SelVector<IO, WHOLE> next_B;
+  const SelRows<IO> rows(p, at);
   auto request = [&](int tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
-    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
+    next_dt.load(rows.dt, sel_tokens(t0, p.sdt), (unsigned)p.sdt, left, channel, j);
+    next_u.load(rows.u, sel_tokens(t0, p.sut), (unsigned)p.sut, left, channel, j);
+    next_B.load(rows.B, sel_tokens(t0, p.sBt), (unsigned)p.sBt, n0, p.N, left, c);
   };
   if (first < last) request(first);
   sel_arrived();
   float total = 0.f;
   bool cut = false;
   for (int tile = first; tile < last; ++tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
     float B[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool live = (m.live >> (4 * q + j)) & 1u;
       const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f;
-      rates[wave][4 * q + j][c] = make_float2(s, live ? s * next_u[q] : 0.f);
+      rates[wave][4 * q + j][c] = make_float2(s, !MASKED || live ? s * next_u[q] : 0.f);
       total += s;
     }
-    next_B.get(B, (m.live >> c) & 1u);
+    next_B.get(B, !MASKED || (m.live >> c) & 1u);
     wave_order();
     if (tile + 1 < last) request(tile + 1);
     if (MASKED) cut = cut || m.starts;
@@ -105,32 +104,32 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
   const bool gated = p.z != nullptr;
   SelStream<IO> next_u, next_dt, next_z;
   SelVector<IO, WHOLE> next_B, next_C;
+  const SelRows<IO> rows(p, at);
+  const long long row_place = (long long)at.b * p.T * p.W;
   auto request = [&](int tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
-    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
-    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
+    next_dt.load(rows.dt, sel_tokens(t0, p.sdt), (unsigned)p.sdt, left, channel, j);
+    next_u.load(rows.u, sel_tokens(t0, p.sut), (unsigned)p.sut, left, channel, j);
+    next_B.load(rows.B, sel_tokens(t0, p.sBt), (unsigned)p.sBt, n0, p.N, left, c);
+    next_C.load(rows.C, sel_tokens(t0, p.sCt), (unsigned)p.sCt, n0, p.N, left, c);
+    next_z.load(rows.z, sel_tokens(t0, p.szt), (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
   };
   if (first + at.turn < last) request(first + at.turn);
   sel_arrived();
   for (int tile = first + at.turn; tile < last; tile += PIPE) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
     float u[4], gate[4], B[4], C[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool live = (m.live >> (4 * q + j)) & 1u;
       const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f, z = next_z[q];
-      u[q] = live ? next_u[q] : 0.f;
+      u[q] = !MASKED || live ? next_u[q] : 0.f;             // (behind the end: zeros, or the token that all share, with a step size of zero)
       gate[q] = gated ? z * sigmoid_fast(z) : 1.f;
       rates[wave][4 * q + j][c] = make_float2(s, s * u[q]);
     }
-    next_B.get(B, (m.live >> c) & 1u);
-    next_C.get(C, (m.live >> c) & 1u);
+    next_B.get(B, !MASKED || (m.live >> c) & 1u);
+    next_C.get(C, !MASKED || (m.live >> c) & 1u);
     wave_order();
     if (tile + PIPE < last) request(tile + PIPE);
     float a[kSelTile][4], x[kSelTile][4];
@@ -202,9 +201,9 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
     for (int q = 0; q < 4; ++q) {
       float out = fmaf(skip, u[q], y[q]) * gate[q];
       sel_made(out);                                        // no branch around it
-      y[q] = (m.live >> (4 * q + j)) & 1u ? out : 0.f;
+      y[q] = !MASKED || (m.live >> (4 * q + j)) & 1u ? out : 0.f;
     }
-    if (SLABS == 1 || at.slab == 0) sel_store<IO>(y, p.y, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
+    if (SLABS == 1 || at.slab == 0) sel_store<IO>(y, p.y, row_place + sel_tokens(t0, p.W), (unsigned)p.W, left, channel, j);
   }
   if ((last - 1 - first) % PIPE == at.turn && at.seg == p.S - 1) sel_store_states(p.h_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
 }

@@ -39,21 +39,20 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   const unsigned channel = SelStream<IO>::channel(w, ok);
   SelStream<IO> next_dt, next_z, next_d;
   SelVector<IO, WHOLE> next_C;
+  const SelRows<IO> rows(p, at);
   auto request = [&](int tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
-    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
+    next_dt.load(rows.dt, sel_tokens(t0, p.sdt), (unsigned)p.sdt, left, channel, j);
+    next_d.load(rows.d, sel_tokens(t0, p.W), (unsigned)p.W, left, channel, j);
+    next_z.load(rows.z, sel_tokens(t0, p.szt), (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
+    next_C.load(rows.C, sel_tokens(t0, p.sCt), (unsigned)p.sCt, n0, p.N, left, c);
   };
   if (first < last) request(last - 1);
   sel_arrived();
   float total = 0.f;
   bool cut = false;
   for (int tile = last - 1; tile >= first; --tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
     float C[4];
 #pragma unroll
@@ -61,11 +60,10 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       const bool live = (m.live >> (4 * q + j)) & 1u;
       const float rate = sel_rate(next_dt[q] + bias, p.softplus).s, s = live ? rate : 0.f, z = next_z[q];
       const float dy = next_d[q] * (gated ? z * sigmoid_fast(z) : 1.f);
-      rates[wave][4 * q + j][c] = make_float2(s, live ? dy : 0.f);
+      rates[wave][4 * q + j][c] = make_float2(s, !MASKED || live ? dy : 0.f);
       total += s;
     }
-    const bool mine = (m.live >> c) & 1u;
-    next_C.get(C, mine);
+    next_C.get(C, !MASKED || (m.live >> c) & 1u);
     wave_order();
     if (tile > first) request(tile - 1);
     if (MASKED) cut = cut || m.starts;
@@ -117,22 +115,24 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   SelStream<IO> next_u, next_dt, next_z, next_d;
   SelVector<IO, WHOLE> next_B, next_C;
   SelStates<WHOLE> next_h;
+  const SelRows<IO> rows(p, at);
+  const float* row_h = p.kept + (long long)at.b * p.tiles * p.W * p.N;
+  const long long row_place = (long long)at.b * p.T * p.W;
   auto request = [&](int tile) {
-    const long long t0 = (long long)tile * kSelTile;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
-    next_dt.load(p.dt, at.b * p.sdb + t0 * p.sdt, (unsigned)p.sdt, left, channel, j);
-    next_u.load(p.u, at.b * p.sub + t0 * p.sut, (unsigned)p.sut, left, channel, j);
-    next_d.load(p.dout, ((long long)at.b * p.T + t0) * p.W, (unsigned)p.W, left, channel, j);
-    next_z.load(p.z, at.b * p.szb + t0 * p.szt, (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
-    next_B.load(p.Bm, at.b * p.sBb + t0 * p.sBt + at.g * p.sBg, (unsigned)p.sBt, n0, p.N, left, c);
-    next_C.load(p.Cm, at.b * p.sCb + t0 * p.sCt + at.g * p.sCg, (unsigned)p.sCt, n0, p.N, left, c);
-    next_h.load(SelStates<WHOLE>::rows(p.kept, ((long long)at.b * p.tiles + tile) * p.W, p.W, p.N), lane_h, n0, p.N);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
+    next_dt.load(rows.dt, sel_tokens(t0, p.sdt), (unsigned)p.sdt, left, channel, j);
+    next_u.load(rows.u, sel_tokens(t0, p.sut), (unsigned)p.sut, left, channel, j);
+    next_d.load(rows.d, sel_tokens(t0, p.W), (unsigned)p.W, left, channel, j);
+    next_z.load(rows.z, sel_tokens(t0, p.szt), (unsigned)p.szt, left, gated ? channel : kOutOfRange, j);
+    next_B.load(rows.B, sel_tokens(t0, p.sBt), (unsigned)p.sBt, n0, p.N, left, c);
+    next_C.load(rows.C, sel_tokens(t0, p.sCt), (unsigned)p.sCt, n0, p.N, left, c);
+    next_h.load(SelStates<WHOLE>::rows(row_h, sel_tokens(tile, p.W), p.W, p.N), lane_h, n0, p.N);
   };
   request(last - 1);
   sel_arrived();
   for (int tile = last - 1; tile >= first; --tile) {
-    const long long t0 = (long long)tile * kSelTile, place = ((long long)at.b * p.T + t0) * p.W;
-    const int left = (int)(p.T - t0 < kSelTile ? p.T - t0 : kSelTile);
+    const int t0 = tile * kSelTile, left = p.T - t0 < kSelTile ? p.T - t0 : kSelTile;
+    const long long place = row_place + sel_tokens(t0, p.W);
     const SelMasks m = sel_masks<MASKED>(p.flags, (long long)at.b * p.T + t0, left, lane);
     float B[4], C[4], before[4];
 #pragma unroll
@@ -140,13 +140,15 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       const bool live = (m.live >> (4 * q + j)) & 1u;
       const SelRate rate = sel_rate(next_dt[q] + bias, p.softplus);
       const float z = next_z[q], sig = sigmoid_fast(z);
-      const float s = live ? rate.s : 0.f, u = live ? next_u[q] : 0.f, d = live ? next_d[q] : 0.f, slope = live ? rate.slope : 0.f;
-      const float dy = live && gated ? d * z * sig : d, dz = live && gated ? d * (sig * fmaf(z, 1.f - sig, 1.f)) : 0.f;
+      // behind the sequence's end d, u and z come as zeros (u and z as the token that all share, where they are one): selections are for masks
+      const float s = live ? rate.s : 0.f, u = !MASKED || live ? next_u[q] : 0.f, d = !MASKED || live ? next_d[q] : 0.f;
+      const float slope = live ? rate.slope : 0.f;
+      const float dy = (!MASKED || live) && gated ? d * z * sig : d, dz = (!MASKED || live) && gated ? d * (sig * fmaf(z, 1.f - sig, 1.f)) : 0.f;
       rates[wave][4 * q + j][c] = (f32x4){s, s * u, dy, u};
       gates[wave][4 * q + j][c] = (f32x4){slope, dz, 0.f, 0.f};
     }
-    next_B.get(B, (m.live >> c) & 1u);
-    next_C.get(C, (m.live >> c) & 1u);
+    next_B.get(B, !MASKED || (m.live >> c) & 1u);
+    next_C.get(C, !MASKED || (m.live >> c) & 1u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) before[i] = __builtin_bit_cast(float, next_h.raw[i]);
     fronts[wave][lane] = (f32x4){before[0], before[1], before[2], before[3]};
@@ -177,7 +179,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     auto finish = [&](int q, float along, float through, const float* y_all) {
       const f32x4 rate = rates[wave][4 * q + j][c], gate = gates[wave][4 * q + j][c];
       const float ddt = fmaf(rate[3], along, through * kLn2) * gate[0];
-      const bool live = (m.live >> (4 * q + j)) & 1u;
+      const bool live = !MASKED || (m.live >> (4 * q + j)) & 1u;  // otherwise the slope is zero behind the end, and nothing is stored there
       const float du = live ? fmaf(rate[0], along, skip * rate[2]) : 0.f, dt_out = live ? ddt : 0.f;
       tile_dD = fmaf(rate[2], rate[3], tile_dD);
       tile_dbias += dt_out;
