@@ -4,7 +4,9 @@
 // gradients dy and ds:
 //   d = ds + inv (w dy - s inv^2 mean(w dy s)),  w = 1 + g,  for both addends;  dg = sum over rows of dy s inv
 // The statistics are those of the stored s, which the backward pass reads again.  A row is held in registers by one wave, by four or sixteen where it
-// is wider than 1024 or 4096 elements: at most sixteen elements a lane; nothing is read twice.  Bound by memory.
+// is wider than 1024 or 4096 elements: at most sixteen elements a lane; nothing is read twice, and the next row is asked for before this one's sum is joined.
+// Bound by memory.  bf16 with an fp32 stream, 16384 rows of 1024: 43 us forward (201 MB, 4.7 TB/s), 47-51 + 5 back (268 MB, 5.3 to 5.7); all bf16 to
+// 8 bits, 16384 rows of 2560: 59 us (294 MB, 5.0 TB/s).  Rows past 4096 elements that are no whole vectors leave 66 of a lane's registers in scratch back.
 
 #include <hip/hip_runtime.h>
 
