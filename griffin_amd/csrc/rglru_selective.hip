@@ -9,7 +9,8 @@
 namespace rglru {
 
 // What a part of a segment leaves of a state of zeros, and its sum of step sizes.  A walk of few registers: four waves share a SIMD, so a segment is cut into
-// parts until they do.  B1 T16384 W2560 N16 (bf16), two of three segments in twelve parts each: 145 us, 1.3 us a tile and SIMD.
+// parts until they do.  B1 T16384 W2560 N16 (bf16), two of three segments in twelve parts each: 137 us, 1.3 us a tile and SIMD
+// (parts for two or six waves a SIMD: 148 and 130, but 8 more in the forward walk, which joins them).
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_summary_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
   const SelPlace at = sel_place<SLABS, 1>(p, p.S * p.parts);
@@ -74,9 +75,10 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
 // Outputs, the last state and, for a backward pass, the state in front of every tile.
 // PIPE waves take a sequence's tiles in turn.  Decays and what is written need no state, so a wave makes those of its tile while the one in front walks; the
 // state then goes through the tile in 16 steps of one multiply-add, and on to the next wave through LDS before anything is made of it.
-// B8 T2048 W2048 N16 (bf16, gated, states kept): 187-200 us, of which 3 TB/s are no bound; B1 T16384 W2560, three segments: 243.  One wave a sequence took
-// 390 and 306, two in turn 210 and 251.  A tile's decays and inputs are 128 registers, so two waves share a SIMD; with three (decays only) the same
-// work took 222 and 280, with four (the last quarter's decays behind the wait) 192 and 290: the walk through a tile got longer.
+// B8 T2048 W2048 N16 (bf16, gated, states kept): 183-193 us (402 MB, 2.1 TB/s); B1 T16384 W2560, three segments: 232.  No part of it bounds it by itself:
+// without the exponentials it takes 5 % less, without the loads and what is made of them 20 %.  One wave a sequence took 390 and 306, two in turn 210 and 251
+// when four took 205 and 256.  A tile's decays and inputs are 128 registers, so two waves share a SIMD; with three (decays only) the same work took 222 and
+// 280, with four (the last quarter's decays behind the wait) 192 and 290: the walk through a tile got longer.
 template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads, 2) void sel_forward_kernel(SelArgs p) {
   constexpr int TEAMS = kSelWaves / (SLABS * PIPE);
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
