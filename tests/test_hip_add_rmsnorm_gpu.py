@@ -116,6 +116,24 @@ def test_one_result_and_one_operand():
     assert not torch.equal(a.grad, b.grad)
 
 
+def test_one_tensor_for_both_addends_and_broadcast_ones():
+    leaves, ups = make((9, 256), F32, F32)
+    x, g, up = leaves[0].cuda().requires_grad_(True), leaves[2].cuda(), ups[0].cuda()
+    copies = [x.detach().clone().requires_grad_(True) for _ in range(2)]
+    y, _ = hip_add_rmsnorm(x, x, g)
+    want, _ = hip_add_rmsnorm(*copies, g)
+    assert torch.equal(y, want)
+    a, b = torch.autograd.grad(want, copies, up)
+    assert torch.equal(torch.autograd.grad(y, x, up)[0], a + b)
+    row = x.detach()[:1].clone().requires_grad_(True)         # one row for all, an upstream gradient of one number
+    y, _ = hip_add_rmsnorm(row.expand(9, 256), x.detach(), g)
+    y.sum().backward()
+    one = row.detach().expand(9, 256).clone().requires_grad_(True)
+    want, _ = hip_add_rmsnorm(one, x.detach(), g)
+    each = torch.autograd.grad(want, one, torch.ones_like(want))[0].double()
+    assert torch.equal(y, want) and ((row.grad.double() - each.sum(0)).abs() <= 9 * HALF_STEP[F32] * each.abs().sum(0)).all()
+
+
 def test_gradients_against_differences():
     leaves, ups = make((5, 200), F32, F32)
     leaves, ups = [t.cuda().requires_grad_(True) for t in leaves], [t.cuda() for t in ups]

@@ -298,6 +298,45 @@ def test_tokens_that_overlap():
     assert torch.equal(hip_short_conv(case["u"], *args, "silu")[0], hip_short_conv(case["u"].contiguous(), *args, "silu")[0])
 
 
+def test_one_tensor_in_several_places():
+    """u, dt and z the same leaf, B and C another, A and the upstream gradient broadcast: the sums of the gradients that copies receive."""
+    for dtype, masked in ((F32, True), (BF16, False)):
+        case = {n: put(t) for n, t in make(2, 45, 20, 2, 16, dtype=dtype).items()}
+        reset, active = masks(2, 45) if masked else (None, None)
+        x, v, row = case["u"], case["B"], case["A"][:1]
+        copies = [x, x.clone(), row.expand(20, 16).clone(), v, v.clone(), case["D"], x.clone(), case["dt_bias"], case["h0"]]
+        copies = [t.detach().requires_grad_(True) for t in copies]
+        want, want_last = scan(*copies, reset=reset, active=active)
+        parts = torch.autograd.grad(want.float().sum(), copies)
+        x, v, row = (t.detach().requires_grad_(True) for t in (x, v, row))
+        got, last = scan(x, x, row.expand(20, 16), v, v, case["D"], x, case["dt_bias"], case["h0"], reset=reset, active=active)
+        grads = torch.autograd.grad(got.float().sum(), [x, row, v])
+        assert torch.equal(got, want) and torch.equal(last, want_last)
+        for grad, terms in zip(grads, ([parts[0], parts[1], parts[6]], [parts[2].split(1)], [parts[3], parts[4]])):
+            terms = [t.double() for t in (terms[0] if isinstance(terms[0], tuple) else terms)]
+            # each addition rounds what there is by then: no more than the sum of all magnitudes, half a step each
+            slack = len(terms) * HALF_STEP[grad.dtype] * sum(t.abs() for t in terms)
+            assert ((grad.double() - sum(terms)).abs() <= slack).all()
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap share nothing: both give what they give alone."""
+    cases = [{n: put(t) for n, t in make(2, 600, 64, 1, 16, dtype=BF16, seed=s).items()} for s in (1, 2)]
+    reset, active = masks(2, 600)
+    alone = [run(scan, c, "cuda", reset=reset, active=active) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(3):
+        for c, stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                both.append(run(scan, c, "cuda", reset=reset, active=active))
+    torch.cuda.synchronize()
+    for i, got in enumerate(both):
+        want = alone[i % 2]
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and all(torch.equal(got[2][n], want[2][n]) for n in want[2])
+
+
 def test_more_elements_than_32_bits_address():
     """2.4e9 elements a tensor, more than 2^31 bytes of kept states: the last document alone gives the same."""
     steps, width, states, tail = 40000, 60000, 4, 20
