@@ -10,6 +10,7 @@
 // B8 T2048 W2048 N16 (bf16, gated, two segments): 63-67 us for the second half's summary, 453-480 for the gradients, 14 for the last sums.  Bound by the
 // vector units: 1450 instructions a tile, 270 of them sums over channels (of 490 us, 90 went with those and 40 with the exponentials).  Its own states
 // instead of recomputed ones would be 4 N bytes a token and channel, 2.1 GB here, 420 us for reading them alone.
+// N 32 and 64: 829 and 1685 us (one segment), the last sums 59 and 231, of 0.27 and 1.07 GB: a workgroup's channels become fewer with more states.
 
 #include <hip/hip_runtime.h>
 
@@ -87,9 +88,20 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
   if (ok && j == 0 && at.slab == 0) { p.sums[2 * row] = total; p.sums[2 * row + 1] = cut ? 1.f : 0.f; }
 }
 
+template <bool VECTOR> struct SelGates;
+template <> struct alignas(16) SelGates<true> {             // one access
+  float slope, dz, y, none;
+  RGLRU_DEVICE void set(float a, float b) { *this = {a, b, 0.f, 0.f}; }
+};
+template <> struct SelGates<false> {
+  float slope, dz, y;
+  RGLRU_DEVICE void set(float a, float b) { slope = a; dz = b; }
+};
+
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads, 2) void sel_backward_kernel(SelArgs p) {
   __shared__ f32x4 rates[kSelWaves][kSelTile][kSelLanes];   // step size, that times u, dy, u
-  __shared__ f32x4 gates[kSelWaves][kSelTile][kSelLanes];   // slope of the step size, d silu'(z), sum over the states of C h
+  // slope of the step size, d silu'(z), sum over the states of C h.  (Packed where slabs exchange sums: 78 KB let two workgroups share a compute unit, 82 do not.)
+  __shared__ SelGates<SLABS == 1> gates[kSelWaves][kSelTile][kSelLanes];
   // what a lane needs once a tile, out of its registers: the state in front of the tile, and its sums over the tiles before
   __shared__ f32x4 fronts[kSelWaves][64], sum_dA[kSelWaves][64];
   __shared__ float2 sum_rows[kSelWaves][64];
@@ -148,7 +160,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       const float slope = live ? rate.slope : 0.f;
       const float dy = (!MASKED || live) && gated ? d * z * sig : d, dz = (!MASKED || live) && gated ? d * (sig * fmaf(z, 1.f - sig, 1.f)) : 0.f;
       rates[wave][4 * q + j][c] = (f32x4){s, s * u, dy, u};
-      gates[wave][4 * q + j][c] = (f32x4){slope, dz, 0.f, 0.f};
+      gates[wave][4 * q + j][c].set(slope, dz);
     }
     next_B.get(B, !MASKED || (m.live >> c) & 1u);
     next_C.get(C, !MASKED || (m.live >> c) & 1u);
@@ -172,7 +184,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
         }
         sums[decltype(token)::value] = bcast_dot<t>(C, h[t]);
       });
-      gates[wave][4 * decltype(group)::value + j][c][2] = four_rows_sum(sums);
+      gates[wave][4 * decltype(group)::value + j][c].y = four_rows_sum(sums);
     });
     // other names for B and C: broadcasts of theirs that the way back shared with the way there would each keep a register
 #pragma unroll
@@ -180,8 +192,9 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
     float tile_dA[4] = {0.f, 0.f, 0.f, 0.f}, tile_dD = 0.f, tile_dbias = 0.f;  // tile by tile: a long sum loses less
     // what one lane makes of its tokens' sums
     auto finish = [&](int q, float along, float through, const float* y_all) {
-      const f32x4 rate = rates[wave][4 * q + j][c], gate = gates[wave][4 * q + j][c];
-      const float ddt = fmaf(rate[3], along, through * kLn2) * gate[0];
+      const f32x4 rate = rates[wave][4 * q + j][c];
+      const SelGates<SLABS == 1> gate = gates[wave][4 * q + j][c];
+      const float ddt = fmaf(rate[3], along, through * kLn2) * gate.slope;
       const bool live = !MASKED || (m.live >> (4 * q + j)) & 1u;  // otherwise the slope is zero behind the end, and nothing is stored there
       const float du = live ? fmaf(rate[0], along, skip * rate[2]) : 0.f, dt_out = live ? ddt : 0.f;
       tile_dD = fmaf(rate[2], rate[3], tile_dD);
@@ -190,7 +203,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
       BufIo<IO>::store((IO)du, SelStream<IO>::tile(p.du, place, (unsigned)p.W, left), off, 0);
       BufIo<IO>::store((IO)dt_out, SelStream<IO>::tile(p.ddt, place, (unsigned)p.W, left), off, 0);
       if (gated) {
-        const float dz = live ? gate[1] * fmaf(skip, rate[3], y_all ? *y_all : gate[2]) : 0.f;
+        const float dz = live ? gate.dz * fmaf(skip, rate[3], y_all ? *y_all : gate.y) : 0.f;
         BufIo<IO>::store((IO)dz, SelStream<IO>::tile(p.dz, place, (unsigned)p.W, left), off, 0);
       }
     };
@@ -229,7 +242,7 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
         finish(g4, along, through, nullptr);
       } else {
         float (*mem)[4][64] = parts[tile & 1][wave];
-        mem[0][g4][lane] = along; mem[1][g4][lane] = through; mem[2][g4][lane] = gates[wave][4 * g4 + j][c][2];
+        mem[0][g4][lane] = along; mem[1][g4][lane] = through; mem[2][g4][lane] = gates[wave][4 * g4 + j][c].y;
       }
     });
     __syncthreads();                                        // the other buffer's readers are past the barrier before

@@ -106,7 +106,7 @@ template <typename IO, bool WHOLE, bool PAST> __global__ __launch_bounds__(kSelT
 static size_t sel_bytes(long long floats) { return ((size_t)floats * 4 + 255) & ~(size_t)255; }
 
 // Segments of a sequence, by a time estimate in microseconds.  A compute unit holds two workgroups at a time and takes `two` a tile of each with both, `one`
-// with one of them (measured: 0.8 and 0.5 forward, 7.8 and 5.5 back).  In segments, all but one are summarised first: a launch of 6, a tile's summary 1.2 on
+// with one of them (measured: 0.8 and 0.5 forward, 2.45 and 1.7 where its waves share states and not tiles, 7.8 and 5.5 back).  In segments, all but one are summarised first: a launch of 6, a tile's summary 1.2 on
 // a SIMD that has no other work and 1.27 / 4 of a unit's time where all have, and 0.25 for each segment that the others are joined from.
 static int sel_segments(long long wgs, long long waves, long long tiles, double two, double one) {
   const long long units = num_compute_units();
@@ -136,7 +136,8 @@ static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int
   a->tiles = (int)((T + kSelTile - 1) / kSelTile);
   const long long wgs = B * G * (backward ? a->per_group : a->pipe_group);
   if (wgs >= (1ll << 24) || (long long)G * N >= (1ll << 22)) return false;
-  a->S = sel_segments(wgs, B * G * columns * slabs, a->tiles, backward ? 7.8 : 0.8, backward ? 5.5 : 0.5);
+  const double two = backward ? 7.8 : slabs > 1 ? 2.45 : 0.8, one = backward ? 5.5 : slabs > 1 ? 1.7 : 0.5;
+  a->S = sel_segments(wgs, B * G * columns * slabs, a->tiles, two, one);
   a->seg_tiles = (a->tiles + a->S - 1) / a->S;
   // the summary is a short walk of few registers: more and shorter ones until four waves share a SIMD
   const long long summaries = B * G * (long long)a->per_group * (a->S - 1), most = a->seg_tiles / 4;
