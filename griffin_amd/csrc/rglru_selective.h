@@ -50,7 +50,7 @@ struct SelArgs {
   int B, T, W, N, G, Wg;                      // Wg: channels of a group
   int per_group, pipe_group;                  // workgroups of a group's channels: one wave, or kSelPipe waves to 16 of them (and states)
   int S, tiles, seg_tiles, parts;             // segments, tiles of a sequence and of a segment, parts that a segment is summarised in
-  int softplus, whole;                        // whole: rows of B, C and the states are whole vectors of four elements
+  int softplus, whole, pipe;                  // whole: rows of B, C and the states are whole vectors of four elements; pipe: kSelPipe waves take tiles in turn
 };
 
 // A place of the walk: what all lanes of a wave share.

@@ -9,8 +9,8 @@
 namespace rglru {
 
 // What a part of a segment leaves of a state of zeros, and its sum of step sizes.  A walk of few registers: four waves share a SIMD, so a segment is cut into
-// parts until they do.  B1 T16384 W2560 N16 (bf16), two of three segments in twelve parts each: 137 us, 1.3 us a tile and SIMD
-// (parts for two or six waves a SIMD: 148 and 130, but 8 more in the forward walk, which joins them).
+// parts until they do.  B1 T16384 W2560 N16 (bf16), eleven of twelve segments in two parts each: 144 us, 0.98 us a tile
+// and SIMD.  (Parts for two or six waves a SIMD, in three segments: 148 and 130 for 137, but 8 more in the forward walk, which joins them.)
 template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads) void sel_summary_kernel(SelArgs p) {
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
   const SelPlace at = sel_place<SLABS, 1>(p, p.S * p.parts);
@@ -73,12 +73,13 @@ template <typename IO, int SLABS, bool MASKED, bool WHOLE> __global__ __launch_b
 }
 
 // Outputs, the last state and, for a backward pass, the state in front of every tile.
-// PIPE waves take a sequence's tiles in turn.  Decays and what is written need no state, so a wave makes those of its tile while the one in front walks; the
-// state then goes through the tile in 16 steps of one multiply-add, and on to the next wave through LDS before anything is made of it.
-// B8 T2048 W2048 N16 (bf16, gated, states kept): 183-193 us (402 MB, 2.1 TB/s); B1 T16384 W2560, three segments: 232.  No part of it bounds it by itself:
-// without the exponentials it takes 5 % less, without the loads and what is made of them 20 %.  One wave a sequence took 390 and 306, two in turn 210 and 251
-// when four took 205 and 256.  A tile's decays and inputs are 128 registers, so two waves share a SIMD; with three (decays only) the same work took 222 and
-// 280, with four (the last quarter's decays behind the wait) 192 and 290: the walk through a tile got longer.
+// PIPE waves take a sequence's tiles in turn, or one takes all of them (sel_plan).  In turn: decays and what is written need no state, so a wave makes those of
+// its tile while the one in front walks; the state then goes through the tile in 16 steps of one multiply-add, and on to the next wave through LDS before
+// anything is made of it.
+// B8 T2048 W2048 N16 (bf16, gated, states kept): 182-193 us (402 MB, 2.1 TB/s); B1 T16384 W2560, twelve segments, a wave each: 225.  No part of it bounds it
+// by itself: without the exponentials it takes 5 % less, without the loads and what is made of them 20 %.  A tile's decays and inputs are 128 registers, so
+// two waves share a SIMD; with three (decays only) the first took 222 for 205 at the time, with four (the last quarter's decays behind the wait) 192: the walk
+// through a tile got longer, and few sequences lost more.
 template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ __launch_bounds__(kSelThreads, 2) void sel_forward_kernel(SelArgs p) {
   constexpr int TEAMS = kSelWaves / (SLABS * PIPE);
   __shared__ float2 rates[kSelWaves][kSelTile][kSelLanes];
@@ -214,14 +215,19 @@ template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> __global__ 
   if ((last - 1 - first) % PIPE == at.turn && at.seg == p.S - 1) sel_store_states(p.h_last, (long long)at.b * p.W + w, n0, p.N, ok, WHOLE, h);
 }
 
-template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_forward_whole(const SelArgs& a, hipStream_t s) {
-  constexpr int PIPE = SLABS == 1 ? kSelPipe : 1;
-  const dim3 block(kSelThreads);
-  if (a.S > 1)
-    hipLaunchKernelGGL((sel_summary_kernel<IO, SLABS, MASKED, WHOLE>), dim3((unsigned)(a.B * (long long)a.S * a.parts * a.G * a.per_group)), block, 0, s, a);
+template <typename IO, int SLABS, int PIPE, bool MASKED, bool WHOLE> static void sel_forward_walk(const SelArgs& a, hipStream_t s) {
   SelArgs f = a;
   f.per_group = PIPE > 1 ? a.pipe_group : a.per_group;
-  hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, PIPE, MASKED, WHOLE>), dim3((unsigned)(f.B * (long long)f.S * f.G * f.per_group)), block, 0, s, f);
+  hipLaunchKernelGGL((sel_forward_kernel<IO, SLABS, PIPE, MASKED, WHOLE>), dim3((unsigned)(f.B * (long long)f.S * f.G * f.per_group)), dim3(kSelThreads), 0, s, f);
+}
+template <typename IO, int SLABS, bool MASKED, bool WHOLE> static void sel_forward_whole(const SelArgs& a, hipStream_t s) {
+  if (a.S > 1)
+    hipLaunchKernelGGL((sel_summary_kernel<IO, SLABS, MASKED, WHOLE>), dim3((unsigned)(a.B * (long long)a.S * a.parts * a.G * a.per_group)), dim3(kSelThreads), 0,
+                       s, a);
+  if constexpr (SLABS == 1) {
+    if (a.pipe) return sel_forward_walk<IO, SLABS, kSelPipe, MASKED, WHOLE>(a, s);
+  }
+  sel_forward_walk<IO, SLABS, 1, MASKED, WHOLE>(a, s);
 }
 template <typename IO, int SLABS> static void sel_forward_slabs(const SelArgs& a, hipStream_t s) {
   if (a.flags) { if (a.whole) sel_forward_whole<IO, SLABS, true, true>(a, s); else sel_forward_whole<IO, SLABS, true, false>(a, s); }

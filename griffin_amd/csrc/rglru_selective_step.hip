@@ -105,23 +105,24 @@ template <typename IO, bool WHOLE, bool PAST> __global__ __launch_bounds__(kSelT
 
 static size_t sel_bytes(long long floats) { return ((size_t)floats * 4 + 255) & ~(size_t)255; }
 
-// Segments of a sequence, by a time estimate in microseconds.  A compute unit holds two workgroups at a time and takes `two` a tile of each with both, `one`
-// with one of them (measured: 0.8 and 0.5 forward, 2.45 and 1.7 where its waves share states and not tiles, 7.8 and 5.5 back).  In segments, all but one are summarised first: a launch of 6, a tile's summary 1.2 on
-// a SIMD that has no other work and 1.27 / 4 of a unit's time where all have, and 0.25 for each segment that the others are joined from.
-static int sel_segments(long long wgs, long long waves, long long tiles, double two, double one) {
+// Segments of a sequence, by a time estimate in microseconds.  A compute unit holds two workgroups at a time, each of which takes 2 to begin and `two` a tile with
+// both there, `one` with one of them (measured, forward: 0.8 and 0.5 where four waves take a sequence's tiles in turn, 2.45 and 1.7 where each has a sequence or
+// states of its own; back: 7.8 and 5.5).  In segments, all but one are summarised first: a launch of 6, a tile's summary 1.2 on a SIMD that has no other work and
+// 1.27 / 4 of a unit's time where all have, and 0.25 for each segment that the others are joined from.
+struct SelSegments { int count; double time; };
+static SelSegments sel_segments(long long wgs, long long waves, long long tiles, double two, double one) {
   const long long units = num_compute_units();
-  int best = 1;
-  double least = 0.;
+  SelSegments best = {1, 0.};
   for (long long s = 1; s <= kSelMaxSegments && s <= tiles; ++s) {
     const long long each = (tiles + s - 1) / s;
     if ((tiles + each - 1) / each != s) continue;            // the same segments as fewer
     const long long all = wgs * s, full = all / (2 * units), rest = all - full * 2 * units;
-    double time = (double)each * (two * (double)full + (rest > units ? two : rest > 0 ? one : 0.));
+    double time = (double)each * (two * (double)full + (rest > units ? two : rest > 0 ? one : 0.)) + 2. * (double)(full + (rest > 0));
     if (s > 1) {
       const double filled = 1.27 * (double)(waves * each * (s - 1)) / (4. * (double)units), alone = 1.2 * (double)(each < 4 ? each : 4);
       time += 6. + 0.25 * (double)s + (filled > alone ? filled : alone);
     }
-    if (s == 1 || time < least) { best = (int)s; least = time; }
+    if (s == 1 || time < best.time) best = {(int)s, time};
   }
   return best;
 }
@@ -136,8 +137,21 @@ static bool sel_plan(SelArgs* a, int64_t B, int64_t T, int64_t W, int64_t G, int
   a->tiles = (int)((T + kSelTile - 1) / kSelTile);
   const long long wgs = B * G * (backward ? a->per_group : a->pipe_group);
   if (wgs >= (1ll << 24) || (long long)G * N >= (1ll << 22)) return false;
-  const double two = backward ? 7.8 : slabs > 1 ? 2.45 : 0.8, one = backward ? 5.5 : slabs > 1 ? 1.7 : 0.5;
-  a->S = sel_segments(wgs, B * G * columns * slabs, a->tiles, two, one);
+  const long long waves = B * G * columns * slabs, alone = B * G * a->per_group;
+  SelSegments plan;
+  if (backward) {
+    plan = sel_segments(alone, waves, a->tiles, 7.8, 5.5);
+  } else {
+    plan = sel_segments(alone, waves, a->tiles, 2.45, 1.7);
+    if (slabs == 1) {
+      // Tiles in turn, where that is estimated to be faster: few sequences, or an uneven number of rounds (N16, bf16, in turn and not: B8 T2048 W2048 173 and
+      // 205 us, B3 T137 W1024 8 and 13; B16 T2048 W2048 352 and 328, B64 T128 102 and 80, B128 T16 67 and 29, B1 T16384 W2560 363 and 343).
+      const SelSegments turns = sel_segments(wgs, waves, a->tiles, 0.8, 0.5);
+      a->pipe = turns.time < plan.time;
+      if (a->pipe) plan = turns;
+    }
+  }
+  a->S = plan.count;
   a->seg_tiles = (a->tiles + a->S - 1) / a->S;
   // the summary is a short walk of few registers: more and shorter ones until four waves share a SIMD
   const long long summaries = B * G * (long long)a->per_group * (a->S - 1), most = a->seg_tiles / 4;

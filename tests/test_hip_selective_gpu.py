@@ -174,6 +174,32 @@ def test_sequences_in_segments(shape, dtype):
     check(case, reset=reset, active=active)
 
 
+@pytest.mark.parametrize("shape", [(96, 33, 256, 1, 16), (64, 20, 130, 2, 7), (1, 500, 1024, 1, 4)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_waves_with_sequences_of_their_own(shape, dtype):
+    """Many short sequences, and wide ones in many segments: no wave shares its tiles with others."""
+    case = make(*shape, dtype=dtype)
+    check(case)
+    reset, active = masks(*shape[:2])
+    check(case, reset=reset, active=active)
+
+
+@pytest.mark.parametrize("shape", [(2, 3000, 768, 1, 16), (1, 5000, 2000, 2, 13), (2, 3000, 384, 1, 40)], ids=str)
+def test_long_sequences_by_pieces(shape):
+    """The whole walked in other segments, by other waves than its pieces: both within the bound of the walk."""
+    steps = shape[1]
+    case = {n: put(t) for n, t in make(*shape).items()}
+    reset, active = (t.cuda() for t in holes(*shape[:2]))
+    for how in ({}, dict(reset=reset, active=active)):
+        whole, last = scan(*(case[n] for n in NAMES), **how)
+        state, pieces = case["h0"], []
+        for a, b in ((0, 900), (900, 1000), (1000, steps)):
+            part = [case[n][:, a:b] if n in ("u", "dt", "B", "C", "z") else case[n] for n in NAMES[:-1]]
+            y, state = scan(*part, state, **{k: m[:, a:b] for k, m in how.items()})
+            pieces.append(y)
+        assert rel_err(torch.cat(pieces, 1), whole) <= 2 * bound(F32, steps) and rel_err(state, last) <= 2 * bound(F32, steps)
+
+
 def test_step_sizes_as_they_are():
     case = make(2, 40, 20, 1, 16)
     case["dt"], case["dt_bias"] = case["dt"].abs() * 0.1, None
